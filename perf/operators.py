@@ -1,0 +1,371 @@
+"""The gated delta rule and the filtered token draw, as timed cases.
+
+  step      dfssm.ops.gated_delta_step: one token per sequence, recurrent form, state in slots
+  prefill   dfssm.ops.gated_delta_prefill: prompts of any lengths, chunked form, state carried on
+  sample    dfssm.ops.sample_filtered: temperature, top-k, top-p and min-p, from given random numbers
+
+`run` computes them from elementary torch operations in 32 bits (in 64 where a rounding would move a
+token across a border), or, with `own`, through the framework's operators. `exact` computes the same
+from the definitions in 64 bits: the delta rule token by token, the draw on the sorted row.
+
+Shapes are those of the 1.3B and 2.7B configurations (64 and 80 heads of 64, 128 state columns,
+vocabulary 50288) and generic neighbours of them. Keys and queries are normal, log decays are those of
+the model's own time steps (softplus of a normal around a small step, times A in 1..16), betas are
+sigmoids, logits are normal with a few raised tokens.
+"""
+import os
+import sys
+
+import torch
+
+own = False
+DEV = "cuda:0"
+TYPES = {"fp16": torch.float16, "bf16": torch.bfloat16, "fp32": torch.float32}
+CHUNK = 64
+
+
+def listed():
+    return [
+        # one user's decode step at the 1.3B shape, the smallest call: latency
+        {"name": "step_b1", "kind": "step", "batch": 1, "hk": 16, "hv": 64, "dk": 128, "dv": 64, "slots": 1,
+         "type": "fp16", "l2norm": True},
+        # a serving batch at the 1.3B shape, its states spread over a larger pool
+        {"name": "step_b32", "kind": "step", "batch": 32, "hk": 16, "hv": 64, "dk": 128, "dv": 64, "slots": 48,
+         "type": "fp16", "l2norm": True},
+        # the 2.7B shape at the framework's largest batch, a key head per value head
+        {"name": "step_b64_2p7b", "kind": "step", "batch": 64, "hk": 80, "hv": 80, "dk": 128, "dv": 64, "slots": 64,
+         "type": "bf16", "l2norm": False},
+        # an odd batch, short keys and wide values
+        {"name": "step_b37_wide", "kind": "step", "batch": 37, "hk": 8, "hv": 24, "dk": 64, "dv": 208, "slots": 37,
+         "type": "bf16", "l2norm": True},
+        # one user's short prompt: latency
+        {"name": "prefill_t33", "kind": "prefill", "lens": "33", "hk": 16, "hv": 64, "dk": 128, "dv": 64,
+         "type": "fp16", "l2norm": True},
+        # a ragged batch of chat turns, lengths that no chunk divides, one sequence with nothing new
+        {"name": "prefill_ragged", "kind": "prefill",
+         "lens": "1 997 64 2049 0 130 511 17 3001 63 65 777", "hk": 16, "hv": 64, "dk": 128, "dv": 64,
+         "type": "bf16", "l2norm": True},
+        # one long document at the 1.3B shape
+        {"name": "prefill_t16411", "kind": "prefill", "lens": "16411", "hk": 16, "hv": 64, "dk": 128, "dv": 64,
+         "type": "fp16", "l2norm": True},
+        # the benchmark's long-prompt configuration: the 2.7B shape, 64 sequences of 512 tokens
+        {"name": "prefill_2p7b_b64_t512", "kind": "prefill", "lens": " ".join(["512"] * 64), "hk": 80, "hv": 80, "dk": 128,
+         "dv": 64, "type": "bf16", "l2norm": False},
+        # few heads of short keys and wide values over a long text
+        {"name": "prefill_wide", "kind": "prefill", "lens": "4099 8000", "hk": 4, "hv": 12, "dk": 64, "dv": 128,
+         "type": "fp16", "l2norm": True},
+        # one user's draw over the model's vocabulary: latency
+        {"name": "sample_b1", "kind": "sample", "batch": 1, "vocab": 50288, "type": "fp16", "masked": 0.0},
+        # a serving batch, every user with settings of their own, a grammar masking half of the tokens
+        {"name": "sample_b32", "kind": "sample", "batch": 32, "vocab": 50288, "type": "fp16", "masked": 0.5},
+        # many users over a large vocabulary, logits kept in 32 bits
+        {"name": "sample_b256_v131072", "kind": "sample", "batch": 256, "vocab": 131072, "type": "fp32",
+         "masked": 0.1},
+    ]
+
+
+def _log(rng, lo, hi):
+    """A whole number in lo..hi, spread over its logarithm."""
+    return max(lo, min(hi, int(lo * (hi / lo) ** rng.random() + 0.5)))
+
+
+def _lens(case):
+    """The lengths of a prefill's sequences, in order."""
+    return [int(x) for x in case["lens"].split()]
+
+
+def draw(rng):
+    kind = rng.choice(["step", "step", "prefill", "prefill", "prefill", "sample"])
+    if kind == "sample":
+        return {"kind": kind, "batch": _log(rng, 1, 256), "vocab": _log(rng, 500, 131072),
+                "type": rng.choice(["fp16", "bf16", "fp32"]), "masked": rng.choice([0.0, 0.0, 0.3, 0.9])}
+    hk, hv = rng.choice([(16, 64), (80, 80), (1, 64), (8, 24), (4, 12), (2, 2), (5, 40)])
+    case = {"kind": kind, "hk": hk, "hv": hv, "dk": rng.choice([64, 128, 128]),
+            "dv": 16 * rng.choice([1, 2, 4, 4, 4, 6, 8, 13, 16]), "type": rng.choice(["fp16", "bf16"]),
+            "l2norm": rng.random() < 0.7}
+    if kind == "step":
+        most = max(1, min(64, 64 * 80 * 64 * 128 // (hv * case["dv"] * case["dk"])))
+        case["batch"] = _log(rng, 1, most)
+        case["slots"] = case["batch"] + rng.randrange(0, 9)
+        return case
+    n = _log(rng, 1, 64)
+    most = min(32768, 32768 * 80 * 64 * 128 // (hv * case["dv"] * case["dk"]) // 2)
+    total = _log(rng, 1, most)
+    lens = [1 + int(rng.random() ** 2 * 2 * total / n) for _ in range(n)]
+    if n > 2 and rng.random() < 0.3:
+        lens[rng.randrange(n)] = 0
+    while sum(lens) > most:
+        lens = [x * 3 // 4 for x in lens]
+    case["lens"] = " ".join(str(x) for x in lens) if sum(lens) else "1"
+    return case
+
+
+# ---------------------------------------------------------------------------------------------
+# inputs
+# ---------------------------------------------------------------------------------------------
+def prepare(case, seed):
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    t = TYPES[case["type"]]
+
+    def normal(*shape):
+        return torch.randn(*shape, generator=gen, device=DEV)
+
+    def uniform(*shape):
+        return torch.rand(*shape, generator=gen, device=DEV)
+
+    if case["kind"] == "sample":
+        B, V = case["batch"], case["vocab"]
+        logits = 2.0 * normal(B, V)
+        raised = (uniform(B, 12) * V).long()
+        logits.scatter_add_(1, raised, 6.0 * uniform(B, 12))
+        if case["masked"]:
+            logits.masked_fill_(uniform(B, V) < case["masked"], float("-inf"))
+            logits[:, V // 2] = 1.0                # a mask leaves something
+        pick = uniform(B, 4)
+        temperature = 0.6 + 0.7 * uniform(B)
+        temperature[pick[:, 0] < 0.1] = 0.0        # greedy users
+        top_k = (1.0 + uniform(B) * 200).int()
+        top_k[pick[:, 1] < 0.5] = 0                # no top-k
+        top_p = 0.5 + 0.5 * uniform(B)
+        top_p[pick[:, 2] < 0.3] = 1.0
+        min_p = 0.1 * uniform(B)
+        min_p[pick[:, 3] < 0.5] = 0.0
+        return {"case": case, "logits": logits.to(t), "u": uniform(B), "temperature": temperature,
+                "top_k": top_k, "top_p": top_p, "min_p": min_p}
+
+    Hk, Hv, Dk, Dv = case["hk"], case["hv"], case["dk"], case["dv"]
+    step = case["kind"] == "step"
+    n = case["batch"] if step else len(_lens(case))
+    T = n if step else sum(_lens(case))
+    size = 1.0 if case["l2norm"] else Dk ** -0.5
+    q = (size * normal(T, Hk, Dk)).to(t)
+    k = (size * normal(T, Hk, Dk)).to(t)
+    v = normal(T, Hv, Dv).to(t)
+    dt = torch.nn.functional.softplus(normal(T, Hv) + (4.0 * uniform(Hv) - 6.0))
+    g = -(1.0 + 15.0 * uniform(Hv)) * dt
+    beta = torch.sigmoid(normal(T, Hv))
+    pool = case["slots"] if step else n
+    state = 0.3 * normal(pool, Hv, Dv, Dk)
+    slots = torch.randperm(pool, generator=gen, device=DEV)[:n].int()
+    s = {"case": case, "q": q, "k": k, "v": v, "g": g, "beta": beta, "state": state, "slots": slots,
+         "state_out": torch.zeros_like(state)}
+    if not step:
+        cu = [0]
+        for x in _lens(case):
+            cu.append(cu[-1] + x)
+        s["cu_seqlens"] = torch.tensor(cu, dtype=torch.int32, device=DEV)
+    return s
+
+
+# ---------------------------------------------------------------------------------------------
+# one pass
+# ---------------------------------------------------------------------------------------------
+def run(s):
+    kind = s["case"]["kind"]
+    if own:
+        return _run_own(s, kind)
+    if kind == "step":
+        return _plain_step(s)
+    return _plain_sample(s) if kind == "sample" else _plain_prefill(s)
+
+
+def _run_own(s, kind):
+    ops = _ops()
+    if kind == "sample":
+        return ops.sample_filtered(s["logits"], s["u"], temperature=s["temperature"], top_k=s["top_k"],
+                                   top_p=s["top_p"], min_p=s["min_p"], want_logprob=True)
+    l2 = s["case"]["l2norm"]
+    if kind == "step":
+        o = ops.gated_delta_step(s["q"], s["k"], s["v"], s["g"], s["beta"], s["state"], slots=s["slots"],
+                                 l2norm=l2, state_out=s["state_out"])
+    else:
+        o = ops.gated_delta_prefill(s["q"], s["k"], s["v"], s["g"], s["beta"], s["state"],
+                                    cu_seqlens=s["cu_seqlens"], slots=s["slots"], l2norm=l2,
+                                    state_out=s["state_out"])
+    return o, s["state_out"]
+
+
+def _ops():
+    pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "df-ssm_amd")
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
+    from dfssm import ops
+    return ops
+
+
+def _unit(x, l2norm):
+    x = x.float()
+    return x / torch.sqrt((x * x).sum(-1, keepdim=True) + 1e-6) if l2norm else x
+
+
+def _plain_step(s):
+    c = s["case"]
+    rep = c["hv"] // c["hk"]
+    slots = s["slots"].long()
+    q = _unit(s["q"], c["l2norm"]).repeat_interleave(rep, 1)
+    k = _unit(s["k"], c["l2norm"]).repeat_interleave(rep, 1)
+    S = s["state"][slots] * torch.exp(s["g"])[..., None, None]
+    u = s["beta"][..., None] * (s["v"].float() - (S * k[..., None, :]).sum(-1))
+    S = S + u[..., None] * k[..., None, :]
+    o = (S * q[..., None, :]).sum(-1) * c["dk"] ** -0.5
+    s["state_out"][slots] = S
+    return o.to(s["v"].dtype), s["state_out"]
+
+
+def _plain_prefill(s):
+    """The chunked form: everything that needs no state for all chunks at once, then the chunks of
+    all sequences one after another, the longest sequences first."""
+    c = s["case"]
+    Hk, Hv, Dk, Dv, C = c["hk"], c["hv"], c["dk"], c["dv"], CHUNK
+    rep = Hv // Hk
+    lens = _lens(c)
+    by_len = sorted(range(len(lens)), key=lambda i: -lens[i])
+    nch = [(lens[i] + C - 1) // C for i in by_len]                # chunks of each, descending
+    cu, dev = s["cu_seqlens"].long(), s["q"].device
+    order = torch.tensor(by_len, device=dev)
+    per = torch.tensor(nch, device=dev)
+    off = torch.cumsum(per, 0) - per                              # first chunk of each
+    seq = torch.repeat_interleave(torch.arange(len(lens), device=dev), per, output_size=sum(nch))
+    tok = (cu[order][seq] + (torch.arange(sum(nch), device=dev) - off[seq]) * C)[:, None] + torch.arange(C, device=dev)
+    real = tok < cu[order + 1][seq][:, None]                      # (chunks, C)
+    tok = torch.where(real, tok, torch.zeros_like(tok))
+    m = real[..., None]
+
+    def chunks(x):                                                # (chunks, heads, C, ...), zero behind the end
+        y = x[tok]
+        y = torch.where(m if y.dim() == 3 else m[..., None], y, torch.zeros_like(y))
+        return y.transpose(1, 2).contiguous()
+
+    q = chunks(_unit(s["q"], c["l2norm"])).repeat_interleave(rep, 1)
+    k = chunks(_unit(s["k"], c["l2norm"])).repeat_interleave(rep, 1)
+    v = chunks(s["v"].float())
+    beta = chunks(s["beta"])
+    G = torch.cumsum(chunks(s["g"]).double(), -1)
+    low = torch.ones(C, C, device=dev, dtype=torch.bool).tril()
+    # the exponent is masked before the exponential: above the diagonal it may overflow
+    D = torch.exp(torch.where(low, G[..., :, None] - G[..., None, :], torch.zeros_like(G[..., None]))).float()
+    kt = k.transpose(-1, -2).contiguous()
+    A = torch.where(low.tril(-1), beta[..., None] * torch.matmul(k, kt) * D, torch.zeros_like(D))
+    P = torch.where(low, torch.matmul(q, kt) * D, torch.zeros_like(D))
+    X = torch.eye(C, device=dev).expand_as(A).contiguous()        # (I + A)^-1, row by row
+    for i in range(1, C):
+        X[..., i, :i] = -torch.matmul(A[..., i:i + 1, :i].contiguous(), X[..., :i, :i].contiguous())[..., 0, :]
+    X = X * beta[..., None, :]
+    eG = torch.exp(G).float()[..., None]
+    eEnd = torch.exp(G[..., -1:] - G).float()[..., None]
+    O = torch.empty(sum(nch), Hv, C, Dv, device=dev)
+    slots = s["slots"].long()[order]
+    S = s["state"][slots].transpose(-1, -2).contiguous()          # (seqs, heads, Dk, Dv)
+    for i in range(nch[0]):
+        na = sum(1 for x in nch if x > i)                         # sequences that reach this chunk
+        ids = off[:na] + i
+        Si, ki = S[:na], k[ids]
+        u = torch.matmul(X[ids], v[ids] - eG[ids] * torch.matmul(ki, Si))
+        O[ids] = eG[ids] * torch.matmul(q[ids], Si) + torch.matmul(P[ids], u)
+        S[:na] = eG[ids][..., -1:, :] * Si + torch.matmul((eEnd[ids] * ki).transpose(-1, -2).contiguous(), u)
+    out = torch.empty(s["v"].shape, dtype=s["v"].dtype, device=dev)
+    out[tok[real]] = (O.transpose(1, 2)[real] * Dk ** -0.5).to(out.dtype)
+    s["state_out"][slots] = S.transpose(-1, -2)
+    return out, s["state_out"]
+
+
+def _plain_sample(s):
+    l = s["logits"].double()
+    V = l.shape[1]
+    l, order = torch.sort(l, dim=1, descending=True, stable=True)  # ties: the lowest index first
+    T = s["temperature"].double()[:, None]
+    greedy = T <= 0
+    e = torch.exp((l - l[:, :1]) / torch.where(greedy, torch.ones_like(T), T))
+    rank = torch.arange(V, device=l.device)[None]
+    top_k = s["top_k"].long()[:, None]
+    top_k = torch.where(top_k <= 0, torch.full_like(top_k, V), top_k)
+    top_k = torch.where(greedy, torch.ones_like(top_k), top_k)
+    e = torch.where(rank < top_k, e, torch.zeros_like(e))
+    C = torch.cumsum(e, 1)
+    above = C - e
+    keep = (rank < top_k) & (above <= s["top_p"].double()[:, None] * C[:, -1:]) & (e >= s["min_p"].double()[:, None])
+    keep[:, 0] = True
+    mass = torch.where(keep, e, torch.zeros_like(e)).sum(1, keepdim=True)
+    j = (keep & (C <= s["u"].double()[:, None] * mass)).sum(1, keepdim=True).clamp(max=V - 1)
+    token = order.gather(1, j)[:, 0]
+    return token, torch.log(e.gather(1, j) / mass)[:, 0].float()
+
+
+# ---------------------------------------------------------------------------------------------
+# what a pass cannot do without
+# ---------------------------------------------------------------------------------------------
+def work(case):
+    b = 4 if case["type"] == "fp32" else 2
+    if case["kind"] == "sample":
+        n = case["batch"] * case["vocab"]
+        return {"bytes": n * b + case["batch"] * 32, "flops": 4 * n}
+    n = case["batch"] if case["kind"] == "step" else len(_lens(case))
+    T = n if case["kind"] == "step" else sum(_lens(case))
+    rows = T * (2 * case["hk"] * case["dk"] + 2 * case["hv"] * case["dv"]) * b + T * case["hv"] * 8
+    state = n * case["hv"] * case["dv"] * case["dk"]
+    return {"bytes": rows + 8 * state, "flops": 6 * T * case["hv"] * case["dv"] * case["dk"]}
+
+
+# ---------------------------------------------------------------------------------------------
+# the definitions in 64 bits
+# ---------------------------------------------------------------------------------------------
+def exact(case, seed):
+    s = prepare(case, seed)
+    if case["kind"] == "sample":
+        return _exact_sample(s)
+    step = case["kind"] == "step"
+    lens = [1] * case["batch"] if step else _lens(case)
+    rep, Dk = case["hv"] // case["hk"], case["dk"]
+    q, k, v, g, beta = (s[x].double() for x in ("q", "k", "v", "g", "beta"))
+    if case["l2norm"]:
+        q = q / (q.pow(2).sum(-1, keepdim=True) + 1e-6).sqrt()
+        k = k / (k.pow(2).sum(-1, keepdim=True) + 1e-6).sqrt()
+    a = g.exp()
+    by_len = sorted(range(len(lens)), key=lambda i: -lens[i])
+    first, n = [], 0
+    for x in lens:
+        first.append(n)
+        n += x
+    start = torch.tensor([first[i] for i in by_len], device=q.device)
+    where = s["slots"].long()[torch.tensor(by_len, device=q.device)]
+    S = s["state"].double()[where]
+    head = torch.arange(case["hv"], device=q.device) // rep
+    o = torch.zeros(v.shape, dtype=torch.float64, device=q.device)
+    na = len(lens)
+    for t in range(lens[by_len[0]]):                              # token by token
+        while lens[by_len[na - 1]] <= t:
+            na -= 1
+        i = start[:na] + t
+        kt, qt = k[i][:, head, :, None], q[i][:, head, :, None]
+        St = S[:na]
+        St.mul_(a[i][..., None, None])
+        u = beta[i][..., None, None] * (v[i][..., None] - torch.matmul(St, kt))
+        St.add_(u * kt.transpose(-1, -2))
+        o[i] = torch.matmul(St, qt)[..., 0]
+    state = torch.zeros(s["state"].shape, dtype=torch.float64, device=q.device)
+    state[where] = S
+    return o * Dk ** -0.5, state
+
+
+def _exact_sample(s):
+    tokens, logp = [], []
+    host = {x: s[x].cpu().double() for x in ("logits", "u", "temperature", "top_k", "top_p", "min_p")}
+    for b in range(host["logits"].shape[0]):
+        l = host["logits"][b]
+        T, k = host["temperature"][b].item(), int(host["top_k"][b].item())
+        order = torch.argsort(l, descending=True, stable=True)
+        if T <= 0:
+            tokens.append(order[0].item())
+            logp.append(0.0)
+            continue
+        order = order[:k] if k > 0 else order
+        p = torch.softmax(l[order] / T, 0)
+        above = torch.cat([torch.zeros(1, dtype=torch.float64), torch.cumsum(p, 0)[:-1]])
+        n = int(((above <= host["top_p"][b]) & (p >= host["min_p"][b] * p[0])).sum().item())
+        p = p[:max(n, 1)] / p[:max(n, 1)].sum()
+        j = int((torch.cumsum(p, 0) <= host["u"][b]).sum().item())
+        j = min(j, len(p) - 1)
+        tokens.append(order[j].item())
+        logp.append(p[j].log().item())
+    dev = s["logits"].device
+    return torch.tensor(tokens, device=dev), torch.tensor(logp, dtype=torch.float64, device=dev)

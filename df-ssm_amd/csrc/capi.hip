@@ -680,6 +680,22 @@ int dfssm_sample(const dfssm_model* model, const uint16_t* logits, int32_t* coun
   return dfssm_embed(model, next, x_next, workspace, stream);
 }
 
+int dfssm_sample_filtered(const void* logits, int type, int64_t ld, int batch, int vocab, const float* u,
+                          const dfssm_filter* filter, int64_t* next, float* logprob, void* stream) {
+  if (!filter) return DFSSM_E_NULL;
+  if (batch < 0) return DFSSM_E_BATCH;
+  if (vocab < 1 || vocab > kDrawMaxVocab || (batch > 1 && ld < vocab)) return DFSSM_E_DIMS;
+  if (type != DFSSM_TYPE_F16 && type != DFSSM_TYPE_BF16 && type != DFSSM_TYPE_F32) return DFSSM_E_DIMS;
+  if (batch == 0) return DFSSM_OK;
+  if (!logits || !u || !next) return DFSSM_E_NULL;
+  const dfssm_filter& f = *filter;
+  DrawArgs a{};
+  a.logits = logits; a.ld = ld; a.u = u; a.V = vocab; a.next = next; a.logprob = logprob;
+  a.temperatures = f.temperatures; a.top_ks = f.top_ks; a.top_ps = f.top_ps; a.min_ps = f.min_ps;
+  a.temperature = f.temperature; a.top_k = f.top_k; a.top_p = f.top_p; a.min_p = f.min_p;
+  return hip_status(launch_draw(a, type, batch, as_stream(stream)));
+}
+
 size_t dfssm_prefill_workspace_bytes(const dfssm_dims* dims, int max_rows) {
   if (!dims || dfssm_check_dims(dims) != DFSSM_OK) return 0;
   if (max_rows < dims->batch || max_rows > kGemmMaxRows) return 0;

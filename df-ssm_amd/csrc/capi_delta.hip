@@ -1,0 +1,63 @@
+// C entry points of the gated delta rule (declared in include/dfssm.h): checks, then the launches.
+#include <hip/hip_runtime.h>
+
+#include "delta.h"
+#include "dfssm.h"
+
+using namespace dfssm;
+
+namespace {
+
+int hip_status(hipError_t e) { return e == hipSuccess ? DFSSM_OK : (int)e; }
+bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+
+int check_delta(const dfssm_delta* d, bool step) {
+  if (!d) return DFSSM_E_NULL;
+  if (d->n_seq < 0 || d->n_tokens < 0 || d->n_slots < 0) return DFSSM_E_RANGE;
+  if (d->k_heads < 1 || d->v_heads < 1 || d->v_heads % d->k_heads) return DFSSM_E_DIMS;
+  if ((d->k_dim != 64 && d->k_dim != 128) || d->v_dim < 16 || d->v_dim > 256 || d->v_dim % 16) return DFSSM_E_DIMS;
+  if (d->type != DFSSM_TYPE_F16 && d->type != DFSSM_TYPE_BF16) return DFSSM_E_DIMS;
+  if (step && (d->n_tokens != d->n_seq || d->cu_seqlens)) return DFSSM_E_RANGE;
+  if (!step && !d->cu_seqlens && d->n_seq > 0 && d->n_tokens % d->n_seq) return DFSSM_E_RANGE;
+  if (d->n_seq == 0) return DFSSM_OK;
+  if (!d->state || !d->state_out) return DFSSM_E_NULL;
+  if (d->n_tokens && (!d->q || !d->k || !d->v || !d->g || !d->beta || !d->out)) return DFSSM_E_NULL;
+  if (!aligned16(d->q) || !aligned16(d->k) || !aligned16(d->v) || !aligned16(d->out) || !aligned16(d->state) ||
+      !aligned16(d->state_out))
+    return DFSSM_E_ALIGN;
+  if (d->ld_q % 8 || d->ld_k % 8 || d->ld_v % 8 || d->ld_out % 8) return DFSSM_E_ALIGN;
+  return DFSSM_OK;
+}
+
+DeltaArgs delta_args(const dfssm_delta* d) {
+  DeltaArgs a{};
+  a.q = (const uint16_t*)d->q; a.k = (const uint16_t*)d->k; a.v = (const uint16_t*)d->v;
+  a.g = d->g; a.beta = d->beta;
+  a.state = d->state; a.state_out = d->state_out;
+  a.slots = d->slots; a.cu = d->cu_seqlens;
+  a.out = (uint16_t*)d->out;
+  a.ld_q = d->ld_q; a.ld_k = d->ld_k; a.ld_v = d->ld_v; a.ld_g = d->ld_g; a.ld_beta = d->ld_beta; a.ld_out = d->ld_out;
+  a.n_tokens = d->n_tokens; a.len = d->n_seq ? d->n_tokens / d->n_seq : 0;
+  a.n_seq = d->n_seq; a.n_slots = d->n_slots;
+  a.Hk = d->k_heads; a.Hv = d->v_heads; a.Dk = d->k_dim; a.Dv = d->v_dim;
+  a.bf16 = d->type == DFSSM_TYPE_BF16; a.l2norm = d->l2norm; a.scale = d->scale;
+  return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dfssm_gated_delta_step(const dfssm_delta* args, void* stream) {
+  const int rc = check_delta(args, true);
+  if (rc || args->n_seq == 0) return rc;
+  return hip_status(launch_delta_token(delta_args(args), (hipStream_t)stream));
+}
+
+int dfssm_gated_delta_prefill(const dfssm_delta* args, void* stream) {
+  const int rc = check_delta(args, false);
+  if (rc || args->n_seq == 0) return rc;
+  return hip_status(launch_delta_token(delta_args(args), (hipStream_t)stream));
+}
+
+}  // extern "C"

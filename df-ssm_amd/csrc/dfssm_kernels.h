@@ -348,4 +348,22 @@ hipError_t launch_ssm_scan(const ScanArgs& a, int batch, hipStream_t s);
 hipError_t launch_last_rows(const uint16_t* src, uint16_t* dst, int batch, int T, int D, hipStream_t s);
 hipError_t launch_tile_emb(const uint8_t* src, uint8_t* dst, int V, int row_bytes, hipStream_t s);
 
+// Token draw with top-k, top-p and min-p (draw.hip). A null pointer of a pair: the scalar for every row.
+struct DrawArgs {
+  const void* logits;        // (batch, V), rows ld elements apart
+  int64_t ld;
+  const float* u;            // (batch)
+  const float* temperatures;
+  const int32_t* top_ks;
+  const float* top_ps;
+  const float* min_ps;
+  float temperature, top_p, min_p;
+  int top_k;
+  int64_t* next;
+  float* logprob;            // or null
+  int V;
+};
+constexpr int kDrawMaxVocab = 1 << 18;
+hipError_t launch_draw(const DrawArgs& a, int type, int batch, hipStream_t s);
+
 }  // namespace dfssm

@@ -49,6 +49,19 @@ class SampleParams(ctypes.Structure):
                 ("mode", ctypes.c_int32), ("seed", ctypes.c_uint64)]
 
 
+class Delta(ctypes.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("q", "k", "v", "g", "beta", "state", "state_out", "slots", "cu_seqlens", "out")]
+                + [(n, ctypes.c_int64) for n in ("ld_q", "ld_k", "ld_v", "ld_g", "ld_beta", "ld_out", "n_tokens")]
+                + [(n, ctypes.c_int32) for n in ("n_seq", "n_slots", "k_heads", "v_heads", "k_dim", "v_dim", "type",
+                                                 "l2norm")] + [("scale", ctypes.c_float)])
+
+
+class Filter(ctypes.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("temperatures", "top_ks", "top_ps", "min_ps")] +
+                [("temperature", ctypes.c_float), ("top_k", ctypes.c_int32), ("top_p", ctypes.c_float),
+                 ("min_p", ctypes.c_float)])
+
+
 _SIGS = {
     "dfssm_version": (c_int, []),
     "dfssm_error_string": (ctypes.c_char_p, [c_int]),
@@ -79,6 +92,9 @@ _SIGS = {
     "dfssm_prefill_workspace_bytes": (c_size_t, [ctypes.POINTER(Dims), c_int]),
     "dfssm_prefill": (c_int, [ctypes.POINTER(Model), P, c_int, P, ctypes.POINTER(State), P, P, c_int, P, P,
                               c_int, P]),
+    "dfssm_sample_filtered": (c_int, [P, c_int, ctypes.c_int64, c_int, c_int, P, ctypes.POINTER(Filter), P, P, P]),
+    "dfssm_gated_delta_step": (c_int, [ctypes.POINTER(Delta), P]),
+    "dfssm_gated_delta_prefill": (c_int, [ctypes.POINTER(Delta), P]),
 }
 
 _lib = None

@@ -251,6 +251,11 @@ int dfssm_decode_step_static(const dfssm_model* model, const int64_t* tokens, ui
                              const dfssm_state* state, uint16_t* logits, int64_t* next, int fuse_next_embed,
                              int* error_out, void* stream);
 
+/* Element types of the operators that take more than one. */
+#define DFSSM_TYPE_F16 0
+#define DFSSM_TYPE_BF16 1
+#define DFSSM_TYPE_F32 2 /* logits of dfssm_sample_filtered only */
+
 /* ---- sampling ------------------------------------------------------------------------ */
 typedef struct dfssm_sample_params {
   float temperature;   /* > 0 */
@@ -276,6 +281,30 @@ typedef struct dfssm_sample_params {
 int dfssm_sample(const dfssm_model* model, const uint16_t* logits, int32_t* counts, uint32_t* step,
                  const dfssm_sample_params* params, int64_t* next, uint16_t* x_next, void* workspace,
                  void* stream);
+
+/* The draw with filters and without a generator: the random numbers are an input. Per row the tokens are
+ * ranked by logit, the lowest index first among equals; with e = exp((logit - largest logit) / temperature),
+ * kept are the first top_k ranks (0: all); of those, with Z their mass, the ranks that have at most top_p Z
+ * ranked above them; and of those the ones with e >= min_p. Rank 0 is always kept. With S the kept mass, the
+ * token is the first rank whose cumulative mass exceeds u S. temperature <= 0 (or NaN) takes rank 0. A NaN
+ * logit counts as -inf; of several +inf logits each has mass 1 and every other token none; a row of nothing
+ * but -inf gives -1. The exponentials are fp64 and summed exactly (to 2^-44 of the largest), so the result
+ * does not depend on any order. eval/gen_test.py:54-95 is the temperature and top_p part of it. */
+typedef struct dfssm_filter {
+  const float* temperatures;   /* (batch) on the device, or NULL: `temperature` for every row; so for each pair */
+  const int32_t* top_ks;
+  const float* top_ps;
+  const float* min_ps;
+  float temperature;
+  int32_t top_k;               /* <= 0: no limit */
+  float top_p;                 /* >= 1: no limit */
+  float min_p;                 /* <= 0: no limit */
+} dfssm_filter;
+/* logits (batch, vocab) of `type` (DFSSM_TYPE_*), rows ld elements apart; u (batch) in [0, 1) (held to it; NaN
+ * counts as 0); next (batch) receives the tokens and logprob (batch, may be NULL) the logarithm of their share
+ * of the kept mass (-inf with -1). vocab <= 262144. */
+int dfssm_sample_filtered(const void* logits, int type, int64_t ld, int batch, int vocab, const float* u,
+                          const dfssm_filter* filter, int64_t* next, float* logprob, void* stream);
 
 /* ---- prompt prefill ------------------------------------------------------------------- */
 /* Workspace of dfssm_prefill for chunks of up to max_rows = batch x tokens-per-chunk rows
@@ -315,6 +344,45 @@ int dfssm_prefill(const dfssm_model* model, const int64_t* tokens, int n_tokens,
  * deterministic. */
 int dfssm_state_density_field(float* h, float* sd_error, int64_t rows, int d_state,
                               const float* thresholds, int kk, int sd_bits, void* stream);
+
+/* ---- gated delta rule ---------------------------------------------------------- */
+/* No counterpart in the reference: the recurrence that stands in the SSM step's place in gated
+ * delta-rule layers. Per value head, with the state S (v_dim, k_dim) fp32 and a = exp(g):
+ *   S' = a S;  u = beta (v - S' k);  S = S' + u k^T;  out = scale S q
+ * Value head h reads key head h / (v_heads / k_heads). With l2norm != 0, q and k are divided by
+ * sqrt(sum x^2 + 1e-6) first. g is the log of the decay: at most 0, -inf allowed. */
+typedef struct dfssm_delta {
+  const void* q;          /* (tokens, k_heads, k_dim), `type`; tokens ld_q elements apart, heads contiguous */
+  const void* k;          /* the same */
+  const void* v;          /* (tokens, v_heads, v_dim), `type` */
+  const float* g;         /* (tokens, v_heads) */
+  const float* beta;      /* (tokens, v_heads) */
+  const float* state;     /* (n_slots, v_heads, v_dim, k_dim), C-contiguous */
+  float* state_out;       /* of that shape: `state` itself (in place) or memory that does not overlap it */
+  const int32_t* slots;   /* (n_seq) the slot of every sequence, or NULL: sequence b has slot b.
+                             A sequence whose slot is negative is padding: its rows of out are zero. One whose
+                             slot is >= n_slots, or that of an earlier sequence of the call, is refused: its
+                             rows of out are NaN. Neither touches a state. */
+  const int32_t* cu_seqlens; /* dfssm_gated_delta_prefill: (n_seq + 1) first tokens, sequence b has tokens
+                             cu_seqlens[b] .. cu_seqlens[b + 1]; NULL: n_tokens / n_seq tokens each. Offsets
+                             outside [0, n_tokens] are held to it; rows of no sequence stay as they were. */
+  void* out;              /* (tokens, v_heads, v_dim), `type` */
+  int64_t ld_q, ld_k, ld_v, ld_g, ld_beta, ld_out; /* elements */
+  int64_t n_tokens;
+  int32_t n_seq, n_slots, k_heads, v_heads;
+  int32_t k_dim;          /* 64 or 128 */
+  int32_t v_dim;          /* a multiple of 16, at most 256 */
+  int32_t type;           /* DFSSM_TYPE_F16 or DFSSM_TYPE_BF16 */
+  int32_t l2norm;
+  float scale;
+} dfssm_delta;
+/* q, k, v, out, state and state_out are 16-byte aligned, ld_q, ld_k, ld_v and ld_out multiples of 8. */
+
+/* One token per sequence (n_tokens = n_seq). */
+int dfssm_gated_delta_step(const dfssm_delta* args, void* stream);
+
+/* The tokens of n_seq sequences of any lengths, from the states they have to the states they leave. */
+int dfssm_gated_delta_prefill(const dfssm_delta* args, void* stream);
 
 #ifdef __cplusplus
 }

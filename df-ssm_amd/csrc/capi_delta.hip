@@ -11,12 +11,18 @@ namespace {
 int hip_status(hipError_t e) { return e == hipSuccess ? DFSSM_OK : (int)e; }
 bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
-int check_delta(const dfssm_delta* d, bool step) {
-  if (!d) return DFSSM_E_NULL;
+int check_dims(const dfssm_delta* d) {
   if (d->n_seq < 0 || d->n_tokens < 0 || d->n_slots < 0) return DFSSM_E_RANGE;
   if (d->k_heads < 1 || d->v_heads < 1 || d->v_heads % d->k_heads) return DFSSM_E_DIMS;
   if ((d->k_dim != 64 && d->k_dim != 128) || d->v_dim < 16 || d->v_dim > 256 || d->v_dim % 16) return DFSSM_E_DIMS;
   if (d->type != DFSSM_TYPE_F16 && d->type != DFSSM_TYPE_BF16) return DFSSM_E_DIMS;
+  return DFSSM_OK;
+}
+
+int check_delta(const dfssm_delta* d, bool step) {
+  if (!d) return DFSSM_E_NULL;
+  const int rc = check_dims(d);
+  if (rc) return rc;
   if (step && (d->n_tokens != d->n_seq || d->cu_seqlens)) return DFSSM_E_RANGE;
   if (!step && !d->cu_seqlens && d->n_seq > 0 && d->n_tokens % d->n_seq) return DFSSM_E_RANGE;
   if (d->n_seq == 0) return DFSSM_OK;
@@ -44,6 +50,11 @@ DeltaArgs delta_args(const dfssm_delta* d) {
   return a;
 }
 
+// Prompts that run token by token: too few tokens for a chunk's fixed work. The lengths behind cu_seqlens are
+// on the device, so the rule there goes by all tokens, which any one sequence may have.
+constexpr int kTokenPath = 8;
+bool by_tokens(const DeltaArgs& a) { return (a.cu ? a.n_tokens : a.len) <= kTokenPath; }
+
 }  // namespace
 
 extern "C" {
@@ -54,10 +65,20 @@ int dfssm_gated_delta_step(const dfssm_delta* args, void* stream) {
   return hip_status(launch_delta_token(delta_args(args), (hipStream_t)stream));
 }
 
-int dfssm_gated_delta_prefill(const dfssm_delta* args, void* stream) {
+size_t dfssm_gated_delta_workspace_bytes(const dfssm_delta* args) {
+  if (!args || args->n_seq <= 0 || check_dims(args) != DFSSM_OK) return 0;
+  const DeltaArgs a = delta_args(args);
+  return by_tokens(a) ? 0 : delta_chunk_workspace(a);
+}
+
+int dfssm_gated_delta_prefill(const dfssm_delta* args, void* workspace, void* stream) {
   const int rc = check_delta(args, false);
   if (rc || args->n_seq == 0) return rc;
-  return hip_status(launch_delta_token(delta_args(args), (hipStream_t)stream));
+  const DeltaArgs a = delta_args(args);
+  if (by_tokens(a)) return hip_status(launch_delta_token(a, (hipStream_t)stream));
+  if (!workspace) return DFSSM_E_NULL;
+  if (!aligned16(workspace)) return DFSSM_E_ALIGN;
+  return hip_status(launch_delta_chunked(a, workspace, (hipStream_t)stream));
 }
 
 }  // extern "C"

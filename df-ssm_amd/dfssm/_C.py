@@ -94,7 +94,8 @@ _SIGS = {
                               c_int, P]),
     "dfssm_sample_filtered": (c_int, [P, c_int, ctypes.c_int64, c_int, c_int, P, ctypes.POINTER(Filter), P, P, P]),
     "dfssm_gated_delta_step": (c_int, [ctypes.POINTER(Delta), P]),
-    "dfssm_gated_delta_prefill": (c_int, [ctypes.POINTER(Delta), P]),
+    "dfssm_gated_delta_workspace_bytes": (c_size_t, [ctypes.POINTER(Delta)]),
+    "dfssm_gated_delta_prefill": (c_int, [ctypes.POINTER(Delta), P, P]),
 }
 
 _lib = None

@@ -190,7 +190,7 @@ def _on_device(t: torch.Tensor, name: str, dev) -> None:
         raise ValueError(f"{name} is on {t.device}, not on {dev}")
 
 
-def _delta_call(entry: str, q, k, v, g, beta, state, cu_seqlens, slots, scale, l2norm, out, state_out, n_seq):
+def _delta_call(step: bool, q, k, v, g, beta, state, cu_seqlens, slots, scale, l2norm, out, state_out, n_seq):
     """Checks (tokens, heads, dim) arguments, launches and returns out."""
     dev = q.device if isinstance(q, torch.Tensor) else None
     kind = _TYPE16.get(q.dtype) if isinstance(q, torch.Tensor) else None
@@ -251,7 +251,12 @@ def _delta_call(entry: str, q, k, v, g, beta, state, cu_seqlens, slots, scale, l
                     n_seq, state.shape[0], Hk, Hv, Dk, Dv, kind, 1 if l2norm else 0,
                     Dk ** -0.5 if scale is None else scale)
     with torch.cuda.device(dev):
-        _C.check(getattr(_C.lib(), "dfssm_" + entry)(args, _C.stream()), entry)
+        if step:
+            _C.check(_C.lib().dfssm_gated_delta_step(args, _C.stream()), "gated_delta_step")
+        else:
+            need = _C.lib().dfssm_gated_delta_workspace_bytes(args)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+            _C.check(_C.lib().dfssm_gated_delta_prefill(args, _C.ptr(ws), _C.stream()), "gated_delta_prefill")
     return out
 
 
@@ -267,7 +272,7 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     the slot of each sequence (default 0..B-1); a negative one marks padding (zeros returned), one past the
     state or taken by an earlier row gives NaN, and neither touches a state. scale defaults to Dk^-0.5;
     l2norm divides q and k by sqrt(sum x^2 + 1e-6) first."""
-    return _delta_call("gated_delta_step", q, k, v, g, beta, state, None, slots, scale, l2norm, out, state_out,
+    return _delta_call(True, q, k, v, g, beta, state, None, slots, scale, l2norm, out, state_out,
                        q.shape[0])
 
 
@@ -285,7 +290,7 @@ def gated_delta_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: to
         _need(cu_seqlens, torch.int32, "cu_seqlens")
         if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
             raise ValueError("cu_seqlens must be (sequences + 1,)")
-        return _delta_call("gated_delta_prefill", q, k, v, g, beta, state, cu_seqlens.contiguous(), slots, scale, l2norm,
+        return _delta_call(False, q, k, v, g, beta, state, cu_seqlens.contiguous(), slots, scale, l2norm,
                            out, state_out, cu_seqlens.numel() - 1)
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4 or g.dim() != 3 or beta.dim() != 3:
         raise ValueError("without cu_seqlens: q, k, v (batch, tokens, heads, dim), g, beta (batch, tokens, heads)")
@@ -294,7 +299,7 @@ def gated_delta_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: to
         raise ValueError("q, k, v, g and beta must agree in batch and tokens")
     if out is not None and not out.is_contiguous():
         raise ValueError("out must be contiguous")
-    o = _delta_call("gated_delta_prefill", q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1), g.flatten(0, 1),
+    o = _delta_call(False, q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1), g.flatten(0, 1),
                     beta.flatten(0, 1), state, None, slots, scale, l2norm,
                     None if out is None else out.flatten(0, 1), state_out, B)
     return o.view(B, T, *v.shape[2:]) if out is None else out

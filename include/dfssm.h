@@ -381,8 +381,12 @@ typedef struct dfssm_delta {
 /* One token per sequence (n_tokens = n_seq). */
 int dfssm_gated_delta_step(const dfssm_delta* args, void* stream);
 
-/* The tokens of n_seq sequences of any lengths, from the states they have to the states they leave. */
-int dfssm_gated_delta_prefill(const dfssm_delta* args, void* stream);
+/* The tokens of n_seq sequences of any lengths, from the states they have to the states they leave: what
+ * dfssm_gated_delta_step gives token by token, up to fp32 rounding. workspace: 16-byte aligned device memory of
+ * dfssm_gated_delta_workspace_bytes(args) bytes (at most about 1 GiB; 0: none needed, NULL allowed), for this
+ * call alone while it runs; its contents do not matter. */
+size_t dfssm_gated_delta_workspace_bytes(const dfssm_delta* args);
+int dfssm_gated_delta_prefill(const dfssm_delta* args, void* workspace, void* stream);
 
 #ifdef __cplusplus
 }

@@ -24,7 +24,7 @@ BAD = [({"q": 0}, -1), ({"state": 0}, -1), ({"out": 0}, -1), ({"beta": 0}, -1), 
 def test_delta(kw, rc):
     L = _C.lib()
     assert L.dfssm_gated_delta_step(_delta(**kw), None) == rc
-    assert L.dfssm_gated_delta_prefill(_delta(**kw), None) == rc
+    assert L.dfssm_gated_delta_prefill(_delta(**kw), None, None) == rc
 
 
 def test_delta_counts():
@@ -32,9 +32,12 @@ def test_delta_counts():
     assert L.dfssm_gated_delta_step(None, None) == -1
     assert L.dfssm_gated_delta_step(_delta(n_tokens=3), None) == -5          # one token per sequence
     assert L.dfssm_gated_delta_step(_delta(cu_seqlens=16), None) == -5
-    assert L.dfssm_gated_delta_prefill(_delta(n_tokens=3), None) == -5       # 3 tokens of 2 equal sequences
+    assert L.dfssm_gated_delta_prefill(_delta(n_tokens=3), None, None) == -5       # 3 tokens of 2 equal sequences
     assert L.dfssm_gated_delta_step(_delta(n_seq=0, n_tokens=0), None) == 0  # nothing to do
-    assert L.dfssm_gated_delta_prefill(_delta(n_seq=0), None) == 0
+    assert L.dfssm_gated_delta_prefill(_delta(n_seq=0), None, None) == 0
+    many = _delta(n_tokens=200)
+    assert L.dfssm_gated_delta_workspace_bytes(many) > 0 and L.dfssm_gated_delta_workspace_bytes(_delta()) == 0
+    assert L.dfssm_gated_delta_prefill(many, None, None) == -1 and L.dfssm_gated_delta_prefill(many, 8, None) == -4
 
 
 def test_draw():

@@ -50,10 +50,10 @@ def recurrence(x, lens, l2norm, slots=None, scale=None):
     return out * (Dk ** -0.5 if scale is None else scale), state
 
 
-def check(got, ref, what):
+def check(got, ref, what, roundings=1):
     got, ref = got.cpu(), ref
     assert torch.isfinite(got.double()).all(), what
-    half = torch.finfo(got.dtype).eps / 2 if got.dtype != torch.float32 else 0.0
+    half = roundings * torch.finfo(got.dtype).eps / 2 if got.dtype != torch.float32 else 0.0
     err = (got.double() - ref).abs()
     if got.dtype == torch.float32:                                     # states (slots, heads, Dv, Dk)
         top = ref.abs().amax((-1, -2), keepdim=True).clamp_min(1e-3)
@@ -253,13 +253,15 @@ def test_prefill_equals_steps():
     for lo, hi in ((0, 37), (37, 90)):
         y = {n: (t if n == "state" else t[lo:hi]) for n, t in dict(d, state=state).items()}
         parts.append(prefill(y, [hi - lo], l2norm=True))
-    check(torch.cat(parts), whole.double().cpu(), "two calls")
+    # both sides are rounded here: two fp32 values a hair apart may fall to either side of a border, one whole
+    # step (half a step from each) apart
+    check(torch.cat(parts), whole.double().cpu(), "two calls", roundings=2)
     check(state, d["state"].double().cpu(), "state of two calls")
     state = st0.clone()
     for t in range(90):
         o = ops.gated_delta_step(*(d[n][t:t + 1] for n in ("q", "k", "v", "g", "beta")), state, l2norm=True)
     check(state, d["state"].double().cpu(), "state of steps")
-    check(o, whole[-1:].double().cpu(), "last token")
+    check(o, whole[-1:].double().cpu(), "last token", roundings=2)
 
 
 def test_bad_offsets_stay_inside():

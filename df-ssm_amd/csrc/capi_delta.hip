@@ -11,6 +11,8 @@ namespace {
 int hip_status(hipError_t e) { return e == hipSuccess ? DFSSM_OK : (int)e; }
 bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
+constexpr int64_t kMaxLd = 1 << 23;
+
 int check_dims(const dfssm_delta* d) {
   if (d->n_seq < 0 || d->n_tokens < 0 || d->n_slots < 0) return DFSSM_E_RANGE;
   if (d->k_heads < 1 || d->v_heads < 1 || d->v_heads % d->k_heads) return DFSSM_E_DIMS;
@@ -31,6 +33,9 @@ int check_delta(const dfssm_delta* d, bool step) {
   if (!aligned16(d->q) || !aligned16(d->k) || !aligned16(d->v) || !aligned16(d->out) || !aligned16(d->state) ||
       !aligned16(d->state_out))
     return DFSSM_E_ALIGN;
+  // (the kernels address a chunk's rows by 32-bit offsets)
+  for (const int64_t ld : {d->ld_q, d->ld_k, d->ld_v, d->ld_g, d->ld_beta, d->ld_out})
+    if (ld < 0 || ld > kMaxLd) return DFSSM_E_RANGE;
   if (d->ld_q % 8 || d->ld_k % 8 || d->ld_v % 8 || d->ld_out % 8) return DFSSM_E_ALIGN;
   return DFSSM_OK;
 }

@@ -26,7 +26,6 @@ struct DeltaArgs {
 hipError_t launch_delta_token(const DeltaArgs& a, hipStream_t s);
 hipError_t launch_delta_chunked(const DeltaArgs& a, void* workspace, hipStream_t s);
 size_t delta_chunk_workspace(const DeltaArgs& a);
-int64_t delta_chunk_slots(int64_t n_tokens, int n_seq);
 
 constexpr int kSlotPad = -1;  // a negative slot: the sequence is padding
 constexpr int kSlotBad = -2;  // past the state, or taken by an earlier sequence of the call

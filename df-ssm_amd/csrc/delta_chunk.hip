@@ -27,7 +27,6 @@ typedef f16 h8 __attribute__((ext_vector_type(8)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 
 constexpr int kC = 64;        // tokens of a chunk
-constexpr int kGroup = 4;     // value heads of one preparing workgroup (a wave each for the inverse)
 
 // What the preparation leaves per chunk and value head. T and P are in the order in which a lane of the matrix
 // cores takes them: fragments of 16 rows x 32 columns, lane (g, r) row r, columns 4 g .. 4 g + 3 and 16 + 4 g ..,
@@ -40,11 +39,28 @@ struct ChunkRec {
   float c2[kC];         // scale e^{G_i} times q's
   float tr[kC], pr[kC]; // row factors of T and P
   float w[kC];          // e^{G_C - G_i} times k's row factor
-  float ks[kC], qs[kC]; // the powers of two that k and q are scaled by (bf16)
   float dec;            // e^{G_C}
   float pad[63];
 };
-static_assert(sizeof(ChunkRec) == 26624, "whole KiB");
+static_assert(sizeof(ChunkRec) == 26112, "T, P, 1.5 KiB of factors");
+
+// Per chunk and key head: k and q as halves, rows past the sequence's end zero. The 16-byte pieces of a row are
+// exchanged so that the same piece of 16 rows, an operand, lies in all 64 LDS banks.
+template <int DK>
+struct KeyRec {
+  f16 k[kC][DK], q[kC][DK];
+};
+template <int DK>
+__device__ __forceinline__ int piece_at(int row, int p) {
+  return p ^ (DK == 128 ? row & 15 : (row >> 1) & 7);
+}
+
+// The records of a launch: the slots' key records, then their chunk records.
+template <int DK>
+struct Records {
+  KeyRec<DK>* keys;
+  ChunkRec* chunks;
+};
 
 __device__ __forceinline__ int frag_of(int t, int j) { return t + (t > 2 ? 1 : 0) + j; }  // row tile, column block
 
@@ -63,10 +79,6 @@ __device__ __forceinline__ float pow2_scale(float m, float& inv) {
   return __builtin_bit_cast(float, (268u << 23) - e);
 }
 
-__device__ __forceinline__ void split(float x, f16& hi, f16& lo) {
-  hi = (f16)x;
-  lo = (f16)(x - (float)hi);
-}
 
 // The largest of v >= 0 over the four lanes of a column (16 apart). As whole numbers, which order as the floats
 // do: the compiler drops a float maximum of the two results of one lane swap.
@@ -78,19 +90,35 @@ __device__ __forceinline__ float max_rows4(float v) {
   return __builtin_bit_cast(float, max((uint32_t)q[0], (uint32_t)q[1]));
 }
 
-// The sequence and chunk of slot s of the launch's chunk numbering: sequence b starts at slot
-// floor(t0 / 64) + b, which needs no sums over the lengths and leaves room for every chunk.
-__device__ __forceinline__ int64_t first_slot(const DeltaArgs& a, int b) {
-  int64_t t0, t1;
-  seq_range(a, b, t0, t1);
-  return t0 / kC + b;
+// A chunk's rows as a buffer of just that many bytes: loads past its last row return zero and stores there are
+// dropped, with no branch (a predicated load cost its own round trip to memory: the compiler joins the loaded
+// value with the zero, and waits for it there), and offsets are 32-bit.
+typedef __amdgpu_buffer_rsrc_t Rsrc;
+__device__ __forceinline__ Rsrc rows_of(const uint16_t* p, int64_t ld, int len, int dim) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, ((len - 1) * (int)ld + dim) * 2, 0x00027000);
 }
+__device__ __forceinline__ u32x4 row_load16(Rsrc r, int voff, int soff) {
+  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, 0));
+}
+
+// The sequence and chunk of slot s of the launch's chunk numbering: sequence b starts at slot
+// floor(t0 / 64) + b, which needs no sums over the lengths and leaves room for every chunk. The lanes of a wave
+// look at 64 sequences at once.
 __device__ bool chunk_of(const DeltaArgs& a, int64_t s, int64_t& tok, int& len) {
-  int lo = 0, hi = a.n_seq;  // the last sequence that starts at or before s
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (first_slot(a, mid) <= s) lo = mid;
-    else hi = mid;
+  const int lane = threadIdx.x & 63;
+  int lo = 0, n = a.n_seq;  // the last sequence that starts at or before s is one of lo .. lo + n - 1
+  while (n > 1) {
+    const int step = (n + 63) / 64, i = lo + lane * step;
+    bool before = false;
+    if (i < lo + n) {
+      int64_t t0, t1;
+      seq_range(a, i, t0, t1);
+      before = t0 / kC + i <= s;
+    }
+    const int k = __popcll(__ballot(before));  // the starts rise, so the first k lanes (lane 0's always does)
+    const int end = lo + n;
+    lo += (k > 0 ? k - 1 : 0) * step;
+    n = min(step, end - lo);
   }
   int64_t t0, t1;
   seq_range(a, lo, t0, t1);
@@ -102,24 +130,18 @@ __device__ bool chunk_of(const DeltaArgs& a, int64_t s, int64_t& tok, int& len) 
 }
 
 // ---------------------------------------------------------------------------------------------
-// Preparation: one chunk, one key head, up to four of its value heads.
+// Preparation: one chunk and value head per wave, which needs no barrier; four to a workgroup, so that the heads
+// of a key head find its rows in the L1 cache.
 // ---------------------------------------------------------------------------------------------
 constexpr int kMS = kC + 4;   // row stride of a matrix in LDS (floats): rows of 16-byte reads start 4 banks apart
 
-template <int DK>
-struct PrepLds {
-  union {
-    struct {
-      f16 k[kC][DK + 8], q[kC][DK + 8];
-    } in;
-    float M[kGroup][kC][kMS];
-  };
-  double G[kGroup][kC];       // in units of log 2
-  float be[kGroup][kC];
-  float rk[kC], rq[kC];
+struct PrepLds {              // of a wave
+  float M[kC][kMS];
+  double G[kC];               // in units of log 2
+  float be[kC], rk[kC], rq[kC];
 };
 
-// 8 values of a 16-bit row as halves times sc (1 for fp16), their squares added to ss.
+// 8 values of a 16-bit row as halves times sc (1 for fp16).
 template <bool BF>
 __device__ __forceinline__ h8 to_halves(u32x4 x, float sc) {
   if constexpr (!BF) return __builtin_bit_cast(h8, x);
@@ -132,37 +154,54 @@ __device__ __forceinline__ h8 to_halves(u32x4 x, float sc) {
   return r;
 }
 
-// A row's quarter (thread t of the four of a row) into LDS; returns the row's power-of-two scale in sc and
-// its factor (normalisation over that scale).
+__device__ __forceinline__ float sum_rows4(float v) {  // over the four lanes of a column
+  const uint32_t x = __builtin_bit_cast(uint32_t, v);
+  const auto p = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  v = __builtin_bit_cast(float, (uint32_t)p[0]) + __builtin_bit_cast(float, (uint32_t)p[1]);
+  const uint32_t y = __builtin_bit_cast(uint32_t, v);
+  const auto q = __builtin_amdgcn_permlane32_swap(y, y, false, false);
+  return __builtin_bit_cast(float, (uint32_t)q[0]) + __builtin_bit_cast(float, (uint32_t)q[1]);
+}
+
+template <int DK>
+__device__ __forceinline__ void load_rows(Rsrc rows, int64_t ld, int t, int lane, u32x4 (&x)[DK / 32]) {
+  const int off = (16 * t + (lane & 15)) * (int)ld * 2 + (lane >> 4) * 16;
+#pragma unroll
+  for (int j = 0; j < DK / 32; ++j) x[j] = row_load16(rows, off, j * 64);
+}
+// 16 rows as operands (lane (g, r): row r, columns 32 j + 8 g ..), also into the key record if given. Returns the
+// factor of the lane's row, normalisation over power-of-two scale.
 template <int DK, bool BF>
-__device__ __forceinline__ float prep_row(const uint16_t* p, f16* dst, int t, bool real, bool l2norm, float& sc) {
-  constexpr int NV = DK / 32;
-  u32x4 x[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) x[i] = real ? *(const u32x4*)(p + (t * NV + i) * 8) : u32x4{0, 0, 0, 0};
-  float ss = 0.0f, inv = 1.0f;
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int d = 0; d < 4; ++d) {
-      const float a = w2f<BF>((uint16_t)x[i][d]), b = w2f<BF>((uint16_t)(x[i][d] >> 16));
-      ss = __builtin_fmaf(a, a, ss);
-      ss = __builtin_fmaf(b, b, ss);
-      const uint32_t u = x[i][d] & 0x7fff7fffu;
-      top = max(top, max(u >> 16, u & 0xffffu));
-    }
-  ss += dpp_f32<0xB1>(ss);
-  ss += dpp_f32<0x4E>(ss);
-  sc = 1.0f;
+__device__ __forceinline__ float make_rows(const u32x4 (&x)[DK / 32], int t, int lane, bool l2norm, f16 (*rec)[DK], h8 (&y)[DK / 32]) {
+  constexpr int NJ = DK / 32;
+  const int row = 16 * t + (lane & 15), g = lane >> 4;
+  float inv = 1.0f, sc = 1.0f, f = 1.0f;
   if constexpr (BF) {
-    top = max(top, (uint32_t)dpp_i32<0xB1>((int)top));
-    top = max(top, (uint32_t)dpp_i32<0x4E>((int)top));
-    sc = pow2_scale(__builtin_bit_cast(float, top << 16), inv);
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int d = 0; d < 4; ++d) top = max(top, max((x[j][d] << 16) & 0x7fff0000u, x[j][d] & 0x7fff0000u));
+    sc = pow2_scale(max_rows4(__builtin_bit_cast(float, top)), inv);
+  }
+  if (l2norm) {
+    float ss = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        const float a = w2f<BF>((uint16_t)x[j][d]), b = w2f<BF>((uint16_t)(x[j][d] >> 16));
+        ss = __builtin_fmaf(a, a, ss);
+        ss = __builtin_fmaf(b, b, ss);
+      }
+    f = l2_factor(sum_rows4(ss));
   }
 #pragma unroll
-  for (int i = 0; i < NV; ++i) *(h8*)(dst + (t * NV + i) * 8) = to_halves<BF>(x[i], sc);
-  return l2norm ? l2_factor(ss) * inv : inv;
+  for (int j = 0; j < NJ; ++j) {
+    y[j] = to_halves<BF>(x[j], sc);
+    if (rec) *(h8*)&rec[row][piece_at<DK>(row, 4 * j + g) * 8] = y[j];
+  }
+  return f * inv;
 }
 
 // Rows of M (LDS) to a fragment row's pair of halves with the row's own scale; returns the row factor.
@@ -187,10 +226,9 @@ __device__ __forceinline__ float store_frags(const float (*M)[kMS], int t, int l
     h8 hi, lo;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      f16 a, b;
-      split(x[2 * j + i / 4][i % 4] * sc, a, b);
-      hi[i] = a;
-      lo[i] = b;
+      const float v = x[2 * j + i / 4][i % 4];
+      hi[i] = (f16)(v * sc);
+      lo[i] = (f16)__builtin_fmaf(v, sc, -(float)hi[i]);
     }
     const int f = frag_of(t, j);
     *(h8*)out[f][0][lane] = hi;
@@ -200,118 +238,127 @@ __device__ __forceinline__ float store_frags(const float (*M)[kMS], int t, int l
 }
 
 template <int DK, bool BF>
-__global__ __launch_bounds__(256) void delta_prep_kernel(DeltaArgs a, ChunkRec* recs, int64_t slot0) {
-  __shared__ __align__(16) PrepLds<DK> L;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c = lane & 15;
-  const int rep = a.Hv / a.Hk, ng = (rep + kGroup - 1) / kGroup;
-  const int64_t bx = blockIdx.x;
-  const int hg = (int)(bx % (a.Hk * ng));
-  const int64_t slot = bx / (a.Hk * ng);
-  const int hk = hg / ng, h0 = hk * rep + (hg % ng) * kGroup;
-  const int nh = min(kGroup, (hk + 1) * rep - h0);
+__global__ __launch_bounds__(256, 2) void delta_prep_kernel(DeltaArgs a, Records<DK> recs, int64_t slot0) {
+  constexpr int NJ = DK / 32;
+  __shared__ __align__(16) PrepLds lds[4];
+  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  PrepLds& L = lds[wave];
+  const int rep = a.Hv / a.Hk, nw = (a.Hv + 3) / 4;
+  const int64_t slot = blockIdx.x / nw;
+  const int h = (int)(blockIdx.x % nw) * 4 + wave, hk = h / rep;
+  if (h >= a.Hv) return;
   int64_t tok;
   int len;
   if (!chunk_of(a, slot0 + slot, tok, len)) return;
-  ChunkRec* rec = recs + slot * a.Hv + h0;
+  ChunkRec* rec = recs.chunks + slot * a.Hv + h;
+  KeyRec<DK>* key = h % rep == 0 ? recs.keys + slot * a.Hk + hk : nullptr;  // the first of a key head's writes it
 
-  float ks, qs;
+  const Rsrc kr = rows_of(a.k + tok * a.ld_k + hk * DK, a.ld_k, len, DK);
+  const Rsrc qr = rows_of(a.q + tok * a.ld_q + hk * DK, a.ld_q, len, DK);
+  u32x4 kx[4][NJ], qx[NJ];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) load_rows<DK>(kr, a.ld_k, t, lane, kx[t]);
+  load_rows<DK>(qr, a.ld_q, 0, lane, qx);
+  double G;
   {
-    const int row = tid >> 2, t = tid & 3;
-    const bool real = row < len;
-    const float rk = prep_row<DK, BF>(a.k + (tok + row) * a.ld_k + hk * DK, L.in.k[row], t, real, a.l2norm, ks);
-    const float rq = prep_row<DK, BF>(a.q + (tok + row) * a.ld_q + hk * DK, L.in.q[row], t, real, a.l2norm, qs) * a.scale;
-    if (t == 0) {
-      L.rk[row] = rk;
-      L.rq[row] = rq;
-    }
-    for (int h = t; h < nh; h += 4) {
-      rec[h].ks[row] = ks;
-      rec[h].qs[row] = qs;
-    }
-  }
-  if (w < nh) {  // wave w: the decays of head w
     const bool real = lane < len;
-    float gv = real ? a.g[(tok + lane) * a.ld_g + h0 + w] : 0.0f;
+    const int64_t at = tok + (real ? lane : 0);
+    const float g0 = a.g[at * a.ld_g + h], b0 = a.beta[at * a.ld_beta + h];
+    float gv = real ? g0 : 0.0f;
     gv = gv < -1e5f ? -1e5f : gv;
-    double G = (double)gv * 1.4426950408889634;
+    G = (double)gv * 1.4426950408889634;
     for (int o = 1; o < 64; o <<= 1) {
       const uint64_t u = __builtin_bit_cast(uint64_t, G);
       const uint32_t lo = (uint32_t)__shfl_up((int)(uint32_t)u, o, 64), hi = (uint32_t)__shfl_up((int)(uint32_t)(u >> 32), o, 64);
       if (lane >= o) G += __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
     }
-    L.G[w][lane] = G;
-    L.be[w][lane] = real ? a.beta[(tok + lane) * a.ld_beta + h0 + w] : 0.0f;
+    L.G[lane] = G;
+    L.be[lane] = real ? b0 : 0.0f;
   }
-  __syncthreads();
-
-  // k_i.k_j and q_i.k_j: wave w has the rows of tile w
-  f32x4 kk[4], qk[4];
+  h8 k[4][NJ];
+  float rkj[4];  // of row 16 t + c
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
-    kk[t] = f32x4{0, 0, 0, 0};
-    qk[t] = f32x4{0, 0, 0, 0};
+    rkj[t] = make_rows<DK, BF>(kx[t], t, lane, a.l2norm, key ? key->k : nullptr, k[t]);
+    if (g == 0) L.rk[16 * t + c] = rkj[t];
   }
+  wave_sync();
+  double Gj[4];
 #pragma unroll
-  for (int s = 0; s < DK / 32; ++s) {
-    const h8 ka = *(const h8*)&L.in.k[16 * w + c][32 * s + 8 * g];
-    const h8 qa = *(const h8*)&L.in.q[16 * w + c][32 * s + 8 * g];
+  for (int t = 0; t < 4; ++t) Gj[t] = L.G[16 * t + c];
+
+  // Row tile by row tile: P to its fragments, A to M. e^{G_i - G_j} is taken apart at the tile's first row where
+  // j lies before it: with g <= 0 neither factor exceeds 1, so a product of two is as good as one exponential.
+  float (*M)[kMS] = L.M;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      if (t > w) continue;
-      const h8 b = *(const h8*)&L.in.k[16 * t + c][32 * s + 8 * g];
-      kk[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, b, kk[t], 0, 0, 0);
-      qk[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qa, b, qk[t], 0, 0, 0);
+  for (int w = 0; w < 4; ++w) {
+    h8 q[NJ];
+    const float rq = make_rows<DK, BF>(qx, w, lane, a.l2norm, key ? key->q : nullptr, q) * a.scale;
+    if (w < 3) load_rows<DK>(qr, a.ld_q, w + 1, lane, qx);
+    if (g == 0) L.rq[16 * w + c] = rq;
+    f32x4 kk[4], qk[4];
+#pragma unroll
+    for (int t = 0; t <= w; ++t) {
+      kk[t] = f32x4{0, 0, 0, 0};
+      qk[t] = f32x4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int t = 0; t <= w; ++t) {
+        kk[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[w][j], k[t][j], kk[t], 0, 0, 0);
+        qk[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[j], k[t][j], qk[t], 0, 0, 0);
+      }
+    wave_sync();
+    const f32x4 rqi = *(const f32x4*)&L.rq[16 * w + 4 * g], rki = *(const f32x4*)&L.rk[16 * w + 4 * g];
+    const f32x4 bei = *(const f32x4*)&L.be[16 * w + 4 * g];
+    const double G0 = L.G[16 * w];
+    double Gi[4];
+    float ei[4], fj[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      Gi[i] = L.G[16 * w + 4 * g + i];
+      ei[i] = __builtin_amdgcn_exp2f((float)(Gi[i] - G0));
+    }
+#pragma unroll
+    for (int t = 0; t < w; ++t) fj[t] = __builtin_amdgcn_exp2f((float)(G0 - Gj[t])) * rkj[t];
+    float dd[4];  // the diagonal tile, whose own differences above the diagonal may be of any size
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dd[i] = c <= 4 * g + i ? __builtin_amdgcn_exp2f((float)(Gi[i] - Gj[w])) * rkj[w] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = 16 * w + 4 * g + i;
+      const float pe = rqi[i] * ei[i];
+#pragma unroll
+      for (int t = 0; t < w; ++t) M[row][16 * t + c] = (qk[t][i] * pe) * fj[t];
+      M[row][16 * w + c] = c <= 4 * g + i ? (qk[w][i] * rqi[i]) * dd[i] : 0.0f;
+      if (!(w & 1)) M[row][16 * w + 16 + c] = 0.0f;  // the rest of the column block
+    }
+    wave_sync();
+    const float pr = store_frags(M, w, lane, rec->P);
+    if (g == 0) rec->pr[16 * w + c] = pr;
+    wave_sync();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = 16 * w + 4 * g + i;
+      const float ke = (bei[i] * rki[i]) * ei[i];
+#pragma unroll
+      for (int t = 0; t < w; ++t) M[row][16 * t + c] = (kk[t][i] * ke) * fj[t];
+      M[row][16 * w + c] = c < 4 * g + i ? (kk[w][i] * (bei[i] * rki[i])) * dd[i] : 0.0f;
     }
   }
-  __syncthreads();  // the rows are read: M takes their place
-
-  if (w < nh) {     // wave w: the row factors of head w
-    const double G = L.G[w][lane], GC = L.G[w][kC - 1];
+  wave_sync();
+  {
+    const double GC = L.G[kC - 1];
     const float eG = __builtin_amdgcn_exp2f((float)G), rk = L.rk[lane];
-    rec[w].c1[lane] = eG * rk;
-    rec[w].c2[lane] = eG * L.rq[lane];
-    rec[w].w[lane] = __builtin_amdgcn_exp2f((float)(GC - G)) * rk;
-    if (lane == 0) rec[w].dec = __builtin_amdgcn_exp2f((float)GC);
+    rec->c1[lane] = eG * rk;
+    rec->c2[lane] = eG * L.rq[lane];
+    rec->w[lane] = __builtin_amdgcn_exp2f((float)(GC - G)) * rk;
+    if (lane == 0) rec->dec = __builtin_amdgcn_exp2f((float)GC);
   }
-  for (int h = 0; h < nh; ++h) {
-    float (*M)[kMS] = L.M[h];
-    f32x4 d[4];
-    float rkj[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      if (t > w) continue;
-      const double Gj = L.G[h][16 * t + c];
-      rkj[t] = L.rk[16 * t + c];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 16 * w + 4 * g + i;
-        // (above the diagonal the difference may be of any size: it is not exponentiated)
-        d[t][i] = 16 * t + c <= row ? __builtin_amdgcn_exp2f((float)(L.G[h][row] - Gj)) : 0.0f;
-        M[row][16 * t + c] = 16 * t + c <= row ? ((qk[t][i] * L.rq[row]) * rkj[t]) * d[t][i] : 0.0f;
-      }
-    }
-    if (!(w & 1))
-#pragma unroll
-      for (int i = 0; i < 4; ++i) M[16 * w + 4 * g + i][16 * w + 16 + c] = 0.0f;  // the rest of the column block
-    wave_sync();
-    const float pr = store_frags(M, w, lane, rec[h].P);
-    if (g == 0) rec[h].pr[16 * w + c] = pr;
-    wave_sync();
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      if (t > w) continue;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 16 * w + 4 * g + i;
-        M[row][16 * t + c] = 16 * t + c < row ? (((kk[t][i] * L.rk[row]) * rkj[t]) * d[t][i]) * L.be[h][row] : 0.0f;
-      }
-    }
-  }
-  __syncthreads();
-  if (w >= nh) return;
 
-  // (I + A)^-1 of head w by 16 x 16 blocks. The diagonal blocks first: lane (b, c) solves column c of block b.
-  float (*M)[kMS] = L.M[w];
+  // (I + A)^-1 by 16 x 16 blocks. The diagonal blocks first: lane (b, c) solves column c of block b.
   {
     float x[16];
 #pragma unroll
@@ -360,7 +407,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaArgs a, ChunkRec* 
   wave_sync();
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float be = L.be[w][16 * j + c];
+    const float be = L.be[16 * j + c];
 #pragma unroll
     for (int i = j; i < 4; ++i)
 #pragma unroll
@@ -374,307 +421,384 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaArgs a, ChunkRec* 
   wave_sync();
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
-    const float tr = store_frags(M, t, lane, rec[w].T);
-    if (g == 0) rec[w].tr[16 * t + c] = tr;
+    const float tr = store_frags(M, t, lane, rec->T);
+    if (g == 0) rec->tr[16 * t + c] = tr;
   }
 }
 
 // ---------------------------------------------------------------------------------------------
-// The chain: one sequence, one value head, 64 value columns, 16 per wave. The state lies in a wave's registers
-// as 16 x 16 results (rows dk, columns dv); each wave needs nothing of the others, they share the operands
-// in LDS. The next chunk's operands are in flight in registers meanwhile.
+// The chain: one sequence, one value head, 16 NW value columns. The state lies in registers as 16 x 16 results
+// (rows of k's columns, 16 value columns per wave), and its waves need nothing of each other. NW waves (the
+// chain proper) carry the state: K S^T, U and the new state. NW others follow them: Q S^T, P U, the outputs,
+// and the loads of the next chunk's operands straight into LDS. A wave of each kind shares a SIMD, so products
+// of one fill the gaps of the other, and what the next chunk needs is off the path that the state takes.
+// Result row 4 g + i of tile 2 j + h is k's column 32 j + 8 g + 4 h + i, so that a lane's part of a 32-deep
+// operand is 16 contiguous bytes of a row of k.
 // ---------------------------------------------------------------------------------------------
 template <int DK>
+struct Operands {
+  KeyRec<DK> key;
+  f16 T[6][2][64][8];
+  float vec[384];                 // c1, c2, tr, pr, w, dec of the record
+};
+template <int DK, int NW>
 struct ChainLds {
-  f16 k[kC][DK + 8], q[kC][DK + 8];  // columns in the order 32 j + 8 g + 4 h + i for dk = 32 j + 16 h + 4 g + i
-  f16 T[6][2][64][8], P[6][2][64][8];
-  float vec[448];                    // c1, c2, tr, pr, w, ks, qs of the record
-  float dec;
+  Operands<DK> op[2];
+  f16 S[NW][DK / 32][2][64][8];   // the state before the chunk, as operands
+  f32x4 u[NW][4][64];
+  float sfac[NW][16];             // per value column: what undoes S's scaling
 };
 
-template <int DK>
-struct Stage {  // a thread's part of a chunk's operands
-  u32x4 k[DK / 32], q[DK / 32];
-  u32x4 tp[6];
-  float v0, v1;
-  float dec;
-};
-
-template <int DK>
-__device__ __forceinline__ void stage_load(const DeltaArgs& a, const ChunkRec* rec, int64_t tok, int len, int hk, Stage<DK>& s) {
-  const int tid = threadIdx.x, row = tid >> 2, t = tid & 3;
-  const bool real = row < len;
-  const uint16_t* kp = a.k + (tok + row) * a.ld_k + hk * DK;
-  const uint16_t* qp = a.q + (tok + row) * a.ld_q + hk * DK;
-#pragma unroll
-  for (int i = 0; i < DK / 32; ++i) {
-    s.k[i] = real ? *(const u32x4*)(kp + (i * 4 + t) * 8) : u32x4{0, 0, 0, 0};
-    s.q[i] = real ? *(const u32x4*)(qp + (i * 4 + t) * 8) : u32x4{0, 0, 0, 0};
-  }
-  const u32x4* r = (const u32x4*)rec;
-#pragma unroll
-  for (int i = 0; i < 6; ++i) s.tp[i] = r[i * 256 + tid];
-  const float* v = rec->c1;
-  s.v0 = v[tid];
-  s.v1 = tid < 192 ? v[256 + tid] : 0.0f;
-  s.dec = rec->dec;
+__device__ __forceinline__ float max4(const f32x4& x, float m) {
+  return fmaxf(fmaxf(m, fmaxf(__builtin_fabsf(x[0]), __builtin_fabsf(x[1]))), fmaxf(__builtin_fabsf(x[2]), __builtin_fabsf(x[3])));
 }
-
-template <int DK, bool BF>
-__device__ __forceinline__ void stage_store(const Stage<DK>& s, ChainLds<DK>& L, float ks, float qs) {
-  const int tid = threadIdx.x, row = tid >> 2, t = tid & 3;
-  // 8 columns 32 i + 8 t ..: halves h = t / 2, groups 2 (t % 2) and the next
-  const int at = 16 * (t & 1) + 4 * (t >> 1);
-#pragma unroll
-  for (int i = 0; i < DK / 32; ++i) {
-    const h8 k = to_halves<BF>(s.k[i], ks), q = to_halves<BF>(s.q[i], qs);
-    *(h4*)&L.k[row][32 * i + at] = __builtin_shufflevector(k, k, 0, 1, 2, 3);
-    *(h4*)&L.k[row][32 * i + at + 8] = __builtin_shufflevector(k, k, 4, 5, 6, 7);
-    *(h4*)&L.q[row][32 * i + at] = __builtin_shufflevector(q, q, 0, 1, 2, 3);
-    *(h4*)&L.q[row][32 * i + at + 8] = __builtin_shufflevector(q, q, 4, 5, 6, 7);
-  }
-  u32x4* d = (u32x4*)&L.T[0][0][0][0];  // T and P are adjacent here as in the record
-#pragma unroll
-  for (int i = 0; i < 6; ++i) d[i * 256 + tid] = s.tp[i];
-  L.vec[tid] = s.v0;
-  if (tid < 192) L.vec[256 + tid] = s.v1;
-  if (tid == 0) L.dec = s.dec;
-}
-
 // The pair of halves of a 32-deep operand from two results' registers, scaled.
 __device__ __forceinline__ void split8(const f32x4& x, const f32x4& y, float sc, h8& hi, h8& lo) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    f16 a, b;
-    split(x[i] * sc, a, b);
-    hi[i] = a;
-    lo[i] = b;
-    split(y[i] * sc, a, b);
-    hi[4 + i] = a;
-    lo[4 + i] = b;
+    hi[i] = (f16)(x[i] * sc);
+    hi[4 + i] = (f16)(y[i] * sc);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    lo[i] = (f16)__builtin_fmaf(x[i], sc, -(float)hi[i]);
+    lo[4 + i] = (f16)__builtin_fmaf(y[i], sc, -(float)hi[4 + i]);
   }
 }
-__device__ __forceinline__ float max4(const f32x4& x, float m) {
-  return fmaxf(fmaxf(m, fmaxf(__builtin_fabsf(x[0]), __builtin_fabsf(x[1]))), fmaxf(__builtin_fabsf(x[2]), __builtin_fabsf(x[3])));
-}
-
 template <int N>
-__device__ __forceinline__ void split_col(const f32x4 (&x)[N], h8 (&hi)[N / 2], h8 (&lo)[N / 2], float& inv) {
-  float m = 0.0f;
+__device__ __forceinline__ float col_max(const f32x4 (&x)[N], float m = 0.0f) {
 #pragma unroll
   for (int t = 0; t < N; ++t) m = max4(x[t], m);
-  const float sc = pow2_scale(max_rows4(m), inv);
+  return max_rows4(m);
+}
+template <int N>
+__device__ __forceinline__ void split_all(const f32x4 (&x)[N], float sc, h8 (&hi)[N / 2], h8 (&lo)[N / 2]) {
 #pragma unroll
   for (int j = 0; j < N / 2; ++j) split8(x[2 * j], x[2 * j + 1], sc, hi[j], lo[j]);
 }
 
+// A barrier that waits for this wave's LDS accesses alone. lds_barrier() also waits for its loads into LDS, which
+// here are for the next chunk.
+__device__ __forceinline__ void step_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 #define DELTA_MFMA(a, b, c) __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0)
 
-// y = M x for a lower triangle M of fragments and a column operand x (both pairs).
-__device__ __forceinline__ void tri_product(const f16 (*F)[2][64][8], int lane, const h8 (&xh)[2], const h8 (&xl)[2], f32x4 (&y)[4]) {
+// Fragments of a triangle in LDS or global memory.
+struct Tri {
+  h8 hi[6], lo[6];
+};
+__device__ __forceinline__ void load_tri(Tri& f, const f16 (*F)[2][64][8], int lane) {
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    f32x4 s = f32x4{0, 0, 0, 0};
+  for (int i = 0; i < 6; ++i) {
+    f.hi[i] = *(const h8*)F[i][0][lane];
+    f.lo[i] = *(const h8*)F[i][1][lane];
+  }
+}
+// y = M x (both pairs), the four row tiles in turn so that no product waits for the one before.
+__device__ __forceinline__ void tri_product(const Tri& f, const h8 (&xh)[2], const h8 (&xl)[2], f32x4 (&y)[4]) {
+  const int at[4] = {0, 1, 2, 4};
 #pragma unroll
-    for (int j = 0; j <= t / 2; ++j) {
-      const int f = t + (t > 2 ? 1 : 0) + j;
-      const h8 hi = *(const h8*)F[f][0][lane], lo = *(const h8*)F[f][1][lane];
-      s = DELTA_MFMA(lo, xh[j], s);
-      s = DELTA_MFMA(hi, xl[j], s);
-      s = DELTA_MFMA(hi, xh[j], s);
-    }
-    y[t] = s;
+  for (int t = 0; t < 4; ++t) y[t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+#pragma unroll
+    for (int t = 2 * j; t < 4; ++t) y[t] = DELTA_MFMA(f.lo[at[t] + j], xh[j], y[t]);
+#pragma unroll
+    for (int t = 2 * j; t < 4; ++t) y[t] = DELTA_MFMA(f.hi[at[t] + j], xl[j], y[t]);
+#pragma unroll
+    for (int t = 2 * j; t < 4; ++t) y[t] = DELTA_MFMA(f.hi[at[t] + j], xh[j], y[t]);
   }
 }
 
-template <int DK, bool BF>
-__global__ __launch_bounds__(256) void delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, int64_t slot0, int64_t slot1) {
-  __shared__ __align__(16) ChainLds<DK> L;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c = lane & 15;
-  const int nb = (a.Dv + 63) / 64;
-  int bx = blockIdx.x;
-  const int vb = bx % nb;
-  bx /= nb;
-  const int h = bx % a.Hv, b = bx / a.Hv, hk = h / (a.Hv / a.Hk);
-  const int dv = 64 * vb + 16 * w + c;
-  const bool active = 64 * vb + 16 * w < a.Dv;  // (whole waves)
+// y = X S^T for 64 rows X of halves in LDS (two row tiles at a time, the next two in flight).
+template <int DK>
+__device__ __forceinline__ void rows_product(const f16 (*X)[DK], int lane, const h8 (&sh)[DK / 32], const h8 (&sl)[DK / 32],
+                                             f32x4 (&y)[4]) {
+  constexpr int NJ = DK / 32;
+  const int g = lane >> 4, c = lane & 15;
+  h8 x[2][2][NJ];
+  auto load = [&](int p) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int row = 16 * (2 * p + t) + c;
+        x[p][t][j] = *(const h8*)&X[row][piece_at<DK>(row, 4 * j + g) * 8];
+      }
+  };
+  load(0);
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    if (p == 0) load(1);
+    __builtin_amdgcn_sched_barrier(0);
+    f32x4 a = f32x4{0, 0, 0, 0}, b = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      a = DELTA_MFMA(x[p][0][j], sl[j], a);
+      b = DELTA_MFMA(x[p][1][j], sl[j], b);
+      a = DELTA_MFMA(x[p][0][j], sh[j], a);
+      b = DELTA_MFMA(x[p][1][j], sh[j], b);
+    }
+    y[2 * p] = a;
+    y[2 * p + 1] = b;
+  }
+}
+
+// A chunk's operands into LDS, 1 KiB per wave and instruction, by wave w of NW.
+template <int DK, int NW>
+__device__ __forceinline__ void fetch_operands(Operands<DK>& op, const KeyRec<DK>* key, const ChunkRec* rec, int w, int lane) {
+  typedef const __attribute__((address_space(1))) void* gptr;
+  typedef __attribute__((address_space(3))) void* lptr;
+  constexpr int nk = sizeof(KeyRec<DK>) / 1024;
+  for (int i = w; i < nk; i += NW)
+    __builtin_amdgcn_global_load_lds((gptr)((const char*)key + i * 1024 + lane * 16), (lptr)((char*)&op.key + i * 1024), 16, 0, 0);
+  for (int i = w; i < 12; i += NW)
+    __builtin_amdgcn_global_load_lds((gptr)((const char*)rec + i * 1024 + lane * 16), (lptr)((char*)op.T + i * 1024), 16, 0, 0);
+  // the factors, 1536 bytes: 4 bytes per lane
+  const char* f = (const char*)rec + offsetof(ChunkRec, c1);
+  for (int i = w; i < 6; i += NW)
+    __builtin_amdgcn_global_load_lds((gptr)(f + i * 256 + lane * 4), (lptr)((char*)op.vec + i * 256), 4, 0, 0);
+}
+
+template <int DK, bool BF, int NW>
+__global__ __launch_bounds__(128 * NW, 1) void delta_chain_kernel(DeltaArgs a, Records<DK> recs, int64_t slot0, int64_t slot1) {
+  constexpr int NM = DK / 16, NJ = DK / 32;
+  __shared__ __align__(16) ChainLds<DK, NW> L;
+  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave % NW;
+  // Workgroups go to the eight dies in turn: all that share a key head run on one, next to its L2.
+  const int rep = a.Hv / a.Hk, nb = (a.Dv + 16 * NW - 1) / (16 * NW);
+  const int64_t bx = blockIdx.x, die = bx & 7, in = bx >> 3;
+  const int64_t unit = in / (rep * nb) * 8 + die;
+  if (unit >= (int64_t)a.n_seq * a.Hk) return;
+  const int vb = (int)(in % nb), hk = (int)(unit % a.Hk), b = (int)(unit / a.Hk), h = hk * rep + (int)(in / nb % rep);
+  const int dv = 16 * (NW * vb + w) + c;
+  const bool active = 16 * (NW * vb + w) < a.Dv;
   int64_t t0, t1;
   seq_range(a, b, t0, t1);
-  const int64_t key = t0 / kC + b, nch = (t1 - t0 + kC - 1) / kC;
-  int64_t cb = slot0 - key, ce = slot1 - key;  // this launch's chunks of the sequence
+  const int64_t first = t0 / kC + b, nch = (t1 - t0 + kC - 1) / kC;
+  int64_t cb = slot0 - first, ce = slot1 - first;  // this launch's chunks of the sequence
   cb = cb < 0 ? 0 : cb;
   ce = ce > nch ? nch : ce;
   if (cb >= ce && !(nch == 0 && slot0 == 0)) return;
   const int slot = slot_of(a, b);
   if (slot < 0) {
     const uint16_t fill = slot == kSlotPad ? 0 : 0x7fff;
-    if (active)
+    if (active && wave < NW)
       for (int64_t t = t0 + cb * kC + g; t < t1 && t < t0 + ce * kC; t += 4) a.out[t * a.ld_out + (int64_t)h * a.Dv + dv] = fill;
     return;
   }
-  constexpr int NM = DK / 16;
-  f32x4 S[NM];
-  const size_t so = (((size_t)slot * a.Hv + h) * a.Dv + (active ? dv : 0)) * DK + 4 * g;
-  const float* sp = (cb == 0 ? a.state : a.state_out) + so;
-#pragma unroll
-  for (int m = 0; m < NM; ++m) S[m] = *(const f32x4*)(sp + 16 * m);
-
-  Stage<DK> st;
-  const ChunkRec* rec = recs + (key + cb - slot0) * a.Hv + h;
-  uint16_t vv[16];
+  const KeyRec<DK>* key = recs.keys + (first + cb - slot0) * a.Hk + hk;
+  const ChunkRec* rec = recs.chunks + (first + cb - slot0) * a.Hv + h;
   int64_t tok = t0 + cb * kC;
-  int len = (int)(t1 - tok < kC ? t1 - tok : kC);
-  const int64_t vcol = (int64_t)h * a.Dv + (active ? dv : 0);
-  auto load_v = [&](int64_t tk, int ln) {
+  const int n = (int)(ce - cb);
+  auto len_at = [&](int64_t t) { return (int)(t1 - t < kC ? t1 - t : kC); };
+
+  if (wave < NW) {  // ------------------------------------------------------------ the state
+    f32x4 S[NM];
+    float sfac = 1.0f;  // S holds the state over sfac, a power of two per value column
+    const size_t so = (((size_t)slot * a.Hv + h) * a.Dv + (active ? dv : 0)) * DK + 8 * g;
+    const float* sp = (cb == 0 ? a.state : a.state_out) + so;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int r = 16 * (i / 4) + 4 * g + (i & 3);
-      vv[i] = r < ln ? a.v[(tk + r) * a.ld_v + vcol] : (uint16_t)0;
-    }
-  };
-  if (cb < ce) {
-    stage_load<DK>(a, rec, tok, len, hk, st);
-    load_v(tok, len);
-  }
-  for (int64_t ch = cb; ch < ce; ++ch) {
-    lds_barrier();  // every wave is done with the last chunk's operands
-    float ks = 1.0f, qs = 1.0f;
-    if constexpr (BF) {
-      ks = rec->ks[tid >> 2];
-      qs = rec->qs[tid >> 2];
-    }
-    stage_store<DK, BF>(st, L, ks, qs);
-    lds_barrier();
-    f32x4 v[4];
+    for (int m = 0; m < NM; ++m) S[m] = *(const f32x4*)(sp + 32 * (m >> 1) + 4 * (m & 1));
+    const int ldv = (int)a.ld_v * 2, vo = 4 * g * ldv + (active ? dv : c) * 2;
+    uint32_t vv[16];
+    auto load_v = [&](int64_t tk) {
+      const Rsrc r = rows_of(a.v + tk * a.ld_v + (int64_t)h * a.Dv, a.ld_v, len_at(tk), a.Dv);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i / 4][i & 3] = w2f<BF>(vv[i]);
-    const int64_t tk = tok;
-    const int ln = len;
-    if (ch + 1 < ce) {
-      rec += a.Hv;
-      tok += kC;
-      len = (int)(t1 - tok < kC ? t1 - tok : kC);
-      stage_load<DK>(a, rec, tok, len, hk, st);
-      load_v(tok, len);
-    }
-    // K S^T and Q S^T
-    h8 sh[NM / 2], sl[NM / 2];
-    float sinv;
-    split_col<NM>(S, sh, sl, sinv);
-    f32x4 ks4[4], qs4[4];
+      for (int i = 0; i < 16; ++i) vv[i] = __builtin_amdgcn_raw_buffer_load_b16(r, vo, (16 * (i / 4) + (i & 3)) * ldv, 0);
+    };
+    __builtin_amdgcn_s_waitcnt(0);  // the state is here: within the loop only v is waited for
+    if (n) load_v(tok);
+    for (int i = 0; i < n; ++i, tok += kC) {
+      const Operands<DK>& op = L.op[i & 1];
+      const f32x4* vec = (const f32x4*)op.vec;
+      h8 sh[NJ], sl[NJ];
+      float sinv;
+      const float smax = col_max<NM>(S), ssc = pow2_scale(smax, sinv);
+      split_all<NM>(S, ssc, sh, sl);
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      f32x4 x = f32x4{0, 0, 0, 0}, y = f32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int j = 0; j < NM / 2; ++j) {
-        const h8 ka = *(const h8*)&L.k[16 * t + c][32 * j + 8 * g], qa = *(const h8*)&L.q[16 * t + c][32 * j + 8 * g];
-        x = DELTA_MFMA(ka, sl[j], x);
-        x = DELTA_MFMA(ka, sh[j], x);
-        y = DELTA_MFMA(qa, sl[j], y);
-        y = DELTA_MFMA(qa, sh[j], y);
+      for (int j = 0; j < NJ; ++j) {
+        *(h8*)L.S[w][j][0][lane] = sh[j];
+        *(h8*)L.S[w][j][1][lane] = sl[j];
       }
-      ks4[t] = x;
-      qs4[t] = y;
-    }
-    const f32x4* vec = (const f32x4*)L.vec;
-    f32x4 u[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const f32x4 c1 = vec[4 * t + g];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[t][i] = __builtin_fmaf(-(c1[i] * sinv), ks4[t][i], v[t][i]);
-    }
-    h8 xh[2], xl[2];
-    float xinv;
-    split_col<4>(v, xh, xl, xinv);
-    tri_product(L.T, lane, xh, xl, u);
-    f32x4 uw[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const f32x4 tr = vec[2 * 16 + 4 * t + g], ww = vec[4 * 16 + 4 * t + g];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        u[t][i] = u[t][i] * (tr[i] * xinv);
-        uw[t][i] = u[t][i] * ww[i];
-      }
-    }
-    // the state
-    h8 wh[2], wl[2];
-    float winv;
-    split_col<4>(uw, wh, wl, winv);
-    const float dec = L.dec;
-#pragma unroll
-    for (int m = 0; m < NM; ++m) {
-      f32x4 x = f32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        // rows dk 16 m + 4 q + e of k^T: the lane's address is token 32 j + 4 g + c / 4 (then 16 more), chunk q = c % 4
-        const f16* p = &L.k[32 * j + 4 * g + (c >> 2)][32 * (m >> 1) + 8 * (c & 3) + 4 * (m & 1)];
-        const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)p);
-        const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(p + 16 * (DK + 8)));
-        const h8 ka = __builtin_bit_cast(h8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-        x = DELTA_MFMA(ka, wl[j], x);
-        x = DELTA_MFMA(ka, wh[j], x);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) S[m][i] = __builtin_fmaf(x[i], winv, dec * S[m][i]);
-    }
-    // the outputs
-    h8 uh[2], ul[2];
-    float uinv;
-    split_col<4>(u, uh, ul, uinv);
-    f32x4 o[4];
-    tri_product(L.P, lane, uh, ul, o);
-    if (active) {
+      sinv *= sfac;
+      if (g == 0) L.sfac[w][c] = sinv;
+      step_barrier();  // the operands of this chunk and the state are in LDS
+      f32x4 v[4], ks[4];
+      rows_product<DK>(op.key.k, lane, sh, sl, ks);
+      Tri T;
+      load_tri(T, op.T, lane);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const f32x4 c2 = vec[16 + 4 * t + g], pr = vec[3 * 16 + 4 * t + g];
+        const f32x4 c1 = vec[4 * t + g];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = 16 * t + 4 * g + i;
-          const float x = __builtin_fmaf(qs4[t][i], c2[i] * sinv, o[t][i] * (pr[i] * uinv));
-          if (r < ln) a.out[(tk + r) * a.ld_out + vcol] = f2w<BF>(x);
+        for (int e = 0; e < 4; ++e) v[t][e] = __builtin_fmaf(-(c1[e] * sinv), ks[t][e], w2f<BF>((uint16_t)vv[4 * t + e]));
+      }
+      load_v(i + 1 < n ? tok + kC : tok);  // (the last time for nothing: a branch would copy the registers)
+      h8 xh[2], xl[2];
+      float xinv;
+      const float xsc = pow2_scale(col_max<4>(v), xinv);
+      split_all<4>(v, xsc, xh, xl);
+      f32x4 u[4];
+      tri_product(T, xh, xl, u);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const f32x4 tr = vec[2 * 16 + 4 * t + g], ww = vec[4 * 16 + 4 * t + g];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) u[t][e] = u[t][e] * (tr[e] * xinv);
+        L.u[w][t][lane] = u[t];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) u[t][e] *= ww[e];
+      }
+      step_barrier();  // U is in LDS
+      // S1 = e^{G_C} S + U'^T K, summed on the matrix cores onto S in a scale that fits both
+      const float dec = op.vec[320];
+      float winv;
+      const float wsc = pow2_scale(fmaxf(col_max<4>(u), dec * (smax * sfac)), winv);
+      const float keep = dec * sfac * wsc;
+      sfac = winv;
+      h8 wh[2], wl[2];
+      split_all<4>(u, wsc, wh, wl);
+#pragma unroll
+      for (int m = 0; m < NM; ++m)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) S[m][e] *= keep;
+#pragma unroll
+      for (int p = 0; p < NM; p += 4) {
+        h8 ka[4][2];
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            // rows of k^T: the lane's address is token 32 j + 4 g + c / 4 (and 16 more), the four columns that
+            // result rows 4 q .. 4 q + 3 stand for, q = c % 4
+            s4 x[2];
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const int row = 32 * j + 16 * y + 4 * g + (c >> 2);
+              const f16* at = &op.key.k[row][piece_at<DK>(row, 4 * ((p + m) >> 1) + (c & 3)) * 8 + 4 * ((p + m) & 1)];
+              x[y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)at);
+            }
+            ka[m][j] = __builtin_bit_cast(h8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
+          }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int m = 0; m < 4; ++m) S[p + m] = DELTA_MFMA(ka[m][j], wl[j], S[p + m]);
+#pragma unroll
+          for (int m = 0; m < 4; ++m) S[p + m] = DELTA_MFMA(ka[m][j], wh[j], S[p + m]);
         }
       }
     }
-  }
-  if (active) {
-    float* op = a.state_out + so;
+    if (active) {
+      float* o = a.state_out + so;
 #pragma unroll
-    for (int m = 0; m < NM; ++m) *(f32x4*)(op + 16 * m) = S[m];
+      for (int m = 0; m < NM; ++m) *(f32x4*)(o + 32 * (m >> 1) + 4 * (m & 1)) = S[m] * sfac;
+    }
+    return;
+  }
+
+  // ---------------------------------------------------------------------------------- the outputs
+  const int ldo = (int)a.ld_out * 2, oo = 4 * g * ldo + dv * 2;
+  Tri P, Pn;
+  if (n) {
+    fetch_operands<DK, NW>(L.op[0], key, rec, w, lane);
+    load_tri(Pn, rec->P, lane);
+    __builtin_amdgcn_s_waitcnt(0);  // everything
+  }
+  for (int i = 0; i < n; ++i, tok += kC) {
+    const Operands<DK>& op = L.op[i & 1];
+    const f32x4* vec = (const f32x4*)op.vec;
+    P = Pn;
+    step_barrier();
+    if (i + 1 < n) {
+      key += a.Hk;
+      rec += a.Hv;
+      fetch_operands<DK, NW>(L.op[(i + 1) & 1], key, rec, w, lane);
+    }
+    load_tri(Pn, rec->P, lane);
+    h8 sh[NJ], sl[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      sh[j] = *(const h8*)L.S[w][j][0][lane];
+      sl[j] = *(const h8*)L.S[w][j][1][lane];
+    }
+    const float sinv = L.sfac[w][c];
+    f32x4 qs[4], u[4], o[4];
+    rows_product<DK>(op.key.q, lane, sh, sl, qs);
+    step_barrier();
+#pragma unroll
+    for (int t = 0; t < 4; ++t) u[t] = L.u[w][t][lane];
+    h8 uh[2], ul[2];
+    float uinv;
+    const float usc = pow2_scale(col_max<4>(u), uinv);
+    split_all<4>(u, usc, uh, ul);
+    tri_product(P, uh, ul, o);
+    // what this wave loads for the next chunk is in before it stores, so that the wait is not for the stores
+    __builtin_amdgcn_s_waitcnt(0);
+    const Rsrc orow = rows_of(a.out + tok * a.ld_out + (int64_t)h * a.Dv, a.ld_out, active ? len_at(tok) : 0, a.Dv);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const f32x4 c2 = vec[16 + 4 * t + g], pr = vec[3 * 16 + 4 * t + g];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = __builtin_fmaf(qs[t][e], c2[e] * sinv, o[t][e] * (pr[e] * uinv));
+        if (active) __builtin_amdgcn_raw_buffer_store_b16((short)f2w<BF>(x), orow, oo, (16 * t + e) * ldo, 0);
+      }
+    }
   }
 }
 
+template <int DK>
+constexpr int64_t slot_bytes(const DeltaArgs& a) {
+  return (int64_t)a.Hk * sizeof(KeyRec<DK>) + (int64_t)a.Hv * sizeof(ChunkRec);
+}
+int64_t slot_bytes(const DeltaArgs& a) { return a.Dk == 128 ? slot_bytes<128>(a) : slot_bytes<64>(a); }
+
+int64_t chunk_slots(const DeltaArgs& a) { return a.n_tokens / kC + a.n_seq; }
+
+// Chunks whose records are held at once: all, or as many as fit 1 GiB.
+int64_t slots_per_pass(const DeltaArgs& a) {
+  const int64_t all = chunk_slots(a), fit = ((int64_t)1 << 30) / slot_bytes(a);
+  return fit < 1 ? 1 : (fit < all ? fit : all);
+}
+
+template <int DK, bool BF, int NW>
+void launch_chain(const DeltaArgs& a, Records<DK> r, int64_t s0, int64_t s1, hipStream_t s) {
+  const int64_t units = (int64_t)a.n_seq * a.Hk, per = (int64_t)(a.Hv / a.Hk) * ((a.Dv + 16 * NW - 1) / (16 * NW));
+  hipLaunchKernelGGL((delta_chain_kernel<DK, BF, NW>), dim3((unsigned)((units + 7) / 8 * 8 * per)), dim3(128 * NW), 0, s, a, r, s0, s1);
+}
+
 template <int DK, bool BF>
-hipError_t launch_chunked(const DeltaArgs& a, void* ws, int64_t per, hipStream_t s) {
+hipError_t launch_chunked(const DeltaArgs& a, void* ws, hipStream_t s) {
   const int rep = a.Hv / a.Hk;
-  const int64_t ng = (int64_t)a.Hk * ((rep + kGroup - 1) / kGroup), slots = delta_chunk_slots(a.n_tokens, a.n_seq);
-  const int64_t chains = (int64_t)a.n_seq * a.Hv * ((a.Dv + 63) / 64);
-  if (chains > 0x7fffffff || per * ng > 0x7fffffff) return hipErrorInvalidValue;
-  ChunkRec* recs = (ChunkRec*)ws;
+  const int64_t ng = (a.Hv + 3) / 4, slots = chunk_slots(a), per = slots_per_pass(a);
+  const int64_t heads = (int64_t)a.n_seq * a.Hv, tiles = a.Dv / 16;
+  if ((heads + 8 * rep) * tiles > 0x7fffffff || per * ng > 0x7fffffff) return hipErrorInvalidValue;
+  const Records<DK> r{(KeyRec<DK>*)ws, (ChunkRec*)((char*)ws + per * a.Hk * sizeof(KeyRec<DK>))};
   for (int64_t s0 = 0; s0 < slots; s0 += per) {
     const int64_t n = s0 + per < slots ? per : slots - s0;
-    hipLaunchKernelGGL((delta_prep_kernel<DK, BF>), dim3((unsigned)(n * ng)), dim3(256), 0, s, a, recs, s0);
-    hipLaunchKernelGGL((delta_chain_kernel<DK, BF>), dim3((unsigned)chains), dim3(256), 0, s, a, recs, s0, s0 + n);
+    hipLaunchKernelGGL((delta_prep_kernel<DK, BF>), dim3((unsigned)(n * ng)), dim3(256), 0, s, a, r, s0);
+    if (heads * ((tiles + 1) / 2) <= 256) launch_chain<DK, BF, 1>(a, r, s0, s0 + n, s);
+    else if (heads * ((tiles + 3) / 4) <= 256) launch_chain<DK, BF, 2>(a, r, s0, s0 + n, s);
+    else launch_chain<DK, BF, 4>(a, r, s0, s0 + n, s);
   }
   return hipGetLastError();
 }
 
 }  // namespace
 
-int64_t delta_chunk_slots(int64_t n_tokens, int n_seq) { return n_tokens / kC + n_seq; }
-
-// Chunks whose records are held at once: all, or as many as fit 1 GiB.
-static int64_t slots_per_pass(const DeltaArgs& a) {
-  const int64_t all = delta_chunk_slots(a.n_tokens, a.n_seq), fit = ((int64_t)1 << 30) / ((int64_t)a.Hv * sizeof(ChunkRec));
-  return fit < 1 ? 1 : (fit < all ? fit : all);
-}
-size_t delta_chunk_workspace(const DeltaArgs& a) { return (size_t)(slots_per_pass(a) * a.Hv) * sizeof(ChunkRec); }
+size_t delta_chunk_workspace(const DeltaArgs& a) { return (size_t)(slots_per_pass(a) * slot_bytes(a)); }
 
 hipError_t launch_delta_chunked(const DeltaArgs& a, void* ws, hipStream_t s) {
-  const int64_t per = slots_per_pass(a);
-  if (a.Dk == 128) return a.bf16 ? launch_chunked<128, true>(a, ws, per, s) : launch_chunked<128, false>(a, ws, per, s);
-  return a.bf16 ? launch_chunked<64, true>(a, ws, per, s) : launch_chunked<64, false>(a, ws, per, s);
+  if (a.Dk == 128) return a.bf16 ? launch_chunked<128, true>(a, ws, s) : launch_chunked<128, false>(a, ws, s);
+  return a.bf16 ? launch_chunked<64, true>(a, ws, s) : launch_chunked<64, false>(a, ws, s);
 }
 
 }  // namespace dfssm

@@ -8,6 +8,7 @@ dfssm/libdfssm_hip.so. Flags:
   -target-feature -fma-mix-insts    no v_fma_mix*: the compiler otherwise folds
                                  fptrunc(fmul_f32(a, b)) into one fma_mix rounding the exact product
                                  straight to fp16, which differs from fp32-then-fp16 on ties
+                                 (not where no result is specified to the bit: MIX_SRCS)
 """
 from __future__ import annotations
 
@@ -26,17 +27,20 @@ LIB = os.path.join(PKG, "libdfssm_hip.so")
 # profiling variant: the one-launch layer with per-phase wall-clock stamps (-DDFSSM_TIMELINE)
 LIB_TIMELINE = os.path.join(PKG, "libdfssm_hip_timeline.so")
 TIMELINE_SRCS = ("fused.hip",)
+# the chunked delta rule splits fp32 values into pairs of halves, one fma_mix each
+MIX_SRCS = ("delta_chunk.hip",)
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc" if os.path.exists("/opt/rocm/bin/hipcc") else "hipcc")
+NO_MIX = ["-Xclang", "-target-feature", "-Xclang", "-fma-mix-insts"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
-         "-Xclang", "-target-feature", "-Xclang", "-fma-mix-insts",
          "-I" + os.path.join(REPO, "include"), "-I" + CSRC]
 
 
 def _compile(src: str, timeline: bool = False) -> str:
     obj = os.path.join(BUILD, os.path.basename(src).replace(".hip", "_tl.o" if timeline else ".o"))
-    cmd = [HIPCC] + FLAGS + (["-DDFSSM_TIMELINE"] if timeline else []) + ["-c", src, "-o", obj]
+    mix = os.path.basename(src) in MIX_SRCS
+    cmd = [HIPCC] + FLAGS + ([] if mix else NO_MIX) + (["-DDFSSM_TIMELINE"] if timeline else []) + ["-c", src, "-o", obj]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"hipcc failed for {src}:\n{r.stderr}")

@@ -376,7 +376,8 @@ typedef struct dfssm_delta {
   int32_t l2norm;
   float scale;
 } dfssm_delta;
-/* q, k, v, out, state and state_out are 16-byte aligned, ld_q, ld_k, ld_v and ld_out multiples of 8. */
+/* q, k, v, out, state and state_out are 16-byte aligned, ld_q, ld_k, ld_v and ld_out multiples of 8,
+ * every ld_* at most 2^23. */
 
 /* One token per sequence (n_tokens = n_seq). */
 int dfssm_gated_delta_step(const dfssm_delta* args, void* stream);

@@ -101,6 +101,35 @@ __device__ __forceinline__ u32x4 row_load16(Rsrc r, int voff, int soff) {
   return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, 0));
 }
 
+// max(m, |x0|, .. |x3|), in two instructions (fmaxf first makes each operand canonical, a third instruction each).
+__device__ __forceinline__ float max4(const f32x4& x, float m) {
+  asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(m) : "v"(x[0]), "v"(x[1]));
+  asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(m) : "v"(x[2]), "v"(x[3]));
+  return m;
+}
+typedef f16 h2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+// x0, x1 times sc as pairs of halves, in 5 instructions: the empty asm keeps the compiler from rounding the high
+// part a second time on the way to the low one.
+__device__ __forceinline__ void split2(float x0, float x1, float sc, h2& hi, h2& lo) {
+  hi = __builtin_convertvector(f32x2{x0 * sc, x1 * sc}, h2);
+  asm("" : "+v"(hi));
+  lo = h2{(f16)__builtin_fmaf(x0, sc, -(float)hi[0]), (f16)__builtin_fmaf(x1, sc, -(float)hi[1])};
+}
+// The pair of halves of a 32-deep operand from two results' registers, scaled.
+__device__ __forceinline__ void split8(const f32x4& x, const f32x4& y, float sc, h8& hi, h8& lo) {
+  h2 h[4], l[4];
+  split2(x[0], x[1], sc, h[0], l[0]);
+  split2(x[2], x[3], sc, h[1], l[1]);
+  split2(y[0], y[1], sc, h[2], l[2]);
+  split2(y[2], y[3], sc, h[3], l[3]);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    hi[i] = h[i / 2][i % 2];
+    lo[i] = l[i / 2][i % 2];
+  }
+}
+
 // The sequence and chunk of slot s of the launch's chunk numbering: sequence b starts at slot
 // floor(t0 / 64) + b, which needs no sums over the lengths and leaves room for every chunk. The lanes of a wave
 // look at 64 sequences at once.
@@ -215,8 +244,7 @@ __device__ __forceinline__ float store_frags(const float (*M)[kMS], int t, int l
     if (j >= nj) continue;
     x[2 * j] = *(const f32x4*)&M[r][32 * j + 4 * g];
     x[2 * j + 1] = *(const f32x4*)&M[r][32 * j + 16 + 4 * g];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) m = fmaxf(m, fmaxf(__builtin_fabsf(x[2 * j][i]), __builtin_fabsf(x[2 * j + 1][i])));
+    m = max4(x[2 * j + 1], max4(x[2 * j], m));
   }
   float inv;
   const float sc = pow2_scale(max_rows4(m), inv);
@@ -224,12 +252,7 @@ __device__ __forceinline__ float store_frags(const float (*M)[kMS], int t, int l
   for (int j = 0; j < 2; ++j) {
     if (j >= nj) continue;
     h8 hi, lo;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float v = x[2 * j + i / 4][i % 4];
-      hi[i] = (f16)(v * sc);
-      lo[i] = (f16)__builtin_fmaf(v, sc, -(float)hi[i]);
-    }
+    split8(x[2 * j], x[2 * j + 1], sc, hi, lo);
     const int f = frag_of(t, j);
     *(h8*)out[f][0][lane] = hi;
     *(h8*)out[f][1][lane] = lo;
@@ -256,10 +279,12 @@ __global__ __launch_bounds__(256, 2) void delta_prep_kernel(DeltaArgs a, Records
 
   const Rsrc kr = rows_of(a.k + tok * a.ld_k + hk * DK, a.ld_k, len, DK);
   const Rsrc qr = rows_of(a.q + tok * a.ld_q + hk * DK, a.ld_q, len, DK);
-  u32x4 kx[4][NJ], qx[NJ];
+  // All rows at once: a load issued after a store waits for the store as well.
+  u32x4 kx[4][NJ], qx[4][NJ];
 #pragma unroll
   for (int t = 0; t < 4; ++t) load_rows<DK>(kr, a.ld_k, t, lane, kx[t]);
-  load_rows<DK>(qr, a.ld_q, 0, lane, qx);
+#pragma unroll
+  for (int t = 0; t < 4; ++t) load_rows<DK>(qr, a.ld_q, t, lane, qx[t]);
   double G;
   {
     const bool real = lane < len;
@@ -294,8 +319,7 @@ __global__ __launch_bounds__(256, 2) void delta_prep_kernel(DeltaArgs a, Records
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
     h8 q[NJ];
-    const float rq = make_rows<DK, BF>(qx, w, lane, a.l2norm, key ? key->q : nullptr, q) * a.scale;
-    if (w < 3) load_rows<DK>(qr, a.ld_q, w + 1, lane, qx);
+    const float rq = make_rows<DK, BF>(qx[w], w, lane, a.l2norm, key ? key->q : nullptr, q) * a.scale;
     if (g == 0) L.rq[16 * w + c] = rq;
     f32x4 kk[4], qk[4];
 #pragma unroll
@@ -361,18 +385,18 @@ __global__ __launch_bounds__(256, 2) void delta_prep_kernel(DeltaArgs a, Records
   // (I + A)^-1 by 16 x 16 blocks. The diagonal blocks first: lane (b, c) solves column c of block b.
   {
     float x[16];
+    f32x4 m[16][4];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float s = i == c ? 1.0f : 0.0f;
+    for (int i = 1; i < 16; ++i)
 #pragma unroll
-      for (int q = 0; q < i; q += 4) {
-        const f32x4 m = *(const f32x4*)&M[16 * g + i][16 * g + q];
+      for (int q = 0; q < i; q += 4) m[i][q / 4] = *(const f32x4*)&M[16 * g + i][16 * g + q];
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (q + e < i) s = __builtin_fmaf(-m[e], x[q + e], s);
-      }
-      x[i] = s;
-    }
+    for (int i = 0; i < 16; ++i) x[i] = i == c ? 1.0f : 0.0f;
+#pragma unroll
+    for (int j = 0; j < 15; ++j)  // column by column: the updates of a step do not wait for each other
+#pragma unroll
+      for (int i = j + 1; i < 16; ++i) x[i] = __builtin_fmaf(-m[i][j / 4][j % 4], x[j], x[i]);
     wave_sync();
 #pragma unroll
     for (int i = 0; i < 16; ++i) M[16 * g + i][16 * g + c] = x[i];
@@ -386,24 +410,29 @@ __global__ __launch_bounds__(256, 2) void delta_prep_kernel(DeltaArgs a, Records
 #pragma unroll
     for (int i = 0; i < 4; ++i) X[j][j][i] = M[16 * j + 4 * g + i][16 * j + c];
 #pragma unroll
-  for (int dist = 1; dist < 4; ++dist)
+  for (int dist = 1; dist < 4; ++dist) {  // the blocks of a diagonal side by side
+    f32x4 y[3], m[3][4];
 #pragma unroll
     for (int j = 0; j + dist < 4; ++j) {
-      const int i = j + dist;
-      f32x4 y = f32x4{0, 0, 0, 0};
+      y[j] = f32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (k < j || k >= i) continue;
-        const f32x4 m = *(const f32x4*)&M[16 * i + c][16 * k + 4 * g];
-#pragma unroll
-        for (int s = 0; s < 4; ++s) y = __builtin_amdgcn_mfma_f32_16x16x4f32(m[s], X[k][j][s], y, 0, 0, 0);
-      }
-      const f32x4 m = *(const f32x4*)&M[16 * i + c][16 * i + 4 * g];
-      f32x4 z = f32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int s = 0; s < 4; ++s) z = __builtin_amdgcn_mfma_f32_16x16x4f32(m[s], -y[s], z, 0, 0, 0);
-      X[i][j] = z;
+      for (int k = 0; k <= dist; ++k) m[j][k] = *(const f32x4*)&M[16 * (j + dist) + c][16 * (j + k) + 4 * g];
     }
+#pragma unroll
+    for (int k = 0; k < dist; ++k)
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int j = 0; j + dist < 4; ++j)
+          y[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(m[j][k][s], X[j + k][j][s], y[j], 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j + dist < 4; ++j) X[j + dist][j] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int j = 0; j + dist < 4; ++j)
+        X[j + dist][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(m[j][dist][s], -y[j][s], X[j + dist][j], 0, 0, 0);
+  }
   wave_sync();
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -449,22 +478,6 @@ struct ChainLds {
   float sfac[NW][16];             // per value column: what undoes S's scaling
 };
 
-__device__ __forceinline__ float max4(const f32x4& x, float m) {
-  return fmaxf(fmaxf(m, fmaxf(__builtin_fabsf(x[0]), __builtin_fabsf(x[1]))), fmaxf(__builtin_fabsf(x[2]), __builtin_fabsf(x[3])));
-}
-// The pair of halves of a 32-deep operand from two results' registers, scaled.
-__device__ __forceinline__ void split8(const f32x4& x, const f32x4& y, float sc, h8& hi, h8& lo) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    hi[i] = (f16)(x[i] * sc);
-    hi[4 + i] = (f16)(y[i] * sc);
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    lo[i] = (f16)__builtin_fmaf(x[i], sc, -(float)hi[i]);
-    lo[4 + i] = (f16)__builtin_fmaf(y[i], sc, -(float)hi[4 + i]);
-  }
-}
 template <int N>
 __device__ __forceinline__ float col_max(const f32x4 (&x)[N], float m = 0.0f) {
 #pragma unroll
@@ -566,7 +579,7 @@ __device__ __forceinline__ void fetch_operands(Operands<DK>& op, const KeyRec<DK
 }
 
 template <int DK, bool BF, int NW>
-__global__ __launch_bounds__(128 * NW, 1) void delta_chain_kernel(DeltaArgs a, Records<DK> recs, int64_t slot0, int64_t slot1) {
+__global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(128 * NW) void delta_chain_kernel(DeltaArgs a, Records<DK> recs, int64_t slot0, int64_t slot1) {
   constexpr int NM = DK / 16, NJ = DK / 32;
   __shared__ __align__(16) ChainLds<DK, NW> L;
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;

@@ -41,7 +41,7 @@ __device__ __forceinline__ uint16_t f2w(float x) {  // RNE
   return f2h(x);
 }
 
-__device__ __forceinline__ float l2_factor(float ss) { return 1.0f / sqrt_rn(ss + 1e-6f); }
+__device__ __forceinline__ float l2_factor(float ss) { return __builtin_amdgcn_rsqf(ss + 1e-6f); }  // (1 ulp)
 
 // Tokens [t0, t1) of sequence b. Offsets read from device memory are held to [0, n_tokens] and an end
 // before its start is an empty sequence, so no value of cu reaches past the tensors.

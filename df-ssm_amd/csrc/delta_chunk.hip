@@ -95,7 +95,7 @@ __device__ __forceinline__ float max_rows4(float v) {
 // value with the zero, and waits for it there), and offsets are 32-bit.
 typedef __amdgpu_buffer_rsrc_t Rsrc;
 __device__ __forceinline__ Rsrc rows_of(const uint16_t* p, int64_t ld, int len, int dim) {
-  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, ((len - 1) * (int)ld + dim) * 2, 0x00027000);
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, len > 0 ? ((len - 1) * (int)ld + dim) * 2 : 0, 0x00027000);
 }
 __device__ __forceinline__ u32x4 row_load16(Rsrc r, int voff, int soff) {
   return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, 0));
@@ -132,8 +132,11 @@ __device__ __forceinline__ void split8(const f32x4& x, const f32x4& y, float sc,
 
 // The sequence and chunk of slot s of the launch's chunk numbering: sequence b starts at slot
 // floor(t0 / 64) + b, which needs no sums over the lengths and leaves room for every chunk. The lanes of a wave
-// look at 64 sequences at once.
-__device__ bool chunk_of(const DeltaArgs& a, int64_t s, int64_t& tok, int& len) {
+// look at 64 sequences at once, and the sequence found is kept for the slots that follow.
+struct Where {
+  int64_t first, t0, t1;  // slot, tokens of a sequence
+};
+__device__ __forceinline__ void find_seq(const DeltaArgs& a, int64_t s, Where& q) {
   const int lane = threadIdx.x & 63;
   int lo = 0, n = a.n_seq;  // the last sequence that starts at or before s is one of lo .. lo + n - 1
   while (n > 1) {
@@ -149,309 +152,342 @@ __device__ bool chunk_of(const DeltaArgs& a, int64_t s, int64_t& tok, int& len) 
     lo += (k > 0 ? k - 1 : 0) * step;
     n = min(step, end - lo);
   }
-  int64_t t0, t1;
-  seq_range(a, lo, t0, t1);
-  const int64_t c = s - (t0 / kC + lo);
-  if (c < 0 || c * kC >= t1 - t0) return false;
-  tok = t0 + c * kC;
-  len = (int)(t1 - tok < kC ? t1 - tok : kC);
-  return true;
+  seq_range(a, lo, q.t0, q.t1);
+  q.first = q.t0 / kC + lo;
+}
+// Tokens [tok, tok + len) of slot s; 0 where it holds none.
+__device__ __forceinline__ int chunk_of(const DeltaArgs& a, int64_t s, Where& q, int64_t& tok) {
+  if (s < q.first || (s - q.first) * kC >= q.t1 - q.t0) find_seq(a, s, q);
+  const int64_t c = s - q.first;
+  tok = 0;
+  if (c < 0 || c * kC >= q.t1 - q.t0) return 0;
+  tok = q.t0 + c * kC;
+  return (int)(q.t1 - tok < kC ? q.t1 - tok : kC);
 }
 
 // ---------------------------------------------------------------------------------------------
-// Preparation: one chunk and value head per wave, which needs no barrier; four to a workgroup, so that the heads
-// of a key head find its rows in the L1 cache.
+// Preparation: a chunk and value head per wave, which needs no barrier. The four waves of a workgroup take four
+// heads, which find a key head's rows in the L1 cache; a workgroup goes over several chunks, and the rows of the
+// next are on their way while it inverts.
+// Products are taken with the operands exchanged, (K Q^T)^T: a lane then holds a row's four neighbouring columns,
+// which is how the next product wants a left operand, so neither P nor A passes through LDS (but the diagonal
+// blocks of A, whose elements every lane of a block reads).
 // ---------------------------------------------------------------------------------------------
-constexpr int kMS = kC + 4;   // row stride of a matrix in LDS (floats): rows of 16-byte reads start 4 banks apart
+constexpr int kBS = 20, kBlock = 16 * kBS + 16;  // a 16 x 16 block in LDS: row and block stride, in floats
 
 struct PrepLds {              // of a wave
-  float M[kC][kMS];
+  float B[6 * kBlock];        // the diagonal blocks, then their inverses, then the blocks below the diagonal
   double G[kC];               // in units of log 2
-  float be[kC], rk[kC], rq[kC];
+  float F[3][kC];             // e^{G_16w - G_j} rk_j for the row tiles w = 1 .. 3
+  float rk[kC], kb[kC], ke[kC], be[kC], et[kC], eG[kC];
+  float ss[kC], inv[kC];
 };
+// Element c of the diagonal of a 16 x 16 result, in its lane (g = c / 4).
+__device__ __forceinline__ float diagonal(const f32x4& x, int c) {
+  return (c & 2) ? ((c & 1) ? x[3] : x[2]) : ((c & 1) ? x[1] : x[0]);
+}
 
 // 8 values of a 16-bit row as halves times sc (1 for fp16).
 template <bool BF>
 __device__ __forceinline__ h8 to_halves(u32x4 x, float sc) {
   if constexpr (!BF) return __builtin_bit_cast(h8, x);
+  h2 h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    h[i] = __builtin_convertvector(f32x2{__builtin_bit_cast(float, x[i] << 16) * sc, __builtin_bit_cast(float, x[i] & 0xffff0000u) * sc}, h2);
   h8 r;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    r[2 * i] = (f16)(__builtin_bit_cast(float, x[i] << 16) * sc);
-    r[2 * i + 1] = (f16)(__builtin_bit_cast(float, x[i] & 0xffff0000u) * sc);
-  }
+  for (int i = 0; i < 8; ++i) r[i] = h[i / 2][i % 2];
   return r;
 }
 
-__device__ __forceinline__ float sum_rows4(float v) {  // over the four lanes of a column
-  const uint32_t x = __builtin_bit_cast(uint32_t, v);
-  const auto p = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-  v = __builtin_bit_cast(float, (uint32_t)p[0]) + __builtin_bit_cast(float, (uint32_t)p[1]);
-  const uint32_t y = __builtin_bit_cast(uint32_t, v);
-  const auto q = __builtin_amdgcn_permlane32_swap(y, y, false, false);
-  return __builtin_bit_cast(float, (uint32_t)q[0]) + __builtin_bit_cast(float, (uint32_t)q[1]);
-}
-
+// 16 rows, lane (g, r): row r, columns 32 j + 8 g ..
 template <int DK>
 __device__ __forceinline__ void load_rows(Rsrc rows, int64_t ld, int t, int lane, u32x4 (&x)[DK / 32]) {
   const int off = (16 * t + (lane & 15)) * (int)ld * 2 + (lane >> 4) * 16;
 #pragma unroll
   for (int j = 0; j < DK / 32; ++j) x[j] = row_load16(rows, off, j * 64);
 }
-// 16 rows as operands (lane (g, r): row r, columns 32 j + 8 g ..), also into the key record if given. Returns the
-// factor of the lane's row, normalisation over power-of-two scale.
+// They as operands, also into the key record if given. Returns what undoes the row's scaling.
 template <int DK, bool BF>
-__device__ __forceinline__ float make_rows(const u32x4 (&x)[DK / 32], int t, int lane, bool l2norm, f16 (*rec)[DK], h8 (&y)[DK / 32]) {
+__device__ __forceinline__ float make_rows(const u32x4 (&x)[DK / 32], int t, int lane, f16 (*rec)[DK], h8 (&y)[DK / 32]) {
+  typedef unsigned short us2 __attribute__((ext_vector_type(2)));
   constexpr int NJ = DK / 32;
   const int row = 16 * t + (lane & 15), g = lane >> 4;
-  float inv = 1.0f, sc = 1.0f, f = 1.0f;
+  float inv = 1.0f, sc = 1.0f;
   if constexpr (BF) {
-    uint32_t top = 0;
+    us2 top = us2{0, 0};
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
 #pragma unroll
-      for (int d = 0; d < 4; ++d) top = max(top, max((x[j][d] << 16) & 0x7fff0000u, x[j][d] & 0x7fff0000u));
-    sc = pow2_scale(max_rows4(__builtin_bit_cast(float, top)), inv);
-  }
-  if (l2norm) {
-    float ss = 0.0f;
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        const float a = w2f<BF>((uint16_t)x[j][d]), b = w2f<BF>((uint16_t)(x[j][d] >> 16));
-        ss = __builtin_fmaf(a, a, ss);
-        ss = __builtin_fmaf(b, b, ss);
-      }
-    f = l2_factor(sum_rows4(ss));
+      for (int d = 0; d < 4; ++d) top = __builtin_elementwise_max(top, __builtin_bit_cast(us2, x[j][d] & 0x7fff7fffu));
+    sc = pow2_scale(max_rows4(__builtin_bit_cast(float, (uint32_t)max(top[0], top[1]) << 16)), inv);
   }
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
     y[j] = to_halves<BF>(x[j], sc);
     if (rec) *(h8*)&rec[row][piece_at<DK>(row, 4 * j + g) * 8] = y[j];
   }
-  return f * inv;
+  return inv;
 }
 
-// Rows of M (LDS) to a fragment row's pair of halves with the row's own scale; returns the row factor.
-__device__ __forceinline__ float store_frags(const float (*M)[kMS], int t, int lane, f16 (*out)[2][64][8]) {
-  const int g = lane >> 4, r = 16 * t + (lane & 15);
-  f32x4 x[4];
+// A row tile of a triangle, x[t] a lane's four columns of column tile t <= w, as pairs of halves with the row's
+// own scale; returns the row factor.
+__device__ __forceinline__ float store_frags(const f32x4 (&x)[4], int w, int lane, f16 (*out)[2][64][8]) {
   float m = 0.0f;
-  const int nj = t / 2 + 1;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    if (j >= nj) continue;
-    x[2 * j] = *(const f32x4*)&M[r][32 * j + 4 * g];
-    x[2 * j + 1] = *(const f32x4*)&M[r][32 * j + 16 + 4 * g];
-    m = max4(x[2 * j + 1], max4(x[2 * j], m));
-  }
+  for (int t = 0; t <= w; ++t) m = max4(x[t], m);
   float inv;
   const float sc = pow2_scale(max_rows4(m), inv);
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    if (j >= nj) continue;
+  for (int j = 0; 2 * j <= w; ++j) {
     h8 hi, lo;
-    split8(x[2 * j], x[2 * j + 1], sc, hi, lo);
-    const int f = frag_of(t, j);
+    split8(x[2 * j], 2 * j + 1 <= w ? x[2 * j + 1] : f32x4{0, 0, 0, 0}, sc, hi, lo);
+    const int f = frag_of(w, j);
     *(h8*)out[f][0][lane] = hi;
     *(h8*)out[f][1][lane] = lo;
   }
   return inv;
 }
 
+template <int DK>
+struct PrepRows {  // what is loaded ahead for a task: all of k, the first rows of q
+  u32x4 k[4][DK / 32], q[DK / 32];
+  float g, be;
+};
+
 template <int DK, bool BF>
-__global__ __launch_bounds__(256, 2) void delta_prep_kernel(DeltaArgs a, Records<DK> recs, int64_t slot0) {
+__global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(256) void delta_prep_kernel(DeltaArgs a, Records<DK> recs,
+                                                                                               int64_t slot0, int64_t n_tasks) {
   constexpr int NJ = DK / 32;
   __shared__ __align__(16) PrepLds lds[4];
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   PrepLds& L = lds[wave];
   const int rep = a.Hv / a.Hk, nw = (a.Hv + 3) / 4;
-  const int64_t slot = blockIdx.x / nw;
-  const int h = (int)(blockIdx.x % nw) * 4 + wave, hk = h / rep;
-  if (h >= a.Hv) return;
-  int64_t tok;
-  int len;
-  if (!chunk_of(a, slot0 + slot, tok, len)) return;
-  ChunkRec* rec = recs.chunks + slot * a.Hv + h;
-  KeyRec<DK>* key = h % rep == 0 ? recs.keys + slot * a.Hk + hk : nullptr;  // the first of a key head's writes it
 
-  const Rsrc kr = rows_of(a.k + tok * a.ld_k + hk * DK, a.ld_k, len, DK);
-  const Rsrc qr = rows_of(a.q + tok * a.ld_q + hk * DK, a.ld_q, len, DK);
-  // All rows at once: a load issued after a store waits for the store as well.
-  u32x4 kx[4][NJ], qx[4][NJ];
-#pragma unroll
-  for (int t = 0; t < 4; ++t) load_rows<DK>(kr, a.ld_k, t, lane, kx[t]);
-#pragma unroll
-  for (int t = 0; t < 4; ++t) load_rows<DK>(qr, a.ld_q, t, lane, qx[t]);
-  double G;
-  {
-    const bool real = lane < len;
-    const int64_t at = tok + (real ? lane : 0);
-    const float g0 = a.g[at * a.ld_g + h], b0 = a.beta[at * a.ld_beta + h];
-    float gv = real ? g0 : 0.0f;
-    gv = gv < -1e5f ? -1e5f : gv;
-    G = (double)gv * 1.4426950408889634;
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint64_t u = __builtin_bit_cast(uint64_t, G);
-      const uint32_t lo = (uint32_t)__shfl_up((int)(uint32_t)u, o, 64), hi = (uint32_t)__shfl_up((int)(uint32_t)(u >> 32), o, 64);
-      if (lane >= o) G += __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+  Where seq{0, 0, 0};
+  PrepRows<DK> in;
+  int64_t task = blockIdx.x, slot = 0;
+  int h = 0, len = 0;
+  const uint16_t* qrows = nullptr;
+  auto load = [&]() {
+    slot = task / nw;
+    h = (int)(task % nw) * 4 + wave;
+    int64_t tok;
+    len = chunk_of(a, slot0 + slot, seq, tok);
+    if (h >= a.Hv) {  // (a head there is, rows there are none)
+      len = 0;
+      h = 0;
     }
-    L.G[lane] = G;
-    L.be[lane] = real ? b0 : 0.0f;
-  }
-  h8 k[4][NJ];
-  float rkj[4];  // of row 16 t + c
+    const int hk = h / rep;
+    const Rsrc kr = rows_of(a.k + tok * a.ld_k + hk * DK, a.ld_k, len, DK);
+    qrows = a.q + tok * a.ld_q + hk * DK;
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    rkj[t] = make_rows<DK, BF>(kx[t], t, lane, a.l2norm, key ? key->k : nullptr, k[t]);
-    if (g == 0) L.rk[16 * t + c] = rkj[t];
-  }
-  wave_sync();
-  double Gj[4];
-#pragma unroll
-  for (int t = 0; t < 4; ++t) Gj[t] = L.G[16 * t + c];
-
-  // Row tile by row tile: P to its fragments, A to M. e^{G_i - G_j} is taken apart at the tile's first row where
-  // j lies before it: with g <= 0 neither factor exceeds 1, so a product of two is as good as one exponential.
-  float (*M)[kMS] = L.M;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    h8 q[NJ];
-    const float rq = make_rows<DK, BF>(qx[w], w, lane, a.l2norm, key ? key->q : nullptr, q) * a.scale;
-    if (g == 0) L.rq[16 * w + c] = rq;
-    f32x4 kk[4], qk[4];
-#pragma unroll
-    for (int t = 0; t <= w; ++t) {
-      kk[t] = f32x4{0, 0, 0, 0};
-      qk[t] = f32x4{0, 0, 0, 0};
-    }
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-      for (int t = 0; t <= w; ++t) {
-        kk[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[w][j], k[t][j], kk[t], 0, 0, 0);
-        qk[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[j], k[t][j], qk[t], 0, 0, 0);
+    for (int t = 0; t < 4; ++t) load_rows<DK>(kr, a.ld_k, t, lane, in.k[t]);
+    load_rows<DK>(rows_of(qrows, a.ld_q, len, DK), a.ld_q, 0, lane, in.q);
+    const int64_t at = tok + (lane < len ? lane : 0);
+    in.g = a.g[at * a.ld_g + h];
+    in.be = a.beta[at * a.ld_beta + h];
+  };
+  load();
+  for (;;) {
+    ChunkRec* rec = recs.chunks + slot * a.Hv + h;
+    KeyRec<DK>* key = h % rep == 0 ? recs.keys + slot * a.Hk + h / rep : nullptr;  // the first of a key head's writes it
+    const bool some = len > 0;
+    f32x4 A[4][4];
+    if (some) {
+      double G;
+      {
+        const bool real = lane < len;
+        float gv = real ? in.g : 0.0f;
+        gv = gv < -1e5f ? -1e5f : gv;
+        G = (double)gv * 1.4426950408889634;
+        for (int o = 1; o < 64; o <<= 1) {
+          const uint64_t u = __builtin_bit_cast(uint64_t, G);
+          const uint32_t lo = (uint32_t)__shfl_up((int)(uint32_t)u, o, 64), hi = (uint32_t)__shfl_up((int)(uint32_t)(u >> 32), o, 64);
+          if (lane >= o) G += __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+        }
       }
-    wave_sync();
-    const f32x4 rqi = *(const f32x4*)&L.rq[16 * w + 4 * g], rki = *(const f32x4*)&L.rk[16 * w + 4 * g];
-    const f32x4 bei = *(const f32x4*)&L.be[16 * w + 4 * g];
-    const double G0 = L.G[16 * w];
-    double Gi[4];
-    float ei[4], fj[4];
+      const float be = lane < len ? in.be : 0.0f;
+      const Rsrc qr = rows_of(qrows, a.ld_q, len, DK);
+      h8 k[4][NJ];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      Gi[i] = L.G[16 * w + 4 * g + i];
-      ei[i] = __builtin_amdgcn_exp2f((float)(Gi[i] - G0));
+      for (int t = 0; t < 4; ++t) {
+        const float ki = make_rows<DK, BF>(in.k[t], t, lane, key ? key->k : nullptr, k[t]);
+        if (BF && g == 0) L.inv[16 * t + c] = ki;
+        if (BF) __builtin_amdgcn_sched_barrier(0);  // (tile by tile: all at once take more registers than there are)
+      }
+      f32x4 kd[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        kd[t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) kd[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][j], k[t][j], kd[t], 0, 0, 0);
+      }
+      // a row's squares are on the diagonal of k k^T: in the lane of that row that has its column
+      if (a.l2norm)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          if (g == (c >> 2)) L.ss[16 * t + c] = diagonal(kd[t], c);
+      L.G[lane] = G;
+      L.be[lane] = be;
+      wave_sync();
+      {  // lane: a token
+        float rk = BF ? L.inv[lane] : 1.0f;
+        if (a.l2norm) rk *= l2_factor((L.ss[lane] * rk) * rk);
+        const double GC = L.G[kC - 1], Gt = L.G[lane & 48];
+        const float eG = __builtin_amdgcn_exp2f((float)G), et = __builtin_amdgcn_exp2f((float)(G - Gt));
+        rec->c1[lane] = eG * rk;
+        L.eG[lane] = eG;
+        rec->w[lane] = __builtin_amdgcn_exp2f((float)(GC - G)) * rk;
+        if (lane == 0) rec->dec = __builtin_amdgcn_exp2f((float)GC);
+        // e^{G_i - G_j} is taken apart at the first row of i's tile where j lies before it: with g <= 0 neither
+        // factor exceeds 1, so the product of two is as good as one exponential
+#pragma unroll
+        for (int w = 1; w < 4; ++w) {
+          const float x = (float)(L.G[16 * w] - G);
+          L.F[w - 1][lane] = __builtin_amdgcn_exp2f(lane < 16 * w ? x : 0.0f) * rk;
+        }
+        L.rk[lane] = rk;
+        L.kb[lane] = be * rk;
+        L.et[lane] = et;
+        L.ke[lane] = (be * rk) * et;
+      }
+      wave_sync();
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const int i = 16 * w + c;  // the lane's row
+        h8 q[NJ];
+        float rq = make_rows<DK, BF>(in.q, w, lane, key ? key->q : nullptr, q);
+        if (w < 3) load_rows<DK>(qr, a.ld_q, w + 1, lane, in.q);
+        f32x4 qd = f32x4{0, 0, 0, 0};
+        if (a.l2norm) {
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) qd = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[j], q[j], qd, 0, 0, 0);
+          if (g == (c >> 2)) L.ss[c] = diagonal(qd, c);
+        }
+        f32x4 P[4];
+#pragma unroll
+        for (int t = 0; t <= w; ++t) {
+          P[t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) P[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][j], q[j], P[t], 0, 0, 0);
+          A[w][t] = f32x4{0, 0, 0, 0};
+          if (t < w)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) A[w][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][j], k[w][j], A[w][t], 0, 0, 0);
+        }
+        wave_sync();
+        if (a.l2norm) rq *= l2_factor((L.ss[c] * rq) * rq);
+        wave_sync();
+        rq *= a.scale;
+        const float pe = rq * L.et[i], ke = L.ke[i], kb = L.kb[i];
+        if (g == 0) rec->c2[i] = L.eG[i] * rq;
+#pragma unroll
+        for (int t = 0; t < w; ++t) {
+          const f32x4 F = *(const f32x4*)&L.F[w - 1][16 * t + 4 * g];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            P[t][e] = (P[t][e] * pe) * F[e];
+            A[w][t][e] = (A[w][t][e] * ke) * F[e];
+          }
+        }
+        const double Gi = L.G[i];
+        const f32x4 rkj = *(const f32x4*)&L.rk[16 * w + 4 * g];
+        f32x4 D;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {  // (beyond the diagonal the difference may be of any size: not exponentiated)
+          const int j = 4 * g + e;
+          const float d = __builtin_amdgcn_exp2f(j <= c ? (float)(Gi - L.G[16 * w + j]) : 0.0f) * rkj[e];
+          P[w][e] = j <= c ? (P[w][e] * rq) * d : 0.0f;
+          D[e] = j < c ? (kd[w][e] * kb) * d : 0.0f;
+        }
+        *(f32x4*)&L.B[w * kBlock + c * kBS + 4 * g] = D;
+        const float pr = store_frags(P, w, lane, rec->P);
+        if (g == 0) rec->pr[i] = pr;
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      wave_sync();
     }
+    task += gridDim.x;
+    const bool more = task < n_tasks;
+    if (more) load();  // the registers of this task's rows are free
+    if (some) {
+      // (I + A)^-1 by 16 x 16 blocks. The diagonal blocks first: lane (b, c) solves column c of block b.
+      {
+        const float* B = &L.B[g * kBlock];
+        float x[16];
 #pragma unroll
-    for (int t = 0; t < w; ++t) fj[t] = __builtin_amdgcn_exp2f((float)(G0 - Gj[t])) * rkj[t];
-    float dd[4];  // the diagonal tile, whose own differences above the diagonal may be of any size
+        for (int i = 0; i < 16; ++i) x[i] = i == c ? 1.0f : 0.0f;
+        f32x4 m[2][4];  // a row's elements, the next row's on their way
+        m[1][0] = *(const f32x4*)&B[kBS];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) dd[i] = c <= 4 * g + i ? __builtin_amdgcn_exp2f((float)(Gi[i] - Gj[w])) * rkj[w] : 0.0f;
+        for (int i = 1; i < 16; ++i) {
+          if (i < 15)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = 16 * w + 4 * g + i;
-      const float pe = rqi[i] * ei[i];
+            for (int q = 0; q <= i; q += 4) m[(i + 1) & 1][q / 4] = *(const f32x4*)&B[(i + 1) * kBS + q];
+          float s[4] = {x[i], 0.0f, 0.0f, 0.0f};  // four partial sums, so that no addition waits for the one before
 #pragma unroll
-      for (int t = 0; t < w; ++t) M[row][16 * t + c] = (qk[t][i] * pe) * fj[t];
-      M[row][16 * w + c] = c <= 4 * g + i ? (qk[w][i] * rqi[i]) * dd[i] : 0.0f;
-      if (!(w & 1)) M[row][16 * w + 16 + c] = 0.0f;  // the rest of the column block
-    }
-    wave_sync();
-    const float pr = store_frags(M, w, lane, rec->P);
-    if (g == 0) rec->pr[16 * w + c] = pr;
-    wave_sync();
+          for (int j = 0; j < i; ++j) s[j & 3] = __builtin_fmaf(-m[i & 1][j / 4][j % 4], x[j], s[j & 3]);
+          x[i] = (s[0] + s[1]) + (s[2] + s[3]);
+        }
+        wave_sync();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = 16 * w + 4 * g + i;
-      const float ke = (bei[i] * rki[i]) * ei[i];
+        for (int i = 0; i < 16; ++i) L.B[g * kBlock + i * kBS + c] = x[i];
+        wave_sync();
+      }
+      // Then X_ij = -X_ii sum_{j <= k < i} A_ik X_kj, one block diagonal after another, in fp32 on the matrix
+      // cores. With the contraction taken in the order 4 g + s (s the step) a result is a right operand as it lies.
+      f32x4 X[4][4], D[4];
 #pragma unroll
-      for (int t = 0; t < w; ++t) M[row][16 * t + c] = (kk[t][i] * ke) * fj[t];
-      M[row][16 * w + c] = c < 4 * g + i ? (kk[w][i] * (bei[i] * rki[i])) * dd[i] : 0.0f;
-    }
-  }
-  wave_sync();
-  {
-    const double GC = L.G[kC - 1];
-    const float eG = __builtin_amdgcn_exp2f((float)G), rk = L.rk[lane];
-    rec->c1[lane] = eG * rk;
-    rec->c2[lane] = eG * L.rq[lane];
-    rec->w[lane] = __builtin_amdgcn_exp2f((float)(GC - G)) * rk;
-    if (lane == 0) rec->dec = __builtin_amdgcn_exp2f((float)GC);
-  }
-
-  // (I + A)^-1 by 16 x 16 blocks. The diagonal blocks first: lane (b, c) solves column c of block b.
-  {
-    float x[16];
-    f32x4 m[16][4];
+      for (int j = 0; j < 4; ++j) {
+        D[j] = *(const f32x4*)&L.B[j * kBlock + c * kBS + 4 * g];
 #pragma unroll
-    for (int i = 1; i < 16; ++i)
+        for (int e = 0; e < 4; ++e) X[j][j][e] = L.B[j * kBlock + (4 * g + e) * kBS + c];
+      }
+      wave_sync();
 #pragma unroll
-      for (int q = 0; q < i; q += 4) m[i][q / 4] = *(const f32x4*)&M[16 * g + i][16 * g + q];
-    __builtin_amdgcn_sched_barrier(0);
+      for (int dist = 1; dist < 4; ++dist) {
+        f32x4 y[3];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = i == c ? 1.0f : 0.0f;
+        for (int j = 0; j + dist < 4; ++j) y[j] = f32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int j = 0; j < 15; ++j)  // column by column: the updates of a step do not wait for each other
+        for (int k = 0; k < dist; ++k)
 #pragma unroll
-      for (int i = j + 1; i < 16; ++i) x[i] = __builtin_fmaf(-m[i][j / 4][j % 4], x[j], x[i]);
-    wave_sync();
+          for (int s = 0; s < 4; ++s)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) M[16 * g + i][16 * g + c] = x[i];
-    wave_sync();
-  }
-  // Then X_ij = -X_ii sum_{j <= k < i} A_ik X_kj down each block column, in fp32 on the matrix cores. With the
-  // contraction taken in the order 4 g + s (s the step), a result is the next product's operand as it lies.
-  f32x4 X[4][4];
+            for (int j = 0; j + dist < 4; ++j)
+              y[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(A[j + dist][j + k][s], X[j + k][j][s], y[j], 0, 0, 0);
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+        for (int j = 0; j + dist < 4; ++j) X[j + dist][j] = f32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) X[j][j][i] = M[16 * j + 4 * g + i][16 * j + c];
+        for (int s = 0; s < 4; ++s)
 #pragma unroll
-  for (int dist = 1; dist < 4; ++dist) {  // the blocks of a diagonal side by side
-    f32x4 y[3], m[3][4];
-#pragma unroll
-    for (int j = 0; j + dist < 4; ++j) {
-      y[j] = f32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int k = 0; k <= dist; ++k) m[j][k] = *(const f32x4*)&M[16 * (j + dist) + c][16 * (j + k) + 4 * g];
-    }
-#pragma unroll
-    for (int k = 0; k < dist; ++k)
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
+          for (int j = 0; j + dist < 4; ++j)
+            X[j + dist][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(D[j + dist][s], -y[j][s], X[j + dist][j], 0, 0, 0);
 #pragma unroll
         for (int j = 0; j + dist < 4; ++j)
-          y[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(m[j][k][s], X[j + k][j][s], y[j], 0, 0, 0);
 #pragma unroll
-    for (int j = 0; j + dist < 4; ++j) X[j + dist][j] = f32x4{0, 0, 0, 0};
+          for (int e = 0; e < 4; ++e) L.B[((j + dist) * (j + dist - 1) / 2 + j) * kBlock + (4 * g + e) * kBS + c] = X[j + dist][j][e];
+      }
+      wave_sync();
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
+      for (int w = 0; w < 4; ++w) {
+        f32x4 T[4];
 #pragma unroll
-      for (int j = 0; j + dist < 4; ++j)
-        X[j + dist][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(m[j][dist][s], -y[j][s], X[j + dist][j], 0, 0, 0);
-  }
-  wave_sync();
+        for (int t = 0; t <= w; ++t) {
+          T[t] = t == w ? D[w] : *(const f32x4*)&L.B[(w * (w - 1) / 2 + t) * kBlock + c * kBS + 4 * g];
+          const f32x4 bej = *(const f32x4*)&L.be[16 * t + 4 * g];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float be = L.be[16 * j + c];
-#pragma unroll
-    for (int i = j; i < 4; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) M[16 * i + 4 * g + e][16 * j + c] = X[i][j][e] * be;
-  }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    M[4 * g + e][16 + c] = 0.0f;
-    M[32 + 4 * g + e][48 + c] = 0.0f;
-  }
-  wave_sync();
-#pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const float tr = store_frags(M, t, lane, rec->T);
-    if (g == 0) rec->tr[16 * t + c] = tr;
+          for (int e = 0; e < 4; ++e) T[t][e] *= bej[e];
+        }
+        const float tr = store_frags(T, w, lane, rec->T);
+        if (g == 0) rec->tr[16 * w + c] = tr;
+      }
+      wave_sync();
+    }
+    if (!more) break;
   }
 }
 
@@ -797,7 +833,8 @@ hipError_t launch_chunked(const DeltaArgs& a, void* ws, hipStream_t s) {
   const Records<DK> r{(KeyRec<DK>*)ws, (ChunkRec*)((char*)ws + per * a.Hk * sizeof(KeyRec<DK>))};
   for (int64_t s0 = 0; s0 < slots; s0 += per) {
     const int64_t n = s0 + per < slots ? per : slots - s0;
-    hipLaunchKernelGGL((delta_prep_kernel<DK, BF>), dim3((unsigned)(n * ng)), dim3(256), 0, s, a, r, s0);
+    const int64_t tasks = n * ng, resident = 512;  // two workgroups to a CU
+    hipLaunchKernelGGL((delta_prep_kernel<DK, BF>), dim3((unsigned)(tasks < resident ? tasks : resident)), dim3(256), 0, s, a, r, s0, tasks);
     if (heads * ((tiles + 1) / 2) <= 256) launch_chain<DK, BF, 1>(a, r, s0, s0 + n, s);
     else if (heads * ((tiles + 3) / 4) <= 256) launch_chain<DK, BF, 2>(a, r, s0, s0 + n, s);
     else launch_chain<DK, BF, 4>(a, r, s0, s0 + n, s);

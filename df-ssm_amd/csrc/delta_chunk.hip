@@ -28,27 +28,27 @@ typedef short s4 __attribute__((ext_vector_type(4)));
 
 constexpr int kC = 64;        // tokens of a chunk
 
-// What the preparation leaves per chunk and value head. T and P are in the order in which a lane of the matrix
-// cores takes them: fragments of 16 rows x 32 columns, lane (g, r) row r, columns 4 g .. 4 g + 3 and 16 + 4 g ..,
-// the order in which 16 x 16 results lie in registers, so results are operands without moving between lanes.
-// Six fragments cover a lower triangle.
+// What the preparation leaves per chunk and value head: T in the order in which a lane of the matrix cores takes
+// it, fragments of 16 rows x 32 columns, lane (g, r) row r, columns 4 g .. 4 g + 3 and 16 + 4 g ..: the order in
+// which 16 x 16 results lie in registers, so results are operands without moving between lanes. Six fragments
+// cover a lower triangle.
 struct ChunkRec {
   f16 T[6][2][64][8];   // [fragment][hi, lo][lane]
-  f16 P[6][2][64][8];
   float c1[kC];         // e^{G_i} times k's row factor
-  float c2[kC];         // scale e^{G_i} times q's
-  float tr[kC], pr[kC]; // row factors of T and P
+  float tr[kC];         // row factor of T
   float w[kC];          // e^{G_C - G_i} times k's row factor
-  float dec;            // e^{G_C}
-  float pad[63];
+  float rk[kC];         // k's row factor: normalisation, and what undoes its scaling
+  float Gh[kC], Gl[kC]; // G_i over log 2, the float nearest and the rest
 };
-static_assert(sizeof(ChunkRec) == 26112, "T, P, 1.5 KiB of factors");
+static_assert(sizeof(ChunkRec) == 13824, "T, 1.5 KiB of factors");
 
-// Per chunk and key head: k and q as halves, rows past the sequence's end zero. The 16-byte pieces of a row are
-// exchanged so that the same piece of 16 rows, an operand, lies in all 64 LDS banks.
+// bf16 inputs, per chunk and key head: k and q as halves, rows past the sequence's end zero, and what undoes q's
+// scaling. (fp16 rows are taken as they lie.) In LDS, and here, the 16-byte pieces of a row are exchanged so that
+// the same piece of 16 rows, an operand, lies in all 64 banks.
 template <int DK>
 struct KeyRec {
   f16 k[kC][DK], q[kC][DK];
+  float qinv[kC];
 };
 template <int DK>
 __device__ __forceinline__ int piece_at(int row, int p) {
@@ -179,7 +179,7 @@ struct PrepLds {              // of a wave
   float B[6 * kBlock];        // the diagonal blocks, then their inverses, then the blocks below the diagonal
   double G[kC];               // in units of log 2
   float F[3][kC];             // e^{G_16w - G_j} rk_j for the row tiles w = 1 .. 3
-  float rk[kC], kb[kC], ke[kC], be[kC], et[kC], eG[kC];
+  float rk[kC], kb[kC], ke[kC], be[kC];
   float ss[kC], inv[kC];
 };
 // Element c of the diagonal of a 16 x 16 result, in its lane (g = c / 4).
@@ -251,8 +251,8 @@ __device__ __forceinline__ float store_frags(const f32x4 (&x)[4], int w, int lan
 }
 
 template <int DK>
-struct PrepRows {  // what is loaded ahead for a task: all of k, the first rows of q
-  u32x4 k[4][DK / 32], q[DK / 32];
+struct PrepRows {  // what is loaded ahead for a task
+  u32x4 k[4][DK / 32];
   float g, be;
 };
 
@@ -282,10 +282,9 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(256) void d
     }
     const int hk = h / rep;
     const Rsrc kr = rows_of(a.k + tok * a.ld_k + hk * DK, a.ld_k, len, DK);
-    qrows = a.q + tok * a.ld_q + hk * DK;
+    qrows = a.q + tok * a.ld_q + hk * DK;  // (bf16)
 #pragma unroll
     for (int t = 0; t < 4; ++t) load_rows<DK>(kr, a.ld_k, t, lane, in.k[t]);
-    load_rows<DK>(rows_of(qrows, a.ld_q, len, DK), a.ld_q, 0, lane, in.q);
     const int64_t at = tok + (lane < len ? lane : 0);
     in.g = a.g[at * a.ld_g + h];
     in.be = a.beta[at * a.ld_beta + h];
@@ -293,7 +292,8 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(256) void d
   load();
   for (;;) {
     ChunkRec* rec = recs.chunks + slot * a.Hv + h;
-    KeyRec<DK>* key = h % rep == 0 ? recs.keys + slot * a.Hk + h / rep : nullptr;  // the first of a key head's writes it
+    // bf16: the first of a key head's value heads writes its record
+    KeyRec<DK>* key = BF && h % rep == 0 ? recs.keys + slot * a.Hk + h / rep : nullptr;
     const bool some = len > 0;
     f32x4 A[4][4];
     if (some) {
@@ -310,7 +310,6 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(256) void d
         }
       }
       const float be = lane < len ? in.be : 0.0f;
-      const Rsrc qr = rows_of(qrows, a.ld_q, len, DK);
       h8 k[4][NJ];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -339,9 +338,10 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(256) void d
         const double GC = L.G[kC - 1], Gt = L.G[lane & 48];
         const float eG = __builtin_amdgcn_exp2f((float)G), et = __builtin_amdgcn_exp2f((float)(G - Gt));
         rec->c1[lane] = eG * rk;
-        L.eG[lane] = eG;
         rec->w[lane] = __builtin_amdgcn_exp2f((float)(GC - G)) * rk;
-        if (lane == 0) rec->dec = __builtin_amdgcn_exp2f((float)GC);
+        rec->rk[lane] = rk;
+        rec->Gh[lane] = (float)G;
+        rec->Gl[lane] = (float)(G - (double)(float)G);
         // e^{G_i - G_j} is taken apart at the first row of i's tile where j lies before it: with g <= 0 neither
         // factor exceeds 1, so the product of two is as good as one exponential
 #pragma unroll
@@ -351,47 +351,24 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(256) void d
         }
         L.rk[lane] = rk;
         L.kb[lane] = be * rk;
-        L.et[lane] = et;
         L.ke[lane] = (be * rk) * et;
       }
       wave_sync();
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const int i = 16 * w + c;  // the lane's row
-        h8 q[NJ];
-        float rq = make_rows<DK, BF>(in.q, w, lane, key ? key->q : nullptr, q);
-        if (w < 3) load_rows<DK>(qr, a.ld_q, w + 1, lane, in.q);
-        f32x4 qd = f32x4{0, 0, 0, 0};
-        if (a.l2norm) {
 #pragma unroll
-          for (int j = 0; j < NJ; ++j) qd = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[j], q[j], qd, 0, 0, 0);
-          if (g == (c >> 2)) L.ss[c] = diagonal(qd, c);
-        }
-        f32x4 P[4];
-#pragma unroll
-        for (int t = 0; t <= w; ++t) {
-          P[t] = f32x4{0, 0, 0, 0};
-#pragma unroll
-          for (int j = 0; j < NJ; ++j) P[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][j], q[j], P[t], 0, 0, 0);
+        for (int t = 0; t < w; ++t) {
           A[w][t] = f32x4{0, 0, 0, 0};
-          if (t < w)
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) A[w][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][j], k[w][j], A[w][t], 0, 0, 0);
+          for (int j = 0; j < NJ; ++j) A[w][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][j], k[w][j], A[w][t], 0, 0, 0);
         }
-        wave_sync();
-        if (a.l2norm) rq *= l2_factor((L.ss[c] * rq) * rq);
-        wave_sync();
-        rq *= a.scale;
-        const float pe = rq * L.et[i], ke = L.ke[i], kb = L.kb[i];
-        if (g == 0) rec->c2[i] = L.eG[i] * rq;
+        const float ke = L.ke[i], kb = L.kb[i];
 #pragma unroll
         for (int t = 0; t < w; ++t) {
           const f32x4 F = *(const f32x4*)&L.F[w - 1][16 * t + 4 * g];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            P[t][e] = (P[t][e] * pe) * F[e];
-            A[w][t][e] = (A[w][t][e] * ke) * F[e];
-          }
+          for (int e = 0; e < 4; ++e) A[w][t][e] = (A[w][t][e] * ke) * F[e];
         }
         const double Gi = L.G[i];
         const f32x4 rkj = *(const f32x4*)&L.rk[16 * w + 4 * g];
@@ -399,16 +376,21 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(256) void d
 #pragma unroll
         for (int e = 0; e < 4; ++e) {  // (beyond the diagonal the difference may be of any size: not exponentiated)
           const int j = 4 * g + e;
-          const float d = __builtin_amdgcn_exp2f(j <= c ? (float)(Gi - L.G[16 * w + j]) : 0.0f) * rkj[e];
-          P[w][e] = j <= c ? (P[w][e] * rq) * d : 0.0f;
+          const float d = __builtin_amdgcn_exp2f(j < c ? (float)(Gi - L.G[16 * w + j]) : 0.0f) * rkj[e];
           D[e] = j < c ? (kd[w][e] * kb) * d : 0.0f;
         }
         *(f32x4*)&L.B[w * kBlock + c * kBS + 4 * g] = D;
-        const float pr = store_frags(P, w, lane, rec->P);
-        if (g == 0) rec->pr[i] = pr;
-        __builtin_amdgcn_sched_barrier(0);
       }
       wave_sync();
+      if (key)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          u32x4 x[NJ];
+          h8 y[NJ];
+          load_rows<DK>(rows_of(qrows, a.ld_q, len, DK), a.ld_q, t, lane, x);
+          const float qi = make_rows<DK, BF>(x, t, lane, key->q, y);
+          if (g == 0) key->qinv[16 * t + c] = qi;
+        }
     }
     task += gridDim.x;
     const bool more = task < n_tasks;
@@ -493,25 +475,32 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(256) void d
 
 // ---------------------------------------------------------------------------------------------
 // The chain: one sequence, one value head, 16 NW value columns. The state lies in registers as 16 x 16 results
-// (rows of k's columns, 16 value columns per wave), and its waves need nothing of each other. NW waves (the
-// chain proper) carry the state: K S^T, U and the new state. NW others follow them: Q S^T, P U, the outputs,
-// and the loads of the next chunk's operands straight into LDS. A wave of each kind shares a SIMD, so products
-// of one fill the gaps of the other, and what the next chunk needs is off the path that the state takes.
+// (rows of k's columns, 16 value columns per wave), and the waves that carry it need nothing of each other.
+//   NW waves, the chain proper: K S^T, U and the new state
+//   NW waves, the outputs: Q S^T, P U
+//   the fetchers: the next chunk's operands, straight into LDS, and P = tril(Q K^T ..) of this one. Two waves of
+//   their own; with NW = 4 the output waves do it beside their work (12 waves would be three to a SIMD and have
+//   168 registers each, and the chain needs 224).
+// So waves of different kinds share a SIMD, products of one fill the gaps of the other, and only what the state
+// needs is on the path from chunk to chunk.
 // Result row 4 g + i of tile 2 j + h is k's column 32 j + 8 g + 4 h + i, so that a lane's part of a 32-deep
 // operand is 16 contiguous bytes of a row of k.
 // ---------------------------------------------------------------------------------------------
 template <int DK>
 struct Operands {
-  KeyRec<DK> key;
+  f16 k[kC][DK], q[kC][DK];
+  float qinv[kC];                 // (bf16)
   f16 T[6][2][64][8];
-  float vec[384];                 // c1, c2, tr, pr, w, dec of the record
+  float vec[384];                 // c1, tr, w, rk, Gh, Gl of the record
 };
 template <int DK, int NW>
 struct ChainLds {
   Operands<DK> op[2];
   f16 S[NW][DK / 32][2][64][8];   // the state before the chunk, as operands
   f32x4 u[NW][4][64];
-  float sfac[NW][16];             // per value column: what undoes S's scaling
+  f16 P[6][2][64][8];
+  float c2[kC], pr[kC];           // scale e^{G_i} times q's row factor; the row factor of P
+  float sfac[NW][16], ufac[NW][16];  // per value column: what undoes the scaling of S and of U
 };
 
 template <int N>
@@ -548,24 +537,28 @@ __device__ __forceinline__ void load_tri(Tri& f, const f16 (*F)[2][64][8], int l
     f.lo[i] = *(const h8*)F[i][1][lane];
   }
 }
-// y = M x (both pairs), the four row tiles in turn so that no product waits for the one before.
+// y = M x (both pairs; with FLIP the transpose), the four row tiles in turn so that no product waits for the one
+// before.
+template <bool FLIP>
 __device__ __forceinline__ void tri_product(const Tri& f, const h8 (&xh)[2], const h8 (&xl)[2], f32x4 (&y)[4]) {
   const int at[4] = {0, 1, 2, 4};
+  auto mm = [&](const h8& u, const h8& v, const f32x4& w) { return FLIP ? DELTA_MFMA(v, u, w) : DELTA_MFMA(u, v, w); };
 #pragma unroll
   for (int t = 0; t < 4; ++t) y[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
 #pragma unroll
-    for (int t = 2 * j; t < 4; ++t) y[t] = DELTA_MFMA(f.lo[at[t] + j], xh[j], y[t]);
+    for (int t = 2 * j; t < 4; ++t) y[t] = mm(f.lo[at[t] + j], xh[j], y[t]);
 #pragma unroll
-    for (int t = 2 * j; t < 4; ++t) y[t] = DELTA_MFMA(f.hi[at[t] + j], xl[j], y[t]);
+    for (int t = 2 * j; t < 4; ++t) y[t] = mm(f.hi[at[t] + j], xl[j], y[t]);
 #pragma unroll
-    for (int t = 2 * j; t < 4; ++t) y[t] = DELTA_MFMA(f.hi[at[t] + j], xh[j], y[t]);
+    for (int t = 2 * j; t < 4; ++t) y[t] = mm(f.hi[at[t] + j], xh[j], y[t]);
   }
 }
 
-// y = X S^T for 64 rows X of halves in LDS (two row tiles at a time, the next two in flight).
-template <int DK>
+// y = X S^T for 64 rows X of halves in LDS (two row tiles at a time, the next two in flight); with FLIP its
+// transpose, a lane then has four neighbouring value columns of a token.
+template <int DK, bool FLIP>
 __device__ __forceinline__ void rows_product(const f16 (*X)[DK], int lane, const h8 (&sh)[DK / 32], const h8 (&sl)[DK / 32],
                                              f32x4 (&y)[4]) {
   constexpr int NJ = DK / 32;
@@ -580,6 +573,7 @@ __device__ __forceinline__ void rows_product(const f16 (*X)[DK], int lane, const
         x[p][t][j] = *(const h8*)&X[row][piece_at<DK>(row, 4 * j + g) * 8];
       }
   };
+  auto mm = [&](const h8& u, const h8& v, const f32x4& w) { return FLIP ? DELTA_MFMA(v, u, w) : DELTA_MFMA(u, v, w); };
   load(0);
 #pragma unroll
   for (int p = 0; p < 2; ++p) {
@@ -588,35 +582,135 @@ __device__ __forceinline__ void rows_product(const f16 (*X)[DK], int lane, const
     f32x4 a = f32x4{0, 0, 0, 0}, b = f32x4{0, 0, 0, 0};
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-      a = DELTA_MFMA(x[p][0][j], sl[j], a);
-      b = DELTA_MFMA(x[p][1][j], sl[j], b);
-      a = DELTA_MFMA(x[p][0][j], sh[j], a);
-      b = DELTA_MFMA(x[p][1][j], sh[j], b);
+      a = mm(x[p][0][j], sl[j], a);
+      b = mm(x[p][1][j], sl[j], b);
+      a = mm(x[p][0][j], sh[j], a);
+      b = mm(x[p][1][j], sh[j], b);
     }
     y[2 * p] = a;
     y[2 * p + 1] = b;
   }
 }
 
-// A chunk's operands into LDS, 1 KiB per wave and instruction, by wave w of NW.
-template <int DK, int NW>
-__device__ __forceinline__ void fetch_operands(Operands<DK>& op, const KeyRec<DK>* key, const ChunkRec* rec, int w, int lane) {
-  typedef const __attribute__((address_space(1))) void* gptr;
-  typedef __attribute__((address_space(3))) void* lptr;
-  constexpr int nk = sizeof(KeyRec<DK>) / 1024;
-  for (int i = w; i < nk; i += NW)
-    __builtin_amdgcn_global_load_lds((gptr)((const char*)key + i * 1024 + lane * 16), (lptr)((char*)&op.key + i * 1024), 16, 0, 0);
-  for (int i = w; i < 12; i += NW)
-    __builtin_amdgcn_global_load_lds((gptr)((const char*)rec + i * 1024 + lane * 16), (lptr)((char*)op.T + i * 1024), 16, 0, 0);
+// Where a chunk's operands come from.
+template <int DK>
+struct Source {
+  const uint16_t *k, *q;  // fp16 rows
+  int64_t ld_k, ld_q;
+  int len;
+  const KeyRec<DK>* key;  // bf16
+  const ChunkRec* rec;
+};
+typedef const __attribute__((address_space(1))) void* gptr;
+typedef __attribute__((address_space(3))) void* lptr;
+
+// 64 rows of halves into LDS, KiB i, i + NP, .. of it by fetcher i: 1 KiB per wave and instruction, the lanes
+// reading the pieces that belong there.
+template <int DK, int NP>
+__device__ __forceinline__ void fetch_rows(f16 (*to)[DK], const uint16_t* p, int64_t ld, int len, int i, int lane) {
+  constexpr int per = 512 / DK, pieces = DK / 8;  // rows of a KiB, pieces of a row
+  const Rsrc r = rows_of(p, ld, len, DK);
+  const int row = lane / pieces, bytes = (int)ld * 2;
+#pragma unroll
+  for (int n = 0; n < kC / per; n += NP) {
+    const int m = n + i;
+    const int off = row * bytes + piece_at<DK>(per * m + row, lane % pieces) * 16;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr)((char*)to + m * 1024), 16, off, per * m * bytes, 0, 0);
+  }
+}
+template <int DK, bool BF, int NP>
+__device__ __forceinline__ void fetch_operands(Operands<DK>& op, const Source<DK>& s, int w, int lane) {
+  if constexpr (BF) {
+    constexpr int nk = DK * kC * 4 / 1024;
+#pragma unroll
+    for (int n = 0; n < nk; n += NP)
+      __builtin_amdgcn_global_load_lds((gptr)((const char*)s.key + (n + w) * 1024 + lane * 16), (lptr)((char*)op.k + (n + w) * 1024), 16, 0, 0);
+    if (w == 0) __builtin_amdgcn_global_load_lds((gptr)(s.key->qinv + lane), (lptr)op.qinv, 4, 0, 0);
+  } else {
+    fetch_rows<DK, NP>(op.k, s.k, s.ld_k, s.len, w, lane);
+    fetch_rows<DK, NP>(op.q, s.q, s.ld_q, s.len, w, lane);
+  }
+#pragma unroll
+  for (int n = 0; n < 12; n += NP)
+    __builtin_amdgcn_global_load_lds((gptr)((const char*)s.rec + (n + w) * 1024 + lane * 16), (lptr)((char*)op.T + (n + w) * 1024), 16, 0, 0);
   // the factors, 1536 bytes: 4 bytes per lane
-  const char* f = (const char*)rec + offsetof(ChunkRec, c1);
-  for (int i = w; i < 6; i += NW)
-    __builtin_amdgcn_global_load_lds((gptr)(f + i * 256 + lane * 4), (lptr)((char*)op.vec + i * 256), 4, 0, 0);
+  for (int n = w; n < 6; n += NP)
+    __builtin_amdgcn_global_load_lds((gptr)(s.rec->c1 + n * 64 + lane), (lptr)(op.vec + n * 64), 4, 0, 0);
 }
 
+// Row tile w of P = tril(q_i.k_j e^{G_i - G_j}) and of q's factors.
 template <int DK, bool BF, int NW>
-__global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(128 * NW) void delta_chain_kernel(DeltaArgs a, Records<DK> recs, int64_t slot0, int64_t slot1) {
-  constexpr int NM = DK / 16, NJ = DK / 32;
+__device__ __forceinline__ void make_p(ChainLds<DK, NW>& L, const Operands<DK>& op, int w, int lane, bool l2norm, float scale) {
+  constexpr int NJ = DK / 32;
+  const int g = lane >> 4, c = lane & 15, i = 16 * w + c;
+  const float *rk = op.vec + 192, *Gh = op.vec + 256, *Gl = op.vec + 320;
+  h8 q[NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) q[j] = *(const h8*)&op.q[i][piece_at<DK>(i, 4 * j + g) * 8];
+  f32x4 x[4], qq = f32x4{0, 0, 0, 0};
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    x[t] = f32x4{0, 0, 0, 0};
+    if (t <= w) {
+      const int row = 16 * t + c;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) x[t] = DELTA_MFMA(*(const h8*)&op.k[row][piece_at<DK>(row, 4 * j + g) * 8], q[j], x[t]);
+    }
+  }
+  float rq = BF ? op.qinv[i] : 1.0f;
+  if (l2norm) {  // the squares are the diagonal of q q^T; lane (c / 4, c) has it for row c
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) qq = DELTA_MFMA(q[j], q[j], qq);
+    const float ss = __shfl(diagonal(qq, c), 16 * (c >> 2) + c, 64);
+    rq *= l2_factor((ss * rq) * rq);
+  }
+  rq *= scale;
+  const float gh = Gh[i], gl = Gl[i], bh = Gh[16 * w], bl = Gl[16 * w];
+  const float pe = rq * __builtin_amdgcn_exp2f((gh - bh) + (gl - bl));
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    if (t > w) continue;
+    const f32x4 jh = *(const f32x4*)&Gh[16 * t + 4 * g], jl = *(const f32x4*)&Gl[16 * t + 4 * g];
+    const f32x4 rj = *(const f32x4*)&rk[16 * t + 4 * g];
+    if (t < w) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[t][e] = (x[t][e] * pe) * (__builtin_amdgcn_exp2f((bh - jh[e]) + (bl - jl[e])) * rj[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool in = 4 * g + e <= c;
+        const float d = __builtin_amdgcn_exp2f(in ? (gh - jh[e]) + (gl - jl[e]) : 0.0f) * rj[e];
+        x[t][e] = in ? (x[t][e] * rq) * d : 0.0f;
+      }
+    }
+  }
+  float m = 0.0f, inv;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) m = max4(x[t], m);
+  const float sc = pow2_scale(max_rows4(m), inv);
+  h8 hi, lo;
+  const int f = frag_of(w, 0);
+  split8(x[0], x[1], sc, hi, lo);
+  *(h8*)L.P[f][0][lane] = hi;
+  *(h8*)L.P[f][1][lane] = lo;
+  if (w >= 2) {
+    split8(x[2], x[3], sc, hi, lo);
+    *(h8*)L.P[f + 1][0][lane] = hi;
+    *(h8*)L.P[f + 1][1][lane] = lo;
+  }
+  if (g == 0) {
+    L.pr[i] = inv;
+    L.c2[i] = rq * __builtin_amdgcn_exp2f(gh + gl);
+  }
+}
+
+template <int NW>
+constexpr int kFetchers = NW == 4 ? 0 : 2;  // waves of their own
+
+template <int DK, bool BF, int NW>
+__global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(64 * (2 * NW + kFetchers<NW>)) void
+delta_chain_kernel(DeltaArgs a, Records<DK> recs, int64_t slot0, int64_t slot1) {
+  constexpr int NM = DK / 16, NJ = DK / 32, NF = kFetchers<NW>, NP = NF ? NF : NW;
   __shared__ __align__(16) ChainLds<DK, NW> L;
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave % NW;
@@ -626,8 +720,8 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(128 * NW) v
   const int64_t unit = in / (rep * nb) * 8 + die;
   if (unit >= (int64_t)a.n_seq * a.Hk) return;
   const int vb = (int)(in % nb), hk = (int)(unit % a.Hk), b = (int)(unit / a.Hk), h = hk * rep + (int)(in / nb % rep);
-  const int dv = 16 * (NW * vb + w) + c;
-  const bool active = 16 * (NW * vb + w) < a.Dv;
+  const int dv0 = 16 * (NW * vb + w), dv = dv0 + c;
+  const bool active = dv0 < a.Dv;
   int64_t t0, t1;
   seq_range(a, b, t0, t1);
   const int64_t first = t0 / kC + b, nch = (t1 - t0 + kC - 1) / kC;
@@ -642,8 +736,6 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(128 * NW) v
       for (int64_t t = t0 + cb * kC + g; t < t1 && t < t0 + ce * kC; t += 4) a.out[t * a.ld_out + (int64_t)h * a.Dv + dv] = fill;
     return;
   }
-  const KeyRec<DK>* key = recs.keys + (first + cb - slot0) * a.Hk + hk;
-  const ChunkRec* rec = recs.chunks + (first + cb - slot0) * a.Hv + h;
   int64_t tok = t0 + cb * kC;
   const int n = (int)(ce - cb);
   auto len_at = [&](int64_t t) { return (int)(t1 - t < kC ? t1 - t : kC); };
@@ -680,7 +772,7 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(128 * NW) v
       if (g == 0) L.sfac[w][c] = sinv;
       step_barrier();  // the operands of this chunk and the state are in LDS
       f32x4 v[4], ks[4];
-      rows_product<DK>(op.key.k, lane, sh, sl, ks);
+      rows_product<DK, false>(op.k, lane, sh, sl, ks);
       Tri T;
       load_tri(T, op.T, lane);
 #pragma unroll
@@ -695,10 +787,10 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(128 * NW) v
       const float xsc = pow2_scale(col_max<4>(v), xinv);
       split_all<4>(v, xsc, xh, xl);
       f32x4 u[4];
-      tri_product(T, xh, xl, u);
+      tri_product<false>(T, xh, xl, u);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const f32x4 tr = vec[2 * 16 + 4 * t + g], ww = vec[4 * 16 + 4 * t + g];
+        const f32x4 tr = vec[16 + 4 * t + g], ww = vec[2 * 16 + 4 * t + g];
 #pragma unroll
         for (int e = 0; e < 4; ++e) u[t][e] = u[t][e] * (tr[e] * xinv);
         L.u[w][t][lane] = u[t];
@@ -707,7 +799,7 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(128 * NW) v
       }
       step_barrier();  // U is in LDS
       // S1 = e^{G_C} S + U'^T K, summed on the matrix cores onto S in a scale that fits both
-      const float dec = op.vec[320];
+      const float dec = __builtin_amdgcn_exp2f(op.vec[256 + kC - 1] + op.vec[320 + kC - 1]);
       float winv;
       const float wsc = pow2_scale(fmaxf(col_max<4>(u), dec * (smax * sfac)), winv);
       const float keep = dec * sfac * wsc;
@@ -731,7 +823,7 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(128 * NW) v
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
               const int row = 32 * j + 16 * y + 4 * g + (c >> 2);
-              const f16* at = &op.key.k[row][piece_at<DK>(row, 4 * ((p + m) >> 1) + (c & 3)) * 8 + 4 * ((p + m) & 1)];
+              const f16* at = &op.k[row][piece_at<DK>(row, 4 * ((p + m) >> 1) + (c & 3)) * 8 + 4 * ((p + m) & 1)];
               x[y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)at);
             }
             ka[m][j] = __builtin_bit_cast(h8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
@@ -753,52 +845,76 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(128 * NW) v
     return;
   }
 
-  // ---------------------------------------------------------------------------------- the outputs
-  const int ldo = (int)a.ld_out * 2, oo = 4 * g * ldo + dv * 2;
-  Tri P, Pn;
-  if (n) {
-    fetch_operands<DK, NW>(L.op[0], key, rec, w, lane);
-    load_tri(Pn, rec->P, lane);
-    __builtin_amdgcn_s_waitcnt(0);  // everything
+  // -------------------------------------------------------------------- the fetchers and the outputs
+  const KeyRec<DK>* key = recs.keys + (first + cb - slot0) * a.Hk + hk;
+  const ChunkRec* rec = recs.chunks + (first + cb - slot0) * a.Hv + h;
+  const bool outputs = wave < 2 * NW, fetches = !NF || !outputs;
+  const int fi = NF ? wave - 2 * NW : w;  // which fetcher
+  auto fetch = [&](int i) {               // chunk i of the launch's
+    const int64_t tk = t0 + (cb + i) * kC;
+    const Source<DK> s{a.k + tk * a.ld_k + hk * DK, a.q + tk * a.ld_q + hk * DK, a.ld_k, a.ld_q, len_at(tk),
+                       key + (int64_t)i * a.Hk, rec + (int64_t)i * a.Hv};
+    fetch_operands<DK, BF, NP>(L.op[i & 1], s, fi, lane);
+  };
+  const int ldo = (int)a.ld_out * 2, oo = c * ldo + (dv0 + 4 * g) * 2;
+  if (fetches && n) {
+    fetch(0);
+    __builtin_amdgcn_s_waitcnt(0);
   }
   for (int i = 0; i < n; ++i, tok += kC) {
     const Operands<DK>& op = L.op[i & 1];
-    const f32x4* vec = (const f32x4*)op.vec;
-    P = Pn;
     step_barrier();
-    if (i + 1 < n) {
-      key += a.Hk;
-      rec += a.Hv;
-      fetch_operands<DK, NW>(L.op[(i + 1) & 1], key, rec, w, lane);
+    if (fetches) {
+      if (i + 1 < n) fetch(i + 1);
+      if constexpr (NP == 2) {  // five of the triangle's ten tiles each
+        make_p<DK, BF>(L, op, fi, lane, a.l2norm, a.scale);
+        make_p<DK, BF>(L, op, 3 - fi, lane, a.l2norm, a.scale);
+      } else {
+        make_p<DK, BF>(L, op, fi, lane, a.l2norm, a.scale);
+      }
     }
-    load_tri(Pn, rec->P, lane);
-    h8 sh[NJ], sl[NJ];
+    f32x4 qs[4];
+    f32x4 sinv;
+    if (outputs) {
+      h8 sh[NJ], sl[NJ];
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      sh[j] = *(const h8*)L.S[w][j][0][lane];
-      sl[j] = *(const h8*)L.S[w][j][1][lane];
+      for (int j = 0; j < NJ; ++j) {
+        sh[j] = *(const h8*)L.S[w][j][0][lane];
+        sl[j] = *(const h8*)L.S[w][j][1][lane];
+      }
+      sinv = *(const f32x4*)&L.sfac[w][4 * g];
+      rows_product<DK, true>(op.q, lane, sh, sl, qs);
     }
-    const float sinv = L.sfac[w][c];
-    f32x4 qs[4], u[4], o[4];
-    rows_product<DK>(op.key.q, lane, sh, sl, qs);
     step_barrier();
+    f32x4 o[4];
+    f32x4 uinv;
+    if (outputs) {
+      Tri P;
+      load_tri(P, L.P, lane);
+      f32x4 u[4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) u[t] = L.u[w][t][lane];
-    h8 uh[2], ul[2];
-    float uinv;
-    const float usc = pow2_scale(col_max<4>(u), uinv);
-    split_all<4>(u, usc, uh, ul);
-    tri_product(P, uh, ul, o);
+      for (int t = 0; t < 4; ++t) u[t] = L.u[w][t][lane];
+      h8 uh[2], ul[2];
+      float inv;
+      const float usc = pow2_scale(col_max<4>(u), inv);
+      if (g == 0) L.ufac[w][c] = inv;
+      split_all<4>(u, usc, uh, ul);
+      tri_product<true>(P, uh, ul, o);
+      wave_sync();
+      uinv = *(const f32x4*)&L.ufac[w][4 * g];
+    }
     // what this wave loads for the next chunk is in before it stores, so that the wait is not for the stores
-    __builtin_amdgcn_s_waitcnt(0);
-    const Rsrc orow = rows_of(a.out + tok * a.ld_out + (int64_t)h * a.Dv, a.ld_out, active ? len_at(tok) : 0, a.Dv);
+    if (fetches) __builtin_amdgcn_s_waitcnt(0);
+    if (outputs && active) {
+      const Rsrc orow = rows_of(a.out + tok * a.ld_out + (int64_t)h * a.Dv, a.ld_out, len_at(tok), a.Dv);
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const f32x4 c2 = vec[16 + 4 * t + g], pr = vec[3 * 16 + 4 * t + g];
+      for (int t = 0; t < 4; ++t) {
+        const float c2 = L.c2[16 * t + c], pr = L.pr[16 * t + c];
+        uint32_t x[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x = __builtin_fmaf(qs[t][e], c2[e] * sinv, o[t][e] * (pr[e] * uinv));
-        if (active) __builtin_amdgcn_raw_buffer_store_b16((short)f2w<BF>(x), orow, oo, (16 * t + e) * ldo, 0);
+        for (int e = 0; e < 4; ++e) x[e] = f2w<BF>(__builtin_fmaf(qs[t][e], c2 * sinv[e], o[t][e] * (pr * uinv[e])));
+        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2{x[0] | x[1] << 16, x[2] | x[3] << 16}, orow, oo, 16 * t * ldo, 0);
       }
     }
   }
@@ -806,7 +922,7 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(128 * NW) v
 
 template <int DK>
 constexpr int64_t slot_bytes(const DeltaArgs& a) {
-  return (int64_t)a.Hk * sizeof(KeyRec<DK>) + (int64_t)a.Hv * sizeof(ChunkRec);
+  return (a.bf16 ? (int64_t)a.Hk * sizeof(KeyRec<DK>) : 0) + (int64_t)a.Hv * sizeof(ChunkRec);
 }
 int64_t slot_bytes(const DeltaArgs& a) { return a.Dk == 128 ? slot_bytes<128>(a) : slot_bytes<64>(a); }
 
@@ -821,7 +937,7 @@ int64_t slots_per_pass(const DeltaArgs& a) {
 template <int DK, bool BF, int NW>
 void launch_chain(const DeltaArgs& a, Records<DK> r, int64_t s0, int64_t s1, hipStream_t s) {
   const int64_t units = (int64_t)a.n_seq * a.Hk, per = (int64_t)(a.Hv / a.Hk) * ((a.Dv + 16 * NW - 1) / (16 * NW));
-  hipLaunchKernelGGL((delta_chain_kernel<DK, BF, NW>), dim3((unsigned)((units + 7) / 8 * 8 * per)), dim3(128 * NW), 0, s, a, r, s0, s1);
+  hipLaunchKernelGGL((delta_chain_kernel<DK, BF, NW>), dim3((unsigned)((units + 7) / 8 * 8 * per)), dim3(64 * (2 * NW + kFetchers<NW>)), 0, s, a, r, s0, s1);
 }
 
 template <int DK, bool BF>
@@ -830,7 +946,7 @@ hipError_t launch_chunked(const DeltaArgs& a, void* ws, hipStream_t s) {
   const int64_t ng = (a.Hv + 3) / 4, slots = chunk_slots(a), per = slots_per_pass(a);
   const int64_t heads = (int64_t)a.n_seq * a.Hv, tiles = a.Dv / 16;
   if ((heads + 8 * rep) * tiles > 0x7fffffff || per * ng > 0x7fffffff) return hipErrorInvalidValue;
-  const Records<DK> r{(KeyRec<DK>*)ws, (ChunkRec*)((char*)ws + per * a.Hk * sizeof(KeyRec<DK>))};
+  const Records<DK> r{(KeyRec<DK>*)ws, (ChunkRec*)((char*)ws + (BF ? per * a.Hk * sizeof(KeyRec<DK>) : 0))};
   for (int64_t s0 = 0; s0 < slots; s0 += per) {
     const int64_t n = s0 + per < slots ? per : slots - s0;
     const int64_t tasks = n * ng, resident = 512;  // two workgroups to a CU

@@ -62,6 +62,11 @@ struct Records {
   ChunkRec* chunks;
 };
 
+template <int N>
+struct Int {
+  static constexpr int value = N;
+};
+
 __device__ __forceinline__ int frag_of(int t, int j) { return t + (t > 2 ? 1 : 0) + j; }  // row tile, column block
 
 // LDS written by other lanes of the same wave is read after this.
@@ -231,19 +236,21 @@ __device__ __forceinline__ float make_rows(const u32x4 (&x)[DK / 32], int t, int
   return inv;
 }
 
-// A row tile of a triangle, x[t] a lane's four columns of column tile t <= w, as pairs of halves with the row's
+// Row tile W of a triangle, x[t] a lane's four columns of column tile t <= W, as pairs of halves with the row's
 // own scale; returns the row factor.
-__device__ __forceinline__ float store_frags(const f32x4 (&x)[4], int w, int lane, f16 (*out)[2][64][8]) {
+template <int W>
+__device__ __forceinline__ float store_frags(const f32x4 (&x)[W + 1], int lane, f16 (*out)[2][64][8]) {
   float m = 0.0f;
 #pragma unroll
-  for (int t = 0; t <= w; ++t) m = max4(x[t], m);
+  for (int t = 0; t <= W; ++t) m = max4(x[t], m);
   float inv;
   const float sc = pow2_scale(max_rows4(m), inv);
 #pragma unroll
-  for (int j = 0; 2 * j <= w; ++j) {
+  for (int j = 0; 2 * j <= W; ++j) {
     h8 hi, lo;
-    split8(x[2 * j], 2 * j + 1 <= w ? x[2 * j + 1] : f32x4{0, 0, 0, 0}, sc, hi, lo);
-    const int f = frag_of(w, j);
+    if (2 * j + 1 <= W) split8(x[2 * j], x[2 * j + 1 <= W ? 2 * j + 1 : W], sc, hi, lo);
+    else split8(x[2 * j], f32x4{0, 0, 0, 0}, sc, hi, lo);
+    const int f = frag_of(W, j);
     *(h8*)out[f][0][lane] = hi;
     *(h8*)out[f][1][lane] = lo;
   }
@@ -454,19 +461,23 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(256) void d
           for (int e = 0; e < 4; ++e) L.B[((j + dist) * (j + dist - 1) / 2 + j) * kBlock + (4 * g + e) * kBS + c] = X[j + dist][j][e];
       }
       wave_sync();
+      auto store_t = [&](auto tile) {
+        constexpr int W = decltype(tile)::value;
+        f32x4 T[W + 1];
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        f32x4 T[4];
-#pragma unroll
-        for (int t = 0; t <= w; ++t) {
-          T[t] = t == w ? D[w] : *(const f32x4*)&L.B[(w * (w - 1) / 2 + t) * kBlock + c * kBS + 4 * g];
+        for (int t = 0; t <= W; ++t) {
+          T[t] = t == W ? D[W] : *(const f32x4*)&L.B[(W * (W - 1) / 2 + t) * kBlock + c * kBS + 4 * g];
           const f32x4 bej = *(const f32x4*)&L.be[16 * t + 4 * g];
 #pragma unroll
           for (int e = 0; e < 4; ++e) T[t][e] *= bej[e];
         }
-        const float tr = store_frags(T, w, lane, rec->T);
-        if (g == 0) rec->tr[16 * w + c] = tr;
-      }
+        const float tr = store_frags<W>(T, lane, rec->T);
+        if (g == 0) rec->tr[16 * W + c] = tr;
+      };
+      store_t(Int<0>{});
+      store_t(Int<1>{});
+      store_t(Int<2>{});
+      store_t(Int<3>{});
       wave_sync();
     }
     if (!more) break;
@@ -478,8 +489,8 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(256) void d
 // (rows of k's columns, 16 value columns per wave), and the waves that carry it need nothing of each other.
 //   NW waves, the chain proper: K S^T, U and the new state
 //   NW waves, the outputs: Q S^T, P U
-//   the fetchers: the next chunk's operands, straight into LDS, and P = tril(Q K^T ..) of this one. Two waves of
-//   their own; with NW = 4 the output waves do it beside their work (12 waves would be three to a SIMD and have
+//   four fetchers: the next chunk's operands, straight into LDS, and a row tile each of this one's P = tril(Q K^T
+//   ..). Waves of their own; with NW = 4 the output waves do it beside their work (12 waves would be three to a SIMD and have
 //   168 registers each, and the chain needs 224).
 // So waves of different kinds share a SIMD, products of one fill the gaps of the other, and only what the state
 // needs is on the path from chunk to chunk.
@@ -499,6 +510,7 @@ struct ChainLds {
   f16 S[NW][DK / 32][2][64][8];   // the state before the chunk, as operands
   f32x4 u[NW][4][64];
   f16 P[6][2][64][8];
+  float F[3][kC];                 // of P's row tiles 1 .. 3, see make_p
   float c2[kC], pr[kC];           // scale e^{G_i} times q's row factor; the row factor of P
   float sfac[NW][16], ufac[NW][16];  // per value column: what undoes the scaling of S and of U
 };
@@ -638,66 +650,60 @@ __device__ __forceinline__ void fetch_operands(Operands<DK>& op, const Source<DK
     __builtin_amdgcn_global_load_lds((gptr)(s.rec->c1 + n * 64 + lane), (lptr)(op.vec + n * 64), 4, 0, 0);
 }
 
-// Row tile w of P = tril(q_i.k_j e^{G_i - G_j}) and of q's factors.
-template <int DK, bool BF, int NW>
-__device__ __forceinline__ void make_p(ChainLds<DK, NW>& L, const Operands<DK>& op, int w, int lane, bool l2norm, float scale) {
+// Row tile W of P = tril(q_i.k_j e^{G_i - G_j}) and of q's factors.
+template <int W, int DK, bool BF, int NW>
+__device__ __forceinline__ void make_p(ChainLds<DK, NW>& L, const Operands<DK>& op, int lane, bool l2norm, float scale) {
   constexpr int NJ = DK / 32;
-  const int g = lane >> 4, c = lane & 15, i = 16 * w + c;
+  const int g = lane >> 4, c = lane & 15, i = 16 * W + c;
   const float *rk = op.vec + 192, *Gh = op.vec + 256, *Gl = op.vec + 320;
-  h8 q[NJ];
+  const float bh = Gh[16 * W], bl = Gl[16 * W];
+  // e^{G_i - G_j} for a j before the tile is taken apart at the tile's first row, as in the preparation
+  if constexpr (W > 0)
+    if (lane < 16 * W) L.F[W - 1][lane] = __builtin_amdgcn_exp2f((bh - Gh[lane]) + (bl - Gl[lane])) * rk[lane];
+  h8 q[NJ], k[W + 1][NJ];
 #pragma unroll
   for (int j = 0; j < NJ; ++j) q[j] = *(const h8*)&op.q[i][piece_at<DK>(i, 4 * j + g) * 8];
-  f32x4 x[4], qq = f32x4{0, 0, 0, 0};
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    x[t] = f32x4{0, 0, 0, 0};
-    if (t <= w) {
-      const int row = 16 * t + c;
+  for (int t = 0; t <= W; ++t)
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) x[t] = DELTA_MFMA(*(const h8*)&op.k[row][piece_at<DK>(row, 4 * j + g) * 8], q[j], x[t]);
-    }
+    for (int j = 0; j < NJ; ++j) k[t][j] = *(const h8*)&op.k[16 * t + c][piece_at<DK>(16 * t + c, 4 * j + g) * 8];
+  f32x4 x[W + 1], qq = f32x4{0, 0, 0, 0};
+#pragma unroll
+  for (int t = 0; t <= W; ++t) x[t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    if (l2norm) qq = DELTA_MFMA(q[j], q[j], qq);
+#pragma unroll
+    for (int t = 0; t <= W; ++t) x[t] = DELTA_MFMA(k[t][j], q[j], x[t]);
   }
+  const float gh = Gh[i], gl = Gl[i];
   float rq = BF ? op.qinv[i] : 1.0f;
   if (l2norm) {  // the squares are the diagonal of q q^T; lane (c / 4, c) has it for row c
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) qq = DELTA_MFMA(q[j], q[j], qq);
     const float ss = __shfl(diagonal(qq, c), 16 * (c >> 2) + c, 64);
     rq *= l2_factor((ss * rq) * rq);
   }
   rq *= scale;
-  const float gh = Gh[i], gl = Gl[i], bh = Gh[16 * w], bl = Gl[16 * w];
-  const float pe = rq * __builtin_amdgcn_exp2f((gh - bh) + (gl - bl));
+  {
+    const f32x4 jh = *(const f32x4*)&Gh[16 * W + 4 * g], jl = *(const f32x4*)&Gl[16 * W + 4 * g];
+    const f32x4 rj = *(const f32x4*)&rk[16 * W + 4 * g];
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    if (t > w) continue;
-    const f32x4 jh = *(const f32x4*)&Gh[16 * t + 4 * g], jl = *(const f32x4*)&Gl[16 * t + 4 * g];
-    const f32x4 rj = *(const f32x4*)&rk[16 * t + 4 * g];
-    if (t < w) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[t][e] = (x[t][e] * pe) * (__builtin_amdgcn_exp2f((bh - jh[e]) + (bl - jl[e])) * rj[e]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool in = 4 * g + e <= c;
-        const float d = __builtin_amdgcn_exp2f(in ? (gh - jh[e]) + (gl - jl[e]) : 0.0f) * rj[e];
-        x[t][e] = in ? (x[t][e] * rq) * d : 0.0f;
-      }
+    for (int e = 0; e < 4; ++e) {
+      const bool in = 4 * g + e <= c;
+      const float d = __builtin_amdgcn_exp2f(in ? (gh - jh[e]) + (gl - jl[e]) : 0.0f) * rj[e];
+      x[W][e] = in ? (x[W][e] * rq) * d : 0.0f;
     }
   }
-  float m = 0.0f, inv;
+  if constexpr (W > 0) {
+    const float pe = rq * __builtin_amdgcn_exp2f((gh - bh) + (gl - bl));
+    wave_sync();
 #pragma unroll
-  for (int t = 0; t < 4; ++t) m = max4(x[t], m);
-  const float sc = pow2_scale(max_rows4(m), inv);
-  h8 hi, lo;
-  const int f = frag_of(w, 0);
-  split8(x[0], x[1], sc, hi, lo);
-  *(h8*)L.P[f][0][lane] = hi;
-  *(h8*)L.P[f][1][lane] = lo;
-  if (w >= 2) {
-    split8(x[2], x[3], sc, hi, lo);
-    *(h8*)L.P[f + 1][0][lane] = hi;
-    *(h8*)L.P[f + 1][1][lane] = lo;
+    for (int t = 0; t < W; ++t) {
+      const f32x4 F = *(const f32x4*)&L.F[W - 1][16 * t + 4 * g];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[t][e] = (x[t][e] * pe) * F[e];
+    }
   }
+  const float inv = store_frags<W>(x, lane, L.P);
   if (g == 0) {
     L.pr[i] = inv;
     L.c2[i] = rq * __builtin_amdgcn_exp2f(gh + gl);
@@ -705,12 +711,12 @@ __device__ __forceinline__ void make_p(ChainLds<DK, NW>& L, const Operands<DK>& 
 }
 
 template <int NW>
-constexpr int kFetchers = NW == 4 ? 0 : 2;  // waves of their own
+constexpr int kFetchers = NW == 4 ? 0 : 4;  // waves of their own
 
 template <int DK, bool BF, int NW>
 __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(64 * (2 * NW + kFetchers<NW>)) void
 delta_chain_kernel(DeltaArgs a, Records<DK> recs, int64_t slot0, int64_t slot1) {
-  constexpr int NM = DK / 16, NJ = DK / 32, NF = kFetchers<NW>, NP = NF ? NF : NW;
+  constexpr int NM = DK / 16, NJ = DK / 32, NF = kFetchers<NW>, NP = 4;
   __shared__ __align__(16) ChainLds<DK, NW> L;
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave % NW;
@@ -866,11 +872,11 @@ delta_chain_kernel(DeltaArgs a, Records<DK> recs, int64_t slot0, int64_t slot1) 
     step_barrier();
     if (fetches) {
       if (i + 1 < n) fetch(i + 1);
-      if constexpr (NP == 2) {  // five of the triangle's ten tiles each
-        make_p<DK, BF>(L, op, fi, lane, a.l2norm, a.scale);
-        make_p<DK, BF>(L, op, 3 - fi, lane, a.l2norm, a.scale);
-      } else {
-        make_p<DK, BF>(L, op, fi, lane, a.l2norm, a.scale);
+      switch (fi) {
+        case 0: make_p<0, DK, BF>(L, op, lane, a.l2norm, a.scale); break;
+        case 1: make_p<1, DK, BF>(L, op, lane, a.l2norm, a.scale); break;
+        case 2: make_p<2, DK, BF>(L, op, lane, a.l2norm, a.scale); break;
+        default: make_p<3, DK, BF>(L, op, lane, a.l2norm, a.scale); break;
       }
     }
     f32x4 qs[4];

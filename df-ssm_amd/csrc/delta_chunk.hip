@@ -507,6 +507,7 @@ struct Operands {
 template <int DK, int NW>
 struct ChainLds {
   Operands<DK> op[2];
+  uint16_t v[NW == 4 ? 1 : 2][NW == 4 ? 8 : kC * 16 * NW];  // NW < 4: rows of v, two chunks; else in registers
   f16 S[NW][DK / 32][2][64][8];   // the state before the chunk, as operands
   f32x4 u[NW][4][64];
   f16 P[6][2][64][8];
@@ -754,14 +755,14 @@ delta_chain_kernel(DeltaArgs a, Records<DK> recs, int64_t slot0, int64_t slot1) 
 #pragma unroll
     for (int m = 0; m < NM; ++m) S[m] = *(const f32x4*)(sp + 32 * (m >> 1) + 4 * (m & 1));
     const int ldv = (int)a.ld_v * 2, vo = 4 * g * ldv + (active ? dv : c) * 2;
-    uint32_t vv[16];
+    uint32_t vv[16];  // (NW = 4)
     auto load_v = [&](int64_t tk) {
       const Rsrc r = rows_of(a.v + tk * a.ld_v + (int64_t)h * a.Dv, a.ld_v, len_at(tk), a.Dv);
 #pragma unroll
       for (int i = 0; i < 16; ++i) vv[i] = __builtin_amdgcn_raw_buffer_load_b16(r, vo, (16 * (i / 4) + (i & 3)) * ldv, 0);
     };
     __builtin_amdgcn_s_waitcnt(0);  // the state is here: within the loop only v is waited for
-    if (n) load_v(tok);
+    if (NW == 4 && n) load_v(tok);
     for (int i = 0; i < n; ++i, tok += kC) {
       const Operands<DK>& op = L.op[i & 1];
       const f32x4* vec = (const f32x4*)op.vec;
@@ -781,13 +782,23 @@ delta_chain_kernel(DeltaArgs a, Records<DK> recs, int64_t slot0, int64_t slot1) 
       rows_product<DK, false>(op.k, lane, sh, sl, ks);
       Tri T;
       load_tri(T, op.T, lane);
+      s4 vx[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        if constexpr (NW == 4)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) vx[t][e] = (short)vv[4 * t + e];
+        else  // four rows of the lane's column: the lane's address is row c / 4 of them, columns 4 (c % 4) ..
+          vx[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)
+              &L.v[i & 1][(16 * t + 4 * g + (c >> 2)) * 16 * NW + 16 * w + 4 * (c & 3)]);
+      }
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const f32x4 c1 = vec[4 * t + g];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[t][e] = __builtin_fmaf(-(c1[e] * sinv), ks[t][e], w2f<BF>((uint16_t)vv[4 * t + e]));
+        for (int e = 0; e < 4; ++e) v[t][e] = __builtin_fmaf(-(c1[e] * sinv), ks[t][e], w2f<BF>((uint16_t)vx[t][e]));
       }
-      load_v(i + 1 < n ? tok + kC : tok);  // (the last time for nothing: a branch would copy the registers)
+      if (NW == 4) load_v(i + 1 < n ? tok + kC : tok);  // (the last time for nothing: a branch would copy the registers)
       h8 xh[2], xl[2];
       float xinv;
       const float xsc = pow2_scale(col_max<4>(v), xinv);
@@ -861,6 +872,13 @@ delta_chain_kernel(DeltaArgs a, Records<DK> recs, int64_t slot0, int64_t slot1) 
     const Source<DK> s{a.k + tk * a.ld_k + hk * DK, a.q + tk * a.ld_q + hk * DK, a.ld_k, a.ld_q, len_at(tk),
                        key + (int64_t)i * a.Hk, rec + (int64_t)i * a.Hv};
     fetch_operands<DK, BF, NP>(L.op[i & 1], s, fi, lane);
+    if constexpr (NW < 4) {  // KiB of 32 / NW rows
+      const Rsrc r = rows_of(a.v + tk * a.ld_v + (int64_t)h * a.Dv + 16 * NW * vb, a.ld_v, s.len, a.Dv - 16 * NW * vb);
+      const int per = 32 / NW, row = lane / (2 * NW), ldb = (int)a.ld_v * 2;
+      if (fi < 2 * NW)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr)((char*)L.v[i & 1] + fi * 1024), 16, row * ldb + lane % (2 * NW) * 16,
+                                                 per * fi * ldb, 0, 0);
+    }
   };
   const int ldo = (int)a.ld_out * 2, oo = c * ldo + (dv0 + 4 * g) * 2;
   if (fetches && n) {
@@ -871,7 +889,9 @@ delta_chain_kernel(DeltaArgs a, Records<DK> recs, int64_t slot0, int64_t slot1) 
     const Operands<DK>& op = L.op[i & 1];
     step_barrier();
     if (fetches) {
-      if (i + 1 < n) fetch(i + 1);
+      // (the fetchers of P's larger tiles wait with their part of the loads until the outputs have P: 1 KiB of
+      // loads into LDS holds a wave for a hundred cycles)
+      if (i + 1 < n && (!NF || fi < 2)) fetch(i + 1);
       switch (fi) {
         case 0: make_p<0, DK, BF>(L, op, lane, a.l2norm, a.scale); break;
         case 1: make_p<1, DK, BF>(L, op, lane, a.l2norm, a.scale); break;
@@ -892,6 +912,7 @@ delta_chain_kernel(DeltaArgs a, Records<DK> recs, int64_t slot0, int64_t slot1) 
       rows_product<DK, true>(op.q, lane, sh, sl, qs);
     }
     step_barrier();
+    if (NF && fetches && i + 1 < n && fi >= 2) fetch(i + 1);
     f32x4 o[4];
     f32x4 uinv;
     if (outputs) {

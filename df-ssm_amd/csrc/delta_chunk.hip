@@ -7,12 +7,14 @@
 // Two launches: delta_prep_kernel makes T and P of all chunks in parallel, delta_chain_kernel walks the chunks
 // of a sequence and head with its state in registers.
 //
-// Numbers. States, sums and everything between products are fp32. The products run on the fp16 matrix cores
-// with fp32 accumulation: q and k are exact there (16-bit inputs; bf16 rows are scaled by a power of two into
-// fp16's range), every other operand is a pair of halves, x 2^s = hi + lo, which holds 22 bits, with s per row
-// of T and P and per value column of S, V - .. and U chosen so that the largest magnitude lies in [2^14, 2^15).
-// A product of two pairs leaves out lo lo, 2^-24 of it. So an fp32 state comes out as from fp32 arithmetic
-// (2e-7 of its norm), at 2 or 3 matrix instructions per product instead of the 8 times as slow fp32 ones.
+// Numbers. States, sums and everything between products are fp32. Products run on the 16-bit matrix cores with
+// fp32 accumulation. q and k are exact operands there, in their own type. A factor of fp32 values is a sum of
+// 16-bit parts: beside fp16 rows, and where both factors are fp32 (T (V - ..), P U), pairs of halves,
+// x 2^s = hi + lo, which hold 22 bits, with s per row of T and P and per value column of S, V - .. and U chosen so
+// that the largest magnitude lies in [2^14, 2^15); beside bf16 rows three bf16 parts, which hold 24 bits and need
+// no scale (for Q S^T, whose result is rounded to bf16, two parts, 16 bits). A product of two pairs leaves out
+// lo lo, 2^-24 of it. So an fp32 state comes out as from fp32 arithmetic (2e-7 of its norm), at 2 or 3 matrix
+// instructions per product instead of the 8 times as slow fp32 ones.
 // G is summed in fp64, so that differences survive a decay of any size in the same chunk; -inf is held to -1e5.
 #include "common.h"
 #include "delta.h"
@@ -22,7 +24,6 @@ namespace dfssm {
 
 namespace {
 
-typedef f16 h4 __attribute__((ext_vector_type(4)));
 typedef f16 h8 __attribute__((ext_vector_type(8)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 
@@ -37,30 +38,17 @@ struct ChunkRec {
   float c1[kC];         // e^{G_i} times k's row factor
   float tr[kC];         // row factor of T
   float w[kC];          // e^{G_C - G_i} times k's row factor
-  float rk[kC];         // k's row factor: normalisation, and what undoes its scaling
+  float rk[kC];         // k's row factor, its normalisation
   float Gh[kC], Gl[kC]; // G_i over log 2, the float nearest and the rest
 };
 static_assert(sizeof(ChunkRec) == 13824, "T, 1.5 KiB of factors");
 
-// bf16 inputs, per chunk and key head: k and q as halves, rows past the sequence's end zero, and what undoes q's
-// scaling. (fp16 rows are taken as they lie.) In LDS, and here, the 16-byte pieces of a row are exchanged so that
-// the same piece of 16 rows, an operand, lies in all 64 banks.
-template <int DK>
-struct KeyRec {
-  f16 k[kC][DK], q[kC][DK];
-  float qinv[kC];
-};
+// Rows of q and k in LDS: the 16-byte pieces of a row are exchanged so that the same piece of 16 rows, an operand,
+// lies in all 64 banks.
 template <int DK>
 __device__ __forceinline__ int piece_at(int row, int p) {
   return p ^ (DK == 128 ? row & 15 : (row >> 1) & 7);
 }
-
-// The records of a launch: the slots' key records, then their chunk records.
-template <int DK>
-struct Records {
-  KeyRec<DK>* keys;
-  ChunkRec* chunks;
-};
 
 template <int N>
 struct Int {
@@ -113,27 +101,49 @@ __device__ __forceinline__ float max4(const f32x4& x, float m) {
   return m;
 }
 typedef f16 h2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 // x0, x1 times sc as pairs of halves, in 5 instructions: the empty asm keeps the compiler from rounding the high
 // part a second time on the way to the low one.
-__device__ __forceinline__ void split2(float x0, float x1, float sc, h2& hi, h2& lo) {
-  hi = __builtin_convertvector(f32x2{x0 * sc, x1 * sc}, h2);
+__device__ __forceinline__ void split2(float x0, float x1, float sc, uint32_t (&part)[2]) {
+  h2 hi = __builtin_convertvector(f32x2{x0 * sc, x1 * sc}, h2);
   asm("" : "+v"(hi));
-  lo = h2{(f16)__builtin_fmaf(x0, sc, -(float)hi[0]), (f16)__builtin_fmaf(x1, sc, -(float)hi[1])};
+  const h2 lo = h2{(f16)__builtin_fmaf(x0, sc, -(float)hi[0]), (f16)__builtin_fmaf(x1, sc, -(float)hi[1])};
+  part[0] = __builtin_bit_cast(uint32_t, hi);
+  part[1] = __builtin_bit_cast(uint32_t, lo);
 }
-// The pair of halves of a 32-deep operand from two results' registers, scaled.
-__device__ __forceinline__ void split8(const f32x4& x, const f32x4& y, float sc, h8& hi, h8& lo) {
-  h2 h[4], l[4];
-  split2(x[0], x[1], sc, h[0], l[0]);
-  split2(x[2], x[3], sc, h[1], l[1]);
-  split2(y[0], y[1], sc, h[2], l[2]);
-  split2(y[2], y[3], sc, h[3], l[3]);
+// x0, x1 in bf16 parts.
+__device__ __forceinline__ void split2(float x0, float x1, float, uint32_t (&part)[3]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    hi[i] = h[i / 2][i % 2];
-    lo[i] = l[i / 2][i % 2];
+  for (int i = 0; i < 3; ++i) {
+    uint32_t p = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x0, x1}, b2));
+    asm("" : "+v"(p));
+    part[i] = p;
+    x0 -= __builtin_bit_cast(float, p << 16);
+    x1 -= __builtin_bit_cast(float, p & 0xffff0000u);
   }
 }
+// The parts of a 32-deep operand from two results' registers, scaled.
+template <int NT>
+__device__ __forceinline__ void split8(const f32x4& x, const f32x4& y, float sc, h8 (&part)[NT]) {
+  uint32_t p[4][NT];
+  split2(x[0], x[1], sc, p[0]);
+  split2(x[2], x[3], sc, p[1]);
+  split2(y[0], y[1], sc, p[2]);
+  split2(y[2], y[3], sc, p[3]);
+#pragma unroll
+  for (int i = 0; i < NT; ++i) part[i] = __builtin_bit_cast(h8, u32x4{p[0][i], p[1][i], p[2][i], p[3][i]});
+}
+
+// The product of two operands of the rows' type (16 bits of either kind are carried as h8).
+template <bool BF>
+__device__ __forceinline__ f32x4 mm(h8 a, h8 b, f32x4 c) {
+  if constexpr (BF) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+template <bool BF>
+constexpr int kParts = BF ? 3 : 2;  // of an fp32 factor beside rows of the type
 
 // The sequence and chunk of slot s of the launch's chunk numbering: sequence b starts at slot
 // floor(t0 / 64) + b, which needs no sums over the lengths and leaves room for every chunk. The lanes of a wave
@@ -185,25 +195,11 @@ struct PrepLds {              // of a wave
   double G[kC];               // in units of log 2
   float F[3][kC];             // e^{G_16w - G_j} rk_j for the row tiles w = 1 .. 3
   float rk[kC], kb[kC], ke[kC], be[kC];
-  float ss[kC], inv[kC];
+  float ss[kC];
 };
 // Element c of the diagonal of a 16 x 16 result, in its lane (g = c / 4).
 __device__ __forceinline__ float diagonal(const f32x4& x, int c) {
   return (c & 2) ? ((c & 1) ? x[3] : x[2]) : ((c & 1) ? x[1] : x[0]);
-}
-
-// 8 values of a 16-bit row as halves times sc (1 for fp16).
-template <bool BF>
-__device__ __forceinline__ h8 to_halves(u32x4 x, float sc) {
-  if constexpr (!BF) return __builtin_bit_cast(h8, x);
-  h2 h[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    h[i] = __builtin_convertvector(f32x2{__builtin_bit_cast(float, x[i] << 16) * sc, __builtin_bit_cast(float, x[i] & 0xffff0000u) * sc}, h2);
-  h8 r;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = h[i / 2][i % 2];
-  return r;
 }
 
 // 16 rows, lane (g, r): row r, columns 32 j + 8 g ..
@@ -213,29 +209,6 @@ __device__ __forceinline__ void load_rows(Rsrc rows, int64_t ld, int t, int lane
 #pragma unroll
   for (int j = 0; j < DK / 32; ++j) x[j] = row_load16(rows, off, j * 64);
 }
-// They as operands, also into the key record if given. Returns what undoes the row's scaling.
-template <int DK, bool BF>
-__device__ __forceinline__ float make_rows(const u32x4 (&x)[DK / 32], int t, int lane, f16 (*rec)[DK], h8 (&y)[DK / 32]) {
-  typedef unsigned short us2 __attribute__((ext_vector_type(2)));
-  constexpr int NJ = DK / 32;
-  const int row = 16 * t + (lane & 15), g = lane >> 4;
-  float inv = 1.0f, sc = 1.0f;
-  if constexpr (BF) {
-    us2 top = us2{0, 0};
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-      for (int d = 0; d < 4; ++d) top = __builtin_elementwise_max(top, __builtin_bit_cast(us2, x[j][d] & 0x7fff7fffu));
-    sc = pow2_scale(max_rows4(__builtin_bit_cast(float, (uint32_t)max(top[0], top[1]) << 16)), inv);
-  }
-#pragma unroll
-  for (int j = 0; j < NJ; ++j) {
-    y[j] = to_halves<BF>(x[j], sc);
-    if (rec) *(h8*)&rec[row][piece_at<DK>(row, 4 * j + g) * 8] = y[j];
-  }
-  return inv;
-}
-
 // Row tile W of a triangle, x[t] a lane's four columns of column tile t <= W, as pairs of halves with the row's
 // own scale; returns the row factor.
 template <int W>
@@ -247,12 +220,11 @@ __device__ __forceinline__ float store_frags(const f32x4 (&x)[W + 1], int lane, 
   const float sc = pow2_scale(max_rows4(m), inv);
 #pragma unroll
   for (int j = 0; 2 * j <= W; ++j) {
-    h8 hi, lo;
-    if (2 * j + 1 <= W) split8(x[2 * j], x[2 * j + 1 <= W ? 2 * j + 1 : W], sc, hi, lo);
-    else split8(x[2 * j], f32x4{0, 0, 0, 0}, sc, hi, lo);
+    h8 part[2];
+    split8(x[2 * j], 2 * j + 1 <= W ? x[2 * j + 1 <= W ? 2 * j + 1 : W] : f32x4{0, 0, 0, 0}, sc, part);
     const int f = frag_of(W, j);
-    *(h8*)out[f][0][lane] = hi;
-    *(h8*)out[f][1][lane] = lo;
+    *(h8*)out[f][0][lane] = part[0];
+    *(h8*)out[f][1][lane] = part[1];
   }
   return inv;
 }
@@ -264,7 +236,7 @@ struct PrepRows {  // what is loaded ahead for a task
 };
 
 template <int DK, bool BF>
-__global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(256) void delta_prep_kernel(DeltaArgs a, Records<DK> recs,
+__global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(256) void delta_prep_kernel(DeltaArgs a, ChunkRec* recs,
                                                                                                int64_t slot0, int64_t n_tasks) {
   constexpr int NJ = DK / 32;
   __shared__ __align__(16) PrepLds lds[4];
@@ -277,7 +249,6 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(256) void d
   PrepRows<DK> in;
   int64_t task = blockIdx.x, slot = 0;
   int h = 0, len = 0;
-  const uint16_t* qrows = nullptr;
   auto load = [&]() {
     slot = task / nw;
     h = (int)(task % nw) * 4 + wave;
@@ -289,7 +260,6 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(256) void d
     }
     const int hk = h / rep;
     const Rsrc kr = rows_of(a.k + tok * a.ld_k + hk * DK, a.ld_k, len, DK);
-    qrows = a.q + tok * a.ld_q + hk * DK;  // (bf16)
 #pragma unroll
     for (int t = 0; t < 4; ++t) load_rows<DK>(kr, a.ld_k, t, lane, in.k[t]);
     const int64_t at = tok + (lane < len ? lane : 0);
@@ -298,9 +268,7 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(256) void d
   };
   load();
   for (;;) {
-    ChunkRec* rec = recs.chunks + slot * a.Hv + h;
-    // bf16: the first of a key head's value heads writes its record
-    KeyRec<DK>* key = BF && h % rep == 0 ? recs.keys + slot * a.Hk + h / rep : nullptr;
+    ChunkRec* rec = recs + slot * a.Hv + h;
     const bool some = len > 0;
     f32x4 A[4][4];
     if (some) {
@@ -319,17 +287,15 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(256) void d
       const float be = lane < len ? in.be : 0.0f;
       h8 k[4][NJ];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const float ki = make_rows<DK, BF>(in.k[t], t, lane, key ? key->k : nullptr, k[t]);
-        if (BF && g == 0) L.inv[16 * t + c] = ki;
-        if (BF) __builtin_amdgcn_sched_barrier(0);  // (tile by tile: all at once take more registers than there are)
-      }
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) k[t][j] = __builtin_bit_cast(h8, in.k[t][j]);
       f32x4 kd[4];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         kd[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) kd[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][j], k[t][j], kd[t], 0, 0, 0);
+        for (int j = 0; j < NJ; ++j) kd[t] = mm<BF>(k[t][j], k[t][j], kd[t]);
       }
       // a row's squares are on the diagonal of k k^T: in the lane of that row that has its column
       if (a.l2norm)
@@ -340,8 +306,7 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(256) void d
       L.be[lane] = be;
       wave_sync();
       {  // lane: a token
-        float rk = BF ? L.inv[lane] : 1.0f;
-        if (a.l2norm) rk *= l2_factor((L.ss[lane] * rk) * rk);
+        const float rk = a.l2norm ? l2_factor(L.ss[lane]) : 1.0f;
         const double GC = L.G[kC - 1], Gt = L.G[lane & 48];
         const float eG = __builtin_amdgcn_exp2f((float)G), et = __builtin_amdgcn_exp2f((float)(G - Gt));
         rec->c1[lane] = eG * rk;
@@ -368,7 +333,7 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(256) void d
         for (int t = 0; t < w; ++t) {
           A[w][t] = f32x4{0, 0, 0, 0};
 #pragma unroll
-          for (int j = 0; j < NJ; ++j) A[w][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][j], k[w][j], A[w][t], 0, 0, 0);
+          for (int j = 0; j < NJ; ++j) A[w][t] = mm<BF>(k[t][j], k[w][j], A[w][t]);
         }
         const float ke = L.ke[i], kb = L.kb[i];
 #pragma unroll
@@ -389,15 +354,6 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(256) void d
         *(f32x4*)&L.B[w * kBlock + c * kBS + 4 * g] = D;
       }
       wave_sync();
-      if (key)
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          u32x4 x[NJ];
-          h8 y[NJ];
-          load_rows<DK>(rows_of(qrows, a.ld_q, len, DK), a.ld_q, t, lane, x);
-          const float qi = make_rows<DK, BF>(x, t, lane, key->q, y);
-          if (g == 0) key->qinv[16 * t + c] = qi;
-        }
     }
     task += gridDim.x;
     const bool more = task < n_tasks;
@@ -500,7 +456,6 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(256) void d
 template <int DK>
 struct Operands {
   f16 k[kC][DK], q[kC][DK];
-  float qinv[kC];                 // (bf16)
   f16 T[6][2][64][8];
   float vec[384];                 // c1, tr, w, rk, Gh, Gl of the record
 };
@@ -522,10 +477,15 @@ __device__ __forceinline__ float col_max(const f32x4 (&x)[N], float m = 0.0f) {
   for (int t = 0; t < N; ++t) m = max4(x[t], m);
   return max_rows4(m);
 }
-template <int N>
-__device__ __forceinline__ void split_all(const f32x4 (&x)[N], float sc, h8 (&hi)[N / 2], h8 (&lo)[N / 2]) {
+template <int N, int NT>
+__device__ __forceinline__ void split_all(const f32x4 (&x)[N], float sc, h8 (&part)[NT][N / 2]) {
 #pragma unroll
-  for (int j = 0; j < N / 2; ++j) split8(x[2 * j], x[2 * j + 1], sc, hi[j], lo[j]);
+  for (int j = 0; j < N / 2; ++j) {
+    h8 p[NT];
+    split8(x[2 * j], x[2 * j + 1], sc, p);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) part[i][j] = p[i];
+  }
 }
 
 // A barrier that waits for this wave's LDS accesses alone. lds_barrier() also waits for its loads into LDS, which
@@ -536,8 +496,6 @@ __device__ __forceinline__ void step_barrier() {
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
-
-#define DELTA_MFMA(a, b, c) __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0)
 
 // Fragments of a triangle in LDS or global memory.
 struct Tri {
@@ -553,27 +511,26 @@ __device__ __forceinline__ void load_tri(Tri& f, const f16 (*F)[2][64][8], int l
 // y = M x (both pairs; with FLIP the transpose), the four row tiles in turn so that no product waits for the one
 // before.
 template <bool FLIP>
-__device__ __forceinline__ void tri_product(const Tri& f, const h8 (&xh)[2], const h8 (&xl)[2], f32x4 (&y)[4]) {
+__device__ __forceinline__ void tri_product(const Tri& f, const h8 (&x)[2][2], f32x4 (&y)[4]) {
   const int at[4] = {0, 1, 2, 4};
-  auto mm = [&](const h8& u, const h8& v, const f32x4& w) { return FLIP ? DELTA_MFMA(v, u, w) : DELTA_MFMA(u, v, w); };
+  auto add = [&](const h8& u, const h8& v, f32x4& w) { w = FLIP ? mm<false>(v, u, w) : mm<false>(u, v, w); };
 #pragma unroll
   for (int t = 0; t < 4; ++t) y[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
 #pragma unroll
-    for (int t = 2 * j; t < 4; ++t) y[t] = mm(f.lo[at[t] + j], xh[j], y[t]);
+    for (int t = 2 * j; t < 4; ++t) add(f.lo[at[t] + j], x[0][j], y[t]);
 #pragma unroll
-    for (int t = 2 * j; t < 4; ++t) y[t] = mm(f.hi[at[t] + j], xl[j], y[t]);
+    for (int t = 2 * j; t < 4; ++t) add(f.hi[at[t] + j], x[1][j], y[t]);
 #pragma unroll
-    for (int t = 2 * j; t < 4; ++t) y[t] = mm(f.hi[at[t] + j], xh[j], y[t]);
+    for (int t = 2 * j; t < 4; ++t) add(f.hi[at[t] + j], x[0][j], y[t]);
   }
 }
 
-// y = X S^T for 64 rows X of halves in LDS (two row tiles at a time, the next two in flight); with FLIP its
-// transpose, a lane then has four neighbouring value columns of a token.
-template <int DK, bool FLIP>
-__device__ __forceinline__ void rows_product(const f16 (*X)[DK], int lane, const h8 (&sh)[DK / 32], const h8 (&sl)[DK / 32],
-                                             f32x4 (&y)[4]) {
+// y = X S^T for 64 rows X in LDS (two row tiles at a time, the next two in flight) and S in NT parts; with FLIP
+// its transpose, a lane then has four neighbouring value columns of a token.
+template <int DK, bool BF, bool FLIP, int NT>
+__device__ __forceinline__ void rows_product(const f16 (*X)[DK], int lane, const h8 (&s)[NT][DK / 32], f32x4 (&y)[4]) {
   constexpr int NJ = DK / 32;
   const int g = lane >> 4, c = lane & 15;
   h8 x[2][2][NJ];
@@ -586,7 +543,7 @@ __device__ __forceinline__ void rows_product(const f16 (*X)[DK], int lane, const
         x[p][t][j] = *(const h8*)&X[row][piece_at<DK>(row, 4 * j + g) * 8];
       }
   };
-  auto mm = [&](const h8& u, const h8& v, const f32x4& w) { return FLIP ? DELTA_MFMA(v, u, w) : DELTA_MFMA(u, v, w); };
+  auto add = [&](const h8& u, const h8& v, f32x4& w) { w = FLIP ? mm<BF>(v, u, w) : mm<BF>(u, v, w); };
   load(0);
 #pragma unroll
   for (int p = 0; p < 2; ++p) {
@@ -594,26 +551,17 @@ __device__ __forceinline__ void rows_product(const f16 (*X)[DK], int lane, const
     __builtin_amdgcn_sched_barrier(0);
     f32x4 a = f32x4{0, 0, 0, 0}, b = f32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      a = mm(x[p][0][j], sl[j], a);
-      b = mm(x[p][1][j], sl[j], b);
-      a = mm(x[p][0][j], sh[j], a);
-      b = mm(x[p][1][j], sh[j], b);
-    }
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int i = NT - 1; i >= 0; --i) {
+        add(x[p][0][j], s[i][j], a);
+        add(x[p][1][j], s[i][j], b);
+      }
     y[2 * p] = a;
     y[2 * p + 1] = b;
   }
 }
 
-// Where a chunk's operands come from.
-template <int DK>
-struct Source {
-  const uint16_t *k, *q;  // fp16 rows
-  int64_t ld_k, ld_q;
-  int len;
-  const KeyRec<DK>* key;  // bf16
-  const ChunkRec* rec;
-};
 typedef const __attribute__((address_space(1))) void* gptr;
 typedef __attribute__((address_space(3))) void* lptr;
 
@@ -631,24 +579,18 @@ __device__ __forceinline__ void fetch_rows(f16 (*to)[DK], const uint16_t* p, int
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr)((char*)to + m * 1024), 16, off, per * m * bytes, 0, 0);
   }
 }
-template <int DK, bool BF, int NP>
-__device__ __forceinline__ void fetch_operands(Operands<DK>& op, const Source<DK>& s, int w, int lane) {
-  if constexpr (BF) {
-    constexpr int nk = DK * kC * 4 / 1024;
-#pragma unroll
-    for (int n = 0; n < nk; n += NP)
-      __builtin_amdgcn_global_load_lds((gptr)((const char*)s.key + (n + w) * 1024 + lane * 16), (lptr)((char*)op.k + (n + w) * 1024), 16, 0, 0);
-    if (w == 0) __builtin_amdgcn_global_load_lds((gptr)(s.key->qinv + lane), (lptr)op.qinv, 4, 0, 0);
-  } else {
-    fetch_rows<DK, NP>(op.k, s.k, s.ld_k, s.len, w, lane);
-    fetch_rows<DK, NP>(op.q, s.q, s.ld_q, s.len, w, lane);
-  }
+// A chunk's operands into LDS, by fetcher w of NP.
+template <int DK, int NP>
+__device__ __forceinline__ void fetch_operands(Operands<DK>& op, const DeltaArgs& a, int64_t tok, int len, int hk,
+                                               const ChunkRec* rec, int w, int lane) {
+  fetch_rows<DK, NP>(op.k, a.k + tok * a.ld_k + hk * DK, a.ld_k, len, w, lane);
+  fetch_rows<DK, NP>(op.q, a.q + tok * a.ld_q + hk * DK, a.ld_q, len, w, lane);
 #pragma unroll
   for (int n = 0; n < 12; n += NP)
-    __builtin_amdgcn_global_load_lds((gptr)((const char*)s.rec + (n + w) * 1024 + lane * 16), (lptr)((char*)op.T + (n + w) * 1024), 16, 0, 0);
+    __builtin_amdgcn_global_load_lds((gptr)((const char*)rec + (n + w) * 1024 + lane * 16), (lptr)((char*)op.T + (n + w) * 1024), 16, 0, 0);
   // the factors, 1536 bytes: 4 bytes per lane
   for (int n = w; n < 6; n += NP)
-    __builtin_amdgcn_global_load_lds((gptr)(s.rec->c1 + n * 64 + lane), (lptr)(op.vec + n * 64), 4, 0, 0);
+    __builtin_amdgcn_global_load_lds((gptr)(rec->c1 + n * 64 + lane), (lptr)(op.vec + n * 64), 4, 0, 0);
 }
 
 // Row tile W of P = tril(q_i.k_j e^{G_i - G_j}) and of q's factors.
@@ -673,17 +615,13 @@ __device__ __forceinline__ void make_p(ChainLds<DK, NW>& L, const Operands<DK>& 
   for (int t = 0; t <= W; ++t) x[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
-    if (l2norm) qq = DELTA_MFMA(q[j], q[j], qq);
+    if (l2norm) qq = mm<BF>(q[j], q[j], qq);
 #pragma unroll
-    for (int t = 0; t <= W; ++t) x[t] = DELTA_MFMA(k[t][j], q[j], x[t]);
+    for (int t = 0; t <= W; ++t) x[t] = mm<BF>(k[t][j], q[j], x[t]);
   }
   const float gh = Gh[i], gl = Gl[i];
-  float rq = BF ? op.qinv[i] : 1.0f;
-  if (l2norm) {  // the squares are the diagonal of q q^T; lane (c / 4, c) has it for row c
-    const float ss = __shfl(diagonal(qq, c), 16 * (c >> 2) + c, 64);
-    rq *= l2_factor((ss * rq) * rq);
-  }
-  rq *= scale;
+  float rq = scale;  // the squares are the diagonal of q q^T; lane (c / 4, c) has it for row c
+  if (l2norm) rq *= l2_factor(__shfl(diagonal(qq, c), 16 * (c >> 2) + c, 64));
   {
     const f32x4 jh = *(const f32x4*)&Gh[16 * W + 4 * g], jl = *(const f32x4*)&Gl[16 * W + 4 * g];
     const f32x4 rj = *(const f32x4*)&rk[16 * W + 4 * g];
@@ -716,8 +654,8 @@ constexpr int kFetchers = NW == 4 ? 0 : 4;  // waves of their own
 
 template <int DK, bool BF, int NW>
 __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(64 * (2 * NW + kFetchers<NW>)) void
-delta_chain_kernel(DeltaArgs a, Records<DK> recs, int64_t slot0, int64_t slot1) {
-  constexpr int NM = DK / 16, NJ = DK / 32, NF = kFetchers<NW>, NP = 4;
+delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, int64_t slot0, int64_t slot1) {
+  constexpr int NM = DK / 16, NJ = DK / 32, NT = kParts<BF>, NF = kFetchers<NW>, NP = 4;
   __shared__ __align__(16) ChainLds<DK, NW> L;
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave % NW;
@@ -766,20 +704,25 @@ delta_chain_kernel(DeltaArgs a, Records<DK> recs, int64_t slot0, int64_t slot1) 
     for (int i = 0; i < n; ++i, tok += kC) {
       const Operands<DK>& op = L.op[i & 1];
       const f32x4* vec = (const f32x4*)op.vec;
-      h8 sh[NJ], sl[NJ];
-      float sinv;
-      const float smax = col_max<NM>(S), ssc = pow2_scale(smax, sinv);
-      split_all<NM>(S, ssc, sh, sl);
+      h8 s[NT][NJ];
+      float smax = 0.0f, ssc = 1.0f, sinv = 1.0f;
+      if constexpr (!BF) {
+        smax = col_max<NM>(S);
+        ssc = pow2_scale(smax, sinv);
+      }
+      split_all<NM>(S, ssc, s);
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        *(h8*)L.S[w][j][0][lane] = sh[j];
-        *(h8*)L.S[w][j][1][lane] = sl[j];
+        *(h8*)L.S[w][j][0][lane] = s[0][j];
+        *(h8*)L.S[w][j][1][lane] = s[1][j];
       }
-      sinv *= sfac;
-      if (g == 0) L.sfac[w][c] = sinv;
+      if constexpr (!BF) {
+        sinv *= sfac;
+        if (g == 0) L.sfac[w][c] = sinv;
+      }
       step_barrier();  // the operands of this chunk and the state are in LDS
       f32x4 v[4], ks[4];
-      rows_product<DK, false>(op.k, lane, sh, sl, ks);
+      rows_product<DK, BF, false>(op.k, lane, s, ks);
       Tri T;
       load_tri(T, op.T, lane);
       s4 vx[4];
@@ -796,15 +739,15 @@ delta_chain_kernel(DeltaArgs a, Records<DK> recs, int64_t slot0, int64_t slot1) 
       for (int t = 0; t < 4; ++t) {
         const f32x4 c1 = vec[4 * t + g];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[t][e] = __builtin_fmaf(-(c1[e] * sinv), ks[t][e], w2f<BF>((uint16_t)vx[t][e]));
+        for (int e = 0; e < 4; ++e) v[t][e] = __builtin_fmaf(-(BF ? c1[e] : c1[e] * sinv), ks[t][e], w2f<BF>((uint16_t)vx[t][e]));
       }
       if (NW == 4) load_v(i + 1 < n ? tok + kC : tok);  // (the last time for nothing: a branch would copy the registers)
-      h8 xh[2], xl[2];
+      h8 x[2][2];
       float xinv;
       const float xsc = pow2_scale(col_max<4>(v), xinv);
-      split_all<4>(v, xsc, xh, xl);
+      split_all<4>(v, xsc, x);
       f32x4 u[4];
-      tri_product<false>(T, xh, xl, u);
+      tri_product<false>(T, x, u);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const f32x4 tr = vec[16 + 4 * t + g], ww = vec[2 * 16 + 4 * t + g];
@@ -815,14 +758,17 @@ delta_chain_kernel(DeltaArgs a, Records<DK> recs, int64_t slot0, int64_t slot1) 
         for (int e = 0; e < 4; ++e) u[t][e] *= ww[e];
       }
       step_barrier();  // U is in LDS
-      // S1 = e^{G_C} S + U'^T K, summed on the matrix cores onto S in a scale that fits both
+      // S1 = e^{G_C} S + U'^T K, summed on the matrix cores onto S (fp16: in a scale that fits both)
       const float dec = __builtin_amdgcn_exp2f(op.vec[256 + kC - 1] + op.vec[320 + kC - 1]);
-      float winv;
-      const float wsc = pow2_scale(fmaxf(col_max<4>(u), dec * (smax * sfac)), winv);
-      const float keep = dec * sfac * wsc;
-      sfac = winv;
-      h8 wh[2], wl[2];
-      split_all<4>(u, wsc, wh, wl);
+      float keep = dec, wsc = 1.0f;
+      if constexpr (!BF) {
+        float winv;
+        wsc = pow2_scale(fmaxf(col_max<4>(u), dec * (smax * sfac)), winv);
+        keep = dec * sfac * wsc;
+        sfac = winv;
+      }
+      h8 uw[NT][2];
+      split_all<4>(u, wsc, uw);
 #pragma unroll
       for (int m = 0; m < NM; ++m)
 #pragma unroll
@@ -848,32 +794,29 @@ delta_chain_kernel(DeltaArgs a, Records<DK> recs, int64_t slot0, int64_t slot1) 
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
 #pragma unroll
-          for (int m = 0; m < 4; ++m) S[p + m] = DELTA_MFMA(ka[m][j], wl[j], S[p + m]);
+          for (int q = NT - 1; q >= 0; --q)
 #pragma unroll
-          for (int m = 0; m < 4; ++m) S[p + m] = DELTA_MFMA(ka[m][j], wh[j], S[p + m]);
+            for (int m = 0; m < 4; ++m) S[p + m] = mm<BF>(ka[m][j], uw[q][j], S[p + m]);
         }
       }
     }
     if (active) {
       float* o = a.state_out + so;
 #pragma unroll
-      for (int m = 0; m < NM; ++m) *(f32x4*)(o + 32 * (m >> 1) + 4 * (m & 1)) = S[m] * sfac;
+      for (int m = 0; m < NM; ++m) *(f32x4*)(o + 32 * (m >> 1) + 4 * (m & 1)) = BF ? S[m] : S[m] * sfac;
     }
     return;
   }
 
   // -------------------------------------------------------------------- the fetchers and the outputs
-  const KeyRec<DK>* key = recs.keys + (first + cb - slot0) * a.Hk + hk;
-  const ChunkRec* rec = recs.chunks + (first + cb - slot0) * a.Hv + h;
+  const ChunkRec* rec = recs + (first + cb - slot0) * a.Hv + h;
   const bool outputs = wave < 2 * NW, fetches = !NF || !outputs;
   const int fi = NF ? wave - 2 * NW : w;  // which fetcher
   auto fetch = [&](int i) {               // chunk i of the launch's
     const int64_t tk = t0 + (cb + i) * kC;
-    const Source<DK> s{a.k + tk * a.ld_k + hk * DK, a.q + tk * a.ld_q + hk * DK, a.ld_k, a.ld_q, len_at(tk),
-                       key + (int64_t)i * a.Hk, rec + (int64_t)i * a.Hv};
-    fetch_operands<DK, BF, NP>(L.op[i & 1], s, fi, lane);
+    fetch_operands<DK, NP>(L.op[i & 1], a, tk, len_at(tk), hk, rec + (int64_t)i * a.Hv, fi, lane);
     if constexpr (NW < 4) {  // KiB of 32 / NW rows
-      const Rsrc r = rows_of(a.v + tk * a.ld_v + (int64_t)h * a.Dv + 16 * NW * vb, a.ld_v, s.len, a.Dv - 16 * NW * vb);
+      const Rsrc r = rows_of(a.v + tk * a.ld_v + (int64_t)h * a.Dv + 16 * NW * vb, a.ld_v, len_at(tk), a.Dv - 16 * NW * vb);
       const int per = 32 / NW, row = lane / (2 * NW), ldb = (int)a.ld_v * 2;
       if (fi < 2 * NW)
         __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr)((char*)L.v[i & 1] + fi * 1024), 16, row * ldb + lane % (2 * NW) * 16,
@@ -902,14 +845,14 @@ delta_chain_kernel(DeltaArgs a, Records<DK> recs, int64_t slot0, int64_t slot1) 
     f32x4 qs[4];
     f32x4 sinv;
     if (outputs) {
-      h8 sh[NJ], sl[NJ];
+      h8 s[2][NJ];
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        sh[j] = *(const h8*)L.S[w][j][0][lane];
-        sl[j] = *(const h8*)L.S[w][j][1][lane];
+        s[0][j] = *(const h8*)L.S[w][j][0][lane];
+        s[1][j] = *(const h8*)L.S[w][j][1][lane];
       }
-      sinv = *(const f32x4*)&L.sfac[w][4 * g];
-      rows_product<DK, true>(op.q, lane, sh, sl, qs);
+      sinv = BF ? f32x4{1.0f, 1.0f, 1.0f, 1.0f} : *(const f32x4*)&L.sfac[w][4 * g];
+      rows_product<DK, BF, true>(op.q, lane, s, qs);
     }
     step_barrier();
     if (NF && fetches && i + 1 < n && fi >= 2) fetch(i + 1);
@@ -921,12 +864,12 @@ delta_chain_kernel(DeltaArgs a, Records<DK> recs, int64_t slot0, int64_t slot1) 
       f32x4 u[4];
 #pragma unroll
       for (int t = 0; t < 4; ++t) u[t] = L.u[w][t][lane];
-      h8 uh[2], ul[2];
+      h8 x[2][2];
       float inv;
       const float usc = pow2_scale(col_max<4>(u), inv);
       if (g == 0) L.ufac[w][c] = inv;
-      split_all<4>(u, usc, uh, ul);
-      tri_product<true>(P, uh, ul, o);
+      split_all<4>(u, usc, x);
+      tri_product<true>(P, x, o);
       wave_sync();
       uinv = *(const f32x4*)&L.ufac[w][4 * g];
     }
@@ -947,22 +890,16 @@ delta_chain_kernel(DeltaArgs a, Records<DK> recs, int64_t slot0, int64_t slot1) 
   }
 }
 
-template <int DK>
-constexpr int64_t slot_bytes(const DeltaArgs& a) {
-  return (a.bf16 ? (int64_t)a.Hk * sizeof(KeyRec<DK>) : 0) + (int64_t)a.Hv * sizeof(ChunkRec);
-}
-int64_t slot_bytes(const DeltaArgs& a) { return a.Dk == 128 ? slot_bytes<128>(a) : slot_bytes<64>(a); }
-
 int64_t chunk_slots(const DeltaArgs& a) { return a.n_tokens / kC + a.n_seq; }
 
 // Chunks whose records are held at once: all, or as many as fit 1 GiB.
 int64_t slots_per_pass(const DeltaArgs& a) {
-  const int64_t all = chunk_slots(a), fit = ((int64_t)1 << 30) / slot_bytes(a);
+  const int64_t all = chunk_slots(a), fit = ((int64_t)1 << 30) / ((int64_t)a.Hv * sizeof(ChunkRec));
   return fit < 1 ? 1 : (fit < all ? fit : all);
 }
 
 template <int DK, bool BF, int NW>
-void launch_chain(const DeltaArgs& a, Records<DK> r, int64_t s0, int64_t s1, hipStream_t s) {
+void launch_chain(const DeltaArgs& a, const ChunkRec* r, int64_t s0, int64_t s1, hipStream_t s) {
   const int64_t units = (int64_t)a.n_seq * a.Hk, per = (int64_t)(a.Hv / a.Hk) * ((a.Dv + 16 * NW - 1) / (16 * NW));
   hipLaunchKernelGGL((delta_chain_kernel<DK, BF, NW>), dim3((unsigned)((units + 7) / 8 * 8 * per)), dim3(64 * (2 * NW + kFetchers<NW>)), 0, s, a, r, s0, s1);
 }
@@ -973,7 +910,7 @@ hipError_t launch_chunked(const DeltaArgs& a, void* ws, hipStream_t s) {
   const int64_t ng = (a.Hv + 3) / 4, slots = chunk_slots(a), per = slots_per_pass(a);
   const int64_t heads = (int64_t)a.n_seq * a.Hv, tiles = a.Dv / 16;
   if ((heads + 8 * rep) * tiles > 0x7fffffff || per * ng > 0x7fffffff) return hipErrorInvalidValue;
-  const Records<DK> r{(KeyRec<DK>*)ws, (ChunkRec*)((char*)ws + (BF ? per * a.Hk * sizeof(KeyRec<DK>) : 0))};
+  ChunkRec* r = (ChunkRec*)ws;
   for (int64_t s0 = 0; s0 < slots; s0 += per) {
     const int64_t n = s0 + per < slots ? per : slots - s0;
     const int64_t tasks = n * ng, resident = 512;  // two workgroups to a CU
@@ -987,7 +924,7 @@ hipError_t launch_chunked(const DeltaArgs& a, void* ws, hipStream_t s) {
 
 }  // namespace
 
-size_t delta_chunk_workspace(const DeltaArgs& a) { return (size_t)(slots_per_pass(a) * slot_bytes(a)); }
+size_t delta_chunk_workspace(const DeltaArgs& a) { return (size_t)(slots_per_pass(a) * a.Hv) * sizeof(ChunkRec); }
 
 hipError_t launch_delta_chunked(const DeltaArgs& a, void* ws, hipStream_t s) {
   if (a.Dk == 128) return a.bf16 ? launch_chunked<128, true>(a, ws, s) : launch_chunked<128, false>(a, ws, s);

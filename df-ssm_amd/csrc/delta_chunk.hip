@@ -142,6 +142,12 @@ __device__ __forceinline__ f32x4 mm(h8 a, h8 b, f32x4 c) {
   if constexpr (BF) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (BF) return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, b2));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, h2));
+}
 template <bool BF>
 constexpr int kParts = BF ? 3 : 2;  // of an fp32 factor beside rows of the type
 
@@ -579,18 +585,15 @@ __device__ __forceinline__ void fetch_rows(f16 (*to)[DK], const uint16_t* p, int
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr)((char*)to + m * 1024), 16, off, per * m * bytes, 0, 0);
   }
 }
-// A chunk's operands into LDS, by fetcher w of NP.
-template <int DK, int NP>
-__device__ __forceinline__ void fetch_operands(Operands<DK>& op, const DeltaArgs& a, int64_t tok, int len, int hk,
-                                               const ChunkRec* rec, int w, int lane) {
-  fetch_rows<DK, NP>(op.k, a.k + tok * a.ld_k + hk * DK, a.ld_k, len, w, lane);
-  fetch_rows<DK, NP>(op.q, a.q + tok * a.ld_q + hk * DK, a.ld_q, len, w, lane);
+// T and the factors of a chunk into LDS, by fetcher w of NP.
+template <int NP>
+__device__ __forceinline__ void fetch_record(f16 (*T)[2][64][8], float* vec, const ChunkRec* rec, int w, int lane) {
 #pragma unroll
   for (int n = 0; n < 12; n += NP)
-    __builtin_amdgcn_global_load_lds((gptr)((const char*)rec + (n + w) * 1024 + lane * 16), (lptr)((char*)op.T + (n + w) * 1024), 16, 0, 0);
+    __builtin_amdgcn_global_load_lds((gptr)((const char*)rec + (n + w) * 1024 + lane * 16), (lptr)((char*)T + (n + w) * 1024), 16, 0, 0);
   // the factors, 1536 bytes: 4 bytes per lane
   for (int n = w; n < 6; n += NP)
-    __builtin_amdgcn_global_load_lds((gptr)(rec->c1 + n * 64 + lane), (lptr)(op.vec + n * 64), 4, 0, 0);
+    __builtin_amdgcn_global_load_lds((gptr)(rec->c1 + n * 64 + lane), (lptr)(vec + n * 64), 4, 0, 0);
 }
 
 // Row tile W of P = tril(q_i.k_j e^{G_i - G_j}) and of q's factors.
@@ -693,17 +696,22 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, int64_t slot0, int64_t slo
 #pragma unroll
     for (int m = 0; m < NM; ++m) S[m] = *(const f32x4*)(sp + 32 * (m >> 1) + 4 * (m & 1));
     const int ldv = (int)a.ld_v * 2, vo = 4 * g * ldv + (active ? dv : c) * 2;
-    uint32_t vv[16];  // (NW = 4)
+    uint32_t vv[16], vn[16];  // (NW = 4) this chunk's and the next one's
     auto load_v = [&](int64_t tk) {
       const Rsrc r = rows_of(a.v + tk * a.ld_v + (int64_t)h * a.Dv, a.ld_v, len_at(tk), a.Dv);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) vv[i] = __builtin_amdgcn_raw_buffer_load_b16(r, vo, (16 * (i / 4) + (i & 3)) * ldv, 0);
+      for (int i = 0; i < 16; ++i) vn[i] = __builtin_amdgcn_raw_buffer_load_b16(r, vo, (16 * (i / 4) + (i & 3)) * ldv, 0);
     };
     __builtin_amdgcn_s_waitcnt(0);  // the state is here: within the loop only v is waited for
     if (NW == 4 && n) load_v(tok);
     for (int i = 0; i < n; ++i, tok += kC) {
       const Operands<DK>& op = L.op[i & 1];
       const f32x4* vec = (const f32x4*)op.vec;
+      if constexpr (NW == 4) {
+#pragma unroll
+        for (int q = 0; q < 16; ++q) vv[q] = vn[q];
+        load_v(i + 1 < n ? tok + kC : tok);  // (the last time for nothing)
+      }
       h8 s[NT][NJ];
       float smax = 0.0f, ssc = 1.0f, sinv = 1.0f;
       if constexpr (!BF) {
@@ -741,7 +749,6 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, int64_t slot0, int64_t slo
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[t][e] = __builtin_fmaf(-(BF ? c1[e] : c1[e] * sinv), ks[t][e], w2f<BF>((uint16_t)vx[t][e]));
       }
-      if (NW == 4) load_v(i + 1 < n ? tok + kC : tok);  // (the last time for nothing: a branch would copy the registers)
       h8 x[2][2];
       float xinv;
       const float xsc = pow2_scale(col_max<4>(v), xinv);
@@ -812,10 +819,20 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, int64_t slot0, int64_t slo
   const ChunkRec* rec = recs + (first + cb - slot0) * a.Hv + h;
   const bool outputs = wave < 2 * NW, fetches = !NF || !outputs;
   const int fi = NF ? wave - 2 * NW : w;  // which fetcher
-  auto fetch = [&](int i) {               // chunk i of the launch's
+  // Chunk i's rows of k, of q, and the rest. In three parts: 1 KiB into LDS takes a CU some 25 cycles and a wave that
+  // has several to issue waits for each, so they are issued between other work.
+  auto fetch_k = [&](int i) {
     const int64_t tk = t0 + (cb + i) * kC;
-    fetch_operands<DK, NP>(L.op[i & 1], a, tk, len_at(tk), hk, rec + (int64_t)i * a.Hv, fi, lane);
-    if constexpr (NW < 4) {  // KiB of 32 / NW rows
+    fetch_rows<DK, NP>(L.op[i & 1].k, a.k + tk * a.ld_k + hk * DK, a.ld_k, len_at(tk), fi, lane);
+  };
+  auto fetch_q = [&](int i) {
+    const int64_t tk = t0 + (cb + i) * kC;
+    fetch_rows<DK, NP>(L.op[i & 1].q, a.q + tk * a.ld_q + hk * DK, a.ld_q, len_at(tk), fi, lane);
+  };
+  auto fetch_rest = [&](int i) {
+    const int64_t tk = t0 + (cb + i) * kC;
+    fetch_record<NP>(L.op[i & 1].T, L.op[i & 1].vec, rec + (int64_t)i * a.Hv, fi, lane);
+    if constexpr (NW < 4) {  // v in KiB of 32 / NW rows
       const Rsrc r = rows_of(a.v + tk * a.ld_v + (int64_t)h * a.Dv + 16 * NW * vb, a.ld_v, len_at(tk), a.Dv - 16 * NW * vb);
       const int per = 32 / NW, row = lane / (2 * NW), ldb = (int)a.ld_v * 2;
       if (fi < 2 * NW)
@@ -825,22 +842,26 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, int64_t slot0, int64_t slo
   };
   const int ldo = (int)a.ld_out * 2, oo = c * ldo + (dv0 + 4 * g) * 2;
   if (fetches && n) {
-    fetch(0);
+    fetch_k(0);
+    fetch_q(0);
+    fetch_rest(0);
     __builtin_amdgcn_s_waitcnt(0);
   }
   for (int i = 0; i < n; ++i, tok += kC) {
     const Operands<DK>& op = L.op[i & 1];
     step_barrier();
     if (fetches) {
-      // (the fetchers of P's larger tiles wait with their part of the loads until the outputs have P: 1 KiB of
-      // loads into LDS holds a wave for a hundred cycles)
-      if (i + 1 < n && (!NF || fi < 2)) fetch(i + 1);
+      const bool next = i + 1 < n;
+      if (!NF && next) fetch_k(i + 1);
       switch (fi) {
         case 0: make_p<0, DK, BF>(L, op, lane, a.l2norm, a.scale); break;
         case 1: make_p<1, DK, BF>(L, op, lane, a.l2norm, a.scale); break;
         case 2: make_p<2, DK, BF>(L, op, lane, a.l2norm, a.scale); break;
         default: make_p<3, DK, BF>(L, op, lane, a.l2norm, a.scale); break;
       }
+      // (of the fetchers by themselves, those with the larger tiles of P leave more until the outputs have P)
+      if (next && NF && fi < 3) fetch_k(i + 1);
+      if (next && (!NF || fi < 2)) fetch_q(i + 1);
     }
     f32x4 qs[4];
     f32x4 sinv;
@@ -854,8 +875,13 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, int64_t slot0, int64_t slo
       sinv = BF ? f32x4{1.0f, 1.0f, 1.0f, 1.0f} : *(const f32x4*)&L.sfac[w][4 * g];
       rows_product<DK, BF, true>(op.q, lane, s, qs);
     }
+    if (!NF && i + 1 < n) fetch_rest(i + 1);
     step_barrier();
-    if (NF && fetches && i + 1 < n && fi >= 2) fetch(i + 1);
+    if (NF && fetches && i + 1 < n) {
+      if (fi == 3) fetch_k(i + 1);
+      if (fi >= 2) fetch_q(i + 1);
+      fetch_rest(i + 1);
+    }
     f32x4 o[4];
     f32x4 uinv;
     if (outputs) {
@@ -880,11 +906,10 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, int64_t slot0, int64_t slo
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const float c2 = L.c2[16 * t + c], pr = L.pr[16 * t + c];
-        uint32_t x[4];
+        float x[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = f2w<BF>(__builtin_fmaf(qs[t][e], c2 * sinv[e], o[t][e] * (pr * uinv[e])));
-        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-        __builtin_amdgcn_raw_buffer_store_b64(u32x2{x[0] | x[1] << 16, x[2] | x[3] << 16}, orow, oo, 16 * t * ldo, 0);
+        for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(qs[t][e], BF ? c2 : c2 * sinv[e], o[t][e] * (pr * uinv[e]));
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2{pack2<BF>(x[0], x[1]), pack2<BF>(x[2], x[3])}, orow, oo, 16 * t * ldo, 0);
       }
     }
   }

@@ -451,8 +451,8 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(256) void d
 // (rows of k's columns, 16 value columns per wave), and the waves that carry it need nothing of each other.
 //   NW waves, the chain proper: K S^T, U and the new state
 //   NW waves, the outputs: Q S^T, P U
-//   four fetchers: the next chunk's operands, straight into LDS, and a row tile each of this one's P = tril(Q K^T
-//   ..). Waves of their own; with NW = 4 the output waves do it beside their work (12 waves would be three to a SIMD and have
+//   the fetchers: this chunk's P = tril(Q K^T ..), a fragment or two each, and the next one's operands, straight
+//   into LDS. Waves of their own, as many as make eight in all; with NW = 4 the output waves do it beside their work (12 waves would be three to a SIMD and have
 //   168 registers each, and the chain needs 224).
 // So waves of different kinds share a SIMD, products of one fill the gaps of the other, and only what the state
 // needs is on the path from chunk to chunk.
@@ -462,8 +462,8 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(256) void d
 template <int DK>
 struct Operands {
   f16 k[kC][DK], q[kC][DK];
-  f16 T[6][2][64][8];
-  float vec[384];                 // c1, tr, w, rk, Gh, Gl of the record
+  f16 T[6][2][64][8];             // the record: T
+  float vec[384];                 // c1, tr, w, rk, Gh, Gl
 };
 template <int DK, int NW>
 struct ChainLds {
@@ -472,8 +472,8 @@ struct ChainLds {
   f16 S[NW][DK / 32][2][64][8];   // the state before the chunk, as operands
   f32x4 u[NW][4][64];
   f16 P[6][2][64][8];
-  float F[3][kC];                 // of P's row tiles 1 .. 3, see make_p
-  float c2[kC], pr[kC];           // scale e^{G_i} times q's row factor; the row factor of P
+  float F[6][32];                 // of P's fragments, see make_p
+  float c2[kC], pr[2][kC];        // scale e^{G_i} times q's row factor; the row factors of P, by column block
   float sfac[NW][16], ufac[NW][16];  // per value column: what undoes the scaling of S and of U
 };
 
@@ -514,22 +514,25 @@ __device__ __forceinline__ void load_tri(Tri& f, const f16 (*F)[2][64][8], int l
     f.lo[i] = *(const h8*)F[i][1][lane];
   }
 }
-// y = M x (both pairs; with FLIP the transpose), the four row tiles in turn so that no product waits for the one
-// before.
-template <bool FLIP>
-__device__ __forceinline__ void tri_product(const Tri& f, const h8 (&x)[2][2], f32x4 (&y)[4]) {
+// y[j] = M_j x_j for the 32-column blocks M_j of a triangle (both pairs; with FLIP the transpose), the row tiles in
+// turn so that no product waits for the one before. With SUM the blocks have one scale and y[0] takes both.
+template <bool FLIP, bool SUM>
+__device__ __forceinline__ void tri_product(const Tri& f, const h8 (&x)[2][2], f32x4 (&y)[2][4]) {
   const int at[4] = {0, 1, 2, 4};
   auto add = [&](const h8& u, const h8& v, f32x4& w) { w = FLIP ? mm<false>(v, u, w) : mm<false>(u, v, w); };
 #pragma unroll
-  for (int t = 0; t < 4; ++t) y[t] = f32x4{0, 0, 0, 0};
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int t = 2 * j; t < 4; ++t) y[j][t] = f32x4{0, 0, 0, 0};
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
+    f32x4 (&z)[4] = y[SUM ? 0 : j];
 #pragma unroll
-    for (int t = 2 * j; t < 4; ++t) add(f.lo[at[t] + j], x[0][j], y[t]);
+    for (int t = 2 * j; t < 4; ++t) add(f.lo[at[t] + j], x[0][j], z[t]);
 #pragma unroll
-    for (int t = 2 * j; t < 4; ++t) add(f.hi[at[t] + j], x[1][j], y[t]);
+    for (int t = 2 * j; t < 4; ++t) add(f.hi[at[t] + j], x[1][j], z[t]);
 #pragma unroll
-    for (int t = 2 * j; t < 4; ++t) add(f.hi[at[t] + j], x[0][j], y[t]);
+    for (int t = 2 * j; t < 4; ++t) add(f.hi[at[t] + j], x[0][j], z[t]);
   }
 }
 
@@ -568,97 +571,114 @@ __device__ __forceinline__ void rows_product(const f16 (*X)[DK], int lane, const
   }
 }
 
-typedef const __attribute__((address_space(1))) void* gptr;
 typedef __attribute__((address_space(3))) void* lptr;
 
-// 64 rows of halves into LDS, KiB i, i + NP, .. of it by fetcher i: 1 KiB per wave and instruction, the lanes
-// reading the pieces that belong there.
-template <int DK, int NP>
-__device__ __forceinline__ void fetch_rows(f16 (*to)[DK], const uint16_t* p, int64_t ld, int len, int i, int lane) {
+// 64 rows into LDS, KiB i, i + 4, .. of it, i < 4: 1 KiB per wave and instruction, the lanes reading the pieces that
+// belong there. Every fourth KiB has the same exchange of pieces, so a lane's offset (rows_off) serves them all.
+template <int DK>
+__device__ __forceinline__ int rows_off(int64_t ld, int i, int lane) {
   constexpr int per = 512 / DK, pieces = DK / 8;  // rows of a KiB, pieces of a row
-  const Rsrc r = rows_of(p, ld, len, DK);
-  const int row = lane / pieces, bytes = (int)ld * 2;
-#pragma unroll
-  for (int n = 0; n < kC / per; n += NP) {
-    const int m = n + i;
-    const int off = row * bytes + piece_at<DK>(per * m + row, lane % pieces) * 16;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr)((char*)to + m * 1024), 16, off, per * m * bytes, 0, 0);
-  }
+  const int row = per * i + lane / pieces;
+  return row * (int)ld * 2 + piece_at<DK>(row, lane % pieces) * 16;
 }
-// T and the factors of a chunk into LDS, by fetcher w of NP.
-template <int NP>
-__device__ __forceinline__ void fetch_record(f16 (*T)[2][64][8], float* vec, const ChunkRec* rec, int w, int lane) {
+template <int DK>
+__device__ __forceinline__ void fetch_rows(f16 (*to)[DK], const uint16_t* p, int64_t ld, int len, int i, int off) {
+  constexpr int per = 512 / DK;
+  const Rsrc r = rows_of(p, ld, len, DK);
+  const int step = per * 8 * (int)ld;
 #pragma unroll
-  for (int n = 0; n < 12; n += NP)
-    __builtin_amdgcn_global_load_lds((gptr)((const char*)rec + (n + w) * 1024 + lane * 16), (lptr)((char*)T + (n + w) * 1024), 16, 0, 0);
-  // the factors, 1536 bytes: 4 bytes per lane
-  for (int n = w; n < 6; n += NP)
-    __builtin_amdgcn_global_load_lds((gptr)(rec->c1 + n * 64 + lane), (lptr)(vec + n * 64), 4, 0, 0);
+  for (int n = 0; n < kC / per / 4; ++n)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr)((char*)to + (4 * n + i) * 1024), 16, off, n * step, 0, 0);
+}
+// KiB i, i + NP, .. of a chunk's record.
+template <int NP>
+__device__ __forceinline__ void fetch_record(void* to, const ChunkRec* rec, int i, int lane) {
+  constexpr int size = sizeof(ChunkRec);
+  const Rsrc r = __builtin_amdgcn_make_buffer_rsrc((void*)rec, 0, size, 0x00027000);
+#pragma unroll
+  for (int n = 0; n < size / 1024; n += NP)
+    if (n + i < size / 1024)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr)((char*)to + (n + i) * 1024), 16, lane * 16, (n + i) * 1024, 0, 0);
+  if (i == NP - 1)  // the last half, 8 bytes a lane: two instructions of 4
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr)((char*)to + size / 1024 * 1024 + n * 256), 4, lane * 4,
+                                               size / 1024 * 1024 + n * 256, 0, 0);
 }
 
-// Row tile W of P = tril(q_i.k_j e^{G_i - G_j}) and of q's factors.
-template <int W, int DK, bool BF, int NW>
+// Fragment (W, J) of P = tril(q_i.k_j e^{G_i - G_j}), rows 16 W .., columns 32 J .., with a scale of its own per row,
+// so that no fragment waits for another; the one on the diagonal also leaves q's factors.
+template <int W, int J, int DK, bool BF, int NW>
 __device__ __forceinline__ void make_p(ChainLds<DK, NW>& L, const Operands<DK>& op, int lane, bool l2norm, float scale) {
-  constexpr int NJ = DK / 32;
+  constexpr int NJ = DK / 32, F = W + (W > 2 ? 1 : 0) + J, T0 = 2 * J, NT = W > T0 ? 2 : 1;  // column tiles T0 .. T0 + NT - 1
+  constexpr bool diag = T0 + NT - 1 == W;
   const int g = lane >> 4, c = lane & 15, i = 16 * W + c;
   const float *rk = op.vec + 192, *Gh = op.vec + 256, *Gl = op.vec + 320;
   const float bh = Gh[16 * W], bl = Gl[16 * W];
-  // e^{G_i - G_j} for a j before the tile is taken apart at the tile's first row, as in the preparation
-  if constexpr (W > 0)
-    if (lane < 16 * W) L.F[W - 1][lane] = __builtin_amdgcn_exp2f((bh - Gh[lane]) + (bl - Gl[lane])) * rk[lane];
-  h8 q[NJ], k[W + 1][NJ];
+  // e^{G_i - G_j} for a j before the row tile is taken apart at the tile's first row, as in the preparation
+  if constexpr (NT == 2 || !diag) {
+    const int j = 32 * J + (lane & 31);
+    const float x = (bh - Gh[j]) + (bl - Gl[j]);
+    if (lane < 32) L.F[F][lane] = __builtin_amdgcn_exp2f(j < 16 * W ? x : 0.0f) * rk[j];
+  }
+  h8 q[NJ], k[NT][NJ];
 #pragma unroll
   for (int j = 0; j < NJ; ++j) q[j] = *(const h8*)&op.q[i][piece_at<DK>(i, 4 * j + g) * 8];
 #pragma unroll
-  for (int t = 0; t <= W; ++t)
+  for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) k[t][j] = *(const h8*)&op.k[16 * t + c][piece_at<DK>(16 * t + c, 4 * j + g) * 8];
-  f32x4 x[W + 1], qq = f32x4{0, 0, 0, 0};
-#pragma unroll
-  for (int t = 0; t <= W; ++t) x[t] = f32x4{0, 0, 0, 0};
+    for (int j = 0; j < NJ; ++j) {
+      const int row = 16 * (T0 + t) + c;
+      k[t][j] = *(const h8*)&op.k[row][piece_at<DK>(row, 4 * j + g) * 8];
+    }
+  f32x4 x[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}}, qq = f32x4{0, 0, 0, 0};
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
     if (l2norm) qq = mm<BF>(q[j], q[j], qq);
 #pragma unroll
-    for (int t = 0; t <= W; ++t) x[t] = mm<BF>(k[t][j], q[j], x[t]);
+    for (int t = 0; t < NT; ++t) x[t] = mm<BF>(k[t][j], q[j], x[t]);
   }
   const float gh = Gh[i], gl = Gl[i];
   float rq = scale;  // the squares are the diagonal of q q^T; lane (c / 4, c) has it for row c
   if (l2norm) rq *= l2_factor(__shfl(diagonal(qq, c), 16 * (c >> 2) + c, 64));
-  {
-    const f32x4 jh = *(const f32x4*)&Gh[16 * W + 4 * g], jl = *(const f32x4*)&Gl[16 * W + 4 * g];
-    const f32x4 rj = *(const f32x4*)&rk[16 * W + 4 * g];
+  const float pe = rq * __builtin_amdgcn_exp2f((gh - bh) + (gl - bl));
+  wave_sync();
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const bool in = 4 * g + e <= c;
-      const float d = __builtin_amdgcn_exp2f(in ? (gh - jh[e]) + (gl - jl[e]) : 0.0f) * rj[e];
-      x[W][e] = in ? (x[W][e] * rq) * d : 0.0f;
+  for (int t = 0; t < NT; ++t) {
+    if (T0 + t < W) {
+      const f32x4 f = *(const f32x4*)&L.F[F][16 * t + 4 * g];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[t][e] = (x[t][e] * pe) * f[e];
+    } else {
+      const f32x4 jh = *(const f32x4*)&Gh[16 * W + 4 * g], jl = *(const f32x4*)&Gl[16 * W + 4 * g];
+      const f32x4 rj = *(const f32x4*)&rk[16 * W + 4 * g];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool in = 4 * g + e <= c;
+        const float d = __builtin_amdgcn_exp2f(in ? (gh - jh[e]) + (gl - jl[e]) : 0.0f) * rj[e];
+        x[t][e] = in ? (x[t][e] * rq) * d : 0.0f;
+      }
     }
   }
-  if constexpr (W > 0) {
-    const float pe = rq * __builtin_amdgcn_exp2f((gh - bh) + (gl - bl));
-    wave_sync();
-#pragma unroll
-    for (int t = 0; t < W; ++t) {
-      const f32x4 F = *(const f32x4*)&L.F[W - 1][16 * t + 4 * g];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[t][e] = (x[t][e] * pe) * F[e];
-    }
-  }
-  const float inv = store_frags<W>(x, lane, L.P);
+  float inv;
+  const float sc = pow2_scale(max_rows4(max4(x[1], max4(x[0], 0.0f))), inv);
+  h8 part[2];
+  split8(x[0], x[1], sc, part);
+  *(h8*)L.P[F][0][lane] = part[0];
+  *(h8*)L.P[F][1][lane] = part[1];
   if (g == 0) {
-    L.pr[i] = inv;
-    L.c2[i] = rq * __builtin_amdgcn_exp2f(gh + gl);
+    L.pr[J][i] = inv;
+    if (diag) L.c2[i] = rq * __builtin_amdgcn_exp2f(gh + gl);
   }
 }
 
 template <int NW>
-constexpr int kFetchers = NW == 4 ? 0 : 4;  // waves of their own
+constexpr int kFetchers = NW == 4 ? 0 : (NW == 2 ? 4 : 6);  // waves of their own
 
 template <int DK, bool BF, int NW>
 __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(64 * (2 * NW + kFetchers<NW>)) void
 delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, int64_t slot0, int64_t slot1) {
-  constexpr int NM = DK / 16, NJ = DK / 32, NT = kParts<BF>, NF = kFetchers<NW>, NP = 4;
+  constexpr int NM = DK / 16, NJ = DK / 32, NT = kParts<BF>, NF = kFetchers<NW>, NP = NF ? NF : NW;
   __shared__ __align__(16) ChainLds<DK, NW> L;
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave % NW;
@@ -753,8 +773,9 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, int64_t slot0, int64_t slo
       float xinv;
       const float xsc = pow2_scale(col_max<4>(v), xinv);
       split_all<4>(v, xsc, x);
-      f32x4 u[4];
-      tri_product<false>(T, x, u);
+      f32x4 y[2][4];
+      tri_product<false, true>(T, x, y);
+      f32x4 (&u)[4] = y[0];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const f32x4 tr = vec[16 + 4 * t + g], ww = vec[2 * 16 + 4 * t + g];
@@ -819,25 +840,27 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, int64_t slot0, int64_t slo
   const ChunkRec* rec = recs + (first + cb - slot0) * a.Hv + h;
   const bool outputs = wave < 2 * NW, fetches = !NF || !outputs;
   const int fi = NF ? wave - 2 * NW : w;  // which fetcher
-  // Chunk i's rows of k, of q, and the rest. In three parts: 1 KiB into LDS takes a CU some 25 cycles and a wave that
-  // has several to issue waits for each, so they are issued between other work.
+  // Chunk i's rows of k, of q, and the rest: four fetchers have the rows, the others (or the same) the rest.
+  const int offk = rows_off<DK>(a.ld_k, fi & 3, lane), offq = rows_off<DK>(a.ld_q, fi & 3, lane);
+  constexpr int NR = NF == 6 ? 2 : 4;
+  const int ri = NF == 6 ? fi - 4 : fi;
   auto fetch_k = [&](int i) {
     const int64_t tk = t0 + (cb + i) * kC;
-    fetch_rows<DK, NP>(L.op[i & 1].k, a.k + tk * a.ld_k + hk * DK, a.ld_k, len_at(tk), fi, lane);
+    if (fi < 4) fetch_rows<DK>(L.op[i & 1].k, a.k + tk * a.ld_k + hk * DK, a.ld_k, len_at(tk), fi, offk);
   };
   auto fetch_q = [&](int i) {
     const int64_t tk = t0 + (cb + i) * kC;
-    fetch_rows<DK, NP>(L.op[i & 1].q, a.q + tk * a.ld_q + hk * DK, a.ld_q, len_at(tk), fi, lane);
+    if (fi < 4) fetch_rows<DK>(L.op[i & 1].q, a.q + tk * a.ld_q + hk * DK, a.ld_q, len_at(tk), fi, offq);
   };
   auto fetch_rest = [&](int i) {
     const int64_t tk = t0 + (cb + i) * kC;
-    fetch_record<NP>(L.op[i & 1].T, L.op[i & 1].vec, rec + (int64_t)i * a.Hv, fi, lane);
+    if (ri >= 0) fetch_record<NR>(L.op[i & 1].T, rec + (int64_t)i * a.Hv, ri, lane);
     if constexpr (NW < 4) {  // v in KiB of 32 / NW rows
       const Rsrc r = rows_of(a.v + tk * a.ld_v + (int64_t)h * a.Dv + 16 * NW * vb, a.ld_v, len_at(tk), a.Dv - 16 * NW * vb);
       const int per = 32 / NW, row = lane / (2 * NW), ldb = (int)a.ld_v * 2;
-      if (fi < 2 * NW)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr)((char*)L.v[i & 1] + fi * 1024), 16, row * ldb + lane % (2 * NW) * 16,
-                                                 per * fi * ldb, 0, 0);
+      if (ri >= 0 && ri < 2 * NW)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr)((char*)L.v[i & 1] + ri * 1024), 16, row * ldb + lane % (2 * NW) * 16,
+                                                 per * ri * ldb, 0, 0);
     }
   };
   const int ldo = (int)a.ld_out * 2, oo = c * ldo + (dv0 + 4 * g) * 2;
@@ -853,15 +876,27 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, int64_t slot0, int64_t slo
     if (fetches) {
       const bool next = i + 1 < n;
       if (!NF && next) fetch_k(i + 1);
-      switch (fi) {
-        case 0: make_p<0, DK, BF>(L, op, lane, a.l2norm, a.scale); break;
-        case 1: make_p<1, DK, BF>(L, op, lane, a.l2norm, a.scale); break;
-        case 2: make_p<2, DK, BF>(L, op, lane, a.l2norm, a.scale); break;
-        default: make_p<3, DK, BF>(L, op, lane, a.l2norm, a.scale); break;
+      auto p = [&](auto w, auto j) {
+        make_p<decltype(w)::value, decltype(j)::value, DK, BF>(L, op, lane, a.l2norm, a.scale);
+      };
+      if constexpr (NP == 6) {
+        switch (fi) {
+          case 0: p(Int<0>{}, Int<0>{}); break;
+          case 1: p(Int<1>{}, Int<0>{}); break;
+          case 2: p(Int<2>{}, Int<0>{}); break;
+          case 3: p(Int<2>{}, Int<1>{}); break;
+          case 4: p(Int<3>{}, Int<0>{}); break;
+          default: p(Int<3>{}, Int<1>{});
+        }
+      } else {  // by fours: three of the ten tiles at most
+        switch (fi) {
+          case 0: p(Int<3>{}, Int<1>{}); break;
+          case 1: p(Int<3>{}, Int<0>{}); break;
+          case 2: p(Int<2>{}, Int<0>{}), p(Int<0>{}, Int<0>{}); break;
+          default: p(Int<1>{}, Int<0>{}), p(Int<2>{}, Int<1>{});
+        }
       }
-      // (of the fetchers by themselves, those with the larger tiles of P leave more until the outputs have P)
-      if (next && NF && fi < 3) fetch_k(i + 1);
-      if (next && (!NF || fi < 2)) fetch_q(i + 1);
+      if (!NF && next) fetch_q(i + 1);
     }
     f32x4 qs[4];
     f32x4 sinv;
@@ -878,11 +913,11 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, int64_t slot0, int64_t slo
     if (!NF && i + 1 < n) fetch_rest(i + 1);
     step_barrier();
     if (NF && fetches && i + 1 < n) {
-      if (fi == 3) fetch_k(i + 1);
-      if (fi >= 2) fetch_q(i + 1);
+      fetch_k(i + 1);
+      fetch_q(i + 1);
       fetch_rest(i + 1);
     }
-    f32x4 o[4];
+    f32x4 o[2][4];
     f32x4 uinv;
     if (outputs) {
       Tri P;
@@ -895,7 +930,7 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, int64_t slot0, int64_t slo
       const float usc = pow2_scale(col_max<4>(u), inv);
       if (g == 0) L.ufac[w][c] = inv;
       split_all<4>(u, usc, x);
-      tri_product<true>(P, x, o);
+      tri_product<true, false>(P, x, o);
       wave_sync();
       uinv = *(const f32x4*)&L.ufac[w][4 * g];
     }
@@ -905,10 +940,13 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, int64_t slot0, int64_t slo
       const Rsrc orow = rows_of(a.out + tok * a.ld_out + (int64_t)h * a.Dv, a.ld_out, len_at(tok), a.Dv);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const float c2 = L.c2[16 * t + c], pr = L.pr[16 * t + c];
+        const float c2 = L.c2[16 * t + c], p0 = L.pr[0][16 * t + c], p1 = t >= 2 ? L.pr[1][16 * t + c] : 0.0f;
         float x[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(qs[t][e], BF ? c2 : c2 * sinv[e], o[t][e] * (pr * uinv[e]));
+        for (int e = 0; e < 4; ++e) {
+          const float pu = t >= 2 ? __builtin_fmaf(o[1][t][e], p1, o[0][t][e] * p0) : o[0][t][e] * p0;
+          x[e] = __builtin_fmaf(qs[t][e], BF ? c2 : c2 * sinv[e], pu * uinv[e]);
+        }
         __builtin_amdgcn_raw_buffer_store_b64(u32x2{pack2<BF>(x[0], x[1]), pack2<BF>(x[2], x[3])}, orow, oo, 16 * t * ldo, 0);
       }
     }

@@ -639,9 +639,7 @@ __device__ __forceinline__ void make_p(ChainLds<DK, NW>& L, const Operands<DK>& 
     for (int t = 0; t < NT; ++t) x[t] = mm<BF>(k[t][j], q[j], x[t]);
   }
   const float gh = Gh[i], gl = Gl[i];
-  float rq = scale;  // the squares are the diagonal of q q^T; lane (c / 4, c) has it for row c
-  if (l2norm) rq *= l2_factor(__shfl(diagonal(qq, c), 16 * (c >> 2) + c, 64));
-  const float pe = rq * __builtin_amdgcn_exp2f((gh - bh) + (gl - bl));
+  const float pe = __builtin_amdgcn_exp2f((gh - bh) + (gl - bl));
   wave_sync();
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
@@ -656,7 +654,7 @@ __device__ __forceinline__ void make_p(ChainLds<DK, NW>& L, const Operands<DK>& 
       for (int e = 0; e < 4; ++e) {
         const bool in = 4 * g + e <= c;
         const float d = __builtin_amdgcn_exp2f(in ? (gh - jh[e]) + (gl - jl[e]) : 0.0f) * rj[e];
-        x[t][e] = in ? (x[t][e] * rq) * d : 0.0f;
+        x[t][e] = in ? x[t][e] * d : 0.0f;
       }
     }
   }
@@ -666,8 +664,11 @@ __device__ __forceinline__ void make_p(ChainLds<DK, NW>& L, const Operands<DK>& 
   split8(x[0], x[1], sc, part);
   *(h8*)L.P[F][0][lane] = part[0];
   *(h8*)L.P[F][1][lane] = part[1];
+  // (the row has a scale of its own, so q's factor goes there, off the way to the operand)
+  float rq = scale;  // the squares are the diagonal of q q^T; lane (c / 4, c) has it for row c
+  if (l2norm) rq *= l2_factor(__shfl(diagonal(qq, c), 16 * (c >> 2) + c, 64));
   if (g == 0) {
-    L.pr[J][i] = inv;
+    L.pr[J][i] = inv * rq;
     if (diag) L.c2[i] = rq * __builtin_amdgcn_exp2f(gh + gl);
   }
 }
@@ -842,8 +843,6 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, int64_t slot0, int64_t slo
   const int fi = NF ? wave - 2 * NW : w;  // which fetcher
   // Chunk i's rows of k, of q, and the rest: four fetchers have the rows, the others (or the same) the rest.
   const int offk = rows_off<DK>(a.ld_k, fi & 3, lane), offq = rows_off<DK>(a.ld_q, fi & 3, lane);
-  constexpr int NR = NF == 6 ? 2 : 4;
-  const int ri = NF == 6 ? fi - 4 : fi;
   auto fetch_k = [&](int i) {
     const int64_t tk = t0 + (cb + i) * kC;
     if (fi < 4) fetch_rows<DK>(L.op[i & 1].k, a.k + tk * a.ld_k + hk * DK, a.ld_k, len_at(tk), fi, offk);
@@ -852,22 +851,23 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, int64_t slot0, int64_t slo
     const int64_t tk = t0 + (cb + i) * kC;
     if (fi < 4) fetch_rows<DK>(L.op[i & 1].q, a.q + tk * a.ld_q + hk * DK, a.ld_q, len_at(tk), fi, offq);
   };
-  auto fetch_rest = [&](int i) {
+  auto fetch_rest = [&](int i, int part) {  // part of 4
     const int64_t tk = t0 + (cb + i) * kC;
-    if (ri >= 0) fetch_record<NR>(L.op[i & 1].T, rec + (int64_t)i * a.Hv, ri, lane);
-    if constexpr (NW < 4) {  // v in KiB of 32 / NW rows
+    fetch_record<4>(L.op[i & 1].T, rec + (int64_t)i * a.Hv, part, lane);
+    if constexpr (NW < 4) {  // v in KiB of 32 / NW rows, by the last parts
       const Rsrc r = rows_of(a.v + tk * a.ld_v + (int64_t)h * a.Dv + 16 * NW * vb, a.ld_v, len_at(tk), a.Dv - 16 * NW * vb);
-      const int per = 32 / NW, row = lane / (2 * NW), ldb = (int)a.ld_v * 2;
-      if (ri >= 0 && ri < 2 * NW)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr)((char*)L.v[i & 1] + ri * 1024), 16, row * ldb + lane % (2 * NW) * 16,
-                                                 per * ri * ldb, 0, 0);
+      const int per = 32 / NW, row = lane / (2 * NW), ldb = (int)a.ld_v * 2, m = part - (4 - 2 * NW);
+      if (m >= 0)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr)((char*)L.v[i & 1] + m * 1024), 16, row * ldb + lane % (2 * NW) * 16,
+                                                 per * m * ldb, 0, 0);
     }
   };
   const int ldo = (int)a.ld_out * 2, oo = c * ldo + (dv0 + 4 * g) * 2;
   if (fetches && n) {
     fetch_k(0);
     fetch_q(0);
-    fetch_rest(0);
+    if (NF < 6) fetch_rest(0, fi);
+    else if (fi < 4) fetch_rest(0, fi);
     __builtin_amdgcn_s_waitcnt(0);
   }
   for (int i = 0; i < n; ++i, tok += kC) {
@@ -875,7 +875,10 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, int64_t slot0, int64_t slo
     step_barrier();
     if (fetches) {
       const bool next = i + 1 < n;
-      if (!NF && next) fetch_k(i + 1);
+      if (next) {
+        fetch_k(i + 1);
+        if (NF) fetch_q(i + 1);
+      }
       auto p = [&](auto w, auto j) {
         make_p<decltype(w)::value, decltype(j)::value, DK, BF>(L, op, lane, a.l2norm, a.scale);
       };
@@ -896,7 +899,9 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, int64_t slot0, int64_t slo
           default: p(Int<1>{}, Int<0>{}), p(Int<2>{}, Int<1>{});
         }
       }
-      if (!NF && next) fetch_q(i + 1);
+      if (next) {
+        if (!NF) fetch_q(i + 1);
+      }
     }
     f32x4 qs[4];
     f32x4 sinv;
@@ -910,12 +915,14 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, int64_t slot0, int64_t slo
       sinv = BF ? f32x4{1.0f, 1.0f, 1.0f, 1.0f} : *(const f32x4*)&L.sfac[w][4 * g];
       rows_product<DK, BF, true>(op.q, lane, s, qs);
     }
-    if (!NF && i + 1 < n) fetch_rest(i + 1);
+    if (i + 1 < n) {  // with six fetchers the output wave, which has less to do, helps
+      if (!NF) fetch_rest(i + 1, fi);
+      if (NF == 6 && outputs) fetch_rest(i + 1, 0), fetch_rest(i + 1, 1);
+    }
     step_barrier();
-    if (NF && fetches && i + 1 < n) {
-      fetch_k(i + 1);
-      fetch_q(i + 1);
-      fetch_rest(i + 1);
+    if (i + 1 < n && fetches) {
+      if (NF == 4) fetch_rest(i + 1, fi);
+      if (NF == 6 && fi >= 4) fetch_rest(i + 1, fi - 2);
     }
     f32x4 o[2][4];
     f32x4 uinv;
@@ -935,7 +942,7 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, int64_t slot0, int64_t slo
       uinv = *(const f32x4*)&L.ufac[w][4 * g];
     }
     // what this wave loads for the next chunk is in before it stores, so that the wait is not for the stores
-    if (fetches) __builtin_amdgcn_s_waitcnt(0);
+    if (fetches || NF == 6) __builtin_amdgcn_s_waitcnt(0);
     if (outputs && active) {
       const Rsrc orow = rows_of(a.out + tok * a.ld_out + (int64_t)h * a.Dv, a.ld_out, len_at(tok), a.Dv);
 #pragma unroll

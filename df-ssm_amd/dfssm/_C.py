@@ -162,3 +162,12 @@ def stream() -> int:
         _get_raw_stream = torch._C._cuda_getCurrentRawStream
         return handle
     return _get_raw_stream(torch._C._cuda_getDevice())
+
+
+def current_device() -> int:
+    """The index of torch's current device. After the first call as stream() asks for it, without
+    torch.cuda.current_device()'s checks."""
+    import torch
+    if _get_raw_stream is None:
+        return torch.cuda.current_device()
+    return torch._C._cuda_getDevice()

@@ -177,87 +177,115 @@ def ssm_step(h: torch.Tensor, xbc: torch.Tensor, dt: torch.Tensor, dt_bias, A_lo
 _TYPE16 = {torch.float16: 0, torch.bfloat16: 1}   # DFSSM_TYPE_F16, DFSSM_TYPE_BF16
 
 
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """(tokens, heads, dim) with heads contiguous and 16-byte aligned tokens: t itself or a copy."""
-    s = t.stride()
-    if s[2] == 1 and s[1] == t.shape[2] and s[0] % 8 == 0 and t.data_ptr() % 16 == 0:
-        return t
-    return t.contiguous() if not t.is_contiguous() else t.clone()
+_MAX_LD = 1 << 23   # elements from token to token: the kernels' offsets within a chunk are 32-bit
 
 
-def _on_device(t: torch.Tensor, name: str, dev) -> None:
-    if t is not None and t.device != dev:
-        raise ValueError(f"{name} is on {t.device}, not on {dev}")
+def _rows16(t: torch.Tensor, width: int):
+    """t (tokens, heads, dim) with heads contiguous and 16-byte aligned tokens, itself or a copy, and the
+    distance of its tokens in elements; width = heads * dim."""
+    ld, h, d = t.stride()
+    if t.shape[0] <= 1:
+        ld = width
+    if d == 1 and h == t.shape[2] and ld % 8 == 0 and ld <= _MAX_LD and t.data_ptr() % 16 == 0:
+        return t, ld
+    return (t.clone(memory_format=torch.contiguous_format)), width
+
+
+def _rows32(t: torch.Tensor):
+    """The same of (tokens, heads) fp32."""
+    ld, h = t.stride()
+    if t.shape[0] <= 1:
+        ld = t.shape[1]
+    if (h == 1 or t.shape[1] == 1) and ld <= _MAX_LD:
+        return t, ld
+    return t.clone(memory_format=torch.contiguous_format), t.shape[1]
 
 
 def _delta_call(step: bool, q, k, v, g, beta, state, cu_seqlens, slots, scale, l2norm, out, state_out, n_seq):
     """Checks (tokens, heads, dim) arguments, launches and returns out."""
-    dev = q.device if isinstance(q, torch.Tensor) else None
-    kind = _TYPE16.get(q.dtype) if isinstance(q, torch.Tensor) else None
+    dt = q.dtype if isinstance(q, torch.Tensor) else None
+    kind = _TYPE16.get(dt)
     if kind is None:
         raise TypeError("q must be a float16 or bfloat16 tensor")
-    for t, n in ((q, "q"), (k, "k"), (v, "v")):
-        _need(t, q.dtype, n)
-        if t.dim() != 3:
-            raise ValueError(f"{n} must have 3 dimensions, got {tuple(t.shape)}")
-    for t, n in ((g, "g"), (beta, "beta"), (state, "state")):
-        _need(t, torch.float32, n)
-    T, Hk, Dk = q.shape
-    Hv, Dv = v.shape[1:]
-    if k.shape != q.shape or v.shape[0] != T or g.shape != (T, Hv) or beta.shape != (T, Hv):
+    dev = q.get_device()
+    f32 = torch.float32
+    for t, d, n in ((q, dt, "q"), (k, dt, "k"), (v, dt, "v"), (g, f32, "g"), (beta, f32, "beta"), (state, f32, "state")):
+        if not isinstance(t, torch.Tensor) or t.dtype is not d or t.get_device() != dev or dev < 0:
+            _need(t, d, n)
+            raise ValueError("all tensors must be on one device")
+    qs, vs, gs = q.shape, v.shape, g.shape
+    if len(qs) != 3 or len(vs) != 3 or k.shape != qs or vs[0] != qs[0] or gs != vs[:2] or beta.shape != gs:
         raise ValueError("shape mismatch: q, k (tokens, key heads, k_dim), v (tokens, value heads, v_dim), "
-                         f"g, beta (tokens, value heads); got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}, "
-                         f"{tuple(g.shape)}, {tuple(beta.shape)}")
+                         f"g, beta (tokens, value heads); got {tuple(qs)}, {tuple(k.shape)}, {tuple(vs)}, "
+                         f"{tuple(gs)}, {tuple(beta.shape)}")
+    T, Hk, Dk = qs
+    _, Hv, Dv = vs
     if Dk not in (64, 128) or Dv % 16 or not 16 <= Dv <= 256 or Hk < 1 or Hv < 1 or Hv % Hk:
         raise ValueError("k_dim must be 64 or 128, v_dim a multiple of 16 up to 256, and the value heads a multiple "
                          f"of the key heads; got k_dim {Dk}, v_dim {Dv}, {Hv} and {Hk} heads")
-    if state.dim() != 4 or state.shape[1:] != (Hv, Dv, Dk) or not state.is_contiguous():
+    ss = state.shape
+    if len(ss) != 4 or ss[1] != Hv or ss[2] != Dv or ss[3] != Dk or not state.is_contiguous():
         raise ValueError(f"state must be contiguous (slots, {Hv}, {Dv}, {Dk})")
-    if state_out is None:
-        state_out = state
-    elif state_out is not state:
+    sp = state.data_ptr()
+    if state_out is None or state_out is state:
+        state_out, so = state, sp
+    else:
         _need(state_out, torch.float32, "state_out")
-        if state_out.shape != state.shape or not state_out.is_contiguous():
-            raise ValueError("state_out must be contiguous and of state's shape")
-        lo, n = state.data_ptr(), state.numel() * 4
-        if lo != state_out.data_ptr() and abs(state_out.data_ptr() - lo) < n:
+        if state_out.shape != ss or not state_out.is_contiguous() or state_out.get_device() != dev:
+            raise ValueError("state_out must be contiguous, of state's shape and on its device")
+        so = state_out.data_ptr()
+        if sp != so and abs(so - sp) < state.numel() * 4:
             raise ValueError("state_out must be state or not overlap it")
+    if sp % 16 or so % 16:
+        raise ValueError("state must be 16-byte aligned")
     if slots is not None:
         _need(slots, torch.int32, "slots")
         if slots.shape != (n_seq,):
             raise ValueError(f"slots must be ({n_seq},)")
+        if slots.get_device() != dev:
+            raise ValueError("slots is on another device than q")
         slots = slots.contiguous()
-    elif state.shape[0] < n_seq:
-        raise ValueError(f"state has {state.shape[0]} slots for {n_seq} sequences")
-    if state.data_ptr() % 16 or state_out.data_ptr() % 16:
-        raise ValueError("state must be 16-byte aligned")
+    elif ss[0] < n_seq:
+        raise ValueError(f"state has {ss[0]} slots for {n_seq} sequences")
+    if cu_seqlens is not None and cu_seqlens.get_device() != dev:
+        raise ValueError("cu_seqlens is on another device than q")
+    width = Hv * Dv
     if out is None:
-        out = torch.empty(T, Hv, Dv, dtype=q.dtype, device=dev)
+        out, ld_out = torch.empty(vs, dtype=dt, device=q.device), width
     else:
-        _need(out, q.dtype, "out")
-        if out.shape != v.shape or (T and _rows16(out) is not out):
-            raise ValueError("out must have v's shape, contiguous heads and 16-byte aligned tokens")
-    for t, n in ((k, "k"), (v, "v"), (g, "g"), (beta, "beta"), (state, "state"), (state_out, "state_out"),
-                 (slots, "slots"), (cu_seqlens, "cu_seqlens"), (out, "out")):
-        _on_device(t, n, dev)
+        _need(out, dt, "out")
+        if out.shape != vs or out.get_device() != dev:
+            raise ValueError("out must have v's shape and be on q's device")
+        row, ld_out = _rows16(out, width)
+        if row is not out or ld_out < width:
+            raise ValueError("out must have contiguous heads and 16-byte aligned tokens that do not overlap")
     if n_seq == 0:
         return out
-    q, k, v = _rows16(q), _rows16(k), _rows16(v)
-    g = g if g.stride(1) == 1 else g.contiguous()
-    beta = beta if beta.stride(1) == 1 else beta.contiguous()
-    args = _C.Delta(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), state.data_ptr(),
-                    state_out.data_ptr(), _C.ptr(slots), _C.ptr(cu_seqlens), out.data_ptr(),
-                    q.stride(0), k.stride(0), v.stride(0), g.stride(0), beta.stride(0), out.stride(0), T,
-                    n_seq, state.shape[0], Hk, Hv, Dk, Dv, kind, 1 if l2norm else 0,
-                    Dk ** -0.5 if scale is None else scale)
-    with torch.cuda.device(dev):
-        if step:
-            _C.check(_C.lib().dfssm_gated_delta_step(args, _C.stream()), "gated_delta_step")
-        else:
-            need = _C.lib().dfssm_gated_delta_workspace_bytes(args)
-            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-            _C.check(_C.lib().dfssm_gated_delta_prefill(args, _C.ptr(ws), _C.stream()), "gated_delta_prefill")
+    q, ld_q = _rows16(q, Hk * Dk)
+    k, ld_k = _rows16(k, Hk * Dk)
+    v, ld_v = _rows16(v, width)
+    g, ld_g = _rows32(g)
+    beta, ld_beta = _rows32(beta)
+    args = _C.Delta(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), sp, so, _C.ptr(slots),
+                    _C.ptr(cu_seqlens), out.data_ptr(), ld_q, ld_k, ld_v, ld_g, ld_beta, ld_out, T, n_seq, ss[0],
+                    Hk, Hv, Dk, Dv, kind, 1 if l2norm else 0, Dk ** -0.5 if scale is None else scale)
+    if dev != _C.current_device():
+        with torch.cuda.device(dev):
+            _delta_launch(step, args, q.device)
+    else:
+        _delta_launch(step, args, q.device)
     return out
+
+
+def _delta_launch(step: bool, args, device) -> None:
+    if step:
+        rc = _C.lib().dfssm_gated_delta_step(args, _C.stream())
+        if rc:
+            _C.check(rc, "gated_delta_step")
+        return
+    need = _C.lib().dfssm_gated_delta_workspace_bytes(args)
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    _C.check(_C.lib().dfssm_gated_delta_prefill(args, _C.ptr(ws), _C.stream()), "gated_delta_prefill")
 
 
 def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
@@ -311,6 +339,24 @@ def gated_delta_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: to
 _LOGIT_TYPE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}   # DFSSM_TYPE_*
 
 
+def _on_device(t: torch.Tensor, name: str, dev) -> None:
+    if t.device != dev:
+        raise ValueError(f"{name} is on {t.device}, not on {dev}")
+
+
+def _per_row(x, dtype, name: str, B: int, dev, held: list):
+    """A parameter as (number, device pointer): one of them counts."""
+    if not isinstance(x, torch.Tensor):
+        return (int(x) if dtype is torch.int32 else float(x)), 0
+    _need(x, dtype, name)
+    if x.shape != (B,):
+        raise ValueError(f"{name} must be a number or ({B},)")
+    _on_device(x, name, dev)
+    x = x.contiguous()
+    held.append(x)
+    return 0, x.data_ptr()
+
+
 def sample_filtered(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
                     want_logprob=False):
     """Tokens (B,) int64 drawn from logits (B, V) fp16, bf16 or fp32 with the random numbers u (B,) fp32 in
@@ -335,27 +381,27 @@ def sample_filtered(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_
     if u.shape != (B,):
         raise ValueError(f"u must be ({B},)")
     _on_device(u, "u", dev)
-    ptrs, values, held = [], [], [u.contiguous()]
-    for x, n, dt in ((temperature, "temperature", torch.float32), (top_k, "top_k", torch.int32),
-                     (top_p, "top_p", torch.float32), (min_p, "min_p", torch.float32)):
-        if isinstance(x, torch.Tensor):
-            _need(x, dt, n)
-            if x.shape != (B,):
-                raise ValueError(f"{n} must be a number or ({B},)")
-            _on_device(x, n, dev)
-            x = x.contiguous()
-            held.append(x)
-            ptrs.append(x.data_ptr())
-            values.append(0)
-        else:
-            ptrs.append(0)
-            values.append(int(x) if dt is torch.int32 else float(x))
-    if logits.stride(1) != 1 or (B > 1 and logits.stride(0) < V):
-        logits = logits.contiguous()
+    u = u.contiguous()
+    held = []   # copies of parameters live until the launch
+    temperature, tp = _per_row(temperature, torch.float32, "temperature", B, dev, held)
+    top_k, kp = _per_row(top_k, torch.int32, "top_k", B, dev, held)
+    top_p, pp = _per_row(top_p, torch.float32, "top_p", B, dev, held)
+    min_p, mp = _per_row(min_p, torch.float32, "min_p", B, dev, held)
+    ld, one = logits.stride()
+    if (one != 1 and V > 1) or (B > 1 and ld < V):
+        logits, ld = logits.clone(memory_format=torch.contiguous_format), V
     tokens = torch.empty(B, dtype=torch.int64, device=dev)
     logprob = torch.empty(B, dtype=torch.float32, device=dev) if want_logprob else None
-    with torch.cuda.device(dev):
-        _C.check(_C.lib().dfssm_sample_filtered(logits.data_ptr(), kind, logits.stride(0), B, V, held[0].data_ptr(),
-                                                _C.Filter(*ptrs, *values), tokens.data_ptr(), _C.ptr(logprob),
-                                                _C.stream()), "sample_filtered")
+    flt = _C.Filter(tp, kp, pp, mp, temperature, top_k, top_p, min_p)
+
+    def launch():
+        rc = _C.lib().dfssm_sample_filtered(logits.data_ptr(), kind, ld, B, V, u.data_ptr(), flt, tokens.data_ptr(),
+                                            _C.ptr(logprob), _C.stream())
+        if rc:
+            _C.check(rc, "sample_filtered")
+    if dev.index != _C.current_device():
+        with torch.cuda.device(dev):
+            launch()
+    else:
+        launch()
     return (tokens, logprob) if want_logprob else tokens

@@ -75,7 +75,7 @@ def prefill(x, lens, **kw):
 
 # batch, heads, key and value dimensions; 208 leaves a part of a 64-row block
 STEP = [(1, 1, 1, 128, 16), (1, 16, 64, 128, 64), (3, 2, 6, 64, 208), (5, 1, 8, 128, 256), (33, 4, 8, 64, 32),
-        (64, 8, 8, 128, 64), (2, 3, 3, 64, 112)]
+        (64, 8, 8, 128, 64), (2, 3, 3, 64, 112), (33, 4, 8, 64, 208), (64, 4, 16, 128, 48)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])

@@ -10,10 +10,13 @@
 // counts and masses. e is computed in fp64 and its masses are held as integers, E = rint(e 2^44), so
 // sums are exact and the same in any order (V <= 2^18, so they stay below 2^62).
 //
-// One workgroup per row. The row is spread over 2048 bins of falling logit (a monotone map, so bins are
-// ranges of the ranking): counts and masses by LDS atomics, then their prefix sums. A search takes its
-// bin from the prefix sums and resolves it by the exact 32-bit order key and the index, a byte at a
-// time: over the bin's tokens gathered into LDS, or over the row where they are too many.
+// One workgroup per row. The row is spread over 2048 bins of falling logit (a monotone map, so bins are ranges of
+// the ranking) whose counts, and masses where all tokens' matter, are summed by LDS atomics.
+//   Few kept: with a top_k (or only a min_p) the first bins hold all that can be kept. If that is at most 2048
+//   tokens they are gathered into LDS and sorted, and nothing but they needs an exponential.
+//   Else every token's mass goes into its bin, and a search takes its bin from the prefix sums and resolves it
+//   there: the bin's tokens gathered and sorted, or, where they are more than 2048, found by the exact 32-bit
+//   order key and the index, a byte at a time over the row.
 #include "common.h"
 #include "dfssm.h"
 #include "dfssm_kernels.h"
@@ -25,7 +28,7 @@ namespace {
 constexpr int kDT = 1024;      // threads of a row's workgroup
 constexpr int kBins = 2048;
 constexpr int kFine = 1024;    // bins of 1/64 in (m - l) / T; the others share what lies below
-constexpr int kList = 2048;    // tokens of a bin held in LDS
+constexpr int kList = 2048;    // tokens that are sorted in LDS
 constexpr double kOne = 17592186044416.0;  // 2^44
 
 typedef unsigned long long u64;
@@ -38,6 +41,38 @@ __device__ __forceinline__ float logit_at(const void* row, int i) {
 }
 // A NaN ranks as -inf; -0 as +0 (they are equal, so their order is that of the indexes).
 __device__ __forceinline__ float clean(float l) { return l != l ? -__builtin_inff() : l + 0.0f; }
+
+// f(index, logit) for every token of the row, by all threads: 16 bytes a load between the row's aligned ends, four
+// loads under way.
+template <int TYPE, class F>
+__device__ __forceinline__ void each_token(const void* row, int V, F f) {
+  constexpr int ES = TYPE == DFSSM_TYPE_F32 ? 4 : 2, N = 16 / ES;
+  const int tid = threadIdx.x;
+  const int head = min(V, (int)((16 - ((uintptr_t)row & 15)) & 15) / ES), nb = (V - head) / N, tail = head + nb * N;
+  if (tid < head) f(tid, clean(logit_at<TYPE>(row, tid)));
+  if (tail + tid < V) f(tail + tid, clean(logit_at<TYPE>(row, tail + tid)));
+  const u32x4* p = (const u32x4*)((const char*)row + head * ES);
+  for (int c = tid; c < nb; c += 4 * kDT) {
+    u32x4 x[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) x[q] = p[min(c + q * kDT, nb - 1)];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int b = c + q * kDT;
+      if (b >= nb) break;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const uint32_t word = x[q][e * ES / 4];  // (a copy: a bit_cast of a vector's element takes the first one)
+        float l;
+        if constexpr (TYPE == DFSSM_TYPE_F32) l = __builtin_bit_cast(float, word);
+        else if constexpr (TYPE == DFSSM_TYPE_BF16) l = __builtin_bit_cast(float, (e & 1) ? word & 0xffff0000u : word << 16);
+        else l = h2f((uint16_t)(word >> (16 * (e & 1))));
+        f(head + b * N + e, clean(l));
+      }
+    }
+  }
+}
+
 // Ascending in falling logit.
 __device__ __forceinline__ uint32_t order_key(float l) {
   const uint32_t b = __builtin_bit_cast(uint32_t, l);
@@ -49,7 +84,8 @@ __device__ __forceinline__ float key_logit(uint32_t k) {
 
 struct RowScale {
   float m, s1, s2;   // bins: x = (m - l) s1 below kFine, then kFine + (x - kFine) s2
-  double it;         // 1 / T
+  double y1;         // 64 log2(e) / T: e = 2^((l - m) y1 / 64)
+  const double* tab; // 2^(j / 64), j = 0 .. 63
 };
 __device__ __forceinline__ int bin_of(const RowScale& r, float l) {
   if (l == r.m) return 0;  // (also where both are +inf)
@@ -58,16 +94,34 @@ __device__ __forceinline__ int bin_of(const RowScale& r, float l) {
   const float y = (x - (float)kFine) * r.s2;
   return kFine + (y < (float)(kBins - kFine - 1) ? (int)y : kBins - kFine - 1);
 }
+// exp((l - m) / T) = 2^(n / 64) e^x, n whole, |x| <= ln 2 / 128: a table and a Taylor polynomial of degree 5, whose
+// rest is below 2^-54. (exp() takes four times as many instructions, and this is most of the work.)
 __device__ __forceinline__ double e_of(const RowScale& r, float l) {
-  return l == r.m ? 1.0 : exp(((double)l - (double)r.m) * r.it);
+  const double y = ((double)l - (double)r.m) * r.y1;
+  if (l == r.m) return 1.0;
+  if (!(y > -64.0 * 1020.0)) return 0.0;
+  const double n = __builtin_rint(y);
+  const double x = (y - n) * (0.693147180559945309417 / 64.0);
+  double p = 1.0 / 120.0;
+  p = __builtin_fma(p, x, 1.0 / 24.0);
+  p = __builtin_fma(p, x, 1.0 / 6.0);
+  p = __builtin_fma(p, x, 0.5);
+  p = __builtin_fma(p, x, 1.0);
+  p = __builtin_fma(p, x, 1.0);
+  const int i = (int)n;
+  return __builtin_amdgcn_ldexp(r.tab[i & 63] * p, i >> 6);
 }
-__device__ __forceinline__ u64 mass_of(double e) { return (u64)__builtin_rint(e * kOne); }
+// rint(e 2^44), 0 <= e <= 1: added to 2^52 it is the low bits of the sum.
+__device__ __forceinline__ u64 mass_of(double e) {
+  return __builtin_bit_cast(u64, __builtin_fma(e, kOne, 4503599627370496.0)) & 0xfffffffffffffull;
+}
 
 struct DrawLds {
+  double tab[64];
   uint32_t cnt[kBins];   // per bin, then tokens in earlier bins
   u64 mass[kBins];       // the same for masses
-  u64 comp[kList];       // (order key << 24) | index of the listed bin's tokens
-  u64 lmass[kList];
+  u64 comp[kList];       // (order key << 24) | index of the listed tokens, sorted
+  u64 lmass[kList];      // mass ranked above each, of those listed
   uint32_t dcnt[256];
   u64 dmass[256];
   uint32_t wc[kDT / 64];
@@ -112,6 +166,56 @@ __device__ __forceinline__ void block_excl(uint32_t& c, u64& m, DrawLds& L) {
   __syncthreads();
 }
 
+// The tokens of bins lo .. hi (n of them, at most kList) into L.comp, sorted, and the masses ranked above them into
+// L.lmass; returns their mass.
+template <int TYPE>
+__device__ u64 sort_bins(const void* row, int V, const RowScale& rs, int lo, int hi, int n, DrawLds& L) {
+  const int tid = threadIdx.x;
+  if (tid == 0) L.nlist = 0;
+  __syncthreads();
+  each_token<TYPE>(row, V, [&](int i, float l) {
+    const int b = bin_of(rs, l);
+    if (b >= lo && b <= hi) {
+      const int p = atomicAdd(&L.nlist, 1);
+      if (p < kList) L.comp[p] = ((u64)order_key(l) << 24) | (uint32_t)i;
+    }
+  });
+  int n2 = 64;  // a power of two, filled up with what sorts last
+  while (n2 < n) n2 *= 2;
+  __syncthreads();
+  for (int i = n + tid; i < n2; i += kDT) L.comp[i] = ~0ull;
+  __syncthreads();
+  for (int k = 2; k <= n2; k *= 2)
+    for (int j = k / 2; j > 0; j /= 2) {  // bitonic; pairs within 64 entries stay in a wave
+      if (tid < n2 / 2) {
+        const int a = (tid / j) * 2 * j + tid % j, b = a + j;
+        const u64 x = L.comp[a], y = L.comp[b];
+        if ((x > y) == ((a & k) == 0)) {
+          L.comp[a] = y;
+          L.comp[b] = x;
+        }
+      }
+      __syncthreads();
+    }
+  u64 m[2];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int i = 2 * tid + q;
+    m[q] = i < n ? mass_of(e_of(rs, key_logit((uint32_t)(L.comp[i] >> 24)))) : 0;
+  }
+  uint32_t c = 0;
+  u64 s = m[0] + m[1];
+  const u64 own = s;
+  block_excl<kDT>(c, s, L);
+  if (2 * tid < n2) {
+    L.lmass[2 * tid] = s;
+    L.lmass[2 * tid + 1] = s + m[0];
+  }
+  if (tid == kDT - 1) L.rmass = s + own;
+  __syncthreads();
+  return L.rmass;
+}
+
 // A question to the ranking: by count (the last rank with fewer than n above it) or by mass (the last
 // rank with mass at most x above it). Rank 0 always qualifies.
 struct Ask {
@@ -125,15 +229,19 @@ struct Found {
   u64 above, mine;  // mass ranked above it, and its own
   uint32_t key, idx;
 };
+__device__ __forceinline__ Found found(uint32_t rank, u64 above, u64 comp, const RowScale& rs) {
+  const uint32_t key = (uint32_t)(comp >> 24);
+  return Found{rank, above, mass_of(e_of(rs, key_logit(key))), key, (uint32_t)(comp & 0xffffffu)};
+}
 
-template <int TYPE>
-__device__ Found search(const Ask q, const void* row, int V, const RowScale& rs, DrawLds& L) {
+// The last bin in use whose first token qualifies.
+__device__ __forceinline__ int last_bin(const Ask q, int V, DrawLds& L) {
   const int tid = threadIdx.x;
   if (tid == 0) L.found = 0;
   __syncthreads();
   int best = -1;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {  // bin 0 is never empty; a bin is empty where the next one's prefix is the same
+  for (int j = 0; j < 2; ++j) {  // a bin is empty where the next one's prefix is the same; bin 0 never is
     const int b = 2 * tid + j;
     const uint32_t next = b + 1 < kBins ? L.cnt[b + 1] : (uint32_t)V;
     if (next != L.cnt[b] && q.holds(L.cnt[b], L.mass[b])) best = b;
@@ -141,28 +249,29 @@ __device__ Found search(const Ask q, const void* row, int V, const RowScale& rs,
   if (best >= 0) atomicMax(&L.found, best);
   __syncthreads();
   const int bin = L.found;
+  __syncthreads();
+  return bin;
+}
+
+template <int TYPE>
+__device__ Found search(const Ask q, const void* row, int V, const RowScale& rs, DrawLds& L) {
+  const int tid = threadIdx.x;
+  const int bin = last_bin(q, V, L);
   uint32_t above = L.cnt[bin];
   u64 mass = L.mass[bin];
   const int n = (int)((bin + 1 < kBins ? L.cnt[bin + 1] : (uint32_t)V) - above);
-  const bool list = n <= kList;
-  if (list && L.listbin != bin) {  // (uniform)
-    __syncthreads();
-    if (tid == 0) {
-      L.nlist = 0;
-      L.listbin = bin;
+  if (n <= kList) {
+    if (L.listbin != bin) {  // (uniform)
+      sort_bins<TYPE>(row, V, rs, bin, bin, n, L);
+      if (tid == 0) L.listbin = bin;
     }
+    if (tid == 0) L.found = 0;
     __syncthreads();
-    for (int i = tid; i < V; i += kDT) {
-      const float l = clean(logit_at<TYPE>(row, i));
-      if (bin_of(rs, l) == bin) {
-        const int p = atomicAdd(&L.nlist, 1);
-        if (p < kList) {
-          L.comp[p] = ((u64)order_key(l) << 24) | (uint32_t)i;
-          L.lmass[p] = mass_of(e_of(rs, l));
-        }
-      }
-    }
+    for (int i = tid; i < n; i += kDT)
+      if (q.holds(above + i, mass + L.lmass[i])) atomicMax(&L.found, i);
     __syncthreads();
+    const int i = L.found;
+    return found(above + i, mass + L.lmass[i], L.comp[i], rs);
   }
   u64 prefix = 0;
   for (int sh = 48; sh >= 0; sh -= 8) {
@@ -172,25 +281,14 @@ __device__ Found search(const Ask q, const void* row, int V, const RowScale& rs,
     }
     if (tid == 0) L.found = -1;
     __syncthreads();
-    if (list) {
-      for (int i = tid; i < n; i += kDT) {
-        const u64 c = L.comp[i];
-        if ((c >> (sh + 8)) == prefix) {
-          atomicAdd(&L.dcnt[(c >> sh) & 255], 1u);
-          atomicAdd(&L.dmass[(c >> sh) & 255], L.lmass[i]);
-        }
+    each_token<TYPE>(row, V, [&](int i, float l) {
+      if (bin_of(rs, l) != bin) return;
+      const u64 c = ((u64)order_key(l) << 24) | (uint32_t)i;
+      if ((c >> (sh + 8)) == prefix) {
+        atomicAdd(&L.dcnt[(c >> sh) & 255], 1u);
+        atomicAdd(&L.dmass[(c >> sh) & 255], mass_of(e_of(rs, l)));
       }
-    } else {
-      for (int i = tid; i < V; i += kDT) {
-        const float l = clean(logit_at<TYPE>(row, i));
-        if (bin_of(rs, l) != bin) continue;
-        const u64 c = ((u64)order_key(l) << 24) | (uint32_t)i;
-        if ((c >> (sh + 8)) == prefix) {
-          atomicAdd(&L.dcnt[(c >> sh) & 255], 1u);
-          atomicAdd(&L.dmass[(c >> sh) & 255], mass_of(e_of(rs, l)));
-        }
-      }
-    }
+    });
     __syncthreads();
     const uint32_t c0 = tid < 256 ? L.dcnt[tid] : 0;
     uint32_t c = c0;
@@ -211,13 +309,7 @@ __device__ Found search(const Ask q, const void* row, int V, const RowScale& rs,
     mass = L.rmass;
     prefix = (prefix << 8) | (u64)d;
   }
-  Found f;
-  f.rank = above;
-  f.above = mass;
-  f.key = (uint32_t)(prefix >> 24);
-  f.idx = (uint32_t)(prefix & 0xffffffu);
-  f.mine = mass_of(e_of(rs, key_logit(f.key)));
-  return f;
+  return found(above, mass, prefix, rs);
 }
 
 template <int TYPE>
@@ -226,68 +318,62 @@ __global__ __launch_bounds__(kDT) void draw_row_kernel(DrawArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, b = blockIdx.x, V = a.V;
   const void* row = (const char*)a.logits + (size_t)b * a.ld * (TYPE == DFSSM_TYPE_F32 ? 4 : 2);
   const float T = a.temperatures ? a.temperatures[b] : a.temperature;
-  int k = a.top_ks ? a.top_ks[b] : a.top_k;
+  const int k = a.top_ks ? a.top_ks[b] : a.top_k;
   const float tp = a.top_ps ? a.top_ps[b] : a.top_p;
   const float mp = a.min_ps ? a.min_ps[b] : a.min_p;
   float u = a.u[b];
   u = u >= 0.0f ? (u < 1.0f ? u : 0.99999994f) : 0.0f;
 
-  // the largest logit, the lowest index that has it, and the least finite one
+  // the largest logit and the least finite one
   float m = -__builtin_inff(), lo = __builtin_inff();
-  int im = 0x7fffffff;
-  for (int i = tid; i < V; i += kDT) {
-    const float l = clean(logit_at<TYPE>(row, i));
-    if (l > m || (l == m && i < im)) {
-      m = l;
-      im = i;
-    }
-    if (l > -__builtin_inff()) lo = fminf(lo, l);
-  }
+  each_token<TYPE>(row, V, [&](int, float l) {
+    m = fmaxf(m, l);
+    lo = fminf(lo, l > -__builtin_inff() ? l : __builtin_inff());
+  });
   for (int i = tid; i < kBins; i += kDT) {
     L.cnt[i] = 0;
     L.mass[i] = 0;
   }
+  if (tid < 64) L.tab[tid] = exp2((double)tid * (1.0 / 64.0));
   for (int o = 32; o > 0; o >>= 1) {
-    const float om = __shfl_xor(m, o, 64);
-    const int oi = __shfl_xor(im, o, 64);
-    if (om > m || (om == m && oi < im)) {
-      m = om;
-      im = oi;
-    }
+    m = fmaxf(m, __shfl_xor(m, o, 64));
     lo = fminf(lo, __shfl_xor(lo, o, 64));
   }
   if (lane == 0) {
     L.wf[w] = m;
     L.wg[w] = lo;
-    L.wc[w] = (uint32_t)im;
+  }
+  if (tid == 0) {
+    L.listbin = -1;
+    L.found = 0x7fffffff;
+    L.rcnt = 0;
+    L.rmass = 0;
   }
   __syncthreads();
   m = L.wf[0];
   lo = L.wg[0];
-  im = (int)L.wc[0];
   for (int i = 1; i < kDT / 64; ++i) {
-    const float om = L.wf[i];
-    const int oi = (int)L.wc[i];
-    if (om > m || (om == m && oi < im)) {
-      m = om;
-      im = oi;
-    }
+    m = fmaxf(m, L.wf[i]);
     lo = fminf(lo, L.wg[i]);
   }
-  __syncthreads();
   if (m == -__builtin_inff() || !(T > 0.0f)) {  // nothing to draw from; greedy
+    const bool none = m == -__builtin_inff();
+    if (!none) each_token<TYPE>(row, V, [&](int i, float l) {
+      if (l == m) atomicMin(&L.found, i);
+    });
+    __syncthreads();
     if (tid == 0) {
-      const bool none = m == -__builtin_inff();
-      a.next[b] = none ? -1 : im;
+      a.next[b] = none ? -1 : L.found;
       if (a.logprob) a.logprob[b] = none ? -__builtin_inff() : 0.0f;
     }
     return;
   }
   RowScale rs;
   rs.m = m;
-  rs.it = 1.0 / (double)T;
+  rs.y1 = 64.0 * 1.4426950408889634074 / (double)T;
+  rs.tab = L.tab;
   {
-    const float span = m - lo;  // finite or +inf (m = +inf), never NaN: lo <= m, and both +inf give NaN
+    const float span = m - lo;  // finite or +inf (m = +inf); both +inf give NaN
     const float s = 64.0f / T;
     rs.s1 = s;
     rs.s2 = 1.0f;
@@ -298,44 +384,87 @@ __global__ __launch_bounds__(kDT) void draw_row_kernel(DrawArgs a) {
     }
   }
 
+  // What can be kept lies in the first bins if there is a top_k, or a min_p and no top_p (whose mass is that of all).
+  const bool by_k = k > 0 && k < V && k <= kList, by_m = !(k > 0 && k < V) && mp > 0.0f && mp <= 1.0f && !(tp < 1.0f);
+  bool counted = false;
+  if (by_k || by_m) {
+    each_token<TYPE>(row, V, [&](int, float l) { atomicAdd(&L.cnt[bin_of(rs, l)], 1u); });
+    __syncthreads();
+    const uint32_t c0 = L.cnt[2 * tid];
+    uint32_t c = c0 + L.cnt[2 * tid + 1];
+    u64 none = 0;
+    block_excl<kDT>(c, none, L);
+    L.cnt[2 * tid] = c;
+    L.cnt[2 * tid + 1] = c + c0;
+    __syncthreads();
+    counted = true;
+    int hi;
+    if (by_k) hi = last_bin(Ask{false, (uint32_t)k, 0.0}, V, L);
+    else hi = min(kBins - 1, bin_of(rs, m + T * __builtin_logf(mp)) + 1);  // (a bin more than the border's, which is rounded)
+    const int n = (int)(hi + 1 < kBins ? L.cnt[hi + 1] : (uint32_t)V);
+    if (n <= kList) {
+      const u64 total = sort_bins<TYPE>(row, V, rs, 0, hi, n, L);
+      const int nk = by_k ? min(k, n) : n;
+      const u64 Z = nk < n ? L.lmass[nk] : total;
+      if (tid == 0) L.found = 0;
+      __syncthreads();
+      for (int i = tid; i < nk; i += kDT) {
+        const double e = e_of(rs, key_logit((uint32_t)(L.comp[i] >> 24)));
+        if ((!(tp < 1.0f) || (double)L.lmass[i] <= (double)(tp > 0.0f ? tp : 0.0f) * (double)Z) && e >= (double)mp)
+          atomicMax(&L.found, i);
+      }
+      __syncthreads();
+      const int kept = L.found + 1;  // (ranks qualify up to a last one; rank 0 stays in any case)
+      const u64 S = kept < n ? L.lmass[kept] : total;
+      __syncthreads();
+      if (tid == 0) L.found = 0;
+      __syncthreads();
+      const double R = (double)u * (double)S;
+      for (int i = tid; i < kept; i += kDT)
+        if ((double)L.lmass[i] <= R) atomicMax(&L.found, i);
+      __syncthreads();
+      if (tid == 0) {
+        const u64 c = L.comp[L.found];
+        a.next[b] = (int64_t)(c & 0xffffffu);
+        if (a.logprob) a.logprob[b] = (float)log(e_of(rs, key_logit((uint32_t)(c >> 24))) * kOne / (double)S);
+      }
+      return;
+    }
+  }
+
   uint32_t nm = 0;
   u64 mm = 0;
-  for (int i = tid; i < V; i += kDT) {
-    const float l = clean(logit_at<TYPE>(row, i));
+  each_token<TYPE>(row, V, [&](int, float l) {
     const double e = e_of(rs, l);
     const u64 E = mass_of(e);
     const int bin = bin_of(rs, l);
-    atomicAdd(&L.cnt[bin], 1u);
+    if (!counted) atomicAdd(&L.cnt[bin], 1u);
     if (E) atomicAdd(&L.mass[bin], E);
     if (e >= (double)mp) {
       ++nm;
       mm += E;
     }
-  }
-  __syncthreads();
-  uint32_t c0 = L.cnt[2 * tid], c = c0 + L.cnt[2 * tid + 1];
-  u64 m0 = L.mass[2 * tid], ms = m0 + L.mass[2 * tid + 1];
-  block_excl<kDT>(c, ms, L);
-  L.cnt[2 * tid] = c;
-  L.cnt[2 * tid + 1] = c + c0;
-  L.mass[2 * tid] = ms;
-  L.mass[2 * tid + 1] = ms + m0;
-  u64 S = 0;  // the mass of the whole row
-  for (int i = 0; i < kDT / 64; ++i) S += L.wm[i];
-  if (tid == kDT - 1) L.listbin = -1;
-  // the tokens with e >= min_p
-  if (tid == 0) {
-    L.rcnt = 0;
-    L.rmass = 0;
-  }
-  __syncthreads();
-  if (nm) {
+  });
+  if (nm) {  // the tokens with e >= min_p
     atomicAdd(&L.rcnt, nm);
     atomicAdd(&L.rmass, mm);
   }
   __syncthreads();
   const uint32_t n_m = L.rcnt;
   const u64 M_m = L.rmass;
+  const uint32_t c0 = counted ? 0 : L.cnt[2 * tid];
+  uint32_t c = counted ? 0 : c0 + L.cnt[2 * tid + 1];
+  const u64 m0 = L.mass[2 * tid];
+  u64 ms = m0 + L.mass[2 * tid + 1];
+  block_excl<kDT>(c, ms, L);
+  if (!counted) {
+    L.cnt[2 * tid] = c;
+    L.cnt[2 * tid + 1] = c + c0;
+  }
+  L.mass[2 * tid] = ms;
+  L.mass[2 * tid + 1] = ms + m0;
+  u64 S = 0;  // the mass of the whole row
+  for (int i = 0; i < kDT / 64; ++i) S += L.wm[i];
   __syncthreads();
   uint32_t n = (uint32_t)V;
   if (k > 0 && k < V) {

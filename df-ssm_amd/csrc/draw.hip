@@ -28,7 +28,7 @@ namespace {
 constexpr int kDT = 1024;      // threads of a row's workgroup
 constexpr int kBins = 2048;
 constexpr int kFine = 1024;    // bins of 1/64 in (m - l) / T; the others share what lies below
-constexpr int kList = 2048;    // tokens that are sorted in LDS
+constexpr int kList = 2046;    // tokens that are sorted in LDS (and their masses, one more)
 constexpr double kOne = 17592186044416.0;  // 2^44
 
 typedef unsigned long long u64;
@@ -42,33 +42,36 @@ __device__ __forceinline__ float logit_at(const void* row, int i) {
 // A NaN ranks as -inf; -0 as +0 (they are equal, so their order is that of the indexes).
 __device__ __forceinline__ float clean(float l) { return l != l ? -__builtin_inff() : l + 0.0f; }
 
-// f(index, logit) for every token of the row, by all threads: 16 bytes a load between the row's aligned ends, four
-// loads under way.
+// f(index, logit) for every token of the row, by all threads: 16 bytes a load between the row's aligned ends, two
+// loads ahead.
 template <int TYPE, class F>
 __device__ __forceinline__ void each_token(const void* row, int V, F f) {
   constexpr int ES = TYPE == DFSSM_TYPE_F32 ? 4 : 2, N = 16 / ES;
   const int tid = threadIdx.x;
   const int head = min(V, (int)((16 - ((uintptr_t)row & 15)) & 15) / ES), nb = (V - head) / N, tail = head + nb * N;
-  if (tid < head) f(tid, clean(logit_at<TYPE>(row, tid)));
-  if (tail + tid < V) f(tail + tid, clean(logit_at<TYPE>(row, tail + tid)));
+  if (tid < head) f(tid, logit_at<TYPE>(row, tid));
+  if (tail + tid < V) f(tail + tid, logit_at<TYPE>(row, tail + tid));
   const u32x4* p = (const u32x4*)((const char*)row + head * ES);
-  for (int c = tid; c < nb; c += 4 * kDT) {
-    u32x4 x[4];
+  auto piece = [&](const u32x4 x, int c) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) x[q] = p[min(c + q * kDT, nb - 1)];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int b = c + q * kDT;
-      if (b >= nb) break;
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const uint32_t word = x[q][e * ES / 4];  // (a copy: a bit_cast of a vector's element takes the first one)
-        float l;
-        if constexpr (TYPE == DFSSM_TYPE_F32) l = __builtin_bit_cast(float, word);
-        else if constexpr (TYPE == DFSSM_TYPE_BF16) l = __builtin_bit_cast(float, (e & 1) ? word & 0xffff0000u : word << 16);
-        else l = h2f((uint16_t)(word >> (16 * (e & 1))));
-        f(head + b * N + e, clean(l));
-      }
+    for (int e = 0; e < N; ++e) {
+      const uint32_t word = x[e * ES / 4];  // (a copy: a bit_cast of a vector's element takes the first one)
+      float l;
+      if constexpr (TYPE == DFSSM_TYPE_F32) l = __builtin_bit_cast(float, word);
+      else if constexpr (TYPE == DFSSM_TYPE_BF16) l = __builtin_bit_cast(float, (e & 1) ? word & 0xffff0000u : word << 16);
+      else l = h2f((uint16_t)(word >> (16 * (e & 1))));
+      f(head + c * N + e, l);
+    }
+  };
+  // (the loop is not unrolled: a body is passed over a few times only, and its fetching from memory would cost more)
+  if (nb > 0) {
+    u32x4 x0 = p[min(tid, nb - 1)], x1 = p[min(tid + kDT, nb - 1)];
+#pragma unroll 1
+    for (int c = tid; c < nb; c += kDT) {
+      const u32x4 x2 = p[min(c + 2 * kDT, nb - 1)];
+      piece(x0, c);
+      x0 = x1;
+      x1 = x2;
     }
   }
 }
@@ -84,30 +87,37 @@ __device__ __forceinline__ float key_logit(uint32_t k) {
 
 struct RowScale {
   float m, s1, s2;   // bins: x = (m - l) s1 below kFine, then kFine + (x - kFine) s2
+  bool top;          // the largest logit is +inf: such tokens count as logit 0 and the others as -inf
   double y1;         // 64 log2(e) / T: e = 2^((l - m) y1 / 64)
   const double* tab; // 2^(j / 64), j = 0 .. 63
 };
-__device__ __forceinline__ int bin_of(const RowScale& r, float l) {
-  if (l == r.m) return 0;  // (also where both are +inf)
-  const float x = (r.m - l) * r.s1;
-  if (x < (float)kFine) return (int)x;
-  const float y = (x - (float)kFine) * r.s2;
-  return kFine + (y < (float)(kBins - kFine - 1) ? (int)y : kBins - kFine - 1);
+// A token's logit as it is ranked: -inf takes no part (nor does a NaN).
+__device__ __forceinline__ float ranked(const RowScale r, float l) {
+  l = clean(l);
+  if (r.top) l = l == __builtin_inff() ? 0.0f : -__builtin_inff();  // (uniform)
+  return l;
 }
-// exp((l - m) / T) = 2^(n / 64) e^x, n whole, |x| <= ln 2 / 128: a table and a Taylor polynomial of degree 5, whose
-// rest is below 2^-54. (exp() takes four times as many instructions, and this is most of the work.)
-__device__ __forceinline__ double e_of(const RowScale& r, float l) {
+__device__ __forceinline__ bool taken(float l) { return l > -__builtin_inff(); }
+// The bin of a token that takes part, 0 <= x (not NaN: T > 0, so s1 is at most +inf and m - l = 0 gives bin 0).
+__device__ __forceinline__ int bin_of(const RowScale r, float l) {
+  const float d = r.m - l, x = d > 0.0f ? d * r.s1 : 0.0f;
+  const float y = (x - (float)kFine) * r.s2;
+  const int low = kFine + (y < (float)(kBins - kFine - 1) ? (int)y : kBins - kFine - 1);
+  return x < (float)kFine ? (int)x : low;
+}
+// exp((l - m) / T) = 2^(n / 64) 2^(t / 64), n whole, |t| <= 1/2: a table and the Taylor polynomial of degree 5 of the
+// second factor, whose rest is below 2^-54. (exp() takes four times as many instructions, and this is most of the
+// work.) What underflows comes out as 0.
+__device__ __forceinline__ double e_of(const RowScale r, float l) {
+  constexpr double c = 0.693147180559945309417 / 64.0;
   const double y = ((double)l - (double)r.m) * r.y1;
-  if (l == r.m) return 1.0;
-  if (!(y > -64.0 * 1020.0)) return 0.0;
-  const double n = __builtin_rint(y);
-  const double x = (y - n) * (0.693147180559945309417 / 64.0);
-  double p = 1.0 / 120.0;
-  p = __builtin_fma(p, x, 1.0 / 24.0);
-  p = __builtin_fma(p, x, 1.0 / 6.0);
-  p = __builtin_fma(p, x, 0.5);
-  p = __builtin_fma(p, x, 1.0);
-  p = __builtin_fma(p, x, 1.0);
+  const double n = __builtin_rint(y), t = y - n;
+  double p = c * c * c * c * c / 120.0;
+  p = __builtin_fma(p, t, c * c * c * c / 24.0);
+  p = __builtin_fma(p, t, c * c * c / 6.0);
+  p = __builtin_fma(p, t, c * c / 2.0);
+  p = __builtin_fma(p, t, c);
+  p = __builtin_fma(p, t, 1.0);
   const int i = (int)n;
   return __builtin_amdgcn_ldexp(r.tab[i & 63] * p, i >> 6);
 }
@@ -118,16 +128,17 @@ __device__ __forceinline__ u64 mass_of(double e) {
 
 struct DrawLds {
   double tab[64];
-  uint32_t cnt[kBins];   // per bin, then tokens in earlier bins
-  u64 mass[kBins];       // the same for masses
-  u64 comp[kList];       // (order key << 24) | index of the listed tokens, sorted
-  u64 lmass[kList];      // mass ranked above each, of those listed
+  uint32_t cnt[kBins + 2];  // per bin, then tokens in earlier bins
+  u64 mass[kBins + 2];      // the same for masses
+  u64 comp[kList + 2];   // (order key << 24) | index of the listed tokens, sorted
+  u64 lmass[kList + 2];  // mass ranked above each, of those listed; at the end that of all
+  int rank[kDT / 2];
   uint32_t dcnt[256];
   u64 dmass[256];
   uint32_t wc[kDT / 64];
   u64 wm[kDT / 64];
   float wf[kDT / 64], wg[kDT / 64];
-  int found, nlist, listbin;
+  int found, nlist;
   uint32_t rcnt;
   u64 rmass;
 };
@@ -166,37 +177,62 @@ __device__ __forceinline__ void block_excl(uint32_t& c, u64& m, DrawLds& L) {
   __syncthreads();
 }
 
-// The tokens of bins lo .. hi (n of them, at most kList) into L.comp, sorted, and the masses ranked above them into
-// L.lmass; returns their mass.
+// The tokens of bins lo .. hi and of bin far > hi (or -1) into L.comp, sorted, and the masses ranked above them
+// within the list into L.lmass. Returns how many they are; more than kList: nothing is listed.
 template <int TYPE>
-__device__ u64 sort_bins(const void* row, int V, const RowScale& rs, int lo, int hi, int n, DrawLds& L) {
+__device__ __forceinline__ int sort_bins(const void* row, int V, const RowScale rs, int lo, int hi, int far, DrawLds& L) {
   const int tid = threadIdx.x;
   if (tid == 0) L.nlist = 0;
   __syncthreads();
-  each_token<TYPE>(row, V, [&](int i, float l) {
+  each_token<TYPE>(row, V, [&](int i, float raw) {
+    const float l = ranked(rs, raw);
     const int b = bin_of(rs, l);
-    if (b >= lo && b <= hi) {
+    if (taken(l) && ((b >= lo && b <= hi) || b == far)) {
       const int p = atomicAdd(&L.nlist, 1);
       if (p < kList) L.comp[p] = ((u64)order_key(l) << 24) | (uint32_t)i;
     }
   });
-  int n2 = 64;  // a power of two, filled up with what sorts last
-  while (n2 < n) n2 *= 2;
   __syncthreads();
-  for (int i = n + tid; i < n2; i += kDT) L.comp[i] = ~0ull;
-  __syncthreads();
-  for (int k = 2; k <= n2; k *= 2)
-    for (int j = k / 2; j > 0; j /= 2) {  // bitonic; pairs within 64 entries stay in a wave
-      if (tid < n2 / 2) {
-        const int a = (tid / j) * 2 * j + tid % j, b = a + j;
-        const u64 x = L.comp[a], y = L.comp[b];
-        if ((x > y) == ((a & k) == 0)) {
-          L.comp[a] = y;
-          L.comp[b] = x;
-        }
-      }
-      __syncthreads();
+  const int n = L.nlist;
+  if (n > kList) return n;
+  if (n <= kDT / 2) {
+    // A token's rank is the number of smaller entries: kDT / n threads count for each, over parts of the list. (No
+    // barriers between, as the stages of a sorting network have; its work grows with the square.)
+    int parts = kDT / max(n, 1);
+    parts = parts > 16 ? 16 : parts;
+    const int i = tid % max(n, 1), part = tid / max(n, 1);
+    for (int q = tid; q < n; q += kDT) L.rank[q] = 0;
+    __syncthreads();
+    u64 own = 0;
+    if (n && part < parts) {
+      own = L.comp[i];
+      const int per = (n + parts - 1) / parts, from = part * per, to = min(n, from + per);
+      int r = 0;
+      for (int q = from; q < to; ++q) r += L.comp[q] < own ? 1 : 0;
+      if (r) atomicAdd(&L.rank[i], r);
     }
+    __syncthreads();
+    const int at = tid < n ? L.rank[tid] : 0;  // (thread tid < n has entry tid)
+    if (tid < n) L.comp[at] = own;
+    __syncthreads();
+  } else {
+    int n2 = kDT;  // a power of two, filled up with what sorts last
+    while (n2 < n) n2 *= 2;
+    for (int i = n + tid; i < n2; i += kDT) L.comp[i] = ~0ull;
+    __syncthreads();
+    for (int k = 2; k <= n2; k *= 2)
+      for (int j = k / 2; j > 0; j /= 2) {  // bitonic
+        if (tid < n2 / 2) {
+          const int a = (tid / j) * 2 * j + tid % j, b = a + j;
+          const u64 x = L.comp[a], y = L.comp[b];
+          if ((x > y) == ((a & k) == 0)) {
+            L.comp[a] = y;
+            L.comp[b] = x;
+          }
+        }
+        __syncthreads();
+      }
+  }
   u64 m[2];
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
@@ -205,15 +241,13 @@ __device__ u64 sort_bins(const void* row, int V, const RowScale& rs, int lo, int
   }
   uint32_t c = 0;
   u64 s = m[0] + m[1];
-  const u64 own = s;
   block_excl<kDT>(c, s, L);
-  if (2 * tid < n2) {
+  if (2 * tid <= n) {  // (one entry more: the list's mass)
     L.lmass[2 * tid] = s;
     L.lmass[2 * tid + 1] = s + m[0];
   }
-  if (tid == kDT - 1) L.rmass = s + own;
   __syncthreads();
-  return L.rmass;
+  return n;
 }
 
 // A question to the ranking: by count (the last rank with fewer than n above it) or by mass (the last
@@ -225,17 +259,17 @@ struct Ask {
   __device__ __forceinline__ bool holds(uint32_t above, u64 mass) const { return by_mass ? (double)mass <= x : above < n; }
 };
 struct Found {
-  uint32_t rank;
   u64 above, mine;  // mass ranked above it, and its own
   uint32_t key, idx;
 };
-__device__ __forceinline__ Found found(uint32_t rank, u64 above, u64 comp, const RowScale& rs) {
+__device__ __forceinline__ Found found(u64 above, u64 comp, const RowScale rs) {
   const uint32_t key = (uint32_t)(comp >> 24);
-  return Found{rank, above, mass_of(e_of(rs, key_logit(key))), key, (uint32_t)(comp & 0xffffffu)};
+  return Found{above, mass_of(e_of(rs, key_logit(key))), key, (uint32_t)(comp & 0xffffffu)};
 }
 
-// The last bin in use whose first token qualifies.
-__device__ __forceinline__ int last_bin(const Ask q, int V, DrawLds& L) {
+// The last bin in use whose first token qualifies. By mass, a bin without mass is not in use: what lies there
+// comes after all that a mass can ask for.
+__device__ __forceinline__ int last_bin(const Ask q, DrawLds& L) {
   const int tid = threadIdx.x;
   if (tid == 0) L.found = 0;
   __syncthreads();
@@ -243,8 +277,8 @@ __device__ __forceinline__ int last_bin(const Ask q, int V, DrawLds& L) {
 #pragma unroll
   for (int j = 0; j < 2; ++j) {  // a bin is empty where the next one's prefix is the same; bin 0 never is
     const int b = 2 * tid + j;
-    const uint32_t next = b + 1 < kBins ? L.cnt[b + 1] : (uint32_t)V;
-    if (next != L.cnt[b] && q.holds(L.cnt[b], L.mass[b])) best = b;
+    const bool used = q.by_mass ? L.mass[b + 1] != L.mass[b] : L.cnt[b + 1] != L.cnt[b];
+    if (used && (q.by_mass ? q.holds(0, L.mass[b]) : q.holds(L.cnt[b], 0))) best = b;
   }
   if (best >= 0) atomicMax(&L.found, best);
   __syncthreads();
@@ -252,27 +286,26 @@ __device__ __forceinline__ int last_bin(const Ask q, int V, DrawLds& L) {
   __syncthreads();
   return bin;
 }
-
-template <int TYPE>
-__device__ Found search(const Ask q, const void* row, int V, const RowScale& rs, DrawLds& L) {
+// The last of entries [from, to) of the list that qualifies; its masses are off by `base` (and its counts by above).
+__device__ __forceinline__ int last_entry(const Ask q, int from, int to, uint32_t above, u64 base, DrawLds& L) {
   const int tid = threadIdx.x;
-  const int bin = last_bin(q, V, L);
-  uint32_t above = L.cnt[bin];
+  if (tid == 0) L.found = from;
+  __syncthreads();
+  for (int i = from + tid; i < to; i += kDT)
+    if (q.holds(above + (uint32_t)(i - from), base + L.lmass[i])) atomicMax(&L.found, i);
+  __syncthreads();
+  const int i = L.found;
+  __syncthreads();
+  return i;
+}
+
+// One question resolved by the exact order key and the index, a byte at a time over the row (more tokens in the bin
+// than the list takes).
+template <int TYPE>
+__device__ __forceinline__ Found search_row(const Ask q, int bin, const void* row, int V, const RowScale rs, DrawLds& L) {
+  const int tid = threadIdx.x;
+  uint32_t above = q.by_mass ? 0 : L.cnt[bin];
   u64 mass = L.mass[bin];
-  const int n = (int)((bin + 1 < kBins ? L.cnt[bin + 1] : (uint32_t)V) - above);
-  if (n <= kList) {
-    if (L.listbin != bin) {  // (uniform)
-      sort_bins<TYPE>(row, V, rs, bin, bin, n, L);
-      if (tid == 0) L.listbin = bin;
-    }
-    if (tid == 0) L.found = 0;
-    __syncthreads();
-    for (int i = tid; i < n; i += kDT)
-      if (q.holds(above + i, mass + L.lmass[i])) atomicMax(&L.found, i);
-    __syncthreads();
-    const int i = L.found;
-    return found(above + i, mass + L.lmass[i], L.comp[i], rs);
-  }
   u64 prefix = 0;
   for (int sh = 48; sh >= 0; sh -= 8) {
     if (tid < 256) {
@@ -281,8 +314,9 @@ __device__ Found search(const Ask q, const void* row, int V, const RowScale& rs,
     }
     if (tid == 0) L.found = -1;
     __syncthreads();
-    each_token<TYPE>(row, V, [&](int i, float l) {
-      if (bin_of(rs, l) != bin) return;
+    each_token<TYPE>(row, V, [&](int i, float raw) {
+      const float l = ranked(rs, raw);
+      if (!taken(l) || bin_of(rs, l) != bin) return;
       const u64 c = ((u64)order_key(l) << 24) | (uint32_t)i;
       if ((c >> (sh + 8)) == prefix) {
         atomicAdd(&L.dcnt[(c >> sh) & 255], 1u);
@@ -291,13 +325,15 @@ __device__ Found search(const Ask q, const void* row, int V, const RowScale& rs,
     });
     __syncthreads();
     const uint32_t c0 = tid < 256 ? L.dcnt[tid] : 0;
+    const u64 m0 = tid < 256 ? L.dmass[tid] : 0;
     uint32_t c = c0;
-    u64 m = tid < 256 ? L.dmass[tid] : 0;
+    u64 m = m0;
     block_excl<256>(c, m, L);
     c += above;
     m += mass;
-    // the first digit in use qualifies always: its prefix was found to
-    if (tid < 256 && c0 && (q.holds(c, m) || c == above)) atomicMax(&L.found, tid);
+    // the first digit in use qualifies always: its prefix was found to (by mass, the first with any)
+    const bool first = q.by_mass ? m == mass : c == above;
+    if (tid < 256 && (q.by_mass ? m0 != 0 : c0 != 0) && (q.holds(c, m) || first)) atomicMax(&L.found, tid);
     __syncthreads();
     const int d = L.found;
     if (tid == d) {
@@ -309,7 +345,23 @@ __device__ Found search(const Ask q, const void* row, int V, const RowScale& rs,
     mass = L.rmass;
     prefix = (prefix << 8) | (u64)d;
   }
-  return found(above, mass, prefix, rs);
+  return found(mass, prefix, rs);
+}
+template <int TYPE>
+__device__ __forceinline__ Found search(const Ask q, const void* row, int V, const RowScale rs, DrawLds& L) {
+  const int bin = last_bin(q, L);
+  const int n = sort_bins<TYPE>(row, V, rs, bin, bin, -1, L);
+  if (n > kList) return search_row<TYPE>(q, bin, row, V, rs, L);
+  const int i = last_entry(q, 0, n, q.by_mass ? 0 : L.cnt[bin], L.mass[bin], L);
+  return found(L.mass[bin] + L.lmass[i], L.comp[i], rs);
+}
+
+__device__ __forceinline__ u64 wave_add64(u64 v) {
+  for (int o = 32; o > 0; o >>= 1) {
+    const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)v, o, 64), hi = (uint32_t)__shfl_xor((int)(uint32_t)(v >> 32), o, 64);
+    v += ((u64)hi << 32) | lo;
+  }
+  return v;
 }
 
 template <int TYPE>
@@ -324,11 +376,12 @@ __global__ __launch_bounds__(kDT) void draw_row_kernel(DrawArgs a) {
   float u = a.u[b];
   u = u >= 0.0f ? (u < 1.0f ? u : 0.99999994f) : 0.0f;
 
-  // the largest logit and the least finite one
+  // the largest logit, and nearly the least finite one (of every eighth: only the bins' width comes from it)
   float m = -__builtin_inff(), lo = __builtin_inff();
-  each_token<TYPE>(row, V, [&](int, float l) {
-    m = fmaxf(m, l);
-    lo = fminf(lo, l > -__builtin_inff() ? l : __builtin_inff());
+  each_token<TYPE>(row, V, [&](int i, float raw) {
+    const float l = clean(raw);
+    m = l > m ? l : m;
+    if ((i & 7) == 0 && l < lo && taken(l)) lo = l;
   });
   for (int i = tid; i < kBins; i += kDT) {
     L.cnt[i] = 0;
@@ -344,10 +397,11 @@ __global__ __launch_bounds__(kDT) void draw_row_kernel(DrawArgs a) {
     L.wg[w] = lo;
   }
   if (tid == 0) {
-    L.listbin = -1;
     L.found = 0x7fffffff;
     L.rcnt = 0;
     L.rmass = 0;
+    L.cnt[kBins] = 0;
+    L.mass[kBins] = 0;
   }
   __syncthreads();
   m = L.wf[0];
@@ -358,8 +412,8 @@ __global__ __launch_bounds__(kDT) void draw_row_kernel(DrawArgs a) {
   }
   if (m == -__builtin_inff() || !(T > 0.0f)) {  // nothing to draw from; greedy
     const bool none = m == -__builtin_inff();
-    if (!none) each_token<TYPE>(row, V, [&](int i, float l) {
-      if (l == m) atomicMin(&L.found, i);
+    if (!none) each_token<TYPE>(row, V, [&](int i, float raw) {
+      if (clean(raw) == m) atomicMin(&L.found, i);
     });
     __syncthreads();
     if (tid == 0) {
@@ -369,43 +423,48 @@ __global__ __launch_bounds__(kDT) void draw_row_kernel(DrawArgs a) {
     return;
   }
   RowScale rs;
-  rs.m = m;
+  rs.top = m == __builtin_inff();
+  rs.m = rs.top ? 0.0f : m;
   rs.y1 = 64.0 * 1.4426950408889634074 / (double)T;
   rs.tab = L.tab;
-  {
-    const float span = m - lo;  // finite or +inf (m = +inf); both +inf give NaN
-    const float s = 64.0f / T;
-    rs.s1 = s;
-    rs.s2 = 1.0f;
-    if (span > 0.0f && span < __builtin_inff()) {
-      const float x = span * s;
-      if (!(x >= (float)kFine)) rs.s1 = (float)(kFine - 1) / span;  // a narrow row spreads over the fine bins
-      else if (x > (float)kBins) rs.s2 = (float)(kBins - kFine - 1) / (x - (float)kFine);
-    }
+  rs.s1 = 64.0f / T;
+  rs.s2 = 1.0f;
+  if (!rs.top && lo < m) {
+    const float span = m - lo, x = span * rs.s1;
+    if (!(x >= (float)kFine)) rs.s1 = (float)(kFine - 1) / span;  // a narrow row spreads over the fine bins
+    else if (x > (float)kBins) rs.s2 = (float)(kBins - kFine - 1) / (x - (float)kFine);
   }
 
+  const bool limit = k > 0 && k < V;
   // What can be kept lies in the first bins if there is a top_k, or a min_p and no top_p (whose mass is that of all).
-  const bool by_k = k > 0 && k < V && k <= kList, by_m = !(k > 0 && k < V) && mp > 0.0f && mp <= 1.0f && !(tp < 1.0f);
-  bool counted = false;
-  if (by_k || by_m) {
-    each_token<TYPE>(row, V, [&](int, float l) { atomicAdd(&L.cnt[bin_of(rs, l)], 1u); });
+  const bool by_k = limit && k <= kList, by_m = !limit && mp > 0.0f && mp <= 1.0f && !(tp < 1.0f) && T <= 1024.0f;
+  if (limit || by_m) {
+    each_token<TYPE>(row, V, [&](int, float raw) {
+      const float l = ranked(rs, raw);
+      if (taken(l)) atomicAdd(&L.cnt[bin_of(rs, l)], 1u);
+    });
     __syncthreads();
-    const uint32_t c0 = L.cnt[2 * tid];
-    uint32_t c = c0 + L.cnt[2 * tid + 1];
+    const uint32_t c0 = L.cnt[2 * tid], c1 = L.cnt[2 * tid + 1];
+    uint32_t c = c0 + c1;
     u64 none = 0;
     block_excl<kDT>(c, none, L);
     L.cnt[2 * tid] = c;
     L.cnt[2 * tid + 1] = c + c0;
+    if (tid == kDT - 1) L.cnt[kBins] = c + c0 + c1;
     __syncthreads();
-    counted = true;
+  }
+  if (by_k || by_m) {
     int hi;
-    if (by_k) hi = last_bin(Ask{false, (uint32_t)k, 0.0}, V, L);
-    else hi = min(kBins - 1, bin_of(rs, m + T * __builtin_logf(mp)) + 1);  // (a bin more than the border's, which is rounded)
-    const int n = (int)(hi + 1 < kBins ? L.cnt[hi + 1] : (uint32_t)V);
+    if (by_k) hi = last_bin(Ask{false, (uint32_t)k, 0.0}, L);
+    else hi = min(kBins - 1, bin_of(rs, rs.m + T * __builtin_logf(mp)) + 1);  // (one more: the border is rounded)
+    int n = kList + 1;
+    if (L.cnt[hi + 1] <= kList) n = sort_bins<TYPE>(row, V, rs, 0, hi, -1, L);
+    // (should the border be further off than the bins tell, the last token listed passes it)
+    if (by_m && n <= kList && n < (int)L.cnt[kBins] && e_of(rs, key_logit((uint32_t)(L.comp[n - 1] >> 24))) >= (double)mp)
+      n = kList + 1;
     if (n <= kList) {
-      const u64 total = sort_bins<TYPE>(row, V, rs, 0, hi, n, L);
       const int nk = by_k ? min(k, n) : n;
-      const u64 Z = nk < n ? L.lmass[nk] : total;
+      const u64 Z = L.lmass[nk];
       if (tid == 0) L.found = 0;
       __syncthreads();
       for (int i = tid; i < nk; i += kDT) {
@@ -415,16 +474,11 @@ __global__ __launch_bounds__(kDT) void draw_row_kernel(DrawArgs a) {
       }
       __syncthreads();
       const int kept = L.found + 1;  // (ranks qualify up to a last one; rank 0 stays in any case)
-      const u64 S = kept < n ? L.lmass[kept] : total;
+      const u64 S = L.lmass[kept];
       __syncthreads();
-      if (tid == 0) L.found = 0;
-      __syncthreads();
-      const double R = (double)u * (double)S;
-      for (int i = tid; i < kept; i += kDT)
-        if ((double)L.lmass[i] <= R) atomicMax(&L.found, i);
-      __syncthreads();
+      const int i = last_entry(Ask{true, 0u, (double)u * (double)S}, 0, kept, 0, 0, L);
       if (tid == 0) {
-        const u64 c = L.comp[L.found];
+        const u64 c = L.comp[i];
         a.next[b] = (int64_t)(c & 0xffffffu);
         if (a.logprob) a.logprob[b] = (float)log(e_of(rs, key_logit((uint32_t)(c >> 24))) * kOne / (double)S);
       }
@@ -432,58 +486,76 @@ __global__ __launch_bounds__(kDT) void draw_row_kernel(DrawArgs a) {
     }
   }
 
-  uint32_t nm = 0;
-  u64 mm = 0;
-  each_token<TYPE>(row, V, [&](int, float l) {
+  u64 mm = 0;  // the mass of the tokens with e >= min_p
+  each_token<TYPE>(row, V, [&](int, float raw) {
+    const float l = ranked(rs, raw);
+    if (!taken(l)) return;
     const double e = e_of(rs, l);
     const u64 E = mass_of(e);
-    const int bin = bin_of(rs, l);
-    if (!counted) atomicAdd(&L.cnt[bin], 1u);
-    if (E) atomicAdd(&L.mass[bin], E);
-    if (e >= (double)mp) {
-      ++nm;
-      mm += E;
-    }
+    if (E) atomicAdd(&L.mass[bin_of(rs, l)], E);
+    if (e >= (double)mp) mm += E;
   });
-  if (nm) {  // the tokens with e >= min_p
-    atomicAdd(&L.rcnt, nm);
-    atomicAdd(&L.rmass, mm);
-  }
+  mm = wave_add64(mm);
+  if (lane == 0) atomicAdd(&L.rmass, mm);
   __syncthreads();
-  const uint32_t n_m = L.rcnt;
-  const u64 M_m = L.rmass;
-  const uint32_t c0 = counted ? 0 : L.cnt[2 * tid];
-  uint32_t c = counted ? 0 : c0 + L.cnt[2 * tid + 1];
-  const u64 m0 = L.mass[2 * tid];
-  u64 ms = m0 + L.mass[2 * tid + 1];
+  // (rank 0, whose mass is 1, is kept in any case)
+  const u64 M_m = L.rmass > mass_of(1.0) ? L.rmass : mass_of(1.0);
+  const u64 m0 = L.mass[2 * tid], m1 = L.mass[2 * tid + 1];
+  uint32_t c = 0;
+  u64 ms = m0 + m1;
   block_excl<kDT>(c, ms, L);
-  if (!counted) {
-    L.cnt[2 * tid] = c;
-    L.cnt[2 * tid + 1] = c + c0;
-  }
   L.mass[2 * tid] = ms;
   L.mass[2 * tid + 1] = ms + m0;
-  u64 S = 0;  // the mass of the whole row
-  for (int i = 0; i < kDT / 64; ++i) S += L.wm[i];
+  if (tid == kDT - 1) L.mass[kBins] = ms + m0 + m1;
   __syncthreads();
-  uint32_t n = (uint32_t)V;
-  if (k > 0 && k < V) {
+  u64 S = L.mass[kBins];  // of what is kept: the shortest of three prefixes has the least
+  if (limit) {
     const Found f = search<TYPE>(Ask{false, (uint32_t)k, 0.0}, row, V, rs, L);
-    n = f.rank + 1;
     S = f.above + f.mine;
   }
+  const double share = (double)(tp > 0.0f ? tp : 0.0f) * (double)S;
+  Found f;
+  bool done = false;
   if (tp < 1.0f) {
-    const Found f = search<TYPE>(Ask{true, 0u, (double)(tp > 0.0f ? tp : 0.0f) * (double)S}, row, V, rs, L);
-    if (f.rank + 1 < n) {
-      n = f.rank + 1;
-      S = f.above + f.mine;
+    // top_p's border and the draw from one list: the border lies in one bin, which bounds the kept mass, and so the
+    // bins that the drawn token may lie in.
+    const Ask border{true, 0u, share};
+    const int far = last_bin(border, L);
+    const u64 most = S < M_m ? S : M_m;
+    const u64 s0 = max(min(most, L.mass[far]), (u64)1), s1 = min(most, L.mass[far + 1]);
+    const int d0 = last_bin(Ask{true, 0u, (double)u * (double)s0}, L), d1 = last_bin(Ask{true, 0u, (double)u * (double)s1}, L);
+    const int n = sort_bins<TYPE>(row, V, rs, d0, d1, far > d1 ? far : -1, L);
+    if (n <= kList) {
+      // entries before `split` are of d0 .. d1; those of far follow, their masses counted from far's own start
+      int split = n;
+      if (far > d1) {
+        if (tid == 0) L.found = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += kDT)
+          if (bin_of(rs, key_logit((uint32_t)(L.comp[i] >> 24))) <= d1) atomicMax(&L.found, i + 1);
+        __syncthreads();
+        split = L.found;
+        __syncthreads();
+        const u64 near = L.mass[d1 + 1] - L.mass[d0];
+        const int p = last_entry(border, split, n, 0, L.mass[far] - near, L);
+        S = min(S, L.mass[far] - near + L.lmass[p + 1]);
+      } else {
+        const int p = last_entry(border, 0, n, 0, L.mass[d0], L);
+        S = min(S, L.mass[d0] + L.lmass[p + 1]);
+      }
+      S = min(S, M_m);
+      const int i = last_entry(Ask{true, 0u, (double)u * (double)S}, 0, split, 0, L.mass[d0], L);
+      f = found(L.mass[d0] + L.lmass[i], L.comp[i], rs);
+      done = true;
+    } else {
+      const Found p = search<TYPE>(border, row, V, rs, L);
+      S = min(S, p.above + p.mine);
     }
   }
-  if (n_m < n) {
-    n = n_m > 1 ? n_m : 1;
-    S = n > 1 ? M_m : mass_of(1.0);
+  if (!done) {
+    S = min(S, M_m);
+    f = search<TYPE>(Ask{true, 0u, (double)u * (double)S}, row, V, rs, L);
   }
-  const Found f = search<TYPE>(Ask{true, 0u, (double)u * (double)S}, row, V, rs, L);
   if (tid == 0) {
     a.next[b] = (int64_t)f.idx;
     if (a.logprob) a.logprob[b] = (float)log(e_of(rs, key_logit(f.key)) * kOne / (double)S);

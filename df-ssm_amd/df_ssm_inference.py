@@ -16,11 +16,14 @@ a fused greedy argmax, and a whole decode step (embedding, all layers, head) is 
 Compatible extensions: generate(n_tokens, prompt=None, return_tokens=False, verbose=True) ingests
 a (batch, T) prompt step by step and does not leave warm-up state behind (the reference's warm-up
 forward advances the state, df_ssm_inference.py:230; the CPU driver resets after it,
-cpu_inference_driver.py:191-192).
+cpu_inference_driver.py:191-192). With a temperature it draws its tokens (top_p, repetition_penalty, or top_k
+and min_p, seed).
 """
 from __future__ import annotations
 
 import ctypes
+import math
+import operator
 import os
 import sys
 import time
@@ -31,7 +34,7 @@ import torch
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 
-from dfssm import _C  # noqa: E402
+from dfssm import _C, ops  # noqa: E402
 from dfssm.format import DFSSMWeights, EMB_I8, LORA_RANK, read_dfssm  # noqa: E402
 
 
@@ -164,6 +167,23 @@ def _check_token_range(t: torch.Tensor, vocab: int) -> None:
     lo, hi = int(t.min()), int(t.max())
     if lo < 0 or hi >= vocab:
         raise IndexError(f"token id out of range [0, {vocab}): min {lo}, max {hi}")
+
+
+def _draw_filters(temperature, top_k, top_p, min_p, penalty, state_df=None) -> bool:
+    """Whether generate()'s arguments ask for the draw with top_k or min_p; ValueError for what it does not do."""
+    if not 0 <= operator.index(top_k) < 2**31:
+        raise ValueError(f"top_k must be an int32 of at least 0, got {top_k}")
+    if not 0.0 <= min_p <= 1.0:
+        raise ValueError(f"min_p must lie in [0, 1], got {min_p}")
+    if top_k == 0 and min_p == 0:
+        return False
+    if temperature is None or state_df is not None:
+        raise ValueError("top_k and min_p filter a draw: they need a temperature, and no state_df")
+    if not 0.0 < temperature < math.inf or not top_p >= 0.0:
+        raise ValueError(f"temperature must be finite and > 0 and top_p >= 0, got {temperature} and {top_p}")
+    if penalty != 1.0:
+        raise ValueError("repetition_penalty is not supported together with top_k or min_p")
+    return True
 
 
 class StateDensityField:
@@ -583,8 +603,71 @@ class DFSSMModel:
         self._next.copy_(out[-1][:, -1])
         return torch.cat(out, dim=1)[:, :n_tokens], time.perf_counter() - start
 
+    def _filtered_step(self, tokens: Optional[torch.Tensor], u: torch.Tensor, out: torch.Tensor) -> None:
+        """One decode step whose next token is drawn by dfssm_sample_filtered with the numbers u (B,);
+        x receives the drawn token's embedding."""
+        B, V = self.batch_size, self.cfg.vocab_size
+        self._decode(tokens, self.logits, self._fnext, fuse=False)
+        _C.check(_C.lib().dfssm_sample_filtered(self.logits.data_ptr(), ops.LOGIT_TYPE[self.logits.dtype], V, B, V,
+                                                u.data_ptr(), ctypes.byref(self._filter), out.data_ptr(), None,
+                                                _C.stream()), "sample_filtered")
+        _C.check(_C.lib().dfssm_embed(self._model, out.data_ptr(), self.x.data_ptr(), self.workspace.data_ptr(),
+                                      _C.stream()), "embed")
+
+    def _filtered_graph(self, S: int):
+        """S filtered steps, reading their random numbers from u (S, B) and the filters from the device, so one
+        graph serves every setting. Returns (graph, u, tokens (S, B))."""
+        if S not in self._filtered_graphs:
+            u = torch.zeros(S, self.batch_size, device=self.device)
+            hist = torch.zeros(S, self.batch_size, dtype=torch.int64, device=self.device)
+
+            def body():
+                for i in range(S):
+                    self._filtered_step(None, u[i], hist[i])
+            self._filtered_graphs[S] = (self._capture(body), u, hist)
+        return self._filtered_graphs[S]
+
+    def _generate_filtered(self, n_tokens, prompt, temperature, top_k, top_p, min_p, seed):
+        """Decode with top_k / min_p (dfssm_sample_filtered). Step t of sequence b draws with number [t, b] of
+        torch.rand(n_tokens, B) from a host generator seeded by seed; returns (tokens (B, n), seconds)."""
+        B, dev = self.batch_size, self.device
+        if getattr(self, "_filter", None) is None:
+            self._fnext = torch.zeros(B, dtype=torch.int64, device=dev)
+            self._filter_f = torch.zeros(3, B, device=dev)
+            self._filter_k = torch.zeros(B, dtype=torch.int32, device=dev)
+            f = self._filter_f
+            self._filter = _C.Filter(f[0].data_ptr(), self._filter_k.data_ptr(), f[1].data_ptr(), f[2].data_ptr(),
+                                     1.0, 0, 1.0, 0.0)
+            self._filtered_graphs = {}
+        for row, value in zip(self._filter_f, (temperature, top_p, min_p)):
+            row.fill_(float(value))
+        self._filter_k.fill_(int(top_k))
+        gen = torch.Generator().manual_seed(int(seed) & (2**63 - 1))
+        u = torch.rand(max(n_tokens, 1), B, generator=gen).to(dev)
+        S = 8 if n_tokens > 8 else 1
+        self._filtered_graph(S)
+        self._filtered_graph(1)
+        if prompt.shape[1] > 1:
+            self.ingest(prompt[:, :-1])
+        first = torch.empty(B, dtype=torch.int64, device=dev)
+        torch.cuda.synchronize(dev)
+        start = time.perf_counter()
+        self._filtered_step(prompt[:, -1].contiguous(), u[0], first)
+        out = [first[:, None]]
+        done = 1
+        while done < n_tokens:
+            s = S if n_tokens - done >= S else 1
+            g, gu, hist = self._filtered_graph(s)
+            gu.copy_(u[done:done + s])
+            g.replay()
+            out.append(hist.t().clone())
+            done += s
+        torch.cuda.synchronize(dev)
+        self._next.copy_(out[-1][:, -1])
+        return torch.cat(out, dim=1)[:, :n_tokens], time.perf_counter() - start
+
     def generate(self, n_tokens=128, prompt=None, return_tokens=False, verbose=True, temperature=None,
-                 top_p=1.0, repetition_penalty=1.0, penalty_mode=0, seed=0, state_df=None):
+                 top_p=1.0, repetition_penalty=1.0, penalty_mode=0, seed=0, state_df=None, top_k=0, min_p=0.0):
         """Greedy decode timed like the reference's generate (df_ssm_inference.py:226-243).
 
         The timed region holds n_tokens decode steps: the first consumes the last prompt token
@@ -595,7 +678,9 @@ class DFSSMModel:
         With a temperature, the tokens are drawn instead (dfssm_sample: temperature, top_p,
         repetition_penalty over the prompt and the tokens drawn so far; penalty_mode 0 is
         eval/gen_test.py:54-95, 1 the training script's :1066-1078), from a generator seeded by
-        `seed`.
+        `seed`. With top_k > 0 or min_p > 0 as well, dfssm_sample_filtered draws (temperature,
+        top_k, top_p and min_p, in that order; vocabularies up to 262144), with random numbers
+        from a host generator seeded by `seed`; that draw takes no repetition_penalty.
 
         With state_df (a StateDensityField; greedy only), the SSM state is quantized at every
         block_len-token chunk boundary as in training (apply_state_density_field).
@@ -609,6 +694,7 @@ class DFSSMModel:
         if prompt.dim() != 2 or prompt.shape[0] != B or prompt.shape[1] < 1:
             raise ValueError(f"prompt must be (batch={B}, T >= 1), got {tuple(prompt.shape)}")
         _check_token_range(prompt, self.cfg.vocab_size)  # before any kernel reads the ids
+        filtered = _draw_filters(temperature, top_k, top_p, min_p, repetition_penalty, state_df)
         self.reset_state()
         prompt = prompt.to(self.device, torch.int64)
         if state_df is not None:
@@ -622,8 +708,11 @@ class DFSSMModel:
                 print(f"  {elapsed*1000:.1f} ms  ({n_tokens * B / elapsed:.0f} tok/s total)")
             return toks if return_tokens else None
         if temperature is not None:
-            toks, elapsed = self._generate_sampled(n_tokens, prompt, temperature, top_p, repetition_penalty,
-                                                   penalty_mode, seed)
+            if filtered:
+                toks, elapsed = self._generate_filtered(n_tokens, prompt, temperature, top_k, top_p, min_p, seed)
+            else:
+                toks, elapsed = self._generate_sampled(n_tokens, prompt, temperature, top_p, repetition_penalty,
+                                                       penalty_mode, seed)
             self.check_errors()
             self.last_elapsed = elapsed
             if verbose:

@@ -336,7 +336,7 @@ def gated_delta_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: to
 # ---------------------------------------------------------------------------------------------
 # token draw
 # ---------------------------------------------------------------------------------------------
-_LOGIT_TYPE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}   # DFSSM_TYPE_*
+LOGIT_TYPE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}   # DFSSM_TYPE_*
 
 
 def _on_device(t: torch.Tensor, name: str, dev) -> None:
@@ -369,7 +369,7 @@ def sample_filtered(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_
     <= 0 takes the most probable token; top_k <= 0, top_p >= 1, min_p <= 0 filter nothing. A row whose logits
     are all -inf gives -1. V at most 262144; rows may be strided. With want_logprob also the logarithm of each
     token's share of what was kept, (B,) fp32."""
-    kind = _LOGIT_TYPE.get(logits.dtype) if isinstance(logits, torch.Tensor) else None
+    kind = LOGIT_TYPE.get(logits.dtype) if isinstance(logits, torch.Tensor) else None
     if kind is None:
         raise TypeError("logits must be a float16, bfloat16 or float32 tensor")
     _need(logits, logits.dtype, "logits")

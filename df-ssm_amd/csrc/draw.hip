@@ -30,6 +30,7 @@ constexpr int kBins = 2048;
 constexpr int kFine = 1024;    // bins of 1/64 in (m - l) / T; the others share what lies below
 constexpr int kList = 2046;    // tokens that are sorted in LDS (and their masses, one more)
 constexpr double kOne = 17592186044416.0;  // 2^44
+constexpr int kTab = 1024;     // entries of the exponential's table
 
 typedef unsigned long long u64;
 
@@ -42,15 +43,15 @@ __device__ __forceinline__ float logit_at(const void* row, int i) {
 // A NaN ranks as -inf; -0 as +0 (they are equal, so their order is that of the indexes).
 __device__ __forceinline__ float clean(float l) { return l != l ? -__builtin_inff() : l + 0.0f; }
 
-// f(index, logit) for every token of the row, by all threads: 16 bytes a load between the row's aligned ends, two
-// loads ahead.
+// f(index, logit, first of its load) for every token of the row, by all threads: 16 bytes a load between the row's
+// aligned ends, two loads ahead.
 template <int TYPE, class F>
 __device__ __forceinline__ void each_token(const void* row, int V, F f) {
   constexpr int ES = TYPE == DFSSM_TYPE_F32 ? 4 : 2, N = 16 / ES;
   const int tid = threadIdx.x;
   const int head = min(V, (int)((16 - ((uintptr_t)row & 15)) & 15) / ES), nb = (V - head) / N, tail = head + nb * N;
-  if (tid < head) f(tid, logit_at<TYPE>(row, tid));
-  if (tail + tid < V) f(tail + tid, logit_at<TYPE>(row, tail + tid));
+  if (tid < head) f(tid, logit_at<TYPE>(row, tid), true);
+  if (tail + tid < V) f(tail + tid, logit_at<TYPE>(row, tail + tid), true);
   const u32x4* p = (const u32x4*)((const char*)row + head * ES);
   auto piece = [&](const u32x4 x, int c) {
 #pragma unroll
@@ -60,7 +61,7 @@ __device__ __forceinline__ void each_token(const void* row, int V, F f) {
       if constexpr (TYPE == DFSSM_TYPE_F32) l = __builtin_bit_cast(float, word);
       else if constexpr (TYPE == DFSSM_TYPE_BF16) l = __builtin_bit_cast(float, (e & 1) ? word & 0xffff0000u : word << 16);
       else l = h2f((uint16_t)(word >> (16 * (e & 1))));
-      f(head + c * N + e, l);
+      f(head + c * N + e, l, e == 0);
     }
   };
   // (the loop is not unrolled: a body is passed over a few times only, and its fetching from memory would cost more)
@@ -86,48 +87,50 @@ __device__ __forceinline__ float key_logit(uint32_t k) {
 }
 
 struct RowScale {
-  float m, s1, s2;   // bins: x = (m - l) s1 below kFine, then kFine + (x - kFine) s2
-  bool top;          // the largest logit is +inf: such tokens count as logit 0 and the others as -inf
-  double y1;         // 64 log2(e) / T: e = 2^((l - m) y1 / 64)
-  const double* tab; // 2^(j / 64), j = 0 .. 63
+  float m;           // the largest logit, finite here (rows with a +inf go their own way)
+  float s1, s2, c2;  // bins: x = (m - l) s1 below kFine, then s2 x + c2, a line that is less steep
+  float reach;       // tokens further than this below m have no mass (31.5 T: e < 2^-45)
+  double y1;         // kTab log2(e) / T: e = 2^((l - m) y1 / kTab)
+  const double* tab; // 2^(44 + j / kTab)
 };
-// A token's logit as it is ranked: -inf takes no part (nor does a NaN).
-__device__ __forceinline__ float ranked(const RowScale r, float l) {
-  l = clean(l);
-  if (r.top) l = l == __builtin_inff() ? 0.0f : -__builtin_inff();  // (uniform)
-  return l;
-}
-__device__ __forceinline__ bool taken(float l) { return l > -__builtin_inff(); }
-// The bin of a token that takes part, 0 <= x (not NaN: T > 0, so s1 is at most +inf and m - l = 0 gives bin 0).
+// -inf takes no part, nor does a NaN: both fail this (l <= m).
+__device__ __forceinline__ bool taken(const RowScale r, float l) { return r.m - l < __builtin_inff(); }
+// The bin of a token that takes part: the lower of the two lines (they cross at kFine).
 __device__ __forceinline__ int bin_of(const RowScale r, float l) {
-  const float d = r.m - l, x = d > 0.0f ? d * r.s1 : 0.0f;
-  const float y = (x - (float)kFine) * r.s2;
-  const int low = kFine + (y < (float)(kBins - kFine - 1) ? (int)y : kBins - kFine - 1);
-  return x < (float)kFine ? (int)x : low;
+  const float x = (r.m - l) * r.s1;
+  return (int)fminf(fminf(x, __builtin_fmaf(x, r.s2, r.c2)), (float)(kBins - 1));
 }
-// exp((l - m) / T) = 2^(n / 64) 2^(t / 64), n whole, |t| <= 1/2: a table and the Taylor polynomial of degree 5 of the
-// second factor, whose rest is below 2^-54. (exp() takes four times as many instructions, and this is most of the
-// work.) What underflows comes out as 0.
-__device__ __forceinline__ double e_of(const RowScale r, float l) {
-  constexpr double c = 0.693147180559945309417 / 64.0;
+// How far below m the upper end of bin b lies, `off` bins of tolerance for the roundings of bin_of (2^-13 of a bin).
+__device__ __forceinline__ float bin_start(const RowScale r, int b, float off) {
+  const float y = (float)b + off;
+  return (y < (float)kFine ? y : (y - r.c2) / r.s2) / r.s1;
+}
+// e 2^44 = 2^44 exp((l - m) / T) for (m - l) <= reach, else 0: 2^((n + t) / kTab), n whole, |t| <= 1/2, from a table,
+// an exponent added to it (44 + j / kTab + n / kTab > -2: it stays a normal number) and the Taylor polynomial of degree 3,
+// whose rest is below 2^-50. n comes by adding 3 2^51, whose sum has it in its low bits. (exp() takes four times as
+// many instructions, and this is most of the work.)
+__device__ __forceinline__ double e44(const RowScale r, float l) {
+  constexpr double c = 0.693147180559945309417 / kTab, big = 6755399441055744.0;
+  if (!(r.m - l <= r.reach)) return 0.0;
   const double y = ((double)l - (double)r.m) * r.y1;
-  const double n = __builtin_rint(y), t = y - n;
-  double p = c * c * c * c * c / 120.0;
-  p = __builtin_fma(p, t, c * c * c * c / 24.0);
-  p = __builtin_fma(p, t, c * c * c / 6.0);
-  p = __builtin_fma(p, t, c * c / 2.0);
+  const double z = y + big, t = y - (z - big);
+  double p = __builtin_fma(c * c * c / 6.0, t, c * c / 2.0);
   p = __builtin_fma(p, t, c);
   p = __builtin_fma(p, t, 1.0);
-  const int i = (int)n;
-  return __builtin_amdgcn_ldexp(r.tab[i & 63] * p, i >> 6);
+  const int n = (int)(uint32_t)__builtin_bit_cast(u64, z);
+  const u64 v = __builtin_bit_cast(u64, r.tab[n & (kTab - 1)] * p);
+  const uint32_t hi = (uint32_t)(v >> 32) + ((uint32_t)(n >> 10) << 20);
+  static_assert(kTab == 1 << 10, "n = kTab times the exponent and j");
+  return __builtin_bit_cast(double, ((u64)hi << 32) | (uint32_t)v);
 }
-// rint(e 2^44), 0 <= e <= 1: added to 2^52 it is the low bits of the sum.
-__device__ __forceinline__ u64 mass_of(double e) {
-  return __builtin_bit_cast(u64, __builtin_fma(e, kOne, 4503599627370496.0)) & 0xfffffffffffffull;
+// The mass E = rint(e 2^44): added to 2^52 it is the low bits of the sum.
+__device__ __forceinline__ u64 mass_of(double e44) {
+  return __builtin_bit_cast(u64, e44 + 4503599627370496.0) & 0xfffffffffffffull;
 }
+constexpr u64 kUnit = 1ull << 44;  // the mass of the most probable token
 
 struct DrawLds {
-  double tab[64];
+  double tab[kTab];
   uint32_t cnt[kBins + 2];  // per bin, then tokens in earlier bins
   u64 mass[kBins + 2];      // the same for masses
   u64 comp[kList + 2];   // (order key << 24) | index of the listed tokens, sorted
@@ -184,12 +187,19 @@ __device__ __forceinline__ int sort_bins(const void* row, int V, const RowScale 
   const int tid = threadIdx.x;
   if (tid == 0) L.nlist = 0;
   __syncthreads();
-  each_token<TYPE>(row, V, [&](int i, float raw) {
-    const float l = ranked(rs, raw);
-    const int b = bin_of(rs, l);
-    if (taken(l) && ((b >= lo && b <= hi) || b == far)) {
-      const int p = atomicAdd(&L.nlist, 1);
-      if (p < kList) L.comp[p] = ((u64)order_key(l) << 24) | (uint32_t)i;
+  // Logits that may lie in the bins, by two compares; what passes is looked at closely.
+  const float inf = __builtin_inff();
+  const float near0 = lo > 0 ? rs.m - bin_start(rs, lo, -0.01f) * 0.99999f : inf;
+  const float near1 = hi < kBins - 1 ? rs.m - bin_start(rs, hi + 1, 0.01f) * 1.00001f : -inf;
+  const float far0 = far >= 0 ? rs.m - bin_start(rs, far, -0.01f) * 0.99999f : -inf;
+  const float far1 = far >= 0 && far < kBins - 1 ? rs.m - bin_start(rs, far + 1, 0.01f) * 1.00001f : far >= 0 ? -inf : inf;
+  each_token<TYPE>(row, V, [&](int i, float l, bool) {
+    if ((l <= near0 && l >= near1) || (l <= far0 && l >= far1)) {
+      const int b = bin_of(rs, l);
+      if (taken(rs, l) && ((b >= lo && b <= hi) || b == far)) {
+        const int p = atomicAdd(&L.nlist, 1);
+        if (p < kList) L.comp[p] = ((u64)order_key(clean(l)) << 24) | (uint32_t)i;
+      }
     }
   });
   __syncthreads();
@@ -237,7 +247,7 @@ __device__ __forceinline__ int sort_bins(const void* row, int V, const RowScale 
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
     const int i = 2 * tid + q;
-    m[q] = i < n ? mass_of(e_of(rs, key_logit((uint32_t)(L.comp[i] >> 24)))) : 0;
+    m[q] = i < n ? mass_of(e44(rs, key_logit((uint32_t)(L.comp[i] >> 24)))) : 0;
   }
   uint32_t c = 0;
   u64 s = m[0] + m[1];
@@ -264,7 +274,7 @@ struct Found {
 };
 __device__ __forceinline__ Found found(u64 above, u64 comp, const RowScale rs) {
   const uint32_t key = (uint32_t)(comp >> 24);
-  return Found{above, mass_of(e_of(rs, key_logit(key))), key, (uint32_t)(comp & 0xffffffu)};
+  return Found{above, mass_of(e44(rs, key_logit(key))), key, (uint32_t)(comp & 0xffffffu)};
 }
 
 // The last bin in use whose first token qualifies. By mass, a bin without mass is not in use: what lies there
@@ -314,13 +324,12 @@ __device__ __forceinline__ Found search_row(const Ask q, int bin, const void* ro
     }
     if (tid == 0) L.found = -1;
     __syncthreads();
-    each_token<TYPE>(row, V, [&](int i, float raw) {
-      const float l = ranked(rs, raw);
-      if (!taken(l) || bin_of(rs, l) != bin) return;
-      const u64 c = ((u64)order_key(l) << 24) | (uint32_t)i;
+    each_token<TYPE>(row, V, [&](int i, float l, bool) {
+      if (!taken(rs, l) || bin_of(rs, l) != bin) return;
+      const u64 c = ((u64)order_key(clean(l)) << 24) | (uint32_t)i;
       if ((c >> (sh + 8)) == prefix) {
         atomicAdd(&L.dcnt[(c >> sh) & 255], 1u);
-        atomicAdd(&L.dmass[(c >> sh) & 255], mass_of(e_of(rs, l)));
+        atomicAdd(&L.dmass[(c >> sh) & 255], mass_of(e44(rs, l)));
       }
     });
     __syncthreads();
@@ -364,6 +373,31 @@ __device__ __forceinline__ u64 wave_add64(u64 v) {
   return v;
 }
 
+// A row with +inf logits: each has mass 1 and nothing else any, ranked by index. Which of them is drawn comes from
+// their number; every thread counts those of a stretch of the row, and the one whose stretch holds it walks along.
+template <int TYPE>
+__device__ __forceinline__ void draw_inf(const DrawArgs& a, const void* row, int k, float tp, float mp, float u, DrawLds& L) {
+  const int tid = threadIdx.x, per = (a.V + kDT - 1) / kDT, from = min(a.V, tid * per), to = min(a.V, from + per);
+  uint32_t mine = 0;
+  for (int i = from; i < to; ++i) mine += logit_at<TYPE>(row, i) == __builtin_inff() ? 1 : 0;
+  uint32_t c = mine;
+  u64 none = 0;
+  block_excl<kDT>(c, none, L);
+  if (tid == kDT - 1) L.rcnt = c + mine;
+  __syncthreads();
+  int n = (int)L.rcnt;
+  if (k > 0) n = min(n, k);
+  if (tp < 1.0f) n = min(n, (int)((double)(tp > 0.0f ? tp : 0.0f) * (double)n) + 1);
+  if (!(mp <= 1.0f)) n = 1;
+  const uint32_t at = (uint32_t)min(n - 1, (int)((double)u * (double)n));
+  if (at < c || at >= c + mine) return;
+  for (int i = from; i < to; ++i)
+    if (logit_at<TYPE>(row, i) == __builtin_inff() && c++ == at) {
+      a.next[blockIdx.x] = i;
+      if (a.logprob) a.logprob[blockIdx.x] = (float)-log((double)n);
+    }
+}
+
 template <int TYPE>
 __global__ __launch_bounds__(kDT) void draw_row_kernel(DrawArgs a) {
   __shared__ DrawLds L;
@@ -376,18 +410,17 @@ __global__ __launch_bounds__(kDT) void draw_row_kernel(DrawArgs a) {
   float u = a.u[b];
   u = u >= 0.0f ? (u < 1.0f ? u : 0.99999994f) : 0.0f;
 
-  // the largest logit, and nearly the least finite one (of every eighth: only the bins' width comes from it)
+  // the largest logit, and nearly the least finite one (of one in each load: only the bins' width comes from it)
   float m = -__builtin_inff(), lo = __builtin_inff();
-  each_token<TYPE>(row, V, [&](int i, float raw) {
-    const float l = clean(raw);
-    m = l > m ? l : m;
-    if ((i & 7) == 0 && l < lo && taken(l)) lo = l;
+  each_token<TYPE>(row, V, [&](int, float l, bool first) {
+    m = fmaxf(m, l);  // (of a NaN and a number, the number)
+    if (first && l < lo && l > -__builtin_inff()) lo = l;
   });
   for (int i = tid; i < kBins; i += kDT) {
     L.cnt[i] = 0;
     L.mass[i] = 0;
   }
-  if (tid < 64) L.tab[tid] = exp2((double)tid * (1.0 / 64.0));
+  for (int i = tid; i < kTab; i += kDT) L.tab[i] = exp2((double)i * (1.0 / kTab)) * kOne;
   for (int o = 32; o > 0; o >>= 1) {
     m = fmaxf(m, __shfl_xor(m, o, 64));
     lo = fminf(lo, __shfl_xor(lo, o, 64));
@@ -412,8 +445,8 @@ __global__ __launch_bounds__(kDT) void draw_row_kernel(DrawArgs a) {
   }
   if (m == -__builtin_inff() || !(T > 0.0f)) {  // nothing to draw from; greedy
     const bool none = m == -__builtin_inff();
-    if (!none) each_token<TYPE>(row, V, [&](int i, float raw) {
-      if (clean(raw) == m) atomicMin(&L.found, i);
+    if (!none) each_token<TYPE>(row, V, [&](int i, float l, bool) {
+      if (l == m) atomicMin(&L.found, i);
     });
     __syncthreads();
     if (tid == 0) {
@@ -422,26 +455,32 @@ __global__ __launch_bounds__(kDT) void draw_row_kernel(DrawArgs a) {
     }
     return;
   }
+  if (m == __builtin_inff()) {
+    draw_inf<TYPE>(a, row, k, tp, mp, u, L);
+    return;
+  }
   RowScale rs;
-  rs.top = m == __builtin_inff();
-  rs.m = rs.top ? 0.0f : m;
-  rs.y1 = 64.0 * 1.4426950408889634074 / (double)T;
+  rs.m = m;
+  rs.y1 = kTab * 1.4426950408889634074 / (double)T;
   rs.tab = L.tab;
+  rs.reach = fminf(31.5f * T, 3.4028234e38f);
   rs.s1 = 64.0f / T;
   rs.s2 = 1.0f;
-  if (!rs.top && lo < m) {
+  if (lo < m) {
     const float span = m - lo, x = span * rs.s1;
     if (!(x >= (float)kFine)) rs.s1 = (float)(kFine - 1) / span;  // a narrow row spreads over the fine bins
     else if (x > (float)kBins) rs.s2 = (float)(kBins - kFine - 1) / (x - (float)kFine);
   }
+  rs.s1 = fminf(rs.s1, 1e38f);  // (so that 0 stays bin 0)
+  rs.c2 = (float)kFine - (float)kFine * rs.s2;
 
   const bool limit = k > 0 && k < V;
+  const double mp44 = (double)mp * kOne;
   // What can be kept lies in the first bins if there is a top_k, or a min_p and no top_p (whose mass is that of all).
   const bool by_k = limit && k <= kList, by_m = !limit && mp > 0.0f && mp <= 1.0f && !(tp < 1.0f) && T <= 1024.0f;
   if (limit || by_m) {
-    each_token<TYPE>(row, V, [&](int, float raw) {
-      const float l = ranked(rs, raw);
-      if (taken(l)) atomicAdd(&L.cnt[bin_of(rs, l)], 1u);
+    each_token<TYPE>(row, V, [&](int, float l, bool) {
+      if (taken(rs, l)) atomicAdd(&L.cnt[bin_of(rs, l)], 1u);
     });
     __syncthreads();
     const uint32_t c0 = L.cnt[2 * tid], c1 = L.cnt[2 * tid + 1];
@@ -460,7 +499,7 @@ __global__ __launch_bounds__(kDT) void draw_row_kernel(DrawArgs a) {
     int n = kList + 1;
     if (L.cnt[hi + 1] <= kList) n = sort_bins<TYPE>(row, V, rs, 0, hi, -1, L);
     // (should the border be further off than the bins tell, the last token listed passes it)
-    if (by_m && n <= kList && n < (int)L.cnt[kBins] && e_of(rs, key_logit((uint32_t)(L.comp[n - 1] >> 24))) >= (double)mp)
+    if (by_m && n <= kList && n < (int)L.cnt[kBins] && e44(rs, key_logit((uint32_t)(L.comp[n - 1] >> 24))) >= mp44)
       n = kList + 1;
     if (n <= kList) {
       const int nk = by_k ? min(k, n) : n;
@@ -468,8 +507,8 @@ __global__ __launch_bounds__(kDT) void draw_row_kernel(DrawArgs a) {
       if (tid == 0) L.found = 0;
       __syncthreads();
       for (int i = tid; i < nk; i += kDT) {
-        const double e = e_of(rs, key_logit((uint32_t)(L.comp[i] >> 24)));
-        if ((!(tp < 1.0f) || (double)L.lmass[i] <= (double)(tp > 0.0f ? tp : 0.0f) * (double)Z) && e >= (double)mp)
+        const double e = e44(rs, key_logit((uint32_t)(L.comp[i] >> 24)));
+        if ((!(tp < 1.0f) || (double)L.lmass[i] <= (double)(tp > 0.0f ? tp : 0.0f) * (double)Z) && e >= mp44)
           atomicMax(&L.found, i);
       }
       __syncthreads();
@@ -480,26 +519,26 @@ __global__ __launch_bounds__(kDT) void draw_row_kernel(DrawArgs a) {
       if (tid == 0) {
         const u64 c = L.comp[i];
         a.next[b] = (int64_t)(c & 0xffffffu);
-        if (a.logprob) a.logprob[b] = (float)log(e_of(rs, key_logit((uint32_t)(c >> 24))) * kOne / (double)S);
+        if (a.logprob) a.logprob[b] = (float)log(e44(rs, key_logit((uint32_t)(c >> 24))) / (double)S);
       }
       return;
     }
   }
 
   u64 mm = 0;  // the mass of the tokens with e >= min_p
-  each_token<TYPE>(row, V, [&](int, float raw) {
-    const float l = ranked(rs, raw);
-    if (!taken(l)) return;
-    const double e = e_of(rs, l);
+  const double border_m = mp <= 0.0f ? __builtin_inf() : mp44;
+  each_token<TYPE>(row, V, [&](int, float l, bool) {
+    if (!(rs.m - l <= rs.reach)) return;
+    const double e = e44(rs, l);
     const u64 E = mass_of(e);
-    if (E) atomicAdd(&L.mass[bin_of(rs, l)], E);
-    if (e >= (double)mp) mm += E;
+    atomicAdd(&L.mass[bin_of(rs, l)], E);
+    if (e >= border_m) mm += E;
   });
   mm = wave_add64(mm);
   if (lane == 0) atomicAdd(&L.rmass, mm);
   __syncthreads();
-  // (rank 0, whose mass is 1, is kept in any case)
-  const u64 M_m = L.rmass > mass_of(1.0) ? L.rmass : mass_of(1.0);
+  // (rank 0 is kept in any case)
+  const u64 M_m = mp <= 0.0f ? ~0ull : L.rmass > kUnit ? L.rmass : kUnit;
   const u64 m0 = L.mass[2 * tid], m1 = L.mass[2 * tid + 1];
   uint32_t c = 0;
   u64 ms = m0 + m1;
@@ -558,7 +597,7 @@ __global__ __launch_bounds__(kDT) void draw_row_kernel(DrawArgs a) {
   }
   if (tid == 0) {
     a.next[b] = (int64_t)f.idx;
-    if (a.logprob) a.logprob[b] = (float)log(e_of(rs, key_logit(f.key)) * kOne / (double)S);
+    if (a.logprob) a.logprob[b] = (float)log(e44(rs, key_logit(f.key)) / (double)S);
   }
 }
 

@@ -24,6 +24,7 @@ def reference(l, u, T, k, tp, mp):
         return int(order[0]), 0.0
     with np.errstate(invalid="ignore", divide="ignore"):
         e = np.where(s == s[0], 1.0, np.exp((s - s[0]) / T))
+        e = np.where((s < s[0]) & ((s == -np.inf) | (s[0] == np.inf)), 0.0, e)   # (at T = inf too: -inf / inf is NaN)
     nk = k if 0 < k < len(l) else len(l)
     above = np.concatenate([[0.0], np.cumsum(e)])
     Z = above[nk]
@@ -209,3 +210,35 @@ def test_refusals():
     with pytest.raises(ValueError):
         ops.sample_filtered(l, u, top_p=torch.ones(3, device=DEV))
     assert ops.sample_filtered(l[:0], u[:0]).shape == (0,)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_infinities_and_signalling_nans(dtype):
+    """Several +inf logits with every filter (each mass 1, in index order); NaNs of either kind beside the largest."""
+    rng = np.random.default_rng(31)
+    V, B = 5003, 9
+    l = rng.normal(0, 2, (B, V)).astype(np.float32)
+    l[:, rng.random(V) < 0.01] = np.inf
+    l[2, 17:] = np.nan
+    l[3] = np.inf
+    l[6:] = rng.normal(0, 2, (3, V))
+    d = torch.from_numpy(l).to(dtype)
+    bits = d.view(torch.int16 if dtype == torch.float16 else torch.int32)
+    quiet = {torch.float16: 0x7C01, torch.float32: 0x7F800001}[dtype]                    # signalling: quiet bit clear
+    bits[6:, rng.random(V) < 0.3] = quiet
+    bits[7, 1::2] = quiet
+    for T, k, tp, mp in [(1.0, 0, 1.0, 0.0), (0.7, 5, 1.0, 0.0), (0.7, 0, 0.5, 0.0), (1.3, 30, 0.4, 1.0),
+                         (0.9, 0, 0.0, 0.0), (0.9, 0, 1.0, 1.5), (float("inf"), 4000, 0.9, 0.0)]:
+        run_check(d, rng.random(B).astype(np.float32), T, k, tp, mp)
+
+
+@pytest.mark.parametrize("spread", [1e-38, 1e-6, 1.0, 1e4, 1e30])
+def test_spreads(spread):
+    """Logits closer together and further apart than any model's, around 0 and around a large value."""
+    rng = np.random.default_rng(37)
+    l = (rng.normal(0, 1, (8, 6007)) * spread).astype(np.float32)
+    l[4:] += np.float32(1000.0 * spread)
+    u = rng.random(8).astype(np.float32)
+    for T in (0.8 * spread, 1.0):
+        run_check(torch.from_numpy(l), u, T, np.array([0, 30, 0, 5000] * 2), np.array([0.9, 0.9, 1.0, 0.99] * 2),
+                  np.array([0.0, 0.0, 0.05, 0.0] * 2))

@@ -130,7 +130,7 @@ __device__ __forceinline__ u64 mass_of(double e44) {
 constexpr u64 kUnit = 1ull << 44;  // the mass of the most probable token
 
 struct DrawLds {
-  double tab[kTab];
+  double tab[kTab], ends[64];
   uint32_t cnt[kBins + 2];  // per bin, then tokens in earlier bins
   u64 mass[kBins + 2];      // the same for masses
   u64 comp[kList + 2];   // (order key << 24) | index of the listed tokens, sorted
@@ -260,6 +260,20 @@ __device__ __forceinline__ int sort_bins(const void* row, int V, const RowScale 
   return n;
 }
 
+// L.cnt: from tokens per bin to tokens in earlier bins, and in all behind the last one.
+__device__ __forceinline__ void count_prefix(DrawLds& L) {
+  const int tid = threadIdx.x;
+  __syncthreads();
+  const uint32_t c0 = L.cnt[2 * tid], c1 = L.cnt[2 * tid + 1];
+  uint32_t c = c0 + c1;
+  u64 none = 0;
+  block_excl<kDT>(c, none, L);
+  L.cnt[2 * tid] = c;
+  L.cnt[2 * tid + 1] = c + c0;
+  if (tid == kDT - 1) L.cnt[kBins] = c + c0 + c1;
+  __syncthreads();
+}
+
 // A question to the ranking: by count (the last rank with fewer than n above it) or by mass (the last
 // rank with mass at most x above it). Rank 0 always qualifies.
 struct Ask {
@@ -277,6 +291,12 @@ __device__ __forceinline__ Found found(u64 above, u64 comp, const RowScale rs) {
   return Found{above, mass_of(e44(rs, key_logit(key))), key, (uint32_t)(comp & 0xffffffu)};
 }
 
+// max of what the lanes hold, one atomic per wave (one address: lane by lane they would queue up).
+__device__ __forceinline__ void raise(int* to, int v) {
+  for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
+  if ((threadIdx.x & 63) == 0 && v >= 0) atomicMax(to, v);
+}
+
 // The last bin in use whose first token qualifies. By mass, a bin without mass is not in use: what lies there
 // comes after all that a mass can ask for.
 __device__ __forceinline__ int last_bin(const Ask q, DrawLds& L) {
@@ -290,7 +310,7 @@ __device__ __forceinline__ int last_bin(const Ask q, DrawLds& L) {
     const bool used = q.by_mass ? L.mass[b + 1] != L.mass[b] : L.cnt[b + 1] != L.cnt[b];
     if (used && (q.by_mass ? q.holds(0, L.mass[b]) : q.holds(L.cnt[b], 0))) best = b;
   }
-  if (best >= 0) atomicMax(&L.found, best);
+  raise(&L.found, best);
   __syncthreads();
   const int bin = L.found;
   __syncthreads();
@@ -301,8 +321,10 @@ __device__ __forceinline__ int last_entry(const Ask q, int from, int to, uint32_
   const int tid = threadIdx.x;
   if (tid == 0) L.found = from;
   __syncthreads();
+  int best = -1;
   for (int i = from + tid; i < to; i += kDT)
-    if (q.holds(above + (uint32_t)(i - from), base + L.lmass[i])) atomicMax(&L.found, i);
+    if (q.holds(above + (uint32_t)(i - from), base + L.lmass[i])) best = i;
+  raise(&L.found, best);
   __syncthreads();
   const int i = L.found;
   __syncthreads();
@@ -420,7 +442,8 @@ __global__ __launch_bounds__(kDT) void draw_row_kernel(DrawArgs a) {
     L.cnt[i] = 0;
     L.mass[i] = 0;
   }
-  for (int i = tid; i < kTab; i += kDT) L.tab[i] = exp2((double)i * (1.0 / kTab)) * kOne;
+  if (tid < 64) L.ends[tid] = tid < 32 ? exp2((double)tid * (1.0 / 32)) * kOne : exp2((double)(tid - 32) * (1.0 / kTab));
+  const float own = m;  // of this thread's tokens
   for (int o = 32; o > 0; o >>= 1) {
     m = fmaxf(m, __shfl_xor(m, o, 64));
     lo = fminf(lo, __shfl_xor(lo, o, 64));
@@ -443,6 +466,8 @@ __global__ __launch_bounds__(kDT) void draw_row_kernel(DrawArgs a) {
     m = fmaxf(m, L.wf[i]);
     lo = fminf(lo, L.wg[i]);
   }
+  L.tab[tid] = L.ends[tid >> 5] * L.ends[32 + (tid & 31)];
+  static_assert(kTab == kDT && kTab == 32 * 32, "an entry per thread");
   if (m == -__builtin_inff() || !(T > 0.0f)) {  // nothing to draw from; greedy
     const bool none = m == -__builtin_inff();
     if (!none) each_token<TYPE>(row, V, [&](int i, float l, bool) {
@@ -477,40 +502,43 @@ __global__ __launch_bounds__(kDT) void draw_row_kernel(DrawArgs a) {
   const bool limit = k > 0 && k < V;
   const double mp44 = (double)mp * kOne;
   // What can be kept lies in the first bins if there is a top_k, or a min_p and no top_p (whose mass is that of all).
-  const bool by_k = limit && k <= kList, by_m = !limit && mp > 0.0f && mp <= 1.0f && !(tp < 1.0f) && T <= 1024.0f;
-  if (limit || by_m) {
+  const bool by_k = limit && k <= kList, by_m = !limit && mp > 0.0f && mp <= 1.0f && !(tp < 1.0f);
+  // A bin that has k threads' largest tokens in it or before it has the first k ranks too. That is nearly the bin of
+  // rank k while k is small beside the threads (k = 512: 0.7 tokens a thread, 710 in all), and needs no pass.
+  const bool by_own = limit && k <= kDT / 2;
+  int hi = kBins - 1, n = kList + 1;
+  if (by_m) hi = bin_of(rs, rs.m + T * (__builtin_logf(mp) * 1.0001f - 1e-6f));  // (what passes min_p lies before it)
+  if (by_own) {
+    if (taken(rs, own)) atomicAdd(&L.cnt[bin_of(rs, own)], 1u);
+    count_prefix(L);
+    if (L.cnt[kBins] >= (uint32_t)k) hi = last_bin(Ask{false, (uint32_t)k, 0.0}, L);
+  }
+  if (by_own || by_m) {
+    __syncthreads();
+    n = sort_bins<TYPE>(row, V, rs, 0, hi, -1, L);
+  }
+  if (limit && n > kList) {
+    for (int i = tid; i < kBins; i += kDT) L.cnt[i] = 0;
+    __syncthreads();
     each_token<TYPE>(row, V, [&](int, float l, bool) {
       if (taken(rs, l)) atomicAdd(&L.cnt[bin_of(rs, l)], 1u);
     });
-    __syncthreads();
-    const uint32_t c0 = L.cnt[2 * tid], c1 = L.cnt[2 * tid + 1];
-    uint32_t c = c0 + c1;
-    u64 none = 0;
-    block_excl<kDT>(c, none, L);
-    L.cnt[2 * tid] = c;
-    L.cnt[2 * tid + 1] = c + c0;
-    if (tid == kDT - 1) L.cnt[kBins] = c + c0 + c1;
-    __syncthreads();
+    count_prefix(L);
+    hi = last_bin(Ask{false, (uint32_t)k, 0.0}, L);
+    if (by_k && L.cnt[hi + 1] <= kList) n = sort_bins<TYPE>(row, V, rs, 0, hi, -1, L);
   }
   if (by_k || by_m) {
-    int hi;
-    if (by_k) hi = last_bin(Ask{false, (uint32_t)k, 0.0}, L);
-    else hi = min(kBins - 1, bin_of(rs, rs.m + T * __builtin_logf(mp)) + 1);  // (one more: the border is rounded)
-    int n = kList + 1;
-    if (L.cnt[hi + 1] <= kList) n = sort_bins<TYPE>(row, V, rs, 0, hi, -1, L);
-    // (should the border be further off than the bins tell, the last token listed passes it)
-    if (by_m && n <= kList && n < (int)L.cnt[kBins] && e44(rs, key_logit((uint32_t)(L.comp[n - 1] >> 24))) >= mp44)
-      n = kList + 1;
     if (n <= kList) {
       const int nk = by_k ? min(k, n) : n;
       const u64 Z = L.lmass[nk];
       if (tid == 0) L.found = 0;
       __syncthreads();
+      int best = -1;
       for (int i = tid; i < nk; i += kDT) {
         const double e = e44(rs, key_logit((uint32_t)(L.comp[i] >> 24)));
-        if ((!(tp < 1.0f) || (double)L.lmass[i] <= (double)(tp > 0.0f ? tp : 0.0f) * (double)Z) && e >= mp44)
-          atomicMax(&L.found, i);
+        if ((!(tp < 1.0f) || (double)L.lmass[i] <= (double)(tp > 0.0f ? tp : 0.0f) * (double)Z) && e >= mp44) best = i;
       }
+      raise(&L.found, best);
       __syncthreads();
       const int kept = L.found + 1;  // (ranks qualify up to a last one; rank 0 stays in any case)
       const u64 S = L.lmass[kept];
@@ -525,6 +553,7 @@ __global__ __launch_bounds__(kDT) void draw_row_kernel(DrawArgs a) {
     }
   }
 
+  __syncthreads();
   u64 mm = 0;  // the mass of the tokens with e >= min_p
   const double border_m = mp <= 0.0f ? __builtin_inf() : mp44;
   each_token<TYPE>(row, V, [&](int, float l, bool) {
@@ -570,8 +599,10 @@ __global__ __launch_bounds__(kDT) void draw_row_kernel(DrawArgs a) {
       if (far > d1) {
         if (tid == 0) L.found = 0;
         __syncthreads();
+        int best = -1;
         for (int i = tid; i < n; i += kDT)
-          if (bin_of(rs, key_logit((uint32_t)(L.comp[i] >> 24))) <= d1) atomicMax(&L.found, i + 1);
+          if (bin_of(rs, key_logit((uint32_t)(L.comp[i] >> 24))) <= d1) best = i + 1;
+        raise(&L.found, best);
         __syncthreads();
         split = L.found;
         __syncthreads();

@@ -493,8 +493,8 @@ __global__ __launch_bounds__(kDT) void draw_row_kernel(DrawArgs a) {
   rs.s2 = 1.0f;
   if (lo < m) {
     const float span = m - lo, x = span * rs.s1;
-    if (!(x >= (float)kFine)) rs.s1 = (float)(kFine - 1) / span;  // a narrow row spreads over the fine bins
-    else if (x > (float)kBins) rs.s2 = (float)(kBins - kFine - 1) / (x - (float)kFine);
+    if (!(x >= (float)kBins)) rs.s1 = (float)(kBins - 1) / span;  // a narrow row spreads over all bins
+    else rs.s2 = (float)(kBins - kFine - 1) / (x - (float)kFine);
   }
   rs.s1 = fminf(rs.s1, 1e38f);  // (so that 0 stays bin 0)
   rs.c2 = (float)kFine - (float)kFine * rs.s2;

@@ -56,8 +56,10 @@ DeltaArgs delta_args(const dfssm_delta* d) {
 }
 
 // Prompts that run token by token: too few tokens for a chunk's fixed work. The lengths behind cu_seqlens are
-// on the device, so the rule there goes by all tokens, which any one sequence may have.
-constexpr int kTokenPath = 8;
+// on the device, so the rule there goes by all tokens, which any one sequence may have. 64 heads of 64 x 128, token
+// by token and in chunks: 32 sequences of 8 tokens 49 and 78 us, 12: 66 and 79, 16: 82 and 79; one sequence of 8
+// tokens 20.3 and 23.6 us, 32: 23.0 and 23.5.
+constexpr int kTokenPath = 12;
 bool by_tokens(const DeltaArgs& a) { return (a.cu ? a.n_tokens : a.len) <= kTokenPath; }
 
 }  // namespace

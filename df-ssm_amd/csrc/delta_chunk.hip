@@ -4,8 +4,16 @@
 // row factors r_i that undo a normalisation or a power-of-two scaling of k_i or q_i:
 //   A_ij = beta_i k_i.k_j e^{G_i - G_j} (i > j),  T = (I + A)^-1 diag(beta),  P_ij = scale q_i.k_j e^{G_i - G_j} (i >= j)
 //   U = T (V - diag(e^G) K S0^T);  O = diag(scale e^G) Q S0^T + P U;  S1 = e^{G_C} S0 + (diag(e^{G_C - G}) U)^T K
-// Two launches: delta_prep_kernel makes T and P of all chunks in parallel, delta_chain_kernel walks the chunks
-// of a sequence and head with its state in registers.
+// Two launches: delta_prep_kernel makes T and the row factors of all chunks in parallel, delta_chain_kernel walks the
+// chunks of a sequence and head with its state in registers and makes P, which is less work than reading it, beside
+// them.
+//
+// What bounds it. One long sequence: the path from chunk to chunk (K S^T, T (V - ..), the new state: three dependent
+// products with a split into 16-bit parts before each), 5500 clocks a chunk; 16411 tokens x 64 heads of 64 x 128 take
+// 0.61 ms, 0.09 of it the preparation (fp16; 403 MB, so 82 us of copying). Many sequences: the instructions of the
+// waves that make P and the outputs, 8000 clocks a chunk of 64 value columns with two workgroups to a CU: 64 x 512
+// tokens x 80 heads 0.99 ms, 0.28 of it the preparation (bf16; 2.35 GB, 0.48 ms of copying; 206 GFLOP of the
+// recurrence, 0.18 ms of matrix products).
 //
 // Numbers. States, sums and everything between products are fp32. Products run on the 16-bit matrix cores with
 // fp32 accumulation. q and k are exact operands there, in their own type. A factor of fp32 values is a sum of
@@ -452,8 +460,8 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(256) void d
 //   NW waves, the chain proper: K S^T, U and the new state
 //   NW waves, the outputs: Q S^T, P U
 //   the fetchers: this chunk's P = tril(Q K^T ..), a fragment or two each, and the next one's operands, straight
-//   into LDS. Waves of their own, as many as make eight in all; with NW = 4 the output waves do it beside their work (12 waves would be three to a SIMD and have
-//   168 registers each, and the chain needs 224).
+//   into LDS. Waves of their own, as many as make eight in all; with NW = 4 the output waves do it beside their work
+//   (12 waves would be three to a SIMD and have 168 registers each, and the chain needs 224).
 // So waves of different kinds share a SIMD, products of one fill the gaps of the other, and only what the state
 // needs is on the path from chunk to chunk.
 // Result row 4 g + i of tile 2 j + h is k's column 32 j + 8 g + 4 h + i, so that a lane's part of a 32-deep
@@ -983,8 +991,12 @@ hipError_t launch_chunked(const DeltaArgs& a, void* ws, hipStream_t s) {
   ChunkRec* r = (ChunkRec*)ws;
   for (int64_t s0 = 0; s0 < slots; s0 += per) {
     const int64_t n = s0 + per < slots ? per : slots - s0;
-    const int64_t tasks = n * ng, resident = 512;  // two workgroups to a CU
+    const int64_t tasks = n * ng, resident = 512;  // two workgroups to a CU (256: 631 us for 615, 1024: 617)
     hipLaunchKernelGGL((delta_prep_kernel<DK, BF>), dim3((unsigned)(tasks < resident ? tasks : resident)), dim3(256), 0, s, a, r, s0, tasks);
+    // Few heads: a value column tile to a workgroup, so that all CUs have one or two and a chunk passes quickly. Many:
+    // four, which make P once for 64 columns. NW = 1, 2, 4: 64 heads of 4 tiles, 16411 tokens 615, 700 and 972 us; 12 x 2
+    // heads of 8 tiles 243, 268 and 360; 12 x 64 heads of 4, ragged, 388, 280 and 269; 64 x 80 heads of 4 tiles 1922, 1240
+    // and 1020.
     if (heads * ((tiles + 1) / 2) <= 256) launch_chain<DK, BF, 1>(a, r, s0, s0 + n, s);
     else if (heads * ((tiles + 3) / 4) <= 256) launch_chain<DK, BF, 2>(a, r, s0, s0 + n, s);
     else launch_chain<DK, BF, 4>(a, r, s0, s0 + n, s);

@@ -12,11 +12,17 @@
 //
 // One workgroup per row. The row is spread over 2048 bins of falling logit (a monotone map, so bins are ranges of
 // the ranking) whose counts, and masses where all tokens' matter, are summed by LDS atomics.
-//   Few kept: with a top_k (or only a min_p) the first bins hold all that can be kept. If that is at most 2048
-//   tokens they are gathered into LDS and sorted, and nothing but they needs an exponential.
+//   Few kept: with a top_k, or only a min_p, the first bins hold all that can be kept. They are gathered into LDS
+//   and sorted, if they are at most 2046 tokens, and nothing but they needs an exponential.
 //   Else every token's mass goes into its bin, and a search takes its bin from the prefix sums and resolves it
-//   there: the bin's tokens gathered and sorted, or, where they are more than 2048, found by the exact 32-bit
+//   there: the bin's tokens gathered and sorted, or, where they are more than 2046, found by the exact 32-bit
 //   order key and the index, a byte at a time over the row.
+//
+// What bounds it. Few kept: two passes over the logits, 256 rows of 131072 fp16, top_k 50: 28 us (67 MB, 4.8 TB/s of
+// a pass's bytes). Else the arithmetic of the masses, about 30 instructions a token of which 11 are fp64, and the LDS
+// atomics beside them: a pass of 50288 tokens takes 12 us, of the 29 that one row takes in all; a row has the
+// arithmetic of one compute unit only, as every part of it needs the sums of the others four times over.
+// 256 rows of 131072 fp32 with settings of all kinds: 86 us.
 #include "common.h"
 #include "dfssm.h"
 #include "dfssm_kernels.h"
@@ -206,8 +212,10 @@ __device__ __forceinline__ int sort_bins(const void* row, int V, const RowScale 
   const int n = L.nlist;
   if (n > kList) return n;
   if (n <= kDT / 2) {
-    // A token's rank is the number of smaller entries: kDT / n threads count for each, over parts of the list. (No
-    // barriers between, as the stages of a sorting network have; its work grows with the square.)
+    // A token's rank is the number of smaller entries: kDT / n threads count for each, over parts of the list. No
+    // barriers between, as the stages of a sorting network have, but its work grows with the square: a whole draw from
+    // a row of 50288 with a list of 20 tokens takes 13.2 us this way and 21.5 by the network, 220: 17.7 and 24.4,
+    // 490: 26.2 and 26.5.
     int parts = kDT / max(n, 1);
     parts = parts > 16 ? 16 : parts;
     const int i = tid % max(n, 1), part = tid / max(n, 1);
@@ -218,7 +226,15 @@ __device__ __forceinline__ int sort_bins(const void* row, int V, const RowScale 
       own = L.comp[i];
       const int per = (n + parts - 1) / parts, from = part * per, to = min(n, from + per);
       int r = 0;
-      for (int q = from; q < to; ++q) r += L.comp[q] < own ? 1 : 0;
+      int q = from;
+      for (; q + 8 <= to; q += 8) {
+        u64 x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = L.comp[q + e];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r += x[e] < own ? 1 : 0;
+      }
+      for (; q < to; ++q) r += L.comp[q] < own ? 1 : 0;
       if (r) atomicAdd(&L.rank[i], r);
     }
     __syncthreads();
@@ -504,7 +520,9 @@ __global__ __launch_bounds__(kDT) void draw_row_kernel(DrawArgs a) {
   // What can be kept lies in the first bins if there is a top_k, or a min_p and no top_p (whose mass is that of all).
   const bool by_k = limit && k <= kList, by_m = !limit && mp > 0.0f && mp <= 1.0f && !(tp < 1.0f);
   // A bin that has k threads' largest tokens in it or before it has the first k ranks too. That is nearly the bin of
-  // rank k while k is small beside the threads (k = 512: 0.7 tokens a thread, 710 in all), and needs no pass.
+  // rank k while k is small beside the threads (k = 512: 0.7 tokens a thread, 710 in all), and needs no pass to
+  // count. 256 rows of 131072, with and without: k = 20 27 and 37 us, 200: 31 and 40, 512: 43 and 53; at 700 and more
+  // both count (54 us; the list is then more often too long than not).
   const bool by_own = limit && k <= kDT / 2;
   int hi = kBins - 1, n = kList + 1;
   if (by_m) hi = bin_of(rs, rs.m + T * (__builtin_logf(mp) * 1.0001f - 1e-6f));  // (what passes min_p lies before it)

@@ -18,11 +18,12 @@
 //   there: the bin's tokens gathered and sorted, or, where they are more than 2046, found by the exact 32-bit
 //   order key and the index, a byte at a time over the row.
 //
-// What bounds it. Few kept: two passes over the logits, 256 rows of 131072 fp16, top_k 50: 28 us (67 MB, 4.8 TB/s of
-// a pass's bytes). Else the arithmetic of the masses, about 30 instructions a token of which 11 are fp64, and the LDS
-// atomics beside them: a pass of 50288 tokens takes 12 us, of the 29 that one row takes in all; a row has the
-// arithmetic of one compute unit only, as every part of it needs the sums of the others four times over.
-// 256 rows of 131072 fp32 with settings of all kinds: 86 us.
+// What bounds it. Few kept: two passes over the logits, 256 rows of 131072 fp16, top_k 50, 27 us (67 MB, 5 TB/s of the
+// passes' bytes); one row of 50288 takes 11 to 13 us, two reads of its logits and a dozen barriers one after the other. Else the
+// arithmetic of the masses, about 30 instructions a token of which 11 are fp64, and the LDS atomics beside them: one
+// row of 50288 takes 29 us, 12 of them that pass, as it has the arithmetic of one compute unit. 256 rows of 131072 fp32
+// with settings of all kinds: 87 us. Spreading a row over up to 24 workgroups (three launches, bins summed in global
+// memory) took 28 us for that one row and 19 for one with top_k 20, which takes 11 this way.
 #include "common.h"
 #include "dfssm.h"
 #include "dfssm_kernels.h"
@@ -147,49 +148,56 @@ struct DrawLds {
   uint32_t wc[kDT / 64];
   u64 wm[kDT / 64];
   float wf[kDT / 64], wg[kDT / 64];
-  int found, nlist;
+  int found, nlist, at[2];
   uint32_t rcnt;
   u64 rmass;
 };
 
-__device__ __forceinline__ u64 shfl_up64(u64 v, int o) {
-  const uint32_t lo = (uint32_t)__shfl_up((int)(uint32_t)v, o, 64), hi = (uint32_t)__shfl_up((int)(uint32_t)(v >> 32), o, 64);
-  return ((u64)hi << 32) | lo;
+// v plus the values of the lanes before (inclusive prefix over the wave), moved within rows of 16 lanes and from row to
+// row by the register file's own paths. (By lane shuffles through LDS a block's prefix took three times as long.)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t moved(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, true);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ void scan_step(uint32_t& v) { v += moved<CTRL, ROWS>(v); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ void scan_step(u64& v) {
+  v += ((u64)moved<CTRL, ROWS>((uint32_t)(v >> 32)) << 32) | moved<CTRL, ROWS>((uint32_t)v);
+}
+template <class X>
+__device__ __forceinline__ X wave_scan(X v) {
+  scan_step<0x111, 0xf>(v);  // from 1, 2, 4 and 8 lanes before, in the row
+  scan_step<0x112, 0xf>(v);
+  scan_step<0x114, 0xf>(v);
+  scan_step<0x118, 0xf>(v);
+  scan_step<0x142, 0xa>(v);  // row 0's last to row 1, 2's to 3; then lane 31's to rows 2 and 3
+  scan_step<0x143, 0xc>(v);
+  return v;
 }
 
-// Exclusive prefix over the block's threads of (c, m); NT threads take part, all call.
-template <int NT>
-__device__ __forceinline__ void block_excl(uint32_t& c, u64& m, DrawLds& L) {
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  uint32_t ci = c;
-  u64 mi = m;
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t x = (uint32_t)__shfl_up((int)ci, o, 64);
-    const u64 y = shfl_up64(mi, o);
-    if (lane >= o) {
-      ci += x;
-      mi += y;
-    }
-  }
-  if (lane == 63 && w < NT / 64) {
-    L.wc[w] = ci;
-    L.wm[w] = mi;
+// Exclusive prefix over the block's threads, of which the first NT hold values; all call. total: of all.
+template <int NT, class X>
+__device__ __forceinline__ X block_excl(X v, X* waves, X& total) {
+  const int tid = threadIdx.x, w = tid >> 6;
+  const X in = wave_scan(v);
+  if ((tid & 63) == 63 && w < NT / 64) waves[w] = in;
+  __syncthreads();
+  X before = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < NT / 64; ++i) {
+    if (i == w) before = all;
+    all += waves[i];
   }
   __syncthreads();
-  c = ci - c;
-  m = mi - m;
-  for (int i = 0; i < NT / 64; ++i)
-    if (i < w) {
-      c += L.wc[i];
-      m += L.wm[i];
-    }
-  __syncthreads();
+  total = all;
+  return (NT == kDT || w < NT / 64 ? before : all) + in - v;
 }
 
-// The tokens of bins lo .. hi and of bin far > hi (or -1) into L.comp, sorted, and the masses ranked above them
-// within the list into L.lmass. Returns how many they are; more than kList: nothing is listed.
+// The tokens of bins lo .. hi and of bin far > hi (or -1) into L.comp, in any order. Returns how many they are; what
+// exceeds kList is not listed.
 template <int TYPE>
-__device__ __forceinline__ int sort_bins(const void* row, int V, const RowScale rs, int lo, int hi, int far, DrawLds& L) {
+__device__ __forceinline__ int gather(const void* row, int V, const RowScale rs, int lo, int hi, int far, DrawLds& L) {
   const int tid = threadIdx.x;
   if (tid == 0) L.nlist = 0;
   __syncthreads();
@@ -209,13 +217,41 @@ __device__ __forceinline__ int sort_bins(const void* row, int V, const RowScale 
     }
   });
   __syncthreads();
-  const int n = L.nlist;
-  if (n > kList) return n;
+  return L.nlist;
+}
+
+// Sorts L.comp's first n <= kList entries and puts the masses ranked above each within the list into L.lmass.
+__device__ __forceinline__ void sort_list(int n, const RowScale rs, DrawLds& L) {
+  const int tid = threadIdx.x;
+  if (n <= 64) {  // by one wave, with no barrier until the end
+    if (tid < 64) {
+      const u64 own = tid < n ? L.comp[tid] : ~0ull;
+      int r = 0;
+      for (int q = 0; q < n; ++q) {
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)own, q);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(own >> 32), q);
+        r += (((u64)hi << 32) | lo) < own ? 1 : 0;
+      }
+      const u64 E = tid < n ? mass_of(e44(rs, key_logit((uint32_t)(own >> 24)))) : 0;
+      if (tid < n) {
+        L.comp[r] = own;
+        L.lmass[r] = E;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      const u64 mine = tid < n ? L.lmass[tid] : 0, upto = wave_scan(mine);
+      if (tid < n) L.lmass[tid] = upto - mine;
+      if (tid == 63) L.lmass[n] = upto;
+    }
+    __syncthreads();
+    return;
+  }
   if (n <= kDT / 2) {
     // A token's rank is the number of smaller entries: kDT / n threads count for each, over parts of the list. No
     // barriers between, as the stages of a sorting network have, but its work grows with the square: a whole draw from
-    // a row of 50288 with a list of 20 tokens takes 13.2 us this way and 21.5 by the network, 220: 17.7 and 24.4,
-    // 490: 26.2 and 26.5.
+    // a row of 50288 with a list of 20 tokens takes 13.2 us this way, 21.5 by the network and 10.9 by one wave; 220: 17.7
+    // and 24.4, 490: 26.2 and 26.5.
     int parts = kDT / max(n, 1);
     parts = parts > 16 ? 16 : parts;
     const int i = tid % max(n, 1), part = tid / max(n, 1);
@@ -265,14 +301,18 @@ __device__ __forceinline__ int sort_bins(const void* row, int V, const RowScale 
     const int i = 2 * tid + q;
     m[q] = i < n ? mass_of(e44(rs, key_logit((uint32_t)(L.comp[i] >> 24)))) : 0;
   }
-  uint32_t c = 0;
-  u64 s = m[0] + m[1];
-  block_excl<kDT>(c, s, L);
+  u64 all;
+  const u64 s = block_excl<kDT>(m[0] + m[1], L.wm, all);
   if (2 * tid <= n) {  // (one entry more: the list's mass)
     L.lmass[2 * tid] = s;
     L.lmass[2 * tid + 1] = s + m[0];
   }
   __syncthreads();
+}
+template <int TYPE>
+__device__ __forceinline__ int sort_bins(const void* row, int V, const RowScale rs, int lo, int hi, int far, DrawLds& L) {
+  const int n = gather<TYPE>(row, V, rs, lo, hi, far, L);
+  if (n <= kList) sort_list(n, rs, L);
   return n;
 }
 
@@ -281,12 +321,24 @@ __device__ __forceinline__ void count_prefix(DrawLds& L) {
   const int tid = threadIdx.x;
   __syncthreads();
   const uint32_t c0 = L.cnt[2 * tid], c1 = L.cnt[2 * tid + 1];
-  uint32_t c = c0 + c1;
-  u64 none = 0;
-  block_excl<kDT>(c, none, L);
+  uint32_t all;
+  const uint32_t c = block_excl<kDT>(c0 + c1, L.wc, all);
   L.cnt[2 * tid] = c;
   L.cnt[2 * tid + 1] = c + c0;
-  if (tid == kDT - 1) L.cnt[kBins] = c + c0 + c1;
+  if (tid == 0) L.cnt[kBins] = all;
+  __syncthreads();
+}
+
+// L.mass: the same for masses.
+__device__ __forceinline__ void mass_prefix(DrawLds& L) {
+  const int tid = threadIdx.x;
+  __syncthreads();
+  const u64 m0 = L.mass[2 * tid], m1 = L.mass[2 * tid + 1];
+  u64 all;
+  const u64 m = block_excl<kDT>(m0 + m1, L.wm, all);
+  L.mass[2 * tid] = m;
+  L.mass[2 * tid + 1] = m + m0;
+  if (tid == 0) L.mass[kBins] = all;
   __syncthreads();
 }
 
@@ -307,44 +359,45 @@ __device__ __forceinline__ Found found(u64 above, u64 comp, const RowScale rs) {
   return Found{above, mass_of(e44(rs, key_logit(key))), key, (uint32_t)(comp & 0xffffffu)};
 }
 
-// max of what the lanes hold, one atomic per wave (one address: lane by lane they would queue up).
-__device__ __forceinline__ void raise(int* to, int v) {
-  for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
-  if ((threadIdx.x & 63) == 0 && v >= 0) atomicMax(to, v);
-}
-
-// The last bin in use whose first token qualifies. By mass, a bin without mass is not in use: what lies there
-// comes after all that a mass can ask for.
-__device__ __forceinline__ int last_bin(const Ask q, DrawLds& L) {
-  const int tid = threadIdx.x;
-  if (tid == 0) L.found = 0;
-  __syncthreads();
-  int best = -1;
+// The last bin in use whose first token qualifies. By mass, a bin without mass is not in use: what lies there comes
+// after all that a mass can ask for. Bins qualify up to a last one, which sees it by itself: the next one in use begins
+// where it ends. (x >= 0 and n >= 1: the first in use qualifies.) L.at[slot] has it after a barrier.
+__device__ __forceinline__ void mark_bin(const Ask q, int slot, DrawLds& L) {
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {  // a bin is empty where the next one's prefix is the same; bin 0 never is
-    const int b = 2 * tid + j;
-    const bool used = q.by_mass ? L.mass[b + 1] != L.mass[b] : L.cnt[b + 1] != L.cnt[b];
-    if (used && (q.by_mass ? q.holds(0, L.mass[b]) : q.holds(L.cnt[b], 0))) best = b;
+  for (int j = 0; j < 2; ++j) {
+    const int b = 2 * threadIdx.x + j;
+    bool it;
+    if (q.by_mass) {
+      const u64 m0 = L.mass[b], m1 = L.mass[b + 1];
+      it = m1 != m0 && q.holds(0, m0) && (!q.holds(0, m1) || m1 == L.mass[kBins]);
+    } else {
+      const uint32_t c0 = L.cnt[b], c1 = L.cnt[b + 1];
+      it = c1 != c0 && q.holds(c0, 0) && (!q.holds(c1, 0) || c1 == L.cnt[kBins]);
+    }
+    if (it) L.at[slot] = b;
   }
-  raise(&L.found, best);
+}
+__device__ __forceinline__ int last_bin(const Ask q, DrawLds& L) {
+  mark_bin(q, 0, L);
   __syncthreads();
-  const int bin = L.found;
+  const int bin = L.at[0];
   __syncthreads();
   return bin;
 }
-// The last of entries [from, to) of the list that qualifies; its masses are off by `base` (and its counts by above).
-__device__ __forceinline__ int last_entry(const Ask q, int from, int to, uint32_t above, u64 base, DrawLds& L) {
-  const int tid = threadIdx.x;
-  if (tid == 0) L.found = from;
+// The last i of [from, to) with f(i), true up to a last one; f(from) counts as true. All threads call; i into L.at[0].
+template <class F>
+__device__ __forceinline__ int last_true(int from, int to, DrawLds& L, F f) {
+  if (threadIdx.x == 0 && to <= from) L.at[0] = from;
+  for (int i = from + threadIdx.x; i < to; i += kDT)
+    if ((i == from || f(i)) && (i + 1 == to || !f(i + 1))) L.at[0] = i;
   __syncthreads();
-  int best = -1;
-  for (int i = from + tid; i < to; i += kDT)
-    if (q.holds(above + (uint32_t)(i - from), base + L.lmass[i])) best = i;
-  raise(&L.found, best);
-  __syncthreads();
-  const int i = L.found;
+  const int i = L.at[0];
   __syncthreads();
   return i;
+}
+// The last of entries [from, to) of the list that qualifies; its masses are off by `base` (and its counts by above).
+__device__ __forceinline__ int last_entry(const Ask q, int from, int to, uint32_t above, u64 base, DrawLds& L) {
+  return last_true(from, to, L, [&](int i) { return q.holds(above + (uint32_t)(i - from), base + L.lmass[i]); });
 }
 
 // One question resolved by the exact order key and the index, a byte at a time over the row (more tokens in the bin
@@ -373,11 +426,10 @@ __device__ __forceinline__ Found search_row(const Ask q, int bin, const void* ro
     __syncthreads();
     const uint32_t c0 = tid < 256 ? L.dcnt[tid] : 0;
     const u64 m0 = tid < 256 ? L.dmass[tid] : 0;
-    uint32_t c = c0;
-    u64 m = m0;
-    block_excl<256>(c, m, L);
-    c += above;
-    m += mass;
+    uint32_t call;
+    u64 mall;
+    const uint32_t c = block_excl<256>(c0, L.wc, call) + above;
+    const u64 m = block_excl<256>(m0, L.wm, mall) + mass;
     // the first digit in use qualifies always: its prefix was found to (by mass, the first with any)
     const bool first = q.by_mass ? m == mass : c == above;
     if (tid < 256 && (q.by_mass ? m0 != 0 : c0 != 0) && (q.holds(c, m) || first)) atomicMax(&L.found, tid);
@@ -411,95 +463,108 @@ __device__ __forceinline__ u64 wave_add64(u64 v) {
   return v;
 }
 
+// A row and its settings.
+template <int TYPE>
+struct Row {
+  const void* at;
+  int b, V, k;
+  float T, tp, mp, u;
+  bool limit;     // a top_k that leaves something out
+  bool by_k, by_m; // what can be kept lies in the first bins: a top_k, or a min_p and no top_p (whose mass is that of all)
+  double mp44, share;  // min_p and top_p, the latter as a factor
+  __device__ __forceinline__ Row(const DrawArgs& a, int row) : b(row), V(a.V) {
+    at = (const char*)a.logits + (size_t)b * a.ld * (TYPE == DFSSM_TYPE_F32 ? 4 : 2);
+    T = a.temperatures ? a.temperatures[b] : a.temperature;
+    k = a.top_ks ? a.top_ks[b] : a.top_k;
+    tp = a.top_ps ? a.top_ps[b] : a.top_p;
+    mp = a.min_ps ? a.min_ps[b] : a.min_p;
+    u = a.u[b];
+    u = u >= 0.0f ? (u < 1.0f ? u : 0.99999994f) : 0.0f;
+    limit = k > 0 && k < V;
+    by_k = limit && k <= kList;
+    by_m = !limit && mp > 0.0f && mp <= 1.0f && !(tp < 1.0f);
+    mp44 = (double)mp * kOne;
+    share = (double)(tp > 0.0f ? tp : 0.0f);
+  }
+  // The last bin that min_p can keep of (the bins are monotone).
+  __device__ __forceinline__ int min_bin(const RowScale rs) const {
+    return bin_of(rs, rs.m + T * (__builtin_logf(mp) * 1.0001f - 1e-6f));
+  }
+};
+
 // A row with +inf logits: each has mass 1 and nothing else any, ranked by index. Which of them is drawn comes from
 // their number; every thread counts those of a stretch of the row, and the one whose stretch holds it walks along.
 template <int TYPE>
-__device__ __forceinline__ void draw_inf(const DrawArgs& a, const void* row, int k, float tp, float mp, float u, DrawLds& L) {
-  const int tid = threadIdx.x, per = (a.V + kDT - 1) / kDT, from = min(a.V, tid * per), to = min(a.V, from + per);
+__device__ __forceinline__ void draw_inf(const DrawArgs& a, const Row<TYPE>& r, DrawLds& L) {
+  const int tid = threadIdx.x, per = (r.V + kDT - 1) / kDT, from = min(r.V, tid * per), to = min(r.V, from + per);
   uint32_t mine = 0;
-  for (int i = from; i < to; ++i) mine += logit_at<TYPE>(row, i) == __builtin_inff() ? 1 : 0;
-  uint32_t c = mine;
-  u64 none = 0;
-  block_excl<kDT>(c, none, L);
-  if (tid == kDT - 1) L.rcnt = c + mine;
-  __syncthreads();
-  int n = (int)L.rcnt;
-  if (k > 0) n = min(n, k);
-  if (tp < 1.0f) n = min(n, (int)((double)(tp > 0.0f ? tp : 0.0f) * (double)n) + 1);
-  if (!(mp <= 1.0f)) n = 1;
-  const uint32_t at = (uint32_t)min(n - 1, (int)((double)u * (double)n));
+  for (int i = from; i < to; ++i) mine += logit_at<TYPE>(r.at, i) == __builtin_inff() ? 1 : 0;
+  uint32_t all;
+  uint32_t c = block_excl<kDT>(mine, L.wc, all);
+  int n = (int)all;
+  if (r.k > 0) n = min(n, r.k);
+  if (r.tp < 1.0f) n = min(n, (int)(r.share * (double)n) + 1);
+  if (!(r.mp <= 1.0f)) n = 1;
+  const uint32_t at = (uint32_t)min(n - 1, (int)((double)r.u * (double)n));
   if (at < c || at >= c + mine) return;
   for (int i = from; i < to; ++i)
-    if (logit_at<TYPE>(row, i) == __builtin_inff() && c++ == at) {
-      a.next[blockIdx.x] = i;
-      if (a.logprob) a.logprob[blockIdx.x] = (float)-log((double)n);
+    if (logit_at<TYPE>(r.at, i) == __builtin_inff() && c++ == at) {
+      a.next[r.b] = i;
+      if (a.logprob) a.logprob[r.b] = (float)-log((double)n);
     }
 }
 
+// The largest logit of the block's tokens, and nearly the least finite one (of one in each load: only the bins' width
+// comes from it). L.wf and L.wg are written; a barrier later block_range has the two.
 template <int TYPE>
-__global__ __launch_bounds__(kDT) void draw_row_kernel(DrawArgs a) {
-  __shared__ DrawLds L;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, b = blockIdx.x, V = a.V;
-  const void* row = (const char*)a.logits + (size_t)b * a.ld * (TYPE == DFSSM_TYPE_F32 ? 4 : 2);
-  const float T = a.temperatures ? a.temperatures[b] : a.temperature;
-  const int k = a.top_ks ? a.top_ks[b] : a.top_k;
-  const float tp = a.top_ps ? a.top_ps[b] : a.top_p;
-  const float mp = a.min_ps ? a.min_ps[b] : a.min_p;
-  float u = a.u[b];
-  u = u >= 0.0f ? (u < 1.0f ? u : 0.99999994f) : 0.0f;
-
-  // the largest logit, and nearly the least finite one (of one in each load: only the bins' width comes from it)
+__device__ __forceinline__ float scan_range(const void* row, int V, DrawLds& L) {
+  const int tid = threadIdx.x;
   float m = -__builtin_inff(), lo = __builtin_inff();
   each_token<TYPE>(row, V, [&](int, float l, bool first) {
     m = fmaxf(m, l);  // (of a NaN and a number, the number)
     if (first && l < lo && l > -__builtin_inff()) lo = l;
   });
-  for (int i = tid; i < kBins; i += kDT) {
-    L.cnt[i] = 0;
-    L.mass[i] = 0;
-  }
-  if (tid < 64) L.ends[tid] = tid < 32 ? exp2((double)tid * (1.0 / 32)) * kOne : exp2((double)(tid - 32) * (1.0 / kTab));
   const float own = m;  // of this thread's tokens
   for (int o = 32; o > 0; o >>= 1) {
     m = fmaxf(m, __shfl_xor(m, o, 64));
     lo = fminf(lo, __shfl_xor(lo, o, 64));
   }
-  if (lane == 0) {
-    L.wf[w] = m;
-    L.wg[w] = lo;
+  if ((tid & 63) == 0) {
+    L.wf[tid >> 6] = m;
+    L.wg[tid >> 6] = lo;
   }
-  if (tid == 0) {
-    L.found = 0x7fffffff;
-    L.rcnt = 0;
-    L.rmass = 0;
-    L.cnt[kBins] = 0;
-    L.mass[kBins] = 0;
-  }
-  __syncthreads();
+  return own;
+}
+__device__ __forceinline__ void block_range(float& m, float& lo, const DrawLds& L) {
   m = L.wf[0];
   lo = L.wg[0];
   for (int i = 1; i < kDT / 64; ++i) {
     m = fmaxf(m, L.wf[i]);
     lo = fminf(lo, L.wg[i]);
   }
-  L.tab[tid] = L.ends[tid >> 5] * L.ends[32 + (tid & 31)];
+}
+
+// Clears the bins and begins the exponential's table, whose entries are products of two; a barrier later table_finish.
+__device__ __forceinline__ void start(DrawLds& L) {
+  const int tid = threadIdx.x;
+  for (int i = tid; i < kBins; i += kDT) {
+    L.cnt[i] = 0;
+    L.mass[i] = 0;
+  }
+  if (tid < 64) L.ends[tid] = tid < 32 ? exp2((double)tid * (1.0 / 32)) * kOne : exp2((double)(tid - 32) * (1.0 / kTab));
+  if (tid == 0) {
+    L.rcnt = 0;
+    L.rmass = 0;
+    L.cnt[kBins] = 0;
+    L.mass[kBins] = 0;
+  }
+}
+__device__ __forceinline__ void table_finish(DrawLds& L) {
+  L.tab[threadIdx.x] = L.ends[threadIdx.x >> 5] * L.ends[32 + (threadIdx.x & 31)];
   static_assert(kTab == kDT && kTab == 32 * 32, "an entry per thread");
-  if (m == -__builtin_inff() || !(T > 0.0f)) {  // nothing to draw from; greedy
-    const bool none = m == -__builtin_inff();
-    if (!none) each_token<TYPE>(row, V, [&](int i, float l, bool) {
-      if (l == m) atomicMin(&L.found, i);
-    });
-    __syncthreads();
-    if (tid == 0) {
-      a.next[b] = none ? -1 : L.found;
-      if (a.logprob) a.logprob[b] = none ? -__builtin_inff() : 0.0f;
-    }
-    return;
-  }
-  if (m == __builtin_inff()) {
-    draw_inf<TYPE>(a, row, k, tp, mp, u, L);
-    return;
-  }
+}
+
+__device__ __forceinline__ RowScale scale_of(float m, float lo, float T, const DrawLds& L) {
   RowScale rs;
   rs.m = m;
   rs.y1 = kTab * 1.4426950408889634074 / (double)T;
@@ -514,140 +579,185 @@ __global__ __launch_bounds__(kDT) void draw_row_kernel(DrawArgs a) {
   }
   rs.s1 = fminf(rs.s1, 1e38f);  // (so that 0 stays bin 0)
   rs.c2 = (float)kFine - (float)kFine * rs.s2;
+  return rs;
+}
 
-  const bool limit = k > 0 && k < V;
-  const double mp44 = (double)mp * kOne;
-  // What can be kept lies in the first bins if there is a top_k, or a min_p and no top_p (whose mass is that of all).
-  const bool by_k = limit && k <= kList, by_m = !limit && mp > 0.0f && mp <= 1.0f && !(tp < 1.0f);
-  // A bin that has k threads' largest tokens in it or before it has the first k ranks too. That is nearly the bin of
-  // rank k while k is small beside the threads (k = 512: 0.7 tokens a thread, 710 in all), and needs no pass to
-  // count. 256 rows of 131072, with and without: k = 20 27 and 37 us, 200: 31 and 40, 512: 43 and 53; at 700 and more
-  // both count (54 us; the list is then more often too long than not).
-  const bool by_own = limit && k <= kDT / 2;
-  int hi = kBins - 1, n = kList + 1;
-  if (by_m) hi = bin_of(rs, rs.m + T * (__builtin_logf(mp) * 1.0001f - 1e-6f));  // (what passes min_p lies before it)
-  if (by_own) {
-    if (taken(rs, own)) atomicAdd(&L.cnt[bin_of(rs, own)], 1u);
-    count_prefix(L);
-    if (L.cnt[kBins] >= (uint32_t)k) hi = last_bin(Ask{false, (uint32_t)k, 0.0}, L);
-  }
-  if (by_own || by_m) {
-    __syncthreads();
-    n = sort_bins<TYPE>(row, V, rs, 0, hi, -1, L);
-  }
-  if (limit && n > kList) {
-    for (int i = tid; i < kBins; i += kDT) L.cnt[i] = 0;
-    __syncthreads();
-    each_token<TYPE>(row, V, [&](int, float l, bool) {
-      if (taken(rs, l)) atomicAdd(&L.cnt[bin_of(rs, l)], 1u);
-    });
-    count_prefix(L);
-    hi = last_bin(Ask{false, (uint32_t)k, 0.0}, L);
-    if (by_k && L.cnt[hi + 1] <= kList) n = sort_bins<TYPE>(row, V, rs, 0, hi, -1, L);
-  }
-  if (by_k || by_m) {
-    if (n <= kList) {
-      const int nk = by_k ? min(k, n) : n;
-      const u64 Z = L.lmass[nk];
-      if (tid == 0) L.found = 0;
-      __syncthreads();
-      int best = -1;
-      for (int i = tid; i < nk; i += kDT) {
-        const double e = e44(rs, key_logit((uint32_t)(L.comp[i] >> 24)));
-        if ((!(tp < 1.0f) || (double)L.lmass[i] <= (double)(tp > 0.0f ? tp : 0.0f) * (double)Z) && e >= mp44) best = i;
-      }
-      raise(&L.found, best);
-      __syncthreads();
-      const int kept = L.found + 1;  // (ranks qualify up to a last one; rank 0 stays in any case)
-      const u64 S = L.lmass[kept];
-      __syncthreads();
-      const int i = last_entry(Ask{true, 0u, (double)u * (double)S}, 0, kept, 0, 0, L);
-      if (tid == 0) {
-        const u64 c = L.comp[i];
-        a.next[b] = (int64_t)(c & 0xffffffu);
-        if (a.logprob) a.logprob[b] = (float)log(e44(rs, key_logit((uint32_t)(c >> 24))) / (double)S);
-      }
-      return;
-    }
-  }
-
-  __syncthreads();
-  u64 mm = 0;  // the mass of the tokens with e >= min_p
-  const double border_m = mp <= 0.0f ? __builtin_inf() : mp44;
+// Counts or masses of the block's tokens into its bins (and L.rmass: the mass of the tokens with e >= min_p).
+template <int TYPE>
+__device__ __forceinline__ void count_tokens(const void* row, int V, const RowScale rs, DrawLds& L) {
+  each_token<TYPE>(row, V, [&](int, float l, bool) {
+    if (taken(rs, l)) atomicAdd(&L.cnt[bin_of(rs, l)], 1u);
+  });
+}
+template <int TYPE>
+__device__ __forceinline__ void add_masses(const void* row, int V, const Row<TYPE>& r, const RowScale rs, DrawLds& L) {
+  u64 mm = 0;
+  const double border = r.mp <= 0.0f ? __builtin_inf() : r.mp44;
   each_token<TYPE>(row, V, [&](int, float l, bool) {
     if (!(rs.m - l <= rs.reach)) return;
     const double e = e44(rs, l);
     const u64 E = mass_of(e);
     atomicAdd(&L.mass[bin_of(rs, l)], E);
-    if (e >= border_m) mm += E;
+    if (e >= border) mm += E;
   });
   mm = wave_add64(mm);
-  if (lane == 0) atomicAdd(&L.rmass, mm);
+  if ((threadIdx.x & 63) == 0) atomicAdd(&L.rmass, mm);
+}
+// Of min_p's tokens (rank 0 is kept in any case).
+__device__ __forceinline__ u64 min_mass(float mp, u64 mm) { return mp <= 0.0f ? ~0ull : mm > kUnit ? mm : kUnit; }
+
+template <int TYPE>
+__device__ __forceinline__ void answer(const DrawArgs& a, const Row<TYPE>& r, const RowScale rs, u64 comp, u64 S) {
+  if (threadIdx.x == 0) {
+    a.next[r.b] = (int64_t)(comp & 0xffffffu);
+    if (a.logprob) a.logprob[r.b] = (float)log(e44(rs, key_logit((uint32_t)(comp >> 24))) / (double)S);
+  }
+}
+
+// The draw where the sorted list holds all that can be kept.
+template <int TYPE>
+__device__ __forceinline__ void pick_few(const DrawArgs& a, const Row<TYPE>& r, const RowScale rs, int n, DrawLds& L) {
+  const int nk = r.by_k ? min(r.k, n) : n;
+  const u64 Z = L.lmass[nk];
+  const int kept = 1 + last_true(0, nk, L, [&](int i) {
+    return (!(r.tp < 1.0f) || (double)L.lmass[i] <= r.share * (double)Z) &&
+           e44(rs, key_logit((uint32_t)(L.comp[i] >> 24))) >= r.mp44;
+  });
+  const u64 S = L.lmass[kept];
+  const int i = last_entry(Ask{true, 0u, (double)r.u * (double)S}, 0, kept, 0, 0, L);
+  answer(a, r, rs, L.comp[i], S);
+}
+
+// The draw by masses from one list, S the mass before top_p: top_p's border lies in one bin, `far`, which bounds the kept
+// mass, and so the bins that the drawn token may lie in, d0 .. d1.
+struct Plan {
+  int d0, d1, far;
+};
+template <int TYPE>
+__device__ __forceinline__ Plan plan(const Row<TYPE>& r, u64 S, u64 M_m, DrawLds& L) {
+  Plan p{0, 0, -1};
+  u64 s0 = S < M_m ? S : M_m, s1 = s0;
+  if (r.tp < 1.0f) {
+    p.far = last_bin(Ask{true, 0u, r.share * (double)S}, L);
+    s0 = max(min(s0, L.mass[p.far]), (u64)1);
+    s1 = min(s1, L.mass[p.far + 1]);
+  }
+  mark_bin(Ask{true, 0u, (double)r.u * (double)s0}, 0, L);
+  mark_bin(Ask{true, 0u, (double)r.u * (double)s1}, 1, L);
   __syncthreads();
-  // (rank 0 is kept in any case)
-  const u64 M_m = mp <= 0.0f ? ~0ull : L.rmass > kUnit ? L.rmass : kUnit;
-  const u64 m0 = L.mass[2 * tid], m1 = L.mass[2 * tid + 1];
-  uint32_t c = 0;
-  u64 ms = m0 + m1;
-  block_excl<kDT>(c, ms, L);
-  L.mass[2 * tid] = ms;
-  L.mass[2 * tid + 1] = ms + m0;
-  if (tid == kDT - 1) L.mass[kBins] = ms + m0 + m1;
+  p.d0 = L.at[0];
+  p.d1 = L.at[1];
   __syncthreads();
+  return p;
+}
+template <int TYPE>
+__device__ __forceinline__ void pick_planned(const DrawArgs& a, const Row<TYPE>& r, const RowScale rs, const Plan p, int n,
+                                             u64 S, u64 M_m, DrawLds& L) {
+  int split = n;  // entries before it are of d0 .. d1; those of far follow, their masses counted from far's own start
+  if (r.tp < 1.0f) {
+    const Ask border{true, 0u, r.share * (double)S};
+    u64 base = L.mass[p.d0];
+    int from = 0;
+    if (p.far > p.d1) {
+      from = split = 1 + last_true(0, n, L, [&](int i) { return bin_of(rs, key_logit((uint32_t)(L.comp[i] >> 24))) <= p.d1; });
+      base = L.mass[p.far] - (L.mass[p.d1 + 1] - L.mass[p.d0]);
+    }
+    const int last = last_entry(border, from, n, 0, base, L);
+    S = min(S, base + L.lmass[last + 1]);
+  }
+  S = min(S, M_m);
+  const int i = last_entry(Ask{true, 0u, (double)r.u * (double)S}, 0, split, 0, L.mass[p.d0], L);
+  answer(a, r, rs, L.comp[i], S);
+}
+
+// A whole row by one workgroup.
+template <int TYPE>
+__device__ __forceinline__ void draw_row(const DrawArgs& a, int row, DrawLds& L) {
+  const int tid = threadIdx.x;
+  const Row<TYPE> r(a, row);
+  const int V = r.V;
+  const float own = scan_range<TYPE>(r.at, V, L);
+  start(L);
+  if (tid == 0) L.found = 0x7fffffff;
+  __syncthreads();
+  float m, lo;
+  block_range(m, lo, L);
+  table_finish(L);
+  if (m == -__builtin_inff() || !(r.T > 0.0f)) {  // nothing to draw from; greedy
+    const bool none = m == -__builtin_inff();
+    if (!none) each_token<TYPE>(r.at, V, [&](int i, float l, bool) {
+      if (l == m) atomicMin(&L.found, i);
+    });
+    __syncthreads();
+    if (tid == 0) {
+      a.next[r.b] = none ? -1 : L.found;
+      if (a.logprob) a.logprob[r.b] = none ? -__builtin_inff() : 0.0f;
+    }
+    return;
+  }
+  if (m == __builtin_inff()) {
+    draw_inf(a, r, L);
+    return;
+  }
+  const RowScale rs = scale_of(m, lo, r.T, L);
+
+  // A bin that has k threads' largest tokens in it or before it has the first k ranks too. That is nearly the bin of
+  // rank k while k is small beside the threads (k = 512: 0.7 tokens a thread, 710 in all), and needs no pass to
+  // count. 256 rows of 131072, with and without: k = 20 27 and 37 us, 200: 31 and 40, 512: 43 and 53; at 700 and more
+  // both count (54 us; the list is then more often too long than not).
+  const bool by_own = r.limit && r.k <= kDT / 2;
+  int hi = kBins - 1, n = kList + 1;
+  if (r.by_m) hi = r.min_bin(rs);
+  if (by_own) {
+    if (taken(rs, own)) atomicAdd(&L.cnt[bin_of(rs, own)], 1u);
+    count_prefix(L);
+    if (L.cnt[kBins] >= (uint32_t)r.k) hi = last_bin(Ask{false, (uint32_t)r.k, 0.0}, L);
+  }
+  if (by_own || r.by_m) {
+    __syncthreads();
+    n = sort_bins<TYPE>(r.at, V, rs, 0, hi, -1, L);
+  }
+  if (r.limit && n > kList) {
+    for (int i = tid; i < kBins; i += kDT) L.cnt[i] = 0;
+    __syncthreads();
+    count_tokens<TYPE>(r.at, V, rs, L);
+    count_prefix(L);
+    hi = last_bin(Ask{false, (uint32_t)r.k, 0.0}, L);
+    if (r.by_k && L.cnt[hi + 1] <= kList) n = sort_bins<TYPE>(r.at, V, rs, 0, hi, -1, L);
+  }
+  if ((r.by_k || r.by_m) && n <= kList) {
+    pick_few(a, r, rs, n, L);
+    return;
+  }
+
+  __syncthreads();
+  add_masses<TYPE>(r.at, V, r, rs, L);
+  mass_prefix(L);
+  const u64 M_m = min_mass(r.mp, L.rmass);
   u64 S = L.mass[kBins];  // of what is kept: the shortest of three prefixes has the least
-  if (limit) {
-    const Found f = search<TYPE>(Ask{false, (uint32_t)k, 0.0}, row, V, rs, L);
+  if (r.limit) {
+    const Found f = search<TYPE>(Ask{false, (uint32_t)r.k, 0.0}, r.at, V, rs, L);
     S = f.above + f.mine;
   }
-  const double share = (double)(tp > 0.0f ? tp : 0.0f) * (double)S;
-  Found f;
-  bool done = false;
-  if (tp < 1.0f) {
-    // top_p's border and the draw from one list: the border lies in one bin, which bounds the kept mass, and so the
-    // bins that the drawn token may lie in.
-    const Ask border{true, 0u, share};
-    const int far = last_bin(border, L);
-    const u64 most = S < M_m ? S : M_m;
-    const u64 s0 = max(min(most, L.mass[far]), (u64)1), s1 = min(most, L.mass[far + 1]);
-    const int d0 = last_bin(Ask{true, 0u, (double)u * (double)s0}, L), d1 = last_bin(Ask{true, 0u, (double)u * (double)s1}, L);
-    const int n = sort_bins<TYPE>(row, V, rs, d0, d1, far > d1 ? far : -1, L);
-    if (n <= kList) {
-      // entries before `split` are of d0 .. d1; those of far follow, their masses counted from far's own start
-      int split = n;
-      if (far > d1) {
-        if (tid == 0) L.found = 0;
-        __syncthreads();
-        int best = -1;
-        for (int i = tid; i < n; i += kDT)
-          if (bin_of(rs, key_logit((uint32_t)(L.comp[i] >> 24))) <= d1) best = i + 1;
-        raise(&L.found, best);
-        __syncthreads();
-        split = L.found;
-        __syncthreads();
-        const u64 near = L.mass[d1 + 1] - L.mass[d0];
-        const int p = last_entry(border, split, n, 0, L.mass[far] - near, L);
-        S = min(S, L.mass[far] - near + L.lmass[p + 1]);
-      } else {
-        const int p = last_entry(border, 0, n, 0, L.mass[d0], L);
-        S = min(S, L.mass[d0] + L.lmass[p + 1]);
-      }
-      S = min(S, M_m);
-      const int i = last_entry(Ask{true, 0u, (double)u * (double)S}, 0, split, 0, L.mass[d0], L);
-      f = found(L.mass[d0] + L.lmass[i], L.comp[i], rs);
-      done = true;
-    } else {
-      const Found p = search<TYPE>(border, row, V, rs, L);
-      S = min(S, p.above + p.mine);
-    }
+  const Plan p = plan(r, S, M_m, L);
+  n = sort_bins<TYPE>(r.at, V, rs, p.d0, p.d1, p.far > p.d1 ? p.far : -1, L);
+  if (n <= kList) {
+    pick_planned(a, r, rs, p, n, S, M_m, L);
+    return;
   }
-  if (!done) {
-    S = min(S, M_m);
-    f = search<TYPE>(Ask{true, 0u, (double)u * (double)S}, row, V, rs, L);
+  if (r.tp < 1.0f) {
+    const Found f = search<TYPE>(Ask{true, 0u, r.share * (double)S}, r.at, V, rs, L);
+    S = min(S, f.above + f.mine);
   }
-  if (tid == 0) {
-    a.next[b] = (int64_t)f.idx;
-    if (a.logprob) a.logprob[b] = (float)log(e44(rs, key_logit(f.key)) / (double)S);
-  }
+  S = min(S, M_m);
+  const Found f = search<TYPE>(Ask{true, 0u, (double)r.u * (double)S}, r.at, V, rs, L);
+  answer(a, r, rs, ((u64)f.key << 24) | f.idx, S);
+}
+
+template <int TYPE>
+__global__ __launch_bounds__(kDT) void draw_row_kernel(DrawArgs a) {
+  __shared__ DrawLds L;
+  draw_row<TYPE>(a, blockIdx.x, L);
 }
 
 }  // namespace

@@ -287,9 +287,10 @@ int dfssm_sample(const dfssm_model* model, const uint16_t* logits, int32_t* coun
  * kept are the first top_k ranks (0: all); of those, with Z their mass, the ranks that have at most top_p Z
  * ranked above them; and of those the ones with e >= min_p. Rank 0 is always kept. With S the kept mass, the
  * token is the first rank whose cumulative mass exceeds u S. temperature <= 0 (or NaN) takes rank 0. A NaN
- * logit counts as -inf; of several +inf logits each has mass 1 and every other token none; a row of nothing
- * but -inf gives -1. The exponentials are fp64 and summed exactly (to 2^-44 of the largest), so the result
- * does not depend on any order. eval/gen_test.py:54-95 is the temperature and top_p part of it. */
+ * logit counts as -inf, and so does one further below the largest than fp32 reaches; of several +inf logits
+ * each has mass 1 and every other token none; a row of nothing but -inf gives -1. The exponentials are fp64 and
+ * summed exactly (to 2^-44 of the largest), so the result does not depend on any order.
+ * eval/gen_test.py:54-95 is the temperature and top_p part of it. */
 typedef struct dfssm_filter {
   const float* temperatures;   /* (batch) on the device, or NULL: `temperature` for every row; so for each pair */
   const int32_t* top_ks;

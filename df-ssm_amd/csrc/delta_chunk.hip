@@ -9,11 +9,12 @@
 // them.
 //
 // What bounds it. One long sequence: the path from chunk to chunk (K S^T, T (V - ..), the new state: three dependent
-// products with a split into 16-bit parts before each), 5500 clocks a chunk; 16411 tokens x 64 heads of 64 x 128 take
-// 0.61 ms, 0.09 of it the preparation (fp16; 403 MB, so 82 us of copying). Many sequences: the instructions of the
-// waves that make P and the outputs, 8000 clocks a chunk of 64 value columns with two workgroups to a CU: 64 x 512
-// tokens x 80 heads 0.99 ms, 0.28 of it the preparation (bf16; 2.35 GB, 0.48 ms of copying; 206 GFLOP of the
-// recurrence, 0.18 ms of matrix products).
+// products with a split into 16-bit parts before each), 4800 clocks a chunk; 16411 tokens x 64 heads of 64 x 128 take
+// 0.61 ms, 0.09 of it the preparation (fp16; 416 MB, 0.085 ms of copying). Ragged ones: that path of the longest at 64
+// value columns to a workgroup (NW = 4), 10000 clocks. Many sequences: memory. 64 x 512 tokens x 80 heads move 2.4 GB that
+// they cannot do without, 0.57 GB of T's records once out and once in, and k twice, 4.2 GB in 1.01 ms, 0.28 of it the
+// preparation (bf16; 4.9 TB/s is what a copy reaches). Records in passes small enough for the last-level cache were slower:
+// each pass reads and writes the states.
 //
 // Numbers. States, sums and everything between products are fp32. Products run on the 16-bit matrix cores with
 // fp32 accumulation. q and k are exact operands there, in their own type. A factor of fp32 values is a sum of
@@ -249,14 +250,33 @@ struct PrepRows {  // what is loaded ahead for a task
   float g, be;
 };
 
+// The sequences from the longest to the shortest, the first one first among equals, into order; by 256 threads.
+constexpr int kOrdered = 256;
+__device__ __forceinline__ void order_by_length(const DeltaArgs& a, int* len, int* order) {
+  const int i = threadIdx.x;
+  int mine = 0, rank = 0;
+  if (i < a.n_seq) {
+    int64_t t0, t1;
+    seq_range(a, i, t0, t1);
+    len[i] = mine = (int)(t1 - t0);
+  }
+  __syncthreads();
+  if (i < a.n_seq) {
+    for (int q = 0; q < a.n_seq; ++q) rank += len[q] > mine || (len[q] == mine && q < i) ? 1 : 0;
+    order[rank] = i;
+  }
+  __syncthreads();
+}
+
 template <int DK, bool BF>
-__global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(256) void delta_prep_kernel(DeltaArgs a, ChunkRec* recs,
+__global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(256) void delta_prep_kernel(DeltaArgs a, ChunkRec* recs, int* order,
                                                                                                int64_t slot0, int64_t n_tasks) {
   constexpr int NJ = DK / 32;
   __shared__ __align__(16) PrepLds lds[4];
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   PrepLds& L = lds[wave];
+  if (order && blockIdx.x == 0) order_by_length(a, (int*)lds, order);
   const int rep = a.Hv / a.Hk, nw = (a.Hv + 3) / 4;
 
   Where seq{0, 0, 0};
@@ -686,7 +706,7 @@ constexpr int kFetchers = NW == 4 ? 0 : (NW == 2 ? 4 : 6);  // waves of their ow
 
 template <int DK, bool BF, int NW>
 __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(64 * (2 * NW + kFetchers<NW>)) void
-delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, int64_t slot0, int64_t slot1) {
+delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, const int* order, int64_t slot0, int64_t slot1) {
   constexpr int NM = DK / 16, NJ = DK / 32, NT = kParts<BF>, NF = kFetchers<NW>, NP = NF ? NF : NW;
   __shared__ __align__(16) ChainLds<DK, NW> L;
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
@@ -696,7 +716,9 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, int64_t slot0, int64_t slo
   const int64_t bx = blockIdx.x, die = bx & 7, in = bx >> 3;
   const int64_t unit = in / (rep * nb) * 8 + die;
   if (unit >= (int64_t)a.n_seq * a.Hk) return;
-  const int vb = (int)(in % nb), hk = (int)(unit % a.Hk), b = (int)(unit / a.Hk), h = hk * rep + (int)(in / nb % rep);
+  const int vb = (int)(in % nb), hk = (int)(unit % a.Hk), h = hk * rep + (int)(in / nb % rep);
+  int b = (int)(unit / a.Hk);
+  if (order) b = order[b];
   const int dv0 = 16 * (NW * vb + w), dv = dv0 + c;
   const bool active = dv0 < a.Dv;
   int64_t t0, t1;
@@ -977,9 +999,9 @@ int64_t slots_per_pass(const DeltaArgs& a) {
 }
 
 template <int DK, bool BF, int NW>
-void launch_chain(const DeltaArgs& a, const ChunkRec* r, int64_t s0, int64_t s1, hipStream_t s) {
+void launch_chain(const DeltaArgs& a, const ChunkRec* r, const int* order, int64_t s0, int64_t s1, hipStream_t s) {
   const int64_t units = (int64_t)a.n_seq * a.Hk, per = (int64_t)(a.Hv / a.Hk) * ((a.Dv + 16 * NW - 1) / (16 * NW));
-  hipLaunchKernelGGL((delta_chain_kernel<DK, BF, NW>), dim3((unsigned)((units + 7) / 8 * 8 * per)), dim3(64 * (2 * NW + kFetchers<NW>)), 0, s, a, r, s0, s1);
+  hipLaunchKernelGGL((delta_chain_kernel<DK, BF, NW>), dim3((unsigned)((units + 7) / 8 * 8 * per)), dim3(64 * (2 * NW + kFetchers<NW>)), 0, s, a, r, order, s0, s1);
 }
 
 template <int DK, bool BF>
@@ -989,24 +1011,28 @@ hipError_t launch_chunked(const DeltaArgs& a, void* ws, hipStream_t s) {
   const int64_t heads = (int64_t)a.n_seq * a.Hv, tiles = a.Dv / 16;
   if ((heads + 8 * rep) * tiles > 0x7fffffff || per * ng > 0x7fffffff) return hipErrorInvalidValue;
   ChunkRec* r = (ChunkRec*)ws;
+  // Workgroups begin in order, and one that begins late with the longest chain ends late: twelve sequences of 0 to 3001
+  // tokens, 64 heads, 275 us in the order they come and 251 by length; 32 of 50 to 2200 tokens 469 and 433; 64 of one
+  // length 1059 and 1058. (More than kOrdered even out by themselves.)
+  int* order = a.cu && a.n_seq > 1 && a.n_seq <= kOrdered ? (int*)(r + slots_per_pass(a) * a.Hv) : nullptr;
   for (int64_t s0 = 0; s0 < slots; s0 += per) {
     const int64_t n = s0 + per < slots ? per : slots - s0;
     const int64_t tasks = n * ng, resident = 512;  // two workgroups to a CU (256: 631 us for 615, 1024: 617)
-    hipLaunchKernelGGL((delta_prep_kernel<DK, BF>), dim3((unsigned)(tasks < resident ? tasks : resident)), dim3(256), 0, s, a, r, s0, tasks);
+    hipLaunchKernelGGL((delta_prep_kernel<DK, BF>), dim3((unsigned)(tasks < resident ? tasks : resident)), dim3(256), 0, s, a, r, order, s0, tasks);
     // Few heads: a value column tile to a workgroup, so that all CUs have one or two and a chunk passes quickly. Many:
     // four, which make P once for 64 columns. NW = 1, 2, 4: 64 heads of 4 tiles, 16411 tokens 615, 700 and 972 us; 12 x 2
     // heads of 8 tiles 243, 268 and 360; 12 x 64 heads of 4, ragged, 388, 280 and 269; 64 x 80 heads of 4 tiles 1922, 1240
     // and 1020.
-    if (heads * ((tiles + 1) / 2) <= 256) launch_chain<DK, BF, 1>(a, r, s0, s0 + n, s);
-    else if (heads * ((tiles + 3) / 4) <= 256) launch_chain<DK, BF, 2>(a, r, s0, s0 + n, s);
-    else launch_chain<DK, BF, 4>(a, r, s0, s0 + n, s);
+    if (heads * ((tiles + 1) / 2) <= 256) launch_chain<DK, BF, 1>(a, r, order, s0, s0 + n, s);
+    else if (heads * ((tiles + 3) / 4) <= 256) launch_chain<DK, BF, 2>(a, r, order, s0, s0 + n, s);
+    else launch_chain<DK, BF, 4>(a, r, order, s0, s0 + n, s);
   }
   return hipGetLastError();
 }
 
 }  // namespace
 
-size_t delta_chunk_workspace(const DeltaArgs& a) { return (size_t)(slots_per_pass(a) * a.Hv) * sizeof(ChunkRec); }
+size_t delta_chunk_workspace(const DeltaArgs& a) { return (size_t)(slots_per_pass(a) * a.Hv) * sizeof(ChunkRec) + kOrdered * sizeof(int); }
 
 hipError_t launch_delta_chunked(const DeltaArgs& a, void* ws, hipStream_t s) {
   if (a.Dk == 128) return a.bf16 ? launch_chunked<128, true>(a, ws, s) : launch_chunked<128, false>(a, ws, s);

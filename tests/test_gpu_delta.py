@@ -351,3 +351,16 @@ def test_refusals():
     with pytest.raises(ValueError):
         ops.gated_delta_prefill(**x)                                   # packed without offsets
     assert ops.gated_delta_step(*(x[n][:0] for n in ("q", "k", "v", "g", "beta")), x["state"]).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("n", [255, 256, 257, 300])
+def test_many_sequences(n):
+    """Around the number up to which sequences are taken by length."""
+    rng = np.random.default_rng(n)
+    lens = [int(x) for x in rng.integers(0, 140, n) * (rng.random(n) < 0.3) + rng.integers(0, 3, n)]
+    x = make(lens, 1, 2, 64, 32, torch.float16, seed=n)
+    ref, ref_state = recurrence(x, lens, True)
+    d = gpu(x)
+    out = prefill(d, lens, l2norm=True)
+    check(out, ref, "out")
+    check(d["state"], ref_state, "state")

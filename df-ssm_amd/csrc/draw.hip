@@ -203,10 +203,13 @@ __device__ __forceinline__ int gather(const void* row, int V, const RowScale rs,
   __syncthreads();
   // Logits that may lie in the bins, by two compares; what passes is looked at closely.
   const float inf = __builtin_inff();
-  const float near0 = lo > 0 ? rs.m - bin_start(rs, lo, -0.01f) * 0.99999f : inf;
-  const float near1 = hi < kBins - 1 ? rs.m - bin_start(rs, hi + 1, 0.01f) * 1.00001f : -inf;
-  const float far0 = far >= 0 ? rs.m - bin_start(rs, far, -0.01f) * 0.99999f : -inf;
-  const float far1 = far >= 0 && far < kBins - 1 ? rs.m - bin_start(rs, far + 1, 0.01f) * 1.00001f : far >= 0 ? -inf : inf;
+  auto upper = [&](int b) {  // of bin b's logits (a start out of fp32's reach bounds nothing)
+    const float d = bin_start(rs, b, -0.01f);
+    return b > 0 && d < 1e38f ? rs.m - d * 0.99999f : inf;
+  };
+  auto lower = [&](int b) { return b < kBins - 1 ? rs.m - bin_start(rs, b + 1, 0.01f) * 1.00001f : -inf; };
+  const float near0 = upper(lo), near1 = lower(hi);
+  const float far0 = far >= 0 ? upper(far) : -inf, far1 = far >= 0 ? lower(far) : inf;
   each_token<TYPE>(row, V, [&](int i, float l, bool) {
     if ((l <= near0 && l >= near1) || (l <= far0 && l >= far1)) {
       const int b = bin_of(rs, l);

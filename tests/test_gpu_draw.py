@@ -242,3 +242,14 @@ def test_spreads(spread):
     for T in (0.8 * spread, 1.0):
         run_check(torch.from_numpy(l), u, T, np.array([0, 30, 0, 5000] * 2), np.array([0.9, 0.9, 1.0, 0.99] * 2),
                   np.array([0.0, 0.0, 0.05, 0.0] * 2))
+
+
+@pytest.mark.parametrize("T", [1e-37, 1e-38, 1e-44])
+def test_bins_out_of_reach(T):
+    """So small a temperature that a bin of the logits further down begins beyond fp32: top_k cuts there."""
+    rng = np.random.default_rng(43)
+    l = torch.from_numpy(rng.normal(0, 4, (5, 7001)).astype(np.float32))
+    l[1] = l[1].round()
+    l[3:, ::2] = l[3:].amax()
+    run_check(l, rng.random(5).astype(np.float32), T, np.array([2100, 5000, 0, 2047, 3600]), np.array([0.9, 1.0, 0.5, 1.0, 0.3]),
+              np.array([0.0, 0.0, 0.0, 0.5, 0.0]))

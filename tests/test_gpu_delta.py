@@ -364,3 +364,18 @@ def test_many_sequences(n):
     out = prefill(d, lens, l2norm=True)
     check(out, ref, "out")
     check(d["state"], ref_state, "state")
+
+
+def test_more_chunks_than_one_pass_holds():
+    """A workspace's worth of chunks and the rest: bit for bit the same prompt in two calls, each of one pass."""
+    lens, Hk, Hv, Dk, Dv = [15000, 9000], 4, 256, 64, 16
+    x = gpu(make(lens, Hk, Hv, Dk, Dv, torch.bfloat16, seed=91))
+    states = [x["state"].clone(), x["state"].clone()]
+    whole = prefill({**x, "state": states[0]}, lens, l2norm=True)
+    parts = torch.empty_like(whole)
+    for b, first, last in ((0, 0, 6400), (1, 15000, 21400), (0, 6400, 15000), (1, 21400, 24000)):
+        ops.gated_delta_prefill(*(x[n][first:last] for n in ("q", "k", "v", "g", "beta")), states[1],
+                                cu_seqlens=torch.tensor([0, last - first], dtype=torch.int32, device=DEV),
+                                slots=torch.tensor([b], dtype=torch.int32, device=DEV), l2norm=True,
+                                out=parts[first:last])
+    assert torch.equal(whole, parts) and torch.equal(states[0], states[1])

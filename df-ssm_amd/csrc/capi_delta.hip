@@ -36,6 +36,7 @@ int check_delta(const dfssm_delta* d, bool step) {
   // (the kernels address a chunk's rows by 32-bit offsets)
   for (const int64_t ld : {d->ld_q, d->ld_k, d->ld_v, d->ld_g, d->ld_beta, d->ld_out})
     if (ld < 0 || ld > kMaxLd) return DFSSM_E_RANGE;
+  if (d->n_tokens > 1 && d->ld_out < (int64_t)d->v_heads * d->v_dim) return DFSSM_E_DIMS;
   if (d->ld_q % 8 || d->ld_k % 8 || d->ld_v % 8 || d->ld_out % 8) return DFSSM_E_ALIGN;
   return DFSSM_OK;
 }

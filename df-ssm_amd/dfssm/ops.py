@@ -7,6 +7,7 @@ to names until its launch, so that the allocator cannot give one's memory to the
 """
 from __future__ import annotations
 
+import operator
 import threading
 
 import torch
@@ -299,7 +300,7 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     shape; slots that no sequence has are left as they are there). Rows of B may be strided. slots (B,) int32:
     the slot of each sequence (default 0..B-1); a negative one marks padding (zeros returned), one past the
     state or taken by an earlier row gives NaN, and neither touches a state. scale defaults to Dk^-0.5;
-    l2norm divides q and k by sqrt(sum x^2 + 1e-6) first."""
+    l2norm divides q and k by sqrt(sum x^2 + 1e-6) first. out, if given, overlaps none of the others."""
     return _delta_call(True, q, k, v, g, beta, state, None, slots, scale, l2norm, out, state_out,
                        q.shape[0])
 
@@ -347,7 +348,7 @@ def _on_device(t: torch.Tensor, name: str, dev) -> None:
 def _per_row(x, dtype, name: str, B: int, dev, held: list):
     """A parameter as (number, device pointer): one of them counts."""
     if not isinstance(x, torch.Tensor):
-        return (int(x) if dtype is torch.int32 else float(x)), 0
+        return (max(-1, min(operator.index(x), 2**31 - 1)) if dtype is torch.int32 else float(x)), 0
     _need(x, dtype, name)
     if x.shape != (B,):
         raise ValueError(f"{name} must be a number or ({B},)")

@@ -378,7 +378,7 @@ typedef struct dfssm_delta {
   float scale;
 } dfssm_delta;
 /* q, k, v, out, state and state_out are 16-byte aligned, ld_q, ld_k, ld_v and ld_out multiples of 8,
- * every ld_* at most 2^23. */
+ * every ld_* at most 2^23; the rows of out do not overlap each other or anything else. */
 
 /* One token per sequence (n_tokens = n_seq). */
 int dfssm_gated_delta_step(const dfssm_delta* args, void* stream);

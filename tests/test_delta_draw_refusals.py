@@ -60,3 +60,17 @@ def test_host_tensors():
                                 cu_seqlens=torch.tensor([0, 1], dtype=torch.int32))
     with pytest.raises(TypeError):
         ops.sample_filtered(torch.zeros(1, 8), torch.zeros(1))
+
+
+def test_overlapping_rows_of_out():
+    L = _C.lib()
+    assert L.dfssm_gated_delta_step(_delta(ld_out=56), None) == -2
+    assert L.dfssm_gated_delta_prefill(_delta(ld_out=56, n_tokens=64), None, None) == -2
+
+
+def test_numbers_of_settings():
+    """A top_k past 32 bits means all, not what is left of it there; a fraction is refused."""
+    value = lambda x: ops._per_row(x, torch.int32, "top_k", 2, None, [])
+    assert value(7) == (7, 0) and value(2**32 + 5) == (2**31 - 1, 0) and value(-2**40) == (-1, 0)
+    with pytest.raises(TypeError):
+        value(2.5)

@@ -497,12 +497,13 @@ template <int DK, int NW>
 struct ChainLds {
   Operands<DK> op[2];
   uint16_t v[NW == 4 ? 1 : 2][NW == 4 ? 8 : kC * 16 * NW];  // NW < 4: rows of v, two chunks; else in registers
-  f16 S[NW][DK / 32][2][64][8];   // the state before the chunk, as operands
+  f16 S[NW == 4 ? 1 : NW][NW == 4 ? 1 : DK / 32][2][64][8];  // NW < 4: the state before the chunk, as operands
+  f32x4 qs[NW == 4 ? NW : 1][NW == 4 ? 4 : 1][64];           // NW = 4: Q S^T
   f32x4 u[NW][4][64];
   f16 P[6][2][64][8];
   float F[6][32];                 // of P's fragments, see make_p
   float c2[kC], pr[2][kC];        // scale e^{G_i} times q's row factor; the row factors of P, by column block
-  float sfac[NW][16], ufac[NW][16];  // per value column: what undoes the scaling of S and of U
+  float sfac[2][NW][16], ufac[NW][16];  // per value column: what undoes the scaling of S and of U
 };
 
 template <int N>
@@ -770,18 +771,25 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, const int* order, int64_t 
         ssc = pow2_scale(smax, sinv);
       }
       split_all<NM>(S, ssc, s);
+      if constexpr (NW < 4)
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        *(h8*)L.S[w][j][0][lane] = s[0][j];
-        *(h8*)L.S[w][j][1][lane] = s[1][j];
-      }
+        for (int j = 0; j < NJ; ++j) {
+          *(h8*)L.S[w][j][0][lane] = s[0][j];
+          *(h8*)L.S[w][j][1][lane] = s[1][j];
+        }
       if constexpr (!BF) {
         sinv *= sfac;
-        if (g == 0) L.sfac[w][c] = sinv;
+        if (g == 0) L.sfac[i & 1][w][c] = sinv;
       }
       step_barrier();  // the operands of this chunk and the state are in LDS
       f32x4 v[4], ks[4];
       rows_product<DK, BF, false>(op.k, lane, s, ks);
+      if constexpr (NW == 4) {
+        f32x4 qs[4];
+        rows_product<DK, BF, true>(op.q, lane, (const h8 (&)[2][NJ])s, qs);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) L.qs[w][t][lane] = qs[t];
+      }
       Tri T;
       load_tri(T, op.T, lane);
       s4 vx[4];
@@ -935,16 +943,16 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, const int* order, int64_t 
     }
     f32x4 qs[4];
     f32x4 sinv;
-    if (outputs) {
+    if (NW < 4 && outputs) {
       h8 s[2][NJ];
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         s[0][j] = *(const h8*)L.S[w][j][0][lane];
         s[1][j] = *(const h8*)L.S[w][j][1][lane];
       }
-      sinv = BF ? f32x4{1.0f, 1.0f, 1.0f, 1.0f} : *(const f32x4*)&L.sfac[w][4 * g];
       rows_product<DK, BF, true>(op.q, lane, s, qs);
     }
+    if (outputs) sinv = BF ? f32x4{1.0f, 1.0f, 1.0f, 1.0f} : *(const f32x4*)&L.sfac[i & 1][w][4 * g];
     if (i + 1 < n) {  // with six fetchers the output wave, which has less to do, helps
       if (!NF) fetch_rest(i + 1, fi);
       if (NF == 6 && outputs) fetch_rest(i + 1, 0), fetch_rest(i + 1, 1);
@@ -970,6 +978,9 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, const int* order, int64_t 
       tri_product<true, false>(P, x, o);
       wave_sync();
       uinv = *(const f32x4*)&L.ufac[w][4 * g];
+      if constexpr (NW == 4)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) qs[t] = L.qs[w][t][lane];
     }
     // what this wave loads for the next chunk is in before it stores, so that the wait is not for the stores
     if (fetches || NF == 6) __builtin_amdgcn_s_waitcnt(0);

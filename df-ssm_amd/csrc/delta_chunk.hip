@@ -11,7 +11,7 @@
 // What bounds it. One long sequence: the path from chunk to chunk (K S^T, T (V - ..), the new state: three dependent
 // products with a split into 16-bit parts before each), 4800 clocks a chunk; 16411 tokens x 64 heads of 64 x 128 take
 // 0.61 ms, 0.09 of it the preparation (fp16; 416 MB, 0.085 ms of copying). Ragged ones: that path of the longest at 64
-// value columns to a workgroup (NW = 4), 10000 clocks. Many sequences: memory. 64 x 512 tokens x 80 heads move 2.4 GB that
+// value columns to a workgroup (NW = 4), 9500 clocks. Many sequences: memory. 64 x 512 tokens x 80 heads move 2.4 GB that
 // they cannot do without, 0.57 GB of T's records once out and once in, and k twice, 4.2 GB in 1.01 ms, 0.28 of it the
 // preparation (bf16; 4.9 TB/s is what a copy reaches). Records in passes small enough for the last-level cache were slower:
 // each pass reads and writes the states.
@@ -477,7 +477,7 @@ __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(256) void d
 // ---------------------------------------------------------------------------------------------
 // The chain: one sequence, one value head, 16 NW value columns. The state lies in registers as 16 x 16 results
 // (rows of k's columns, 16 value columns per wave), and the waves that carry it need nothing of each other.
-//   NW waves, the chain proper: K S^T, U and the new state
+//   NW waves, the chain proper: K S^T, U and the new state; with NW = 4, where it is not what a chunk waits for, Q S^T too
 //   NW waves, the outputs: Q S^T, P U
 //   the fetchers: this chunk's P = tril(Q K^T ..), a fragment or two each, and the next one's operands, straight
 //   into LDS. Waves of their own, as many as make eight in all; with NW = 4 the output waves do it beside their work
@@ -1023,7 +1023,7 @@ hipError_t launch_chunked(const DeltaArgs& a, void* ws, hipStream_t s) {
   if ((heads + 8 * rep) * tiles > 0x7fffffff || per * ng > 0x7fffffff) return hipErrorInvalidValue;
   ChunkRec* r = (ChunkRec*)ws;
   // Workgroups begin in order, and one that begins late with the longest chain ends late: twelve sequences of 0 to 3001
-  // tokens, 64 heads, 275 us in the order they come and 251 by length; 32 of 50 to 2200 tokens 469 and 433; 64 of one
+  // tokens, 64 heads, 275 us in the order they come and 251 by length (bf16); 32 of 50 to 2200 tokens 469 and 433; 64 of one
   // length 1059 and 1058. (More than kOrdered even out by themselves.)
   int* order = a.cu && a.n_seq > 1 && a.n_seq <= kOrdered ? (int*)(r + slots_per_pass(a) * a.Hv) : nullptr;
   for (int64_t s0 = 0; s0 < slots; s0 += per) {
@@ -1031,8 +1031,8 @@ hipError_t launch_chunked(const DeltaArgs& a, void* ws, hipStream_t s) {
     const int64_t tasks = n * ng, resident = 512;  // two workgroups to a CU (256: 631 us for 615, 1024: 617)
     hipLaunchKernelGGL((delta_prep_kernel<DK, BF>), dim3((unsigned)(tasks < resident ? tasks : resident)), dim3(256), 0, s, a, r, order, s0, tasks);
     // Few heads: a value column tile to a workgroup, so that all CUs have one or two and a chunk passes quickly. Many:
-    // four, which make P once for 64 columns. NW = 1, 2, 4: 64 heads of 4 tiles, 16411 tokens 615, 700 and 972 us; 12 x 2
-    // heads of 8 tiles 243, 268 and 360; 12 x 64 heads of 4, ragged, 388, 280 and 269; 64 x 80 heads of 4 tiles 1922, 1240
+    // four, which make P once for 64 columns. NW = 1, 2, 4: 64 heads of 4 tiles, 16411 tokens 613, 704 and 927 us; 12 x 2
+    // heads of 8 tiles 235, 265 and 350; 12 x 64 heads of 4, ragged, 389, 263 and 248; 64 x 80 heads of 4 tiles 1912, 1222
     // and 1020.
     if (heads * ((tiles + 1) / 2) <= 256) launch_chain<DK, BF, 1>(a, r, order, s0, s0 + n, s);
     else if (heads * ((tiles + 3) / 4) <= 256) launch_chain<DK, BF, 2>(a, r, order, s0, s0 + n, s);

@@ -269,8 +269,8 @@ __device__ __forceinline__ void order_by_length(const DeltaArgs& a, int* len, in
 }
 
 template <int DK, bool BF>
-__global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(256) void delta_prep_kernel(DeltaArgs a, ChunkRec* recs, int* order,
-                                                                                               int64_t slot0, int64_t n_tasks) {
+__global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(256) void
+delta_prep_kernel(DeltaArgs a, ChunkRec* recs, int* order, int64_t slot0, int64_t n_tasks) {
   constexpr int NJ = DK / 32;
   __shared__ __align__(16) PrepLds lds[4];
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
@@ -1012,7 +1012,8 @@ int64_t slots_per_pass(const DeltaArgs& a) {
 template <int DK, bool BF, int NW>
 void launch_chain(const DeltaArgs& a, const ChunkRec* r, const int* order, int64_t s0, int64_t s1, hipStream_t s) {
   const int64_t units = (int64_t)a.n_seq * a.Hk, per = (int64_t)(a.Hv / a.Hk) * ((a.Dv + 16 * NW - 1) / (16 * NW));
-  hipLaunchKernelGGL((delta_chain_kernel<DK, BF, NW>), dim3((unsigned)((units + 7) / 8 * 8 * per)), dim3(64 * (2 * NW + kFetchers<NW>)), 0, s, a, r, order, s0, s1);
+  const dim3 grid((unsigned)((units + 7) / 8 * 8 * per)), block(64 * (2 * NW + kFetchers<NW>));
+  hipLaunchKernelGGL((delta_chain_kernel<DK, BF, NW>), grid, block, 0, s, a, r, order, s0, s1);
 }
 
 template <int DK, bool BF>
@@ -1023,13 +1024,14 @@ hipError_t launch_chunked(const DeltaArgs& a, void* ws, hipStream_t s) {
   if ((heads + 8 * rep) * tiles > 0x7fffffff || per * ng > 0x7fffffff) return hipErrorInvalidValue;
   ChunkRec* r = (ChunkRec*)ws;
   // Workgroups begin in order, and one that begins late with the longest chain ends late: twelve sequences of 0 to 3001
-  // tokens, 64 heads, 275 us in the order they come and 251 by length (bf16); 32 of 50 to 2200 tokens 469 and 433; 64 of one
-  // length 1059 and 1058. (More than kOrdered even out by themselves.)
+  // tokens, 64 heads, 275 us in the order they come and 251 by length (bf16); 32 of 50 to 2200 tokens 469 and 433; 64
+  // of one length 1059 and 1058. (More than kOrdered even out by themselves.)
   int* order = a.cu && a.n_seq > 1 && a.n_seq <= kOrdered ? (int*)(r + slots_per_pass(a) * a.Hv) : nullptr;
   for (int64_t s0 = 0; s0 < slots; s0 += per) {
     const int64_t n = s0 + per < slots ? per : slots - s0;
     const int64_t tasks = n * ng, resident = 512;  // two workgroups to a CU (256: 631 us for 615, 1024: 617)
-    hipLaunchKernelGGL((delta_prep_kernel<DK, BF>), dim3((unsigned)(tasks < resident ? tasks : resident)), dim3(256), 0, s, a, r, order, s0, tasks);
+    const dim3 grid((unsigned)(tasks < resident ? tasks : resident));
+    hipLaunchKernelGGL((delta_prep_kernel<DK, BF>), grid, dim3(256), 0, s, a, r, order, s0, tasks);
     // Few heads: a value column tile to a workgroup, so that all CUs have one or two and a chunk passes quickly. Many:
     // four, which make P once for 64 columns. NW = 1, 2, 4: 64 heads of 4 tiles, 16411 tokens 613, 704 and 927 us; 12 x 2
     // heads of 8 tiles 235, 265 and 350; 12 x 64 heads of 4, ragged, 389, 263 and 248; 64 x 80 heads of 4 tiles 1912, 1222
@@ -1043,7 +1045,9 @@ hipError_t launch_chunked(const DeltaArgs& a, void* ws, hipStream_t s) {
 
 }  // namespace
 
-size_t delta_chunk_workspace(const DeltaArgs& a) { return (size_t)(slots_per_pass(a) * a.Hv) * sizeof(ChunkRec) + kOrdered * sizeof(int); }
+size_t delta_chunk_workspace(const DeltaArgs& a) {
+  return (size_t)(slots_per_pass(a) * a.Hv) * sizeof(ChunkRec) + kOrdered * sizeof(int);
+}
 
 hipError_t launch_delta_chunked(const DeltaArgs& a, void* ws, hipStream_t s) {
   if (a.Dk == 128) return a.bf16 ? launch_chunked<128, true>(a, ws, s) : launch_chunked<128, false>(a, ws, s);

@@ -19,8 +19,8 @@
 //   order key and the index, a byte at a time over the row.
 //
 // What bounds it. Few kept: two passes over the logits, 256 rows of 131072 fp16, top_k 50, 27 us (67 MB, 5 TB/s of the
-// passes' bytes); one row of 50288 takes 11 to 13 us, two reads of its logits and a dozen barriers one after the other. Else the
-// arithmetic of the masses, about 30 instructions a token of which 11 are fp64, and the LDS atomics beside them: one
+// passes' bytes); one row of 50288 takes 11 to 13 us, two reads of its logits and a dozen barriers one after the
+// other. Else the arithmetic of the masses, about 30 instructions a token of which 11 are fp64, and the LDS atomics beside them: one
 // row of 50288 takes 29 us, 12 of them that pass, as it has the arithmetic of one compute unit. 256 rows of 131072 fp32
 // with settings of all kinds: 87 us. Spreading a row over up to 24 workgroups (three launches, bins summed in global
 // memory) took 28 us for that one row and 19 for one with top_k 20, which takes 11 this way.
@@ -662,7 +662,8 @@ __device__ __forceinline__ void pick_planned(const DrawArgs& a, const Row<TYPE>&
     u64 base = L.mass[p.d0];
     int from = 0;
     if (p.far > p.d1) {
-      from = split = 1 + last_true(0, n, L, [&](int i) { return bin_of(rs, key_logit((uint32_t)(L.comp[i] >> 24))) <= p.d1; });
+      auto near = [&](int i) { return bin_of(rs, key_logit((uint32_t)(L.comp[i] >> 24))) <= p.d1; };
+      from = split = 1 + last_true(0, n, L, near);
       base = L.mass[p.far] - (L.mass[p.d1 + 1] - L.mass[p.d0]);
     }
     const int last = last_entry(border, from, n, 0, base, L);

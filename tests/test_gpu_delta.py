@@ -379,3 +379,33 @@ def test_more_chunks_than_one_pass_holds():
                                 slots=torch.tensor([b], dtype=torch.int32, device=DEV), l2norm=True,
                                 out=parts[first:last])
     assert torch.equal(whole, parts) and torch.equal(states[0], states[1])
+
+
+def test_offsets_past_32_bits():
+    """Slots behind 2^31 values of the state, and tokens so far apart that they pass 2^31 elements: the same bits as
+    close together."""
+    lens, (Hk, Hv, Dk, Dv), ld = [290, 3], (1, 2, 128, 64), 1 << 23
+    x = gpu(make(lens, Hk, Hv, Dk, Dv, torch.float16, seed=97))
+    pool = (1 << 31) // (Hv * Dv * Dk) + 3
+    near, state = x["state"].clone(), torch.zeros(pool, Hv, Dv, Dk, device=DEV)
+    slots = torch.tensor([pool - 1, pool - 2], dtype=torch.int32, device=DEV)
+    state[slots.long()] = near
+    want = prefill({**x, "state": near}, lens, l2norm=True)
+    wide, wide32 = torch.empty(sum(lens) * ld, dtype=torch.float16, device=DEV), torch.empty(sum(lens) * ld, device=DEV)
+    at, far = 0, {}
+    for n in ("q", "k", "v", "out"):
+        t = x[n] if n in x else want
+        far[n] = wide.as_strided(t.shape, (ld, t.shape[2], 1), at)
+        at += t.shape[1] * t.shape[2]
+    for i, n in enumerate(("g", "beta")):
+        far[n] = wide32.as_strided(x[n].shape, (ld, 1), i * Hv)
+    for n in ("q", "k", "v", "g", "beta"):
+        far[n].copy_(x[n])
+    out = prefill({**far, "state": state}, lens, l2norm=True, slots=slots, out=far["out"])
+    assert torch.equal(out, want) and torch.equal(state[slots.long()], near) and not state[:pool - 2].any()
+    # one token of each, which are 290 tokens apart
+    step = {n: far[n][::290][:2] for n in ("q", "k", "v", "g", "beta")}
+    assert step["q"].stride(0) > 1 << 31
+    a = ops.gated_delta_step(*(step[n] for n in ("q", "k", "v", "g", "beta")), state, slots=slots, l2norm=True)
+    b = ops.gated_delta_step(*(step[n].contiguous() for n in ("q", "k", "v", "g", "beta")), near, l2norm=True)
+    assert torch.equal(a, b) and torch.equal(state[slots.long()], near)

@@ -253,3 +253,16 @@ def test_bins_out_of_reach(T):
     l[3:, ::2] = l[3:].amax()
     run_check(l, rng.random(5).astype(np.float32), T, np.array([2100, 5000, 0, 2047, 3600]), np.array([0.9, 1.0, 0.5, 1.0, 0.3]),
               np.array([0.0, 0.0, 0.0, 0.5, 0.0]))
+
+
+def test_rows_past_32_bits():
+    """Rows further apart than 2^31 elements."""
+    V, ld = 9001, (1 << 31) + 24
+    wide = torch.empty(ld + V, dtype=torch.float16, device=DEV)
+    l = wide.as_strided((2, V), (ld, 1))
+    l.copy_(torch.from_numpy(np.random.default_rng(47).normal(0, 2, (2, V)).astype(np.float32)))
+    u = torch.tensor([0.3, 0.8], device=DEV)
+    for kw in (dict(top_k=40), dict(top_p=0.9)):
+        got = ops.sample_filtered(l, u, temperature=0.9, want_logprob=True, **kw)
+        want = ops.sample_filtered(l.contiguous(), u, temperature=0.9, want_logprob=True, **kw)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

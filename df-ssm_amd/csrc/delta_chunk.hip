@@ -11,7 +11,7 @@
 // What bounds it. One long sequence: the path from chunk to chunk (K S^T, T (V - ..), the new state: three dependent
 // products with a split into 16-bit parts before each), 4800 clocks a chunk; 16411 tokens x 64 heads of 64 x 128 take
 // 0.61 ms, 0.09 of it the preparation (fp16; 416 MB, 0.085 ms of copying). Ragged ones: that path of the longest at 64
-// value columns to a workgroup (NW = 4), 9500 clocks. Many sequences: memory. 64 x 512 tokens x 80 heads move 2.4 GB that
+// value columns to a workgroup (NW = 4), 8500 clocks. Many sequences: memory. 64 x 512 tokens x 80 heads move 2.4 GB that
 // they cannot do without, 0.57 GB of T's records once out and once in, and k twice, 4.2 GB in 1.01 ms, 0.28 of it the
 // preparation (bf16; 4.9 TB/s is what a copy reaches). Records in passes small enough for the last-level cache were slower:
 // each pass reads and writes the states.
@@ -879,15 +879,31 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, const int* order, int64_t 
   const ChunkRec* rec = recs + (first + cb - slot0) * a.Hv + h;
   const bool outputs = wave < 2 * NW, fetches = !NF || !outputs;
   const int fi = NF ? wave - 2 * NW : w;  // which fetcher
-  // Chunk i's rows of k, of q, and the rest: four fetchers have the rows, the others (or the same) the rest.
-  const int offk = rows_off<DK>(a.ld_k, fi & 3, lane), offq = rows_off<DK>(a.ld_q, fi & 3, lane);
+  // Chunk i's rows of k, of q, and the rest: four fetchers have the rows, the others (or the same) the rest. Of the
+  // four output waves that fetch where NW = 4, the two with one fragment of P have all of it, one k and one q.
+  int off[4];
+#pragma unroll
+  for (int m = 0; m < 4; ++m)
+    off[m] = NF ? rows_off<DK>(m == 0 ? a.ld_k : a.ld_q, fi & 3, lane) : rows_off<DK>(fi ? a.ld_q : a.ld_k, m, lane);
   auto fetch_k = [&](int i) {
     const int64_t tk = t0 + (cb + i) * kC;
-    if (fi < 4) fetch_rows<DK>(L.op[i & 1].k, a.k + tk * a.ld_k + hk * DK, a.ld_k, len_at(tk), fi, offk);
+    const uint16_t* p = a.k + tk * a.ld_k + hk * DK;
+    if (NF) {
+      if (fi < 4) fetch_rows<DK>(L.op[i & 1].k, p, a.ld_k, len_at(tk), fi, off[0]);
+    } else if (fi == 0) {
+#pragma unroll
+      for (int m = 0; m < 4; ++m) fetch_rows<DK>(L.op[i & 1].k, p, a.ld_k, len_at(tk), m, off[m]);
+    }
   };
   auto fetch_q = [&](int i) {
     const int64_t tk = t0 + (cb + i) * kC;
-    if (fi < 4) fetch_rows<DK>(L.op[i & 1].q, a.q + tk * a.ld_q + hk * DK, a.ld_q, len_at(tk), fi, offq);
+    const uint16_t* p = a.q + tk * a.ld_q + hk * DK;
+    if (NF) {
+      if (fi < 4) fetch_rows<DK>(L.op[i & 1].q, p, a.ld_q, len_at(tk), fi, off[1]);
+    } else if (fi == 1) {
+#pragma unroll
+      for (int m = 0; m < 4; ++m) fetch_rows<DK>(L.op[i & 1].q, p, a.ld_q, len_at(tk), m, off[m]);
+    }
   };
   auto fetch_rest = [&](int i, int part) {  // part of 4
     const int64_t tk = t0 + (cb + i) * kC;
@@ -915,16 +931,16 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, const int* order, int64_t 
       const bool next = i + 1 < n;
       if (next) {
         fetch_k(i + 1);
-        if (NF) fetch_q(i + 1);
+        fetch_q(i + 1);
       }
       auto p = [&](auto w, auto j) {
         make_p<decltype(w)::value, decltype(j)::value, DK, BF>(L, op, lane, a.l2norm, a.scale);
       };
       if constexpr (NP == 6) {
         switch (fi) {
-          case 0: p(Int<0>{}, Int<0>{}); break;
+          case 0: p(Int<2>{}, Int<0>{}); break;
           case 1: p(Int<1>{}, Int<0>{}); break;
-          case 2: p(Int<2>{}, Int<0>{}); break;
+          case 2: p(Int<0>{}, Int<0>{}); break;  // (one tile: it shares its SIMD with the chain)
           case 3: p(Int<2>{}, Int<1>{}); break;
           case 4: p(Int<3>{}, Int<0>{}); break;
           default: p(Int<3>{}, Int<1>{});
@@ -936,9 +952,6 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, const int* order, int64_t 
           case 2: p(Int<2>{}, Int<0>{}), p(Int<0>{}, Int<0>{}); break;
           default: p(Int<1>{}, Int<0>{}), p(Int<2>{}, Int<1>{});
         }
-      }
-      if (next) {
-        if (!NF) fetch_q(i + 1);
       }
     }
     f32x4 qs[4];
@@ -954,7 +967,7 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, const int* order, int64_t 
     }
     if (outputs) sinv = BF ? f32x4{1.0f, 1.0f, 1.0f, 1.0f} : *(const f32x4*)&L.sfac[i & 1][w][4 * g];
     if (i + 1 < n) {  // with six fetchers the output wave, which has less to do, helps
-      if (!NF) fetch_rest(i + 1, fi);
+      if (!NF && fi < 2) fetch_rest(i + 1, 2 * fi), fetch_rest(i + 1, 2 * fi + 1);
       if (NF == 6 && outputs) fetch_rest(i + 1, 0), fetch_rest(i + 1, 1);
     }
     step_barrier();

@@ -12,7 +12,7 @@
 // products with a split into 16-bit parts before each), 4800 clocks a chunk; 16411 tokens x 64 heads of 64 x 128 take
 // 0.61 ms, 0.09 of it the preparation (fp16; 416 MB, 0.085 ms of copying). Ragged ones: that path of the longest at 64
 // value columns to a workgroup (NW = 4), 8500 clocks. Many sequences: memory. 64 x 512 tokens x 80 heads move 2.4 GB that
-// they cannot do without, 0.57 GB of T's records once out and once in, and k twice, 4.2 GB in 1.01 ms, 0.28 of it the
+// they cannot do without, 0.57 GB of T's records once out and once in, and k twice, 4.2 GB in 0.99 ms, 0.27 of it the
 // preparation (bf16; 4.9 TB/s is what a copy reaches). Records in passes small enough for the last-level cache were slower:
 // each pass reads and writes the states.
 //
@@ -1047,8 +1047,8 @@ hipError_t launch_chunked(const DeltaArgs& a, void* ws, hipStream_t s) {
     hipLaunchKernelGGL((delta_prep_kernel<DK, BF>), grid, dim3(256), 0, s, a, r, order, s0, tasks);
     // Few heads: a value column tile to a workgroup, so that all CUs have one or two and a chunk passes quickly. Many:
     // four, which make P once for 64 columns. NW = 1, 2, 4: 64 heads of 4 tiles, 16411 tokens 613, 704 and 927 us; 12 x 2
-    // heads of 8 tiles 235, 265 and 350; 12 x 64 heads of 4, ragged, 389, 263 and 248; 64 x 80 heads of 4 tiles 1912, 1222
-    // and 1020.
+    // heads of 8 tiles 235, 265 and 350; 12 x 64 heads of 4, ragged, 389, 263 and 223; 64 x 80 heads of 4 tiles 1912, 1222
+    // and 1000.
     if (heads * ((tiles + 1) / 2) <= 256) launch_chain<DK, BF, 1>(a, r, order, s0, s0 + n, s);
     else if (heads * ((tiles + 3) / 4) <= 256) launch_chain<DK, BF, 2>(a, r, order, s0, s0 + n, s);
     else launch_chain<DK, BF, 4>(a, r, order, s0, s0 + n, s);

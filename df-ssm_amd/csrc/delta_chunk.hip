@@ -244,6 +244,15 @@ __device__ __forceinline__ float store_frags(const f32x4 (&x)[W + 1], int lane, 
   return inv;
 }
 
+// v as another lane has it, moved by the register file; 0 where there is none.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double moved(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xf, true);
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+
 template <int DK>
 struct PrepRows {  // what is loaded ahead for a task
   u32x4 k[4][DK / 32];
@@ -312,11 +321,12 @@ delta_prep_kernel(DeltaArgs a, ChunkRec* recs, int* order, int64_t slot0, int64_
         float gv = real ? in.g : 0.0f;
         gv = gv < -1e5f ? -1e5f : gv;
         G = (double)gv * 1.4426950408889634;
-        for (int o = 1; o < 64; o <<= 1) {
-          const uint64_t u = __builtin_bit_cast(uint64_t, G);
-          const uint32_t lo = (uint32_t)__shfl_up((int)(uint32_t)u, o, 64), hi = (uint32_t)__shfl_up((int)(uint32_t)(u >> 32), o, 64);
-          if (lane >= o) G += __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
-        }
+        G += moved<0x111, 0xf>(G);  // running sums: from 1, 2, 4 and 8 lanes before, in the row of 16
+        G += moved<0x112, 0xf>(G);
+        G += moved<0x114, 0xf>(G);
+        G += moved<0x118, 0xf>(G);
+        G += moved<0x142, 0xa>(G);  // row 0's last to row 1, 2's to 3; then lane 31's to rows 2 and 3
+        G += moved<0x143, 0xc>(G);
       }
       const float be = lane < len ? in.be : 0.0f;
       h8 k[4][NJ];

@@ -185,18 +185,7 @@ def _run_own(s, kind):
     return o, s["state_out"]
 
 
-_ops_module = None
-
-
 def _ops():
-    """The framework's operators, imported at the first use as a program would, not at every pass."""
-    global _ops_module
-    if _ops_module is None:
-        _ops_module = _import_ops()
-    return _ops_module
-
-
-def _import_ops():
     pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "df-ssm_amd")
     if pkg not in sys.path:
         sys.path.insert(0, pkg)

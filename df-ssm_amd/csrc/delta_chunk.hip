@@ -27,6 +27,7 @@
 // G is summed in fp64, so that differences survive a decay of any size in the same chunk; -inf is held to -1e5.
 #include "common.h"
 #include "delta.h"
+#include "delta_plan.h"
 #include "dfssm_kernels.h"
 
 namespace dfssm {
@@ -735,19 +736,18 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, const int* order, int64_t 
   int64_t t0, t1;
   seq_range(a, b, t0, t1);
   const int64_t first = t0 / kC + b, nch = (t1 - t0 + kC - 1) / kC;
-  int64_t cb = slot0 - first, ce = slot1 - first;  // this launch's chunks of the sequence
-  cb = cb < 0 ? 0 : cb;
-  ce = ce > nch ? nch : ce;
-  if (cb >= ce && !(nch == 0 && slot0 == 0)) return;
+  const PassChunks pass = pass_chunks(first, nch, slot0, slot1);  // this launch's chunks of the sequence
+  const int64_t cb = pass.begin;
+  const int n = (int)pass.count;
+  if (n == 0 && !(nch == 0 && slot0 == 0)) return;  // (an empty sequence's state is passed on by the first launch)
   const int slot = slot_of(a, b);
   if (slot < 0) {
     const uint16_t fill = slot == kSlotPad ? 0 : 0x7fff;
     if (active && wave < NW)
-      for (int64_t t = t0 + cb * kC + g; t < t1 && t < t0 + ce * kC; t += 4) a.out[t * a.ld_out + (int64_t)h * a.Dv + dv] = fill;
+      for (int64_t t = t0 + cb * kC + g; t < t1 && t < t0 + (cb + n) * kC; t += 4) a.out[t * a.ld_out + (int64_t)h * a.Dv + dv] = fill;
     return;
   }
   int64_t tok = t0 + cb * kC;
-  const int n = (int)(ce - cb);
   auto len_at = [&](int64_t t) { return (int)(t1 - t < kC ? t1 - t : kC); };
 
   if (wave < NW) {  // ------------------------------------------------------------ the state
@@ -765,7 +765,7 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, const int* order, int64_t 
       for (int i = 0; i < 16; ++i) vn[i] = __builtin_amdgcn_raw_buffer_load_b16(r, vo, (16 * (i / 4) + (i & 3)) * ldv, 0);
     };
     __builtin_amdgcn_s_waitcnt(0);  // the state is here: within the loop only v is waited for
-    if (NW == 4 && n) load_v(tok);
+    if (NW == 4 && n > 0) load_v(tok);
     for (int i = 0; i < n; ++i, tok += kC) {
       const Operands<DK>& op = L.op[i & 1];
       const f32x4* vec = (const f32x4*)op.vec;
@@ -927,7 +927,7 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, const int* order, int64_t 
     }
   };
   const int ldo = (int)a.ld_out * 2, oo = c * ldo + (dv0 + 4 * g) * 2;
-  if (fetches && n) {
+  if (fetches && n > 0) {
     fetch_k(0);
     fetch_q(0);
     if (NF < 6) fetch_rest(0, fi);

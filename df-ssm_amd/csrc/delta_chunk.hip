@@ -21,9 +21,10 @@
 // 16-bit parts: beside fp16 rows, and where both factors are fp32 (T (V - ..), P U), pairs of halves,
 // x 2^s = hi + lo, which hold 22 bits, with s per row of T and P and per value column of S, V - .. and U chosen so
 // that the largest magnitude lies in [2^14, 2^15); beside bf16 rows three bf16 parts, which hold 24 bits and need
-// no scale (for Q S^T, whose result is rounded to bf16, two parts, 16 bits). A product of two pairs leaves out
-// lo lo, 2^-24 of it. So an fp32 state comes out as from fp32 arithmetic (2e-7 of its norm), at 2 or 3 matrix
-// instructions per product instead of the 8 times as slow fp32 ones.
+// no scale. (Q S^T is no exception, though its sum with P U is rounded to 16 bits: where a token overwrites what the
+// state has for its key, the two nearly cancel.) A product of two pairs leaves out lo lo, 2^-24 of it. So an fp32 state
+// comes out as from fp32 arithmetic (2e-7 of its norm), at 2 or 3 matrix instructions per product instead of the 8 times
+// as slow fp32 ones.
 // G is summed in fp64, so that differences survive a decay of any size in the same chunk; -inf is held to -1e5.
 #include "common.h"
 #include "delta.h"
@@ -504,11 +505,11 @@ struct Operands {
   f16 T[6][2][64][8];             // the record: T
   float vec[384];                 // c1, tr, w, rk, Gh, Gl
 };
-template <int DK, int NW>
+template <int DK, int NW, int NT>
 struct ChainLds {
   Operands<DK> op[2];
   uint16_t v[NW == 4 ? 1 : 2][NW == 4 ? 8 : kC * 16 * NW];  // NW < 4: rows of v, two chunks; else in registers
-  f16 S[NW == 4 ? 1 : NW][NW == 4 ? 1 : DK / 32][2][64][8];  // NW < 4: the state before the chunk, as operands
+  f16 S[NW == 4 ? 1 : NW][NW == 4 ? 1 : DK / 32][NT][64][8];  // NW < 4: the state before the chunk, as operands
   f32x4 qs[NW == 4 ? NW : 1][NW == 4 ? 4 : 1][64];           // NW = 4: Q S^T
   f32x4 u[NW][4][64];
   f16 P[6][2][64][8];
@@ -649,7 +650,7 @@ __device__ __forceinline__ void fetch_record(void* to, const ChunkRec* rec, int 
 // Fragment (W, J) of P = tril(q_i.k_j e^{G_i - G_j}), rows 16 W .., columns 32 J .., with a scale of its own per row,
 // so that no fragment waits for another; the one on the diagonal also leaves q's factors.
 template <int W, int J, int DK, bool BF, int NW>
-__device__ __forceinline__ void make_p(ChainLds<DK, NW>& L, const Operands<DK>& op, int lane, bool l2norm, float scale) {
+__device__ __forceinline__ void make_p(ChainLds<DK, NW, kParts<BF>>& L, const Operands<DK>& op, int lane, bool l2norm, float scale) {
   constexpr int NJ = DK / 32, F = W + (W > 2 ? 1 : 0) + J, T0 = 2 * J, NT = W > T0 ? 2 : 1;  // column tiles T0 .. T0 + NT - 1
   constexpr bool diag = T0 + NT - 1 == W;
   const int g = lane >> 4, c = lane & 15, i = 16 * W + c;
@@ -720,7 +721,7 @@ template <int DK, bool BF, int NW>
 __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(64 * (2 * NW + kFetchers<NW>)) void
 delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, const int* order, int64_t slot0, int64_t slot1) {
   constexpr int NM = DK / 16, NJ = DK / 32, NT = kParts<BF>, NF = kFetchers<NW>, NP = NF ? NF : NW;
-  __shared__ __align__(16) ChainLds<DK, NW> L;
+  __shared__ __align__(16) ChainLds<DK, NW, NT> L;
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave % NW;
   // Workgroups go to the eight dies in turn: all that share a key head run on one, next to its L2.
@@ -783,10 +784,9 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, const int* order, int64_t 
       split_all<NM>(S, ssc, s);
       if constexpr (NW < 4)
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          *(h8*)L.S[w][j][0][lane] = s[0][j];
-          *(h8*)L.S[w][j][1][lane] = s[1][j];
-        }
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int q = 0; q < NT; ++q) *(h8*)L.S[w][j][q][lane] = s[q][j];
       if constexpr (!BF) {
         sinv *= sfac;
         if (g == 0) L.sfac[i & 1][w][c] = sinv;
@@ -796,7 +796,7 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, const int* order, int64_t 
       rows_product<DK, BF, false>(op.k, lane, s, ks);
       if constexpr (NW == 4) {
         f32x4 qs[4];
-        rows_product<DK, BF, true>(op.q, lane, (const h8 (&)[2][NJ])s, qs);
+        rows_product<DK, BF, true>(op.q, lane, s, qs);
 #pragma unroll
         for (int t = 0; t < 4; ++t) L.qs[w][t][lane] = qs[t];
       }
@@ -967,12 +967,11 @@ delta_chain_kernel(DeltaArgs a, const ChunkRec* recs, const int* order, int64_t 
     f32x4 qs[4];
     f32x4 sinv;
     if (NW < 4 && outputs) {
-      h8 s[2][NJ];
+      h8 s[NT][NJ];
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        s[0][j] = *(const h8*)L.S[w][j][0][lane];
-        s[1][j] = *(const h8*)L.S[w][j][1][lane];
-      }
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int q = 0; q < NT; ++q) s[q][j] = *(const h8*)L.S[w][j][q][lane];
       rows_product<DK, BF, true>(op.q, lane, s, qs);
     }
     if (outputs) sinv = BF ? f32x4{1.0f, 1.0f, 1.0f, 1.0f} : *(const f32x4*)&L.sfac[i & 1][w][4 * g];

@@ -75,14 +75,14 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// 2^s with m 2^s in [2^14, 2^15) for m > 0 (s at most 126: smaller m stay small), and 2^-s.
+// 2^s with m 2^s in [2^14, 2^15) for m > 0 (s at most 126: smaller m stay small), and 2^-s. Of a maximum that is not
+// finite 2^-s is infinite, so that what was too small beside it does not come back as zero.
 __device__ __forceinline__ float pow2_scale(float m, float& inv) {
   uint32_t e = __builtin_bit_cast(uint32_t, m) & 0x7f800000u;
   e = e < (15u << 23) ? (15u << 23) : e;
-  inv = __builtin_bit_cast(float, e - (14u << 23));
+  inv = __builtin_bit_cast(float, e) * 0x1p-14f;
   return __builtin_bit_cast(float, (268u << 23) - e);
 }
-
 
 // The largest of v >= 0 over the four lanes of a column (16 apart). As whole numbers, which order as the floats
 // do: the compiler drops a float maximum of the two results of one lane swap.

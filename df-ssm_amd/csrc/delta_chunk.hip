@@ -105,10 +105,11 @@ __device__ __forceinline__ u32x4 row_load16(Rsrc r, int voff, int soff) {
   return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, 0));
 }
 
-// max(m, |x0|, .. |x3|), in two instructions (fmaxf first makes each operand canonical, a third instruction each).
+// max(m, |x0|, .. |x3|), a NaN if one is: two instructions. (Left to the compiler, which knows what has to pass between a
+// matrix instruction and the first reading of its result; for inline assembly it keeps no such distance.)
 __device__ __forceinline__ float max4(const f32x4& x, float m) {
-  asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(m) : "v"(x[0]), "v"(x[1]));
-  asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(m) : "v"(x[2]), "v"(x[3]));
+#pragma unroll
+  for (int e = 0; e < 4; ++e) m = __builtin_elementwise_maximum(m, __builtin_fabsf(x[e]));
   return m;
 }
 typedef f16 h2 __attribute__((ext_vector_type(2)));

@@ -1055,13 +1055,11 @@ hipError_t launch_chunked(const DeltaArgs& a, void* ws, hipStream_t s) {
     const int64_t tasks = n * ng, resident = 512;  // two workgroups to a CU (256: 631 us for 615, 1024: 617)
     const dim3 grid((unsigned)(tasks < resident ? tasks : resident));
     hipLaunchKernelGGL((delta_prep_kernel<DK, BF>), grid, dim3(256), 0, s, a, r, order, s0, tasks);
-    // Few heads: a value column tile to a workgroup, so that all CUs have one or two and a chunk passes quickly. Many:
-    // four, which make P once for 64 columns. NW = 1, 2, 4: 64 heads of 4 tiles, 16411 tokens 613, 704 and 927 us; 12 x 2
-    // heads of 8 tiles 235, 265 and 350; 12 x 64 heads of 4, ragged, 389, 263 and 223; 64 x 80 heads of 4 tiles 1912, 1222
-    // and 1000.
-    if (heads * ((tiles + 1) / 2) <= 256) launch_chain<DK, BF, 1>(a, r, order, s0, s0 + n, s);
-    else if (heads * ((tiles + 3) / 4) <= 256) launch_chain<DK, BF, 2>(a, r, order, s0, s0 + n, s);
-    else launch_chain<DK, BF, 4>(a, r, order, s0, s0 + n, s);
+    switch (chain_tiles(heads, tiles)) {
+      case 1: launch_chain<DK, BF, 1>(a, r, order, s0, s0 + n, s); break;
+      case 2: launch_chain<DK, BF, 2>(a, r, order, s0, s0 + n, s); break;
+      default: launch_chain<DK, BF, 4>(a, r, order, s0, s0 + n, s);
+    }
   }
   return hipGetLastError();
 }

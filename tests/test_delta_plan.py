@@ -1,5 +1,6 @@
-"""The chunked delta rule's arithmetic of passes (csrc/delta_plan.h, which host and device share), built for the CPU:
-no launch reads a record that its workspace does not hold. No GPU needed."""
+"""The chunked delta rule's arithmetic of launches (csrc/delta_plan.h, which host and device share), built for the CPU:
+no launch reads a record that its workspace does not hold, and the GPU tests' shapes reach every width of the chain.
+No GPU needed."""
 import ctypes
 import os
 import subprocess
@@ -15,6 +16,7 @@ extern "C" void pass_chunks(int64_t first, int64_t nch, int64_t slot0, int64_t s
   out[0] = p.begin;
   out[1] = p.count;
 }
+extern "C" int chain_tiles(int64_t heads, int64_t tiles) { return dfssm::chain_tiles(heads, tiles); }
 """
 
 
@@ -55,3 +57,18 @@ def test_records_of_a_pass(plan, name, per):
                 assert begin == done and slot0 <= at + begin and at + begin + count <= slot1, (b, slot0)
                 done += count
         assert done == nch
+
+
+def tiles_of(plan, lens, Hv, Dv):
+    return plan.chain_tiles(ctypes.c_int64(len(lens) * Hv), ctypes.c_int64(Dv // 16))
+
+
+def test_shapes_of_the_gpu_tests(plan):
+    """A change of the rule must not leave a width without a test."""
+    import test_gpu_delta_nonfinite as nonfinite
+    import test_gpu_delta_overwrite as overwrite
+    import test_gpu_delta_widths as widths
+    for want, (lens, _, Hv, Dv) in widths.SHAPES:
+        assert tiles_of(plan, lens, Hv, Dv) == want
+    for module in (nonfinite, overwrite):
+        assert {(tiles_of(plan, lens, Hv, Dv)) for lens, _, Hv, _, Dv in module.SHAPES} == {1, 2, 4}

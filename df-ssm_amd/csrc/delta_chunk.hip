@@ -24,7 +24,10 @@
 // no scale. (Q S^T is no exception, though its sum with P U is rounded to 16 bits: where a token overwrites what the
 // state has for its key, the two nearly cancel.) A product of two pairs leaves out lo lo, 2^-24 of it. So an fp32 state
 // comes out as from fp32 arithmetic (2e-7 of its norm), at 2 or 3 matrix instructions per product instead of the 8 times
-// as slow fp32 ones.
+// as slow fp32 ones. A pair's value far below the largest M of its scale keeps fewer bits than 22: below 2^-17 M it is off
+// by up to 2^-39 M, the last of a subnormal half. That shows where a large v - .. is forgotten again in the same 64
+// tokens and small ones follow (three bf16 parts of T, P, V - .. and U would need six products for three, and 18 KiB more
+// LDS, which 32 columns to a workgroup do not have).
 // G is summed in fp64, so that differences survive a decay of any size in the same chunk; -inf is held to -1e5.
 #include "common.h"
 #include "delta.h"

@@ -210,7 +210,7 @@ def _rows32(t: torch.Tensor, width: int):
 
 
 def _delta_call(step: bool, q, k, v, g, beta, state, cu_seqlens, slots, scale, l2norm, out, state_out, n_seq):
-    """Checks (tokens, heads, dim) arguments, launches and returns out."""
+    """Checks (tokens, heads, dim) arguments, launches and returns out. n_seq None: a sequence per token."""
     T_, f32 = torch.Tensor, torch.float32
     dt = q.dtype if isinstance(q, T_) else None
     kind = _TYPE16.get(dt)
@@ -232,6 +232,8 @@ def _delta_call(step: bool, q, k, v, g, beta, state, cu_seqlens, slots, scale, l
                          f"{tuple(gs)}, {tuple(beta.shape)}")
     T, Hk, Dk = qs
     _, Hv, Dv = vs
+    if n_seq is None:
+        n_seq = T
     if Dk not in (64, 128) or Dv % 16 or not 16 <= Dv <= 256 or Hk < 1 or Hv < 1 or Hv % Hk:
         raise ValueError("k_dim must be 64 or 128, v_dim a multiple of 16 up to 256, and the value heads a multiple "
                          f"of the key heads; got k_dim {Dk}, v_dim {Dv}, {Hv} and {Hk} heads")
@@ -313,8 +315,7 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     the slot of each sequence (default 0..B-1); a negative one marks padding (zeros returned), one past the
     state or taken by an earlier row gives NaN, and neither touches a state. scale defaults to Dk^-0.5;
     l2norm divides q and k by sqrt(sum x^2 + 1e-6) first. out, if given, overlaps none of the others."""
-    return _delta_call(True, q, k, v, g, beta, state, None, slots, scale, l2norm, out, state_out,
-                       q.shape[0])
+    return _delta_call(True, q, k, v, g, beta, state, None, slots, scale, l2norm, out, state_out, None)
 
 
 def gated_delta_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
@@ -336,13 +337,18 @@ def gated_delta_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: to
             raise ValueError("cu_seqlens must be (sequences + 1,)")
         return _delta_call(False, q, k, v, g, beta, state, cu_seqlens.contiguous(), slots, scale, l2norm,
                            out, state_out, cu_seqlens.numel() - 1)
+    for t, n in ((q, "q"), (k, "k"), (v, "v"), (g, "g"), (beta, "beta")):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{n} must be a tensor")
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4 or g.dim() != 3 or beta.dim() != 3:
         raise ValueError("without cu_seqlens: q, k, v (batch, tokens, heads, dim), g, beta (batch, tokens, heads)")
     B, T = q.shape[:2]
     if any(t.shape[:2] != (B, T) for t in (k, v, g, beta)):
         raise ValueError("q, k, v, g and beta must agree in batch and tokens")
-    if out is not None and not out.is_contiguous():
-        raise ValueError("out must be contiguous")
+    if out is not None:
+        _need(out, q.dtype, "out")
+        if out.shape != v.shape or not out.is_contiguous():
+            raise ValueError("out must be contiguous and have v's shape")
     o = _delta_call(False, q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1), g.flatten(0, 1),
                     beta.flatten(0, 1), state, None, slots, scale, l2norm,
                     None if out is None else out.flatten(0, 1), state_out, B)

@@ -390,9 +390,10 @@ def sample_filtered(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_
     rank by index.
 
     temperature, top_p, min_p: numbers, or (B,) fp32 on the device; top_k: a number, or (B,) int32. temperature
-    <= 0 takes the most probable token; top_k <= 0, top_p >= 1, min_p <= 0 filter nothing. NaN counts as -inf; a
-    row whose logits are all -inf gives -1. V at most 262144; rows may be strided. With want_logprob also the
-    logarithm of each token's share of what was kept, (B,) fp32."""
+    <= 0 or NaN takes the most probable token; top_k <= 0, top_p >= 1 or NaN, min_p <= 0 filter nothing, min_p > 1
+    or NaN leaves the most probable one. A NaN logit counts as -inf; a row whose logits are all -inf gives -1. V at
+    most 262144; rows may be strided. With want_logprob also the logarithm of each token's share of what was kept,
+    (B,) fp32."""
     kind = LOGIT_TYPE.get(logits.dtype) if isinstance(logits, torch.Tensor) else None
     if kind is None:
         raise TypeError("logits must be a float16, bfloat16 or float32 tensor")

@@ -298,8 +298,8 @@ typedef struct dfssm_filter {
   const float* min_ps;
   float temperature;
   int32_t top_k;               /* <= 0: no limit */
-  float top_p;                 /* >= 1: no limit */
-  float min_p;                 /* <= 0: no limit */
+  float top_p;                 /* >= 1 or NaN: no limit */
+  float min_p;                 /* <= 0: no limit; > 1 or NaN: rank 0 alone */
 } dfssm_filter;
 /* logits (batch, vocab) of `type` (DFSSM_TYPE_*), rows ld elements apart; u (batch) in [0, 1) (held to it; NaN
  * counts as 0); next (batch) receives the tokens and logprob (batch, may be NULL) the logarithm of their share

@@ -169,7 +169,7 @@ def _check_token_range(t: torch.Tensor, vocab: int) -> None:
         raise IndexError(f"token id out of range [0, {vocab}): min {lo}, max {hi}")
 
 
-def _draw_filters(temperature, top_k, top_p, min_p, penalty, state_df=None) -> bool:
+def _draw_filters(temperature, top_k, top_p, min_p, penalty, state_df=None, vocab=1) -> bool:
     """Whether generate()'s arguments ask for the draw with top_k or min_p; ValueError for what it does not do."""
     if not 0 <= operator.index(top_k) < 2**31:
         raise ValueError(f"top_k must be an int32 of at least 0, got {top_k}")
@@ -183,6 +183,8 @@ def _draw_filters(temperature, top_k, top_p, min_p, penalty, state_df=None) -> b
         raise ValueError(f"temperature must be finite and > 0 and top_p >= 0, got {temperature} and {top_p}")
     if penalty != 1.0:
         raise ValueError("repetition_penalty is not supported together with top_k or min_p")
+    if vocab > ops.MAX_DRAW_VOCAB:
+        raise ValueError(f"top_k and min_p draw from vocabularies of up to {ops.MAX_DRAW_VOCAB}, not of {vocab}")
     return True
 
 
@@ -694,7 +696,7 @@ class DFSSMModel:
         if prompt.dim() != 2 or prompt.shape[0] != B or prompt.shape[1] < 1:
             raise ValueError(f"prompt must be (batch={B}, T >= 1), got {tuple(prompt.shape)}")
         _check_token_range(prompt, self.cfg.vocab_size)  # before any kernel reads the ids
-        filtered = _draw_filters(temperature, top_k, top_p, min_p, repetition_penalty, state_df)
+        filtered = _draw_filters(temperature, top_k, top_p, min_p, repetition_penalty, state_df, self.cfg.vocab_size)
         self.reset_state()
         prompt = prompt.to(self.device, torch.int64)
         if state_df is not None:

@@ -358,6 +358,7 @@ def gated_delta_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: to
 # ---------------------------------------------------------------------------------------------
 # token draw
 # ---------------------------------------------------------------------------------------------
+MAX_DRAW_VOCAB = 262144   # tokens of a row of sample_filtered
 LOGIT_TYPE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}   # DFSSM_TYPE_*
 
 
@@ -399,8 +400,8 @@ def sample_filtered(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_
         raise TypeError("logits must be a float16, bfloat16 or float32 tensor")
     _need(logits, logits.dtype, "logits")
     _need(u, torch.float32, "u")
-    if logits.dim() != 2 or not 1 <= logits.shape[1] <= 262144:
-        raise ValueError(f"logits must be (B, V) with 1 <= V <= 262144, got {tuple(logits.shape)}")
+    if logits.dim() != 2 or not 1 <= logits.shape[1] <= MAX_DRAW_VOCAB:
+        raise ValueError(f"logits must be (B, V) with 1 <= V <= {MAX_DRAW_VOCAB}, got {tuple(logits.shape)}")
     dev = logits.device
     B, V = logits.shape
     if u.shape != (B,):

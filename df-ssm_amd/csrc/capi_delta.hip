@@ -57,9 +57,13 @@ DeltaArgs delta_args(const dfssm_delta* d) {
 }
 
 // Prompts that run token by token: too few tokens for a chunk's fixed work. The lengths behind cu_seqlens are
-// on the device, so the rule there goes by all tokens, which any one sequence may have. 64 heads of 64 x 128, token
-// by token and in chunks: 32 sequences of 8 tokens 49 and 78 us, 12: 66 and 79, 16: 82 and 79; one sequence of 8
-// tokens 20.3 and 23.6 us, 32: 23.0 and 23.5.
+// on the device, so the rule there goes by all tokens, which any one sequence may have (32 packed sequences of one token
+// run 32 chunks). Kernels in a replayed graph, token by token and in chunks, for sequences of 12 | 16 | 24 tokens, fp16:
+//   64 heads of 64 x 128   one sequence 9.9, 12.5 | 12.1, 12.6 | 17.2, 12.8 us   32: 68, 78 | 84, 79 | 117, 81
+//   80 heads of 64 x 128                10.3, 16.8 | 12.8, 17.3 | 18.0, 17.0         83, 93 | 99, 97 | 142, 100
+//   2 heads of 256 x 64                 7.9, 11.2 | 9.7, 11.3 | 13.4, 11.3           12.5, 17.5 | 15.4, 16.8 | 20.8, 17.3
+//   12 heads of 128 x 64                8.4, 11.5 | 10.5, 11.9 | 14.7, 11.9          20.7, 27.2 | 25.6, 27.4 | 35, 27
+//   40 heads of 128 x 128               10.1, 17.3 | 12.6, 17.2 | 17.3, 17.8         78, 89 | 98, 89 | 139, 90
 constexpr int kTokenPath = 12;
 bool by_tokens(const DeltaArgs& a) { return (a.cu ? a.n_tokens : a.len) <= kTokenPath; }
 

@@ -44,7 +44,8 @@ __device__ __forceinline__ uint16_t f2w(float x) {  // RNE
 __device__ __forceinline__ float l2_factor(float ss) { return __builtin_amdgcn_rsqf(ss + 1e-6f); }  // (1 ulp)
 
 // Tokens [t0, t1) of sequence b. Offsets read from device memory are held to [0, n_tokens] and an end
-// before its start is an empty sequence, so no value of cu reaches past the tensors.
+// before its start is an empty sequence, so no value of cu reaches past the tensors. (Offsets that fall may still make
+// sequences overlap, or leave chunks that nothing prepared: the results are then not specified.)
 __device__ __forceinline__ void seq_range(const DeltaArgs& a, int b, int64_t& t0, int64_t& t1) {
   if (!a.cu) {
     t0 = (int64_t)b * a.len;

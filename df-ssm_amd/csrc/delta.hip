@@ -134,8 +134,9 @@ static void launch_rows(const DeltaArgs& a, hipStream_t s) {
 }
 // 16 KiB of state to a workgroup where there are plenty of them, else 16 rows. One token, state streamed, with
 // 4, 8, 16 and 32 KiB: Dk = 64, 37 x 24 heads of 208 rows 33.5, 24.0 and 23.8 us; Dk = 128, 32 x 64 heads of 64
-// rows 29.7 (8), 28.5 and 27.4 us, 64 x 80 heads of 64 rows 63.0, 62.8 and 64.1 us. With one sequence of 64 heads
-// 16 rows make 256 workgroups and 15.0 us per call, 32 rows 15.8.
+// rows 29.7 (8), 28.5 and 27.4 us, 64 x 80 heads of 64 rows 63.0, 62.8 and 64.1 us. Few, the kernel in a replayed graph
+// with 16 rows and with 16 KiB: 64 heads of 64 x 128, one sequence 3.4 and 3.7 us, two 4.0 and 4.1, four 5.3 and 4.9;
+// one of 2 heads of 256 x 64 3.0 and 4.0, eight of 12 heads of 128 x 64 4.1 and 4.4.
 template <int DK, bool BF>
 static hipError_t launch_token(const DeltaArgs& a, hipStream_t s) {
   const int64_t tiles = (int64_t)a.n_seq * a.Hv * (a.Dv / 16);

@@ -9,12 +9,13 @@
 // them.
 //
 // What bounds it. One long sequence: the path from chunk to chunk (K S^T, T (V - ..), the new state: three dependent
-// products with a split into 16-bit parts before each), 4800 clocks a chunk; 16411 tokens x 64 heads of 64 x 128 take
-// 0.61 ms, 0.09 of it the preparation (fp16; 416 MB, 0.085 ms of copying). Ragged ones: that path of the longest at 64
-// value columns to a workgroup (NW = 4), 8500 clocks. Many sequences: memory. 64 x 512 tokens x 80 heads move 2.4 GB that
-// they cannot do without, 0.57 GB of T's records once out and once in, and k twice, 4.2 GB in 0.99 ms, 0.27 of it the
-// preparation (bf16; 4.9 TB/s is what a copy reaches). Records in passes small enough for the last-level cache were slower:
-// each pass reads and writes the states.
+// products with a split into 16-bit parts before each, all of a chunk's on one wave), 4700 clocks a chunk; 16411 tokens x
+// 64 heads of 64 x 128 take 0.59 ms, 0.09 of it the preparation (fp16; 416 MB, 0.085 ms of copying; the matrix cores are
+// busy 16% of the chain). Ragged ones: that path of the longest at 64 value columns to a workgroup (NW = 4), 8200 clocks.
+// Many sequences: memory. 64 x 512 tokens x 80 heads move 2.4 GB that they cannot do without, 0.57 GB of T's records once
+// out and once in, and k twice, 4.2 GB in 1.00 ms, 0.27 of it the preparation (bf16; 4.9 TB/s is what a copy reaches; of
+// the chain the matrix cores are busy 32%). Records in passes small enough for the last-level cache were slower: each
+// pass reads and writes the states.
 //
 // Numbers. States, sums and everything between products are fp32. Products run on the 16-bit matrix cores with
 // fp32 accumulation. q and k are exact operands there, in their own type. A factor of fp32 values is a sum of
@@ -1050,12 +1051,14 @@ hipError_t launch_chunked(const DeltaArgs& a, void* ws, hipStream_t s) {
   if ((heads + 8 * rep) * tiles > 0x7fffffff || per * ng > 0x7fffffff) return hipErrorInvalidValue;
   ChunkRec* r = (ChunkRec*)ws;
   // Workgroups begin in order, and one that begins late with the longest chain ends late: twelve sequences of 0 to 3001
-  // tokens, 64 heads, 275 us in the order they come and 251 by length (bf16); 32 of 50 to 2200 tokens 469 and 433; 64
-  // of one length 1059 and 1058. (More than kOrdered even out by themselves.)
+  // tokens, 64 heads, 235 us in the order they come and 211 by length (bf16); 32 of 50 to 2200 tokens 837 and 815; 64
+  // of one length 1006 and 1005. (More than kOrdered even out by themselves.)
   int* order = a.cu && a.n_seq > 1 && a.n_seq <= kOrdered ? (int*)(r + slots_per_pass(a) * a.Hv) : nullptr;
   for (int64_t s0 = 0; s0 < slots; s0 += per) {
     const int64_t n = s0 + per < slots ? per : slots - s0;
-    const int64_t tasks = n * ng, resident = 512;  // two workgroups to a CU (256: 631 us for 615, 1024: 617)
+    // Two workgroups to a CU: 16411 tokens x 64 heads 592 us (with 256 workgroups 605, with 1024 591), twelve ragged
+    // sequences 211 (218, 214).
+    const int64_t tasks = n * ng, resident = 512;
     const dim3 grid((unsigned)(tasks < resident ? tasks : resident));
     hipLaunchKernelGGL((delta_prep_kernel<DK, BF>), grid, dim3(256), 0, s, a, r, order, s0, tasks);
     switch (chain_tiles(heads, tiles)) {

@@ -21,8 +21,8 @@ constexpr PassChunks pass_chunks(int64_t first, int64_t nch, int64_t slot0, int6
 
 // Tiles of 16 value columns to a workgroup of the chain, of `heads` sequences times value heads and `tiles` tiles a head.
 // Few: one, so that all CUs have one or two and a chunk passes quickly. Many: four, which make P once for 64 columns.
-// With 1, 2, 4: 64 heads of 4 tiles, 16411 tokens 613, 704 and 927 us; 12 x 2 heads of 8 tiles 235, 265 and 350; 12 x 64
-// heads of 4, ragged, 389, 263 and 223; 64 x 80 heads of 4 tiles 1912, 1222 and 1000.
+// With 1, 2, 4: 64 heads of 4 tiles, 16411 tokens 593, 695 and 890 us; 12 x 2 heads of 8 tiles 227, 264 and 327; 12 x 64
+// heads of 4, ragged, 367, 234 and 211; 64 x 80 heads of 4 tiles 1884, 1235 and 1005.
 constexpr int chain_tiles(int64_t heads, int64_t tiles) {
   return heads * ((tiles + 1) / 2) <= 256 ? 1 : (heads * ((tiles + 3) / 4) <= 256 ? 2 : 4);
 }

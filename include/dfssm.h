@@ -365,8 +365,10 @@ typedef struct dfssm_delta {
                              slot is >= n_slots, or that of an earlier sequence of the call, is refused: its
                              rows of out are NaN. Neither touches a state. */
   const int32_t* cu_seqlens; /* dfssm_gated_delta_prefill: (n_seq + 1) first tokens, sequence b has tokens
-                             cu_seqlens[b] .. cu_seqlens[b + 1]; NULL: n_tokens / n_seq tokens each. Offsets
-                             outside [0, n_tokens] are held to it; rows of no sequence stay as they were. */
+                             cu_seqlens[b] .. cu_seqlens[b + 1], none below the one before; NULL: n_tokens / n_seq
+                             tokens each. Offsets outside [0, n_tokens] are held to it; rows of no sequence stay as
+                             they were. Where offsets fall, outputs and states are not specified; nothing outside
+                             the tensors is read or written. */
   void* out;              /* (tokens, v_heads, v_dim), `type` */
   int64_t ld_q, ld_k, ld_v, ld_g, ld_beta, ld_out; /* elements */
   int64_t n_tokens;

@@ -28,7 +28,10 @@
 // as slow fp32 ones. A pair's value far below the largest M of its scale keeps fewer bits than 22: below 2^-17 M it is off
 // by up to 2^-39 M, the last of a subnormal half. That shows where a large v - .. is forgotten again in the same 64
 // tokens and small ones follow (three bf16 parts of T, P, V - .. and U would need six products for three, and 18 KiB more
-// LDS, which 32 columns to a workgroup do not have).
+// LDS, which 32 columns to a workgroup do not have). And the chunk's equations have as many factors A_ij as pairs of
+// tokens, each rounded by itself: where neighbouring keys are alike and beta |k|^2 is close to 2, so that each token undoes
+// the one before and nothing dies out, a state is off by 2^-15 of its largest value after a few chunks, in fp32
+// throughout too.
 // G is summed in fp64, so that differences survive a decay of any size in the same chunk; -inf is held to -1e5.
 #include "common.h"
 #include "delta.h"

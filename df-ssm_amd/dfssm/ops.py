@@ -324,7 +324,8 @@ def gated_delta_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: to
     """The gated delta rule over whole prompts (dfssm_gated_delta_prefill), from the states the sequences
     have to those they leave: what gated_delta_step gives token by token, up to rounding in fp32 (relative to
     the largest v - S' k of the value column in 64 tokens: beside one more than 2^17 times as large, a token's
-    own is off by up to 2^-39 of that one).
+    own is off by up to 2^-39 of that one; and where 64 tokens have one key and beta |k|^2 close to 2, rounding
+    grows to about 2^-15 of the state).
 
     Either packed, q, k (T, Hk, Dk), v (T, Hv, Dv), g, beta (T, Hv) with cu_seqlens (n + 1,) int32 on the
     device (sequence b has tokens cu_seqlens[b] .. cu_seqlens[b + 1], which must not fall; any length, zero

@@ -329,8 +329,8 @@ def gated_delta_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: to
 
     Either packed, q, k (T, Hk, Dk), v (T, Hv, Dv), g, beta (T, Hv) with cu_seqlens (n + 1,) int32 on the
     device (sequence b has tokens cu_seqlens[b] .. cu_seqlens[b + 1], which must not fall; any length, zero
-    included; rows of no sequence are left as they are in out), or one dimension more in front and no cu_seqlens: (B, T, ...).
-    The other arguments are those of gated_delta_step. A value that is not finite may also make up to 63 tokens
+    included; rows of no sequence are left as they are in out), or one dimension more in front and no
+    cu_seqlens: (B, T, ...). The other arguments are those of gated_delta_step. A value that is not finite may also make up to 63 tokens
     before it not finite."""
     if cu_seqlens is not None:
         _need(cu_seqlens, torch.int32, "cu_seqlens")

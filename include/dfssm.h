@@ -389,8 +389,9 @@ int dfssm_gated_delta_step(const dfssm_delta* args, void* stream);
  * dfssm_gated_delta_step gives token by token, up to fp32 rounding (relative to the largest v - S' k that the value
  * column has in 64 tokens: beside one more than 2^17 times as large, forgotten or not, a token's own is off by up to
  * 2^-39 of that one; and where 64 tokens have one key and beta |k|^2 close to 2, each undoing the one before, rounding
- * grows to about 2^-15 of the state). workspace: 16-byte aligned device memory of dfssm_gated_delta_workspace_bytes(args) bytes (at
- * most about 1 GiB; 0: none needed, NULL allowed), for this call alone while it runs; its contents do not matter.
+ * grows to about 2^-15 of the state). workspace: 16-byte aligned device memory of
+ * dfssm_gated_delta_workspace_bytes(args) bytes (at most about 1 GiB; 0: none needed, NULL allowed), for this call
+ * alone while it runs; its contents do not matter.
  * A value that is not finite reaches what it does token by token and may also reach up to 63 tokens before it in its
  * sequence (of its value column, or of the heads that read it): their rows of out are not finite there. */
 size_t dfssm_gated_delta_workspace_bytes(const dfssm_delta* args);

@@ -170,41 +170,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 template <bool BF>
 constexpr int kParts = BF ? 3 : 2;  // of an fp32 factor beside rows of the type
 
-// The sequence and chunk of slot s of the launch's chunk numbering: sequence b starts at slot
-// floor(t0 / 64) + b, which needs no sums over the lengths and leaves room for every chunk. The lanes of a wave
-// look at 64 sequences at once, and the sequence found is kept for the slots that follow.
-struct Where {
-  int64_t first, t0, t1;  // slot, tokens of a sequence
-};
-__device__ __forceinline__ void find_seq(const DeltaArgs& a, int64_t s, Where& q) {
-  const int lane = threadIdx.x & 63;
-  int lo = 0, n = a.n_seq;  // the last sequence that starts at or before s is one of lo .. lo + n - 1
-  while (n > 1) {
-    const int step = (n + 63) / 64, i = lo + lane * step;
-    bool before = false;
-    if (i < lo + n) {
-      int64_t t0, t1;
-      seq_range(a, i, t0, t1);
-      before = t0 / kC + i <= s;
-    }
-    const int k = __popcll(__ballot(before));  // the starts rise, so the first k lanes (lane 0's always does)
-    const int end = lo + n;
-    lo += (k > 0 ? k - 1 : 0) * step;
-    n = min(step, end - lo);
-  }
-  seq_range(a, lo, q.t0, q.t1);
-  q.first = q.t0 / kC + lo;
-}
-// Tokens [tok, tok + len) of slot s; 0 where it holds none.
-__device__ __forceinline__ int chunk_of(const DeltaArgs& a, int64_t s, Where& q, int64_t& tok) {
-  if (s < q.first || (s - q.first) * kC >= q.t1 - q.t0) find_seq(a, s, q);
-  const int64_t c = s - q.first;
-  tok = 0;
-  if (c < 0 || c * kC >= q.t1 - q.t0) return 0;
-  tok = q.t0 + c * kC;
-  return (int)(q.t1 - tok < kC ? q.t1 - tok : kC);
-}
-
 // ---------------------------------------------------------------------------------------------
 // Preparation: a chunk and value head per wave, which needs no barrier. The four waves of a workgroup take four
 // heads, which find a key head's rows in the L1 cache; a workgroup goes over several chunks, and the rows of the
@@ -298,7 +263,7 @@ delta_prep_kernel(DeltaArgs a, ChunkRec* recs, int* order, int64_t slot0, int64_
   if (order && blockIdx.x == 0) order_by_length(a, (int*)lds, order);
   const int rep = a.Hv / a.Hk, nw = (a.Hv + 3) / 4;
 
-  Where seq{0, 0, 0};
+  Where seq{0, 0, 0, 0};
   PrepRows<DK> in;
   int64_t task = blockIdx.x, slot = 0;
   int h = 0, len = 0;
@@ -306,7 +271,7 @@ delta_prep_kernel(DeltaArgs a, ChunkRec* recs, int* order, int64_t slot0, int64_
     slot = task / nw;
     h = (int)(task % nw) * 4 + wave;
     int64_t tok;
-    len = chunk_of(a, slot0 + slot, seq, tok);
+    len = (int)tile_of<kC>(a, slot0 + slot, seq, tok);
     if (h >= a.Hv) {  // (a head there is, rows there are none)
       len = 0;
       h = 0;

@@ -56,6 +56,33 @@ class Delta(ctypes.Structure):
                                                  "l2norm")] + [("scale", ctypes.c_float)])
 
 
+class Conv(ctypes.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("x", "weight", "bias", "state", "state_out", "slots", "cu_seqlens", "out")] +
+                [(n, ctypes.c_int64) for n in ("ld_x", "ld_out", "n_tokens")] +
+                [(n, ctypes.c_int32) for n in ("n_seq", "n_slots", "channels", "width", "type", "silu")])
+
+
+class Scan(ctypes.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("x", "dt", "B", "C", "A_log", "D", "dt_bias", "state", "state_out", "slots",
+                                         "cu_seqlens", "out")] +
+                [(n, ctypes.c_int64) for n in ("ld_x", "ld_dt", "ld_B", "ld_C", "ld_out", "n_tokens")] +
+                [(n, ctypes.c_int32) for n in ("n_seq", "n_slots", "heads", "groups", "dim", "cols", "type", "dt_type",
+                                               "softplus")])
+
+
+class Gated(ctypes.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("x", "gate", "weight", "out")] +
+                [(n, ctypes.c_int64) for n in ("ld_x", "ld_gate", "ld_out", "rows")] +
+                [(n, ctypes.c_int32) for n in ("cols", "groups", "type", "gate_first")] + [("eps", ctypes.c_float)])
+
+
+class Residual(ctypes.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("x", "residual", "post_weight", "scales", "weight", "out", "residual_out")] +
+                [(n, ctypes.c_int64) for n in ("ld_x", "ld_residual", "ld_out", "ld_residual_out", "rows")] +
+                [(n, ctypes.c_int32) for n in ("cols", "type", "residual_type")] +
+                [("scale", ctypes.c_float), ("eps", ctypes.c_float)])
+
+
 class Filter(ctypes.Structure):
     _fields_ = ([(n, c_void_p) for n in ("temperatures", "top_ks", "top_ps", "min_ps")] +
                 [("temperature", ctypes.c_float), ("top_k", ctypes.c_int32), ("top_p", ctypes.c_float),
@@ -96,6 +123,12 @@ _SIGS = {
     "dfssm_gated_delta_step": (c_int, [ctypes.POINTER(Delta), P]),
     "dfssm_gated_delta_workspace_bytes": (c_size_t, [ctypes.POINTER(Delta)]),
     "dfssm_gated_delta_prefill": (c_int, [ctypes.POINTER(Delta), P, P]),
+    "dfssm_causal_conv_step": (c_int, [ctypes.POINTER(Conv), P]),
+    "dfssm_causal_conv_prefill": (c_int, [ctypes.POINTER(Conv), P]),
+    "dfssm_selective_scan_step": (c_int, [ctypes.POINTER(Scan), P]),
+    "dfssm_selective_scan_prefill": (c_int, [ctypes.POINTER(Scan), P]),
+    "dfssm_gated_norm": (c_int, [ctypes.POINTER(Gated), P]),
+    "dfssm_residual_norm": (c_int, [ctypes.POINTER(Residual), P]),
 }
 
 _lib = None

@@ -357,6 +357,415 @@ def gated_delta_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: to
 
 
 # ---------------------------------------------------------------------------------------------
+# a state space layer between its projections
+# ---------------------------------------------------------------------------------------------
+MAX_NORM_COLS = 16384   # DFSSM_NORM_MAX_COLS
+
+
+def _rows(t: torch.Tensor, width: int):
+    """t (rows, width) with contiguous rows at any distance up to 2^30, itself or a copy, that distance and its address."""
+    if t.is_contiguous():
+        return t, width, t.data_ptr()
+    ld, one = t.stride()
+    if t.shape[0] <= 1:
+        ld = width
+    if (one == 1 or width == 1) and 0 <= ld <= 1 << 30:
+        return t, ld, t.data_ptr()
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, width, t.data_ptr()
+
+
+def _need_all(dev: int, *named) -> None:
+    """Tensors of their types on device dev: (tensor, type, name) each."""
+    for t, dt, n in named:
+        _need(t, dt, n)
+    for t, _, n in named:
+        if t.get_device() != dev:
+            raise ValueError(f"{n} is on another device than x")
+
+
+def _own_rows(t: torch.Tensor, rows: int, ld: int, p: int, width: int, name: str) -> None:
+    """Refuses an output whose rows are not written in place (a copy was made) or overlap."""
+    if t.data_ptr() != p or (rows > 1 and ld < width):
+        raise ValueError(f"{name} must have contiguous rows that do not overlap")
+
+
+def _apart(t: torch.Tensor, u: torch.Tensor) -> bool:
+    """Whether no byte of t (rows, ..) lies among those of u: other memory, or other columns of the same rows."""
+    def span(x):
+        n = sum((s - 1) * d for s, d in zip(x.shape, x.stride())) + 1
+        return x.data_ptr(), x.data_ptr() + n * x.element_size()
+    if t.numel() == 0 or u.numel() == 0:
+        return True
+    (a0, a1), (b0, b1) = span(t), span(u)
+    if a1 <= b0 or b1 <= a0:
+        return True
+    ld = t.stride(0) * t.element_size()
+    if ld <= 0 or ld != u.stride(0) * u.element_size():
+        return False
+    wa, wb = (span(x[:1])[1] - span(x[:1])[0] for x in (t, u))
+    d = (b0 - a0) % ld
+    return d >= wa and d + wb <= ld
+
+
+def _states(state: torch.Tensor, state_out, shape, dev: int):
+    """state_out and both addresses."""
+    if state.dim() != len(shape) + 1 or state.shape[1:] != shape or not state.is_contiguous():
+        raise ValueError(f"state must be contiguous (slots, {', '.join(str(x) for x in shape)})")
+    p = state.data_ptr()
+    if state_out is None or state_out is state:
+        return state, p, p
+    _need(state_out, state.dtype, "state_out")
+    if state_out.shape != state.shape or not state_out.is_contiguous() or state_out.get_device() != dev:
+        raise ValueError("state_out must be contiguous, of state's shape and on its device")
+    o = state_out.data_ptr()
+    if o != p and abs(o - p) < state.numel() * state.element_size():
+        raise ValueError("state_out must be state or not overlap it")
+    return state_out, p, o
+
+
+def _slots(slots, state: torch.Tensor, n_seq: int, dev: int):
+    if slots is None:
+        if state.shape[0] < n_seq:
+            raise ValueError(f"state has {state.shape[0]} slots for {n_seq} sequences")
+        return None
+    _need(slots, torch.int32, "slots")
+    if slots.shape != (n_seq,):
+        raise ValueError(f"slots must be ({n_seq},)")
+    if slots.get_device() != dev:
+        raise ValueError("slots is on another device than x")
+    return slots.contiguous()
+
+
+def _offsets(cu_seqlens, dev: int):
+    _need(cu_seqlens, torch.int32, "cu_seqlens")
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+        raise ValueError("cu_seqlens must be (sequences + 1,)")
+    if cu_seqlens.get_device() != dev:
+        raise ValueError("cu_seqlens is on another device than x")
+    return cu_seqlens.contiguous()
+
+
+def _kind16(x) -> int:
+    kind = _TYPE16.get(x.dtype) if isinstance(x, torch.Tensor) else None
+    if kind is None:
+        raise TypeError("x must be a float16 or bfloat16 tensor")
+    if x.get_device() < 0:
+        raise TypeError("x must be a CUDA (HIP) tensor")
+    return kind
+
+
+def _run(dev: int, call, args, what: str) -> None:
+    """call(args, current stream) on device dev."""
+    if dev != _C.current_device():
+        with torch.cuda.device(dev):
+            rc = call(args, _C.stream())
+    else:
+        rc = call(args, _C.stream())
+    if rc:
+        _C.check(rc, what)
+
+
+def _conv_call(step: bool, x, weight, bias, state, cu_seqlens, slots, silu, out, state_out, n_seq):
+    kind = _kind16(x)
+    dt, dev = x.dtype, x.get_device()
+    _need_all(dev, (weight, dt, "weight"), (state, dt, "state"))
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"x must be (tokens, channels), got {tuple(x.shape)}")
+    T, C = x.shape
+    if weight.dim() != 2 or weight.shape[0] != C or not 2 <= weight.shape[1] <= 4:
+        raise ValueError(f"weight must be ({C}, 2 .. 4), got {tuple(weight.shape)}")
+    W = weight.shape[1]
+    if bias is not None:
+        _need_all(dev, (bias, dt, "bias"))
+        if bias.shape != (C,):
+            raise ValueError(f"bias must be ({C},)")
+        bias = bias.contiguous()
+    if cu_seqlens is not None:
+        cu_seqlens = _offsets(cu_seqlens, dev)
+        n_seq = cu_seqlens.numel() - 1
+    state_out, sp, so = _states(state, state_out, (C, W - 1), dev)
+    slots = _slots(slots, state, n_seq, dev)
+    if out is None:
+        out = x.new_empty(T, C)
+        ld_out, op = C, out.data_ptr()
+    else:
+        _need_all(dev, (out, dt, "out"))
+        if out.shape != x.shape:
+            raise ValueError("out must have x's shape")
+        _, ld_out, op = _rows(out, C)
+        _own_rows(out, T, ld_out, op, C, "out")
+        same = op == x.data_ptr() and (T <= 1 or ld_out == x.stride(0)) and (C == 1 or x.stride(1) == 1)
+        if not (step and same) and not _apart(out, x):
+            raise ValueError("out must not overlap x" + (" (or be x itself)" if step else ""))
+    if n_seq == 0:
+        return out
+    x, ld_x, xp = _rows(x, C)   # (copies live until the launch)
+    weight = weight.contiguous()
+    args = _C.Conv(xp, weight.data_ptr(), _C.ptr(bias), sp, so, _C.ptr(slots), _C.ptr(cu_seqlens), op, ld_x, ld_out, T,
+                   n_seq, state.shape[0], C, W, kind, 1 if silu else 0)
+    L = _C.lib()
+    _run(dev, L.dfssm_causal_conv_step if step else L.dfssm_causal_conv_prefill, args, "causal_conv")
+    return out
+
+
+def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, bias, state: torch.Tensor, slots=None, silu=True, out=None,
+                     state_out=None) -> torch.Tensor:
+    """One token per sequence of the short causal convolution (dfssm_causal_conv_step): per channel,
+    y = f(bias + sum_k weight[k] x_{t - W + 1 + k}), f(y) = y / (1 + e^-y) with silu, else y.
+
+    x (B, C), weight (C, W) with W = 2, 3 or 4 and bias (C,) or None, all fp16 or bf16; state (slots, C, W - 1) of the
+    same type, contiguous, the oldest first, updated in place or written to state_out (of the same shape; slots that no
+    sequence has are left as they are there). Rows of x and out may be strided; out may be x itself, and overlaps
+    nothing else. slots (B,) int32: the slot of each sequence (default 0..B-1); a negative one marks padding (zeros
+    returned), one past the state or taken by an earlier row gives NaN, and neither touches a state. Sums are fp32, out is
+    rounded once."""
+    return _conv_call(True, x, weight, bias, state, None, slots, silu, out, state_out,
+                      x.shape[0] if isinstance(x, torch.Tensor) and x.dim() else 0)
+
+
+def causal_conv_prefill(x: torch.Tensor, weight: torch.Tensor, bias, state: torch.Tensor, cu_seqlens=None, slots=None,
+                        silu=True, out=None, state_out=None) -> torch.Tensor:
+    """The short causal convolution over whole prompts (dfssm_causal_conv_prefill), from the states the sequences have to
+    those they leave: what causal_conv_step gives token by token, bit for bit.
+
+    Either packed, x (T, C) with cu_seqlens (n + 1,) int32 on the device (sequence b has tokens cu_seqlens[b] ..
+    cu_seqlens[b + 1], which must not fall; any length, zero included; rows of no sequence are left as they are in
+    out), or (B, T, C) and no cu_seqlens. The other arguments are those of causal_conv_step, but out overlaps no input."""
+    if cu_seqlens is not None:
+        return _conv_call(False, x, weight, bias, state, cu_seqlens, slots, silu, out, state_out, 0)
+    _kind16(x)
+    if x.dim() != 3:
+        raise ValueError("without cu_seqlens: x (batch, tokens, channels)")
+    if out is not None:
+        _need(out, x.dtype, "out")
+        if out.shape != x.shape or not out.is_contiguous():
+            raise ValueError("out must be contiguous and have x's shape")
+        out = out.flatten(0, 1)
+    return _conv_call(False, x.flatten(0, 1), weight, bias, state, None, slots, silu, out, state_out,
+                      x.shape[0]).view(x.shape)
+
+
+def _scan_call(step: bool, x, dt, A_log, B, C, state, D, dt_bias, cu_seqlens, slots, softplus, out, state_out, n_seq):
+    T_, f32 = torch.Tensor, torch.float32
+    kind = _kind16(x)
+    ty, dev = x.dtype, x.get_device()
+    if not (isinstance(dt, T_) and isinstance(A_log, T_) and isinstance(B, T_) and isinstance(C, T_)
+            and isinstance(state, T_) and (dt.dtype is ty or dt.dtype is f32) and A_log.dtype is f32 and B.dtype is ty
+            and C.dtype is ty and state.dtype is f32 and dt.get_device() == dev and A_log.get_device() == dev
+            and B.get_device() == dev and C.get_device() == dev and state.get_device() == dev):
+        _need_all(dev, (dt, f32 if isinstance(dt, T_) and dt.dtype is f32 else ty, "dt"), (A_log, f32, "A_log"), (B, ty, "B"),
+                  (C, ty, "C"), (state, f32, "state"))
+    xs, bs = x.shape, B.shape
+    if len(xs) != 3 or len(bs) != 3 or C.shape != bs or bs[0] != xs[0] or dt.shape != xs[:2]:
+        raise ValueError("shape mismatch: x (tokens, heads, dim), dt (tokens, heads), B, C (tokens, groups, cols); got "
+                         f"{tuple(xs)}, {tuple(dt.shape)}, {tuple(bs)}, {tuple(C.shape)}")
+    T, H, P = xs
+    _, G, N = bs
+    if N not in (64, 128) or P % 16 or not 16 <= P <= 256 or H < 1 or G < 1 or H % G:
+        raise ValueError("cols must be 64 or 128, dim a multiple of 16 up to 256, and the heads a multiple of the "
+                         f"groups; got cols {N}, dim {P}, {H} heads and {G} groups")
+    for t, n in ((A_log, "A_log"), (D, "D"), (dt_bias, "dt_bias")):
+        if t is not None:
+            if t is not A_log:
+                _need_all(dev, (t, f32, n))
+            if t.shape != (H,):
+                raise ValueError(f"{n} must be ({H},)")
+    if cu_seqlens is not None:
+        cu_seqlens = _offsets(cu_seqlens, dev)
+        n_seq = cu_seqlens.numel() - 1
+    state_out, sp, so = _states(state, state_out, (H, P, N), dev)
+    if sp % 16 or so % 16:
+        raise ValueError("state must be 16-byte aligned")
+    slots = _slots(slots, state, n_seq, dev)
+    width = H * P
+    if out is None:
+        out, ld_out = x.new_empty(xs), width
+    else:
+        _need_all(dev, (out, ty, "out"))
+        if out.shape != xs:
+            raise ValueError("out must have x's shape")
+        row, ld_out, _ = _rows16(out, width)
+        if row is not out or (T > 1 and ld_out < width):
+            raise ValueError("out must have contiguous heads and 16-byte aligned tokens that do not overlap")
+        if not all(_apart(out, t) for t in (x, B, C)):
+            raise ValueError("out must not overlap x, B or C")
+    if n_seq == 0:
+        return out
+    # (copies live until the launch)
+    x, ld_x, xp = _rows16(x, width)
+    B, ld_B, bp = _rows16(B, G * N)
+    C, ld_C, cp = _rows16(C, G * N)
+    dt, ld_dt, dp = _rows32(dt, H)
+    A_log = A_log.contiguous()
+    D = None if D is None else D.contiguous()
+    dt_bias = None if dt_bias is None else dt_bias.contiguous()
+    args = _C.Scan(xp, dp, bp, cp, A_log.data_ptr(), _C.ptr(D), _C.ptr(dt_bias), sp, so, _C.ptr(slots), _C.ptr(cu_seqlens),
+                   out.data_ptr(), ld_x, ld_dt, ld_B, ld_C, ld_out, T, n_seq, state.shape[0], H, G, P, N, kind,
+                   2 if dt.dtype is f32 else kind, 1 if softplus else 0)
+    L = _C.lib()
+    _run(dev, L.dfssm_selective_scan_step if step else L.dfssm_selective_scan_prefill, args, "selective_scan")
+    return out
+
+
+def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A_log: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
+                        state: torch.Tensor, D=None, dt_bias=None, slots=None, softplus=True, out=None,
+                        state_out=None) -> torch.Tensor:
+    """One token per sequence of the selective state space scan (dfssm_selective_scan_step): per head, with
+    d = max(softplus(dt + dt_bias), 0), h = exp(-d exp(A_log)) h + (d x) B^T, and returns h C + D x.
+
+    x (B, H, P) fp16 or bf16, P a multiple of 16 up to 256; dt (B, H) of x's type or fp32; B, C (B, G, N) of x's type, N 64
+    or 128, head h reads group h // (H // G); A_log (H,) fp32, D and dt_bias (H,) fp32 or None (zero); state
+    (slots, H, P, N) fp32, contiguous, updated in place, or written to state_out (of the same shape; slots that no
+    sequence has are left as they are there). Rows may be strided. softplus=False takes d = max(dt + dt_bias, 0). slots as
+    in causal_conv_step. out, if given, overlaps none of the others."""
+    return _scan_call(True, x, dt, A_log, B, C, state, D, dt_bias, None, slots, softplus, out, state_out,
+                      x.shape[0] if isinstance(x, torch.Tensor) and x.dim() else 0)
+
+
+def selective_scan_prefill(x: torch.Tensor, dt: torch.Tensor, A_log: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
+                           state: torch.Tensor, D=None, dt_bias=None, cu_seqlens=None, slots=None, softplus=True, out=None,
+                           state_out=None) -> torch.Tensor:
+    """The selective state space scan over whole prompts (dfssm_selective_scan_prefill), from the states the sequences have
+    to those they leave: what selective_scan_step gives token by token, up to rounding.
+
+    Either packed, x (T, H, P), dt (T, H), B, C (T, G, N) with cu_seqlens (n + 1,) int32 on the device (sequence b has
+    tokens cu_seqlens[b] .. cu_seqlens[b + 1], which must not fall; any length, zero included; rows of no sequence are
+    left as they are in out), or one dimension more in front and no cu_seqlens: (B, T, ...). The other arguments are
+    those of selective_scan_step."""
+    if cu_seqlens is not None:
+        return _scan_call(False, x, dt, A_log, B, C, state, D, dt_bias, cu_seqlens, slots, softplus, out, state_out, 0)
+    _kind16(x)
+    for t, n in ((dt, "dt"), (B, "B"), (C, "C")):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{n} must be a tensor")
+    if x.dim() != 4 or B.dim() != 4 or C.dim() != 4 or dt.dim() != 3:
+        raise ValueError("without cu_seqlens: x, B, C (batch, tokens, heads or groups, dim or cols), dt (batch, tokens, heads)")
+    if any(t.shape[:2] != x.shape[:2] for t in (dt, B, C)):
+        raise ValueError("x, dt, B and C must agree in batch and tokens")
+    if out is not None:
+        _need(out, x.dtype, "out")
+        if out.shape != x.shape or not out.is_contiguous():
+            raise ValueError("out must be contiguous and have x's shape")
+        out = out.flatten(0, 1)
+    return _scan_call(False, x.flatten(0, 1), dt.flatten(0, 1), A_log, B.flatten(0, 1), C.flatten(0, 1), state, D, dt_bias, None,
+                      slots, softplus, out, state_out, x.shape[0]).view(x.shape)
+
+
+def _norm_rows(x):
+    """x (.., cols) as rows."""
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("x must be (.., cols)")
+    return x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+
+
+def _norm_weight(t, name: str, cols: int, dev: int):
+    _need_all(dev, (t, torch.float32, name))
+    if t.shape != (cols,):
+        raise ValueError(f"{name} must be ({cols},)")
+    return t.contiguous()
+
+
+def _eps(eps) -> float:
+    eps = float(eps)
+    if not eps >= 2.0 ** -126:
+        raise ValueError("eps must be at least 2^-126")
+    return eps
+
+
+def _norm_out(out, x, name: str, dtype, dev: int, cols: int, inputs):
+    """out (a new tensor if None), its rows' distance and address. It may be one of `inputs`, (tensor, distance, address)
+    each, and overlaps none otherwise."""
+    if out is None:
+        out = x.new_empty(x.shape, dtype=dtype)
+        return out, cols, out.data_ptr()
+    _need_all(dev, (out, dtype, name))
+    if out.shape != x.shape:
+        raise ValueError(f"{name} must have x's shape")
+    rows = _norm_rows(out)
+    _, ld, p = _rows(rows, cols)
+    _own_rows(out, rows.shape[0], ld, p, cols, name)
+    for t, ld_t, p_t in inputs:
+        same = p == p_t and (rows.shape[0] <= 1 or ld == ld_t) and t.dtype is dtype
+        if not same and not _apart(rows, t):
+            raise ValueError(f"{name} must be an input itself or overlap none")
+    return out, ld, p
+
+
+def gated_norm(x: torch.Tensor, gate, weight: torch.Tensor, groups: int = 1, eps: float = 1e-5, gate_first=True,
+               out=None) -> torch.Tensor:
+    """RMSNorm with a gate (dfssm_gated_norm): rmsnorm(x s(gate)) weight, or with gate_first=False
+    rmsnorm(x) weight s(gate); s(z) = z / (1 + e^-z), rmsnorm(v) = v / sqrt(mean(v^2) + eps) over each of `groups` equal
+    parts of a row.
+
+    x (.., cols) and gate of its shape fp16 or bf16, rows may be strided; gate None: none. weight (cols,) fp32. cols /
+    groups at most 16384. In fp32, rounded once. out may be x or gate itself, and overlaps them no other way."""
+    kind = _kind16(x)
+    dt, dev = x.dtype, x.get_device()
+    r = _norm_rows(x)
+    rows, cols = r.shape
+    groups = operator.index(groups)
+    if groups < 1 or cols % groups or cols // groups > MAX_NORM_COLS:
+        raise ValueError(f"groups must divide {cols} into parts of at most {MAX_NORM_COLS}, got {groups}")
+    weight = _norm_weight(weight, "weight", cols, dev)
+    eps = _eps(eps)
+    r, ld, p = _rows(r, cols)
+    inputs = [(r, ld, p)]
+    z, ld_z, zp = None, 0, 0
+    if gate is not None:
+        _need_all(dev, (gate, dt, "gate"))
+        if gate.shape != x.shape:
+            raise ValueError("gate must have x's shape")
+        z, ld_z, zp = _rows(_norm_rows(gate), cols)
+        inputs.append((z, ld_z, zp))
+    out, ld_out, op = _norm_out(out, x, "out", dt, dev, cols, inputs)
+    if rows:
+        args = _C.Gated(p, zp, weight.data_ptr(), op, ld, ld_z, ld_out, rows, cols, groups, kind, 1 if gate_first else 0, eps)
+        _run(dev, _C.lib().dfssm_gated_norm, args, "gated_norm")
+    return out
+
+
+def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, post_weight=None, scale=1.0,
+                  eps: float = 1e-5, out=None, residual_out=None):
+    """A block's end and the next one's start (dfssm_residual_norm): r = residual + scale (rmsnorm(x) post_weight), or
+    residual + scale x without post_weight; returns (rmsnorm(r) weight, r), with rmsnorm(v) = v / sqrt(mean(v^2) + eps).
+
+    x (.., cols) fp16 or bf16, residual of its shape, of its type or fp32; rows may be strided; weight and post_weight
+    (cols,) fp32; scale a number or (cols,) fp32; cols at most 16384. In fp32; the first result has x's type, r the
+    residual's, each rounded once. residual_out may be residual itself and out x; they overlap the inputs no other way,
+    nor each other."""
+    kind = _kind16(x)
+    dt, dev = x.dtype, x.get_device()
+    f32 = torch.float32
+    rt = f32 if isinstance(residual, torch.Tensor) and residual.dtype is f32 else dt
+    _need_all(dev, (residual, rt, "residual"))
+    if residual.shape != x.shape:
+        raise ValueError("residual must have x's shape")
+    r = _norm_rows(x)
+    rows, cols = r.shape
+    if cols > MAX_NORM_COLS:
+        raise ValueError(f"x must have at most {MAX_NORM_COLS} columns, got {cols}")
+    weight = _norm_weight(weight, "weight", cols, dev)
+    post_weight = None if post_weight is None else _norm_weight(post_weight, "post_weight", cols, dev)
+    scales = None
+    if isinstance(scale, torch.Tensor):
+        scales, scale = _norm_weight(scale, "scale", cols, dev), 0.0
+    eps = _eps(eps)
+    r, ld, p = _rows(r, cols)
+    s, ld_s, sp = _rows(_norm_rows(residual), cols)
+    inputs = [(r, ld, p), (s, ld_s, sp)]
+    out, ld_out, op = _norm_out(out, x, "out", dt, dev, cols, inputs)
+    residual_out, ld_ro, rop = _norm_out(residual_out, x, "residual_out", rt, dev, cols, inputs)
+    if not _apart(_norm_rows(out), _norm_rows(residual_out)):
+        raise ValueError("out and residual_out must not overlap")
+    if rows:
+        args = _C.Residual(p, sp, _C.ptr(post_weight), _C.ptr(scales), weight.data_ptr(), op, rop, ld, ld_s, ld_out, ld_ro,
+                           rows, cols, kind, 2 if rt is f32 else kind, float(scale), eps)
+        _run(dev, _C.lib().dfssm_residual_norm, args, "residual_norm")
+    return out, residual_out
+
+
+# ---------------------------------------------------------------------------------------------
 # token draw
 # ---------------------------------------------------------------------------------------------
 MAX_DRAW_VOCAB = 262144   # tokens of a row of sample_filtered

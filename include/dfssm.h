@@ -254,7 +254,7 @@ int dfssm_decode_step_static(const dfssm_model* model, const int64_t* tokens, ui
 /* Element types of the operators that take more than one. */
 #define DFSSM_TYPE_F16 0
 #define DFSSM_TYPE_BF16 1
-#define DFSSM_TYPE_F32 2 /* logits of dfssm_sample_filtered only */
+#define DFSSM_TYPE_F32 2 /* logits of dfssm_sample_filtered, dt of the selective scan, residuals of dfssm_residual_norm */
 
 /* ---- sampling ------------------------------------------------------------------------ */
 typedef struct dfssm_sample_params {
@@ -396,6 +396,106 @@ int dfssm_gated_delta_step(const dfssm_delta* args, void* stream);
  * sequence (of its value column, or of the heads that read it): their rows of out are not finite there. */
 size_t dfssm_gated_delta_workspace_bytes(const dfssm_delta* args);
 int dfssm_gated_delta_prefill(const dfssm_delta* args, void* workspace, void* stream);
+
+/* ---- a state space layer between its projections ----------------------------------------- */
+/* Sequences and slots are those of dfssm_delta: sequence b has tokens cu_seqlens[b] .. cu_seqlens[b + 1] (any length, zero
+ * included; held to [0, n_tokens]; rows of no sequence stay as they were; where offsets fall, results are not specified and
+ * nothing outside the tensors is read or written), or n_tokens / n_seq each with NULL, and the state in slot
+ * slots[b], or b with NULL. A negative slot is padding: zeros in out; one that is >= n_slots or an earlier sequence's: NaN.
+ * Neither touches a state. state_out is `state` itself or memory that does not overlap it; slots that no sequence has
+ * stay as they are there. */
+
+/* Short causal convolution of each channel, y_t = f(bias + sum_k weight_k x_{t - width + 1 + k}), f(y) = y / (1 + e^-y) with
+ * silu, else y, in fp32 with one rounding; the x before a sequence are its state's, which takes the last width - 1. */
+typedef struct dfssm_conv {
+  const void* x;          /* (tokens, channels), `type`; rows ld_x elements apart */
+  const void* weight;     /* (channels, width), `type`, the last one is the token's own */
+  const void* bias;       /* (channels), `type`, or NULL */
+  const void* state;      /* (n_slots, channels, width - 1), `type`, the oldest first, C-contiguous */
+  void* state_out;
+  const int32_t* slots;
+  const int32_t* cu_seqlens; /* dfssm_causal_conv_prefill only */
+  void* out;              /* (tokens, channels), `type`; rows ld_out apart that do not overlap */
+  int64_t ld_x, ld_out, n_tokens;
+  int32_t n_seq, n_slots, channels;
+  int32_t width;          /* 2, 3 or 4 */
+  int32_t type;           /* DFSSM_TYPE_F16 or DFSSM_TYPE_BF16 */
+  int32_t silu;
+} dfssm_conv;
+/* One token per sequence (n_tokens = n_seq); out may be x itself. */
+int dfssm_causal_conv_step(const dfssm_conv* args, void* stream);
+/* Whole prompts; out must not overlap x. */
+int dfssm_causal_conv_prefill(const dfssm_conv* args, void* stream);
+
+/* Selective state space scan. Per head, h (dim, cols) fp32, with d = max(dt', 0), dt' = softplus(dt + dt_bias) or, without
+ * softplus, dt + dt_bias:  h = exp(-d exp(A_log)) h + (d x) B^T,  out = h C + D x, in fp32 with one rounding of out. */
+typedef struct dfssm_scan {
+  const void* x;          /* (tokens, heads, dim), `type`; tokens ld_x elements apart, heads contiguous */
+  const void* dt;         /* (tokens, heads), `dt_type` */
+  const void* B;          /* (tokens, groups, cols), `type`: head h reads group h / (heads / groups) */
+  const void* C;          /* the same */
+  const float* A_log;     /* (heads) */
+  const float* D;         /* (heads), or NULL: 0 */
+  const float* dt_bias;   /* (heads), or NULL: 0 */
+  const float* state;     /* (n_slots, heads, dim, cols), C-contiguous */
+  float* state_out;
+  const int32_t* slots;
+  const int32_t* cu_seqlens; /* dfssm_selective_scan_prefill only */
+  void* out;              /* (tokens, heads, dim), `type` */
+  int64_t ld_x, ld_dt, ld_B, ld_C, ld_out, n_tokens;
+  int32_t n_seq, n_slots, heads;
+  int32_t groups;         /* divides heads */
+  int32_t dim;            /* a multiple of 16, at most 256 */
+  int32_t cols;           /* 64 or 128 */
+  int32_t type;           /* DFSSM_TYPE_F16 or DFSSM_TYPE_BF16 */
+  int32_t dt_type;        /* `type` or DFSSM_TYPE_F32 */
+  int32_t softplus;
+} dfssm_scan;
+/* x, B, C, out, state and state_out are 16-byte aligned, ld_x, ld_B, ld_C and ld_out multiples of 8, every ld_* at most
+ * 2^23; the rows of out do not overlap each other or anything else. */
+
+/* One token per sequence (n_tokens = n_seq). */
+int dfssm_selective_scan_step(const dfssm_scan* args, void* stream);
+/* Whole prompts, from the states the sequences have to those they leave: what dfssm_selective_scan_step gives token by
+ * token, up to rounding. */
+int dfssm_selective_scan_prefill(const dfssm_scan* args, void* stream);
+
+/* out = rmsnorm(x s(gate)) weight (gate_first) or rmsnorm(x) weight s(gate), s(z) = z / (1 + e^-z), rmsnorm(v) =
+ * v / sqrt(mean(v^2) + eps) over each of `groups` equal parts of a row; gate NULL: none. In fp32 with one rounding. out may be
+ * x or gate itself. */
+typedef struct dfssm_gated {
+  const void* x;          /* (rows, cols), `type`; rows ld_x elements apart */
+  const void* gate;       /* the same, or NULL */
+  const float* weight;    /* (cols) */
+  void* out;              /* (rows, cols), `type` */
+  int64_t ld_x, ld_gate, ld_out, rows;
+  int32_t cols;
+  int32_t groups;         /* divides cols; cols / groups at most DFSSM_NORM_MAX_COLS */
+  int32_t type;           /* DFSSM_TYPE_F16 or DFSSM_TYPE_BF16 */
+  int32_t gate_first;
+  float eps;              /* at least 2^-126 */
+} dfssm_gated;
+#define DFSSM_NORM_MAX_COLS 16384
+int dfssm_gated_norm(const dfssm_gated* args, void* stream);
+
+/* r = residual + scale (rmsnorm(x) post_weight, or x where post_weight is NULL); residual_out = r; out = rmsnorm(r) weight, of r
+ * before residual_out's rounding. In fp32 with one rounding each. residual_out may be residual itself, out x. */
+typedef struct dfssm_residual {
+  const void* x;            /* (rows, cols), `type`; rows ld_x elements apart */
+  const void* residual;     /* (rows, cols), `residual_type` */
+  const float* post_weight; /* (cols) or NULL */
+  const float* scales;      /* (cols), or NULL: `scale` */
+  const float* weight;      /* (cols) */
+  void* out;                /* (rows, cols), `type` */
+  void* residual_out;       /* (rows, cols), `residual_type` */
+  int64_t ld_x, ld_residual, ld_out, ld_residual_out, rows;
+  int32_t cols;             /* at most DFSSM_NORM_MAX_COLS */
+  int32_t type;             /* DFSSM_TYPE_F16 or DFSSM_TYPE_BF16 */
+  int32_t residual_type;    /* `type` or DFSSM_TYPE_F32 */
+  float scale;
+  float eps;                /* at least 2^-126 */
+} dfssm_residual;
+int dfssm_residual_norm(const dfssm_residual* args, void* stream);
 
 #ifdef __cplusplus
 }

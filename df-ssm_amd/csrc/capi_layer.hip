@@ -57,12 +57,16 @@ ConvArgs conv_args(const dfssm_conv* d) {
   return a;
 }
 
-int check_scan(const dfssm_scan* d, bool step) {
-  if (!d) return DFSSM_E_NULL;
+int check_scan_dims(const dfssm_scan* d) {
   if (d->groups < 1 || d->heads < 1 || d->heads % d->groups) return DFSSM_E_DIMS;
   if ((d->cols != 64 && d->cols != 128) || d->dim < 16 || d->dim > 256 || d->dim % 16) return DFSSM_E_DIMS;
-  if (!type16(d->type) || (d->dt_type != d->type && d->dt_type != DFSSM_TYPE_F32)) return DFSSM_E_DIMS;
-  const int rc = check_sequences(d, step);
+  return type16(d->type) && (d->dt_type == d->type || d->dt_type == DFSSM_TYPE_F32) ? DFSSM_OK : DFSSM_E_DIMS;
+}
+
+int check_scan(const dfssm_scan* d, bool step) {
+  if (!d) return DFSSM_E_NULL;
+  int rc = check_scan_dims(d);
+  if (!rc) rc = check_sequences(d, step);
   if (rc || d->n_seq == 0) return rc;
   if (!d->A_log || !d->state || !d->state_out || (d->n_tokens && (!d->x || !d->dt || !d->B || !d->C || !d->out)))
     return DFSSM_E_NULL;
@@ -88,6 +92,11 @@ ScanArgs scan_args(const dfssm_scan* d) {
   a.bf16 = d->type == DFSSM_TYPE_BF16; a.dt32 = d->dt_type == DFSSM_TYPE_F32; a.softplus = d->softplus;
   return a;
 }
+
+// Prompts that run token by token: too few tokens for a chunk's fixed work. The lengths behind cu_seqlens are on the device,
+// so the rule there goes by all tokens, which any one sequence may have.
+constexpr int kTokenPath = 12;
+bool by_tokens(const ScanArgs& a) { return (a.cu ? a.n_tokens : a.len) <= kTokenPath; }
 
 // Rows of a norm.
 int check_rows(int64_t rows, int cols, std::initializer_list<int64_t> in, std::initializer_list<int64_t> out, float eps) {
@@ -123,10 +132,22 @@ int dfssm_selective_scan_step(const dfssm_scan* args, void* stream) {
   return hip_status(launch_scan_token(scan_args(args), (hipStream_t)stream));
 }
 
-int dfssm_selective_scan_prefill(const dfssm_scan* args, void* stream) {
+size_t dfssm_selective_scan_workspace_bytes(const dfssm_scan* args) {
+  if (!args || check_scan_dims(args) != DFSSM_OK || check_sequences(args, false) != DFSSM_OK || args->n_seq == 0) return 0;
+  const ScanArgs a = scan_args(args);
+  return by_tokens(a) ? 0 : scan_chunk_workspace(a);
+}
+
+int dfssm_selective_scan_prefill(const dfssm_scan* args, void* workspace, void* stream) {
   const int rc = check_scan(args, false);
   if (rc || args->n_seq == 0) return rc;
-  return hip_status(launch_scan_token(scan_args(args), (hipStream_t)stream));
+  const ScanArgs a = scan_args(args);
+  if (by_tokens(a)) return hip_status(launch_scan_token(a, (hipStream_t)stream));
+  if (scan_chunk_workspace(a)) {
+    if (!workspace) return DFSSM_E_NULL;
+    if (!aligned(workspace, 16)) return DFSSM_E_ALIGN;
+  }
+  return hip_status(launch_scan_chunked(a, workspace, (hipStream_t)stream));
 }
 
 int dfssm_gated_norm(const dfssm_gated* d, void* stream) {

@@ -33,7 +33,10 @@ struct ScanArgs {
   int n_seq, n_slots, H, G, P, N;
   int bf16, dt32, softplus;
 };
+// Token by token (scan.hip), and over chunks with the workspace of scan_chunk_workspace (scan_chunk.hip).
 hipError_t launch_scan_token(const ScanArgs& a, hipStream_t s);
+hipError_t launch_scan_chunked(const ScanArgs& a, void* workspace, hipStream_t s);
+size_t scan_chunk_workspace(const ScanArgs& a);
 
 struct GatedNormArgs {
   const uint16_t *x, *gate;  // rows ld_* elements apart; gate may be null

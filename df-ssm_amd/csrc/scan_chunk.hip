@@ -1,0 +1,472 @@
+// The selective state space scan over chunks of 64 tokens (gfx950 matrix cores).
+//
+// Per head and chunk, with a_t = -d_t e^{A_log}, G_i = a_1 + .. + a_i, h0 (P x N) the state before it and w_j = e^{G_64 - G_j} d_j:
+//   M_ij = C_i.B_j e^{G_i - G_j} d_j (i >= j) + D (i = j);  y_i = e^{G_i} h0 C_i + sum_j M_ij x_j
+//   h1 = e^{G_64} h0 + sum_j (w_j x_j) B_j^T
+// A workgroup walks the chunks of a sequence, or of a segment of one, with four waves that share B and C in LDS; each has
+// 32 columns p of a head, their state in registers and their x to itself. Products are taken so that results lie in
+// registers as the next product wants its operand: the state as rows n of 32 x 32 results (a lane has a column p), the
+// scores transposed (a lane has a row i of M), y transposed (a lane has a token, and stores 8 bytes of its row).
+// Sequences longer than a segment take three launches: states of the segments from zero, their chain, everything.
+#include "common.h"
+#include "layer.h"
+#include "parts.h"
+#include "scan_math.h"
+#include "scan_plan.h"
+
+namespace dfssm {
+
+namespace {
+
+constexpr int kC = kScanChunk, kW = kScanWaves;
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <bool BF>
+__device__ __forceinline__ f32x16 mm32(h8 a, h8 b, f32x16 c) {
+  if constexpr (BF) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// Eight values as NT parts: pairs of halves of x sc, or NT parts of bf16 (sc is 1).
+template <bool BF, int NT>
+__device__ __forceinline__ void parts8(const float (&x)[8], float sc, h8 (&part)[NT]) {
+  uint32_t p[NT][4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if constexpr (!BF) {
+      uint32_t t[2];
+      split2(x[2 * q], x[2 * q + 1], sc, t);
+      p[0][q] = t[0];
+      p[1][q] = t[1];
+    } else {
+      float x0 = x[2 * q], x1 = x[2 * q + 1];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        uint32_t t = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x0, x1}, b2));
+        asm("" : "+v"(t));
+        p[i][q] = t;
+        x0 -= __builtin_bit_cast(float, t << 16);
+        x1 -= __builtin_bit_cast(float, t & 0xffff0000u);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NT; ++i) part[i] = __builtin_bit_cast(h8, u32x4{p[i][0], p[i][1], p[i][2], p[i][3]});
+}
+
+// The larger of v >= 0 in the two lanes of a column (32 apart).
+__device__ __forceinline__ float max_halves(float v) {
+  const uint32_t x = __builtin_bit_cast(uint32_t, v);
+  const auto q = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return __builtin_bit_cast(float, max((uint32_t)q[0], (uint32_t)q[1]));
+}
+template <int N>
+__device__ __forceinline__ float max_abs(const float (&x)[N], float m) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) m = __builtin_elementwise_maximum(m, __builtin_fabsf(x[e]));
+  return m;
+}
+
+// Rows of B and C in LDS: their 16-byte pieces are exchanged so that one piece of 8 rows, and two neighbouring ones of
+// four rows, lie in different banks.
+template <int N>
+__device__ __forceinline__ int swap_of(int row) {
+  return N == 128 ? ((row & 7) << 1) | ((row >> 3) & 1) : (row & 2) | (row & 4) | ((row >> 3) & 1);
+}
+
+typedef __attribute__((address_space(3))) s4* tptr;
+
+template <int N, bool STATE>
+struct ScanLds {
+  f16 B[2][kC][N];
+  f16 C[STATE ? 1 : kC][STATE ? 8 : N];
+  f16 x[kW][kC][kScanCols];
+  struct {
+    float Gh[kC], Gl[kC], d[kC], w[kC], F[kScanCols], s[kScanCols];
+  } v[kW];
+};
+
+// A wave's quarter of 64 rows of B or C, into LDS.
+template <int N>
+__device__ __forceinline__ void fetch_shared(f16 (*to)[N], const uint16_t* p, int64_t ld, int len, int wave, int off) {
+  constexpr int per = 512 / N;  // rows of a KiB
+  const Rsrc r = rows_of(p, ld, len, N);
+#pragma unroll
+  for (int n = 0; n < kC / per / kW; ++n)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr)((char*)to + (kW * n + wave) * 1024), 16, off + n * (kW * per * 2) * (int)ld, 0,
+                                             0, 0);
+}
+
+// STATE: the states that a segment leaves from zero, and its decay, of all segments but the last of a sequence.
+template <int N, bool BF, bool STATE>
+__global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(64 * kW) void
+scan_chunk_kernel(ScanArgs a, int64_t seg, int64_t places, float* seg_state, float* seg_decay) {
+  constexpr int NB = N / 16, NN = N / 32, NU = kParts<BF>, pieces = N / 8;
+  __shared__ __align__(16) ScanLds<N, STATE> L;
+  const int lane = threadIdx.x & 63, hi = lane >> 5, c = lane & 31, l = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // Workgroups go to the eight dies in turn: all that share a group's B and C run on one, next to its L2.
+  const int rep = a.H / a.G, ncb = (a.P + kScanCols - 1) / kScanCols, nwg = (rep * ncb + kW - 1) / kW;
+  const int64_t bx = blockIdx.x, in = bx >> 3, unit = in / nwg * 8 + (bx & 7);
+  if (unit >= places * a.G) return;
+  const int64_t place = unit / a.G;
+  const int gr = (int)(unit % a.G), blk = (int)(in % nwg) * kW + wave;
+  Where q{0, 0, 0, 0};
+  int64_t tok;
+  const int64_t len = tile_of<0>(a, place, q, tok, seg);
+  if (len == 0) tok = q.t0;
+  const bool last = tok + len >= q.t1;
+  if (len == 0 && !(!STATE && place == q.first && q.t0 == q.t1)) return;  // (an empty sequence's state is passed on)
+  if (STATE && last) return;
+  const bool active = blk < rep * ncb;
+  const int h = gr * rep + (active ? blk / ncb : 0), p0 = active ? blk % ncb * kScanCols : 0;
+  const bool wide = p0 + 16 < a.P;
+  const int slot = slot_of(a, q.seq);
+  if (slot < 0) {
+    const uint16_t fill = slot == kSlotPad ? 0 : 0x7fff;
+    if (!STATE && active && (c < 16 || wide))
+      for (int64_t t = hi; t < len; t += 2) a.out[(tok + t) * a.ld_out + (int64_t)h * a.P + p0 + c] = fill;
+    return;
+  }
+  const bool whole = place == q.first && last;  // the sequence is one segment
+
+  // S[t][8 b + e] is the state of row n = 32 t + 16 b + 8 hi + e and column p0 + c, over sfac.
+  f32x16 S[NN];
+  float sfac = 1.0f, decay = 1.0f;
+  const int pc = c < 16 || wide ? p0 + c : p0 + c - 16;  // (columns that are not there do their neighbours' work)
+  const int64_t so = ((int64_t)h * a.P + pc) * N + 8 * hi, size = (int64_t)a.H * a.P * N;
+  if constexpr (STATE) {
+#pragma unroll
+    for (int t = 0; t < NN; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) S[t][r] = 0.0f;
+  } else {
+    const float* sp = (whole || len == 0 ? a.state + slot * size : seg_state + place * size) + so;
+#pragma unroll
+    for (int t = 0; t < NN; ++t)
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        const f32x4 v = *(const f32x4*)(sp + 32 * t + 16 * (m >> 1) + 4 * (m & 1));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) S[t][4 * m + e] = v[e];
+      }
+  }
+  const HeadParams hp = head_params(a, h);
+  auto& V = L.v[wave];
+  f16 (&X)[kC][kScanCols] = L.x[wave];
+  const int off_row = 512 / N * wave + lane / pieces, off_piece = ((lane % pieces) ^ swap_of<N>(off_row)) * 16;
+  const int off_b = off_row * (int)a.ld_B * 2 + off_piece, off_c = off_row * (int)a.ld_C * 2 + off_piece;
+  const int off_x = (lane >> 2) * (int)a.ld_x * 2 + (lane & 3) * 16;
+  const int xw = a.P - p0 < kScanCols ? a.P - p0 : kScanCols;
+  const int n_chunks = (int)((len + kC - 1) / kC);
+  auto rows_at = [&](int i) { return (int)(len - (int64_t)i * kC < kC ? len - (int64_t)i * kC : kC); };
+  auto fetch_b = [&](int i) {
+    fetch_shared<N>(L.B[i & 1], a.B + (tok + (int64_t)i * kC) * a.ld_B + gr * N, a.ld_B, rows_at(i), wave, off_b);
+  };
+  auto fetch_c = [&](int i) {
+    if constexpr (!STATE) fetch_shared<N>(L.C, a.C + (tok + (int64_t)i * kC) * a.ld_C + gr * N, a.ld_C, rows_at(i), wave, off_c);
+  };
+  auto fetch_x = [&](int i) {
+    const Rsrc r = rows_of(a.x + (tok + (int64_t)i * kC) * a.ld_x + (int64_t)h * a.P + p0, a.ld_x, rows_at(i), xw);
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr)((char*)X + n * 1024), 16, off_x + n * 32 * (int)a.ld_x, 0, 0, 0);
+  };
+  float raw = 0.0f;
+  auto fetch_dt = [&](int i) {
+    const int n = rows_at(i);
+    raw = load_dt<BF>(a, tok + (int64_t)i * kC + (lane < n ? lane : n - 1), h);
+  };
+  if (n_chunks) {
+    fetch_b(0);
+    fetch_c(0);
+    fetch_x(0);
+    fetch_dt(0);
+  }
+  __builtin_amdgcn_s_waitcnt(0);
+
+  for (int i = 0; i < n_chunks; ++i) {
+    const int n = rows_at(i);
+    const bool more = i + 1 < n_chunks;
+    step_barrier();  // this chunk's B and C are in LDS, and the next one's place for B is free
+    // the time steps; lane: a token
+    const float d = lane < n ? time_step(raw, hp, a.softplus) : 0.0f;
+    float al = d * hp.A;
+    al = al < -1e5f ? -1e5f : al;
+    double G = (double)al * 1.4426950408889634;
+    G += moved<0x111, 0xf>(G);  // running sums: from 1, 2, 4 and 8 lanes before, in the row of 16
+    G += moved<0x112, 0xf>(G);
+    G += moved<0x114, 0xf>(G);
+    G += moved<0x118, 0xf>(G);
+    G += moved<0x142, 0xa>(G);  // row 0's last to row 1, 2's to 3; then lane 31's to rows 2 and 3
+    G += moved<0x143, 0xc>(G);
+    const double GC = readlane_f64(G, 63);
+    const float dec = __builtin_amdgcn_exp2f((float)GC);
+    V.w[lane] = __builtin_amdgcn_exp2f((float)(GC - G)) * d;
+    if constexpr (!STATE) {
+      V.Gh[lane] = (float)G;
+      V.Gl[lane] = (float)(G - (double)(float)G);
+      V.d[lane] = d;
+      const float f = __builtin_amdgcn_exp2f(lane < 32 ? (float)(readlane_f64(G, 32) - G) : 0.0f) * d;
+      if (lane < 32) V.F[lane] = f;
+    }
+    wave_sync();
+    // x as operands: column p0 + c, tokens 16 k + 4 hi + 0 .. 3 and 8 more
+    h8 xf[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      s4 t[2];
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+        t[y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tptr)&X[16 * k + 8 * y + 4 * hi + (l >> 2)][16 * ((lane >> 4) & 1) + 4 * (l & 3)]);
+      xf[k] = __builtin_bit_cast(h8, __builtin_shufflevector(t[0], t[1], 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): x is in registers, its place free
+    asm volatile("" ::: "memory");
+    if (more) {
+      fetch_b(i + 1);
+      fetch_x(i + 1);
+      fetch_dt(i + 1);
+    }
+    float smax = 0.0f;
+    if constexpr (!BF) {
+#pragma unroll
+      for (int t = 0; t < NN; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) smax = __builtin_elementwise_maximum(smax, __builtin_fabsf(S[t][r]));
+      smax = max_halves(smax);
+    }
+    if constexpr (!STATE) {
+      float ssc = 1.0f, sinv = 1.0f;
+      if constexpr (!BF) {
+        ssc = pow2_scale(smax, sinv);
+        if (hi == 0) V.s[c] = sinv * sfac;
+      }
+      f32x16 sc[3], y[2];  // scores (columns 0 .. 31 of rows 0 .. 31; of rows 32 .. 63; columns 32 ..), y by tokens
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sc[0][r] = sc[1][r] = sc[2][r] = y[0][r] = y[1][r] = 0.0f;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        h8 cf[2], bf[2], s[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int row = 32 * t + c, at = ((2 * b + hi) ^ swap_of<N>(c)) * 8;
+          cf[t] = *(const h8*)&L.C[row][at];
+          bf[t] = *(const h8*)&L.B[i & 1][row][at];
+        }
+        float sv[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sv[e] = S[b >> 1][8 * (b & 1) + e];
+        parts8<BF, 2>(sv, ssc, s);
+        sc[0] = mm32<BF>(bf[0], cf[0], sc[0]);
+        sc[1] = mm32<BF>(bf[0], cf[1], sc[1]);
+        sc[2] = mm32<BF>(bf[1], cf[1], sc[2]);
+#pragma unroll
+        for (int p = 1; p >= 0; --p)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) y[t] = mm32<BF>(s[p], cf[t], y[t]);
+      }
+      step_barrier();  // C is free
+      if (more) fetch_c(i + 1);
+      // M: a lane has row 32 t + c, columns 8 q + 4 hi + e
+      float pinv[2] = {1.0f, 1.0f}, eG[2];
+      h8 m[6][2];
+      const float Gb = V.Gh[32], gb = V.Gl[32];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const float Gi = V.Gh[32 * t + c], gi = V.Gl[32 * t + c];
+        eG[t] = __builtin_amdgcn_exp2f(Gi + gi);
+        float x[32];
+        if (t) {
+          const float ei = __builtin_amdgcn_exp2f((Gi - Gb) + (gi - gb));
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4) {
+            const f32x4 F = *(const f32x4*)&V.F[8 * q4 + 4 * hi];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 * q4 + e] = (sc[1][4 * q4 + e] * ei) * F[e];
+          }
+        }
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+          const int j0 = 8 * q4 + 4 * hi;
+          const f32x4 jh = *(const f32x4*)&V.Gh[32 * t + j0], jl = *(const f32x4*)&V.Gl[32 * t + j0], dj = *(const f32x4*)&V.d[32 * t + j0];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {  // (beyond the diagonal the difference may be of any size: not exponentiated)
+            const bool low = j0 + e <= c;
+            const float ex = __builtin_amdgcn_exp2f(low ? (Gi - jh[e]) + (gi - jl[e]) : 0.0f) * dj[e];
+            float v = low ? sc[2 * t][4 * q4 + e] * ex : 0.0f;
+            v += j0 + e == c ? hp.D : 0.0f;
+            x[16 * t + 4 * q4 + e] = v;
+          }
+        }
+        float msc = 1.0f;
+        if constexpr (!BF) {
+          float top = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 16 * (t + 1); ++e) top = __builtin_elementwise_maximum(top, __builtin_fabsf(x[e]));
+          msc = pow2_scale(max_halves(top), pinv[t]);
+        }
+#pragma unroll
+        for (int k = 0; k < 2 * (t + 1); ++k) {
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = x[8 * k + e];
+          parts8<BF, 2>(v, msc, m[2 * t + k]);
+        }
+      }
+      f32x16 yx[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) yx[t][r] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 2 * (t + 1); ++k)
+#pragma unroll
+          for (int p = 1; p >= 0; --p) yx[t] = mm32<BF>(xf[k], m[2 * t + k][p], yx[t]);
+      }
+      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): what is on its way for the next chunk, so that no later wait is for the stores
+      if (active) {
+        const Rsrc orow = rows_of(a.out + (tok + (int64_t)i * kC) * a.ld_out + (int64_t)h * a.P + p0, a.ld_out, n, xw);
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+          if (q4 >= 2 && !wide) break;
+          const f32x4 sv = BF ? f32x4{1.0f, 1.0f, 1.0f, 1.0f} : *(const f32x4*)&V.s[8 * q4 + 4 * hi];
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            float o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              o[e] = __builtin_fmaf(y[t][4 * q4 + e], BF ? eG[t] : eG[t] * sv[e], BF ? yx[t][4 * q4 + e] : yx[t][4 * q4 + e] * pinv[t]);
+            __builtin_amdgcn_raw_buffer_store_b64(u32x2{pack2<BF>(o[0], o[1]), pack2<BF>(o[2], o[3])}, orow,
+                                                  (32 * t + c) * (int)a.ld_out * 2 + (8 * q4 + 4 * hi) * 2, 0, 0);
+          }
+        }
+      }
+    } else {
+      decay *= dec;
+    }
+    // the new state
+    float u[4][8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const f32x4 w = *(const f32x4*)&V.w[16 * k + 8 * y + 4 * hi];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const f16 v = xf[k][4 * y + e];  // (a bit cast of the element itself takes the vector's first one)
+          u[k][4 * y + e] = w2f<BF>(__builtin_bit_cast(uint16_t, v)) * w[e];
+        }
+      }
+    float keep = dec, usc = 1.0f;
+    if constexpr (!BF) {
+      float top = 0.0f, uinv;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) top = max_abs(u[k], top);
+      usc = pow2_scale(__builtin_elementwise_maximum(max_halves(top), dec * (smax * sfac)), uinv);
+      keep = dec * sfac * usc;
+      sfac = uinv;
+    }
+#pragma unroll
+    for (int t = 0; t < NN; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) S[t][r] *= keep;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      h8 up[NU];
+      parts8<BF, NU>(u[k], usc, up);
+#pragma unroll
+      for (int t = 0; t < NN; ++t) {
+        // rows of B^T: result row 4 m + e of 16 is n = 4 m' + e, m' being m with its two bits exchanged
+        s4 b[2];
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const int row = 16 * k + 8 * y + 4 * hi + (l >> 2), mm = (l & 3) >> 1 | (l & 1) << 1;
+          const int piece = (4 * t + 2 * ((lane >> 4) & 1) + (mm >> 1)) ^ swap_of<N>(row & 15);
+          b[y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tptr)&L.B[i & 1][row][piece * 8 + 4 * (mm & 1)]);
+        }
+        const h8 bt = __builtin_bit_cast(h8, __builtin_shufflevector(b[0], b[1], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+        for (int p = NU - 1; p >= 0; --p) S[t] = mm32<BF>(bt, up[p], S[t]);
+      }
+    }
+    if constexpr (STATE) __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  }
+
+  if (!active || !(c < 16 || wide) || !(STATE || last)) return;
+  float* o = (STATE ? seg_state + place * size : a.state_out + slot * size) + so;
+#pragma unroll
+  for (int t = 0; t < NN; ++t)
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      f32x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = BF ? S[t][4 * m + e] : S[t][4 * m + e] * sfac;
+      *(f32x4*)(o + 32 * t + 16 * (m >> 1) + 4 * (m & 1)) = v;
+    }
+  if (STATE && p0 == 0 && lane == 0) seg_decay[place * a.H + h] = decay;
+}
+
+// The states before each segment of a sequence of several, in place of those that its segments leave from zero. A thread
+// has four values of a head.
+__global__ __launch_bounds__(256) void scan_states_kernel(ScanArgs a, int64_t seg, float* seg_state, const float* seg_decay) {
+  const int64_t size = (int64_t)a.H * a.P * a.N, per = (size / 4 + 255) / 256;
+  const int b = (int)(blockIdx.x / per);
+  const int64_t at = (blockIdx.x % per * 256 + threadIdx.x) * 4;
+  int64_t t0, t1;
+  seq_range(a, b, t0, t1);
+  const int64_t n = (t1 - t0 + seg - 1) / seg, first = t0 / seg + b;
+  if (n < 2) return;
+  const int slot = slot_of(a, b);
+  if (slot < 0 || at >= size) return;
+  const int h = (int)(at / ((int64_t)a.P * a.N));
+  float* p = seg_state + first * size + at;
+  f32x4 S = *(const f32x4*)(a.state + slot * size + at);
+  for (int64_t k = 0; k < n; ++k, p += size) {
+    f32x4 next = S;
+    if (k + 1 < n) {
+      const f32x4 own = *(const f32x4*)p;
+      const float d = seg_decay[(first + k) * a.H + h];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) next[e] = __builtin_fmaf(d, S[e], own[e]);
+    }
+    *(f32x4*)p = S;
+    S = next;
+  }
+}
+
+int64_t segment(const ScanArgs& a) {
+  const int64_t longest = a.cu ? a.n_tokens : a.len, seg = scan_segment(a.n_tokens, a.n_seq, scan_wgs(a.H, a.G, a.P));
+  return seg >= longest ? (longest + kC - 1) / kC * kC + kC : seg;  // (one segment each, and a place more than that: see places)
+}
+bool split(const ScanArgs& a) { return segment(a) < (a.cu ? a.n_tokens : a.len); }
+
+template <int N, bool BF>
+hipError_t launch(const ScanArgs& a, void* ws, hipStream_t s) {
+  const int64_t seg = segment(a), places = scan_places(a.n_tokens, a.n_seq, seg), wgs = scan_wgs(a.H, a.G, a.P) / a.G;
+  const int64_t units = places * a.G, grid = (units + 7) / 8 * 8 * wgs, size = (int64_t)a.H * a.P * N;
+  const int64_t chain = a.n_seq * ((size / 4 + 255) / 256);
+  if (grid > 0x7fffffff || chain > 0x7fffffff) return hipErrorInvalidValue;
+  float *st = (float*)ws, *de = st + (ws ? places * size : 0);
+  if (split(a)) {
+    hipLaunchKernelGGL((scan_chunk_kernel<N, BF, true>), dim3((unsigned)grid), dim3(64 * kW), 0, s, a, seg, places, st, de);
+    hipLaunchKernelGGL(scan_states_kernel, dim3((unsigned)chain), dim3(256), 0, s, a, seg, st, (const float*)de);
+  }
+  hipLaunchKernelGGL((scan_chunk_kernel<N, BF, false>), dim3((unsigned)grid), dim3(64 * kW), 0, s, a, seg, places, st, de);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+size_t scan_chunk_workspace(const ScanArgs& a) {
+  if (!split(a)) return 0;
+  const int64_t places = scan_places(a.n_tokens, a.n_seq, segment(a));
+  return (size_t)places * ((size_t)a.H * a.P * a.N + a.H) * sizeof(float);
+}
+
+hipError_t launch_scan_chunked(const ScanArgs& a, void* ws, hipStream_t s) {
+  if (a.N == 128) return a.bf16 ? launch<128, true>(a, ws, s) : launch<128, false>(a, ws, s);
+  return a.bf16 ? launch<64, true>(a, ws, s) : launch<64, false>(a, ws, s);
+}
+
+}  // namespace dfssm

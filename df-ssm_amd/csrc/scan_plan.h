@@ -1,0 +1,30 @@
+// Arithmetic of the chunked selective scan's launches, for the host and the device alike (constexpr functions serve both),
+// with nothing of HIP in it.
+#pragma once
+#include <stdint.h>
+
+namespace dfssm {
+
+constexpr int kScanChunk = 64;  // tokens of a chunk
+constexpr int kScanCols = 32;   // columns p of a wave
+constexpr int kScanWaves = 4;   // waves of a workgroup, which share B and C
+
+// Workgroups of a sequence (or a segment of one): each has up to four blocks of 32 columns of one group's heads.
+constexpr int64_t scan_wgs(int H, int G, int P) {
+  const int64_t blocks = (int64_t)(H / G) * ((P + kScanCols - 1) / kScanCols);
+  return G * ((blocks + kScanWaves - 1) / kScanWaves);
+}
+
+// Tokens of a segment. A sequence longer than that is cut into segments that run beside each other, from states
+// that a pass over all but the last of them makes first.
+constexpr int64_t scan_segment(int64_t n_tokens, int n_seq, int64_t wgs) {
+  const int64_t chunks = n_tokens / kScanChunk + n_seq;
+  int64_t m = (chunks * wgs + 511) / 512;
+  m = m < 4 ? 4 : m;
+  return m * kScanChunk;
+}
+
+// Places of the launch's numbering: segments of `seg` tokens, sequence b from floor(t0 / seg) + b on.
+constexpr int64_t scan_places(int64_t n_tokens, int n_seq, int64_t seg) { return n_tokens / seg + n_seq; }
+
+}  // namespace dfssm

@@ -126,7 +126,8 @@ _SIGS = {
     "dfssm_causal_conv_step": (c_int, [ctypes.POINTER(Conv), P]),
     "dfssm_causal_conv_prefill": (c_int, [ctypes.POINTER(Conv), P]),
     "dfssm_selective_scan_step": (c_int, [ctypes.POINTER(Scan), P]),
-    "dfssm_selective_scan_prefill": (c_int, [ctypes.POINTER(Scan), P]),
+    "dfssm_selective_scan_workspace_bytes": (c_size_t, [ctypes.POINTER(Scan)]),
+    "dfssm_selective_scan_prefill": (c_int, [ctypes.POINTER(Scan), P, P]),
     "dfssm_gated_norm": (c_int, [ctypes.POINTER(Gated), P]),
     "dfssm_residual_norm": (c_int, [ctypes.POINTER(Residual), P]),
 }

@@ -27,8 +27,8 @@ LIB = os.path.join(PKG, "libdfssm_hip.so")
 # profiling variant: the one-launch layer with per-phase wall-clock stamps (-DDFSSM_TIMELINE)
 LIB_TIMELINE = os.path.join(PKG, "libdfssm_hip_timeline.so")
 TIMELINE_SRCS = ("fused.hip",)
-# the chunked delta rule splits fp32 values into pairs of halves, one fma_mix each
-MIX_SRCS = ("delta_chunk.hip",)
+# the chunked operators split fp32 values into pairs of halves, one fma_mix each
+MIX_SRCS = ("delta_chunk.hip", "scan_chunk.hip")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc" if os.path.exists("/opt/rocm/bin/hipcc") else "hipcc")
 NO_MIX = ["-Xclang", "-target-feature", "-Xclang", "-fma-mix-insts"]

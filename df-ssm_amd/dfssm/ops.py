@@ -604,7 +604,12 @@ def _scan_call(step: bool, x, dt, A_log, B, C, state, D, dt_bias, cu_seqlens, sl
                    out.data_ptr(), ld_x, ld_dt, ld_B, ld_C, ld_out, T, n_seq, state.shape[0], H, G, P, N, kind,
                    2 if dt.dtype is f32 else kind, 1 if softplus else 0)
     L = _C.lib()
-    _run(dev, L.dfssm_selective_scan_step if step else L.dfssm_selective_scan_prefill, args, "selective_scan")
+    if step:
+        _run(dev, L.dfssm_selective_scan_step, args, "selective_scan_step")
+        return out
+    need = L.dfssm_selective_scan_workspace_bytes(args)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    _run(dev, lambda a, stream: L.dfssm_selective_scan_prefill(a, _C.ptr(ws), stream), args, "selective_scan_prefill")
     return out
 
 

@@ -457,8 +457,10 @@ typedef struct dfssm_scan {
 /* One token per sequence (n_tokens = n_seq). */
 int dfssm_selective_scan_step(const dfssm_scan* args, void* stream);
 /* Whole prompts, from the states the sequences have to those they leave: what dfssm_selective_scan_step gives token by
- * token, up to rounding. */
-int dfssm_selective_scan_prefill(const dfssm_scan* args, void* stream);
+ * token, up to rounding. workspace: 16-byte aligned device memory of dfssm_selective_scan_workspace_bytes(args) bytes (0:
+ * none needed, NULL allowed), for this call alone while it runs; its contents do not matter. */
+size_t dfssm_selective_scan_workspace_bytes(const dfssm_scan* args);
+int dfssm_selective_scan_prefill(const dfssm_scan* args, void* workspace, void* stream);
 
 /* out = rmsnorm(x s(gate)) weight (gate_first) or rmsnorm(x) weight s(gate), s(z) = z / (1 + e^-z), rmsnorm(v) =
  * v / sqrt(mean(v^2) + eps) over each of `groups` equal parts of a row; gate NULL: none. In fp32 with one rounding. out may be

@@ -41,18 +41,24 @@ def test_conv(kw, rc):
 def test_scan(kw, rc):
     L = _C.lib()
     assert L.dfssm_selective_scan_step(fill(_C.Scan, SCAN, kw), None) == rc
-    assert L.dfssm_selective_scan_prefill(fill(_C.Scan, SCAN, kw), None) == rc
+    assert L.dfssm_selective_scan_prefill(fill(_C.Scan, SCAN, kw), None, None) == rc
 
 
 def test_counts():
     L = _C.lib()
+    scan = lambda args, stream: L.dfssm_selective_scan_prefill(args, None, stream)
     for cls, base, step, whole in ((_C.Conv, CONV, L.dfssm_causal_conv_step, L.dfssm_causal_conv_prefill),
-                                   (_C.Scan, SCAN, L.dfssm_selective_scan_step, L.dfssm_selective_scan_prefill)):
+                                   (_C.Scan, SCAN, L.dfssm_selective_scan_step, scan)):
         assert step(None, None) == -1 and whole(None, None) == -1
         assert step(fill(cls, base, {"n_tokens": 3}), None) == -5 and step(fill(cls, base, {"cu_seqlens": 16}), None) == -5
         assert whole(fill(cls, base, {"n_tokens": 3}), None) == -5
         assert step(fill(cls, base, {"n_tokens": 0, "n_seq": 0}), None) == 0 and whole(fill(cls, base, {"n_seq": 0}), None) == 0
     assert L.dfssm_causal_conv_prefill(fill(_C.Conv, CONV, {"out": 16}), None) == -5      # out is x
+    bytes_ = L.dfssm_selective_scan_workspace_bytes
+    long = fill(_C.Scan, SCAN, {"n_tokens": 40000, "n_seq": 1})
+    assert bytes_(long) > 0 and bytes_(fill(_C.Scan, SCAN, {})) == 0 and bytes_(None) == 0
+    assert bytes_(fill(_C.Scan, SCAN, {"n_tokens": 40000, "n_seq": 1, "cols": 96})) == 0
+    assert L.dfssm_selective_scan_prefill(long, None, None) == -1 and L.dfssm_selective_scan_prefill(long, 8, None) == -4
 
 
 @pytest.mark.parametrize("kw,rc", [({"x": 0}, -1), ({"weight": 0}, -1), ({"out": 0}, -1), ({"cols": 0}, -2), ({"groups": 3}, -2),

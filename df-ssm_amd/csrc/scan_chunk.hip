@@ -121,6 +121,8 @@ scan_chunk_kernel(ScanArgs a, int64_t seg, int64_t places, float* seg_state, flo
   const bool active = blk < rep * ncb;
   const int h = gr * rep + (active ? blk / ncb : 0), p0 = active ? blk % ncb * kScanCols : 0;
   const bool wide = p0 + 16 < a.P;
+  // Row 8 m + 4 h + e of a 32 x 32 result is column 16 h + 4 m + e, so that a lane has 16 neighbouring columns of a token.
+  const int col = 16 * ((c >> 2) & 1) + 4 * (c >> 3) + (c & 3);
   const int slot = slot_of(a, q.seq);
   if (slot < 0) {
     const uint16_t fill = slot == kSlotPad ? 0 : 0x7fff;
@@ -130,10 +132,10 @@ scan_chunk_kernel(ScanArgs a, int64_t seg, int64_t places, float* seg_state, flo
   }
   const bool whole = place == q.first && last;  // the sequence is one segment
 
-  // S[t][8 b + e] is the state of row n = 32 t + 16 b + 8 hi + e and column p0 + c, over sfac.
+  // S[t][8 b + e] is the state of row n = 32 t + 16 b + 8 hi + e and column p0 + col, over sfac.
   f32x16 S[NN];
   float sfac = 1.0f, decay = 1.0f;
-  const int pc = c < 16 || wide ? p0 + c : p0 + c - 16;  // (columns that are not there do their neighbours' work)
+  const int pc = col < 16 || wide ? p0 + col : p0 + col - 16;  // (columns that are not there do their neighbours' work)
   const int64_t so = ((int64_t)h * a.P + pc) * N + 8 * hi, size = (int64_t)a.H * a.P * N;
   if constexpr (STATE) {
 #pragma unroll
@@ -211,14 +213,14 @@ scan_chunk_kernel(ScanArgs a, int64_t seg, int64_t places, float* seg_state, flo
       if (lane < 32) V.F[lane] = f;
     }
     wave_sync();
-    // x as operands: column p0 + c, tokens 16 k + 4 hi + 0 .. 3 and 8 more
+    // x as operands: column p0 + col, tokens 16 k + 4 hi + 0 .. 3 and 8 more
     h8 xf[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       s4 t[2];
 #pragma unroll
       for (int y = 0; y < 2; ++y)
-        t[y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tptr)&X[16 * k + 8 * y + 4 * hi + (l >> 2)][16 * ((lane >> 4) & 1) + 4 * (l & 3)]);
+        t[y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tptr)&X[16 * k + 8 * y + 4 * hi + (l >> 2)][16 * (l & 1) + 8 * ((lane >> 4) & 1) + 4 * ((l >> 1) & 1)]);
       xf[k] = __builtin_bit_cast(h8, __builtin_shufflevector(t[0], t[1], 0, 1, 2, 3, 4, 5, 6, 7));
     }
     __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): x is in registers, its place free
@@ -240,7 +242,7 @@ scan_chunk_kernel(ScanArgs a, int64_t seg, int64_t places, float* seg_state, flo
       float ssc = 1.0f, sinv = 1.0f;
       if constexpr (!BF) {
         ssc = pow2_scale(smax, sinv);
-        if (hi == 0) V.s[c] = sinv * sfac;
+        if (hi == 0) V.s[col] = sinv * sfac;
       }
       f32x16 sc[3], y[2];  // scores (columns 0 .. 31 of rows 0 .. 31; of rows 32 .. 63; columns 32 ..), y by tokens
 #pragma unroll
@@ -325,22 +327,26 @@ scan_chunk_kernel(ScanArgs a, int64_t seg, int64_t places, float* seg_state, flo
           for (int p = 1; p >= 0; --p) yx[t] = mm32<BF>(xf[k], m[2 * t + k][p], yx[t]);
       }
       __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): what is on its way for the next chunk, so that no later wait is for the stores
-      if (active) {
+      if (active && (hi == 0 || wide)) {
         const Rsrc orow = rows_of(a.out + (tok + (int64_t)i * kC) * a.ld_out + (int64_t)h * a.P + p0, a.ld_out, n, xw);
 #pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-          if (q4 >= 2 && !wide) break;
-          const f32x4 sv = BF ? f32x4{1.0f, 1.0f, 1.0f, 1.0f} : *(const f32x4*)&V.s[8 * q4 + 4 * hi];
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            float o[4];
+          for (int r = 0; r < 16; r += 8) {
+            uint32_t o[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              o[e] = __builtin_fmaf(y[t][4 * q4 + e], BF ? eG[t] : eG[t] * sv[e], BF ? yx[t][4 * q4 + e] : yx[t][4 * q4 + e] * pinv[t]);
-            __builtin_amdgcn_raw_buffer_store_b64(u32x2{pack2<BF>(o[0], o[1]), pack2<BF>(o[2], o[3])}, orow,
-                                                  (32 * t + c) * (int)a.ld_out * 2 + (8 * q4 + 4 * hi) * 2, 0, 0);
+            for (int e = 0; e < 8; e += 4) {
+              const f32x4 sv = BF ? f32x4{1.0f, 1.0f, 1.0f, 1.0f} : *(const f32x4*)&V.s[16 * hi + r + e];
+              float v[4];
+#pragma unroll
+              for (int z = 0; z < 4; ++z)
+                v[z] = __builtin_fmaf(y[t][r + e + z], BF ? eG[t] : eG[t] * sv[z], BF ? yx[t][r + e + z] : yx[t][r + e + z] * pinv[t]);
+              o[e / 2] = pack2<BF>(v[0], v[1]);
+              o[e / 2 + 1] = pack2<BF>(v[2], v[3]);
+            }
+            __builtin_amdgcn_raw_buffer_store_b128(u32x4{o[0], o[1], o[2], o[3]}, orow,
+                                                   (32 * t + c) * (int)a.ld_out * 2 + (16 * hi + r) * 2, 0, 0);
           }
-        }
       }
     } else {
       decay *= dec;
@@ -393,7 +399,7 @@ scan_chunk_kernel(ScanArgs a, int64_t seg, int64_t places, float* seg_state, flo
     if constexpr (STATE) __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
   }
 
-  if (!active || !(c < 16 || wide) || !(STATE || last)) return;
+  if (!active || !(col < 16 || wide) || !(STATE || last)) return;
   float* o = (STATE ? seg_state + place * size : a.state_out + slot * size) + so;
 #pragma unroll
   for (int t = 0; t < NN; ++t)

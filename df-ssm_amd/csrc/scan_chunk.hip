@@ -82,7 +82,9 @@ struct ScanLds {
   f16 C[STATE ? 1 : kC][STATE ? 8 : N];
   f16 x[kW][kC][kScanCols];
   struct {
-    float Gh[kC], Gl[kC], d[kC], w[kC], F[kScanCols], s[kScanCols];
+    float Gh[kC], Gl[kC], d[kC], w[kC];  // by tokens: G over log 2, the float nearest and the rest; d; w
+    float F[32], F16[32];                // d e^{G_32 - G_j}, j < 32; d e^{G_16 - G_j}, j < 16, and of tokens 32 .. 47
+    float s[kScanCols];                  // by columns: what undoes the scaling of the state
   } v[kW];
 };
 
@@ -209,8 +211,11 @@ scan_chunk_kernel(ScanArgs a, int64_t seg, int64_t places, float* seg_state, flo
       V.Gh[lane] = (float)G;
       V.Gl[lane] = (float)(G - (double)(float)G);
       V.d[lane] = d;
-      const float f = __builtin_amdgcn_exp2f(lane < 32 ? (float)(readlane_f64(G, 32) - G) : 0.0f) * d;
+      const float f = __builtin_amdgcn_exp2f((float)(readlane_f64(G, 32) - G)) * d;
+      const double G16 = readlane_f64(G, 16), G48 = readlane_f64(G, 48);
+      const float near = __builtin_amdgcn_exp2f((float)((lane < 32 ? G16 : G48) - G)) * d;
       if (lane < 32) V.F[lane] = f;
+      if (!(lane & 16)) V.F16[(lane & 15) + (lane >> 5) * 16] = near;
     }
     wave_sync();
     // x as operands: column p0 + col, tokens 16 k + 4 hi + 0 .. 3 and 8 more
@@ -270,17 +275,16 @@ scan_chunk_kernel(ScanArgs a, int64_t seg, int64_t places, float* seg_state, flo
       }
       step_barrier();  // C is free
       if (more) fetch_c(i + 1);
-      // M: a lane has row 32 t + c, columns 8 q + 4 hi + e
-      float pinv[2] = {1.0f, 1.0f}, eG[2];
-      h8 m[6][2];
-      const float Gb = V.Gh[32], gb = V.Gl[32];
+      // M: a lane has row 32 t + c, columns 8 q + 4 hi + e of each block of 32. Of a block on the diagonal it has 8 exponentials, of
+      // its own 16 columns; the other 16 are before its row, and e^{G_i - G_j} is taken apart at column 16, or behind it.
+      float pinv[2] = {1.0f, 1.0f};
+      const int own = c & 16;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const float Gi = V.Gh[32 * t + c], gi = V.Gl[32 * t + c];
-        eG[t] = __builtin_amdgcn_exp2f(Gi + gi);
         float x[32];
         if (t) {
-          const float ei = __builtin_amdgcn_exp2f((Gi - Gb) + (gi - gb));
+          const float ei = __builtin_amdgcn_exp2f((Gi - V.Gh[32]) + (gi - V.Gl[32]));
 #pragma unroll
           for (int q4 = 0; q4 < 4; ++q4) {
             const f32x4 F = *(const f32x4*)&V.F[8 * q4 + 4 * hi];
@@ -288,43 +292,47 @@ scan_chunk_kernel(ScanArgs a, int64_t seg, int64_t places, float* seg_state, flo
             for (int e = 0; e < 4; ++e) x[4 * q4 + e] = (sc[1][4 * q4 + e] * ei) * F[e];
           }
         }
+        const float ei = __builtin_amdgcn_exp2f((Gi - V.Gh[32 * t + 16]) + (gi - V.Gl[32 * t + 16]));
 #pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-          const int j0 = 8 * q4 + 4 * hi;
-          const f32x4 jh = *(const f32x4*)&V.Gh[32 * t + j0], jl = *(const f32x4*)&V.Gl[32 * t + j0], dj = *(const f32x4*)&V.d[32 * t + j0];
+        for (int z = 0; z < 2; ++z) {
+          const int j0 = 8 * z + 4 * hi;
+          const f32x4 jh = *(const f32x4*)&V.Gh[32 * t + own + j0], jl = *(const f32x4*)&V.Gl[32 * t + own + j0];
+          const f32x4 dj = *(const f32x4*)&V.d[32 * t + own + j0], F = *(const f32x4*)&V.F16[16 * t + j0];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {  // (beyond the diagonal the difference may be of any size: not exponentiated)
-            const bool low = j0 + e <= c;
-            const float ex = __builtin_amdgcn_exp2f(low ? (Gi - jh[e]) + (gi - jl[e]) : 0.0f) * dj[e];
-            float v = low ? sc[2 * t][4 * q4 + e] * ex : 0.0f;
-            v += j0 + e == c ? hp.D : 0.0f;
-            x[16 * t + 4 * q4 + e] = v;
+          for (int e = 0; e < 4; ++e) {  // (right of the diagonal the exponential may be infinite: not used)
+            const bool low = j0 + e <= (c & 15);
+            const float ex = __builtin_amdgcn_exp2f((Gi - jh[e]) + (gi - jl[e])) * dj[e], D = j0 + e == (c & 15) ? hp.D : 0.0f;
+            const float left = __builtin_fmaf(sc[2 * t][4 * z + e], own ? ei * F[e] : ex, own ? 0.0f : D);
+            const float right = __builtin_fmaf(sc[2 * t][8 + 4 * z + e], ex, D);
+            x[16 * t + 4 * z + e] = own || low ? left : 0.0f;
+            x[16 * t + 8 + 4 * z + e] = own && low ? right : 0.0f;
           }
         }
-        float msc = 1.0f;
+        // y of the state comes into M's scale (at most 2^40: what is lost of smaller M is below 2^-60)
+        float ys = __builtin_amdgcn_exp2f(Gi + gi), msc = 1.0f;
         if constexpr (!BF) {
           float top = 0.0f;
 #pragma unroll
           for (int e = 0; e < 16 * (t + 1); ++e) top = __builtin_elementwise_maximum(top, __builtin_fabsf(x[e]));
-          msc = pow2_scale(max_halves(top), pinv[t]);
+          msc = pow2_scale(__builtin_elementwise_maximum(max_halves(top), 0x1p-26f), pinv[t]);
+          ys *= msc;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+          const f32x4 sv = BF ? f32x4{1.0f, 1.0f, 1.0f, 1.0f} : *(const f32x4*)&V.s[16 * hi + r];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[t][r + e] *= BF ? ys : ys * sv[e];
         }
 #pragma unroll
         for (int k = 0; k < 2 * (t + 1); ++k) {
           float v[8];
+          h8 m[2];
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] = x[8 * k + e];
-          parts8<BF, 2>(v, msc, m[2 * t + k]);
+          parts8<BF, 2>(v, msc, m);
+#pragma unroll
+          for (int p = 1; p >= 0; --p) y[t] = mm32<BF>(xf[k], m[p], y[t]);
         }
-      }
-      f32x16 yx[2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) yx[t][r] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 2 * (t + 1); ++k)
-#pragma unroll
-          for (int p = 1; p >= 0; --p) yx[t] = mm32<BF>(xf[k], m[2 * t + k][p], yx[t]);
       }
       __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): what is on its way for the next chunk, so that no later wait is for the stores
       if (active && (hi == 0 || wide)) {
@@ -335,15 +343,9 @@ scan_chunk_kernel(ScanArgs a, int64_t seg, int64_t places, float* seg_state, flo
           for (int r = 0; r < 16; r += 8) {
             uint32_t o[4];
 #pragma unroll
-            for (int e = 0; e < 8; e += 4) {
-              const f32x4 sv = BF ? f32x4{1.0f, 1.0f, 1.0f, 1.0f} : *(const f32x4*)&V.s[16 * hi + r + e];
-              float v[4];
-#pragma unroll
-              for (int z = 0; z < 4; ++z)
-                v[z] = __builtin_fmaf(y[t][r + e + z], BF ? eG[t] : eG[t] * sv[z], BF ? yx[t][r + e + z] : yx[t][r + e + z] * pinv[t]);
-              o[e / 2] = pack2<BF>(v[0], v[1]);
-              o[e / 2 + 1] = pack2<BF>(v[2], v[3]);
-            }
+            for (int e = 0; e < 4; ++e)
+              o[e] = BF ? pack2<BF>(y[t][r + 2 * e], y[t][r + 2 * e + 1])
+                        : pack2<BF>(y[t][r + 2 * e] * pinv[t], y[t][r + 2 * e + 1] * pinv[t]);
             __builtin_amdgcn_raw_buffer_store_b128(u32x4{o[0], o[1], o[2], o[3]}, orow,
                                                    (32 * t + c) * (int)a.ld_out * 2 + (16 * hi + r) * 2, 0, 0);
           }

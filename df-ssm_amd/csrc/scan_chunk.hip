@@ -27,10 +27,13 @@ __device__ __forceinline__ f32x16 mm32(h8 a, h8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-// Eight values as NT parts: pairs of halves of x sc, or NT parts of bf16 (sc is 1).
-template <bool BF, int NT>
+// Eight values as NT parts: pairs of halves of x sc, or NT parts of bf16 (sc is 1). What a bf16 part leaves of two values
+// comes from a dot product each, x + (-1, 0) (p0, p1) and x + (0, -1) (p0, p1), which is exact. (The factors are in registers: the
+// compiler writes the first as the constant -1.0, which the instruction takes as the second.)
+template <bool BF, int NT, bool DIES = true>
 __device__ __forceinline__ void parts8(const float (&x)[8], float sc, h8 (&part)[NT]) {
-  uint32_t p[NT][4];
+  uint32_t p[NT][4], k0 = 0x0000bf80u, k1 = 0xbf800000u;
+  asm("" : "+s"(k0), "+s"(k1));
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     if constexpr (!BF) {
@@ -42,11 +45,15 @@ __device__ __forceinline__ void parts8(const float (&x)[8], float sc, h8 (&part)
       float x0 = x[2 * q], x1 = x[2 * q + 1];
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        uint32_t t = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x0, x1}, b2));
-        asm("" : "+v"(t));
-        p[i][q] = t;
-        x0 -= __builtin_bit_cast(float, t << 16);
-        x1 -= __builtin_bit_cast(float, t & 0xffff0000u);
+        const b2 t = __builtin_convertvector(f32x2{x0, x1}, b2);
+        p[i][q] = __builtin_bit_cast(uint32_t, t);
+        if (i + 1 < NT && !DIES) {
+          x0 -= __builtin_bit_cast(float, p[i][q] << 16);
+          x1 -= __builtin_bit_cast(float, p[i][q] & 0xffff0000u);
+        } else if (i + 1 < NT) {
+          x0 = __builtin_amdgcn_fdot2_f32_bf16(t, __builtin_bit_cast(b2, k0), x0, false);
+          x1 = __builtin_amdgcn_fdot2_f32_bf16(t, __builtin_bit_cast(b2, k1), x1, false);
+        }
       }
     }
   }
@@ -76,36 +83,55 @@ __device__ __forceinline__ int swap_of(int row) {
 
 typedef __attribute__((address_space(3))) s4* tptr;
 
+// Row 8 m + 4 h + e of a 32 x 32 result is column 16 h + 4 m + e, so that a lane has 16 neighbouring columns of a token. The
+// column of a lane that has a column of the state:
+__device__ __forceinline__ int scan_col(int lane) { return 16 * ((lane >> 2) & 1) + 4 * ((lane & 31) >> 3) + (lane & 3); }
+
+// The lane, as a value that the compiler derives offsets from anew where it is asked for: held over the whole loop they are more
+// registers than there are.
+__device__ __forceinline__ int lane_again() {
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));
+  return lane;
+}
+
+__device__ __forceinline__ float uniform(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+}
+
 template <int N, bool STATE>
 struct ScanLds {
-  f16 B[2][kC][N];
+  f16 B[kC][N];
   f16 C[STATE ? 1 : kC][STATE ? 8 : N];
   f16 x[kW][kC][kScanCols];
   struct {
-    float Gh[kC], Gl[kC], d[kC], w[kC];  // by tokens: G over log 2, the float nearest and the rest; d; w
+    float Gh[kC], Gl[kC], d[kC];         // by tokens: G over log 2, the float nearest (then w) and the rest; d
     float F[32], F16[32];                // d e^{G_32 - G_j}, j < 32; d e^{G_16 - G_j}, j < 16, and of tokens 32 .. 47
     float s[kScanCols];                  // by columns: what undoes the scaling of the state
   } v[kW];
 };
 
+// `len` rows, ld bytes apart, of `bytes` bytes: loads behind the last one give zero, stores are dropped.
+__device__ __forceinline__ Rsrc bytes_of(const void* p, int ld, int len, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (len - 1) * ld + bytes, 0x00027000);
+}
+
 // A wave's quarter of 64 rows of B or C, into LDS.
 template <int N>
-__device__ __forceinline__ void fetch_shared(f16 (*to)[N], const uint16_t* p, int64_t ld, int len, int wave, int off) {
+__device__ __forceinline__ void fetch_shared(f16 (*to)[N], const char* p, int ld, int len, int wave, int off) {
   constexpr int per = 512 / N;  // rows of a KiB
-  const Rsrc r = rows_of(p, ld, len, N);
+  const Rsrc r = bytes_of(p, ld, len, 2 * N);
 #pragma unroll
   for (int n = 0; n < kC / per / kW; ++n)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr)((char*)to + (kW * n + wave) * 1024), 16, off + n * (kW * per * 2) * (int)ld, 0,
-                                             0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr)((char*)to + (kW * n + wave) * 1024), 16, off + n * kW * per * ld, 0, 0, 0);
 }
 
 // STATE: the states that a segment leaves from zero, and its decay, of all segments but the last of a sequence.
 template <int N, bool BF, bool STATE>
-__global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(64 * kW) void
+__global__ __attribute__((amdgpu_waves_per_eu(3))) __launch_bounds__(64 * kW) void
 scan_chunk_kernel(ScanArgs a, int64_t seg, int64_t places, float* seg_state, float* seg_decay) {
   constexpr int NB = N / 16, NN = N / 32, NU = kParts<BF>, pieces = N / 8;
   __shared__ __align__(16) ScanLds<N, STATE> L;
-  const int lane = threadIdx.x & 63, hi = lane >> 5, c = lane & 31, l = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Workgroups go to the eight dies in turn: all that share a group's B and C run on one, next to its L2.
   const int rep = a.H / a.G, ncb = (a.P + kScanCols - 1) / kScanCols, nwg = (rep * ncb + kW - 1) / kW;
@@ -115,7 +141,7 @@ scan_chunk_kernel(ScanArgs a, int64_t seg, int64_t places, float* seg_state, flo
   const int gr = (int)(unit % a.G), blk = (int)(in % nwg) * kW + wave;
   Where q{0, 0, 0, 0};
   int64_t tok;
-  const int64_t len = tile_of<0>(a, place, q, tok, seg);
+  const int len = (int)tile_of<0>(a, place, q, tok, seg);  // (tokens fit 31 bits)
   if (len == 0) tok = q.t0;
   const bool last = tok + len >= q.t1;
   if (len == 0 && !(!STATE && place == q.first && q.t0 == q.t1)) return;  // (an empty sequence's state is passed on)
@@ -123,22 +149,24 @@ scan_chunk_kernel(ScanArgs a, int64_t seg, int64_t places, float* seg_state, flo
   const bool active = blk < rep * ncb;
   const int h = gr * rep + (active ? blk / ncb : 0), p0 = active ? blk % ncb * kScanCols : 0;
   const bool wide = p0 + 16 < a.P;
-  // Row 8 m + 4 h + e of a 32 x 32 result is column 16 h + 4 m + e, so that a lane has 16 neighbouring columns of a token.
-  const int col = 16 * ((c >> 2) & 1) + 4 * (c >> 3) + (c & 3);
   const int slot = slot_of(a, q.seq);
   if (slot < 0) {
     const uint16_t fill = slot == kSlotPad ? 0 : 0x7fff;
+    const int c = threadIdx.x & 31;
     if (!STATE && active && (c < 16 || wide))
-      for (int64_t t = hi; t < len; t += 2) a.out[(tok + t) * a.ld_out + (int64_t)h * a.P + p0 + c] = fill;
+      for (int64_t t = threadIdx.x >> 5 & 1; t < len; t += 2) a.out[(tok + t) * a.ld_out + (int64_t)h * a.P + p0 + c] = fill;
     return;
   }
   const bool whole = place == q.first && last;  // the sequence is one segment
 
-  // S[t][8 b + e] is the state of row n = 32 t + 16 b + 8 hi + e and column p0 + col, over sfac.
+  // S[t][8 b + e] is the state of row n = 32 t + 16 b + 8 hi + e and column p0 + scan_col, over sfac.
   f32x16 S[NN];
   float sfac = 1.0f, decay = 1.0f;
-  const int pc = col < 16 || wide ? p0 + col : p0 + col - 16;  // (columns that are not there do their neighbours' work)
-  const int64_t so = ((int64_t)h * a.P + pc) * N + 8 * hi, size = (int64_t)a.H * a.P * N;
+  const int64_t size = (int64_t)a.H * a.P * N, so = ((int64_t)h * a.P + p0) * N;
+  auto state_at = [&](int lane) {  // (columns that are not there do their neighbours' work)
+    const int col = scan_col(lane);
+    return (uint32_t)((col < 16 || wide ? col : col - 16) * N + 8 * (lane >> 5));
+  };
   if constexpr (STATE) {
 #pragma unroll
     for (int t = 0; t < NN; ++t)
@@ -146,175 +174,182 @@ scan_chunk_kernel(ScanArgs a, int64_t seg, int64_t places, float* seg_state, flo
       for (int r = 0; r < 16; ++r) S[t][r] = 0.0f;
   } else {
     const float* sp = (whole || len == 0 ? a.state + slot * size : seg_state + place * size) + so;
+    const uint32_t at = state_at(threadIdx.x & 63);
 #pragma unroll
     for (int t = 0; t < NN; ++t)
 #pragma unroll
       for (int m = 0; m < 4; ++m) {
-        const f32x4 v = *(const f32x4*)(sp + 32 * t + 16 * (m >> 1) + 4 * (m & 1));
+        const f32x4 v = *(const f32x4*)(sp + at + 32 * t + 16 * (m >> 1) + 4 * (m & 1));
 #pragma unroll
         for (int e = 0; e < 4; ++e) S[t][4 * m + e] = v[e];
       }
   }
-  const HeadParams hp = head_params(a, h);
+  HeadParams hp = head_params(a, h);
+  hp.A = uniform(hp.A), hp.D = uniform(hp.D), hp.bias = uniform(hp.bias);
   auto& V = L.v[wave];
   f16 (&X)[kC][kScanCols] = L.x[wave];
-  const int off_row = 512 / N * wave + lane / pieces, off_piece = ((lane % pieces) ^ swap_of<N>(off_row)) * 16;
-  const int off_b = off_row * (int)a.ld_B * 2 + off_piece, off_c = off_row * (int)a.ld_C * 2 + off_piece;
-  const int off_x = (lane >> 2) * (int)a.ld_x * 2 + (lane & 3) * 16;
-  const int xw = a.P - p0 < kScanCols ? a.P - p0 : kScanCols;
-  const int n_chunks = (int)((len + kC - 1) / kC);
-  auto rows_at = [&](int i) { return (int)(len - (int64_t)i * kC < kC ? len - (int64_t)i * kC : kC); };
-  auto fetch_b = [&](int i) {
-    fetch_shared<N>(L.B[i & 1], a.B + (tok + (int64_t)i * kC) * a.ld_B + gr * N, a.ld_B, rows_at(i), wave, off_b);
-  };
-  auto fetch_c = [&](int i) {
-    if constexpr (!STATE) fetch_shared<N>(L.C, a.C + (tok + (int64_t)i * kC) * a.ld_C + gr * N, a.ld_C, rows_at(i), wave, off_c);
-  };
-  auto fetch_x = [&](int i) {
-    const Rsrc r = rows_of(a.x + (tok + (int64_t)i * kC) * a.ld_x + (int64_t)h * a.P + p0, a.ld_x, rows_at(i), xw);
+  const int xw = 2 * (a.P - p0 < kScanCols ? a.P - p0 : kScanCols);  // bytes of a row
+  // (in bytes from here on; 64 rows are 2^30 at most)
+  const int ld_b = (int)a.ld_B * 2, ld_c = (int)a.ld_C * 2, ld_x = (int)a.ld_x * 2, ld_o = (int)a.ld_out * 2;
+  const int dt_size = a.dt32 ? 4 : 2, ld_t = (int)a.ld_dt * dt_size;
+  const char *pb = (const char*)(a.B + tok * a.ld_B + gr * N), *pc = (const char*)(a.C + tok * a.ld_C + gr * N);
+  const char *px = (const char*)(a.x + tok * a.ld_x + (int64_t)h * a.P + p0), *pt = (const char*)a.dt + tok * ld_t + h * dt_size;
+  char* po = (char*)(a.out + tok * a.ld_out + (int64_t)h * a.P + p0);
+  // x as an operand: column p0 + scan_col, tokens 16 k + 4 hi + 0 .. 3 and 8 more
+  auto x_frag = [&](int lane, int k) {
+    const int row = 4 * (lane >> 5) + ((lane & 15) >> 2), at = 16 * (lane & 1) + 8 * ((lane >> 4) & 1) + 4 * ((lane >> 1) & 1);
+    s4 t[2];
 #pragma unroll
-    for (int n = 0; n < 4; ++n)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr)((char*)X + n * 1024), 16, off_x + n * 32 * (int)a.ld_x, 0, 0, 0);
+    for (int y = 0; y < 2; ++y) t[y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tptr)&X[16 * k + 8 * y + row][at]);
+    return __builtin_bit_cast(h8, __builtin_shufflevector(t[0], t[1], 0, 1, 2, 3, 4, 5, 6, 7));
   };
   float raw = 0.0f;
-  auto fetch_dt = [&](int i) {
-    const int n = rows_at(i);
-    raw = load_dt<BF>(a, tok + (int64_t)i * kC + (lane < n ? lane : n - 1), h);
+  auto fetch_dt = [&](int left) {  // (zero behind the last token)
+    const Rsrc r = bytes_of(pt, ld_t, left < kC ? left : kC, dt_size);
+    const int at = lane_again() * ld_t;
+    raw = a.dt32 ? __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0))
+                 : w2f<BF>(__builtin_amdgcn_raw_buffer_load_b16(r, at, 0, 0));
+    pt += kC * ld_t;
   };
-  if (n_chunks) {
-    fetch_b(0);
-    fetch_c(0);
-    fetch_x(0);
-    fetch_dt(0);
-  }
-  __builtin_amdgcn_s_waitcnt(0);
+  if (len) fetch_dt(len);
 
-  for (int i = 0; i < n_chunks; ++i) {
-    const int n = rows_at(i);
-    const bool more = i + 1 < n_chunks;
-    step_barrier();  // this chunk's B and C are in LDS, and the next one's place for B is free
-    // the time steps; lane: a token
-    const float d = lane < n ? time_step(raw, hp, a.softplus) : 0.0f;
-    float al = d * hp.A;
-    al = al < -1e5f ? -1e5f : al;
-    double G = (double)al * 1.4426950408889634;
-    G += moved<0x111, 0xf>(G);  // running sums: from 1, 2, 4 and 8 lanes before, in the row of 16
-    G += moved<0x112, 0xf>(G);
-    G += moved<0x114, 0xf>(G);
-    G += moved<0x118, 0xf>(G);
-    G += moved<0x142, 0xa>(G);  // row 0's last to row 1, 2's to 3; then lane 31's to rows 2 and 3
-    G += moved<0x143, 0xc>(G);
-    const double GC = readlane_f64(G, 63);
-    const float dec = __builtin_amdgcn_exp2f((float)GC);
-    V.w[lane] = __builtin_amdgcn_exp2f((float)(GC - G)) * d;
-    if constexpr (!STATE) {
-      V.Gh[lane] = (float)G;
-      V.Gl[lane] = (float)(G - (double)(float)G);
-      V.d[lane] = d;
-      const float f = __builtin_amdgcn_exp2f((float)(readlane_f64(G, 32) - G)) * d;
-      const double G16 = readlane_f64(G, 16), G48 = readlane_f64(G, 48);
-      const float near = __builtin_amdgcn_exp2f((float)((lane < 32 ? G16 : G48) - G)) * d;
-      if (lane < 32) V.F[lane] = f;
-      if (!(lane & 16)) V.F16[(lane & 15) + (lane >> 5) * 16] = near;
-    }
-    wave_sync();
-    // x as operands: column p0 + col, tokens 16 k + 4 hi + 0 .. 3 and 8 more
-    h8 xf[4];
+  for (int left = len; left > 0; left -= kC) {
+    const int n = left < kC ? left : kC;
+    {
+      const int lane = lane_again(), row = 512 / N * wave + lane / pieces, piece = ((lane % pieces) ^ swap_of<N>(row)) * 16;
+      fetch_shared<N>(L.B, pb, ld_b, n, wave, row * ld_b + piece);
+      if constexpr (!STATE) fetch_shared<N>(L.C, pc, ld_c, n, wave, row * ld_c + piece);
+      const Rsrc r = bytes_of(px, ld_x, n, xw);
+      const int off = (lane >> 2) * ld_x + (lane & 3) * 16;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      s4 t[2];
-#pragma unroll
-      for (int y = 0; y < 2; ++y)
-        t[y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tptr)&X[16 * k + 8 * y + 4 * hi + (l >> 2)][16 * (l & 1) + 8 * ((lane >> 4) & 1) + 4 * ((l >> 1) & 1)]);
-      xf[k] = __builtin_bit_cast(h8, __builtin_shufflevector(t[0], t[1], 0, 1, 2, 3, 4, 5, 6, 7));
+      for (int m = 0; m < 4; ++m)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr)((char*)X + m * 1024), 16, off + m * 16 * ld_x, 0, 0, 0);
     }
-    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): x is in registers, its place free
-    asm volatile("" ::: "memory");
-    if (more) {
-      fetch_b(i + 1);
-      fetch_x(i + 1);
-      fetch_dt(i + 1);
+    pb += kC * ld_b;
+    pc += kC * ld_c;
+    px += kC * ld_x;
+    // While they are on their way: the time steps; a lane has a token.
+    float dec, wj;
+    {
+      const int lane = lane_again();
+      const float d = lane < n ? time_step(raw, hp, a.softplus) : 0.0f;
+      float al = d * hp.A;
+      al = al < -1e5f ? -1e5f : al;
+      double G = (double)al * 1.4426950408889634;
+      G += moved<0x111, 0xf>(G);  // running sums: from 1, 2, 4 and 8 lanes before, in the row of 16
+      G += moved<0x112, 0xf>(G);
+      G += moved<0x114, 0xf>(G);
+      G += moved<0x118, 0xf>(G);
+      G += moved<0x142, 0xa>(G);  // row 0's last to row 1, 2's to 3; then lane 31's to rows 2 and 3
+      G += moved<0x143, 0xc>(G);
+      const double GC = readlane_f64(G, 63);
+      dec = __builtin_amdgcn_exp2f((float)GC);
+      wj = __builtin_amdgcn_exp2f((float)(GC - G)) * d;
+      if constexpr (!STATE) {
+        V.Gh[lane] = (float)G;
+        V.Gl[lane] = (float)(G - (double)(float)G);
+        V.d[lane] = d;
+        const float f = __builtin_amdgcn_exp2f((float)(readlane_f64(G, 32) - G)) * d;
+        const double G16 = readlane_f64(G, 16), G48 = readlane_f64(G, 48);
+        const float near = __builtin_amdgcn_exp2f((float)((lane < 32 ? G16 : G48) - G)) * d;
+        if (lane < 32) V.F[lane] = f;
+        if (!(lane & 16)) V.F16[(lane & 15) + (lane >> 5) * 16] = near;
+      }
     }
-    float smax = 0.0f;
+    if (left > kC) fetch_dt(left - kC);
+    float smax = 0.0f, ssc = 1.0f;
     if constexpr (!BF) {
 #pragma unroll
       for (int t = 0; t < NN; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) smax = __builtin_elementwise_maximum(smax, __builtin_fabsf(S[t][r]));
       smax = max_halves(smax);
+      float sinv;
+      ssc = pow2_scale(smax, sinv);
+      if (!(threadIdx.x & 32)) V.s[scan_col(lane_again())] = sinv * sfac;
     }
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    step_barrier();                      // B, C and x are in LDS
     if constexpr (!STATE) {
-      float ssc = 1.0f, sinv = 1.0f;
-      if constexpr (!BF) {
-        ssc = pow2_scale(smax, sinv);
-        if (hi == 0) V.s[col] = sinv * sfac;
-      }
-      f32x16 sc[3], y[2];  // scores (columns 0 .. 31 of rows 0 .. 31; of rows 32 .. 63; columns 32 ..), y by tokens
+      f32x16 y[2], sc[2];  // y by tokens; scores
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sc[0][r] = sc[1][r] = sc[2][r] = y[0][r] = y[1][r] = 0.0f;
+      for (int r = 0; r < 16; ++r) y[0][r] = y[1][r] = 0.0f;
+      const int lane = lane_again(), hi = lane >> 5, c = lane & 31;
+      auto row_frag = [&](const f16 (*rows)[N], int t, int b) {
+        return *(const h8*)&rows[32 * t + c][((2 * b + hi) ^ swap_of<N>(c)) * 8];
+      };
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        h8 cf[2], bf[2], s[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int row = 32 * t + c, at = ((2 * b + hi) ^ swap_of<N>(c)) * 8;
-          cf[t] = *(const h8*)&L.C[row][at];
-          bf[t] = *(const h8*)&L.B[i & 1][row][at];
-        }
+        const h8 c0 = row_frag(L.C, 0, b), c1 = row_frag(L.C, 1, b);
         float sv[8];
+        h8 s[2];
 #pragma unroll
         for (int e = 0; e < 8; ++e) sv[e] = S[b >> 1][8 * (b & 1) + e];
-        parts8<BF, 2>(sv, ssc, s);
-        sc[0] = mm32<BF>(bf[0], cf[0], sc[0]);
-        sc[1] = mm32<BF>(bf[0], cf[1], sc[1]);
-        sc[2] = mm32<BF>(bf[1], cf[1], sc[2]);
-#pragma unroll
-        for (int p = 1; p >= 0; --p)
-#pragma unroll
-          for (int t = 0; t < 2; ++t) y[t] = mm32<BF>(s[p], cf[t], y[t]);
+        parts8<BF, 2, false>(sv, ssc, s);
+        y[0] = mm32<BF>(s[1], c0, y[0]);
+        y[1] = mm32<BF>(s[1], c1, y[1]);
+        y[0] = mm32<BF>(s[0], c0, y[0]);
+        y[1] = mm32<BF>(s[0], c1, y[1]);
       }
-      step_barrier();  // C is free
-      if (more) fetch_c(i + 1);
+      __builtin_amdgcn_sched_barrier(0);
       // M: a lane has row 32 t + c, columns 8 q + 4 hi + e of each block of 32. Of a block on the diagonal it has 8 exponentials, of
       // its own 16 columns; the other 16 are before its row, and e^{G_i - G_j} is taken apart at column 16, or behind it.
-      float pinv[2] = {1.0f, 1.0f};
-      const int own = c & 16;
+      const Rsrc orow = bytes_of(po, ld_o, n, xw);
+      const bool own = c & 16;
+      const int lim = (c & 15) - 4 * hi;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
+        f32x16& D = sc[t ? 1 : 0];
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u <= t; ++u)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sc[u][r] = 0.0f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const h8 ct = row_frag(L.C, t, b);
+#pragma unroll
+          for (int u = 0; u <= t; ++u) sc[u] = mm32<BF>(row_frag(L.B, u, b), ct, sc[u]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
         const float Gi = V.Gh[32 * t + c], gi = V.Gl[32 * t + c];
-        float x[32];
         if (t) {
           const float ei = __builtin_amdgcn_exp2f((Gi - V.Gh[32]) + (gi - V.Gl[32]));
 #pragma unroll
           for (int q4 = 0; q4 < 4; ++q4) {
             const f32x4 F = *(const f32x4*)&V.F[8 * q4 + 4 * hi];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[4 * q4 + e] = (sc[1][4 * q4 + e] * ei) * F[e];
+            for (int e = 0; e < 4; ++e) sc[0][4 * q4 + e] = (sc[0][4 * q4 + e] * ei) * F[e];
           }
         }
+        __builtin_amdgcn_sched_barrier(0);
         const float ei = __builtin_amdgcn_exp2f((Gi - V.Gh[32 * t + 16]) + (gi - V.Gl[32 * t + 16]));
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
+          __builtin_amdgcn_sched_barrier(0);
           const int j0 = 8 * z + 4 * hi;
-          const f32x4 jh = *(const f32x4*)&V.Gh[32 * t + own + j0], jl = *(const f32x4*)&V.Gl[32 * t + own + j0];
-          const f32x4 dj = *(const f32x4*)&V.d[32 * t + own + j0], F = *(const f32x4*)&V.F16[16 * t + j0];
+          const f32x4 jh = *(const f32x4*)&V.Gh[32 * t + (c & 16) + j0], jl = *(const f32x4*)&V.Gl[32 * t + (c & 16) + j0];
+          const f32x4 dj = *(const f32x4*)&V.d[32 * t + (c & 16) + j0], F = *(const f32x4*)&V.F16[16 * t + j0];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {  // (right of the diagonal the exponential may be infinite: not used)
-            const bool low = j0 + e <= (c & 15);
-            const float ex = __builtin_amdgcn_exp2f((Gi - jh[e]) + (gi - jl[e])) * dj[e], D = j0 + e == (c & 15) ? hp.D : 0.0f;
-            const float left = __builtin_fmaf(sc[2 * t][4 * z + e], own ? ei * F[e] : ex, own ? 0.0f : D);
-            const float right = __builtin_fmaf(sc[2 * t][8 + 4 * z + e], ex, D);
-            x[16 * t + 4 * z + e] = own || low ? left : 0.0f;
-            x[16 * t + 8 + 4 * z + e] = own && low ? right : 0.0f;
+            const int k = 4 * z + e;
+            const float ex = __builtin_amdgcn_exp2f((Gi - jh[e]) + (gi - jl[e])) * dj[e];
+            float v = __builtin_fmaf(own ? D[8 + k] : D[k], ex, 8 * z + e == lim ? hp.D : 0.0f);
+            v = 8 * z + e <= lim ? v : 0.0f;
+            D[k] = own ? D[k] * (ei * F[e]) : v;
+            D[8 + k] = own ? v : 0.0f;
           }
         }
+        __builtin_amdgcn_sched_barrier(0);
         // y of the state comes into M's scale (at most 2^40: what is lost of smaller M is below 2^-60)
-        float ys = __builtin_amdgcn_exp2f(Gi + gi), msc = 1.0f;
+        float ys = __builtin_amdgcn_exp2f(Gi + gi), msc = 1.0f, pinv = 1.0f;
         if constexpr (!BF) {
-          float top = 0.0f;
+          float top = 0x1p-26f;
 #pragma unroll
-          for (int e = 0; e < 16 * (t + 1); ++e) top = __builtin_elementwise_maximum(top, __builtin_fabsf(x[e]));
-          msc = pow2_scale(__builtin_elementwise_maximum(max_halves(top), 0x1p-26f), pinv[t]);
+          for (int u = 0; u <= t; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = __builtin_elementwise_maximum(top, __builtin_fabsf(sc[u][r]));
+          msc = pow2_scale(max_halves(top), pinv);
           ys *= msc;
         }
 #pragma unroll
@@ -328,49 +363,54 @@ scan_chunk_kernel(ScanArgs a, int64_t seg, int64_t places, float* seg_state, flo
           float v[8];
           h8 m[2];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = x[8 * k + e];
+          for (int e = 0; e < 8; ++e) v[e] = sc[k >> 1][8 * (k & 1) + e];
+          __builtin_amdgcn_sched_barrier(0);
           parts8<BF, 2>(v, msc, m);
+          const h8 x = x_frag(lane, k);
 #pragma unroll
-          for (int p = 1; p >= 0; --p) y[t] = mm32<BF>(xf[k], m[p], y[t]);
+          for (int p = 1; p >= 0; --p) y[t] = mm32<BF>(x, m[p], y[t]);
         }
-      }
-      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): what is on its way for the next chunk, so that no later wait is for the stores
-      if (active && (hi == 0 || wide)) {
-        const Rsrc orow = rows_of(a.out + (tok + (int64_t)i * kC) * a.ld_out + (int64_t)h * a.P + p0, a.ld_out, n, xw);
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
+        if (active && (hi == 0 || wide))
 #pragma unroll
           for (int r = 0; r < 16; r += 8) {
             uint32_t o[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               o[e] = BF ? pack2<BF>(y[t][r + 2 * e], y[t][r + 2 * e + 1])
-                        : pack2<BF>(y[t][r + 2 * e] * pinv[t], y[t][r + 2 * e + 1] * pinv[t]);
-            __builtin_amdgcn_raw_buffer_store_b128(u32x4{o[0], o[1], o[2], o[3]}, orow,
-                                                   (32 * t + c) * (int)a.ld_out * 2 + (16 * hi + r) * 2, 0, 0);
+                        : pack2<BF>(y[t][r + 2 * e] * pinv, y[t][r + 2 * e + 1] * pinv);
+            __builtin_amdgcn_raw_buffer_store_b128(u32x4{o[0], o[1], o[2], o[3]}, orow, (32 * t + c) * ld_o + 32 * hi + 2 * r, 0, 0);
           }
       }
+      po += kC * ld_o;
     } else {
       decay *= dec;
     }
+    __builtin_amdgcn_sched_barrier(0);
     // the new state
-    float u[4][8];
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
+    const int lane = lane_again(), hi = lane >> 5, l = lane & 15;
+    V.Gh[lane] = wj;
+    wave_sync();
+    float keep = dec, usc = 1.0f;
+    auto weighted = [&](int k, float (&u)[8]) {
+      const h8 x = x_frag(lane, k);
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-        const f32x4 w = *(const f32x4*)&V.w[16 * k + 8 * y + 4 * hi];
+        const f32x4 w = *(const f32x4*)&V.Gh[16 * k + 8 * y + 4 * hi];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const f16 v = xf[k][4 * y + e];  // (a bit cast of the element itself takes the vector's first one)
-          u[k][4 * y + e] = w2f<BF>(__builtin_bit_cast(uint16_t, v)) * w[e];
+          const f16 v = x[4 * y + e];  // (a bit cast of the element itself takes the vector's first one)
+          u[4 * y + e] = w2f<BF>(__builtin_bit_cast(uint16_t, v)) * w[e];
         }
       }
-    float keep = dec, usc = 1.0f;
+    };
+    float u[4][8];
     if constexpr (!BF) {
       float top = 0.0f, uinv;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) top = max_abs(u[k], top);
+      for (int k = 0; k < 4; ++k) {
+        weighted(k, u[k]);
+        top = max_abs(u[k], top);
+      }
       usc = pow2_scale(__builtin_elementwise_maximum(max_halves(top), dec * (smax * sfac)), uinv);
       keep = dec * sfac * usc;
       sfac = uinv;
@@ -381,6 +421,8 @@ scan_chunk_kernel(ScanArgs a, int64_t seg, int64_t places, float* seg_state, flo
       for (int r = 0; r < 16; ++r) S[t][r] *= keep;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (BF) weighted(k, u[k]);
       h8 up[NU];
       parts8<BF, NU>(u[k], usc, up);
 #pragma unroll
@@ -389,20 +431,21 @@ scan_chunk_kernel(ScanArgs a, int64_t seg, int64_t places, float* seg_state, flo
         s4 b[2];
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
-          const int row = 16 * k + 8 * y + 4 * hi + (l >> 2), mm = (l & 3) >> 1 | (l & 1) << 1;
-          const int piece = (4 * t + 2 * ((lane >> 4) & 1) + (mm >> 1)) ^ swap_of<N>(row & 15);
-          b[y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tptr)&L.B[i & 1][row][piece * 8 + 4 * (mm & 1)]);
+          const int row = 16 * k + 8 * y + 4 * hi + (l >> 2), m = (l & 3) >> 1 | (l & 1) << 1;
+          const int piece = (4 * t + 2 * ((lane >> 4) & 1) + (m >> 1)) ^ swap_of<N>(row & 15);
+          b[y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tptr)&L.B[row][piece * 8 + 4 * (m & 1)]);
         }
         const h8 bt = __builtin_bit_cast(h8, __builtin_shufflevector(b[0], b[1], 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
         for (int p = NU - 1; p >= 0; --p) S[t] = mm32<BF>(bt, up[p], S[t]);
       }
     }
-    if constexpr (STATE) __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    step_barrier();  // B, C and x are free
   }
 
-  if (!active || !(col < 16 || wide) || !(STATE || last)) return;
-  float* o = (STATE ? seg_state + place * size : a.state_out + slot * size) + so;
+  const int lane = lane_again();
+  if (!active || !(scan_col(lane) < 16 || wide) || !(STATE || last)) return;
+  float* o = (STATE ? seg_state + place * size : a.state_out + slot * size) + so + state_at(lane);
 #pragma unroll
   for (int t = 0; t < NN; ++t)
 #pragma unroll

@@ -459,30 +459,40 @@ scan_chunk_kernel(ScanArgs a, int64_t seg, int64_t places, float* seg_state, flo
 }
 
 // The states before each segment of a sequence of several, in place of those that its segments leave from zero. A thread
-// has four values of a head.
-__global__ __launch_bounds__(256) void scan_states_kernel(ScanArgs a, int64_t seg, float* seg_state, const float* seg_decay) {
-  const int64_t size = (int64_t)a.H * a.P * a.N, per = (size / 4 + 255) / 256;
+// has four values of a head at a time, and those of eight segments on their way together (one by one, 16 segments of 64 heads
+// took 13 us); `per` workgroups to a sequence.
+__global__ __launch_bounds__(256) void scan_states_kernel(ScanArgs a, int64_t seg, int64_t per, float* seg_state, const float* seg_decay) {
+  constexpr int kAhead = 8;
+  const int64_t size = (int64_t)a.H * a.P * a.N;
   const int b = (int)(blockIdx.x / per);
-  const int64_t at = (blockIdx.x % per * 256 + threadIdx.x) * 4;
   int64_t t0, t1;
   seq_range(a, b, t0, t1);
   const int64_t n = (t1 - t0 + seg - 1) / seg, first = t0 / seg + b;
   if (n < 2) return;
   const int slot = slot_of(a, b);
-  if (slot < 0 || at >= size) return;
-  const int h = (int)(at / ((int64_t)a.P * a.N));
-  float* p = seg_state + first * size + at;
-  f32x4 S = *(const f32x4*)(a.state + slot * size + at);
-  for (int64_t k = 0; k < n; ++k, p += size) {
-    f32x4 next = S;
-    if (k + 1 < n) {
-      const f32x4 own = *(const f32x4*)p;
-      const float d = seg_decay[(first + k) * a.H + h];
+  if (slot < 0) return;
+  for (int64_t at = (blockIdx.x % per * 256 + threadIdx.x) * 4; at < size; at += per * 1024) {
+    const float* dec = seg_decay + first * a.H + at / ((int64_t)a.P * a.N);
+    float* p = seg_state + first * size + at;
+    f32x4 S = *(const f32x4*)(a.state + slot * size + at);
+    for (int64_t k = 0; k < n; k += kAhead, p += kAhead * size, dec += (int64_t)kAhead * a.H) {
+      f32x4 own[kAhead];
+      float d[kAhead];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) next[e] = __builtin_fmaf(d, S[e], own[e]);
+      for (int i = 0; i < kAhead; ++i)
+        if (k + i + 1 < n) {  // (the last segment leaves its state itself)
+          own[i] = *(const f32x4*)(p + i * size);
+          d[i] = dec[(int64_t)i * a.H];
+        }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (k + i < n) {
+          *(f32x4*)(p + i * size) = S;
+          if (k + i + 1 < n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) S[e] = __builtin_fmaf(d[i], S[e], own[i][e]);
+        }
     }
-    *(f32x4*)p = S;
-    S = next;
   }
 }
 
@@ -496,12 +506,13 @@ template <int N, bool BF>
 hipError_t launch(const ScanArgs& a, void* ws, hipStream_t s) {
   const int64_t seg = segment(a), places = scan_places(a.n_tokens, a.n_seq, seg), wgs = scan_wgs(a.H, a.G, a.P) / a.G;
   const int64_t units = places * a.G, grid = (units + 7) / 8 * 8 * wgs, size = (int64_t)a.H * a.P * N;
-  const int64_t chain = a.n_seq * ((size / 4 + 255) / 256);
-  if (grid > 0x7fffffff || chain > 0x7fffffff) return hipErrorInvalidValue;
+  if (grid > 0x7fffffff) return hipErrorInvalidValue;
   float *st = (float*)ws, *de = st + (ws ? places * size : 0);
   if (split(a)) {
     hipLaunchKernelGGL((scan_chunk_kernel<N, BF, true>), dim3((unsigned)grid), dim3(64 * kW), 0, s, a, seg, places, st, de);
-    hipLaunchKernelGGL(scan_states_kernel, dim3((unsigned)chain), dim3(256), 0, s, a, seg, st, (const float*)de);
+    // (sequences of one segment end at once: 64 of them with 640 workgroups each took 33 us)
+    const int64_t most = (size / 4 + 255) / 256, few = 2048 / a.n_seq, per = few < 1 ? 1 : (few < most ? few : most);
+    hipLaunchKernelGGL(scan_states_kernel, dim3((unsigned)(a.n_seq * per)), dim3(256), 0, s, a, seg, per, st, (const float*)de);
   }
   hipLaunchKernelGGL((scan_chunk_kernel<N, BF, false>), dim3((unsigned)grid), dim3(64 * kW), 0, s, a, seg, places, st, de);
   return hipGetLastError();

@@ -3,6 +3,10 @@
 //   residual_norm  r' = r + scale (rmsnorm(x) pw, or x);  out = rmsnorm(r') w
 // with rmsnorm(v) = v / sqrt(mean(v^2) + eps). Everything is fp32 up to one rounding of each output (out is made of r' before
 // its own rounding). What bounds them: memory, each input read once and each output written once.
+//
+// A row, or a group of one, lies in registers over one wave or a workgroup: a lane has V columns at a time (8 where the width
+// is a multiple of 8, else 2 or 1, at any address). A workgroup goes over many rows with its columns' weights in registers,
+// and the next row is on its way while it reduces this one.
 #include "common.h"
 #include "layer.h"
 
@@ -10,159 +14,290 @@ namespace dfssm {
 
 namespace {
 
-// The sum over the workgroup, the same in every thread, in the same order for every row. slot alternates between
-// calls, so that one barrier is enough.
-template <int WAVES>
-__device__ __forceinline__ float wg_sum(float v, float (*part)[WAVES], int slot) {
-#pragma unroll
-  for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m, 64);
-  if constexpr (WAVES == 1) return v;
+// The sum over W waves, the same in every lane, in the same order for every row. The slot alternates from sum to sum, so that
+// one barrier is enough: a wave that writes a slot again has passed the barrier behind all reads of its former values.
+template <int W>
+__device__ __forceinline__ float row_sum(float v, float (*part)[W], int& slot) {
+  v += dpp_f32<0xB1>(v);
+  v += dpp_f32<0x4E>(v);
+  v += dpp_f32<0x124>(v);
+  v += dpp_f32<0x128>(v);
+  const int x = __builtin_bit_cast(int, v);
+  v = (__builtin_bit_cast(float, __builtin_amdgcn_readlane(x, 0)) + __builtin_bit_cast(float, __builtin_amdgcn_readlane(x, 16))) +
+      (__builtin_bit_cast(float, __builtin_amdgcn_readlane(x, 32)) + __builtin_bit_cast(float, __builtin_amdgcn_readlane(x, 48)));
+  if constexpr (W == 1) return v;
   if ((threadIdx.x & 63) == 0) part[slot][threadIdx.x >> 6] = v;
-  __syncthreads();
+  lds_barrier();
   float s = 0.0f;
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) s += part[slot][w];
+  for (int w = 0; w < W; ++w) s += part[slot][w];
+  slot ^= 1;
   return s;
 }
 
-__device__ __forceinline__ float rms_factor(float ss, int n, float eps) {
-  return __builtin_amdgcn_rsqf(ss / (float)n + eps);  // (1 ulp)
+__device__ __forceinline__ float rms_factor(float ss, float inv_n, float eps) {
+  return __builtin_amdgcn_rsqf(__builtin_fmaf(ss, inv_n, eps));  // (1 ulp)
 }
 
-// A row, or a group of one, over a workgroup: thread i has columns V (i + 64 WAVES k) .., k < K.
-template <int WAVES, int V, int K, bool BF>
-__global__ __launch_bounds__(64 * WAVES) void gated_norm_kernel(GatedNormArgs a) {
-  __shared__ float part[2][WAVES];
-  const int n = a.cols / a.groups;
-  const int64_t row = blockIdx.x / a.groups, c0 = (int64_t)(blockIdx.x % a.groups) * n;
-  const uint16_t *x = a.x + row * a.ld_x + c0, *z = a.gate ? a.gate + row * a.ld_gate + c0 : nullptr;
-  float v[K][V], g[K][V], ss = 0.0f;
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int c = V * (threadIdx.x + 64 * WAVES * k);
-    if (c < n) {
-      load16<V, BF>(x + c, v[k]);
-      if (z) load16<V, BF>(z + c, g[k]);
-    }
-  }
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    if (V * (int)(threadIdx.x + 64 * WAVES * k) >= n) continue;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      g[k][i] = z ? silu_f32(g[k][i]) : 1.0f;
-      if (a.gate_first) v[k][i] *= g[k][i], g[k][i] = 1.0f;
-      ss = __builtin_fmaf(v[k][i], v[k][i], ss);
-    }
-  }
-  const float f = rms_factor(wg_sum<WAVES>(ss, part, 0), n, a.eps);
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int c = V * (threadIdx.x + 64 * WAVES * k);
-    if (c >= n) continue;
-    float y[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) y[i] = v[k][i] * f * a.weight[c0 + c + i] * g[k][i];
-    store16<V, BF>(a.out + row * a.ld_out + c0 + c, y);
-  }
-}
-
-template <int WAVES, int V, int K, bool BF>
-__global__ __launch_bounds__(64 * WAVES) void residual_norm_kernel(ResidualNormArgs a) {
-  __shared__ float part[2][WAVES];
-  const int n = a.cols;
-  const int64_t row = blockIdx.x;
-  float v[K][V], r[K][V], ss = 0.0f;
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int c = V * (threadIdx.x + 64 * WAVES * k);
-    if (c < n) {
-      load16<V, BF>(a.x + row * a.ld_x + c, v[k]);
-      if (a.res32) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) r[k][i] = ((const float*)a.residual)[row * a.ld_res + c + i];
-      } else {
-        load16<V, BF>((const uint16_t*)a.residual + row * a.ld_res + c, r[k]);
-      }
-#pragma unroll
-      for (int i = 0; i < V; ++i) ss = __builtin_fmaf(v[k][i], v[k][i], ss);
-    }
-  }
-  const float f = a.post_weight ? rms_factor(wg_sum<WAVES>(ss, part, 0), n, a.eps) : 1.0f;
-  ss = 0.0f;
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int c = V * (threadIdx.x + 64 * WAVES * k);
-    if (c >= n) continue;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float p = a.post_weight ? v[k][i] * f * a.post_weight[c + i] : v[k][i];
-      r[k][i] = __builtin_fmaf(a.scales ? a.scales[c + i] : a.scale, p, r[k][i]);
-      ss = __builtin_fmaf(r[k][i], r[k][i], ss);
-    }
-  }
-  const float f2 = rms_factor(wg_sum<WAVES>(ss, part, 1), n, a.eps);
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int c = V * (threadIdx.x + 64 * WAVES * k);
-    if (c >= n) continue;
-    float y[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) y[i] = r[k][i] * f2 * a.weight[c + i];
-    store16<V, BF>(a.out + row * a.ld_out + c, y);
-    if (a.res32) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) ((float*)a.residual_out)[row * a.ld_res_out + c + i] = r[k][i];
-    } else {
-      store16<V, BF>((uint16_t*)a.residual_out + row * a.ld_res_out + c, r[k]);
-    }
-  }
-}
-
-// 16384 columns at most: 16 waves of 16 values a lane.
-template <bool BF, class Launch>
-hipError_t by_width(int n, Launch launch) {
-  if (n % 8 == 0) {
-    if (n <= 512) launch.template go<1, 8, 1, BF>();
-    else if (n <= 2048) launch.template go<4, 8, 1, BF>();
-    else if (n <= 8192) launch.template go<8, 8, 2, BF>();
-    else launch.template go<16, 8, 2, BF>();
+template <int V>
+struct Raw {
+  typename Pack16<V>::type v;
+};
+template <int V, bool BF>
+__device__ __forceinline__ void widen(const Raw<V>& r, float (&x)[V]) {
+  if constexpr (V == 1) {
+    x[0] = w2f<BF>(r.v);
   } else {
-    if (n <= 256) launch.template go<1, 1, 4, BF>();
-    else if (n <= 4096) launch.template go<4, 1, 16, BF>();
-    else launch.template go<16, 1, 16, BF>();
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = w2f<BF>(r.v[i]);
   }
-  return hipGetLastError();
 }
+template <int V>
+__device__ __forceinline__ Raw<V> load_raw(const uint16_t* p) {
+  return Raw<V>{*(const typename Pack16<V>::loose*)p};
+}
+template <int V>
+struct Wide {
+  typedef float type __attribute__((ext_vector_type(V)));
+  typedef type loose __attribute__((aligned(4)));
+};
+template <>
+struct Wide<1> {
+  typedef float type, loose;
+};
+template <int V>
+__device__ __forceinline__ void load32(const float* p, float (&x)[V]) {
+  const typename Wide<V>::type v = *(const typename Wide<V>::loose*)p;
+  if constexpr (V == 1) {
+    x[0] = v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = v[i];
+  }
+}
+template <int V>
+__device__ __forceinline__ void store32(float* p, const float (&x)[V]) {
+  typename Wide<V>::type v;
+  if constexpr (V == 1) {
+    v = x[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = x[i];
+  }
+  *(typename Wide<V>::loose*)p = v;
+}
+
+// W waves to a row or group; thread i has columns V (i + 64 W k) .., k < K. Workgroup: 4 rows of a wave each where W is 1.
+template <int W, int V, int K, bool BF>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_kernel(GatedNormArgs a, int64_t workers) {
+  __shared__ float part[2][W];
+  const int i = W == 1 ? threadIdx.x & 63 : threadIdx.x, n = a.cols / a.groups;
+  const int64_t worker = W == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  const int64_t c0 = worker % a.groups * n, step = workers / a.groups;
+  int64_t row = worker / a.groups;
+  if (worker >= workers || row >= a.rows) return;  // (workers is a multiple of the groups)
+  const float inv_n = 1.0f / (float)n;
+  bool in[K];
+  int at[K];
+  float w[K][V];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    in[k] = V * (i + 64 * W * k) < n;
+    at[k] = in[k] ? V * (i + 64 * W * k) : 0;
+  }
+  Raw<V> x[K], z[K];
+  auto load = [&](int64_t r) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      x[k] = load_raw<V>(a.x + r * a.ld_x + c0 + at[k]);
+      if (a.gate) z[k] = load_raw<V>(a.gate + r * a.ld_gate + c0 + at[k]);
+    }
+  };
+  load(row);
+#pragma unroll
+  for (int k = 0; k < K; ++k) load32<V>(a.weight + c0 + at[k], w[k]);
+  int slot = 0;
+  for (;;) {
+    float v[K][V], g[K][V], ss = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      widen<V, BF>(x[k], v[k]);
+      if (a.gate) widen<V, BF>(z[k], g[k]);
+    }
+    const int64_t next = row + step;
+    const bool more = next < a.rows;
+    if (more) load(next);
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        g[k][e] = a.gate ? silu_f32(g[k][e]) : 1.0f;
+        if (a.gate_first) v[k][e] *= g[k][e];
+        ss = __builtin_fmaf(v[k][e], in[k] ? v[k][e] : 0.0f, ss);
+      }
+    const float f = rms_factor(row_sum<W>(ss, part, slot), inv_n, a.eps);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      float y[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        y[e] = v[k][e] * f * w[k][e];
+        if (!a.gate_first) y[e] *= g[k][e];
+      }
+      if (in[k]) store16<V, BF>(a.out + row * a.ld_out + c0 + at[k], y);
+    }
+    if (!more) break;
+    row = next;
+  }
+}
+
+template <int W, int V, int K, bool BF, bool R32>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void residual_norm_kernel(ResidualNormArgs a, int64_t workers) {
+  __shared__ float part[2][W];
+  const int i = W == 1 ? threadIdx.x & 63 : threadIdx.x, n = a.cols;
+  int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  if (row >= a.rows) return;
+  const float inv_n = 1.0f / (float)n;
+  bool in[K];
+  int at[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    in[k] = V * (i + 64 * W * k) < n;
+    at[k] = in[k] ? V * (i + 64 * W * k) : 0;
+  }
+  Raw<V> x[K], rh[R32 ? 1 : K];
+  float r[K][V];
+  auto load = [&](int64_t t) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      x[k] = load_raw<V>(a.x + t * a.ld_x + at[k]);
+      if constexpr (R32) load32<V>((const float*)a.residual + t * a.ld_res + at[k], r[k]);
+      else rh[k] = load_raw<V>((const uint16_t*)a.residual + t * a.ld_res + at[k]);
+    }
+  };
+  load(row);
+  float w[K][V], m[K][V];  // the norm's weight; what rmsnorm(x), or x, is multiplied by
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    load32<V>(a.weight + at[k], w[k]);
+#pragma unroll
+    for (int e = 0; e < V; ++e) m[k][e] = a.scale;
+    if (a.scales) load32<V>(a.scales + at[k], m[k]);
+  }
+  int slot = 0;
+  for (;;) {
+    float v[K][V], s[K][V], ss = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      widen<V, BF>(x[k], v[k]);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        if constexpr (R32) s[k][e] = r[k][e];
+        ss = __builtin_fmaf(v[k][e], in[k] ? v[k][e] : 0.0f, ss);
+      }
+      if constexpr (!R32) widen<V, BF>(rh[k], s[k]);
+    }
+    const int64_t next = row + workers;
+    const bool more = next < a.rows;
+    if (more) load(next);
+    if (a.post_weight) {
+      const float f = rms_factor(row_sum<W>(ss, part, slot), inv_n, a.eps);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        float pw[V];
+        load32<V>(a.post_weight + at[k], pw);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[k][e] = v[k][e] * f * pw[e];
+      }
+    }
+    ss = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        s[k][e] = __builtin_fmaf(m[k][e], v[k][e], s[k][e]);
+        ss = __builtin_fmaf(s[k][e], in[k] ? s[k][e] : 0.0f, ss);
+      }
+    const float f = rms_factor(row_sum<W>(ss, part, slot), inv_n, a.eps);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (!in[k]) continue;
+      float y[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) y[e] = s[k][e] * f * w[k][e];
+      store16<V, BF>(a.out + row * a.ld_out + at[k], y);
+      if constexpr (R32) store32<V>((float*)a.residual_out + row * a.ld_res_out + at[k], s[k]);
+      else store16<V, BF>((uint16_t*)a.residual_out + row * a.ld_res_out + at[k], s[k]);
+    }
+    if (!more) break;
+    row = next;
+  }
+}
+
+// Waves, columns at a time and times that a lane has a row in: 16 values a lane at most, up to 16384 columns.
+template <class Launch>
+void by_width(int n, Launch launch) {
+  if (n % 8 == 0) {
+    if (n <= 512) launch.template go<1, 8, 1>();
+    else if (n <= 1024) launch.template go<1, 8, 2>();
+    else if (n <= 2048) launch.template go<4, 8, 1>();
+    else if (n <= 4096) launch.template go<4, 8, 2>();
+    else if (n <= 8192) launch.template go<8, 8, 2>();
+    else launch.template go<16, 8, 2>();
+  } else if (n % 2 == 0) {
+    if (n <= 512) launch.template go<1, 2, 4>();
+    else if (n <= 4096) launch.template go<4, 2, 8>();
+    else launch.template go<16, 2, 8>();
+  } else {
+    if (n <= 256) launch.template go<1, 1, 4>();
+    else if (n <= 2048) launch.template go<4, 1, 8>();
+    else launch.template go<16, 1, 16>();
+  }
+}
+// Rows or groups at once: as many as are resident, so that each has several in turn.
+template <int W>
+constexpr int64_t kResident = W == 1 ? 256 * 32 : (256 * 32) / W;
 
 struct LaunchGated {
   const GatedNormArgs& a;
   hipStream_t s;
-  template <int WAVES, int V, int K, bool BF>
+  template <int W, int V, int K>
   void go() const {
-    hipLaunchKernelGGL((gated_norm_kernel<WAVES, V, K, BF>), dim3((unsigned)(a.rows * a.groups)), dim3(64 * WAVES), 0, s, a);
+    int64_t rows = kResident<W> / a.groups;  // of a row's groups each
+    rows = rows < 1 ? 1 : (rows < a.rows ? rows : a.rows);
+    const int64_t workers = rows * a.groups;
+    const dim3 grid((unsigned)(W == 1 ? (workers + 3) / 4 : workers)), block(W == 1 ? 256 : 64 * W);
+    if (a.bf16) hipLaunchKernelGGL((gated_norm_kernel<W, V, K, true>), grid, block, 0, s, a, workers);
+    else hipLaunchKernelGGL((gated_norm_kernel<W, V, K, false>), grid, block, 0, s, a, workers);
   }
 };
 struct LaunchResidual {
   const ResidualNormArgs& a;
   hipStream_t s;
-  template <int WAVES, int V, int K, bool BF>
+  template <int W, int V, int K>
   void go() const {
-    hipLaunchKernelGGL((residual_norm_kernel<WAVES, V, K, BF>), dim3((unsigned)a.rows), dim3(64 * WAVES), 0, s, a);
+    const int64_t most = W == 1 ? (kResident<W> + 3) / 4 * 4 : kResident<W>, up = W == 1 ? (a.rows + 3) / 4 * 4 : a.rows;
+    const int64_t workers = most < up ? most : up;
+    const dim3 grid((unsigned)(W == 1 ? workers / 4 : workers)), block(W == 1 ? 256 : 64 * W);
+    if (a.bf16) type<W, V, K, true>(grid, block, workers);
+    else type<W, V, K, false>(grid, block, workers);
+  }
+  template <int W, int V, int K, bool BF>
+  void type(dim3 grid, dim3 block, int64_t workers) const {
+    if (a.res32) hipLaunchKernelGGL((residual_norm_kernel<W, V, K, BF, true>), grid, block, 0, s, a, workers);
+    else hipLaunchKernelGGL((residual_norm_kernel<W, V, K, BF, false>), grid, block, 0, s, a, workers);
   }
 };
 
 }  // namespace
 
 hipError_t launch_gated_norm(const GatedNormArgs& a, hipStream_t s) {
-  if (a.rows * a.groups > 0x7fffffff) return hipErrorInvalidValue;
-  const LaunchGated l{a, s};
-  return a.bf16 ? by_width<true>(a.cols / a.groups, l) : by_width<false>(a.cols / a.groups, l);
+  by_width(a.cols / a.groups, LaunchGated{a, s});
+  return hipGetLastError();
 }
 hipError_t launch_residual_norm(const ResidualNormArgs& a, hipStream_t s) {
-  if (a.rows > 0x7fffffff) return hipErrorInvalidValue;
-  const LaunchResidual l{a, s};
-  return a.bf16 ? by_width<true>(a.cols, l) : by_width<false>(a.cols, l);
+  by_width(a.cols, LaunchResidual{a, s});
+  return hipGetLastError();
 }
 
 }  // namespace dfssm

@@ -102,13 +102,21 @@ __global__ __launch_bounds__(256) void conv_prefill_kernel(ConvArgs a, int64_t t
 #pragma unroll
     for (int k = 0; k < W - 1; ++k) load16<V, BF>(x + (tok - (W - 1) + k) * a.ld_x, win[k]);
   }
-  for (int t = 0; t < len; ++t) {
-    load16<V, BF>(x + (tok + t) * a.ld_x, win[W - 1]);
-    l.apply(win, a.silu, a.out + (tok + t) * a.ld_out + c);
+  // Eight rows on their way together (one by one, a load waits for the store before it).
+  for (int t0 = 0; t0 < len; t0 += 8) {
+    Raw16<V> row[8];
 #pragma unroll
-    for (int k = 0; k < W - 1; ++k)
+    for (int t = 0; t < 8; ++t) row[t] = load_raw<V>(x + (tok + (t0 + t < len ? t0 + t : len - 1)) * a.ld_x);
 #pragma unroll
-      for (int i = 0; i < V; ++i) win[k][i] = win[k + 1][i];
+    for (int t = 0; t < 8; ++t) {
+      if (t0 + t >= len) break;
+      widen<V, BF>(row[t], win[W - 1]);
+      l.apply(win, a.silu, a.out + (tok + t0 + t) * a.ld_out + c);
+#pragma unroll
+      for (int k = 0; k < W - 1; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) win[k][i] = win[k + 1][i];
+    }
   }
 }
 
@@ -168,7 +176,7 @@ hipError_t launch(const ConvArgs& a, bool step, hipStream_t s) {
   return a.W == 2 ? launch<V, 2>(a, step, s) : (a.W == 3 ? launch<V, 3>(a, step, s) : launch<V, 4>(a, step, s));
 }
 hipError_t launch(const ConvArgs& a, bool step, hipStream_t s) {
-  return a.C % 8 == 0 ? launch<8>(a, step, s) : launch<1>(a, step, s);
+  return a.C % 8 == 0 ? launch<8>(a, step, s) : (a.C % 2 == 0 ? launch<2>(a, step, s) : launch<1>(a, step, s));
 }
 
 }  // namespace

@@ -79,15 +79,26 @@ struct Pack16<1> {
   typedef uint16_t type;
   typedef uint16_t loose;
 };
+template <int V>
+struct Raw16 {
+  typename Pack16<V>::type v;
+};
+template <int V>
+__device__ __forceinline__ Raw16<V> load_raw(const uint16_t* p) {
+  return Raw16<V>{*(const typename Pack16<V>::loose*)p};
+}
 template <int V, bool BF>
-__device__ __forceinline__ void load16(const uint16_t* p, float (&x)[V]) {
-  const typename Pack16<V>::type v = *(const typename Pack16<V>::loose*)p;
+__device__ __forceinline__ void widen(const Raw16<V>& r, float (&x)[V]) {
   if constexpr (V == 1) {
-    x[0] = w2f<BF>(v);
+    x[0] = w2f<BF>(r.v);
   } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = w2f<BF>(v[i]);
+    for (int i = 0; i < V; ++i) x[i] = w2f<BF>(r.v[i]);
   }
+}
+template <int V, bool BF>
+__device__ __forceinline__ void load16(const uint16_t* p, float (&x)[V]) {
+  widen<V, BF>(load_raw<V>(p), x);
 }
 template <int V, bool BF>
 __device__ __forceinline__ void store16(uint16_t* p, const float (&x)[V]) {

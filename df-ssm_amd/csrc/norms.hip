@@ -40,23 +40,6 @@ __device__ __forceinline__ float rms_factor(float ss, float inv_n, float eps) {
 }
 
 template <int V>
-struct Raw {
-  typename Pack16<V>::type v;
-};
-template <int V, bool BF>
-__device__ __forceinline__ void widen(const Raw<V>& r, float (&x)[V]) {
-  if constexpr (V == 1) {
-    x[0] = w2f<BF>(r.v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = w2f<BF>(r.v[i]);
-  }
-}
-template <int V>
-__device__ __forceinline__ Raw<V> load_raw(const uint16_t* p) {
-  return Raw<V>{*(const typename Pack16<V>::loose*)p};
-}
-template <int V>
 struct Wide {
   typedef float type __attribute__((ext_vector_type(V)));
   typedef type loose __attribute__((aligned(4)));
@@ -105,7 +88,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void gated_norm_kernel(Gated
     in[k] = V * (i + 64 * W * k) < n;
     at[k] = in[k] ? V * (i + 64 * W * k) : 0;
   }
-  Raw<V> x[K], z[K];
+  Raw16<V> x[K], z[K];
   auto load = [&](int64_t r) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -165,7 +148,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void residual_norm_kernel(Re
     in[k] = V * (i + 64 * W * k) < n;
     at[k] = in[k] ? V * (i + 64 * W * k) : 0;
   }
-  Raw<V> x[K], rh[R32 ? 1 : K];
+  Raw16<V> x[K], rh[R32 ? 1 : K];
   float r[K][V];
   auto load = [&](int64_t t) {
 #pragma unroll

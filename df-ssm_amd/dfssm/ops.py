@@ -378,9 +378,8 @@ def _rows(t: torch.Tensor, width: int):
 def _need_all(dev: int, *named) -> None:
     """Tensors of their types on device dev: (tensor, type, name) each."""
     for t, dt, n in named:
-        _need(t, dt, n)
-    for t, _, n in named:
-        if t.get_device() != dev:
+        if not (isinstance(t, torch.Tensor) and t.dtype is dt and t.get_device() == dev):
+            _need(t, dt, n)
             raise ValueError(f"{n} is on another device than x")
 
 
@@ -393,7 +392,7 @@ def _own_rows(t: torch.Tensor, rows: int, ld: int, p: int, width: int, name: str
 def _apart(t: torch.Tensor, u: torch.Tensor) -> bool:
     """Whether no byte of t (rows, ..) lies among those of u: other memory, or other columns of the same rows."""
     def span(x):
-        n = sum((s - 1) * d for s, d in zip(x.shape, x.stride())) + 1
+        n = x.numel() if x.is_contiguous() else sum((s - 1) * d for s, d in zip(x.shape, x.stride())) + 1
         return x.data_ptr(), x.data_ptr() + n * x.element_size()
     if t.numel() == 0 or u.numel() == 0:
         return True
@@ -487,7 +486,7 @@ def _conv_call(step: bool, x, weight, bias, state, cu_seqlens, slots, silu, out,
     state_out, sp, so = _states(state, state_out, (C, W - 1), dev)
     slots = _slots(slots, state, n_seq, dev)
     if out is None:
-        out = x.new_empty(T, C)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
         ld_out, op = C, out.data_ptr()
     else:
         _need_all(dev, (out, dt, "out"))
@@ -608,7 +607,7 @@ def _scan_call(step: bool, x, dt, A_log, B, C, state, D, dt_bias, cu_seqlens, sl
         _run(dev, L.dfssm_selective_scan_step, args, "selective_scan_step")
         return out
     need = L.dfssm_selective_scan_workspace_bytes(args)
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    ws = x.new_empty(need, dtype=torch.uint8) if need else None
     _run(dev, lambda a, stream: L.dfssm_selective_scan_prefill(a, _C.ptr(ws), stream), args, "selective_scan_prefill")
     return out
 
@@ -665,10 +664,11 @@ def _norm_rows(x):
 
 
 def _norm_weight(t, name: str, cols: int, dev: int):
-    _need_all(dev, (t, torch.float32, name))
+    if not (isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.get_device() == dev):
+        _need_all(dev, (t, torch.float32, name))
     if t.shape != (cols,):
         raise ValueError(f"{name} must be ({cols},)")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _eps(eps) -> float:
@@ -682,7 +682,7 @@ def _norm_out(out, x, name: str, dtype, dev: int, cols: int, inputs):
     """out (a new tensor if None), its rows' distance and address. It may be one of `inputs`, (tensor, distance, address)
     each, and overlaps none otherwise."""
     if out is None:
-        out = x.new_empty(x.shape, dtype=dtype)
+        out = torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format)
         return out, cols, out.data_ptr()
     _need_all(dev, (out, dtype, name))
     if out.shape != x.shape:
@@ -759,9 +759,10 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
     r, ld, p = _rows(r, cols)
     s, ld_s, sp = _rows(_norm_rows(residual), cols)
     inputs = [(r, ld, p), (s, ld_s, sp)]
+    given = out is not None and residual_out is not None
     out, ld_out, op = _norm_out(out, x, "out", dt, dev, cols, inputs)
     residual_out, ld_ro, rop = _norm_out(residual_out, x, "residual_out", rt, dev, cols, inputs)
-    if not _apart(_norm_rows(out), _norm_rows(residual_out)):
+    if given and not _apart(_norm_rows(out), _norm_rows(residual_out)):
         raise ValueError("out and residual_out must not overlap")
     if rows:
         args = _C.Residual(p, sp, _C.ptr(post_weight), _C.ptr(scales), weight.data_ptr(), op, rop, ld, ld_s, ld_out, ld_ro,

@@ -56,6 +56,7 @@ struct Where {
   int64_t first, t0, t1;  // place, tokens of a sequence
   int seq;
 };
+// (C = 0: c tokens, and tokens that fit 31 bits.)
 template <int64_t C, class Args>
 __device__ __forceinline__ void find_seq(const Args& a, int64_t s, Where& q, int64_t c = C) {
   const int lane = threadIdx.x & 63;
@@ -66,7 +67,7 @@ __device__ __forceinline__ void find_seq(const Args& a, int64_t s, Where& q, int
     if (i < lo + n) {
       int64_t t0, t1;
       seq_range(a, i, t0, t1);
-      before = t0 / (C ? C : c) + i <= s;
+      before = (C ? t0 / (C ? C : 1) : (int64_t)((uint32_t)t0 / (uint32_t)c)) + i <= s;
     }
     const int k = __popcll(__ballot(before));  // the starts rise, so the first k lanes (lane 0's always does)
     const int end = lo + n;
@@ -74,19 +75,18 @@ __device__ __forceinline__ void find_seq(const Args& a, int64_t s, Where& q, int
     n = min(step, end - lo);
   }
   seq_range(a, lo, q.t0, q.t1);
-  q.first = q.t0 / (C ? C : c) + lo;
+  q.first = (C ? q.t0 / (C ? C : 1) : (int64_t)((uint32_t)q.t0 / (uint32_t)c)) + lo;
   q.seq = lo;
 }
-// Tokens [tok, tok + the result) of place s; 0 where it holds none. C = 0: c tokens a tile.
+// Tokens [tok, tok + the result) of place s; 0 where it holds none.
 template <int64_t C, class Args>
-__device__ __forceinline__ int64_t tile_of(const Args& a, int64_t s, Where& q, int64_t& tok, int64_t c = C) {
-  const int64_t n = C ? C : c;
-  if (s < q.first || (s - q.first) * n >= q.t1 - q.t0) find_seq<C>(a, s, q, c);
+__device__ __forceinline__ int64_t tile_of(const Args& a, int64_t s, Where& q, int64_t& tok) {
+  if (s < q.first || (s - q.first) * C >= q.t1 - q.t0) find_seq<C>(a, s, q);
   const int64_t i = s - q.first;
   tok = 0;
-  if (i < 0 || i * n >= q.t1 - q.t0) return 0;
-  tok = q.t0 + i * n;
-  return q.t1 - tok < n ? q.t1 - tok : n;
+  if (i < 0 || i * C >= q.t1 - q.t0) return 0;
+  tok = q.t0 + i * C;
+  return q.t1 - tok < C ? q.t1 - tok : C;
 }
 
 }  // namespace dfssm

@@ -6,8 +6,25 @@
 // A workgroup walks the chunks of a sequence, or of a segment of one, with four waves that share B and C in LDS; each has
 // 32 columns p of a head, their state in registers and their x to itself. Products are taken so that results lie in
 // registers as the next product wants its operand: the state as rows n of 32 x 32 results (a lane has a column p), the
-// scores transposed (a lane has a row i of M), y transposed (a lane has a token, and stores 8 bytes of its row).
+// scores transposed (a lane has a row i of M), y transposed (a lane has a token, and 32 bytes of its row to store). What a step of
+// a product needs is loaded from LDS and split beside the step before; B, C, x and dt of the next chunk are on their way.
 // Sequences longer than a segment take three launches: states of the segments from zero, their chain, everything.
+//
+// What bounds it. Per chunk and 32 columns (N = 128, bf16) 116 matrix instructions of 32 clocks and about 1100 others: the
+// scores and M are made by each wave anew, the state is split into parts for C h0, U for the new state. 64 x 512 tokens x 80 heads
+// take 0.41 ms, of which the matrix cores are busy a third and the other pipe nearly half (1.03 GB, 0.21 ms of copying); two waves
+// to a SIMD overlap them little. Sharing M between the two waves of a head (10% fewer matrix instructions, 20% fewer others, a
+// barrier more and 24 KiB) and three waves to a SIMD (168 registers, B not held twice) both came out the same. One sequence of
+// 16411 tokens x 64 heads: 0.07 ms for the segments' states, 0.01 for their chain, 0.16 for the rest (fp16; 0.06 ms of copying). One
+// chunk: 15 us, most of it the code's way into the instruction cache and the loads before the first product.
+//
+// Numbers. States, sums and everything between products are fp32; G is summed in fp64, and its differences taken of float pairs,
+// so that they survive a decay of any size in the same chunk (a_t is held to -1e5). x, B and C are exact operands of the 16-bit
+// matrix cores in their own type. An fp32 factor beside them is a sum of 16-bit parts. Beside bf16: three parts of w_j x_j, which
+// hold 24 bits and go into the state; two of h0 and M, 16 bits, each off by up to 2^-17, which go into y, rounded to 8 bits. Beside
+// fp16: pairs of halves, x 2^s = hi + lo, 22 bits, with s per column of h0 and w x and per row of M so that the largest magnitude
+// lies in [2^14, 2^15); a value below 2^-17 of the largest M of its scale is off by up to 2^-39 M. So a state comes out as from
+// fp32 arithmetic, and y is off by 2^-16 of its terms' magnitudes at most, besides its own rounding. D is on M's diagonal.
 #include "common.h"
 #include "layer.h"
 #include "parts.h"
@@ -101,11 +118,11 @@ __device__ __forceinline__ float uniform(float x) {
 
 template <int N, bool STATE>
 struct ScanLds {
-  f16 B[kC][N];
+  f16 B[2][kC][N];
   f16 C[STATE ? 1 : kC][STATE ? 8 : N];
   f16 x[kW][kC][kScanCols];
   struct {
-    float Gh[kC], Gl[kC], d[kC];         // by tokens: G over log 2, the float nearest (then w) and the rest; d
+    float Gh[kC], Gl[kC], d[kC], w[kC];  // by tokens: G over log 2, the float nearest and the rest; d; w
     float F[32], F16[32];                // d e^{G_32 - G_j}, j < 32; d e^{G_16 - G_j}, j < 16, and of tokens 32 .. 47
     float s[kScanCols];                  // by columns: what undoes the scaling of the state
   } v[kW];
@@ -126,25 +143,91 @@ __device__ __forceinline__ void fetch_shared(f16 (*to)[N], const char* p, int ld
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr)((char*)to + (kW * n + wave) * 1024), 16, off + n * kW * per * ld, 0, 0, 0);
 }
 
+// Places of the launch's numbering of segments (of `seg` tokens; one for an empty sequence). Up to kCounted sequences the
+// segments are counted, so that places are taken without gaps and the dies have equally many: with the numbering of tile_of 64
+// sequences of 512 tokens gave one die nine and another seven. Beyond, they even out by themselves.
+constexpr int kCounted = 512;
+__device__ __forceinline__ int segments_of(int64_t len, int seg) {  // (tokens and segments fit 31 bits)
+  return len > seg ? (int)(((uint32_t)len + seg - 1) / (uint32_t)seg) : 1;
+}
+// The segments of 64 sequences from `from` on, a lane's and those before it; all of them returned.
+__device__ __forceinline__ int count_segments(const ScanArgs& a, int from, int seg, int& own, int& before) {
+  const int lane = threadIdx.x & 63, i = from + lane;
+  own = 0;
+  if (i < a.n_seq) {
+    int64_t t0, t1;
+    seq_range(a, i, t0, t1);
+    own = segments_of(t1 - t0, seg);
+  }
+  int sum = own;
+  sum += __builtin_amdgcn_update_dpp(0, sum, 0x111, 0xf, 0xf, true);  // from 1, 2, 4 and 8 lanes before, in the row of 16
+  sum += __builtin_amdgcn_update_dpp(0, sum, 0x112, 0xf, 0xf, true);
+  sum += __builtin_amdgcn_update_dpp(0, sum, 0x114, 0xf, 0xf, true);
+  sum += __builtin_amdgcn_update_dpp(0, sum, 0x118, 0xf, 0xf, true);
+  sum += __builtin_amdgcn_update_dpp(0, sum, 0x142, 0xa, 0xf, true);  // row 0's last to row 1, 2's to 3; lane 31's to rows 2 and 3
+  sum += __builtin_amdgcn_update_dpp(0, sum, 0x143, 0xc, 0xf, true);
+  before = sum - own;
+  return __builtin_amdgcn_readlane(sum, 63);
+}
+// The sequence of a place; false where there is none.
+__device__ __forceinline__ bool sequence_at(const ScanArgs& a, int place, int seg, Where& q) {
+  if (!a.cu) {
+    const int per = segments_of(a.len, seg);
+    q.seq = (int)((uint32_t)place / (uint32_t)per);
+    q.first = (int64_t)q.seq * per;
+    if (q.seq >= a.n_seq) return false;
+    seq_range(a, q.seq, q.t0, q.t1);
+    return true;
+  }
+  if (a.n_seq > kCounted) {
+    find_seq<0>(a, place, q, seg);
+    return place - q.first < segments_of(q.t1 - q.t0, seg);
+  }
+  int base = 0;
+  for (int from = 0; from < a.n_seq; from += 64) {
+    int own, before;
+    const int all = count_segments(a, from, seg, own, before);
+    if (place < base + all) {
+      const int at = __ffsll((unsigned long long)__ballot(place < base + before + own)) - 1;
+      q.seq = from + at;
+      q.first = base + __builtin_amdgcn_readlane(before, at);
+      seq_range(a, q.seq, q.t0, q.t1);
+      return true;
+    }
+    base += all;
+  }
+  return false;
+}
+// The first place of a sequence.
+__device__ __forceinline__ int64_t first_place(const ScanArgs& a, int b, int seg, int64_t t0) {
+  if (!a.cu) return (int64_t)b * segments_of(a.len, seg);
+  if (a.n_seq > kCounted) return (uint32_t)t0 / (uint32_t)seg + b;
+  int base = 0;
+  for (int from = 0;; from += 64) {
+    int own, before;
+    const int all = count_segments(a, from, seg, own, before);
+    if (b < from + 64) return base + __builtin_amdgcn_readlane(before, b - from);
+    base += all;
+  }
+}
+
 // STATE: the states that a segment leaves from zero, and its decay, of all segments but the last of a sequence.
 template <int N, bool BF, bool STATE>
-__global__ __attribute__((amdgpu_waves_per_eu(3))) __launch_bounds__(64 * kW) void
-scan_chunk_kernel(ScanArgs a, int64_t seg, int64_t places, float* seg_state, float* seg_decay) {
+__global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(64 * kW) void
+scan_chunk_kernel(ScanArgs a, int seg, int places, float* seg_state, float* seg_decay) {
   constexpr int NB = N / 16, NN = N / 32, NU = kParts<BF>, pieces = N / 8;
   __shared__ __align__(16) ScanLds<N, STATE> L;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Workgroups go to the eight dies in turn: all that share a group's B and C run on one, next to its L2.
   const int rep = a.H / a.G, ncb = (a.P + kScanCols - 1) / kScanCols, nwg = (rep * ncb + kW - 1) / kW;
-  const int64_t bx = blockIdx.x, in = bx >> 3, unit = in / nwg * 8 + (bx & 7);
-  if (unit >= places * a.G) return;
-  const int64_t place = unit / a.G;
-  const int gr = (int)(unit % a.G), blk = (int)(in % nwg) * kW + wave;
-  Where q{0, 0, 0, 0};
-  int64_t tok;
-  const int len = (int)tile_of<0>(a, place, q, tok, seg);  // (tokens fit 31 bits)
-  if (len == 0) tok = q.t0;
-  const bool last = tok + len >= q.t1;
-  if (len == 0 && !(!STATE && place == q.first && q.t0 == q.t1)) return;  // (an empty sequence's state is passed on)
+  const uint32_t in = blockIdx.x >> 3, unit = in / (uint32_t)nwg * 8 + (blockIdx.x & 7), place = unit / (uint32_t)a.G;
+  if (place >= (uint32_t)places) return;
+  const int gr = (int)(unit % (uint32_t)a.G), blk = (int)(in % (uint32_t)nwg) * kW + wave;
+  Where q;
+  if (!sequence_at(a, (int)place, seg, q)) return;
+  const int64_t tok = q.t0 + (place - q.first) * seg;
+  const bool last = q.t1 - tok <= seg;
+  const int len = (int)(last ? q.t1 - tok : seg);  // (of an empty sequence 0: its state is passed on)
   if (STATE && last) return;
   const bool active = blk < rep * ncb;
   const int h = gr * rep + (active ? blk / ncb : 0), p0 = active ? blk % ncb * kScanCols : 0;
@@ -203,60 +286,92 @@ scan_chunk_kernel(ScanArgs a, int64_t seg, int64_t places, float* seg_state, flo
     for (int y = 0; y < 2; ++y) t[y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tptr)&X[16 * k + 8 * y + row][at]);
     return __builtin_bit_cast(h8, __builtin_shufflevector(t[0], t[1], 0, 1, 2, 3, 4, 5, 6, 7));
   };
-  float raw = 0.0f;
+  int raw = 0;
   auto fetch_dt = [&](int left) {  // (zero behind the last token)
     const Rsrc r = bytes_of(pt, ld_t, left < kC ? left : kC, dt_size);
     const int at = lane_again() * ld_t;
-    raw = a.dt32 ? __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0))
-                 : w2f<BF>(__builtin_amdgcn_raw_buffer_load_b16(r, at, 0, 0));
-    pt += kC * ld_t;
+    raw = a.dt32 ? (int)__builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0) : (int)__builtin_amdgcn_raw_buffer_load_b16(r, at, 0, 0);
+    pt += (int64_t)kC * ld_t;
   };
-  if (len) fetch_dt(len);
-
-  for (int left = len; left > 0; left -= kC) {
-    const int n = left < kC ? left : kC;
-    {
-      const int lane = lane_again(), row = 512 / N * wave + lane / pieces, piece = ((lane % pieces) ^ swap_of<N>(row)) * 16;
-      fetch_shared<N>(L.B, pb, ld_b, n, wave, row * ld_b + piece);
-      if constexpr (!STATE) fetch_shared<N>(L.C, pc, ld_c, n, wave, row * ld_c + piece);
-      const Rsrc r = bytes_of(px, ld_x, n, xw);
-      const int off = (lane >> 2) * ld_x + (lane & 3) * 16;
-#pragma unroll
-      for (int m = 0; m < 4; ++m)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr)((char*)X + m * 1024), 16, off + m * 16 * ld_x, 0, 0, 0);
-    }
+  const int xo = 16 * ld_x;
+  auto fetch_b = [&](int i, int n) {
+    const int lane = lane_again(), row = 512 / N * wave + lane / pieces, piece = ((lane % pieces) ^ swap_of<N>(row)) * 16;
+    fetch_shared<N>(L.B[i], pb, ld_b, n, wave, row * ld_b + piece);
     pb += kC * ld_b;
-    pc += kC * ld_c;
+  };
+  auto fetch_c = [&](int n) {
+    if constexpr (!STATE) {
+      const int lane = lane_again(), row = 512 / N * wave + lane / pieces, piece = ((lane % pieces) ^ swap_of<N>(row)) * 16;
+      fetch_shared<N>(L.C, pc, ld_c, n, wave, row * ld_c + piece);
+      pc += kC * ld_c;
+    }
+  };
+  auto fetch_x = [&](int n) {
+    const Rsrc r = bytes_of(px, ld_x, n, xw);
+    const int lane = lane_again(), off = (lane >> 2) * ld_x + (lane & 3) * 16;
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr)((char*)X + m * 1024), 16, off + m * xo, 0, 0, 0);
     px += kC * ld_x;
-    // While they are on their way: the time steps; a lane has a token.
-    float dec, wj;
+  };
+  // The time steps; a lane has a token. Returns e^{G_64}.
+  auto times = [&](int n) {
+    const int lane = lane_again();
+    const float dt = a.dt32 ? __builtin_bit_cast(float, raw) : w2f<BF>((uint16_t)raw);
+    const float d = lane < n ? time_step(dt, hp, a.softplus) : 0.0f;
+    float al = d * hp.A;
+    al = al < -1e5f ? -1e5f : al;
+    double G = (double)al * 1.4426950408889634;
+    G += moved<0x111, 0xf>(G);  // running sums: from 1, 2, 4 and 8 lanes before, in the row of 16
+    G += moved<0x112, 0xf>(G);
+    G += moved<0x114, 0xf>(G);
+    G += moved<0x118, 0xf>(G);
+    G += moved<0x142, 0xa>(G);  // row 0's last to row 1, 2's to 3; then lane 31's to rows 2 and 3
+    G += moved<0x143, 0xc>(G);
+    const double GC = readlane_f64(G, 63);
+    V.w[lane] = __builtin_amdgcn_exp2f((float)(GC - G)) * d;
+    if constexpr (!STATE) {
+      V.Gh[lane] = (float)G;
+      V.Gl[lane] = (float)(G - (double)(float)G);
+      V.d[lane] = d;
+      const float f = __builtin_amdgcn_exp2f((float)(readlane_f64(G, 32) - G)) * d;
+      const double G16 = readlane_f64(G, 16), G48 = readlane_f64(G, 48);
+      const float near = __builtin_amdgcn_exp2f((float)((lane < 32 ? G16 : G48) - G)) * d;
+      if (lane < 32) V.F[lane] = f;
+      if (!(lane & 16)) V.F16[(lane & 15) + (lane >> 5) * 16] = near;
+    }
+    return __builtin_amdgcn_exp2f((float)GC);
+  };
+  if (len) {
+    const int n = len < kC ? len : kC;
+    fetch_b(0, n);
+    fetch_c(n);
+    fetch_x(n);
+    fetch_dt(len);
+  }
+  __builtin_amdgcn_s_waitcnt(0);
+
+  // B, x and the time steps of the next chunk are loaded from the start of this one on, C once all waves have their scores; they
+  // are in before a wave stores y, so that no wait is for the stores.
+  int cur = 0;
+  for (int left = len; left > 0; left -= kC, cur ^= 1) {
+    const int n = left < kC ? left : kC, next = left - kC < kC ? left - kC : kC;
+    step_barrier();  // this chunk's B, C and x are in LDS, and the next one's place for B is free
+    const f16 (*LB)[N] = L.B[cur];
+    h8 xf[4];
     {
       const int lane = lane_again();
-      const float d = lane < n ? time_step(raw, hp, a.softplus) : 0.0f;
-      float al = d * hp.A;
-      al = al < -1e5f ? -1e5f : al;
-      double G = (double)al * 1.4426950408889634;
-      G += moved<0x111, 0xf>(G);  // running sums: from 1, 2, 4 and 8 lanes before, in the row of 16
-      G += moved<0x112, 0xf>(G);
-      G += moved<0x114, 0xf>(G);
-      G += moved<0x118, 0xf>(G);
-      G += moved<0x142, 0xa>(G);  // row 0's last to row 1, 2's to 3; then lane 31's to rows 2 and 3
-      G += moved<0x143, 0xc>(G);
-      const double GC = readlane_f64(G, 63);
-      dec = __builtin_amdgcn_exp2f((float)GC);
-      wj = __builtin_amdgcn_exp2f((float)(GC - G)) * d;
-      if constexpr (!STATE) {
-        V.Gh[lane] = (float)G;
-        V.Gl[lane] = (float)(G - (double)(float)G);
-        V.d[lane] = d;
-        const float f = __builtin_amdgcn_exp2f((float)(readlane_f64(G, 32) - G)) * d;
-        const double G16 = readlane_f64(G, 16), G48 = readlane_f64(G, 48);
-        const float near = __builtin_amdgcn_exp2f((float)((lane < 32 ? G16 : G48) - G)) * d;
-        if (lane < 32) V.F[lane] = f;
-        if (!(lane & 16)) V.F16[(lane & 15) + (lane >> 5) * 16] = near;
-      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) xf[k] = x_frag(lane, k);
     }
-    if (left > kC) fetch_dt(left - kC);
+    const float dec = times(n);
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): x is in registers, its place free
+    asm volatile("" ::: "memory");
+    if (next > 0) {
+      fetch_b(cur ^ 1, next);
+      fetch_x(next);
+      fetch_dt(next);
+    }
     float smax = 0.0f, ssc = 1.0f;
     if constexpr (!BF) {
 #pragma unroll
@@ -268,50 +383,64 @@ scan_chunk_kernel(ScanArgs a, int64_t seg, int64_t places, float* seg_state, flo
       ssc = pow2_scale(smax, sinv);
       if (!(threadIdx.x & 32)) V.s[scan_col(lane_again())] = sinv * sfac;
     }
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-    step_barrier();                      // B, C and x are in LDS
     if constexpr (!STATE) {
-      f32x16 y[2], sc[2];  // y by tokens; scores
+      f32x16 y[2], sc[3];  // y by tokens; scores: columns 0 .. 31 of rows 0 .. 31; of rows 32 .. 63; columns 32 .. of those
 #pragma unroll
-      for (int r = 0; r < 16; ++r) y[0][r] = y[1][r] = 0.0f;
+      for (int r = 0; r < 16; ++r) y[0][r] = y[1][r] = sc[0][r] = sc[1][r] = sc[2][r] = 0.0f;
       const int lane = lane_again(), hi = lane >> 5, c = lane & 31;
       auto row_frag = [&](const f16 (*rows)[N], int t, int b) {
         return *(const h8*)&rows[32 * t + c][((2 * b + hi) ^ swap_of<N>(c)) * 8];
       };
+      // What the products of a step need is loaded and split beside those of the step before.
+      {
+        h8 cf[2][2], sp[2][2];
+        auto load = [&](int b) { cf[b & 1][0] = row_frag(L.C, 0, b), cf[b & 1][1] = row_frag(L.C, 1, b); };
+        auto split = [&](int b) {
+          float v[8];
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const h8 c0 = row_frag(L.C, 0, b), c1 = row_frag(L.C, 1, b);
-        float sv[8];
-        h8 s[2];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sv[e] = S[b >> 1][8 * (b & 1) + e];
-        parts8<BF, 2, false>(sv, ssc, s);
-        y[0] = mm32<BF>(s[1], c0, y[0]);
-        y[1] = mm32<BF>(s[1], c1, y[1]);
-        y[0] = mm32<BF>(s[0], c0, y[0]);
-        y[1] = mm32<BF>(s[0], c1, y[1]);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      // M: a lane has row 32 t + c, columns 8 q + 4 hi + e of each block of 32. Of a block on the diagonal it has 8 exponentials, of
-      // its own 16 columns; the other 16 are before its row, and e^{G_i - G_j} is taken apart at column 16, or behind it.
-      const Rsrc orow = bytes_of(po, ld_o, n, xw);
-      const bool own = c & 16;
-      const int lim = (c & 15) - 4 * hi;
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        f32x16& D = sc[t ? 1 : 0];
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int u = 0; u <= t; ++u)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) sc[u][r] = 0.0f;
+          for (int e = 0; e < 8; ++e) v[e] = S[b >> 1][8 * (b & 1) + e];
+          parts8<BF, 2, false>(v, ssc, sp[b & 1]);
+        };
+        load(0);
+        split(0);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-          const h8 ct = row_frag(L.C, t, b);
+          __builtin_amdgcn_sched_barrier(0);
+          if (b + 1 < NB) load(b + 1);
 #pragma unroll
-          for (int u = 0; u <= t; ++u) sc[u] = mm32<BF>(row_frag(L.B, u, b), ct, sc[u]);
+          for (int p = 1; p >= 0; --p)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) y[t] = mm32<BF>(sp[b & 1][p], cf[b & 1][t], y[t]);
+          if (b + 1 < NB) split(b + 1);
         }
-        __builtin_amdgcn_sched_barrier(0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      {
+        h8 cf[2][2], bf[2][2];
+        auto load = [&](int b) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) cf[b & 1][t] = row_frag(L.C, t, b), bf[b & 1][t] = row_frag(LB, t, b);
+        };
+        load(0);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          __builtin_amdgcn_sched_barrier(0);
+          if (b + 1 < NB) load(b + 1);
+          sc[0] = mm32<BF>(bf[b & 1][0], cf[b & 1][0], sc[0]);
+          sc[1] = mm32<BF>(bf[b & 1][0], cf[b & 1][1], sc[1]);
+          sc[2] = mm32<BF>(bf[b & 1][1], cf[b & 1][1], sc[2]);
+        }
+      }
+      step_barrier();  // C is free
+      if (next > 0) fetch_c(next);
+      // M: a lane has row 32 t + c, columns 8 q + 4 hi + e of each block of 32. Of a block on the diagonal it has 8 exponentials, of
+      // its own 16 columns; the other 16 are before its row, and e^{G_i - G_j} is taken apart at column 16, or behind it.
+      const bool own = c & 16;
+      const int lim = (c & 15) - 4 * hi;
+      float pinv[2] = {1.0f, 1.0f};
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        f32x16& D = sc[2 * t];
         const float Gi = V.Gh[32 * t + c], gi = V.Gl[32 * t + c];
         if (t) {
           const float ei = __builtin_amdgcn_exp2f((Gi - V.Gh[32]) + (gi - V.Gl[32]));
@@ -319,14 +448,12 @@ scan_chunk_kernel(ScanArgs a, int64_t seg, int64_t places, float* seg_state, flo
           for (int q4 = 0; q4 < 4; ++q4) {
             const f32x4 F = *(const f32x4*)&V.F[8 * q4 + 4 * hi];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sc[0][4 * q4 + e] = (sc[0][4 * q4 + e] * ei) * F[e];
+            for (int e = 0; e < 4; ++e) sc[1][4 * q4 + e] = (sc[1][4 * q4 + e] * ei) * F[e];
           }
         }
-        __builtin_amdgcn_sched_barrier(0);
         const float ei = __builtin_amdgcn_exp2f((Gi - V.Gh[32 * t + 16]) + (gi - V.Gl[32 * t + 16]));
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
-          __builtin_amdgcn_sched_barrier(0);
           const int j0 = 8 * z + 4 * hi;
           const f32x4 jh = *(const f32x4*)&V.Gh[32 * t + (c & 16) + j0], jl = *(const f32x4*)&V.Gl[32 * t + (c & 16) + j0];
           const f32x4 dj = *(const f32x4*)&V.d[32 * t + (c & 16) + j0], F = *(const f32x4*)&V.F16[16 * t + j0];
@@ -334,22 +461,22 @@ scan_chunk_kernel(ScanArgs a, int64_t seg, int64_t places, float* seg_state, flo
           for (int e = 0; e < 4; ++e) {  // (right of the diagonal the exponential may be infinite: not used)
             const int k = 4 * z + e;
             const float ex = __builtin_amdgcn_exp2f((Gi - jh[e]) + (gi - jl[e])) * dj[e];
-            float v = __builtin_fmaf(own ? D[8 + k] : D[k], ex, 8 * z + e == lim ? hp.D : 0.0f);
+            const float near = D[k], far = D[8 + k];
+            float v = __builtin_fmaf(own ? far : near, ex, 8 * z + e == lim ? hp.D : 0.0f);
             v = 8 * z + e <= lim ? v : 0.0f;
-            D[k] = own ? D[k] * (ei * F[e]) : v;
+            D[k] = own ? near * (ei * F[e]) : v;
             D[8 + k] = own ? v : 0.0f;
           }
         }
-        __builtin_amdgcn_sched_barrier(0);
         // y of the state comes into M's scale (at most 2^40: what is lost of smaller M is below 2^-60)
-        float ys = __builtin_amdgcn_exp2f(Gi + gi), msc = 1.0f, pinv = 1.0f;
+        float ys = __builtin_amdgcn_exp2f(Gi + gi), msc = 1.0f;
         if constexpr (!BF) {
           float top = 0x1p-26f;
 #pragma unroll
-          for (int u = 0; u <= t; ++u)
+          for (int u = 2 * t; u >= t; --u)
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = __builtin_elementwise_maximum(top, __builtin_fabsf(sc[u][r]));
-          msc = pow2_scale(max_halves(top), pinv);
+          msc = pow2_scale(max_halves(top), pinv[t]);
           ys *= msc;
         }
 #pragma unroll
@@ -363,21 +490,24 @@ scan_chunk_kernel(ScanArgs a, int64_t seg, int64_t places, float* seg_state, flo
           float v[8];
           h8 m[2];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = sc[k >> 1][8 * (k & 1) + e];
-          __builtin_amdgcn_sched_barrier(0);
+          for (int e = 0; e < 8; ++e) v[e] = sc[(k >> 1) + t][8 * (k & 1) + e];
           parts8<BF, 2>(v, msc, m);
-          const h8 x = x_frag(lane, k);
 #pragma unroll
-          for (int p = 1; p >= 0; --p) y[t] = mm32<BF>(x, m[p], y[t]);
+          for (int p = 1; p >= 0; --p) y[t] = mm32<BF>(xf[k], m[p], y[t]);
         }
-        if (active && (hi == 0 || wide))
+      }
+      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+      if (active && (hi == 0 || wide)) {
+        const Rsrc orow = bytes_of(po, ld_o, n, xw);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int r = 0; r < 16; r += 8) {
             uint32_t o[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               o[e] = BF ? pack2<BF>(y[t][r + 2 * e], y[t][r + 2 * e + 1])
-                        : pack2<BF>(y[t][r + 2 * e] * pinv, y[t][r + 2 * e + 1] * pinv);
+                        : pack2<BF>(y[t][r + 2 * e] * pinv[t], y[t][r + 2 * e + 1] * pinv[t]);
             __builtin_amdgcn_raw_buffer_store_b128(u32x4{o[0], o[1], o[2], o[3]}, orow, (32 * t + c) * ld_o + 32 * hi + 2 * r, 0, 0);
           }
       }
@@ -388,17 +518,14 @@ scan_chunk_kernel(ScanArgs a, int64_t seg, int64_t places, float* seg_state, flo
     __builtin_amdgcn_sched_barrier(0);
     // the new state
     const int lane = lane_again(), hi = lane >> 5, l = lane & 15;
-    V.Gh[lane] = wj;
-    wave_sync();
     float keep = dec, usc = 1.0f;
     auto weighted = [&](int k, float (&u)[8]) {
-      const h8 x = x_frag(lane, k);
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-        const f32x4 w = *(const f32x4*)&V.Gh[16 * k + 8 * y + 4 * hi];
+        const f32x4 w = *(const f32x4*)&V.w[16 * k + 8 * y + 4 * hi];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const f16 v = x[4 * y + e];  // (a bit cast of the element itself takes the vector's first one)
+          const f16 v = xf[k][4 * y + e];  // (a bit cast of the element itself takes the vector's first one)
           u[4 * y + e] = w2f<BF>(__builtin_bit_cast(uint16_t, v)) * w[e];
         }
       }
@@ -419,28 +546,40 @@ scan_chunk_kernel(ScanArgs a, int64_t seg, int64_t places, float* seg_state, flo
     for (int t = 0; t < NN; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r) S[t][r] *= keep;
+    {
+      h8 up[2][NU], bt[2][NN];
+      auto load = [&](int k) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      __builtin_amdgcn_sched_barrier(0);
-      if constexpr (BF) weighted(k, u[k]);
-      h8 up[NU];
-      parts8<BF, NU>(u[k], usc, up);
+        for (int t = 0; t < NN; ++t) {
+          // rows of B^T: result row 4 m + e of 16 is n = 4 m' + e, m' being m with its two bits exchanged
+          s4 b[2];
 #pragma unroll
-      for (int t = 0; t < NN; ++t) {
-        // rows of B^T: result row 4 m + e of 16 is n = 4 m' + e, m' being m with its two bits exchanged
-        s4 b[2];
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const int row = 16 * k + 8 * y + 4 * hi + (l >> 2), m = (l & 3) >> 1 | (l & 1) << 1;
-          const int piece = (4 * t + 2 * ((lane >> 4) & 1) + (m >> 1)) ^ swap_of<N>(row & 15);
-          b[y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tptr)&L.B[row][piece * 8 + 4 * (m & 1)]);
+          for (int y = 0; y < 2; ++y) {
+            const int row = 16 * k + 8 * y + 4 * hi + (l >> 2), m = (l & 3) >> 1 | (l & 1) << 1;
+            const int piece = (4 * t + 2 * ((lane >> 4) & 1) + (m >> 1)) ^ swap_of<N>(row & 15);
+            b[y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tptr)&LB[row][piece * 8 + 4 * (m & 1)]);
+          }
+          bt[k & 1][t] = __builtin_bit_cast(h8, __builtin_shufflevector(b[0], b[1], 0, 1, 2, 3, 4, 5, 6, 7));
         }
-        const h8 bt = __builtin_bit_cast(h8, __builtin_shufflevector(b[0], b[1], 0, 1, 2, 3, 4, 5, 6, 7));
+      };
+      auto split = [&](int k) {
+        if constexpr (BF) weighted(k, u[k]);
+        parts8<BF, NU>(u[k], usc, up[k & 1]);
+      };
+      load(0);
+      split(0);
 #pragma unroll
-        for (int p = NU - 1; p >= 0; --p) S[t] = mm32<BF>(bt, up[p], S[t]);
+      for (int k = 0; k < 4; ++k) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (k < 3) load(k + 1);
+#pragma unroll
+        for (int p = NU - 1; p >= 0; --p)
+#pragma unroll
+          for (int t = 0; t < NN; ++t) S[t] = mm32<BF>(bt[k & 1][t], up[k & 1][p], S[t]);
+        if (k < 3) split(k + 1);
       }
     }
-    step_barrier();  // B, C and x are free
+    if constexpr (STATE) __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
   }
 
   const int lane = lane_again();
@@ -461,21 +600,22 @@ scan_chunk_kernel(ScanArgs a, int64_t seg, int64_t places, float* seg_state, flo
 // The states before each segment of a sequence of several, in place of those that its segments leave from zero. A thread
 // has four values of a head at a time, and those of eight segments on their way together (one by one, 16 segments of 64 heads
 // took 13 us); `per` workgroups to a sequence.
-__global__ __launch_bounds__(256) void scan_states_kernel(ScanArgs a, int64_t seg, int64_t per, float* seg_state, const float* seg_decay) {
+__global__ __launch_bounds__(256) void scan_states_kernel(ScanArgs a, int seg, int64_t per, float* seg_state, const float* seg_decay) {
   constexpr int kAhead = 8;
   const int64_t size = (int64_t)a.H * a.P * a.N;
   const int b = (int)(blockIdx.x / per);
   int64_t t0, t1;
   seq_range(a, b, t0, t1);
-  const int64_t n = (t1 - t0 + seg - 1) / seg, first = t0 / seg + b;
+  const int n = segments_of(t1 - t0, seg);
   if (n < 2) return;
+  const int64_t first = first_place(a, b, seg, t0);
   const int slot = slot_of(a, b);
   if (slot < 0) return;
   for (int64_t at = (blockIdx.x % per * 256 + threadIdx.x) * 4; at < size; at += per * 1024) {
     const float* dec = seg_decay + first * a.H + at / ((int64_t)a.P * a.N);
     float* p = seg_state + first * size + at;
     f32x4 S = *(const f32x4*)(a.state + slot * size + at);
-    for (int64_t k = 0; k < n; k += kAhead, p += kAhead * size, dec += (int64_t)kAhead * a.H) {
+    for (int k = 0; k < n; k += kAhead, p += kAhead * size, dec += (int64_t)kAhead * a.H) {
       f32x4 own[kAhead];
       float d[kAhead];
 #pragma unroll
@@ -498,7 +638,7 @@ __global__ __launch_bounds__(256) void scan_states_kernel(ScanArgs a, int64_t se
 
 int64_t segment(const ScanArgs& a) {
   const int64_t longest = a.cu ? a.n_tokens : a.len, seg = scan_segment(a.n_tokens, a.n_seq, scan_wgs(a.H, a.G, a.P));
-  return seg >= longest ? (longest + kC - 1) / kC * kC + kC : seg;  // (one segment each, and a place more than that: see places)
+  return seg >= longest ? (longest + kC) / kC * kC : seg;
 }
 bool split(const ScanArgs& a) { return segment(a) < (a.cu ? a.n_tokens : a.len); }
 
@@ -506,15 +646,15 @@ template <int N, bool BF>
 hipError_t launch(const ScanArgs& a, void* ws, hipStream_t s) {
   const int64_t seg = segment(a), places = scan_places(a.n_tokens, a.n_seq, seg), wgs = scan_wgs(a.H, a.G, a.P) / a.G;
   const int64_t units = places * a.G, grid = (units + 7) / 8 * 8 * wgs, size = (int64_t)a.H * a.P * N;
-  if (grid > 0x7fffffff) return hipErrorInvalidValue;
+  if (grid > 0x7fffffff || seg > 0x7fffffff) return hipErrorInvalidValue;
   float *st = (float*)ws, *de = st + (ws ? places * size : 0);
   if (split(a)) {
-    hipLaunchKernelGGL((scan_chunk_kernel<N, BF, true>), dim3((unsigned)grid), dim3(64 * kW), 0, s, a, seg, places, st, de);
+    hipLaunchKernelGGL((scan_chunk_kernel<N, BF, true>), dim3((unsigned)grid), dim3(64 * kW), 0, s, a, (int)seg, (int)places, st, de);
     // (sequences of one segment end at once: 64 of them with 640 workgroups each took 33 us)
     const int64_t most = (size / 4 + 255) / 256, few = 2048 / a.n_seq, per = few < 1 ? 1 : (few < most ? few : most);
-    hipLaunchKernelGGL(scan_states_kernel, dim3((unsigned)(a.n_seq * per)), dim3(256), 0, s, a, seg, per, st, (const float*)de);
+    hipLaunchKernelGGL(scan_states_kernel, dim3((unsigned)(a.n_seq * per)), dim3(256), 0, s, a, (int)seg, per, st, (const float*)de);
   }
-  hipLaunchKernelGGL((scan_chunk_kernel<N, BF, false>), dim3((unsigned)grid), dim3(64 * kW), 0, s, a, seg, places, st, de);
+  hipLaunchKernelGGL((scan_chunk_kernel<N, BF, false>), dim3((unsigned)grid), dim3(64 * kW), 0, s, a, (int)seg, (int)places, st, de);
   return hipGetLastError();
 }
 

@@ -600,7 +600,7 @@ scan_chunk_kernel(ScanArgs a, int seg, int places, float* seg_state, float* seg_
 // The states before each segment of a sequence of several, in place of those that its segments leave from zero. A thread
 // has four values of a head at a time, and those of eight segments on their way together (one by one, 16 segments of 64 heads
 // took 13 us); `per` workgroups to a sequence.
-__global__ __launch_bounds__(256) void scan_states_kernel(ScanArgs a, int seg, int64_t per, float* seg_state, const float* seg_decay) {
+__global__ __launch_bounds__(256) void scan_states_kernel(ScanArgs a, int seg, int places, int64_t per, float* seg_state, const float* seg_decay) {
   constexpr int kAhead = 8;
   const int64_t size = (int64_t)a.H * a.P * a.N;
   const int b = (int)(blockIdx.x / per);
@@ -609,6 +609,7 @@ __global__ __launch_bounds__(256) void scan_states_kernel(ScanArgs a, int seg, i
   const int n = segments_of(t1 - t0, seg);
   if (n < 2) return;
   const int64_t first = first_place(a, b, seg, t0);
+  if (first + n > places) return;  // (only where offsets fall)
   const int slot = slot_of(a, b);
   if (slot < 0) return;
   for (int64_t at = (blockIdx.x % per * 256 + threadIdx.x) * 4; at < size; at += per * 1024) {
@@ -652,7 +653,7 @@ hipError_t launch(const ScanArgs& a, void* ws, hipStream_t s) {
     hipLaunchKernelGGL((scan_chunk_kernel<N, BF, true>), dim3((unsigned)grid), dim3(64 * kW), 0, s, a, (int)seg, (int)places, st, de);
     // (sequences of one segment end at once: 64 of them with 640 workgroups each took 33 us)
     const int64_t most = (size / 4 + 255) / 256, few = 2048 / a.n_seq, per = few < 1 ? 1 : (few < most ? few : most);
-    hipLaunchKernelGGL(scan_states_kernel, dim3((unsigned)(a.n_seq * per)), dim3(256), 0, s, a, (int)seg, per, st, (const float*)de);
+    hipLaunchKernelGGL(scan_states_kernel, dim3((unsigned)(a.n_seq * per)), dim3(256), 0, s, a, (int)seg, (int)places, per, st, (const float*)de);
   }
   hipLaunchKernelGGL((scan_chunk_kernel<N, BF, false>), dim3((unsigned)grid), dim3(64 * kW), 0, s, a, (int)seg, (int)places, st, de);
   return hipGetLastError();

@@ -148,3 +148,30 @@ def test_values_that_are_not_finite_stay_in_their_window():
     bad[39, 5] = True
     assert torch.equal(out.cpu()[:, [3, 7]].isnan(), bad[:, [3, 7]])
     assert out.cpu()[~bad].isfinite().all()
+
+
+def test_rows_past_32_bits():
+    C, W, T = 8192, 4, (1 << 18) + 40
+    x = torch.zeros(T, C, dtype=torch.float16, device=DEV)
+    tail = make([40], C, W, torch.float16)
+    x[-40:] = tail["x"].to(DEV)
+    g = gpu(tail)
+    state = torch.zeros(2, C, W - 1, dtype=torch.float16, device=DEV)
+    state[1] = g["state"][0]
+    cu = torch.tensor([0, T - 40, T], dtype=torch.int32, device=DEV)
+    out = ops.causal_conv_prefill(x, g["weight"], g["bias"], state, cu_seqlens=cu)
+    ref, mag, after = lm.conv(tail["x"], tail["weight"], tail["bias"], tail["state"], [40])
+    check(out[-40:], ref, mag, True, "out")
+    assert torch.equal(state[1].cpu(), after[0])
+
+
+@pytest.mark.parametrize("offsets", [[0, 300, 0, 300], [-5, 400, 1 << 30, 7], [300, 200, 100, 0]])
+def test_bad_offsets_stay_inside(offsets):
+    T, C = 300, 40
+    x = gpu(make([T], C, 4, torch.float16, pool=3))
+    around = torch.full((3 * T, C), 5.0, dtype=torch.float16, device=DEV)
+    states = torch.full((9, C, 3), 7.0, dtype=torch.float16, device=DEV)
+    ops.causal_conv_prefill(x["x"], x["weight"], x["bias"], states[3:6], out=around[T:2 * T],
+                            cu_seqlens=torch.tensor(offsets, dtype=torch.int32, device=DEV))
+    torch.cuda.synchronize()
+    assert (around[:T] == 5).all() and (around[2 * T:] == 5).all() and (states[:3] == 7).all() and (states[6:] == 7).all()

@@ -106,3 +106,25 @@ def test_rows_none_zero_and_not_finite():
     out, r = ops.residual_norm(x, x, w, post_weight=w)
     assert out[1].isnan().all() and out[[0, 2, 3]].isfinite().all() and r[[0, 2, 3]].isfinite().all()
     assert ops.gated_norm(x, x, w)[1].isnan().all()
+
+
+def test_rows_past_32_bits_and_many_in_turn():
+    """2.2 * 10^9 values; and more rows than are resident at once, in several turns, in place."""
+    cols, rows = 8192, (1 << 18) + 100
+    gen = torch.Generator().manual_seed(5)
+    w = 1 + 0.2 * rnd(gen, cols)
+    x = torch.zeros(rows, cols, dtype=torch.float16, device=DEV)
+    tail = rnd(gen, 3, cols).half()
+    x[-3:] = tail.to(DEV)
+    check(ops.gated_norm(x, x, w.to(DEV), out=x)[-3:], lm.gated(tail, tail, w), 128 * 2.0 ** -24, "gated")
+    x[-3:] = tail.to(DEV)
+    out, r = ops.residual_norm(x, x, w.to(DEV), scale=0.5, out=x)
+    ref, new, mag = lm.residual(tail, tail, w, None, 0.5)
+    check(out[-3:], ref, 2.0 ** -17, "out")
+    check(r[-3:], new, 64 * 2.0 ** -24, "residual", mag)
+    for n in (64, 65, 1000):
+        x, z = rnd(gen, 20000, n).half(), rnd(gen, 20000, n).half()
+        wn = 1 + 0.2 * rnd(gen, n)
+        check(ops.gated_norm(x.to(DEV), z.to(DEV), wn.to(DEV)), lm.gated(x, z, wn), 128 * 2.0 ** -24, f"{n}")
+        out, r = ops.residual_norm(x.to(DEV), z.to(DEV), wn.to(DEV), post_weight=wn.to(DEV))
+        check(r, lm.residual(x, z, wn, wn)[1], 64 * 2.0 ** -24, f"{n}", lm.residual(x, z, wn, wn)[2])

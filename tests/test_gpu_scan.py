@@ -186,3 +186,61 @@ def test_repeats_are_equal():
         out = prefill(g, lens, state=s)
         first = first or (out, s)
         assert torch.equal(out, first[0]) and torch.equal(s, first[1])
+
+
+@pytest.mark.parametrize("n", [63, 64, 65, 511, 512, 513, 700])
+def test_many_sequences(n):
+    """Both numberings of the segments (counted up to 512 sequences), with empty and long ones among them."""
+    gen = torch.Generator().manual_seed(n)
+    lens = torch.randint(0, 4, (n,), generator=gen).tolist()
+    lens[n // 2], lens[n - 1], lens[1] = 900, 300, 70
+    x = make(lens, 2, 1, 32, 64, torch.bfloat16)
+    ref = reference(x, lens)
+    g = gpu(x)
+    check(prefill(g, lens), g["state"], ref)
+
+
+@pytest.mark.parametrize("offsets", [[0, 3000, 0, 3000, 0, 3000], [-5, 4000, 1 << 30, 0, 64, 63], [3000, 2000, 1000, 0, 0, 0]])
+def test_bad_offsets_stay_inside(offsets):
+    """Offsets that fall or lie outside: results are not specified, but nothing outside the tensors is written."""
+    T, H, P, N = 3000, 4, 32, 64
+    x = gpu(make([T], H, 1, P, N, torch.float16, pool=8))
+    around = torch.full((3 * T, H, P), 5.0, dtype=torch.float16, device=DEV)
+    states = torch.full((24, H, P, N), 7.0, device=DEV)
+    states[8:16] = x["state"]
+    cu = torch.tensor(offsets, dtype=torch.int32, device=DEV)
+    for _ in range(2):
+        ops.selective_scan_prefill(x["x"], x["dt"], x["A_log"], x["B"], x["C"], states[8:16], D=x["D"], dt_bias=x["dt_bias"],
+                                   cu_seqlens=cu, out=around[T:2 * T])
+    torch.cuda.synchronize()
+    assert (around[:T] == 5).all() and (around[2 * T:] == 5).all() and (states[:8] == 7).all() and (states[16:] == 7).all()
+
+
+def test_states_past_32_bits():
+    H, P, N = 64, 64, 128
+    pool = 4200                                                                 # 2.2 * 10^9 values
+    state = torch.zeros(pool, H, P, N, device=DEV)
+    for lens in ([70], [5]):
+        x = make(lens, H, 1, P, N, torch.float16)
+        state[pool - 1] = x["state"][0].to(DEV)
+        g = gpu(x)
+        slots = torch.tensor([pool - 1], dtype=torch.int32, device=DEV)
+        out = prefill(g, lens, state=state, slots=slots)
+        check(out, state[pool - 1:], reference(x, lens))
+    assert not state[:pool - 1].any()
+
+
+def test_a_value_that_is_not_finite():
+    """It stays in its sequence, its column of x or its head, and the tokens from 63 before it on; NaN comes back as NaN."""
+    lens = [200, 100]
+    x = make(lens, 2, 1, 64, 64, torch.bfloat16)
+    x["x"][150, 0, 5] = float("nan")
+    x["dt"][230, 1] = float("nan")
+    g = gpu(x)
+    out = prefill(g, lens).cpu()
+    bad = out.isnan()
+    assert bad[150:200, 0, 5].all() and bad[230:, 1].all()
+    bad[87:200, 0, 5] = False
+    bad[200:, 1] = False
+    assert not bad.any() and not g["state"].cpu()[0, 1].isnan().any() and g["state"].cpu()[1, 1].isnan().all()
+    assert g["state"].cpu()[0, 0, 5].isnan().all() and not g["state"].cpu()[0, 0, 6].isnan().any()

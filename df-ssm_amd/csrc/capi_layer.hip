@@ -94,8 +94,12 @@ ScanArgs scan_args(const dfssm_scan* d) {
 }
 
 // Prompts that run token by token: too few tokens for a chunk's fixed work. The lengths behind cu_seqlens are on the device,
-// so the rule there goes by all tokens, which any one sequence may have.
-constexpr int kTokenPath = 12;
+// so the rule there goes by all tokens, which any one sequence may have. Sequences of 8 | 12 | 16 tokens, token by token and in
+// chunks, kernels in a replayed graph, fp16 (one sequence of one group spread over the dies since, 2 us less in chunks):
+//   64 heads of 64 x 128   one sequence 9.2, 14.4 | 12.1, 14.3 | 15.0, 14.0 us   32: 45, 39 | 59, 40 | 71, 38
+//   40 heads of 128 x 128, 5 groups     9.3, 11.8 | 12.3, 11.9 | 15.3, 11.9          55, 49 | 72, 49 | 96, 49
+//   6 heads of 256 x 64                 8.2, 8.8 | 10.7, 8.8 | 13.1, 8.9             17, 14 | 22, 14 | 27, 14
+constexpr int kTokenPath = 8;
 bool by_tokens(const ScanArgs& a) { return (a.cu ? a.n_tokens : a.len) <= kTokenPath; }
 
 // Rows of a norm.

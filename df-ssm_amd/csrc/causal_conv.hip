@@ -2,7 +2,10 @@
 //   y_t = f(b + sum_{k < W} w_k x_{t - W + 1 + k}),  f(y) = y or y / (1 + e^-y),  W = 2 .. 4 taps per channel
 // where the x before a sequence are its state's, which is left as the last W - 1 of state and sequence together.
 // Sums are fp32, in the order b, w_0 x, .. w_{W-1} x; y is rounded once. States are copied, never rounded.
-// What bounds it: memory; 2 W + 6 operations an element.
+// What bounds it: memory. 64 x 512 tokens of 5376 channels (bf16, 709 MB) 0.149 ms, 4.8 TB/s, where a copy reaches 4.9; twelve
+// ragged sequences of 4352 channels (fp16, 134 MB) 31 us. A wave reads 1 KiB of a row at a time, eight rows on their way
+// together (one by one, a load waits for the store before it: 0.160 ms); a tile's three rows before it come out of L2. Few rows:
+// the launch; one of 4352 channels 4.0 us in a replayed graph.
 #include "common.h"
 #include "layer.h"
 
@@ -10,7 +13,7 @@ namespace dfssm {
 
 namespace {
 
-constexpr int kRows = 16;  // tokens of a tile
+constexpr int kRows = 16;  // tokens of a tile, which reads W - 1 rows more
 
 // A lane's V channels from c on: their weights, and rows of x and of the state.
 template <int V, int W, bool BF>
@@ -175,6 +178,7 @@ template <int V>
 hipError_t launch(const ConvArgs& a, bool step, hipStream_t s) {
   return a.W == 2 ? launch<V, 2>(a, step, s) : (a.W == 3 ? launch<V, 3>(a, step, s) : launch<V, 4>(a, step, s));
 }
+// Channels to a lane: those of 16 bytes where a row has whole ones (at any address), else a pair, else one.
 hipError_t launch(const ConvArgs& a, bool step, hipStream_t s) {
   return a.C % 8 == 0 ? launch<8>(a, step, s) : (a.C % 2 == 0 ? launch<2>(a, step, s) : launch<1>(a, step, s));
 }

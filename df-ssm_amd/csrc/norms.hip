@@ -6,7 +6,9 @@
 //
 // A row, or a group of one, lies in registers over one wave or a workgroup: a lane has V columns at a time (8 where the width
 // is a multiple of 8, else 2 or 1, at any address). A workgroup goes over many rows with its columns' weights in registers,
-// and the next row is on its way while it reduces this one.
+// and the next row is on its way while it reduces this one. 32768 rows of 5120, eight groups (bf16, 1.01 GB), 0.206 ms; 32768 of 2560
+// with a residual in 32 bits (1.01 GB) 0.200 ms: 4.9 and 5.0 TB/s, what a copy reaches. (A row to a workgroup at a time, weights
+// read for each: 0.366 and 0.399 ms.) Few rows: the launch; one of 4096 3.6 us, 32 of 2048 3.3 us in a replayed graph.
 #include "common.h"
 #include "layer.h"
 

@@ -2,7 +2,8 @@
 //
 // Per head, with the state h (P x N) fp32 and the head's group of B and C (N):
 //   d_t = max(softplus(dt_t + dt_bias), 0);  h_t = e^{-d_t e^{A_log}} h_{t-1} + (d_t x_t) B_t^T;  y_t = h_t C_t + D x_t
-// All of it in fp32; y is rounded once. What bounds it: the states, read and written once per call.
+// All of it in fp32; y is rounded once. What bounds it: the states, read and written once per call; 32 tokens x 64 heads of
+// 64 x 128 (135 MB) 25 us, 5.4 TB/s. A prompt's tokens wait for each other, 0.75 us each.
 #include "common.h"
 #include "layer.h"
 #include "scan_math.h"

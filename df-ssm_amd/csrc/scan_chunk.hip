@@ -36,6 +36,10 @@ namespace dfssm {
 namespace {
 
 constexpr int kC = kScanChunk, kW = kScanWaves;
+// Fewer groups of B and C than this, over all places, are spread over all dies. One prompt of 45 tokens, 64 heads in one group, 14.9
+// us on one die and 12.4 on eight; with 25 and 37 places (16411 tokens, and the ragged batch) 241 and 162 us by dies, 251 and 154
+// spread.
+constexpr int kSpread = 16;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 template <bool BF>
@@ -218,9 +222,12 @@ scan_chunk_kernel(ScanArgs a, int seg, int places, float* seg_state, float* seg_
   constexpr int NB = N / 16, NN = N / 32, NU = kParts<BF>, pieces = N / 8;
   __shared__ __align__(16) ScanLds<N, STATE> L;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // Workgroups go to the eight dies in turn: all that share a group's B and C run on one, next to its L2.
+  // Workgroups go to the eight dies in turn: all that share a group's B and C run on one, next to its L2, unless there are so few
+  // that dies would be idle.
   const int rep = a.H / a.G, ncb = (a.P + kScanCols - 1) / kScanCols, nwg = (rep * ncb + kW - 1) / kW;
-  const uint32_t in = blockIdx.x >> 3, unit = in / (uint32_t)nwg * 8 + (blockIdx.x & 7), place = unit / (uint32_t)a.G;
+  const bool spread = (int64_t)places * a.G < kSpread;
+  const uint32_t in = spread ? blockIdx.x : blockIdx.x >> 3, turn = in / (uint32_t)nwg;
+  const uint32_t unit = spread ? turn : turn * 8 + (blockIdx.x & 7), place = unit / (uint32_t)a.G;
   if (place >= (uint32_t)places) return;
   const int gr = (int)(unit % (uint32_t)a.G), blk = (int)(in % (uint32_t)nwg) * kW + wave;
   Where q;

@@ -1,7 +1,7 @@
 """Single-operator wrappers over the C ABI, taking torch tensors on the GPU.
 
 These are the operator-level entry points (scaffold GEMM, RMSNorm+quantize, conv step, SSM step,
-bit/embedding tiling). Every call launches on torch's current stream and raises on any error;
+bit/embedding tiling, the gated delta rule, a state space layer between its projections, the token draw). Every call launches on torch's current stream and raises on any error;
 there is no CPU fallback. Arguments that are not contiguous are copied; all copies of a call stay bound
 to names until its launch, so that the allocator cannot give one's memory to the next.
 """
@@ -631,7 +631,9 @@ def selective_scan_prefill(x: torch.Tensor, dt: torch.Tensor, A_log: torch.Tenso
                            state: torch.Tensor, D=None, dt_bias=None, cu_seqlens=None, slots=None, softplus=True, out=None,
                            state_out=None) -> torch.Tensor:
     """The selective state space scan over whole prompts (dfssm_selective_scan_prefill), from the states the sequences have
-    to those they leave: what selective_scan_step gives token by token, up to rounding.
+    to those they leave: what selective_scan_step gives token by token, up to rounding (a state within 2^-18 of the sum
+    of its terms' magnitudes, an output within 2^-16 of its terms', besides its own rounding). A value of x that is not
+    finite may also make up to 63 tokens before it, in its sequence and column, not finite.
 
     Either packed, x (T, H, P), dt (T, H), B, C (T, G, N) with cu_seqlens (n + 1,) int32 on the device (sequence b has
     tokens cu_seqlens[b] .. cu_seqlens[b + 1], which must not fall; any length, zero included; rows of no sequence are

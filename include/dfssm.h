@@ -403,7 +403,7 @@ int dfssm_gated_delta_prefill(const dfssm_delta* args, void* workspace, void* st
  * nothing outside the tensors is read or written), or n_tokens / n_seq each with NULL, and the state in slot
  * slots[b], or b with NULL. A negative slot is padding: zeros in out; one that is >= n_slots or an earlier sequence's: NaN.
  * Neither touches a state. state_out is `state` itself or memory that does not overlap it; slots that no sequence has
- * stay as they are there. */
+ * stay as they are there. n_tokens is at most 2^30; rows of the convolution and the norms lie at most 2^30 elements apart. */
 
 /* Short causal convolution of each channel, y_t = f(bias + sum_k weight_k x_{t - width + 1 + k}), f(y) = y / (1 + e^-y) with
  * silu, else y, in fp32 with one rounding; the x before a sequence are its state's, which takes the last width - 1. */
@@ -457,7 +457,9 @@ typedef struct dfssm_scan {
 /* One token per sequence (n_tokens = n_seq). */
 int dfssm_selective_scan_step(const dfssm_scan* args, void* stream);
 /* Whole prompts, from the states the sequences have to those they leave: what dfssm_selective_scan_step gives token by
- * token, up to rounding. workspace: 16-byte aligned device memory of dfssm_selective_scan_workspace_bytes(args) bytes (0:
+ * token, up to rounding: a state is off by less than 2^-18 of the sum of its terms' magnitudes, out by less than 2^-16 of its
+ * terms', besides its own rounding. A value of x that is not finite may also reach up to 63 tokens before it in its sequence and column.
+ * workspace: 16-byte aligned device memory of dfssm_selective_scan_workspace_bytes(args) bytes (0:
  * none needed, NULL allowed), for this call alone while it runs; its contents do not matter. */
 size_t dfssm_selective_scan_workspace_bytes(const dfssm_scan* args);
 int dfssm_selective_scan_prefill(const dfssm_scan* args, void* workspace, void* stream);

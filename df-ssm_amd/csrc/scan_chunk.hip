@@ -15,8 +15,8 @@
 // take 0.41 ms, of which the matrix cores are busy a third and the other pipe nearly half (1.03 GB, 0.21 ms of copying); two waves
 // to a SIMD overlap them little. Sharing M between the two waves of a head (10% fewer matrix instructions, 20% fewer others, a
 // barrier more and 24 KiB) and three waves to a SIMD (168 registers, B not held twice) both came out the same. One sequence of
-// 16411 tokens x 64 heads: 0.07 ms for the segments' states, 0.01 for their chain, 0.16 for the rest (fp16; 0.06 ms of copying). One
-// chunk: 15 us, most of it the code's way into the instruction cache and the loads before the first product.
+// 16411 tokens x 64 heads: 0.07 ms for the segments' states, 0.02 for their chain, 0.16 for the rest (fp16; 0.06 ms of copying). One
+// chunk: 12 us, most of it the code's way into the instruction cache and the loads before the first product.
 //
 // Numbers. States, sums and everything between products are fp32; G is summed in fp64, and its differences taken of float pairs,
 // so that they survive a decay of any size in the same chunk (a_t is held to -1e5). x, B and C are exact operands of the 16-bit

@@ -383,6 +383,15 @@ def _need_all(dev: int, *named) -> None:
             raise ValueError(f"{n} is on another device than x")
 
 
+def _per_column(t, name: str, cols: int, dev: int):
+    """t (cols,) fp32 on device dev, contiguous."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.get_device() == dev):
+        _need_all(dev, (t, torch.float32, name))
+    if t.shape != (cols,):
+        raise ValueError(f"{name} must be ({cols},)")
+    return t if t.is_contiguous() else t.contiguous()
+
+
 def _own_rows(t: torch.Tensor, rows: int, ld: int, p: int, width: int, name: str) -> None:
     """Refuses an output whose rows are not written in place (a copy was made) or overlap."""
     if t.data_ptr() != p or (rows > 1 and ld < width):
@@ -564,12 +573,12 @@ def _scan_call(step: bool, x, dt, A_log, B, C, state, D, dt_bias, cu_seqlens, sl
     if N not in (64, 128) or P % 16 or not 16 <= P <= 256 or H < 1 or G < 1 or H % G:
         raise ValueError("cols must be 64 or 128, dim a multiple of 16 up to 256, and the heads a multiple of the "
                          f"groups; got cols {N}, dim {P}, {H} heads and {G} groups")
-    for t, n in ((A_log, "A_log"), (D, "D"), (dt_bias, "dt_bias")):
-        if t is not None:
-            if t is not A_log:
-                _need_all(dev, (t, f32, n))
-            if t.shape != (H,):
-                raise ValueError(f"{n} must be ({H},)")
+    if A_log.shape != (H,):
+        raise ValueError(f"A_log must be ({H},)")
+    if D is not None:
+        D = _per_column(D, "D", H, dev)
+    if dt_bias is not None:
+        dt_bias = _per_column(dt_bias, "dt_bias", H, dev)
     if cu_seqlens is not None:
         cu_seqlens = _offsets(cu_seqlens, dev)
         n_seq = cu_seqlens.numel() - 1
@@ -597,8 +606,6 @@ def _scan_call(step: bool, x, dt, A_log, B, C, state, D, dt_bias, cu_seqlens, sl
     C, ld_C, cp = _rows16(C, G * N)
     dt, ld_dt, dp = _rows32(dt, H)
     A_log = A_log.contiguous()
-    D = None if D is None else D.contiguous()
-    dt_bias = None if dt_bias is None else dt_bias.contiguous()
     args = _C.Scan(xp, dp, bp, cp, A_log.data_ptr(), _C.ptr(D), _C.ptr(dt_bias), sp, so, _C.ptr(slots), _C.ptr(cu_seqlens),
                    out.data_ptr(), ld_x, ld_dt, ld_B, ld_C, ld_out, T, n_seq, state.shape[0], H, G, P, N, kind,
                    2 if dt.dtype is f32 else kind, 1 if softplus else 0)
@@ -665,14 +672,6 @@ def _norm_rows(x):
     return x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
 
 
-def _norm_weight(t, name: str, cols: int, dev: int):
-    if not (isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.get_device() == dev):
-        _need_all(dev, (t, torch.float32, name))
-    if t.shape != (cols,):
-        raise ValueError(f"{name} must be ({cols},)")
-    return t if t.is_contiguous() else t.contiguous()
-
-
 def _eps(eps) -> float:
     eps = float(eps)
     if not eps >= 2.0 ** -126:
@@ -714,7 +713,7 @@ def gated_norm(x: torch.Tensor, gate, weight: torch.Tensor, groups: int = 1, eps
     groups = operator.index(groups)
     if groups < 1 or cols % groups or cols // groups > MAX_NORM_COLS:
         raise ValueError(f"groups must divide {cols} into parts of at most {MAX_NORM_COLS}, got {groups}")
-    weight = _norm_weight(weight, "weight", cols, dev)
+    weight = _per_column(weight, "weight", cols, dev)
     eps = _eps(eps)
     r, ld, p = _rows(r, cols)
     inputs = [(r, ld, p)]
@@ -752,11 +751,11 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
     rows, cols = r.shape
     if cols > MAX_NORM_COLS:
         raise ValueError(f"x must have at most {MAX_NORM_COLS} columns, got {cols}")
-    weight = _norm_weight(weight, "weight", cols, dev)
-    post_weight = None if post_weight is None else _norm_weight(post_weight, "post_weight", cols, dev)
+    weight = _per_column(weight, "weight", cols, dev)
+    post_weight = None if post_weight is None else _per_column(post_weight, "post_weight", cols, dev)
     scales = None
     if isinstance(scale, torch.Tensor):
-        scales, scale = _norm_weight(scale, "scale", cols, dev), 0.0
+        scales, scale = _per_column(scale, "scale", cols, dev), 0.0
     eps = _eps(eps)
     r, ld, p = _rows(r, cols)
     s, ld_s, sp = _rows(_norm_rows(residual), cols)

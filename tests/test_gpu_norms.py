@@ -128,3 +128,35 @@ def test_rows_past_32_bits_and_many_in_turn():
         check(ops.gated_norm(x.to(DEV), z.to(DEV), wn.to(DEV)), lm.gated(x, z, wn), 128 * 2.0 ** -24, f"{n}")
         out, r = ops.residual_norm(x.to(DEV), z.to(DEV), wn.to(DEV), post_weight=wn.to(DEV))
         check(r, lm.residual(x, z, wn, wn)[1], 64 * 2.0 ** -24, f"{n}", lm.residual(x, z, wn, wn)[2])
+
+
+@pytest.mark.parametrize("cols", [2, 7, 9, 15, 63, 65, 127, 129, 511, 513, 1023, 1025, 2047, 2049, 4095, 4097, 8191, 8193, 16381])
+def test_widths_that_end_inside_a_lane(cols):
+    """The last lane's columns overlap its neighbour's: what lies beside the rows stays, in place too."""
+    gen = torch.Generator().manual_seed(cols)
+    wide = rnd(gen, 70, cols + 10).half()
+    x, z, w = wide[:, 5:5 + cols], rnd(gen, 70, cols).half(), 1 + 0.2 * rnd(gen, cols)
+    g = wide.to(DEV)
+    out = ops.gated_norm(g[:, 5:5 + cols], z.to(DEV), w.to(DEV), out=g[:, 5:5 + cols])
+    check(out, lm.gated(x, z, w), 128 * 2.0 ** -24, "gated")
+    assert torch.equal(g[:, :5].cpu(), wide[:, :5]) and torch.equal(g[:, 5 + cols:].cpu(), wide[:, 5 + cols:])
+    for res in (torch.float16, torch.float32):
+        r = rnd(gen, 70, cols + 10).to(res)
+        ref, new, mag = lm.residual(x, r[:, 3:3 + cols], w, w, 0.5)
+        g, gr = wide.to(DEV), r.to(DEV)
+        out, ro = ops.residual_norm(g[:, 5:5 + cols], gr[:, 3:3 + cols], w.to(DEV), post_weight=w.to(DEV), scale=0.5,
+                                    out=g[:, 5:5 + cols], residual_out=gr[:, 3:3 + cols])
+        check(ro, new, 64 * 2.0 ** -24, "residual", mag)
+        f = (w.double().abs() / (new.pow(2).mean(-1, keepdim=True) + 1e-5).sqrt())
+        check(out, ref, 2.0 ** -17, "out", ref.abs() / 2 + mag * f / 2)
+        assert torch.equal(gr[:, :3].cpu(), r[:, :3]) and torch.equal(gr[:, 3 + cols:].cpu(), r[:, 3 + cols:])
+        assert torch.equal(g[:, :5].cpu(), wide[:, :5]) and torch.equal(g[:, 5 + cols:].cpu(), wide[:, 5 + cols:])
+
+
+@pytest.mark.parametrize("n,groups", [(8, 8), (9, 5), (13, 40), (64, 3), (100, 7), (3, 11)])
+def test_small_groups(n, groups):
+    gen = torch.Generator().manual_seed(n)
+    x, z, w = rnd(gen, 300, n * groups).bfloat16(), rnd(gen, 300, n * groups).bfloat16(), 1 + 0.2 * rnd(gen, n * groups)
+    for first in (True, False):
+        check(ops.gated_norm(x.to(DEV), z.to(DEV), w.to(DEV), groups=groups, gate_first=first), lm.gated(x, z, w, groups, first),
+              128 * 2.0 ** -24, "out")

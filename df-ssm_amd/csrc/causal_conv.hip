@@ -2,10 +2,11 @@
 //   y_t = f(b + sum_{k < W} w_k x_{t - W + 1 + k}),  f(y) = y or y / (1 + e^-y),  W = 2 .. 4 taps per channel
 // where the x before a sequence are its state's, which is left as the last W - 1 of state and sequence together.
 // Sums are fp32, in the order b, w_0 x, .. w_{W-1} x; y is rounded once. States are copied, never rounded.
-// What bounds it: memory. 64 x 512 tokens of 5376 channels (bf16, 709 MB) 0.149 ms, 4.8 TB/s, where a copy reaches 4.9; twelve
-// ragged sequences of 4352 channels (fp16, 134 MB) 31 us. A wave reads 1 KiB of a row at a time, eight rows on their way
-// together (one by one, a load waits for the store before it: 0.160 ms); a tile's three rows before it come out of L2. Few rows:
-// the launch; one of 4352 channels 4.0 us in a replayed graph.
+// What bounds it: memory. 64 x 512 tokens of 5376 channels (bf16, 709 MB) 0.136 ms, 5.2 TB/s, where a copy of 1 GiB reaches 5.3; twelve
+// ragged sequences of 4352 channels (fp16, 134 MB) 29 us. A wave reads 1 KiB of a row at a time, eight rows on their way
+// together (one by one, a load waits for the store before it); a tile's three rows before it come out of L2. States and weights
+// go in the same wide pieces: by 2 bytes each, 0.150 ms, and 700 sequences of 9 tokens of 2048 channels 34 us instead of 19 (14 at a
+// copy's rate). Few rows: the launch; one of 4352 channels 3.5 us in a replayed graph.
 #include "common.h"
 #include "layer.h"
 
@@ -15,17 +16,53 @@ namespace {
 
 constexpr int kRows = 16;  // tokens of a tile, which reads W - 1 rows more
 
+template <int V>
+__device__ __forceinline__ uint16_t value(const Raw16<V>& r, int i) {
+  if constexpr (V == 1) return r.v;
+  else return r.v[i];
+}
+// M values of each of a lane's V channels, as they lie in memory: V M of them in a row.
+template <int V, int M>
+struct Channels {
+  uint16_t v[V * M];
+  __device__ __forceinline__ void load(const uint16_t* p) {
+#pragma unroll
+    for (int j = 0; j < M; ++j) {
+      const Raw16<V> r = load_raw<V>(p + j * V);
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[j * V + i] = value<V>(r, i);
+    }
+  }
+  __device__ __forceinline__ void store(uint16_t* p) const {
+#pragma unroll
+    for (int j = 0; j < M; ++j) {
+      Raw16<V> r;
+      if constexpr (V == 1) {
+        r.v = v[j];
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) r.v[i] = v[j * V + i];
+      }
+      *(typename Pack16<V>::loose*)(p + j * V) = r.v;
+    }
+  }
+  __device__ __forceinline__ uint16_t& at(int i, int k) { return v[i * M + k]; }
+};
+
 // A lane's V channels from c on: their weights, and rows of x and of the state.
 template <int V, int W, bool BF>
 struct Lane {
   float w[W][V], b[V];
   __device__ __forceinline__ void weights(const ConvArgs& a, int c) {
+    Channels<V, W> m;
+    m.load(a.weight + (int64_t)c * W);
 #pragma unroll
     for (int i = 0; i < V; ++i)
 #pragma unroll
-      for (int k = 0; k < W; ++k) w[k][i] = w2f<BF>(a.weight[(int64_t)(c + i) * W + k]);
+      for (int k = 0; k < W; ++k) w[k][i] = w2f<BF>(m.at(i, k));
 #pragma unroll
-    for (int i = 0; i < V; ++i) b[i] = a.bias ? w2f<BF>(a.bias[c + i]) : 0.0f;
+    for (int i = 0; i < V; ++i) b[i] = 0.0f;
+    if (a.bias) load16<V, BF>(a.bias + c, b);
   }
   __device__ __forceinline__ void apply(const float (&x)[W][V], bool silu, uint16_t* out) const {
     float y[V];
@@ -75,32 +112,31 @@ __global__ __launch_bounds__(256) void conv_prefill_kernel(ConvArgs a, int64_t t
   float win[W][V];  // the window, moved on by a token at a time
   if (first) {
     const int64_t at = ((int64_t)slot * a.C + c) * (W - 1), n = q.t1 - q.t0;
-    uint16_t h[W - 1][V];
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-#pragma unroll
-      for (int k = 0; k < W - 1; ++k) h[k][i] = a.state[at + i * (W - 1) + k];
+    Channels<V, W - 1> h, left;
+    h.load(a.state + at);
 #pragma unroll
     for (int k = 0; k < W - 1; ++k)
 #pragma unroll
-      for (int i = 0; i < V; ++i) win[k][i] = w2f<BF>(h[k][i]);
+      for (int i = 0; i < V; ++i) win[k][i] = w2f<BF>(h.at(i, k));
 #pragma unroll
     for (int k = 0; k < W - 1; ++k) {  // element k from the end of state and sequence
       const int64_t p = n - (W - 1) + k;
+      if (p >= 0) {
+        const Raw16<V> r = load_raw<V>(x + (q.t0 + p) * a.ld_x);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        uint16_t v;
-        if (p >= 0) {
-          v = x[(q.t0 + p) * a.ld_x + i];
-        } else {
-          v = h[k][i];
+        for (int i = 0; i < V; ++i) left.at(i, k) = value<V>(r, i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          uint16_t v = h.at(i, k);
 #pragma unroll
           for (int j = 1; j < W - 1; ++j)
-            if (n == j && k + j < W - 1) v = h[k + j < W - 1 ? k + j : 0][i];
+            if (n == j && k + j < W - 1) v = h.at(i, k + j < W - 1 ? k + j : 0);
+          left.at(i, k) = v;
         }
-        a.state_out[at + i * (W - 1) + k] = v;
       }
     }
+    left.store(a.state_out + at);
   } else {
 #pragma unroll
     for (int k = 0; k < W - 1; ++k) load16<V, BF>(x + (tok - (W - 1) + k) * a.ld_x, win[k]);
@@ -143,21 +179,18 @@ __global__ __launch_bounds__(256) void conv_step_kernel(ConvArgs a, int64_t task
   l.weights(a, c);
   const int64_t at = ((int64_t)slot * a.C + c) * (W - 1);
   float win[W][V];
-  uint16_t h[W][V];
+  Channels<V, W - 1> h, left;
+  h.load(a.state + at);
+  const Raw16<V> x = load_raw<V>(a.x + t * a.ld_x + c);
+  widen<V, BF>(x, win[W - 1]);
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
+  for (int k = 0; k < W - 1; ++k)
 #pragma unroll
-    for (int k = 0; k < W - 1; ++k) h[k][i] = a.state[at + i * (W - 1) + k];
-    h[W - 1][i] = a.x[t * a.ld_x + c + i];
-  }
-#pragma unroll
-  for (int k = 0; k < W; ++k)
-#pragma unroll
-    for (int i = 0; i < V; ++i) win[k][i] = w2f<BF>(h[k][i]);
-#pragma unroll
-  for (int i = 0; i < V; ++i)
-#pragma unroll
-    for (int k = 0; k < W - 1; ++k) a.state_out[at + i * (W - 1) + k] = h[k + 1][i];
+    for (int i = 0; i < V; ++i) {
+      win[k][i] = w2f<BF>(h.at(i, k));
+      left.at(i, k) = k < W - 2 ? h.at(i, k + 1 < W - 1 ? k + 1 : 0) : value<V>(x, i);
+    }
+  left.store(a.state_out + at);
   l.apply(win, a.silu, out);
 }
 

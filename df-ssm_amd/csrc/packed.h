@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include "common.h"
+#include "places.h"
 
 namespace dfssm {
 
@@ -56,27 +57,25 @@ struct Where {
   int64_t first, t0, t1;  // place, tokens of a sequence
   int seq;
 };
-// (C = 0: c tokens, and tokens that fit 31 bits.)
+// (C = 0: c tokens, and tokens that fit 31 bits.) The sequence found may start behind the place, if it is the first.
 template <int64_t C, class Args>
 __device__ __forceinline__ void find_seq(const Args& a, int64_t s, Where& q, int64_t c = C) {
   const int lane = threadIdx.x & 63;
-  int lo = 0, n = a.n_seq;  // the last sequence that starts at or before s is one of lo .. lo + n - 1
-  while (n > 1) {
-    const int step = (n + 63) / 64, i = lo + lane * step;
+  auto start = [&](int64_t t0, int b) {
+    return C ? place_of(t0, b, C ? C : 1) : (int64_t)((uint32_t)t0 / (uint32_t)c) + b;
+  };
+  q.seq = last_started(a.n_seq, [&](int lo, int step, int end) {
+    const int i = lo + lane * step;
     bool before = false;
-    if (i < lo + n) {
+    if (i < end) {
       int64_t t0, t1;
       seq_range(a, i, t0, t1);
-      before = (C ? t0 / (C ? C : 1) : (int64_t)((uint32_t)t0 / (uint32_t)c)) + i <= s;
+      before = start(t0, i) <= s;
     }
-    const int k = __popcll(__ballot(before));  // the starts rise, so the first k lanes (lane 0's always does)
-    const int end = lo + n;
-    lo += (k > 0 ? k - 1 : 0) * step;
-    n = min(step, end - lo);
-  }
-  seq_range(a, lo, q.t0, q.t1);
-  q.first = (C ? q.t0 / (C ? C : 1) : (int64_t)((uint32_t)q.t0 / (uint32_t)c)) + lo;
-  q.seq = lo;
+    return (int)__popcll(__ballot(before));
+  });
+  seq_range(a, q.seq, q.t0, q.t1);
+  q.first = start(q.t0, q.seq);
 }
 // Tokens [tok, tok + the result) of place s; 0 where it holds none.
 template <int64_t C, class Args>

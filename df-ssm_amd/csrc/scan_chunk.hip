@@ -151,9 +151,6 @@ __device__ __forceinline__ void fetch_shared(f16 (*to)[N], const char* p, int ld
 // segments are counted, so that places are taken without gaps and the dies have equally many: with the numbering of tile_of 64
 // sequences of 512 tokens gave one die nine and another seven. Beyond, they even out by themselves.
 constexpr int kCounted = 512;
-__device__ __forceinline__ int segments_of(int64_t len, int seg) {  // (tokens and segments fit 31 bits)
-  return len > seg ? (int)(((uint32_t)len + seg - 1) / (uint32_t)seg) : 1;
-}
 // The segments of 64 sequences from `from` on, a lane's and those before it; all of them returned.
 __device__ __forceinline__ int count_segments(const ScanArgs& a, int from, int seg, int& own, int& before) {
   const int lane = threadIdx.x & 63, i = from + lane;
@@ -161,7 +158,7 @@ __device__ __forceinline__ int count_segments(const ScanArgs& a, int from, int s
   if (i < a.n_seq) {
     int64_t t0, t1;
     seq_range(a, i, t0, t1);
-    own = segments_of(t1 - t0, seg);
+    own = scan_segments(t1 - t0, seg);
   }
   int sum = own;
   sum += __builtin_amdgcn_update_dpp(0, sum, 0x111, 0xf, 0xf, true);  // from 1, 2, 4 and 8 lanes before, in the row of 16
@@ -176,7 +173,7 @@ __device__ __forceinline__ int count_segments(const ScanArgs& a, int from, int s
 // The sequence of a place; false where there is none.
 __device__ __forceinline__ bool sequence_at(const ScanArgs& a, int place, int seg, Where& q) {
   if (!a.cu) {
-    const int per = segments_of(a.len, seg);
+    const int per = scan_segments(a.len, seg);
     q.seq = (int)((uint32_t)place / (uint32_t)per);
     q.first = (int64_t)q.seq * per;
     if (q.seq >= a.n_seq) return false;
@@ -185,7 +182,7 @@ __device__ __forceinline__ bool sequence_at(const ScanArgs& a, int place, int se
   }
   if (a.n_seq > kCounted) {
     find_seq<0>(a, place, q, seg);
-    return place - q.first < segments_of(q.t1 - q.t0, seg);
+    return scan_holds(place, q.first, q.t1 - q.t0, seg);
   }
   int base = 0;
   for (int from = 0; from < a.n_seq; from += 64) {
@@ -204,8 +201,8 @@ __device__ __forceinline__ bool sequence_at(const ScanArgs& a, int place, int se
 }
 // The first place of a sequence.
 __device__ __forceinline__ int64_t first_place(const ScanArgs& a, int b, int seg, int64_t t0) {
-  if (!a.cu) return (int64_t)b * segments_of(a.len, seg);
-  if (a.n_seq > kCounted) return (uint32_t)t0 / (uint32_t)seg + b;
+  if (!a.cu) return (int64_t)b * scan_segments(a.len, seg);
+  if (a.n_seq > kCounted) return (int64_t)((uint32_t)t0 / (uint32_t)seg) + b;
   int base = 0;
   for (int from = 0;; from += 64) {
     int own, before;
@@ -613,7 +610,7 @@ __global__ __launch_bounds__(256) void scan_states_kernel(ScanArgs a, int seg, i
   const int b = (int)(blockIdx.x / per);
   int64_t t0, t1;
   seq_range(a, b, t0, t1);
-  const int n = segments_of(t1 - t0, seg);
+  const int n = scan_segments(t1 - t0, seg);
   if (n < 2) return;
   const int64_t first = first_place(a, b, seg, t0);
   if (first + n > places) return;  // (only where offsets fall)

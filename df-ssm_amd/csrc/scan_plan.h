@@ -3,6 +3,8 @@
 #pragma once
 #include <stdint.h>
 
+#include "places.h"
+
 namespace dfssm {
 
 constexpr int kScanChunk = 64;  // tokens of a chunk
@@ -26,7 +28,16 @@ constexpr int64_t scan_segment(int64_t n_tokens, int n_seq, int64_t wgs) {
   return m * kScanChunk;
 }
 
-// Places of the launch's numbering: segments of `seg` tokens, sequence b from floor(t0 / seg) + b on.
+// Segments of a sequence of `len` tokens; one of an empty sequence, whose state is passed on. (Tokens and segments fit 31 bits.)
+constexpr int scan_segments(int64_t len, int seg) { return len > seg ? (int)(((uint32_t)len + seg - 1) / (uint32_t)seg) : 1; }
+
+// Whether a place has a segment of the sequence that was found for it, whose first place is `first`: places behind the
+// sequence's last segment have none, nor have those before the first of all sequences, which begins behind row 0 then.
+constexpr bool scan_holds(int64_t place, int64_t first, int64_t len, int seg) {
+  return place >= first && place - first < scan_segments(len, seg);
+}
+
+// Places of the launch's numbering: segments of `seg` tokens, sequence b from place_of(t0, b, seg) on.
 constexpr int64_t scan_places(int64_t n_tokens, int n_seq, int64_t seg) { return n_tokens / seg + n_seq; }
 
 }  // namespace dfssm

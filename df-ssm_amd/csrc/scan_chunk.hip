@@ -10,21 +10,20 @@
 // a product needs is loaded from LDS and split beside the step before; B, C, x and dt of the next chunk are on their way.
 // Sequences longer than a segment take three launches: states of the segments from zero, their chain, everything.
 //
-// What bounds it. Per chunk and 32 columns (N = 128, bf16) 116 matrix instructions of 32 clocks and about 1100 others: the
+// What bounds it. Per chunk and 32 columns (N = 128, bf16) 138 matrix instructions of 32 clocks and about 1400 others: the
 // scores and M are made by each wave anew, the state is split into parts for C h0, U for the new state. 64 x 512 tokens x 80 heads
-// take 0.41 ms, of which the matrix cores are busy a third and the other pipe nearly half (1.03 GB, 0.21 ms of copying); two waves
-// to a SIMD overlap them little. Sharing M between the two waves of a head (10% fewer matrix instructions, 20% fewer others, a
-// barrier more and 24 KiB) and three waves to a SIMD (168 registers, B not held twice) both came out the same. One sequence of
-// 16411 tokens x 64 heads: 0.07 ms for the segments' states, 0.02 for their chain, 0.16 for the rest (fp16; 0.06 ms of copying). One
-// chunk: 12 us, most of it the code's way into the instruction cache and the loads before the first product.
+// take 0.45 ms (1.03 GB, 0.21 ms of copying); two waves to a SIMD overlap the matrix cores and the other pipe little. One sequence
+// of 16411 tokens x 64 heads: 0.07 ms for the segments' states, 0.02 for their chain, 0.16 for the rest (fp16; 0.06 ms of copying).
+// One chunk: 12 us, most of it the code's way into the instruction cache and the loads before the first product. Measured with two
+// bf16 parts of h0 and M (0.40 ms) and not kept: M shared between the two waves of a head (10% fewer matrix instructions, 20% fewer
+// others, a barrier more and 24 KiB), three waves to a SIMD (168 registers, B not held twice); both came out the same.
 //
 // Numbers. States, sums and everything between products are fp32; G is summed in fp64, and its differences taken of float pairs,
 // so that they survive a decay of any size in the same chunk (a_t is held to -1e5). x, B and C are exact operands of the 16-bit
-// matrix cores in their own type. An fp32 factor beside them is a sum of 16-bit parts. Beside bf16: three parts of w_j x_j, which
-// hold 24 bits and go into the state; two of h0 and M, 16 bits, each off by up to 2^-17, which go into y, rounded to 8 bits. Beside
-// fp16: pairs of halves, x 2^s = hi + lo, 22 bits, with s per column of h0 and w x and per row of M so that the largest magnitude
-// lies in [2^14, 2^15); a value below 2^-17 of the largest M of its scale is off by up to 2^-39 M. So a state comes out as from
-// fp32 arithmetic, and y is off by 2^-16 of its terms' magnitudes at most, besides its own rounding. D is on M's diagonal.
+// matrix cores in their own type. An fp32 factor beside them (h0, M, w_j x_j) is a sum of 16-bit parts. Beside bf16 three of them,
+// which hold its 24 bits (two of h0 and M, 16 bits, took 0.40 ms instead of 0.45, but an output that is small beside its terms
+// was off by more than its rounding). Beside fp16 pairs of halves, x 2^s = hi + lo, 22 bits, with s per column of h0 and w x and per row of M so that the largest magnitude
+// lies in [2^14, 2^15); a value below 2^-17 of the largest M of its scale is off by up to 2^-39 M. D is on M's diagonal.
 #include "common.h"
 #include "layer.h"
 #include "parts.h"
@@ -397,13 +396,13 @@ scan_chunk_kernel(ScanArgs a, int seg, int places, float* seg_state, float* seg_
       };
       // What the products of a step need is loaded and split beside those of the step before.
       {
-        h8 cf[2][2], sp[2][2];
+        h8 cf[2][2], sp[2][NU];
         auto load = [&](int b) { cf[b & 1][0] = row_frag(L.C, 0, b), cf[b & 1][1] = row_frag(L.C, 1, b); };
         auto split = [&](int b) {
           float v[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] = S[b >> 1][8 * (b & 1) + e];
-          parts8<BF, 2, false>(v, ssc, sp[b & 1]);
+          parts8<BF, NU, false>(v, ssc, sp[b & 1]);
         };
         load(0);
         split(0);
@@ -412,7 +411,7 @@ scan_chunk_kernel(ScanArgs a, int seg, int places, float* seg_state, float* seg_
           __builtin_amdgcn_sched_barrier(0);
           if (b + 1 < NB) load(b + 1);
 #pragma unroll
-          for (int p = 1; p >= 0; --p)
+          for (int p = NU - 1; p >= 0; --p)
 #pragma unroll
             for (int t = 0; t < 2; ++t) y[t] = mm32<BF>(sp[b & 1][p], cf[b & 1][t], y[t]);
           if (b + 1 < NB) split(b + 1);
@@ -492,12 +491,12 @@ scan_chunk_kernel(ScanArgs a, int seg, int places, float* seg_state, float* seg_
 #pragma unroll
         for (int k = 0; k < 2 * (t + 1); ++k) {
           float v[8];
-          h8 m[2];
+          h8 m[NU];
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] = sc[(k >> 1) + t][8 * (k & 1) + e];
-          parts8<BF, 2>(v, msc, m);
+          parts8<BF, NU>(v, msc, m);
 #pragma unroll
-          for (int p = 1; p >= 0; --p) y[t] = mm32<BF>(xf[k], m[p], y[t]);
+          for (int p = NU - 1; p >= 0; --p) y[t] = mm32<BF>(xf[k], m[p], y[t]);
         }
       }
       __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)

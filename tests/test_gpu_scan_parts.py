@@ -1,0 +1,52 @@
+"""The chunked selective scan where its factors' splitting into 16-bit parts shows.
+
+Tolerances: see each test. Decays are switched off (A_log -200: e^-200 is zero in fp32), so that nothing else rounds."""
+import pytest
+import torch
+
+import layer_math as lm
+from dfssm import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+# Two values 2^-22 apart. Of 1 + 2^-9 + 2^-17 -+ 2^-23 two parts of 8 bits hold 1 + 2^-9 and 1 + 2^-9 + 2^-16, 2^-16 apart.
+NEAR, FAR = 1 + 2.0 ** -9 + 2.0 ** -17 - 2.0 ** -23, 1 + 2.0 ** -9 + 2.0 ** -17 + 2.0 ** -23
+
+
+def call(x, dt, B, C, state, lens, softplus=False, D=None):
+    state = state.to(DEV)
+    A_log = torch.full((x.shape[1],), -200.0, device=DEV)
+    out = ops.selective_scan_prefill(x.to(DEV), dt.to(DEV), A_log, B.to(DEV), C.to(DEV), state, D=D, cu_seqlens=lm.offsets(lens, DEV),
+                                     softplus=softplus)
+    return out.cpu().double(), state.cpu().double()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("P,N", [(64, 128), (48, 64)])
+@pytest.mark.parametrize("n", [0, 17, 62])
+def test_a_state_whose_terms_cancel(n, P, N, dtype):
+    """y = h_n - h_{n+1}, no time passes. The sums of two terms of size 1 in a few parts each take less than 16 roundings of 2^-24
+    of 1: 2^-20. (Two bf16 parts are off by 2^-16.) Parts of halves are off by 2^-23 each."""
+    T = 100
+    x, B, C = torch.ones(T, 2, P).to(dtype), torch.ones(T, 1, N).to(dtype), torch.zeros(T, 1, N).to(dtype)
+    C[:, 0, n], C[:, 0, n + 1] = 1, -1
+    state = torch.zeros(1, 2, P, N)
+    state[..., n], state[..., n + 1] = NEAR, FAR
+    out, after = call(x, torch.zeros(T, 2), B, C, state, [T])
+    assert (out - (NEAR - FAR)).abs().max() <= 2.0 ** -20 and torch.equal(after, state.double())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("P,N", [(64, 128), (48, 64)])
+@pytest.mark.parametrize("j", [0, 15, 17, 31, 40, 62])
+def test_scores_that_cancel(j, P, N, dtype):
+    """y_i = d_j x_j + d_{j+1} x_{j+1} with x = 1, -1, scores of 1: as above, in the matrix of scores and decays."""
+    T = 64
+    x, B, C = torch.zeros(T, 2, P).to(dtype), torch.zeros(T, 1, N).to(dtype), torch.zeros(T, 1, N).to(dtype)
+    x[j], x[j + 1] = 1, -1
+    B[:, 0, 3] = C[:, 0, 3] = 1
+    dt = torch.zeros(T, 2)
+    dt[j], dt[j + 1] = NEAR, FAR
+    out, _ = call(x, dt, B, C, torch.zeros(1, 2, P, N), [T])
+    assert not out[:j].any() and (out[j] - NEAR).abs().max() <= lm.half_step(dtype)[0] * NEAR
+    assert (out[j + 1:] - (NEAR - FAR)).abs().max() <= 2.0 ** -20

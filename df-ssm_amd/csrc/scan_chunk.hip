@@ -22,8 +22,9 @@
 // so that they survive a decay of any size in the same chunk (a_t is held to -1e5). x, B and C are exact operands of the 16-bit
 // matrix cores in their own type. An fp32 factor beside them (h0, M, w_j x_j) is a sum of 16-bit parts. Beside bf16 three of them,
 // which hold its 24 bits (two of h0 and M, 16 bits, took 0.40 ms instead of 0.45, but an output that is small beside its terms
-// was off by more than its rounding). Beside fp16 pairs of halves, x 2^s = hi + lo, 22 bits, with s per column of h0 and w x and per row of M so that the largest magnitude
-// lies in [2^14, 2^15); a value below 2^-17 of the largest M of its scale is off by up to 2^-39 M. D is on M's diagonal.
+// was off by more than its rounding). Beside fp16 pairs of halves, x 2^s = hi + lo, 22 bits, with s per column of h0 and w x
+// and per row of M so that the largest magnitude lies in [2^14, 2^15); a value below 2^-17 of the largest M of its scale is off
+// by up to 2^-39 M. D is on M's diagonal.
 #include "common.h"
 #include "layer.h"
 #include "parts.h"
@@ -541,7 +542,8 @@ scan_chunk_kernel(ScanArgs a, int seg, int places, float* seg_state, float* seg_
         weighted(k, u[k]);
         top = max_abs(u[k], top);
       }
-      usc = pow2_scale(__builtin_elementwise_maximum(max_halves(top), dec * (smax * sfac)), uinv);
+      top = __builtin_elementwise_maximum(max_halves(top), dec * (smax * sfac));
+      usc = pow2_scale(__builtin_elementwise_maximum(top, sfac * 0x1p-100f), uinv);  // (so that sfac usc is finite)
       keep = dec * sfac * usc;
       sfac = uinv;
     }

@@ -50,3 +50,17 @@ def test_scores_that_cancel(j, P, N, dtype):
     out, _ = call(x, dt, B, C, torch.zeros(1, 2, P, N), [T])
     assert not out[:j].any() and (out[j] - NEAR).abs().max() <= lm.half_step(dtype)[0] * NEAR
     assert (out[j + 1:] - (NEAR - FAR)).abs().max() <= 2.0 ** -20
+
+
+@pytest.mark.parametrize("x0,d0", [(20000.0, 10.0), (60000.0, 1e30), (1.0, 0.5)])
+def test_nothing_after_large_values(x0, d0):
+    """Tokens whose B is zero leave no state, however large their d x; what follows is zero, not NaN."""
+    T, H, P, N = 256, 2, 32, 64
+    x, B = torch.zeros(T, H, P).half(), torch.zeros(T, 1, N).half()
+    x[:64] = x0
+    out, after = call(x, torch.full((T, H), d0), B, torch.ones(T, 1, N).half(), torch.zeros(1, H, P, N), [T])
+    assert not out.any() and not after.any()
+    x[200:], B[200:] = 1.0, 0.5                                                 # and what comes then is there in full
+    _, after = call(x, torch.full((T, H), min(d0, 1.0)), B, torch.ones(T, 1, N).half(), torch.zeros(1, H, P, N), [T])
+    ref = 56 * 0.5 * min(d0, 1.0)
+    assert ((after - ref).abs() <= 2.0 ** -18 * ref).all()

@@ -542,8 +542,10 @@ scan_chunk_kernel(ScanArgs a, int seg, int places, float* seg_state, float* seg_
         weighted(k, u[k]);
         top = max_abs(u[k], top);
       }
-      top = __builtin_elementwise_maximum(max_halves(top), dec * (smax * sfac));
-      usc = pow2_scale(__builtin_elementwise_maximum(top, sfac * 0x1p-100f), uinv);  // (so that sfac usc is finite)
+      // The state is only added to, in fp32: it may be 2^60 times what it gets, which is split by its own size. (The last term keeps
+      // sfac usc finite.)
+      top = __builtin_elementwise_maximum(max_halves(top), dec * (smax * sfac) * 0x1p-60f);
+      usc = pow2_scale(__builtin_elementwise_maximum(top, sfac * 0x1p-100f), uinv);
       keep = dec * sfac * usc;
       sfac = uinv;
     }

@@ -1,4 +1,5 @@
-"""The chunked selective scan where its factors' splitting into 16-bit parts shows.
+"""The chunked selective scan where its factors' splitting into 16-bit parts shows: terms that cancel, and beside fp16 rows values of
+very different size in one column.
 
 Tolerances: see each test. Decays are switched off (A_log -200: e^-200 is zero in fp32), so that nothing else rounds."""
 import pytest
@@ -50,6 +51,26 @@ def test_scores_that_cancel(j, P, N, dtype):
     out, _ = call(x, dt, B, C, torch.zeros(1, 2, P, N), [T])
     assert not out[:j].any() and (out[j] - NEAR).abs().max() <= lm.half_step(dtype)[0] * NEAR
     assert (out[j + 1:] - (NEAR - FAR)).abs().max() <= 2.0 ** -20
+
+
+def ordinary(lens, H, P, N, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=gen)
+    T = sum(lens)
+    return r(T, H, P).half(), 0.1 + 0.1 * torch.rand(T, H, generator=gen), r(T, 1, N).half(), r(T, 1, N).half(), 0.01 * r(len(lens), H, P, N)
+
+
+@pytest.mark.parametrize("large", [1e6, 1e8, 1e20])
+@pytest.mark.parametrize("lens", [[100], [900, 70]])
+def test_small_states_beside_a_large_one(lens, large):
+    """fp16 rows: a state value far above the others of its column takes no bits from them: within 2^-18 of their own terms."""
+    H, P, N = 2, 32, 64
+    x, dt, B, C, state = ordinary(lens, H, P, N)
+    state[..., 7] = large
+    _, _, s, smag = lm.scan(x, dt, torch.full((H,), -200.0), B, C, state, None, None, lens, softplus=False)
+    _, after = call(x, dt, B, C, state, lens)
+    bad = (after - s).abs() > 2.0 ** -18 * smag
+    assert not bad.any(), f"{int(bad.sum())} off, worst {float(((after - s).abs() / smag).max()):.3g}"
 
 
 @pytest.mark.parametrize("x0,d0", [(20000.0, 10.0), (60000.0, 1e30), (1.0, 0.5)])

@@ -23,8 +23,8 @@
 // matrix cores in their own type. An fp32 factor beside them (h0, M, w_j x_j) is a sum of 16-bit parts. Beside bf16 three of them,
 // which hold its 24 bits (two of h0 and M, 16 bits, took 0.40 ms instead of 0.45, but an output that is small beside its terms
 // was off by more than its rounding). Beside fp16 pairs of halves, x 2^s = hi + lo, 22 bits, with s per column of h0 and w x
-// and per row of M so that the largest magnitude lies in [2^14, 2^15); a value below 2^-17 of the largest M of its scale is off
-// by up to 2^-39 M. D is on M's diagonal.
+// and per row of M so that the largest magnitude lies in [2^14, 2^15); a value below 2^-16 of the largest M of its scale is off
+// by up to 2^-39 M, whatever it is multiplied by. The state's own values are kept and added to in fp32. D is on M's diagonal.
 #include "common.h"
 #include "layer.h"
 #include "parts.h"

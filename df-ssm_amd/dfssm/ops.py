@@ -639,8 +639,10 @@ def selective_scan_prefill(x: torch.Tensor, dt: torch.Tensor, A_log: torch.Tenso
                            state_out=None) -> torch.Tensor:
     """The selective state space scan over whole prompts (dfssm_selective_scan_prefill), from the states the sequences have
     to those they leave: what selective_scan_step gives token by token, up to rounding (a state within 2^-18 of the sum
-    of its terms' magnitudes, an output within 2^-16 of its terms', besides its own rounding). A value of x that is not
-    finite may also make up to 63 tokens before it, in its sequence and column, not finite.
+    of its terms' magnitudes, an output within 2^-16 of its terms', besides its own rounding, where a term that has decayed
+    by e^-t counts 1 + t / 8 times; beside fp16 rows each term's fp32 factor, d x, the state or d C.B, may also be off by
+    2^-39 of the largest of its column, or row, in 64 tokens). A value of x that is not finite may also make up to 63 tokens
+    before it, in its sequence and column, not finite.
 
     Either packed, x (T, H, P), dt (T, H), B, C (T, G, N) with cu_seqlens (n + 1,) int32 on the device (sequence b has
     tokens cu_seqlens[b] .. cu_seqlens[b + 1], which must not fall; any length, zero included; rows of no sequence are

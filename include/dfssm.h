@@ -458,7 +458,11 @@ typedef struct dfssm_scan {
 int dfssm_selective_scan_step(const dfssm_scan* args, void* stream);
 /* Whole prompts, from the states the sequences have to those they leave: what dfssm_selective_scan_step gives token by
  * token, up to rounding: a state is off by less than 2^-18 of the sum of its terms' magnitudes, out by less than 2^-16 of its
- * terms', besides its own rounding. A value of x that is not finite may also reach up to 63 tokens before it in its sequence and column.
+ * terms', besides its own rounding, where a term that has decayed by e^-t counts 1 + t / 8 times (exponents are fp32). Beside fp16
+ * rows the fp32 factor of each term may also be off by 2^-39 of the largest of its kind: in a state, of d x (and of 2^-60 of the
+ * state) in its column and chunk of 64 tokens; in out, of the state in its column, and of d C.B and D in its row of the chunk. So
+ * a large value takes bits from much smaller ones beside it even where the sum has it times zero.
+ * A value of x that is not finite may also reach up to 63 tokens before it in its sequence and column.
  * workspace: 16-byte aligned device memory of dfssm_selective_scan_workspace_bytes(args) bytes (0:
  * none needed, NULL allowed), for this call alone while it runs; its contents do not matter. */
 size_t dfssm_selective_scan_workspace_bytes(const dfssm_scan* args);

@@ -85,3 +85,39 @@ def test_nothing_after_large_values(x0, d0):
     _, after = call(x, torch.full((T, H), min(d0, 1.0)), B, torch.ones(T, 1, N).half(), torch.zeros(1, H, P, N), [T])
     ref = 56 * 0.5 * min(d0, 1.0)
     assert ((after - ref).abs() <= 2.0 ** -18 * ref).all()
+
+
+def off(got, ref, tol, what):
+    bad = (got - ref).abs() > tol
+    assert not bad.any(), f"{what}: {int(bad.sum())} off, worst {float(((got - ref).abs() / tol).max()):.3g} of the bound"
+
+
+@pytest.mark.parametrize("lens", [[100], [900, 70]])
+def test_small_values_beside_a_large_one_that_a_sum_leaves_out(lens):
+    """fp16 rows: a factor may be off by 2^-39 of the largest of its kind, also where that one is multiplied by zero."""
+    H, P, N = 2, 32, 64
+    x, dt, B, C, state = ordinary(lens, H, P, N)
+    A_log, rel, tiny = torch.full((H,), -200.0), *lm.half_step(torch.float16)
+    total = lambda t: torch.stack([t[a:b].double().abs().sum(0) for a, b in lm.slices(lens)])          # over each sequence
+
+    # d x of a token, its B zero in half the columns: those states
+    X, dT, b = x.clone(), dt.clone(), B.clone()
+    X[5], dT[5], b[5, :, :32] = 30000.0, 200.0, 0
+    _, _, s, smag = lm.scan(X, dT, A_log, b, C, state, None, None, lens, softplus=False)
+    _, after = call(X, dT, b, C, state, lens)
+    off(after, s, 2.0 ** -18 * smag + 2.0 ** -39 * 6e6 * total(b)[:, :, None], "state")
+
+    # a state that C leaves out
+    S, c = state.clone(), C.clone()
+    S[..., 7], c[..., 7] = 1e8, 0
+    y, mag, _, _ = lm.scan(x, dt, A_log, B, c, S, None, None, lens, softplus=False)
+    out, _ = call(x, dt, B, c, S, lens)
+    off(out, y, rel * (1 + 2.0 ** -7) * y.abs() + 2.0 ** -16 * mag + tiny + 2.0 ** -39 * 1e8 * c.double().abs().sum(-1)[..., None], "state's out")
+
+    # a score whose x is zero
+    X, dT = x.clone(), dt.clone()
+    X[3], dT[3] = 0, 1e5
+    y, mag, _, _ = lm.scan(X, dT, A_log, B, C, state, None, None, lens, softplus=False)
+    out, _ = call(X, dT, B, C, state, lens)
+    score = 1e5 * (C.double() @ B[3, 0].double()).abs().amax()
+    off(out, y, rel * (1 + 2.0 ** -7) * y.abs() + 2.0 ** -16 * mag + tiny + 2.0 ** -39 * score * total(x)[:1], "scores' out")

@@ -95,6 +95,7 @@ struct Columns {
     }
   }
   __device__ __forceinline__ bool any(int k) const { return skip[k] < V; }
+  // x, or zero in another's column, before it is squared: an infinity times zero would be NaN.
   __device__ __forceinline__ float own(int k, int e, float x) const { return (TAIL ? e >= skip[k] : skip[k] == 0) ? x : 0.0f; }
 };
 
@@ -141,7 +142,8 @@ __global__ __launch_bounds__(kThreads<T>) void gated_norm_kernel(GatedNormArgs a
       for (int e = 0; e < V; ++e) {
         g[k][e] = a.gate ? silu_f32(g[k][e]) : 1.0f;
         if (a.gate_first) v[k][e] *= g[k][e];
-        ss = __builtin_fmaf(v[k][e], cs.own(k, e, v[k][e]), ss);
+        const float o = cs.own(k, e, v[k][e]);
+        ss = __builtin_fmaf(o, o, ss);
       }
     const float f = rms_factor(row_sum<T>(ss, part, slot), inv_n, a.eps);
 #pragma unroll
@@ -196,7 +198,8 @@ __global__ __launch_bounds__(kThreads<T>) void residual_norm_kernel(ResidualNorm
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         if constexpr (R32) s[k][e] = r[k][e];
-        ss = __builtin_fmaf(v[k][e], cs.own(k, e, v[k][e]), ss);
+        const float o = cs.own(k, e, v[k][e]);
+        ss = __builtin_fmaf(o, o, ss);
       }
       if constexpr (!R32) widen<V, BF>(rh[k], s[k]);
     }
@@ -219,7 +222,8 @@ __global__ __launch_bounds__(kThreads<T>) void residual_norm_kernel(ResidualNorm
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         s[k][e] = __builtin_fmaf(m[k][e], v[k][e], s[k][e]);
-        ss = __builtin_fmaf(s[k][e], cs.own(k, e, s[k][e]), ss);
+        const float o = cs.own(k, e, s[k][e]);
+        ss = __builtin_fmaf(o, o, ss);
       }
     const float f = rms_factor(row_sum<T>(ss, part, slot), inv_n, a.eps);
 #pragma unroll

@@ -46,8 +46,8 @@ int check_conv(const dfssm_conv* d, bool step) {
   return DFSSM_OK;
 }
 
-ConvArgs conv_args(const dfssm_conv* d) {
-  ConvArgs a{};
+PackedConvArgs conv_args(const dfssm_conv* d) {
+  PackedConvArgs a{};
   a.x = (const uint16_t*)d->x; a.weight = (const uint16_t*)d->weight; a.bias = (const uint16_t*)d->bias;
   a.state = (const uint16_t*)d->state; a.state_out = (uint16_t*)d->state_out;
   a.slots = d->slots; a.cu = d->cu_seqlens; a.out = (uint16_t*)d->out;
@@ -80,8 +80,8 @@ int check_scan(const dfssm_scan* d, bool step) {
   return DFSSM_OK;
 }
 
-ScanArgs scan_args(const dfssm_scan* d) {
-  ScanArgs a{};
+PackedScanArgs scan_args(const dfssm_scan* d) {
+  PackedScanArgs a{};
   a.x = (const uint16_t*)d->x; a.B = (const uint16_t*)d->B; a.C = (const uint16_t*)d->C; a.dt = d->dt;
   a.A_log = d->A_log; a.D = d->D; a.dt_bias = d->dt_bias;
   a.state = d->state; a.state_out = d->state_out;
@@ -100,7 +100,7 @@ ScanArgs scan_args(const dfssm_scan* d) {
 //   40 heads of 128 x 128, 5 groups     9.3, 11.8 | 12.3, 11.9 | 15.3, 11.9          55, 49 | 72, 49 | 96, 49
 //   6 heads of 256 x 64                 8.2, 8.8 | 10.7, 8.8 | 13.1, 8.9             17, 14 | 22, 14 | 27, 14
 constexpr int kTokenPath = 8;
-bool by_tokens(const ScanArgs& a) { return (a.cu ? a.n_tokens : a.len) <= kTokenPath; }
+bool by_tokens(const PackedScanArgs& a) { return (a.cu ? a.n_tokens : a.len) <= kTokenPath; }
 
 // Rows of a norm.
 int check_rows(int64_t rows, int cols, std::initializer_list<int64_t> in, std::initializer_list<int64_t> out, float eps) {
@@ -138,14 +138,14 @@ int dfssm_selective_scan_step(const dfssm_scan* args, void* stream) {
 
 size_t dfssm_selective_scan_workspace_bytes(const dfssm_scan* args) {
   if (!args || check_scan_dims(args) != DFSSM_OK || check_sequences(args, false) != DFSSM_OK || args->n_seq == 0) return 0;
-  const ScanArgs a = scan_args(args);
+  const PackedScanArgs a = scan_args(args);
   return by_tokens(a) ? 0 : scan_chunk_workspace(a);
 }
 
 int dfssm_selective_scan_prefill(const dfssm_scan* args, void* workspace, void* stream) {
   const int rc = check_scan(args, false);
   if (rc || args->n_seq == 0) return rc;
-  const ScanArgs a = scan_args(args);
+  const PackedScanArgs a = scan_args(args);
   if (by_tokens(a)) return hip_status(launch_scan_token(a, (hipStream_t)stream));
   if (scan_chunk_workspace(a)) {
     if (!workspace) return DFSSM_E_NULL;

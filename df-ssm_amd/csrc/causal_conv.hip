@@ -53,7 +53,7 @@ struct Channels {
 template <int V, int W, bool BF>
 struct Lane {
   float w[W][V], b[V];
-  __device__ __forceinline__ void weights(const ConvArgs& a, int c) {
+  __device__ __forceinline__ void weights(const PackedConvArgs& a, int c) {
     Channels<V, W> m;
     m.load(a.weight + (int64_t)c * W);
 #pragma unroll
@@ -87,7 +87,7 @@ __device__ __forceinline__ void fill_rows(uint16_t* out, int64_t ld, int64_t n, 
 // One wave: 64 V channels of a tile of kRows tokens of one sequence; the first tile also leaves the state, which it alone
 // reads (so that it may be the same memory).
 template <int V, int W, bool BF>
-__global__ __launch_bounds__(256) void conv_prefill_kernel(ConvArgs a, int64_t tasks) {
+__global__ __launch_bounds__(256) void conv_prefill_kernel(PackedConvArgs a, int64_t tasks) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nc = (a.C + 64 * V - 1) / (64 * V);
   const int64_t task = (int64_t)blockIdx.x * 4 + wave;
@@ -161,7 +161,7 @@ __global__ __launch_bounds__(256) void conv_prefill_kernel(ConvArgs a, int64_t t
 
 // One token of each sequence: a wave per 64 V channels of a row.
 template <int V, int W, bool BF>
-__global__ __launch_bounds__(256) void conv_step_kernel(ConvArgs a, int64_t tasks) {
+__global__ __launch_bounds__(256) void conv_step_kernel(PackedConvArgs a, int64_t tasks) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nc = (a.C + 64 * V - 1) / (64 * V);
   const int64_t task = (int64_t)blockIdx.x * 4 + wave;
@@ -195,7 +195,7 @@ __global__ __launch_bounds__(256) void conv_step_kernel(ConvArgs a, int64_t task
 }
 
 template <int V, int W, bool BF>
-hipError_t launch(const ConvArgs& a, bool step, hipStream_t s) {
+hipError_t launch(const PackedConvArgs& a, bool step, hipStream_t s) {
   const int64_t nc = (a.C + 64 * V - 1) / (64 * V), places = step ? a.n_seq : a.n_tokens / kRows + a.n_seq;
   const int64_t tasks = places * nc, wgs = (tasks + 3) / 4;
   if (wgs > 0x7fffffff) return hipErrorInvalidValue;
@@ -204,23 +204,23 @@ hipError_t launch(const ConvArgs& a, bool step, hipStream_t s) {
   return hipGetLastError();
 }
 template <int V, int W>
-hipError_t launch(const ConvArgs& a, bool step, hipStream_t s) {
+hipError_t launch(const PackedConvArgs& a, bool step, hipStream_t s) {
   return a.bf16 ? launch<V, W, true>(a, step, s) : launch<V, W, false>(a, step, s);
 }
 template <int V>
-hipError_t launch(const ConvArgs& a, bool step, hipStream_t s) {
+hipError_t launch(const PackedConvArgs& a, bool step, hipStream_t s) {
   return a.W == 2 ? launch<V, 2>(a, step, s) : (a.W == 3 ? launch<V, 3>(a, step, s) : launch<V, 4>(a, step, s));
 }
 // Channels to a lane: 16 bytes of them (at any address) where a row has whole ones and fills a wave, else a pair, else one. 8096 tokens
 // of 64 channels 4.9 us by one, 19 by eight; of 4350 channels 29 by pairs, of 4351 38 by one (29 at a copy's rate).
-hipError_t launch(const ConvArgs& a, bool step, hipStream_t s) {
+hipError_t launch(const PackedConvArgs& a, bool step, hipStream_t s) {
   if (a.C % 8 == 0 && a.C >= 512) return launch<8>(a, step, s);
   return a.C % 2 == 0 && a.C >= 128 ? launch<2>(a, step, s) : launch<1>(a, step, s);
 }
 
 }  // namespace
 
-hipError_t launch_conv_step(const ConvArgs& a, hipStream_t s) { return launch(a, true, s); }
-hipError_t launch_conv_prefill(const ConvArgs& a, hipStream_t s) { return launch(a, false, s); }
+hipError_t launch_conv_step(const PackedConvArgs& a, hipStream_t s) { return launch(a, true, s); }
+hipError_t launch_conv_prefill(const PackedConvArgs& a, hipStream_t s) { return launch(a, false, s); }
 
 }  // namespace dfssm

@@ -8,7 +8,7 @@
 
 namespace dfssm {
 
-struct ConvArgs {
+struct PackedConvArgs {
   const uint16_t *x, *weight, *bias;  // (tokens, C) rows ld_x elements apart, (C, W), (C) or null
   const uint16_t* state;              // (n_slots, C, W - 1), the oldest first
   uint16_t* state_out;                // the same tensor, or one of its shape
@@ -18,10 +18,10 @@ struct ConvArgs {
   int n_seq, n_slots, C, W;
   int bf16, silu;
 };
-hipError_t launch_conv_step(const ConvArgs& a, hipStream_t s);
-hipError_t launch_conv_prefill(const ConvArgs& a, hipStream_t s);
+hipError_t launch_conv_step(const PackedConvArgs& a, hipStream_t s);
+hipError_t launch_conv_prefill(const PackedConvArgs& a, hipStream_t s);
 
-struct ScanArgs {
+struct PackedScanArgs {
   const uint16_t *x, *B, *C;            // (tokens, H, P), (tokens, G, N), 16-bit, heads contiguous
   const void* dt;                       // (tokens, H), of x's type or fp32
   const float *A_log, *D, *dt_bias;     // (H); D and dt_bias may be null
@@ -34,9 +34,9 @@ struct ScanArgs {
   int bf16, dt32, softplus;
 };
 // Token by token (scan.hip), and over chunks with the workspace of scan_chunk_workspace (scan_chunk.hip).
-hipError_t launch_scan_token(const ScanArgs& a, hipStream_t s);
-hipError_t launch_scan_chunked(const ScanArgs& a, void* workspace, hipStream_t s);
-size_t scan_chunk_workspace(const ScanArgs& a);
+hipError_t launch_scan_token(const PackedScanArgs& a, hipStream_t s);
+hipError_t launch_scan_chunked(const PackedScanArgs& a, void* workspace, hipStream_t s);
+size_t scan_chunk_workspace(const PackedScanArgs& a);
 
 struct GatedNormArgs {
   const uint16_t *x, *gate;  // rows ld_* elements apart; gate may be null

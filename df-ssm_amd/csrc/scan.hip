@@ -24,7 +24,7 @@ __device__ __forceinline__ float row_sum16(float v) {
 // A workgroup: 16 NI rows p of a sequence's head. A row's N columns lie over 16 lanes, lane j with columns
 // 64 i + 4 j .., so that a row is read in whole 256-byte pieces and its sum with C needs no LDS.
 template <int N, bool BF, int NI>
-__global__ __launch_bounds__(256) void scan_token_kernel(ScanArgs a) {
+__global__ __launch_bounds__(256) void scan_token_kernel(PackedScanArgs a) {
   constexpr int NV = N / 16;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, j = lane & 15, sub = lane >> 4;
   const int nrb = (a.P + 16 * NI - 1) / (16 * NI);
@@ -95,7 +95,7 @@ __global__ __launch_bounds__(256) void scan_token_kernel(ScanArgs a) {
 }
 
 template <int N, bool BF, int NI>
-void launch_rows(const ScanArgs& a, hipStream_t s) {
+void launch_rows(const PackedScanArgs& a, hipStream_t s) {
   const int64_t wgs = (int64_t)a.n_seq * a.H * ((a.P + 16 * NI - 1) / (16 * NI));
   hipLaunchKernelGGL((scan_token_kernel<N, BF, NI>), dim3((unsigned)wgs), dim3(256), 0, s, a);
 }
@@ -103,7 +103,7 @@ void launch_rows(const ScanArgs& a, hipStream_t s) {
 // 64 x 128, one sequence 3.7, 4.1 and 4.9 us in a replayed graph, four 5.8, 5.1 and 5.6, 32 26.5, 25.4 and 24.2; 64 x 80 heads
 // 60.7, 59.8 and 61.8; 30 x 8 heads of 208 x 64 10.6, 8.2 and 7.0.
 template <int N, bool BF>
-hipError_t launch_token(const ScanArgs& a, hipStream_t s) {
+hipError_t launch_token(const PackedScanArgs& a, hipStream_t s) {
   const int64_t tiles = (int64_t)a.n_seq * a.H * (a.P / 16);
   if (tiles > 0x7fffffff) return hipErrorInvalidValue;
   if (tiles >= 1024) launch_rows<N, BF, 256 / N>(a, s);
@@ -113,7 +113,7 @@ hipError_t launch_token(const ScanArgs& a, hipStream_t s) {
 
 }  // namespace
 
-hipError_t launch_scan_token(const ScanArgs& a, hipStream_t s) {
+hipError_t launch_scan_token(const PackedScanArgs& a, hipStream_t s) {
   if (a.N == 128) return a.bf16 ? launch_token<128, true>(a, s) : launch_token<128, false>(a, s);
   return a.bf16 ? launch_token<64, true>(a, s) : launch_token<64, false>(a, s);
 }

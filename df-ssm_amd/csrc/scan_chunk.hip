@@ -152,7 +152,7 @@ __device__ __forceinline__ void fetch_shared(f16 (*to)[N], const char* p, int ld
 // sequences of 512 tokens gave one die nine and another seven. Beyond, they even out by themselves.
 constexpr int kCounted = 512;
 // The segments of 64 sequences from `from` on, a lane's and those before it; all of them returned.
-__device__ __forceinline__ int count_segments(const ScanArgs& a, int from, int seg, int& own, int& before) {
+__device__ __forceinline__ int count_segments(const PackedScanArgs& a, int from, int seg, int& own, int& before) {
   const int lane = threadIdx.x & 63, i = from + lane;
   own = 0;
   if (i < a.n_seq) {
@@ -171,7 +171,7 @@ __device__ __forceinline__ int count_segments(const ScanArgs& a, int from, int s
   return __builtin_amdgcn_readlane(sum, 63);
 }
 // The sequence of a place; false where there is none.
-__device__ __forceinline__ bool sequence_at(const ScanArgs& a, int place, int seg, Where& q) {
+__device__ __forceinline__ bool sequence_at(const PackedScanArgs& a, int place, int seg, Where& q) {
   if (!a.cu) {
     const int per = scan_segments(a.len, seg);
     q.seq = (int)((uint32_t)place / (uint32_t)per);
@@ -200,7 +200,7 @@ __device__ __forceinline__ bool sequence_at(const ScanArgs& a, int place, int se
   return false;
 }
 // The first place of a sequence.
-__device__ __forceinline__ int64_t first_place(const ScanArgs& a, int b, int seg, int64_t t0) {
+__device__ __forceinline__ int64_t first_place(const PackedScanArgs& a, int b, int seg, int64_t t0) {
   if (!a.cu) return (int64_t)b * scan_segments(a.len, seg);
   if (a.n_seq > kCounted) return (int64_t)((uint32_t)t0 / (uint32_t)seg) + b;
   int base = 0;
@@ -215,7 +215,7 @@ __device__ __forceinline__ int64_t first_place(const ScanArgs& a, int b, int seg
 // STATE: the states that a segment leaves from zero, and its decay, of all segments but the last of a sequence.
 template <int N, bool BF, bool STATE>
 __global__ __attribute__((amdgpu_waves_per_eu(2))) __launch_bounds__(64 * kW) void
-scan_chunk_kernel(ScanArgs a, int seg, int places, float* seg_state, float* seg_decay) {
+scan_chunk_kernel(PackedScanArgs a, int seg, int places, float* seg_state, float* seg_decay) {
   constexpr int NB = N / 16, NN = N / 32, NU = kParts<BF>, pieces = N / 8;
   __shared__ __align__(16) ScanLds<N, STATE> L;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -607,7 +607,8 @@ scan_chunk_kernel(ScanArgs a, int seg, int places, float* seg_state, float* seg_
 // The states before each segment of a sequence of several, in place of those that its segments leave from zero. A thread
 // has four values of a head at a time, and those of eight segments on their way together (one by one, 16 segments of 64 heads
 // took 13 us); `per` workgroups to a sequence.
-__global__ __launch_bounds__(256) void scan_states_kernel(ScanArgs a, int seg, int places, int64_t per, float* seg_state, const float* seg_decay) {
+__global__ __launch_bounds__(256) void scan_states_kernel(PackedScanArgs a, int seg, int places, int64_t per, float* seg_state,
+                                                          const float* seg_decay) {
   constexpr int kAhead = 8;
   const int64_t size = (int64_t)a.H * a.P * a.N;
   const int b = (int)(blockIdx.x / per);
@@ -644,14 +645,14 @@ __global__ __launch_bounds__(256) void scan_states_kernel(ScanArgs a, int seg, i
   }
 }
 
-int64_t segment(const ScanArgs& a) {
+int64_t segment(const PackedScanArgs& a) {
   const int64_t longest = a.cu ? a.n_tokens : a.len, seg = scan_segment(a.n_tokens, a.n_seq, scan_wgs(a.H, a.G, a.P));
   return seg >= longest ? (longest + kC) / kC * kC : seg;
 }
-bool split(const ScanArgs& a) { return segment(a) < (a.cu ? a.n_tokens : a.len); }
+bool split(const PackedScanArgs& a) { return segment(a) < (a.cu ? a.n_tokens : a.len); }
 
 template <int N, bool BF>
-hipError_t launch(const ScanArgs& a, void* ws, hipStream_t s) {
+hipError_t launch(const PackedScanArgs& a, void* ws, hipStream_t s) {
   const int64_t seg = segment(a), places = scan_places(a.n_tokens, a.n_seq, seg), wgs = scan_wgs(a.H, a.G, a.P) / a.G;
   const int64_t units = places * a.G, grid = (units + 7) / 8 * 8 * wgs, size = (int64_t)a.H * a.P * N;
   if (grid > 0x7fffffff || seg > 0x7fffffff) return hipErrorInvalidValue;
@@ -668,13 +669,13 @@ hipError_t launch(const ScanArgs& a, void* ws, hipStream_t s) {
 
 }  // namespace
 
-size_t scan_chunk_workspace(const ScanArgs& a) {
+size_t scan_chunk_workspace(const PackedScanArgs& a) {
   if (!split(a)) return 0;
   const int64_t places = scan_places(a.n_tokens, a.n_seq, segment(a));
   return (size_t)places * ((size_t)a.H * a.P * a.N + a.H) * sizeof(float);
 }
 
-hipError_t launch_scan_chunked(const ScanArgs& a, void* ws, hipStream_t s) {
+hipError_t launch_scan_chunked(const PackedScanArgs& a, void* ws, hipStream_t s) {
   if (a.N == 128) return a.bf16 ? launch<128, true>(a, ws, s) : launch<128, false>(a, ws, s);
   return a.bf16 ? launch<64, true>(a, ws, s) : launch<64, false>(a, ws, s);
 }

@@ -7,12 +7,12 @@ namespace dfssm {
 struct HeadParams {
   float A, D, bias;  // A = -e^{A_log}
 };
-__device__ __forceinline__ HeadParams head_params(const ScanArgs& a, int h) {
+__device__ __forceinline__ HeadParams head_params(const PackedScanArgs& a, int h) {
   return HeadParams{-dev_expf(a.A_log[h]), a.D ? a.D[h] : 0.0f, a.dt_bias ? a.dt_bias[h] : 0.0f};
 }
 
 template <bool BF>
-__device__ __forceinline__ float load_dt(const ScanArgs& a, int64_t t, int h) {
+__device__ __forceinline__ float load_dt(const PackedScanArgs& a, int64_t t, int h) {
   if (a.dt32) return ((const float*)a.dt)[t * a.ld_dt + h];
   return w2f<BF>(((const uint16_t*)a.dt)[t * a.ld_dt + h]);
 }

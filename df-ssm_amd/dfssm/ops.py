@@ -1,8 +1,8 @@
 """Single-operator wrappers over the C ABI, taking torch tensors on the GPU.
 
 These are the operator-level entry points (scaffold GEMM, RMSNorm+quantize, conv step, SSM step,
-bit/embedding tiling, the gated delta rule, a state space layer between its projections, the token draw). Every call launches on torch's current stream and raises on any error;
-there is no CPU fallback. Arguments that are not contiguous are copied; all copies of a call stay bound
+bit/embedding tiling, the gated delta rule, a state space layer between its projections, the token draw). Every call
+launches on torch's current stream and raises on any error; there is no CPU fallback. Arguments that are not contiguous are copied; all copies of a call stay bound
 to names until its launch, so that the allocator cannot give one's memory to the next.
 """
 from __future__ import annotations
@@ -357,7 +357,8 @@ def gated_delta_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: to
 
 
 # ---------------------------------------------------------------------------------------------
-# a state space layer between its projections
+# a state space layer between its projections. None of these operators has a backward pass: with gradients enabled, a
+# tensor that requires one is refused.
 # ---------------------------------------------------------------------------------------------
 MAX_NORM_COLS = 16384   # DFSSM_NORM_MAX_COLS
 
@@ -463,6 +464,15 @@ def _kind16(x) -> int:
     return kind
 
 
+def _no_gradient(*tensors) -> None:
+    """Refuses tensors whose gradient would be lost: a layer's operators have no backward pass."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError("an argument requires a gradient, and this operator has no backward pass: detach it, or call "
+                                 "under torch.no_grad()")
+
+
 def _run(dev: int, call, args, what: str) -> None:
     """call(args, current stream) on device dev."""
     if dev != _C.current_device():
@@ -506,6 +516,7 @@ def _conv_call(step: bool, x, weight, bias, state, cu_seqlens, slots, silu, out,
         same = op == x.data_ptr() and (T <= 1 or ld_out == x.stride(0)) and (C == 1 or x.stride(1) == 1)
         if not (step and same) and not _apart(out, x):
             raise ValueError("out must not overlap x" + (" (or be x itself)" if step else ""))
+    _no_gradient(x, weight, bias, state)
     if n_seq == 0:
         return out
     x, ld_x, xp = _rows(x, C)   # (copies live until the launch)
@@ -527,7 +538,7 @@ def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, bias, state: torch.T
     sequence has are left as they are there). Rows of x and out may be strided; out may be x itself, and overlaps
     nothing else. slots (B,) int32: the slot of each sequence (default 0..B-1); a negative one marks padding (zeros
     returned), one past the state or taken by an earlier row gives NaN, and neither touches a state. Sums are fp32, out is
-    rounded once."""
+    rounded once. There is no backward pass: with gradients enabled, tensors that require one are refused."""
     return _conv_call(True, x, weight, bias, state, None, slots, silu, out, state_out,
                       x.shape[0] if isinstance(x, torch.Tensor) and x.dim() else 0)
 
@@ -598,6 +609,7 @@ def _scan_call(step: bool, x, dt, A_log, B, C, state, D, dt_bias, cu_seqlens, sl
             raise ValueError("out must have contiguous heads and 16-byte aligned tokens that do not overlap")
         if not all(_apart(out, t) for t in (x, B, C)):
             raise ValueError("out must not overlap x, B or C")
+    _no_gradient(x, dt, A_log, B, C, D, dt_bias, state)
     if n_seq == 0:
         return out
     # (copies live until the launch)
@@ -628,8 +640,8 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A_log: torch.Tensor, 
     x (B, H, P) fp16 or bf16, P a multiple of 16 up to 256; dt (B, H) of x's type or fp32; B, C (B, G, N) of x's type, N 64
     or 128, head h reads group h // (H // G); A_log (H,) fp32, D and dt_bias (H,) fp32 or None (zero); state
     (slots, H, P, N) fp32, contiguous, updated in place, or written to state_out (of the same shape; slots that no
-    sequence has are left as they are there). Rows may be strided. softplus=False takes d = max(dt + dt_bias, 0). slots as
-    in causal_conv_step. out, if given, overlaps none of the others."""
+    sequence has are left as they are there). Rows may be strided. softplus=False takes d = max(dt + dt_bias, 0). slots and
+    gradients as in causal_conv_step. out, if given, overlaps none of the others."""
     return _scan_call(True, x, dt, A_log, B, C, state, D, dt_bias, None, slots, softplus, out, state_out,
                       x.shape[0] if isinstance(x, torch.Tensor) and x.dim() else 0)
 
@@ -707,7 +719,8 @@ def gated_norm(x: torch.Tensor, gate, weight: torch.Tensor, groups: int = 1, eps
     parts of a row.
 
     x (.., cols) and gate of its shape fp16 or bf16, rows may be strided; gate None: none. weight (cols,) fp32. cols /
-    groups at most 16384. In fp32, rounded once. out may be x or gate itself, and overlaps them no other way."""
+    groups at most 16384. In fp32, rounded once. out may be x or gate itself, and overlaps them no other way.
+    There is no backward pass: with gradients enabled, tensors that require one are refused."""
     kind = _kind16(x)
     dt, dev = x.dtype, x.get_device()
     r = _norm_rows(x)
@@ -727,6 +740,7 @@ def gated_norm(x: torch.Tensor, gate, weight: torch.Tensor, groups: int = 1, eps
         z, ld_z, zp = _rows(_norm_rows(gate), cols)
         inputs.append((z, ld_z, zp))
     out, ld_out, op = _norm_out(out, x, "out", dt, dev, cols, inputs)
+    _no_gradient(x, gate, weight)
     if rows:
         args = _C.Gated(p, zp, weight.data_ptr(), op, ld, ld_z, ld_out, rows, cols, groups, kind, 1 if gate_first else 0, eps)
         _run(dev, _C.lib().dfssm_gated_norm, args, "gated_norm")
@@ -741,7 +755,7 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
     x (.., cols) fp16 or bf16, residual of its shape, of its type or fp32; rows may be strided; weight and post_weight
     (cols,) fp32; scale a number or (cols,) fp32; cols at most 16384. In fp32; the first result has x's type, r the
     residual's, each rounded once. residual_out may be residual itself and out x; they overlap the inputs no other way,
-    nor each other."""
+    nor each other. There is no backward pass: with gradients enabled, tensors that require one are refused."""
     kind = _kind16(x)
     dt, dev = x.dtype, x.get_device()
     f32 = torch.float32
@@ -767,6 +781,7 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
     residual_out, ld_ro, rop = _norm_out(residual_out, x, "residual_out", rt, dev, cols, inputs)
     if given and not _apart(_norm_rows(out), _norm_rows(residual_out)):
         raise ValueError("out and residual_out must not overlap")
+    _no_gradient(x, residual, weight, post_weight, scales)
     if rows:
         args = _C.Residual(p, sp, _C.ptr(post_weight), _C.ptr(scales), weight.data_ptr(), op, rop, ld, ld_s, ld_out, ld_ro,
                            rows, cols, kind, 2 if rt is f32 else kind, float(scale), eps)

@@ -398,7 +398,7 @@ size_t dfssm_gated_delta_workspace_bytes(const dfssm_delta* args);
 int dfssm_gated_delta_prefill(const dfssm_delta* args, void* workspace, void* stream);
 
 /* ---- a state space layer between its projections ----------------------------------------- */
-/* Sequences and slots are those of dfssm_delta: sequence b has tokens cu_seqlens[b] .. cu_seqlens[b + 1] (any length, zero
+/* Forward only: none of these has a backward pass. Sequences and slots are those of dfssm_delta: sequence b has tokens cu_seqlens[b] .. cu_seqlens[b + 1] (any length, zero
  * included; held to [0, n_tokens]; rows of no sequence stay as they were; where offsets fall, results are not specified and
  * nothing outside the tensors is read or written), or n_tokens / n_seq each with NULL, and the state in slot
  * slots[b], or b with NULL. A negative slot is padding: zeros in out; one that is >= n_slots or an earlier sequence's: NaN.

@@ -472,7 +472,8 @@ scan_chunk_kernel(PackedScanArgs a, int seg, int places, float* seg_state, float
             D[8 + k] = own ? v : 0.0f;
           }
         }
-        // y of the state comes into M's scale (at most 2^40: what is lost of smaller M is below 2^-60)
+        // y of the state comes into M's scale (at most 2^40: what is lost of smaller M is below 2^-60), by a finite factor: where it
+        // would not be, y is infinite, unless C leaves the state out
         float ys = __builtin_amdgcn_exp2f(Gi + gi), msc = 1.0f;
         if constexpr (!BF) {
           float top = 0x1p-26f;
@@ -487,7 +488,7 @@ scan_chunk_kernel(PackedScanArgs a, int seg, int places, float* seg_state, float
         for (int r = 0; r < 16; r += 4) {
           const f32x4 sv = BF ? f32x4{1.0f, 1.0f, 1.0f, 1.0f} : *(const f32x4*)&V.s[16 * hi + r];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y[t][r + e] *= BF ? ys : ys * sv[e];
+          for (int e = 0; e < 4; ++e) y[t][r + e] *= BF ? ys : __builtin_fminf(ys * sv[e], 0x1.fffffep127f);
         }
 #pragma unroll
         for (int k = 0; k < 2 * (t + 1); ++k) {

@@ -121,3 +121,31 @@ def test_small_values_beside_a_large_one_that_a_sum_leaves_out(lens):
     out, _ = call(X, dT, B, C, state, lens)
     score = 1e5 * (C.double() @ B[3, 0].double()).abs().amax()
     off(out, y, rel * (1 + 2.0 ** -7) * y.abs() + 2.0 ** -16 * mag + tiny + 2.0 ** -39 * score * total(x)[:1], "scores' out")
+
+
+@pytest.mark.parametrize("large", [1e30, 1e35])
+def test_outputs_that_leave_a_very_large_state_out(large):
+    """fp16 rows: C is zero, so out is x's share alone (zero without D), however large the state and small the scores."""
+    T, H, P, N = 100, 2, 32, 64
+    gen = torch.Generator().manual_seed(0)
+    x, B = torch.randn(T, H, P, generator=gen).half(), torch.randn(T, 1, N, generator=gen).half()
+    state = torch.full((1, H, P, N), large)
+    for D in (None, torch.tensor([2.0 ** -30, 1.0], device=DEV)):
+        out, after = call(x, torch.zeros(T, H), B, torch.zeros(T, 1, N).half(), state, [T], D=D)
+        ref = torch.zeros(T, H, P) if D is None else D.cpu().double()[:, None] * x.double()
+        assert ((out - ref).abs() <= 2.0 ** -11 * ref.abs() + 2.0 ** -25).all() and torch.equal(after, state.double())
+
+
+def test_a_very_large_state_that_decays():
+    """e^-80 of 1e35, within a chunk and in the next: 1.8 C. (An exponent of 80 in fp32 is off by 80 2^-21 at most: 4e-5.)"""
+    T, H, P, N = 100, 1, 32, 64
+    x, B, C = torch.zeros(T, H, P).half(), torch.zeros(T, 1, N).half(), torch.zeros(T, 1, N).half()
+    C[20:, 0, 3] = 1
+    dt = torch.zeros(T, H)
+    dt[10:20] = 8.0
+    state = torch.full((1, H, P, N), 1e35, device=DEV)
+    out = ops.selective_scan_prefill(x.to(DEV), dt.to(DEV), torch.zeros(H, device=DEV), B.to(DEV), C.to(DEV), state,
+                                     cu_seqlens=lm.offsets([T], DEV), softplus=False).cpu().double()
+    ref = float(torch.tensor(1e35, dtype=torch.float32)) * torch.exp(torch.tensor(-80.0, dtype=torch.float64))
+    assert not out[:20].any() and ((out[20:] - ref).abs() <= (2.0 ** -11 + 4.1e-5) * ref).all()
+    assert ((state.cpu().double() - ref).abs() <= 4.1e-5 * ref).all()

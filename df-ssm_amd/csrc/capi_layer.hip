@@ -94,11 +94,14 @@ PackedScanArgs scan_args(const dfssm_scan* d) {
 }
 
 // Prompts that run token by token: too few tokens for a chunk's fixed work. The lengths behind cu_seqlens are on the device,
-// so the rule there goes by all tokens, which any one sequence may have. Sequences of 8 | 12 | 16 tokens, token by token and in
-// chunks, kernels in a replayed graph, fp16 (one sequence of one group spread over the dies since, 2 us less in chunks):
-//   64 heads of 64 x 128   one sequence 9.2, 14.4 | 12.1, 14.3 | 15.0, 14.0 us   32: 45, 39 | 59, 40 | 71, 38
-//   40 heads of 128 x 128, 5 groups     9.3, 11.8 | 12.3, 11.9 | 15.3, 11.9          55, 49 | 72, 49 | 96, 49
-//   6 heads of 256 x 64                 8.2, 8.8 | 10.7, 8.8 | 13.1, 8.9             17, 14 | 22, 14 | 27, 14
+// so the rule there goes by all tokens, which any one sequence may have; without offsets it goes by the length, whatever the number
+// of sequences. That is right for few of them: 32 and 64 of 7 or 8 tokens would take up to 15% less in chunks. Sequences of
+// 4 | 6 | 8 | 12 tokens, token by token and in chunks, kernels in a replayed graph, fp16:
+//   64 heads of 64 x 128                one 6.3, 11.9 | 7.8, 11.8 | 9.3, 11.9 | 12.1, 11.8 us   32: 31, 39 | 39, 39 | 45, 39 | 58, 40
+//                                      four 8.6, 13.5 | 10.5, 13.5 | 12.4, 13.3 | 16.2, 13.4    64: 59, 70 | 72, 71 | 83, 72 | 116, 72
+//   40 heads of 128 x 128, 5 groups     one 6.5, 11.8 | 8.1, 11.9 | 9.6, 11.9 | 12.4, 11.9      32: 39, 49 | 47, 49 | 54, 48 | 71, 49
+//                                      four 9.7, 13.5 | 11.9, 13.5 | 14.3, 13.6 | 18.4, 13.5    64: 72, 90 | 89, 92 | 107, 92 | 139, 95
+//   6 heads of 256 x 64                 one 5.7, 8.8 | 6.9, 8.8 | 8.3, 8.8 | 10.8, 8.9          32: 11, 14 | 14, 14 | 17, 14 | 22, 14
 constexpr int kTokenPath = 8;
 bool by_tokens(const PackedScanArgs& a) { return (a.cu ? a.n_tokens : a.len) <= kTokenPath; }
 

@@ -62,8 +62,9 @@ struct ResidualNormArgs {
 };
 hipError_t launch_residual_norm(const ResidualNormArgs& a, hipStream_t s);
 
-// x / (1 + e^-x). Relative error at most (1 + |x|) 2^-23: of e^(-x), from the rounding of x log2 e, and the hardware's
-// exponential and reciprocal (1 ulp each); outputs have 12 bits at most.
+// x / (1 + e^-x). Relative error at most (3 + |x|) 2^-23: the rounding of x log2 e is |x| 2^-23 of e^-x, the hardware's exponential
+// and reciprocal 2^-23 each (1 ulp), the sum and the last product 2^-24 each; outputs have 12 bits at most. Below x = -87 the
+// reciprocal leaves the normal numbers: off by up to 2^-119.
 __device__ __forceinline__ float silu_f32(float x) {
   return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.44269504f));
 }

@@ -7,9 +7,9 @@
 // A row, or a group of one, lies in registers over 8, 16 or 64 lanes or a workgroup; a lane has eight columns at a time, loaded
 // from any address. Where a width is no multiple of 8, the last lane's columns end with the row and overlap its neighbour's: it
 // leaves those out of sums, and both store the same values. A workgroup goes over many rows with its columns' weights in
-// registers, and the next row is on its way while it reduces this one. 32768 rows of 5120, eight groups (bf16, 1.01 GB), 0.206 ms; 32768
-// of 2560 with a residual in 32 bits (1.01 GB) 0.200 ms: 4.9 and 5.0 TB/s, what a copy reaches. (A row to a workgroup at a time, weights
-// read for each: 0.366 and 0.399 ms.) Few rows: the launch; one of 4096 3.6 us, 32 of 2048 3.3 us in a replayed graph.
+// registers, and the next row is on its way while it reduces this one. 32768 rows of 5120, eight groups (bf16, 1.01 GB), 0.206 ms;
+// 32768 of 2560 with a residual in 32 bits (1.01 GB) 0.199 ms: 4.9 and 5.0 TB/s, what a copy reaches. (A row to a workgroup at a
+// time, weights read for each: 0.366 and 0.399 ms.) Few rows: the launch; one of 4096 3.7 us, 32 of 2048 3.3 us in a replayed graph.
 #include "common.h"
 #include "layer.h"
 

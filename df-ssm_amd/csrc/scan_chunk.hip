@@ -36,8 +36,8 @@ namespace dfssm {
 namespace {
 
 constexpr int kC = kScanChunk, kW = kScanWaves;
-// Fewer groups of B and C than this, over all places, are spread over all dies. One prompt of 45 tokens, 64 heads in one group, 14.9
-// us on one die and 12.4 on eight; with 25 and 37 places (16411 tokens, and the ragged batch) 241 and 162 us by dies, 251 and 154
+// Fewer groups of B and C than this, over all places, are spread over all dies. One prompt of 45 tokens, 64 heads in one group, 15.0
+// us on one die and 12.4 on eight; with 25 and 37 places (16411 tokens, and the ragged batch) 242 and 175 us by dies, 247 and 164
 // spread.
 constexpr int kSpread = 16;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -662,7 +662,8 @@ hipError_t launch(const PackedScanArgs& a, void* ws, hipStream_t s) {
     hipLaunchKernelGGL((scan_chunk_kernel<N, BF, true>), dim3((unsigned)grid), dim3(64 * kW), 0, s, a, (int)seg, (int)places, st, de);
     // (sequences of one segment end at once: 64 of them with 640 workgroups each took 33 us)
     const int64_t most = (size / 4 + 255) / 256, few = 2048 / a.n_seq, per = few < 1 ? 1 : (few < most ? few : most);
-    hipLaunchKernelGGL(scan_states_kernel, dim3((unsigned)(a.n_seq * per)), dim3(256), 0, s, a, (int)seg, (int)places, per, st, (const float*)de);
+    hipLaunchKernelGGL(scan_states_kernel, dim3((unsigned)(a.n_seq * per)), dim3(256), 0, s, a, (int)seg, (int)places, per, st,
+                       (const float*)de);
   }
   hipLaunchKernelGGL((scan_chunk_kernel<N, BF, false>), dim3((unsigned)grid), dim3(64 * kW), 0, s, a, (int)seg, (int)places, st, de);
   return hipGetLastError();

@@ -18,9 +18,10 @@ constexpr int64_t scan_wgs(int H, int G, int P) {
 }
 
 // Tokens of a segment. A sequence longer than that is cut into segments that run beside each other, from states
-// that a pass over all but the last of them makes first: 768 workgroups, three to a CU. (With 512, 1024 and 1536: 16411 tokens
-// x 64 heads 236, 253 and 264 us, 231 with 768; twelve ragged sequences 176, 184 and 149, 154; 64 x 512 tokens x 80 heads 448, 474
-// and 430, 440.)
+// that a pass over all but the last of them makes first: about 768 workgroups, where two are resident on each of 256 CUs. Fewer
+// leave CUs idle where sequences are unequal, more have longer chains and more states to move. (With 512, 768, 1024 and 1536, in
+// replayed graphs: 16411 tokens x 64 heads 232, 242, 259 and 277 us; twelve ragged sequences 199, 175, 171 and 176; 64 x 512
+// tokens x 80 heads, cut by none, 447, 448, 445 and 446.)
 constexpr int64_t scan_segment(int64_t n_tokens, int n_seq, int64_t wgs) {
   const int64_t chunks = n_tokens / kScanChunk + n_seq;
   int64_t m = (chunks * wgs + 768 - 1) / 768;

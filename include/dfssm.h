@@ -469,8 +469,8 @@ size_t dfssm_selective_scan_workspace_bytes(const dfssm_scan* args);
 int dfssm_selective_scan_prefill(const dfssm_scan* args, void* workspace, void* stream);
 
 /* out = rmsnorm(x s(gate)) weight (gate_first) or rmsnorm(x) weight s(gate), s(z) = z / (1 + e^-z), rmsnorm(v) =
- * v / sqrt(mean(v^2) + eps) over each of `groups` equal parts of a row; gate NULL: none. In fp32 with one rounding. out may be
- * x or gate itself. */
+ * v / sqrt(mean(v^2) + eps) over each of `groups` equal parts of a row; gate NULL: none. In fp32 with one rounding: where the sum
+ * of squares is infinite (one of 2^128 and more is), the outputs are zeros, of an infinite value NaN. out may be x or gate itself. */
 typedef struct dfssm_gated {
   const void* x;          /* (rows, cols), `type`; rows ld_x elements apart */
   const void* gate;       /* the same, or NULL */
@@ -487,7 +487,8 @@ typedef struct dfssm_gated {
 int dfssm_gated_norm(const dfssm_gated* args, void* stream);
 
 /* r = residual + scale (rmsnorm(x) post_weight, or x where post_weight is NULL); residual_out = r; out = rmsnorm(r) weight, of r
- * before residual_out's rounding. In fp32 with one rounding each. residual_out may be residual itself, out x. */
+ * before residual_out's rounding. In fp32 with one rounding each; infinite sums of squares as above. residual_out may be residual
+ * itself, out x. */
 typedef struct dfssm_residual {
   const void* x;            /* (rows, cols), `type`; rows ld_x elements apart */
   const void* residual;     /* (rows, cols), `residual_type` */

@@ -64,3 +64,13 @@ def test_residual(n, res):
     only_there(out, at)
     _, r = ops.residual_norm(x, torch.zeros_like(one).to(res), w, post_weight=w)      # (x's norm: zeros and a NaN)
     only_there(r, at)
+
+
+@pytest.mark.parametrize("n", [40, 1000, 5120])
+def test_squares_past_fp32(n):
+    """bf16 rows of finite values whose squares are infinite in fp32 come out as zeros, those of 2^50 as ones."""
+    x, w = torch.full((3, n), 2.0 ** 70, dtype=torch.bfloat16, device=DEV), torch.ones(n, device=DEV)
+    x[1] = 2.0 ** 50
+    zero, one = torch.zeros(n, device=DEV), torch.ones(n, device=DEV)
+    for out in (ops.gated_norm(x, None, w), ops.residual_norm(x, torch.zeros_like(x), w)[0]):
+        assert torch.equal(out[0].float(), zero) and torch.equal(out[1].float(), one) and torch.equal(out[2].float(), zero)
